@@ -278,13 +278,15 @@ def _run_lora(st):
     case = st["case"]
     if own:
         ops = _ops()
-        if "ws" not in st:
-            st["ws"] = ops.lora_workspace(st["x"].shape[0], case["k"], case["rank"])
+        if "ws" not in st:  # the workspace and the output buffer that a serving loop keeps
+            T = st["x"].shape[0]
+            st["ws"] = ops.lora_workspace(T, case["k"], case["rank"])
+            st["out"] = torch.empty(T, case["n"], device=st["x"].device,
+                                    dtype=torch.float32 if case["partial"] else torch.bfloat16)
+        keep = dict(q_indptr=st["indptr"], max_q_len=st["max_q"], workspace=st["ws"], out=st["out"])
         if case["partial"]:
-            return ops.lora_partial(st["x"], st["a"], st["b"], st["scales"], st["ids"],
-                                    q_indptr=st["indptr"], max_q_len=st["max_q"], workspace=st["ws"])
-        return ops.lora_add(st["x"], st["a"], st["b"], st["scales"], st["ids"], st["y"],
-                            q_indptr=st["indptr"], max_q_len=st["max_q"], workspace=st["ws"])
+            return ops.lora_partial(st["x"], st["a"], st["b"], st["scales"], st["ids"], **keep)
+        return ops.lora_add(st["x"], st["a"], st["b"], st["scales"], st["ids"], st["y"], **keep)
     n, R, K = st["a"].shape
     of = st["of_token"].long()
     h = (st["x"].float() @ st["a"].float().view(n * R, K).T).view(-1, n, R)
@@ -301,9 +303,11 @@ def _run_store(st):
         ops = _ops()
         src, call = ((st["parts"], ops.qknorm_mrope_store_kv_partials) if case["parts"]
                      else (st["qkv"], ops.qknorm_mrope_store_kv))
+        if "out" not in st:  # kept by a serving loop
+            st["out"] = torch.empty(T, hq, HD, dtype=torch.bfloat16, device=src.device)
         q = call(src, st["k_pool"], st["v_pool"], st["positions"], st["slots"], st["table"],
                  st["qn"], st["kn"], hq, hkv, EPS, sections=st["sections"],
-                 interleaved=case["interleaved"])
+                 interleaved=case["interleaved"], out=st["out"])
         return {"q": q, "k_pool": st["k_pool"], "v_pool": st["v_pool"]}
     x = st["parts"].sum(0) if case["parts"] else st["qkv"].float()
     x = x.view(T, hq + 2 * hkv, HD)
@@ -346,15 +350,19 @@ def _run_sparse(st):
     hq, hkv, top = case["hq"], case["hkv"], case["top"]
     if own:
         ops = _ops()
-        if "ws" not in st:
-            st["ws"] = ops.select_pages_workspace(st["q"].shape[0], st["max_seq"], hkv)
+        if "ws" not in st:  # the workspace and the output buffers that a serving loop keeps
+            T, dev = st["q"].shape[0], st["q"].device
+            st["ws"] = ops.select_pages_workspace(T, st["max_seq"], hkv)
+            st["ids"] = torch.empty(T, hkv, top, dtype=torch.int32, device=dev)
+            st["out"] = torch.empty(T, hq, HD, dtype=torch.bfloat16, device=dev)
         ids = ops.select_pages(st["q"], st["bounds"], st["page_table"], st["seq_lens"],
                                st["max_seq"], top, hq, hkv, sink_pages=case["sink"],
                                recent_pages=case["recent"], q_indptr=st["indptr"],
-                               max_q_len=st["max_q"], workspace=st["ws"])
+                               max_q_len=st["max_q"], workspace=st["ws"], out=st["ids"])
         out = ops.paged_attention_pages(st["q"], st["k_pool"], st["v_pool"], st["page_table"],
                                         st["seq_lens"], ids, hq, hkv, q_indptr=st["indptr"],
-                                        max_q_len=st["max_q"])
+                                        max_q_len=st["max_q"], max_seq_len=st["max_seq"],
+                                        out=st["out"])
         return {"page_ids": ids, "out": out}
     q, of, at = st["q"], st["of_token"], st["at"]
     T, G, B, n = q.shape[0], hq // hkv, case["reqs"], st["page_table"].shape[1]
