@@ -134,6 +134,40 @@ MSGL_API int msgl_qknorm_rope_store_kv_partials(const float* parts, int nparts, 
                                                 int num_q_heads, int num_kv_heads, int head_dim,
                                                 float eps, msgl_stream_t stream);
 
+/* Rotary positions of three axes (time, height, width of image and video tokens; no counterpart
+ * in the reference). Which axis turns the rotary pair (d, d + D / 2), with sections {s0, s1, s2}
+ * (a HOST array; s0 + s1 + s2 = D / 2):
+ *   MSGL_MROPE_SECTIONS     consecutive ranges: s0 pairs of axis 0, then s1 of axis 1, s2 of 2;
+ *   MSGL_MROPE_INTERLEAVED  axis 1 where d % 3 == 1 and d < 3 s1, axis 2 where d % 3 == 2 and
+ *                           d < 3 s2, axis 0 elsewhere (s1 and s2 at most D / 6). */
+typedef enum { MSGL_MROPE_SECTIONS = 0, MSGL_MROPE_INTERLEAVED = 1 } msgl_mrope_layout;
+/* msgl_qknorm_rope_store_kv with positions [3][position_stride] (axis-major, the first num_tokens
+ * of each row used; position_stride >= num_tokens, or 0: one row for all axes) into the fp32 table
+ * cos_sin_cache [max_position, D]. Equal rows give the one-axis rotation. A position outside
+ * [0, max_position) counts as 0 and is recorded (MSGL_ERR_BOUNDS, site 102), a slot >= num_slots
+ * is skipped and recorded (site 103), a negative slot skips the store. Two tokens of one call must
+ * not name the same slot. qkv / parts, q_out, pools and norm weights 16-byte aligned. */
+MSGL_API int msgl_qknorm_mrope_store_kv(const void* qkv, void* q_out, void* k_pool, void* v_pool,
+                                        int64_t num_slots, const int* positions,
+                                        int64_t position_stride, const int* sections, int layout,
+                                        const int* slot_mapping, const float* cos_sin_cache,
+                                        int max_position, const void* q_norm_w,
+                                        const void* k_norm_w, int num_tokens, int num_q_heads,
+                                        int num_kv_heads, int head_dim, float eps,
+                                        msgl_stream_t stream);
+/* The same, with the QKV row the sum (in p order) of fp32 split-K partials
+ * parts [nparts][T][(Hq + 2 Hkv) D] (msgl_gemm_bf16_partials, msgl_lora_partial). */
+MSGL_API int msgl_qknorm_mrope_store_kv_partials(const float* parts, int nparts, void* q_out,
+                                                 void* k_pool, void* v_pool, int64_t num_slots,
+                                                 const int* positions, int64_t position_stride,
+                                                 const int* sections, int layout,
+                                                 const int* slot_mapping,
+                                                 const float* cos_sin_cache, int max_position,
+                                                 const void* q_norm_w, const void* k_norm_w,
+                                                 int num_tokens, int num_q_heads,
+                                                 int num_kv_heads, int head_dim, float eps,
+                                                 msgl_stream_t stream);
+
 /* ---------------------------------------------------------------- sampling */
 /* Next-token sampling per row of fp32 logits [num_rows, vocab] with per-row SamplingParams
  * (include/minisgl/core/types.h:12-20; device arrays temperature, top_k, top_p). Rows with
@@ -250,6 +284,56 @@ MSGL_API int msgl_paged_attention_extend(const void* q, const void* k_pool, cons
                                 int max_q_len, int num_q_heads, int num_kv_heads, int head_dim,
                                 int page_size, float scale, void* out, msgl_stream_t stream);
 
+/* ---------------------------------------------------------------- page-sparse attention */
+/* Attention over the few pages of a long context that a query needs (no counterpart in the
+ * reference). Common to the three calls: head_dim 128, page_size 16, Hq / Hkv in {1, 2, 4, 8};
+ * request r owns query rows [q_indptr[r], q_indptr[r+1]) of total_q rows, row i of an n-row
+ * request at position seq_lens[r] - n + i (q_indptr NULL: one row per request, max_q_len 1);
+ * max_q_len bounds the rows per request, max_seq_len (<= 524288, <= max_pages * 16) the contexts.
+ * Rows behind the last request are left as they were. Recorded as MSGL_ERR_BOUNDS in the device
+ * error word: a context outside [0, max_seq_len] (clamped, site 800), a request with more than
+ * max_q_len rows or rows outside total_q (site 801: its extra rows get empty lists, attention
+ * skips the request), a page-table entry outside the pool (site 802: page 0 is read in its place,
+ * its bounds are not written), a listed page behind the query's own (site 803: skipped).
+ *
+ * Bounds: bounds [num_pages, Hkv, 2, D] bf16 holds, per physical page, the smallest and the
+ * largest stored key of each dimension (NaN keys give NaN bounds). Written for every page that
+ * the last rows of each request touch, from the keys before the context's end: call it after the
+ * step's keys are stored. */
+MSGL_API int msgl_kv_page_bounds(const void* k_pool, int64_t num_slots, const int* page_table,
+                                 int max_pages, const int* seq_lens, const int* q_indptr,
+                                 int num_reqs, int max_q_len, int num_kv_heads, int head_dim,
+                                 int page_size, void* bounds, msgl_stream_t stream);
+/* Selection, per query row and kv head (its query heads share the list): with n visible pages
+ * (position / 16 + 1), all of them if n <= top_pages; else the first sink_pages, the last
+ * recent_pages (>= 1: the row's own page may be incomplete), and of the others the
+ * top_pages - sink_pages - recent_pages with the largest
+ *   max over the group's heads g of sum_d max(q_gd, 0) hi_d + min(q_gd, 0) lo_d,
+ * an upper bound of every q_g . k of the page. Scores compare as in exact arithmetic (near ties are
+ * scored again in fp64), equal scores go to the lower page, NaN scores rank highest.
+ * page_ids [total_q, Hkv, top_pages] int32: logical pages (page-table columns), ascending, filled
+ * up with -1. top_pages <= 1024. The workspace (msgl_select_pages_workspace_size, 16-byte aligned)
+ * needs no clearing; calls that overlap on the GPU need one each. */
+MSGL_API size_t msgl_select_pages_workspace_size(int total_q, int max_seq_len, int num_kv_heads);
+MSGL_API int msgl_select_pages(const void* q, const void* bounds, int64_t num_pages,
+                               const int* page_table, int max_pages, const int* seq_lens,
+                               const int* q_indptr, int num_reqs, int total_q, int max_q_len,
+                               int max_seq_len, int num_q_heads, int num_kv_heads, int head_dim,
+                               int page_size, int top_pages, int sink_pages, int recent_pages,
+                               int* page_ids, void* workspace, size_t workspace_bytes,
+                               msgl_stream_t stream);
+/* Attention of each query row over the listed pages of its kv head, keys up to its own position.
+ * A list is a set: order and repeats do not matter, negative entries are skipped; an empty list
+ * gives a zero row. Keys and values of pages that a row did not list, or behind its position, do
+ * not reach it whatever they hold. q / out [total_q, Hq, D] bf16. */
+MSGL_API int msgl_paged_attention_pages(const void* q, const void* k_pool, const void* v_pool,
+                                        int64_t num_slots, const int* page_table, int max_pages,
+                                        const int* seq_lens, const int* q_indptr, int num_reqs,
+                                        int total_q, int max_q_len, int max_seq_len,
+                                        const int* page_ids, int top_pages, int num_q_heads,
+                                        int num_kv_heads, int head_dim, int page_size, float scale,
+                                        void* out, msgl_stream_t stream);
+
 /* ---------------------------------------------------------------- tcgen05 GEMMs */
 /* Linear::forward (layer.cpp:122-143): y[M,N] = x[M,K] * W[N,K]^T, W in the reference's
  * [out, in] row-major layout. x, W bf16; y bf16 (out_dtype MSGL_BF16) or fp32 (MSGL_F32).
@@ -277,6 +361,35 @@ MSGL_API int msgl_gemm_gate_up_silu(const void* x, const void* w_packed, void* y
 MSGL_API int msgl_gemm_partials_splits(int M, int N, int K);
 MSGL_API int msgl_gemm_bf16_partials(const void* x, const void* w, float* parts, int M, int N, int K,
                                      int splits, msgl_stream_t stream);
+
+/* ---------------------------------------------------------------- low-rank adapters */
+/* Low-rank adapters of many requests at once beside a shared projection y = x W^T (no counterpart
+ * in the reference). Adapter a holds lora_a[a] [rank, K] and lora_b[a] [N, rank] (bf16, pools of
+ * num_adapters; smaller ranks are zero-padded to the pool's) and scales[a] (fp32). Request r owns
+ * rows [q_indptr[r], q_indptr[r+1]) of x (q_indptr NULL: one row per request, max_q_len 1) and
+ * uses adapter_ids[r] (device; negative: none):
+ *   msgl_lora_add      out[t] = y[t] + scales[a] * lora_b[a] (lora_a[a] x[t]), bf16; y rows of
+ *                      requests without an adapter are copied (out may be y itself);
+ *   msgl_lora_partial  part[t] = scales[a] * lora_b[a] (lora_a[a] x[t]) (zero without an adapter),
+ *                      fp32: the split-K partial behind those of msgl_gemm_bf16_partials.
+ * x [num_tokens, K], y / out / part [num_tokens, N] with row strides ldx, ldy, ldo, ldp in elements
+ * (rows 16-byte aligned), so that a column range of a fused projection can be given. K, N, rank
+ * multiples of 8, rank <= 128. Rows behind the last request are left as they were. Recorded as
+ * MSGL_ERR_BOUNDS: an adapter id >= num_adapters (treated as none, site 810), a request with more
+ * than max_q_len rows or rows outside num_tokens (skipped, site 811). The workspace
+ * (msgl_lora_workspace_size, 16-byte aligned) needs no clearing; calls that overlap on the GPU need
+ * one each. */
+MSGL_API size_t msgl_lora_workspace_size(int num_tokens, int K, int rank);
+MSGL_API int msgl_lora_add(const void* x, int64_t ldx, const void* lora_a, const void* lora_b,
+                           const float* scales, int num_adapters, const int* adapter_ids,
+                           const int* q_indptr, int num_reqs, int max_q_len, const void* y,
+                           int64_t ldy, void* out, int64_t ldo, int num_tokens, int N, int K,
+                           int rank, void* workspace, size_t workspace_bytes, msgl_stream_t stream);
+MSGL_API int msgl_lora_partial(const void* x, int64_t ldx, const void* lora_a, const void* lora_b,
+                               const float* scales, int num_adapters, const int* adapter_ids,
+                               const int* q_indptr, int num_reqs, int max_q_len, float* part,
+                               int64_t ldp, int num_tokens, int N, int K, int rank, void* workspace,
+                               size_t workspace_bytes, msgl_stream_t stream);
 
 /* lm_head (qwen3.cpp:178) fused with greedy sampling (scheduler.cpp:117-124): ids[m] = argmax_n
  * of the fp32 logits x[m] . W[n]; ties to the lowest id. `packed` is [M] uint64 scratch. */

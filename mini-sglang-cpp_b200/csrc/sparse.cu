@@ -1,0 +1,1109 @@
+// sparse.cu -- page-sparse attention: key bounds per page, page selection, attention over lists.
+//
+//  * msgl_kv_page_bounds        smallest / largest key of each page a step touched
+//  * msgl_select_pages          per query token and kv head, the pages with the largest bound of
+//                               their attention logits (plus forced first and last pages)
+//  * msgl_paged_attention_pages softmax attention over the listed pages only
+//
+// For page j with key bounds lo, hi (elementwise), every key k of the page and query head g:
+//   q_g . k <= s_g(j) = sum_d max(q_gd, 0) hi_d + min(q_gd, 0) lo_d.
+// A kv head's query group shares one list, so its score is max_g s_g(j): the largest logit any
+// head of the group can have in the page. Bounds are bf16 like the keys, hence exact, and 1/16 of
+// the page's key and value bytes.
+//
+// The selection is the one of exact arithmetic, whatever order the sums are taken in: scores are
+// computed with bf16 MMAs in fp32, and pages whose fp32 score lies within the error bound of the
+// k-th largest are scored again in fp64 (products of bf16 values are exact there).
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace msgl {
+namespace {
+
+constexpr int kPage = 16;
+constexpr int kHd = 128;
+constexpr int kMaxPagesPerReq = 32768;  // context bound of the selection: 524288 tokens
+constexpr int kMaxTopPages = 1024;
+constexpr float kNegInf = -__builtin_huge_valf();
+
+// ------------------------------------------------------------------ request window
+// Context length and query rows of request r: row i sits at position L - qn + i.
+struct Window {
+    int L, qn, q0;
+};
+
+__device__ __forceinline__ Window request_window(int r, const int* seq_lens, const int* q_indptr,
+                                                 int max_len, bool report, int* err) {
+    Window w;
+    w.L = seq_lens[r];
+    if (w.L < 0 || w.L > max_len) {
+        if (report) record_error(err, MSGL_ERR_BOUNDS, 800);
+        w.L = w.L < 0 ? 0 : max_len;
+    }
+    w.q0 = q_indptr ? q_indptr[r] : r;
+    w.qn = q_indptr ? q_indptr[r + 1] - w.q0 : 1;
+    return w;
+}
+
+// ------------------------------------------------------------------ bounds
+constexpr int kBoundWarps = 8;
+
+__device__ __forceinline__ uint32_t min_nan2(uint32_t a, uint32_t b) {
+    __nv_bfloat162 r = __hmin2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t max_nan2(uint32_t a, uint32_t b) {
+    __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<uint32_t*>(&r);
+}
+
+// One warp per (request, touched page, kv head): half-warps take alternate token rows, 16 bytes a
+// lane, all eight row loads in flight. Rows at or behind the context's end are not read.
+__global__ void __launch_bounds__(kBoundWarps * 32)
+page_bounds_kernel(const __nv_bfloat16* __restrict__ k_pool, int pool_pages,
+                   const int* __restrict__ page_table, int max_pages,
+                   const int* __restrict__ seq_lens, const int* __restrict__ q_indptr, int max_q_len,
+                   int hkv, int pages_per_req, int64_t total, __nv_bfloat16* __restrict__ bounds,
+                   int* err) {
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31;
+    const int64_t wid = static_cast<int64_t>(blockIdx.x) * kBoundWarps + (threadIdx.x >> 5);
+    if (wid >= total) return;
+    const int h = static_cast<int>(wid % hkv);
+    const int64_t rp = wid / hkv;
+    const int p = static_cast<int>(rp % pages_per_req), r = static_cast<int>(rp / pages_per_req);
+    const bool report = p == 0 && h == 0 && lane == 0;
+    Window w = request_window(r, seq_lens, q_indptr, max_pages * kPage, report, err);
+    if (w.qn > max_q_len) {
+        if (report) record_error(err, MSGL_ERR_BOUNDS, 801);
+        w.qn = max_q_len;
+    }
+    if (w.qn <= 0 || w.L == 0) return;
+    const int page = max(w.L - w.qn, 0) / kPage + p;
+    if (page * kPage >= w.L) return;
+    const int phys = page_table[static_cast<int64_t>(r) * max_pages + page];
+    if (static_cast<unsigned>(phys) >= static_cast<unsigned>(pool_pages)) {
+        if (h == 0 && lane == 0) record_error(err, MSGL_ERR_BOUNDS, 802);
+        return;
+    }
+    const int rows = min(kPage, w.L - page * kPage);
+    const int half = lane >> 4, col = (lane & 15) * 8;
+    const int64_t stride = static_cast<int64_t>(hkv) * kHd;
+    const __nv_bfloat16* src = k_pool + (static_cast<int64_t>(phys) * kPage) * stride + h * kHd + col;
+    uint4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {  // a missing row repeats row 0
+        const int row = 2 * i + half;
+        v[i] = *reinterpret_cast<const uint4*>(src + (row < rows ? row : 0) * stride);
+    }
+    uint32_t lo[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+    uint32_t hi[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            lo[e] = min_nan2(lo[e], u[e]);
+            hi[e] = max_nan2(hi[e], u[e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        lo[e] = min_nan2(lo[e], __shfl_xor_sync(0xffffffffu, lo[e], 16));
+        hi[e] = max_nan2(hi[e], __shfl_xor_sync(0xffffffffu, hi[e], 16));
+    }
+    __nv_bfloat16* dst = bounds + ((static_cast<int64_t>(phys) * hkv + h) * 2 + half) * kHd + col;
+    *reinterpret_cast<uint4*>(dst) = half ? make_uint4(hi[0], hi[1], hi[2], hi[3])
+                                          : make_uint4(lo[0], lo[1], lo[2], lo[3]);
+}
+
+// ------------------------------------------------------------------ scores
+// Scores of 64 pages (16 a warp) for a tile of one request's query rows. The bounds of 16 pages
+// are the A operand (16 x 256: lo then hi) and stay in registers; the B operand is (min(q, 0),
+// max(q, 0)) of 8 columns = 8 / G tokens x G query heads. Both are loaded straight from global
+// memory as 16-byte pieces: lane (g, c) takes elements 32 i + 8 c .. + 7 of row g, which fixes one
+// order of the 256 products for A and B alike.
+constexpr int kScoreWarps = 4;
+constexpr int kScorePages = kScoreWarps * 16;
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t abs2(uint32_t a) { return a & 0x7fff7fffu; }
+
+struct SelectArgs {
+    const __nv_bfloat16 *q, *bounds;
+    int pool_pages;
+    const int* page_table;
+    int max_pages;
+    const int *seq_lens, *q_indptr;
+    int num_reqs, total_q, max_q_len, max_len;
+    int hq, hkv, top, sink, recent;
+    int t0, t1;        // query rows of this launch
+    int stride;        // pages per score row
+    float *scores, *mags;
+    int* page_ids;
+    int* err;
+};
+
+template <int G>
+__global__ void __launch_bounds__(kScoreWarps * 32)
+page_scores_kernel(const SelectArgs a, int tile_rows, int tiles, int page_tiles) {
+    pdl_wait();
+    pdl_trigger();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    int64_t id = blockIdx.x;
+    const int pt = static_cast<int>(id % page_tiles);
+    id /= page_tiles;
+    const int h = static_cast<int>(id % a.hkv);
+    id /= a.hkv;
+    const int tile = static_cast<int>(id % tiles), r = static_cast<int>(id / tiles);
+    const bool report = pt == 0 && h == 0 && tile == 0 && threadIdx.x == 0;
+    const Window w = request_window(r, a.seq_lens, a.q_indptr, a.max_len, report, a.err);
+    if (report && (w.qn > a.max_q_len || w.qn < 0 || w.q0 < 0 || w.q0 + static_cast<int64_t>(w.qn) > a.total_q))
+        record_error(a.err, MSGL_ERR_BOUNDS, 801);
+    const int first = max(w.q0, a.t0);  // the request's first row of this launch: holds its mags
+    const int i0 = max(tile * tile_rows, first - w.q0);
+    const int i1 = min(min(w.qn, a.max_q_len), min((tile + 1) * tile_rows, a.t1 - w.q0));
+    if (w.q0 < 0 || i0 >= i1) return;
+    const int seen = (w.L - w.qn + i1 - 1) >> 4;  // pages before the last row's own page
+    const int last = seen + 1 - a.recent;         // pages [sink, last) are scored
+    if (seen + 1 <= a.top) return;                // every row of the tile sees all its pages
+    const int pg0 = pt * kScorePages + warp * 16;
+    if (pg0 >= last || pg0 + 16 <= a.sink) return;
+
+    uint32_t af[8][2][4];
+    float mag[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int page = pg0 + g + 8 * u;
+        int phys = -1;
+        if (page < last) {
+            phys = a.page_table[static_cast<int64_t>(r) * a.max_pages + page];
+            if (static_cast<unsigned>(phys) >= static_cast<unsigned>(a.pool_pages)) {
+                record_error(a.err, MSGL_ERR_BOUNDS, 802);
+                phys = -1;
+            }
+        }
+        const __nv_bfloat16* src = a.bounds + (static_cast<int64_t>(max(phys, 0)) * a.hkv + h) * 2 * kHd + 8 * c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (phys >= 0) v = *reinterpret_cast<const uint4*>(src + 32 * i);
+            af[i][u][0] = v.x; af[i][u][1] = v.y; af[i][u][2] = v.z; af[i][u][3] = v.w;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {  // largest magnitude of the page's bounds
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m = max_nan2(m, abs2(af[i][u][e]));
+        mag[u] = fmaxf(bf16lo(m), bf16hi(m));
+        mag[u] = fmaxf(mag[u], __shfl_xor_sync(0xffffffffu, mag[u], 1));
+        mag[u] = fmaxf(mag[u], __shfl_xor_sync(0xffffffffu, mag[u], 2));
+        const int page = pg0 + g + 8 * u;
+        if (c == 0 && page < last)
+            a.mags[(static_cast<int64_t>(first - a.t0) * a.hkv + h) * a.stride + page] = mag[u];
+    }
+
+    constexpr int TPN = 8 / G;  // tokens per 8-column tile
+    for (int i = i0; i < i1; i += TPN) {
+        const int tok = i + g / G, head = g % G;
+        const bool live = tok < i1;
+        const __nv_bfloat16* qr =
+            a.q + (static_cast<int64_t>(w.q0 + tok) * a.hq + h * G + head) * kHd + 8 * c;
+        uint32_t qf[4][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (live) v = *reinterpret_cast<const uint4*>(qr + 32 * k);
+            qf[k][0] = v.x; qf[k][1] = v.y; qf[k][2] = v.z; qf[k][3] = v.w;
+        }
+        float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const uint32_t n0 = min_nan2(qf[k][2 * s], 0u), n1 = min_nan2(qf[k][2 * s + 1], 0u);
+                const uint32_t p0 = max_nan2(qf[k][2 * s], 0u), p1 = max_nan2(qf[k][2 * s + 1], 0u);
+                mma_bf16_16816(d0, af[k][0][2 * s], af[k][1][2 * s], af[k][0][2 * s + 1],
+                               af[k][1][2 * s + 1], n0, n1);
+                mma_bf16_16816(d1, af[4 + k][0][2 * s], af[4 + k][1][2 * s], af[4 + k][0][2 * s + 1],
+                               af[4 + k][1][2 * s + 1], p0, p1);
+            }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int page = pg0 + g + 8 * u;
+            const float v0 = d0[2 * u] + d1[2 * u], v1 = d0[2 * u + 1] + d1[2 * u + 1];
+            if (G == 1) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int tt = i + 2 * c + e;
+                    if (tt < i1 && page < last)
+                        a.scores[(static_cast<int64_t>(w.q0 + tt - a.t0) * a.hkv + h) * a.stride + page] = e ? v1 : v0;
+                }
+            } else {
+                float m = max_nan(v0, v1);
+                if (G >= 4) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                if (G >= 8) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                const int tt = i + 2 * c / G;
+                if ((2 * c) % G == 0 && tt < i1 && page < last)
+                    a.scores[(static_cast<int64_t>(w.q0 + tt - a.t0) * a.hkv + h) * a.stride + page] = m;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ selection
+constexpr int kSelThreads = 256;
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kBandCap = 256;  // fp64 keys kept in shared memory
+
+// Order-preserving integer keys; NaN ranks highest, the two zeros are one value.
+__device__ __forceinline__ uint32_t key_of(float v) {
+    if (v != v) return 0xffffffffu;
+    const uint32_t b = __float_as_uint(v + 0.f);
+    return (b >> 31) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t k) {
+    return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
+}
+__device__ __forceinline__ unsigned long long key_of(double v) {
+    if (v != v) return ~0ull;
+    const unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(v + 0.0));
+    return (b >> 63) ? ~b : b | 0x8000000000000000ull;
+}
+
+struct SelShared {
+    int hist[kBins];
+    int scan[32];
+    unsigned long long red[2 * kSelWarps];
+    unsigned long long band_key[kBandCap];
+    int band_page[kBandCap];
+    float q[8 * kHd];
+    float qnorm[8];
+    float mag[kSelWarps];
+    unsigned long long bc_key;
+    int bc_need, band_n, above_n, req;
+};
+
+// The need-th largest key (1-based) among those the block visits: for_each(f) calls f(key) once
+// per key, spread over the threads in any way, and is executed by every thread. The key range is
+// cut into up to 2048 equal bins of a power-of-two width, the bin that holds the wanted key
+// becomes the next range. On return `need` is the count still to take among keys equal to it.
+template <class ForEach>
+__device__ unsigned long long nth_largest(ForEach for_each, int& need, SelShared& sh) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned long long lo = ~0ull, hi = 0ull;
+    for_each([&](unsigned long long k) {
+        lo = min(lo, k);
+        hi = max(hi, k);
+    });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    if (lane == 0) {
+        sh.red[warp] = lo;
+        sh.red[kSelWarps + warp] = hi;
+    }
+    __syncthreads();
+    for (int i = 0; i < kSelWarps; ++i) {
+        lo = min(lo, sh.red[i]);
+        hi = max(hi, sh.red[kSelWarps + i]);
+    }
+    __syncthreads();
+    while (lo < hi) {
+        const int bits = 64 - __clzll(hi - lo);
+        const int shift = bits > 11 ? bits - 11 : 0;
+        for (int i = threadIdx.x; i < kBins; i += kSelThreads) sh.hist[i] = 0;
+        __syncthreads();
+        for_each([&](unsigned long long k) {
+            if (k >= lo && k <= hi) atomicAdd(&sh.hist[(k - lo) >> shift], 1);
+        });
+        __syncthreads();
+        // thread t counts bins [kBins - 8 (t + 1), kBins - 8 t): from the top
+        constexpr int kPer = kBins / kSelThreads;
+        const int b0 = kBins - kPer * (threadIdx.x + 1);
+        int sum = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) sum += sh.hist[b0 + i];
+        int total;
+        int before = block_excl_scan(sum, sh.scan, total);
+        if (before < need && need <= before + sum) {
+            int b = b0 + kPer - 1;
+            while (before + sh.hist[b] < need) before += sh.hist[b--];
+            sh.bc_key = lo + (static_cast<unsigned long long>(b) << shift);
+            sh.bc_need = need - before;
+        }
+        __syncthreads();
+        lo = sh.bc_key;
+        hi = min(hi, lo + ((1ull << shift) - 1));
+        need = sh.bc_need;
+        __syncthreads();
+    }
+    return lo;
+}
+
+// Score key of one page in fp64, by a whole warp (every lane gets it).
+__device__ unsigned long long exact_key(const __nv_bfloat16* bounds_row, const float* sq, int G, int lane) {
+    const uint2 l = *reinterpret_cast<const uint2*>(bounds_row + 4 * lane);
+    const uint2 u = *reinterpret_cast<const uint2*>(bounds_row + kHd + 4 * lane);
+    const float lo[4] = {bf16lo(l.x), bf16hi(l.x), bf16lo(l.y), bf16hi(l.y)};
+    const float hi[4] = {bf16lo(u.x), bf16hi(u.x), bf16lo(u.y), bf16hi(u.y)};
+    unsigned long long best = 0ull;
+    for (int g = 0; g < G; ++g) {
+        double s = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float q = sq[g * kHd + 4 * lane + e];
+            // fmax / fmin drop a NaN operand: keep it
+            const double p = q != q ? q : fmaxf(q, 0.f), n = q != q ? q : fminf(q, 0.f);
+            s += p * hi[e] + n * lo[e];
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        best = max(best, key_of(s));
+    }
+    return best;
+}
+
+// One CTA per (query row, kv head). Shared memory: the row's keys and a bit per page.
+__global__ void __launch_bounds__(kSelThreads)
+select_pages_kernel(const SelectArgs a) {
+    extern __shared__ uint32_t dyn[];
+    __shared__ SelShared sh;
+    uint32_t* keys = dyn;                  // [stride]
+    uint32_t* chosen = dyn + a.stride;     // [stride / 32 + 1]
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int t = a.t0 + static_cast<int>(blockIdx.x) / a.hkv, h = static_cast<int>(blockIdx.x) % a.hkv;
+    if (a.q_indptr) {  // the request that owns row t
+        if (threadIdx.x == 0) sh.req = -1;
+        __syncthreads();
+        for (int r = threadIdx.x; r < a.num_reqs; r += kSelThreads)
+            if (a.q_indptr[r] <= t && t < a.q_indptr[r + 1]) sh.req = r;
+        __syncthreads();
+    }
+    const int r = a.q_indptr ? sh.req : t;
+    if (r < 0) return;  // a row behind the last sequence: left as it was
+    const bool report = h == 0 && threadIdx.x == 0;
+    const Window w = request_window(r, a.seq_lens, a.q_indptr, a.max_len, report, a.err);
+    int* out = a.page_ids + (static_cast<int64_t>(t) * a.hkv + h) * a.top;
+    if (t - w.q0 >= a.max_q_len) {  // more rows than the caller announced
+        if (report) record_error(a.err, MSGL_ERR_BOUNDS, 801);
+        for (int i = threadIdx.x; i < a.top; i += kSelThreads) out[i] = -1;
+        return;
+    }
+    const int pos = w.L - w.qn + (t - w.q0);
+    const int seen = pos < 0 ? 0 : pos / kPage + 1;
+    if (seen <= a.top) {
+        for (int i = threadIdx.x; i < a.top; i += kSelThreads) out[i] = i < seen ? i : -1;
+        return;
+    }
+    const int first = a.sink, last = seen - a.recent;  // candidates; forced pages outside
+    const int need0 = a.top - a.sink - a.recent;
+    const int G = a.hq / a.hkv;
+    for (int i = threadIdx.x; i < (seen + 31) / 32; i += kSelThreads) chosen[i] = 0;
+
+    // keys, the largest bound magnitude, and the query group's 1-norms
+    const float* srow = a.scores + (static_cast<int64_t>(t - a.t0) * a.hkv + h) * a.stride;
+    const float* mrow = a.mags + (static_cast<int64_t>(max(w.q0, a.t0) - a.t0) * a.hkv + h) * a.stride;
+    float mag = 0.f;
+    for (int j = first + threadIdx.x; j < last; j += kSelThreads) {
+        keys[j] = key_of(srow[j]);
+        mag = fmaxf(mag, mrow[j]);
+    }
+    mag = warp_max(mag);
+    if (lane == 0) sh.mag[warp] = mag;
+    const __nv_bfloat16* qrow = a.q + (static_cast<int64_t>(t) * a.hq + h * G) * kHd;
+    for (int g = warp; g < G; g += kSelWarps) {
+        const uint2 u = *reinterpret_cast<const uint2*>(qrow + g * kHd + 4 * lane);
+        const float v[4] = {bf16lo(u.x), bf16hi(u.x), bf16lo(u.y), bf16hi(u.y)};
+        float n = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            sh.q[g * kHd + 4 * lane + e] = v[e];
+            n += fabsf(v[e]);
+        }
+        n = warp_sum(n);
+        if (lane == 0) sh.qnorm[g] = n;
+    }
+    if (threadIdx.x == 0) sh.band_n = sh.above_n = 0;
+    __syncthreads();
+    if (need0 > 0) {
+        // |fp32 score - exact| <= 2^-13 sum |products| <= 2^-13 |q|_1 max|bound|: two chains of 8
+        // MMA steps of 16 products and one addition round or truncate at most 2^-22 of the partial
+        // sums' magnitude per product (2^-14 in all); the factor 2 is margin.
+        float scale = 0.f;
+        for (int g = 0; g < G; ++g) scale = fmaxf(scale, sh.qnorm[g] != sh.qnorm[g] ? __builtin_huge_valf() : sh.qnorm[g]);
+        mag = 0.f;
+        for (int i = 0; i < kSelWarps; ++i) mag = fmaxf(mag, sh.mag[i]);
+        scale *= mag;
+        const bool bounded = scale < 1e37f;  // else fp32 may have overflowed: all pages again in fp64
+        const float eps = scale * 1.220703125e-4f + 1e-30f;
+
+        int need = need0;
+        const auto approx = [&](auto f) {
+            for (int j = first + threadIdx.x; j < last; j += kSelThreads) f(static_cast<unsigned long long>(keys[j]));
+        };
+        const uint32_t kth = static_cast<uint32_t>(nth_largest(approx, need, sh));
+        // exact k-th largest is within eps of the approximate one, so pages more than 2 eps above
+        // are in, more than 2 eps below are out
+        uint32_t top_key = 0xffffffffu, low_key = 0u;
+        if (bounded) {
+            if (kth == 0xffffffffu) {
+                low_key = kth;
+            } else {
+                const float v = value_of(kth);
+                top_key = key_of(__fadd_ru(v, 2.f * eps));
+                low_key = key_of(__fadd_rd(v, -2.f * eps));
+            }
+        }
+        int above = 0, band = 0;
+        for (int j = first + threadIdx.x; j < last; j += kSelThreads) {
+            const uint32_t k = keys[j];
+            if (k > top_key) {
+                ++above;
+                atomicOr(&chosen[j >> 5], 1u << (j & 31));
+            } else if (k >= low_key) {
+                ++band;
+            }
+        }
+        above = __reduce_add_sync(0xffffffffu, above);
+        band = __reduce_add_sync(0xffffffffu, band);
+        if (lane == 0) {
+            if (above) atomicAdd(&sh.above_n, above);
+            if (band) atomicAdd(&sh.band_n, band);
+        }
+        __syncthreads();
+        const int want = need0 - sh.above_n, nband = sh.band_n;
+        __syncthreads();
+        const auto in_band = [&](int j) { return keys[j] >= low_key && keys[j] <= top_key; };
+        const auto row_of = [&](int j) {
+            int phys = a.page_table[static_cast<int64_t>(r) * a.max_pages + j];
+            if (static_cast<unsigned>(phys) >= static_cast<unsigned>(a.pool_pages)) phys = 0;
+            return a.bounds + (static_cast<int64_t>(phys) * a.hkv + h) * 2 * kHd;
+        };
+        if (nband == want) {
+            for (int j = first + threadIdx.x; j < last; j += kSelThreads)
+                if (in_band(j)) atomicOr(&chosen[j >> 5], 1u << (j & 31));
+        } else if (nband <= kBandCap) {
+            if (threadIdx.x == 0) sh.band_n = 0;
+            __syncthreads();
+            for (int j = first + threadIdx.x; j < last; j += kSelThreads)
+                if (in_band(j)) sh.band_page[atomicAdd(&sh.band_n, 1)] = j;
+            __syncthreads();
+            for (int i = warp; i < nband; i += kSelWarps) {
+                const unsigned long long k = exact_key(row_of(sh.band_page[i]), sh.q, G, lane);
+                if (lane == 0) sh.band_key[i] = k;
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < nband; i += kSelThreads) {  // rank by (key, lower page)
+                const unsigned long long k = sh.band_key[i];
+                const int j = sh.band_page[i];
+                int rank = 0;
+                for (int o = 0; o < nband; ++o)
+                    rank += sh.band_key[o] > k || (sh.band_key[o] == k && sh.band_page[o] < j);
+                if (rank < want) atomicOr(&chosen[j >> 5], 1u << (j & 31));
+            }
+        } else {
+            // a wide band (equal pages, huge values): the same search on fp64 keys, computed again
+            // in every pass by a warp per page
+            const auto exact = [&](auto f) {
+                for (int j0 = first + warp * 32; j0 < last; j0 += kSelWarps * 32) {
+                    unsigned m = __ballot_sync(0xffffffffu, j0 + lane < last && in_band(j0 + lane));
+                    while (m) {
+                        const int j = j0 + __ffs(m) - 1;
+                        m &= m - 1;
+                        const unsigned long long k = exact_key(row_of(j), sh.q, G, lane);
+                        if (lane == 0) f(k);
+                    }
+                }
+            };
+            int eq = want;
+            const unsigned long long edge = nth_largest(exact, eq, sh);
+            // pages above the edge, and the first `eq` pages at it: the ones at it are marked in
+            // the keys (0 = not at the edge) and counted in page order
+            for (int j0 = first + warp * 32; j0 < last; j0 += kSelWarps * 32) {
+                const bool mine = j0 + lane < last && in_band(j0 + lane);
+                unsigned m = __ballot_sync(0xffffffffu, mine);
+                unsigned at = 0;
+                while (m) {
+                    const int b = __ffs(m) - 1;
+                    m &= m - 1;
+                    const unsigned long long k = exact_key(row_of(j0 + b), sh.q, G, lane);
+                    if (k > edge) {
+                        if (lane == 0) atomicOr(&chosen[(j0 + b) >> 5], 1u << ((j0 + b) & 31));
+                    } else if (k == edge) {
+                        at |= 1u << b;
+                    }
+                }
+                if (j0 + lane < last) keys[j0 + lane] = (at >> lane) & 1u;
+            }
+            __syncthreads();
+            int taken = 0;
+            for (int j0 = first; j0 < last && taken < eq; j0 += kSelThreads) {
+                const int j = j0 + threadIdx.x;
+                const int one = j < last ? static_cast<int>(keys[j]) : 0;
+                int total;
+                const int before = taken + block_excl_scan(one, sh.scan, total);
+                if (one && before < eq) atomicOr(&chosen[j >> 5], 1u << (j & 31));
+                taken += total;
+            }
+        }
+        __syncthreads();
+    }
+    // ascending output: sink pages, the chosen ones, the recent pages
+    for (int i = threadIdx.x; i < a.sink; i += kSelThreads) out[i] = i;
+    int at = a.sink;
+    const int words = (seen + 31) / 32;
+    for (int w0 = 0; w0 < words; w0 += kSelThreads) {
+        const int wd = w0 + threadIdx.x;
+        uint32_t bits = wd < words ? chosen[wd] : 0u;
+        int total;
+        int o = at + block_excl_scan(__popc(bits), sh.scan, total);
+        while (bits) {
+            out[o++] = wd * 32 + __ffs(bits) - 1;
+            bits &= bits - 1;
+        }
+        at += total;
+    }
+    for (int i = threadIdx.x; i < a.recent; i += kSelThreads) out[a.top - a.recent + i] = last + i;
+}
+
+// ------------------------------------------------------------------ attention over the lists
+// One CTA per (tile of one request's query rows, kv head): TQ = min(8, 16 / G) rows of a chunk,
+// one row in decode; the 16 MMA rows are tile row x query head. The rows' lists are joined into
+// one ascending list of pages with a mask of the rows that asked for each, so a page that several
+// neighbouring queries chose is loaded once. Four warps take the joined pages in turn, each with
+// a ring of its own (cp.async, 16 bytes a lane), an online softmax, and their partial results are
+// joined at the end.
+constexpr int kAttWarps = 4;
+constexpr int kAttThreads = kAttWarps * 32;
+constexpr int kAttStages = 3;
+constexpr int kPageBytes = 2 * kPage * kHd * 2;  // K and V of one page and kv head
+constexpr int kAttRing = kAttWarps * kAttStages * kPageBytes;
+
+struct AttArgs {
+    const __nv_bfloat16 *q, *k_pool, *v_pool;
+    int pool_pages;
+    const int* page_table;
+    int max_pages;
+    const int *seq_lens, *q_indptr;
+    int total_q, max_q_len, max_len;
+    const int* page_ids;
+    int top, hq, hkv;
+    float sl2e;
+    __nv_bfloat16* out;
+    int* err;
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// One page (16 keys) for one warp. K and V tiles: halves of 64 dims, rows of 128 bytes, 16-byte
+// pieces swizzled by the row. lim0 / lim1: last visible offset in the page for MMA rows g / g + 8
+// (< 0: the page is not of that row). With `part`, only rows whose own limit is >= 0 take the new
+// sums (the others' P is zero, but zero times a NaN or infinite value of a page that is not theirs
+// must not reach them), and V rows behind vlim count as zero for the same reason.
+template <bool TWO>
+__device__ __forceinline__ void attend(uint32_t base, const uint32_t (&qa)[8][4], float (&o)[16][4],
+                                       float (&m)[2], float (&l)[2], int lim0, int lim1, bool part,
+                                       int vlim, float sl2e, int lane) {
+    const int mi = lane >> 3, c = lane & 3;
+    float s[2][4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+        const int row = ((mi >> 1) << 3) + (lane & 7);
+        const int piece = ((kk & 3) << 1) + (mi & 1);
+        uint32_t b0, b1, b2, b3;
+        ldsm_x4(base + ((kk >> 2) << 11) + row * 128 + ((piece ^ (row & 7)) << 4), b0, b1, b2, b3);
+        mma_bf16_16816(s[0], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], b0, b1);
+        mma_bf16_16816(s[1], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], b2, b3);
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int tk = n * 8 + 2 * c + e;
+            s[n][e] = tk <= lim0 ? s[n][e] * sl2e : kNegInf;
+            if (TWO) s[n][2 + e] = tk <= lim1 ? s[n][2 + e] * sl2e : kNegInf;
+        }
+    float p[2][4];
+#pragma unroll
+    for (int r = 0; r < (TWO ? 2 : 1); ++r) {
+        float mx = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float m_new = fmaxf(m[r], mx);
+        float alpha = 1.f, ref = 0.f;
+        if (m_new != kNegInf) {
+            alpha = exp2f(m[r] - m_new);
+            ref = m_new;
+        }
+        float ps = 0.f;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float v = exp2f(s[n][2 * r + e] - ref);
+                p[n][2 * r + e] = v;
+                ps += v;
+            }
+        l[r] = l[r] * alpha + ps;
+        m[r] = m_new;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            o[j][2 * r] *= alpha;
+            o[j][2 * r + 1] *= alpha;
+        }
+    }
+    // P in bf16, as V is: relative error 2^-9 a weight, averaged over the keys
+    const uint32_t pa0 = pack_bf16x2(p[0][0], p[0][1]);
+    const uint32_t pa2 = pack_bf16x2(p[1][0], p[1][1]);
+    const uint32_t pa1 = TWO ? pack_bf16x2(p[0][2], p[0][3]) : 0u;
+    const uint32_t pa3 = TWO ? pack_bf16x2(p[1][2], p[1][3]) : 0u;
+    const uint32_t vb = base + kPageBytes / 2;
+    // V fragments hold tokens (2c, 2c + 1) and (2c + 8, 2c + 9)
+    uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+    if (part) {
+        keep0 = (2 * c <= vlim ? 0xffffu : 0u) | (2 * c + 1 <= vlim ? 0xffff0000u : 0u);
+        keep1 = (2 * c + 8 <= vlim ? 0xffffu : 0u) | (2 * c + 9 <= vlim ? 0xffff0000u : 0u);
+    }
+#pragma unroll
+    for (int j2 = 0; j2 < 8; ++j2) {
+        const int row = ((mi & 1) << 3) + (lane & 7);
+        const int piece = ((j2 & 3) << 1) + (mi >> 1);
+        uint32_t b0, b1, b2, b3;
+        ldsm_x4_t(vb + ((j2 >> 2) << 11) + row * 128 + ((piece ^ (row & 7)) << 4), b0, b1, b2, b3);
+        if (!part) {
+            mma_bf16_16816(o[2 * j2], pa0, pa1, pa2, pa3, b0, b1);
+            mma_bf16_16816(o[2 * j2 + 1], pa0, pa1, pa2, pa3, b2, b3);
+        } else {
+            float d[2][4];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) d[n][e] = o[2 * j2 + n][e];
+            mma_bf16_16816(d[0], pa0, pa1, pa2, pa3, b0 & keep0, b1 & keep1);
+            mma_bf16_16816(d[1], pa0, pa1, pa2, pa3, b2 & keep0, b3 & keep1);
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if ((e < 2 ? lim0 : lim1) >= 0) o[2 * j2 + n][e] = d[n][e];
+        }
+    }
+}
+
+template <bool CHUNK>
+__global__ void __launch_bounds__(kAttThreads, 2)
+attend_pages_kernel(const AttArgs a, int tiles, int words) {
+    constexpr bool TWO = CHUNK;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int G = a.hq / a.hkv;
+    const int TQ = CHUNK ? min(8, 16 / G) : 1;
+    uint8_t* ring = smem;                                                    // kAttRing
+    uint32_t* bits = reinterpret_cast<uint32_t*>(smem + kAttRing);           // [TQ][words]
+    int* list_phys = reinterpret_cast<int*>(bits + TQ * words);              // [min(TQ top, 32 words)]
+    const int cap = min(TQ * a.top, 32 * words);
+    uint32_t* list_info = reinterpret_cast<uint32_t*>(list_phys + cap);      // page << 8 | row mask
+    __shared__ int scan[32];
+
+    pdl_wait();
+    pdl_trigger();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    int64_t id = blockIdx.x;
+    const int h = static_cast<int>(id % a.hkv);
+    id /= a.hkv;
+    const int tile = static_cast<int>(id % tiles), r = static_cast<int>(id / tiles);
+    const bool report = tile == 0 && h == 0 && threadIdx.x == 0;
+    const Window w = request_window(r, a.seq_lens, a.q_indptr, a.max_len, report, a.err);
+    const bool fits = w.q0 >= 0 && w.qn >= 0 && w.qn <= a.max_q_len && w.q0 + static_cast<int64_t>(w.qn) <= a.total_q;
+    if (report && !fits) record_error(a.err, MSGL_ERR_BOUNDS, 801);
+    const int i0 = tile * TQ;
+    const int rows = min(TQ, w.qn - i0);
+    if (!fits || rows <= 0) return;
+    const int pos0 = w.L - w.qn + i0;                         // position of the tile's first row
+
+    // ---- the rows' lists as bit sets, then one joined list
+    for (int i = threadIdx.x; i < TQ * words; i += kAttThreads) bits[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * a.top; i += kAttThreads) {
+        const int row = i / a.top;
+        const int page = a.page_ids[(static_cast<int64_t>(w.q0 + i0 + row) * a.hkv + h) * a.top + (i - row * a.top)];
+        if (page < 0) continue;
+        const int pos = pos0 + row;
+        if (pos < 0 || page > pos / kPage) {
+            record_error(a.err, MSGL_ERR_BOUNDS, 803);
+            continue;
+        }
+        atomicOr(&bits[row * words + (page >> 5)], 1u << (page & 31));
+    }
+    __syncthreads();
+    int count = 0;
+    for (int w0 = 0; w0 < words; w0 += kAttThreads) {
+        const int wd = w0 + threadIdx.x;
+        uint32_t any = 0;
+        if (wd < words)
+            for (int row = 0; row < TQ; ++row) any |= bits[row * words + wd];
+        int total;
+        int at = count + block_excl_scan(__popc(any), scan, total);
+        while (any) {
+            const int b = __ffs(any) - 1;
+            any &= any - 1;
+            uint32_t mask = 0;
+            for (int row = 0; row < TQ; ++row) mask |= ((bits[row * words + wd] >> b) & 1u) << row;
+            const int page = wd * 32 + b;
+            int phys = a.page_table[static_cast<int64_t>(r) * a.max_pages + page];
+            if (static_cast<unsigned>(phys) >= static_cast<unsigned>(a.pool_pages)) {
+                record_error(a.err, MSGL_ERR_BOUNDS, 802);
+                phys = 0;
+            }
+            list_phys[at] = phys;
+            list_info[at] = static_cast<uint32_t>(page) << 8 | mask;
+            ++at;
+        }
+        count += total;
+    }
+    __syncthreads();
+
+    // ---- this warp's pages: warp, warp + 4, ...
+    const int row0 = g / G, row1 = (g + 8) / G;  // tile rows of MMA rows g, g + 8
+    uint32_t qa[8][4];
+    {
+        const bool real0 = row0 < rows, real1 = TWO && row1 < rows;
+        const __nv_bfloat16* qr = a.q + (static_cast<int64_t>(w.q0 + i0) * a.hq + h * G) * kHd;
+        const __nv_bfloat16* q0p = qr + (static_cast<int64_t>(row0) * a.hq + g % G) * kHd;
+        const __nv_bfloat16* q1p = qr + (static_cast<int64_t>(row1) * a.hq + (g + 8) % G) * kHd;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+            qa[kk][0] = real0 ? *reinterpret_cast<const uint32_t*>(q0p + 16 * kk + 2 * c) : 0u;
+            qa[kk][2] = real0 ? *reinterpret_cast<const uint32_t*>(q0p + 16 * kk + 8 + 2 * c) : 0u;
+            qa[kk][1] = real1 ? *reinterpret_cast<const uint32_t*>(q1p + 16 * kk + 2 * c) : 0u;
+            qa[kk][3] = real1 ? *reinterpret_cast<const uint32_t*>(q1p + 16 * kk + 8 + 2 * c) : 0u;
+        }
+    }
+    float o[16][4];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    float m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};
+
+    const int mine = count > warp ? (count - warp + kAttWarps - 1) / kAttWarps : 0;
+    const uint32_t ring0 = smem_u32(ring) + warp * kAttStages * kPageBytes;
+    const int64_t stride = static_cast<int64_t>(a.hkv) * kHd;
+    const int last_pos = pos0 + rows - 1;
+    const auto issue = [&](int i) {
+        const int e = warp + i * kAttWarps;
+        const uint32_t dst = ring0 + (i % kAttStages) * kPageBytes;
+        const int live = last_pos - static_cast<int>(list_info[e] >> 8) * kPage;  // last row to load
+        const int64_t off = static_cast<int64_t>(list_phys[e]) * kPage * stride + h * kHd;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            const int row = 2 * x + (lane >> 4), piece = lane & 15;
+            const int64_t src = off + row * stride + piece * 8;
+            const uint32_t d = dst + ((piece >> 3) << 11) + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
+            cp_async16(d, a.k_pool + src, row <= live);  // rows nobody sees are zero-filled
+            cp_async16(d + kPageBytes / 2, a.v_pool + src, row <= live);
+        }
+    };
+    for (int i = 0; i < kAttStages - 1; ++i) {
+        if (i < mine) issue(i);
+        cp_async_commit();
+    }
+    for (int i = 0; i < mine; ++i) {
+        cp_async_wait<kAttStages - 2>();
+        __syncwarp();
+        if (i + kAttStages - 1 < mine) issue(i + kAttStages - 1);
+        cp_async_commit();
+        const uint32_t info = list_info[warp + i * kAttWarps];
+        const uint32_t base = ring0 + (i % kAttStages) * kPageBytes;
+        const int rel = pos0 - static_cast<int>(info >> 8) * kPage;  // first row's position in the page
+        const uint32_t mask = info & 0xffu;
+        if (!CHUNK) {
+            attend<false>(base, qa, o, m, l, rel, -1, false, 0, a.sl2e, lane);
+        } else if (rel >= kPage - 1) {  // the page lies before every row
+            const bool all = mask == (1u << rows) - 1u;
+            attend<true>(base, qa, o, m, l, ((mask >> row0) & 1u) ? kPage : -1,
+                         ((mask >> row1) & 1u) ? kPage : -1, !all, kPage, a.sl2e, lane);
+        } else {  // rows end inside the page: one row after the other
+            for (int row = 0; row < rows; ++row) {
+                if (!((mask >> row) & 1u)) continue;
+                attend<true>(base, qa, o, m, l, row0 == row ? rel + row : -1,
+                             row1 == row ? rel + row : -1, true, rel + row, a.sl2e, lane);
+            }
+        }
+        __syncwarp();
+    }
+
+    // ---- join the warps' results (shared memory over the drained rings)
+    float ls[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        ls[u] = l[u] + __shfl_xor_sync(0xffffffffu, l[u], 1);
+        ls[u] += __shfl_xor_sync(0xffffffffu, ls[u], 2);
+    }
+    cp_async_wait<0>();
+    __syncthreads();
+    constexpr int kRows = TWO ? 16 : 8;
+    float* mo = reinterpret_cast<float*>(ring);          // [4][kRows][128]
+    float* mm = mo + kAttWarps * kRows * kHd;            // [4][kRows]
+    float* ml = mm + kAttWarps * kRows;
+#pragma unroll
+    for (int u = 0; u < (TWO ? 2 : 1); ++u) {
+        const int row = warp * kRows + g + 8 * u;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            *reinterpret_cast<float2*>(mo + row * kHd + 8 * j + 2 * c) = make_float2(o[j][2 * u], o[j][2 * u + 1]);
+        if (c == 0) {
+            mm[row] = m[u];
+            ml[row] = ls[u];
+        }
+    }
+    __syncthreads();
+    for (int item = threadIdx.x; item < rows * G * 16; item += kAttThreads) {
+        const int mr = item >> 4, d0 = (item & 15) * 8;
+        float M = kNegInf;
+        for (int k = 0; k < kAttWarps; ++k) M = fmaxf(M, mm[k * kRows + mr]);
+        float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, L = 0.f;
+        for (int k = 0; k < kAttWarps; ++k) {
+            const float mk = mm[k * kRows + mr];
+            if (mk == kNegInf && ml[k * kRows + mr] == 0.f) continue;  // saw no key
+            const float sc = exp2f(mk - M);
+            L += ml[k * kRows + mr] * sc;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] += mo[(k * kRows + mr) * kHd + d0 + e] * sc;
+        }
+        const float inv = L == 0.f ? 0.f : 1.f / L;  // an empty list gives a zero row
+        uint4 u;
+        u.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+        u.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+        u.z = pack_bf16x2(acc[4] * inv, acc[5] * inv);
+        u.w = pack_bf16x2(acc[6] * inv, acc[7] * inv);
+        const int tr = mr / G;
+        *reinterpret_cast<uint4*>(a.out + (static_cast<int64_t>(w.q0 + i0 + tr) * a.hq + h * G + mr % G) * kHd + d0) = u;
+    }
+}
+
+// ------------------------------------------------------------------ host checks
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int check_heads(int hq, int hkv, int head_dim, int page_size) {
+    if (head_dim != kHd) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "sparse attention: head_dim must be 128");
+    if (page_size != kPage) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "sparse attention: page_size must be 16");
+    if (hkv <= 0 || hq <= 0 || hq % hkv) return set_error(MSGL_ERR_INVALID_ARG, "sparse attention: Hq % Hkv != 0");
+    const int group = hq / hkv;
+    if (group > 8 || (8 % group)) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "sparse attention: Hq/Hkv must be 1,2,4 or 8");
+    return MSGL_OK;
+}
+
+int pages_of(int tokens) { return tokens / kPage + (tokens % kPage != 0); }
+
+// Score rows of one launch pair: as many query rows as keep the scores within 64 MB (they are
+// written and read once, from L2), at least 16.
+constexpr int64_t kScoreBytes = int64_t(64) << 20;
+int slab_rows(int total_q, int stride, int hkv) {
+    const int64_t rows = std::max<int64_t>(16, kScoreBytes / (int64_t(4) * stride * hkv));
+    return static_cast<int>(std::min<int64_t>(total_q, rows));
+}
+int score_stride(int max_seq_len) { return (pages_of(max_seq_len) + 3) / 4 * 4; }
+
+}  // namespace
+}  // namespace msgl
+
+using namespace msgl;
+
+extern "C" {
+
+int msgl_kv_page_bounds(const void* k_pool, int64_t num_slots, const int* page_table, int max_pages,
+                        const int* seq_lens, const int* q_indptr, int num_reqs, int max_q_len,
+                        int num_kv_heads, int head_dim, int page_size, void* bounds,
+                        msgl_stream_t stream) {
+    if (head_dim != kHd) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "kv_page_bounds: head_dim must be 128");
+    if (page_size != kPage) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "kv_page_bounds: page_size must be 16");
+    if (num_kv_heads <= 0 || num_reqs < 0 || max_q_len < 0 || max_pages <= 0 || max_pages > INT32_MAX / kPage ||
+        num_slots <= 0 || num_slots % kPage || num_slots / kPage > INT32_MAX)
+        return set_error(MSGL_ERR_INVALID_ARG, "kv_page_bounds: bad sizes");
+    if (!q_indptr && max_q_len != 1)
+        return set_error(MSGL_ERR_INVALID_ARG, "kv_page_bounds: max_q_len must be 1 without q_indptr");
+    if (num_reqs == 0 || max_q_len == 0) return MSGL_OK;
+    if (!k_pool || !page_table || !seq_lens || !bounds || !aligned16(k_pool) || !aligned16(bounds))
+        return set_error(MSGL_ERR_INVALID_ARG, "kv_page_bounds: null or unaligned pointer");
+    int* err = device_error_word();
+    if (!err) return set_error(MSGL_ERR_CUDA, "device error word unavailable");
+    const int per = std::min<int64_t>((int64_t(max_q_len) + 14) / kPage + 1, max_pages);
+    const int64_t total = int64_t(num_reqs) * per * num_kv_heads;
+    const int64_t blocks = (total + kBoundWarps - 1) / kBoundWarps;
+    if (blocks > INT32_MAX) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "kv_page_bounds: batch too large");
+    launch_pdl(page_bounds_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kBoundWarps * 32), 0, stream,
+               static_cast<const __nv_bfloat16*>(k_pool), static_cast<int>(num_slots / kPage), page_table,
+               max_pages, seq_lens, q_indptr, max_q_len, num_kv_heads, per, total,
+               static_cast<__nv_bfloat16*>(bounds), err);
+    MSGL_LAUNCH_CHECK();
+    return MSGL_OK;
+}
+
+size_t msgl_select_pages_workspace_size(int total_q, int max_seq_len, int num_kv_heads) {
+    if (total_q <= 0 || max_seq_len <= 0 || num_kv_heads <= 0 || pages_of(max_seq_len) > kMaxPagesPerReq) return 0;
+    const int stride = score_stride(max_seq_len);
+    return size_t(2) * slab_rows(total_q, stride, num_kv_heads) * num_kv_heads * stride * sizeof(float);
+}
+
+int msgl_select_pages(const void* q, const void* bounds, int64_t num_pages, const int* page_table,
+                      int max_pages, const int* seq_lens, const int* q_indptr, int num_reqs,
+                      int total_q, int max_q_len, int max_seq_len, int num_q_heads, int num_kv_heads,
+                      int head_dim, int page_size, int top_pages, int sink_pages, int recent_pages,
+                      int* page_ids, void* workspace, size_t workspace_bytes, msgl_stream_t stream) {
+    int rc = check_heads(num_q_heads, num_kv_heads, head_dim, page_size);
+    if (rc) return rc;
+    if (num_reqs < 0 || total_q < 0 || max_q_len < 0 || max_seq_len < 0 || max_pages <= 0 || num_pages <= 0 ||
+        num_pages > INT32_MAX)
+        return set_error(MSGL_ERR_INVALID_ARG, "select_pages: bad sizes");
+    if (!q_indptr && (max_q_len != 1 || total_q != num_reqs))
+        return set_error(MSGL_ERR_INVALID_ARG, "select_pages: one query row per request without q_indptr");
+    if (top_pages <= 0 || sink_pages < 0 || recent_pages < 1 || sink_pages > top_pages - recent_pages)
+        return set_error(MSGL_ERR_INVALID_ARG, "select_pages: need recent_pages >= 1 and sink_pages + recent_pages <= top_pages");
+    if (top_pages > kMaxTopPages) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "select_pages: top_pages > 1024");
+    if (pages_of(max_seq_len) > max_pages)
+        return set_error(MSGL_ERR_INVALID_ARG, "select_pages: max_seq_len exceeds page-table width");
+    if (pages_of(max_seq_len) > kMaxPagesPerReq)
+        return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "select_pages: max_seq_len > 524288");
+    if (num_reqs == 0 || total_q == 0 || max_q_len == 0) return MSGL_OK;
+    if (!q || !bounds || !page_table || !seq_lens || !page_ids || !aligned16(q) || !aligned16(bounds))
+        return set_error(MSGL_ERR_INVALID_ARG, "select_pages: null or unaligned pointer");
+    if (!workspace || !aligned16(workspace) ||
+        workspace_bytes < msgl_select_pages_workspace_size(total_q, max_seq_len, num_kv_heads))
+        return set_error(MSGL_ERR_WORKSPACE, "select_pages: workspace missing, unaligned or too small");
+    SelectArgs a = {};
+    a.q = static_cast<const __nv_bfloat16*>(q);
+    a.bounds = static_cast<const __nv_bfloat16*>(bounds);
+    a.pool_pages = static_cast<int>(num_pages);
+    a.page_table = page_table;
+    a.max_pages = max_pages;
+    a.seq_lens = seq_lens;
+    a.q_indptr = q_indptr;
+    a.num_reqs = num_reqs;
+    a.total_q = total_q;
+    a.max_q_len = max_q_len;
+    a.max_len = max_seq_len;
+    a.hq = num_q_heads;
+    a.hkv = num_kv_heads;
+    a.top = top_pages;
+    a.sink = sink_pages;
+    a.recent = recent_pages;
+    a.page_ids = page_ids;
+    a.err = device_error_word();
+    if (!a.err) return set_error(MSGL_ERR_CUDA, "device error word unavailable");
+    a.stride = std::max(4, score_stride(max_seq_len));
+    const int slab = slab_rows(total_q, a.stride, num_kv_heads);
+    a.scores = static_cast<float*>(workspace);
+    a.mags = a.scores + int64_t(slab) * num_kv_heads * a.stride;
+
+    const int G = num_q_heads / num_kv_heads;
+    const auto score = G == 1 ? page_scores_kernel<1> : G == 2 ? page_scores_kernel<2>
+                       : G == 4 ? page_scores_kernel<4> : page_scores_kernel<8>;
+    const int tile_rows = max_q_len == 1 ? 1 : 64;
+    const int tiles = (max_q_len + tile_rows - 1) / tile_rows;
+    const int page_tiles = (pages_of(max_seq_len) + kScorePages - 1) / kScorePages;
+    const int64_t blocks = int64_t(num_reqs) * tiles * num_kv_heads * page_tiles;
+    const int64_t sel_blocks = int64_t(slab) * num_kv_heads;
+    if (blocks > INT32_MAX || sel_blocks > INT32_MAX)
+        return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "select_pages: batch too large");
+    const size_t smem = (size_t(a.stride) + a.stride / 32 + 2) * sizeof(uint32_t);
+    static std::atomic<int> optin[kMaxDevices];
+    cudaError_t e = smem_optin(select_pages_kernel, smem, optin);
+    if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
+    for (int t0 = 0; t0 < total_q; t0 += slab) {
+        a.t0 = t0;
+        a.t1 = std::min(total_q, t0 + slab);
+        if (page_tiles > 0 && pages_of(max_seq_len) > top_pages) {
+            launch_pdl(score, dim3(static_cast<unsigned>(blocks)), dim3(kScoreWarps * 32), 0, stream, a,
+                       tile_rows, tiles, page_tiles);
+            MSGL_LAUNCH_CHECK();
+        }
+        launch_pdl(select_pages_kernel, dim3((a.t1 - t0) * num_kv_heads), dim3(kSelThreads), smem, stream, a);
+        MSGL_LAUNCH_CHECK();
+    }
+    return MSGL_OK;
+}
+
+int msgl_paged_attention_pages(const void* q, const void* k_pool, const void* v_pool,
+                               int64_t num_slots, const int* page_table, int max_pages,
+                               const int* seq_lens, const int* q_indptr, int num_reqs, int total_q,
+                               int max_q_len, int max_seq_len, const int* page_ids, int top_pages,
+                               int num_q_heads, int num_kv_heads, int head_dim, int page_size,
+                               float scale, void* out, msgl_stream_t stream) {
+    int rc = check_heads(num_q_heads, num_kv_heads, head_dim, page_size);
+    if (rc) return rc;
+    if (num_reqs < 0 || total_q < 0 || max_q_len < 0 || max_seq_len < 0 || max_pages <= 0 || num_slots <= 0 ||
+        num_slots % kPage || num_slots / kPage > INT32_MAX || top_pages <= 0)
+        return set_error(MSGL_ERR_INVALID_ARG, "attention_pages: bad sizes");
+    if (!q_indptr && (max_q_len != 1 || total_q != num_reqs))
+        return set_error(MSGL_ERR_INVALID_ARG, "attention_pages: one query row per request without q_indptr");
+    if (top_pages > kMaxTopPages) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "attention_pages: top_pages > 1024");
+    if (pages_of(max_seq_len) > max_pages)
+        return set_error(MSGL_ERR_INVALID_ARG, "attention_pages: max_seq_len exceeds page-table width");
+    if (pages_of(max_seq_len) > kMaxPagesPerReq)
+        return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "attention_pages: max_seq_len > 524288");
+    if (num_reqs == 0 || total_q == 0 || max_q_len == 0) return MSGL_OK;
+    if (!q || !k_pool || !v_pool || !page_table || !seq_lens || !page_ids || !out || !aligned16(q) ||
+        !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out))
+        return set_error(MSGL_ERR_INVALID_ARG, "attention_pages: null or unaligned pointer");
+    AttArgs a = {};
+    a.q = static_cast<const __nv_bfloat16*>(q);
+    a.k_pool = static_cast<const __nv_bfloat16*>(k_pool);
+    a.v_pool = static_cast<const __nv_bfloat16*>(v_pool);
+    a.pool_pages = static_cast<int>(num_slots / kPage);
+    a.page_table = page_table;
+    a.max_pages = max_pages;
+    a.seq_lens = seq_lens;
+    a.q_indptr = q_indptr;
+    a.total_q = total_q;
+    a.max_q_len = max_q_len;
+    a.max_len = max_seq_len;
+    a.page_ids = page_ids;
+    a.top = top_pages;
+    a.hq = num_q_heads;
+    a.hkv = num_kv_heads;
+    a.sl2e = scale * 1.4426950408889634f;
+    a.out = static_cast<__nv_bfloat16*>(out);
+    a.err = device_error_word();
+    if (!a.err) return set_error(MSGL_ERR_CUDA, "device error word unavailable");
+    const bool chunk = max_q_len > 1;
+    const int G = num_q_heads / num_kv_heads;
+    const int TQ = chunk ? std::min(8, 16 / G) : 1;
+    const int tiles = (max_q_len + TQ - 1) / TQ;
+    const int words = pages_of(max_seq_len) / 32 + 1;
+    const size_t smem = kAttRing + size_t(TQ) * words * 4 + size_t(std::min(TQ * top_pages, 32 * words)) * 8;
+    const int64_t blocks = int64_t(num_reqs) * tiles * num_kv_heads;
+    if (blocks > INT32_MAX) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "attention_pages: batch too large");
+    static std::atomic<int> optin[2][kMaxDevices];
+    const auto kern = chunk ? attend_pages_kernel<true> : attend_pages_kernel<false>;
+    cudaError_t e = smem_optin(kern, smem, optin[chunk]);
+    if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
+    launch_pdl(kern, dim3(static_cast<unsigned>(blocks)), dim3(kAttThreads), smem, stream, a, tiles, words);
+    MSGL_LAUNCH_CHECK();
+    return MSGL_OK;
+}
+
+}  // extern "C"

@@ -32,6 +32,15 @@ SIGNATURES = {
     "msgl_paged_attention_cascade_workspace_size": (SZ, [I, I, I, I, I, I]),
     "msgl_paged_attention_decode_cascade": (I, [P, P, P, I64, P, I, P, I, I, I, I, I, I, I, F, P, P, SZ, P]),
     "msgl_paged_attention_decode_noalloc": (I, [P, P, P, I64, P, I, P, I, I, I, I, I, I, F, P, P]),
+    "msgl_qknorm_mrope_store_kv": (I, [P, P, P, P, I64, P, I64, P, I, P, P, I, P, P, I, I, I, I, F, P]),
+    "msgl_qknorm_mrope_store_kv_partials": (I, [P, I, P, P, P, I64, P, I64, P, I, P, P, I, P, P, I, I, I, I, F, P]),
+    "msgl_kv_page_bounds": (I, [P, I64, P, I, P, P, I, I, I, I, I, P, P]),
+    "msgl_select_pages_workspace_size": (SZ, [I, I, I]),
+    "msgl_select_pages": (I, [P, P, I64, P, I, P, P, I, I, I, I, I, I, I, I, I, I, I, P, P, SZ, P]),
+    "msgl_paged_attention_pages": (I, [P, P, P, I64, P, I, P, P, I, I, I, I, P, I, I, I, I, I, F, P, P]),
+    "msgl_lora_workspace_size": (SZ, [I, I, I]),
+    "msgl_lora_add": (I, [P, I64, P, P, P, I, P, P, I, I, P, I64, P, I64, I, I, I, I, P, SZ, P]),
+    "msgl_lora_partial": (I, [P, I64, P, P, P, I, P, P, I, I, P, I64, I, I, I, I, P, SZ, P]),
     "msgl_gemm_workspace_size": (SZ, [I, I, I]),
     "msgl_gemm_bf16": (I, [P, P, P, I, I, I, I, P, SZ, P]),
     "msgl_pack_gate_up": (I, [P, P, I, I, P]),

@@ -5,12 +5,15 @@ current torch stream. No function here computes anything itself.
 """
 from __future__ import annotations
 
+import ctypes as C
+
 import torch
 
 from ._lib import check, lib
 
 BF16, F32 = 1, 0
 _DT = {torch.bfloat16: BF16, torch.float32: F32}
+_SECTIONS = C.c_int * 3
 
 
 def _s():
@@ -113,6 +116,57 @@ def qknorm_rope_store_kv_partials(parts, k_pool, v_pool, positions, slot_mapping
         _p(slot_mapping), _p(cos_sin), _p(q_norm), _p(k_norm), T, num_q_heads, num_kv_heads,
         head_dim, eps, _s()))
     return q
+
+
+def _mrope_args(positions, sections, interleaved):
+    """Checked [3, T] positions (any row stride), their row stride, and the host section array."""
+    assert positions.is_cuda and positions.dtype == torch.int32, "expected CUDA int32 positions"
+    assert positions.dim() == 2 and positions.shape[0] == 3, "expected positions [3, T]"
+    assert positions.stride(1) == 1 or positions.shape[1] <= 1, "expected contiguous position rows"
+    return positions.stride(0), _SECTIONS(*sections), int(interleaved)
+
+
+def qknorm_mrope_store_kv(qkv, k_pool, v_pool, positions, slot_mapping, cos_sin, q_norm, k_norm,
+                          num_q_heads, num_kv_heads, eps, sections, interleaved=False, head_dim=128,
+                          out=None):
+    """As qknorm_rope_store_kv with positions [3, T] (time, height, width rows) and `sections`, the
+    rotary pairs of each axis (sum head_dim / 2): consecutive ranges, or interleaved."""
+    _c(qkv, torch.bfloat16), _c(k_pool, torch.bfloat16), _c(v_pool, torch.bfloat16)
+    _c(slot_mapping, torch.int32), _c(cos_sin, torch.float32)
+    _c(q_norm, torch.bfloat16), _c(k_norm, torch.bfloat16)
+    stride, sec, layout = _mrope_args(positions, sections, interleaved)
+    T = positions.shape[1]
+    assert qkv.numel() == T * (num_q_heads + 2 * num_kv_heads) * head_dim and slot_mapping.numel() == T
+    if out is None:
+        out = torch.empty(T, num_q_heads, head_dim, dtype=torch.bfloat16, device=qkv.device)
+    num_slots = k_pool.numel() // (num_kv_heads * head_dim)
+    check(lib().msgl_qknorm_mrope_store_kv(
+        _p(qkv), _p(out), _p(k_pool), _p(v_pool), num_slots, _p(positions), stride, sec, layout,
+        _p(slot_mapping), _p(cos_sin), cos_sin.shape[0], _p(q_norm), _p(k_norm), T, num_q_heads,
+        num_kv_heads, head_dim, eps, _s()))
+    return out
+
+
+def qknorm_mrope_store_kv_partials(parts, k_pool, v_pool, positions, slot_mapping, cos_sin, q_norm,
+                                   k_norm, num_q_heads, num_kv_heads, eps, sections,
+                                   interleaved=False, head_dim=128, out=None):
+    """As qknorm_mrope_store_kv with the QKV rows the sum of fp32 partials [P, T, (Hq+2Hkv) D]."""
+    _c(parts, torch.float32), _c(k_pool, torch.bfloat16), _c(v_pool, torch.bfloat16)
+    _c(slot_mapping, torch.int32), _c(cos_sin, torch.float32)
+    _c(q_norm, torch.bfloat16), _c(k_norm, torch.bfloat16)
+    stride, sec, layout = _mrope_args(positions, sections, interleaved)
+    T = positions.shape[1]
+    row = T * (num_q_heads + 2 * num_kv_heads) * head_dim
+    nparts = parts.shape[0]
+    assert parts.numel() == nparts * row and slot_mapping.numel() == T
+    if out is None:
+        out = torch.empty(T, num_q_heads, head_dim, dtype=torch.bfloat16, device=parts.device)
+    num_slots = k_pool.numel() // (num_kv_heads * head_dim)
+    check(lib().msgl_qknorm_mrope_store_kv_partials(
+        _p(parts), nparts, _p(out), _p(k_pool), _p(v_pool), num_slots, _p(positions), stride, sec,
+        layout, _p(slot_mapping), _p(cos_sin), cos_sin.shape[0], _p(q_norm), _p(k_norm), T,
+        num_q_heads, num_kv_heads, head_dim, eps, _s()))
+    return out
 
 
 def decode_advance(next_tokens, input_ids, positions, slot_mapping, page_table, seq_lens,
@@ -219,6 +273,140 @@ def paged_attention_extend(q, k_pool, v_pool, page_table, seq_lens, q_indptr, ma
     return out
 
 
+# ------------------------------------------------------------------ page-sparse attention
+def _rows(page_table, seq_lens, q_indptr, max_q_len, total_q):
+    """Checked request metadata of the page-sparse calls: the request count."""
+    _c(page_table, torch.int32), _c(seq_lens, torch.int32)
+    B = seq_lens.numel()
+    assert page_table.dim() == 2 and page_table.shape[0] == B, "expected a page-table row per request"
+    if q_indptr is None:
+        assert max_q_len == 1 and total_q in (None, B), "one query row per request without q_indptr"
+    else:
+        assert _c(q_indptr, torch.int32).numel() == B + 1, "expected q_indptr [num_reqs + 1]"
+    return B
+
+
+def kv_page_bounds_(bounds, k_pool, page_table, seq_lens, num_kv_heads, q_indptr=None, max_q_len=1,
+                    head_dim=128, page_size=16):
+    """msgl_kv_page_bounds: smallest / largest key of the pages the last rows of each request
+    touch, into bounds [num_pages, Hkv, 2, D] bf16 (in place)."""
+    _c(bounds, torch.bfloat16), _c(k_pool, torch.bfloat16)
+    B = _rows(page_table, seq_lens, q_indptr, max_q_len, None)
+    num_slots = k_pool.numel() // (num_kv_heads * head_dim)
+    assert bounds.numel() * page_size == 2 * k_pool.numel(), "expected bounds [num_pages, Hkv, 2, D]"
+    check(lib().msgl_kv_page_bounds(_p(k_pool), num_slots, _p(page_table), page_table.shape[1],
+                                    _p(seq_lens), _p(q_indptr), B, max_q_len, num_kv_heads,
+                                    head_dim, page_size, _p(bounds), _s()))
+    return bounds
+
+
+def select_pages_workspace(total_q, max_seq_len, num_kv_heads, device="cuda"):
+    n = lib().msgl_select_pages_workspace_size(total_q, max_seq_len, num_kv_heads)
+    return torch.empty(max(n, 256), dtype=torch.uint8, device=device)
+
+
+def select_pages(q, bounds, page_table, seq_lens, max_seq_len, top_pages, hq, hkv, sink_pages=1,
+                 recent_pages=1, q_indptr=None, max_q_len=1, page_size=16, workspace=None, out=None):
+    """msgl_select_pages: page ids [total_q, Hkv, top_pages] int32 for query rows q [total_q, Hq, D]
+    (rows behind the last request: -1 unless `out` is given)."""
+    _c(q, torch.bfloat16), _c(bounds, torch.bfloat16)
+    T = q.numel() // (hq * 128)
+    B = _rows(page_table, seq_lens, q_indptr, max_q_len, T)
+    if workspace is None:
+        workspace = select_pages_workspace(T, max_seq_len, hkv, q.device)
+    if out is None:
+        shape = (T, hkv, top_pages)
+        out = (torch.empty(shape, dtype=torch.int32, device=q.device) if q_indptr is None else
+               torch.full(shape, -1, dtype=torch.int32, device=q.device))
+    assert _c(out, torch.int32).numel() == T * hkv * top_pages
+    check(lib().msgl_select_pages(_p(q), _p(bounds), bounds.numel() // (hkv * 256), _p(page_table),
+                                  page_table.shape[1], _p(seq_lens), _p(q_indptr), B, T, max_q_len,
+                                  max_seq_len, hq, hkv, 128, page_size, top_pages, sink_pages,
+                                  recent_pages, _p(out), _p(workspace), workspace.numel(), _s()))
+    return out
+
+
+def paged_attention_pages(q, k_pool, v_pool, page_table, seq_lens, page_ids, hq, hkv, scale=None,
+                          q_indptr=None, max_q_len=1, max_seq_len=None, page_size=16, out=None):
+    """msgl_paged_attention_pages: attention of q [total_q, Hq, D] over the pages listed in
+    page_ids [total_q, Hkv, top_pages] (select_pages, or lists of the caller's)."""
+    _c(q, torch.bfloat16), _c(k_pool, torch.bfloat16), _c(v_pool, torch.bfloat16)
+    _c(page_ids, torch.int32)
+    T = q.numel() // (hq * 128)
+    B = _rows(page_table, seq_lens, q_indptr, max_q_len, T)
+    assert page_ids.dim() == 3 and page_ids.shape[:2] == (T, hkv), "expected page_ids [total_q, Hkv, top]"
+    assert k_pool.numel() == v_pool.numel(), "expected pools of one size"
+    if scale is None:
+        scale = 1.0 / (128 ** 0.5)
+    if max_seq_len is None:
+        max_seq_len = page_table.shape[1] * page_size
+    if out is None:
+        out = torch.empty_like(q) if q_indptr is None else torch.zeros_like(q)
+    num_slots = k_pool.numel() // (hkv * 128)
+    check(lib().msgl_paged_attention_pages(_p(q), _p(k_pool), _p(v_pool), num_slots, _p(page_table),
+                                           page_table.shape[1], _p(seq_lens), _p(q_indptr), B, T,
+                                           max_q_len, max_seq_len, _p(page_ids), page_ids.shape[2],
+                                           hq, hkv, 128, page_size, scale, _p(_c(out, torch.bfloat16)),
+                                           _s()))
+    return out
+
+
+# ------------------------------------------------------------------ low-rank adapters
+def lora_workspace(num_tokens, K, rank, device="cuda"):
+    n = lib().msgl_lora_workspace_size(num_tokens, K, rank)
+    return torch.empty(max(n, 256), dtype=torch.uint8, device=device)
+
+
+def _r(t, dtype):
+    """A 2-D CUDA tensor with contiguous rows: its row stride."""
+    assert t.is_cuda and t.dtype == dtype and t.dim() == 2, f"expected 2-D CUDA {dtype} rows"
+    assert t.stride(1) == 1 or t.shape[1] == 1, "expected contiguous rows"
+    return max(t.stride(0), t.shape[1])
+
+
+def _lora(x, lora_a, lora_b, scales, adapter_ids, q_indptr, max_q_len, workspace):
+    _c(lora_a, torch.bfloat16), _c(lora_b, torch.bfloat16), _c(scales, torch.float32)
+    _c(adapter_ids, torch.int32)
+    n, R, K = lora_a.shape
+    assert lora_b.shape[0] == n and lora_b.shape[2] == R and scales.numel() == n and x.shape[1] == K
+    B = adapter_ids.numel()
+    if q_indptr is None:
+        assert max_q_len == 1 and B == x.shape[0], "one row per request without q_indptr"
+    else:
+        assert _c(q_indptr, torch.int32).numel() == B + 1, "expected q_indptr [num_reqs + 1]"
+    if workspace is None:
+        workspace = lora_workspace(x.shape[0], K, R, x.device)
+    return (_p(x), _r(x, torch.bfloat16), _p(lora_a), _p(lora_b), _p(scales), n, _p(adapter_ids),
+            _p(q_indptr), B, max_q_len), (x.shape[0], lora_b.shape[1], K, R), workspace
+
+
+def lora_add(x, lora_a, lora_b, scales, adapter_ids, y, q_indptr=None, max_q_len=1, workspace=None,
+             out=None):
+    """msgl_lora_add: y + scales[a] * (x A[a]^T) B[a]^T, a = adapter_ids[r] of the request that owns
+    the row (negative: y as it is). out may be y (in place); rows of x, y, out may be strided."""
+    head, sizes, workspace = _lora(x, lora_a, lora_b, scales, adapter_ids, q_indptr, max_q_len, workspace)
+    if out is None:
+        out = torch.empty(y.shape, dtype=y.dtype, device=y.device) if q_indptr is None else y.clone()
+    assert y.shape == out.shape == sizes[:2], "expected y / out [T, N]"
+    check(lib().msgl_lora_add(*head, _p(y), _r(y, torch.bfloat16), _p(out), _r(out, torch.bfloat16),
+                              *sizes, _p(workspace), workspace.numel(), _s()))
+    return out
+
+
+def lora_partial(x, lora_a, lora_b, scales, adapter_ids, q_indptr=None, max_q_len=1, workspace=None,
+                 out=None):
+    """msgl_lora_partial: fp32 [T, N] scales[a] * (x A[a]^T) B[a]^T, e.g. into the last slab of the
+    partials of linear_partials."""
+    head, sizes, workspace = _lora(x, lora_a, lora_b, scales, adapter_ids, q_indptr, max_q_len, workspace)
+    if out is None:
+        make = torch.empty if q_indptr is None else torch.zeros
+        out = make(sizes[:2], dtype=torch.float32, device=x.device)
+    assert out.shape == sizes[:2], "expected out [T, N]"
+    check(lib().msgl_lora_partial(*head, _p(out), _r(out, torch.float32), *sizes, _p(workspace),
+                                  workspace.numel(), _s()))
+    return out
+
+
 # ------------------------------------------------------------------ GEMMs
 def gemm_workspace(M, N, K, device="cuda"):
     n = lib().msgl_gemm_workspace_size(M, N, K)
@@ -302,7 +490,6 @@ def fill_normal_(t, seed, stream_id=0, mean=0.0, std=1.0):
 
 
 def device_error(reset=True):
-    import ctypes as C
     code, info = C.c_int(0), C.c_int(0)
     check(lib().msgl_device_error(C.addressof(code), C.addressof(info), int(reset), _s()))
     return code.value, info.value
