@@ -309,8 +309,9 @@ MSGL_API int msgl_kv_page_bounds(const void* k_pool, int64_t num_slots, const in
  * recent_pages (>= 1: the row's own page may be incomplete), and of the others the
  * top_pages - sink_pages - recent_pages with the largest
  *   max over the group's heads g of sum_d max(q_gd, 0) hi_d + min(q_gd, 0) lo_d,
- * an upper bound of every q_g . k of the page. Scores compare as in exact arithmetic (near ties are
- * scored again in fp64), equal scores go to the lower page, NaN scores rank highest.
+ * an upper bound of every q_g . k of the page. Scores whose order fp32 cannot tell are compared to
+ * 2^-46 or better, so the choice does not hang on an order of summation; equal scores go to the
+ * lower page, NaN scores rank highest.
  * page_ids [total_q, Hkv, top_pages] int32: logical pages (page-table columns), ascending, filled
  * up with -1. top_pages <= 1024. The workspace (msgl_select_pages_workspace_size, 16-byte aligned)
  * needs no clearing; calls that overlap on the GPU need one each. */

@@ -11,9 +11,9 @@
 // head of the group can have in the page. Bounds are bf16 like the keys, hence exact, and 1/16 of
 // the page's key and value bytes.
 //
-// The selection is the one of exact arithmetic, whatever order the sums are taken in: scores are
-// computed with bf16 MMAs in fp32, and pages whose fp32 score lies within the error bound of the
-// k-th largest are scored again in fp64 (products of bf16 values are exact there).
+// The selection does not hang on the order the sums are taken in: scores are computed with bf16
+// MMAs in fp32, and where the error bound leaves open which page is the k-th, the pages in question
+// are scored again to 2^-46 or better.
 #include <algorithm>
 
 #include "common.cuh"
@@ -145,7 +145,9 @@ struct SelectArgs {
     int hq, hkv, top, sink, recent;
     int t0, t1;        // query rows of this launch
     int stride;        // pages per score row
-    float *scores, *mags;
+    float* scores;             // [rows][Hkv][stride]
+    float* mags;               // [rows][Hkv][stride / 16]: in the request's first row
+    unsigned long long* wide;  // [rows][Hkv][stride]: keys beyond fp32 where many scores are close
     int* page_ids;
     int* err;
 };
@@ -177,7 +179,6 @@ page_scores_kernel(const SelectArgs a, int tile_rows, int tiles, int page_tiles)
     if (pg0 >= last || pg0 + 16 <= a.sink) return;
 
     uint32_t af[8][2][4];
-    float mag[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         const int page = pg0 + g + 8 * u;
@@ -197,19 +198,24 @@ page_scores_kernel(const SelectArgs a, int tile_rows, int tiles, int page_tiles)
             af[i][u][0] = v.x; af[i][u][1] = v.y; af[i][u][2] = v.z; af[i][u][3] = v.w;
         }
     }
+    {   // largest 2-norm of max(|lo|, |hi|) among the 16 pages: what the scores' error scales with
+        float m[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {  // largest magnitude of the page's bounds
-        uint32_t m = 0;
+        for (int u = 0; u < 2; ++u) {
+            m[u] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) m = max_nan2(m, abs2(af[i][u][e]));
-        mag[u] = fmaxf(bf16lo(m), bf16hi(m));
-        mag[u] = fmaxf(mag[u], __shfl_xor_sync(0xffffffffu, mag[u], 1));
-        mag[u] = fmaxf(mag[u], __shfl_xor_sync(0xffffffffu, mag[u], 2));
-        const int page = pg0 + g + 8 * u;
-        if (c == 0 && page < last)
-            a.mags[(static_cast<int64_t>(first - a.t0) * a.hkv + h) * a.stride + page] = mag[u];
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t x = max_nan2(abs2(af[i][u][e]), abs2(af[4 + i][u][e]));
+                    m[u] += bf16lo(x) * bf16lo(x) + bf16hi(x) * bf16hi(x);
+                }
+            m[u] += __shfl_xor_sync(0xffffffffu, m[u], 1);
+            m[u] += __shfl_xor_sync(0xffffffffu, m[u], 2);
+        }
+        const float most = sqrtf(warp_max(fmaxf(m[0], m[1])));
+        if (lane == 0)
+            a.mags[(static_cast<int64_t>(first - a.t0) * a.hkv + h) * (a.stride / 16) + pg0 / 16] = most;
     }
 
     constexpr int TPN = 8 / G;  // tokens per 8-column tile
@@ -261,12 +267,7 @@ page_scores_kernel(const SelectArgs a, int tile_rows, int tiles, int page_tiles)
 }
 
 // ------------------------------------------------------------------ selection
-constexpr int kSelThreads = 256;
-constexpr int kSelWarps = kSelThreads / 32;
-constexpr int kBins = 2048;
-constexpr int kBandCap = 256;  // fp64 keys kept in shared memory
-
-// Order-preserving integer keys; NaN ranks highest, the two zeros are one value.
+// Order-preserving integer keys; NaN ranks highest, the two zeros are one value. No key is 0.
 __device__ __forceinline__ uint32_t key_of(float v) {
     if (v != v) return 0xffffffffu;
     const uint32_t b = __float_as_uint(v + 0.f);
@@ -275,310 +276,437 @@ __device__ __forceinline__ uint32_t key_of(float v) {
 __device__ __forceinline__ float value_of(uint32_t k) {
     return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
 }
+constexpr uint32_t kInfKey = 0xff800000u;  // key_of(+inf): above it only NaN
 __device__ __forceinline__ unsigned long long key_of(double v) {
     if (v != v) return ~0ull;
     const unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(v + 0.0));
     return (b >> 63) ? ~b : b | 0x8000000000000000ull;
 }
 
-struct SelShared {
-    int hist[kBins];
-    int scan[32];
-    unsigned long long red[2 * kSelWarps];
-    unsigned long long band_key[kBandCap];
-    int band_page[kBandCap];
-    float q[8 * kHd];
-    float qnorm[8];
-    float mag[kSelWarps];
-    unsigned long long bc_key;
-    int bc_need, band_n, above_n, req;
-};
-
-// The need-th largest key (1-based) among those the block visits: for_each(f) calls f(key) once
-// per key, spread over the threads in any way, and is executed by every thread. The key range is
-// cut into up to 2048 equal bins of a power-of-two width, the bin that holds the wanted key
-// becomes the next range. On return `need` is the count still to take among keys equal to it.
-template <class ForEach>
-__device__ unsigned long long nth_largest(ForEach for_each, int& need, SelShared& sh) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    unsigned long long lo = ~0ull, hi = 0ull;
-    for_each([&](unsigned long long k) {
-        lo = min(lo, k);
-        hi = max(hi, k);
-    });
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    if (lane == 0) {
-        sh.red[warp] = lo;
-        sh.red[kSelWarps + warp] = hi;
-    }
-    __syncthreads();
-    for (int i = 0; i < kSelWarps; ++i) {
-        lo = min(lo, sh.red[i]);
-        hi = max(hi, sh.red[kSelWarps + i]);
-    }
-    __syncthreads();
-    while (lo < hi) {
-        const int bits = 64 - __clzll(hi - lo);
-        const int shift = bits > 11 ? bits - 11 : 0;
-        for (int i = threadIdx.x; i < kBins; i += kSelThreads) sh.hist[i] = 0;
-        __syncthreads();
-        for_each([&](unsigned long long k) {
-            if (k >= lo && k <= hi) atomicAdd(&sh.hist[(k - lo) >> shift], 1);
-        });
-        __syncthreads();
-        // thread t counts bins [kBins - 8 (t + 1), kBins - 8 t): from the top
-        constexpr int kPer = kBins / kSelThreads;
-        const int b0 = kBins - kPer * (threadIdx.x + 1);
-        int sum = 0;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) sum += sh.hist[b0 + i];
-        int total;
-        int before = block_excl_scan(sum, sh.scan, total);
-        if (before < need && need <= before + sum) {
-            int b = b0 + kPer - 1;
-            while (before + sh.hist[b] < need) before += sh.hist[b--];
-            sh.bc_key = lo + (static_cast<unsigned long long>(b) << shift);
-            sh.bc_need = need - before;
-        }
-        __syncthreads();
-        lo = sh.bc_key;
-        hi = min(hi, lo + ((1ull << shift) - 1));
-        need = sh.bc_need;
-        __syncthreads();
-    }
-    return lo;
-}
-
-// Score key of one page in fp64, by a whole warp (every lane gets it).
-__device__ unsigned long long exact_key(const __nv_bfloat16* bounds_row, const float* sq, int G, int lane) {
-    const uint2 l = *reinterpret_cast<const uint2*>(bounds_row + 4 * lane);
-    const uint2 u = *reinterpret_cast<const uint2*>(bounds_row + kHd + 4 * lane);
-    const float lo[4] = {bf16lo(l.x), bf16hi(l.x), bf16lo(l.y), bf16hi(l.y)};
-    const float hi[4] = {bf16lo(u.x), bf16hi(u.x), bf16lo(u.y), bf16hi(u.y)};
+// Score key of one page beyond fp32, by each group of eight lanes (every lane of the group gets it;
+// all lanes of the warp call it). bounds_row: lo then hi of the page; q: the group's G query heads.
+// A term is q (q > 0 ? hi : lo) plus zero times the other bound (NaN where that is infinite or NaN).
+// With `narrow` (scores well inside the fp32 range) the products of two bf16 values are exact in
+// fp32 and are summed as an unevaluated pair of fp32 values (Knuth's two-sum, about 2^-46 relative),
+// several times faster here than in fp64, which takes the rest. Equal bounds give equal keys. The
+// loops stay rolled: few rows come here, and most of what a long body would cost them is fetching it.
+template <bool NARROW>
+__device__ __noinline__ unsigned long long exact_key(const __nv_bfloat16* __restrict__ bounds_row,
+                                                     const __nv_bfloat16* __restrict__ q, int G, int lane) {
+    const int d = 16 * (lane & 7);
     unsigned long long best = 0ull;
+#pragma unroll 1
     for (int g = 0; g < G; ++g) {
-        double s = 0.0;
+        float sum = 0.f, rest = 0.f;
+        double wide = 0.0;
+        // (sum, rest) += (t, r); the same bits whichever side is which
+        const auto add = [&](float t, float r) {
+            const float n = __fadd_rn(sum, t), z = __fadd_rn(n, -sum);
+            const float err = __fadd_rn(__fadd_rn(sum, -__fadd_rn(n, -z)), __fadd_rn(t, -z));
+            rest = __fadd_rn(__fadd_rn(rest, r), err);
+            sum = n;
+        };
+#pragma unroll 1
+        for (int i = 0; i < 16; i += 8) {
+            const uint4 xv = *reinterpret_cast<const uint4*>(q + g * kHd + d + i);
+            const uint4 lv = *reinterpret_cast<const uint4*>(bounds_row + d + i);
+            const uint4 hv = *reinterpret_cast<const uint4*>(bounds_row + kHd + d + i);
+            const uint32_t x[4] = {xv.x, xv.y, xv.z, xv.w};
+            const uint32_t lo[4] = {lv.x, lv.y, lv.z, lv.w};
+            const uint32_t hi[4] = {hv.x, hv.y, hv.z, hv.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float q = sq[g * kHd + 4 * lane + e];
-            // fmax / fmin drop a NaN operand: keep it
-            const double p = q != q ? q : fmaxf(q, 0.f), n = q != q ? q : fminf(q, 0.f);
-            s += p * hi[e] + n * lo[e];
+            for (int e = 0; e < 8; ++e) {
+                const float f = e & 1 ? bf16hi(x[e >> 1]) : bf16lo(x[e >> 1]);
+                const float l = e & 1 ? bf16hi(lo[e >> 1]) : bf16lo(lo[e >> 1]);
+                const float h = e & 1 ? bf16hi(hi[e >> 1]) : bf16lo(hi[e >> 1]);
+                const float mine = f > 0.f ? h : l, other = __fmul_rn(0.f, f > 0.f ? l : h);
+                if constexpr (NARROW) add(__fmul_rn(f, mine), other);
+                else wide += static_cast<double>(f) * mine + other;
+            }
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        best = max(best, key_of(s));
+#pragma unroll 1
+        for (int o = 4; o > 0; o >>= 1) {
+            if constexpr (NARROW) {
+                const float t = __shfl_xor_sync(0xffffffffu, sum, o);
+                add(t, __shfl_xor_sync(0xffffffffu, rest, o));
+            } else {
+                wide += __shfl_xor_sync(0xffffffffu, wide, o);
+            }
+        }
+        if constexpr (NARROW) {
+            const float top = __fadd_rn(sum, rest), low = __fadd_rn(rest, -__fadd_rn(top, -sum));
+            best = max(best, static_cast<unsigned long long>(key_of(top)) << 32 | key_of(low));
+        } else {
+            best = max(best, key_of(wide));
+        }
     }
     return best;
 }
 
-// One CTA per (query row, kv head). Shared memory: the row's keys and a bit per page.
-__global__ void __launch_bounds__(kSelThreads)
-select_pages_kernel(const SelectArgs a) {
-    extern __shared__ uint32_t dyn[];
-    __shared__ SelShared sh;
-    uint32_t* keys = dyn;                  // [stride]
-    uint32_t* chosen = dyn + a.stride;     // [stride / 32 + 1]
+// Bit number of the lane group's set bit: the group's index (0 .. 3) from the lowest, at most the last.
+__device__ __forceinline__ int group_bit(unsigned m, int lane) {
+    int b = __ffs(m) - 1;
+#pragma unroll
+    for (int e = 1; e < 4; ++e) {
+        m &= m - 1;
+        if (e <= (lane >> 3) && m) b = __ffs(m) - 1;
+    }
+    return b;
+}
+
+constexpr int kListCap = 32;    // candidates resolved by one warp, one a lane
+constexpr int kListGoal = 16;   // the search stops at that many
+
+// The W warps of one row. With W = 1 the CTA's warps hold rows of their own.
+template <int W>
+struct RowGroup {
+    struct Shared {
+        uint32_t red[2][32];
+        unsigned long long red64[2][32];
+        uint32_t key[kListCap];
+        int page[kListCap];
+        int n, req;
+    };
+    Shared& sh;
+    int warp, lane, turn;
+
+    __device__ __forceinline__ void sync() const {
+        if (W == 1) __syncwarp();
+        else __syncthreads();
+    }
+    // Sums / minima / maxima over the row's threads, one barrier each (the slots alternate).
+    template <class Op>
+    __device__ __forceinline__ uint32_t reduce(uint32_t v, uint32_t none, Op op) {
+        v = op(v);
+        if (W == 1) return v;
+        turn ^= 1;
+        if (lane == 0) sh.red[turn][warp] = v;
+        __syncthreads();
+        return op(lane < W ? sh.red[turn][lane] : none);
+    }
+    __device__ __forceinline__ uint32_t sum(uint32_t v) {
+        return reduce(v, 0u, [](uint32_t x) { return __reduce_add_sync(0xffffffffu, x); });
+    }
+    __device__ __forceinline__ uint32_t least(uint32_t v) {
+        return reduce(v, 0xffffffffu, [](uint32_t x) { return __reduce_min_sync(0xffffffffu, x); });
+    }
+    __device__ __forceinline__ uint32_t most(uint32_t v) {
+        return reduce(v, 0u, [](uint32_t x) { return __reduce_max_sync(0xffffffffu, x); });
+    }
+    template <bool MAX>
+    __device__ __forceinline__ unsigned long long pick64(unsigned long long v) {
+        const auto op = [](unsigned long long x) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                const unsigned long long y = __shfl_xor_sync(0xffffffffu, x, o);
+                x = MAX ? max(x, y) : min(x, y);
+            }
+            return x;
+        };
+        v = op(v);
+        if (W == 1) return v;
+        turn ^= 1;
+        if (lane == 0) sh.red64[turn][warp] = v;
+        __syncthreads();
+        return op(lane < W ? sh.red64[turn][lane] : (MAX ? 0ull : ~0ull));
+    }
+    // The count of the warps before this one; v is uniform in a warp.
+    __device__ __forceinline__ uint32_t before(uint32_t v) {
+        if (W == 1) return 0;
+        turn ^= 1;
+        if (lane == 0) sh.red[turn][warp] = v;
+        __syncthreads();
+        return __reduce_add_sync(0xffffffffu, lane < warp ? sh.red[turn][lane] : 0u);
+    }
+};
+
+// W warps per row, K pages per lane: lane l of warp w holds pages 32 (w K + i) + l, i < K, as keys
+// in registers. R rows per CTA (W = 1 only). The k-th largest key is found by bisection of the
+// key range (a count per step); once at most kListGoal keys are left between the bounds, the keys
+// within two error bounds of them go to a list of one key a lane, which one warp resolves by
+// ranks, scored again beyond fp32 where that cannot tell.
+template <int W, int K, int R>
+__global__ void __launch_bounds__(32 * W * R)
+select_pages_kernel(const SelectArgs a, int num_rows) {
+    __shared__ typename RowGroup<W>::Shared shared[R];
+    __shared__ uint32_t picked[R][W * K];  // bits of listed pages that were taken
     pdl_wait();
     pdl_trigger();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int t = a.t0 + static_cast<int>(blockIdx.x) / a.hkv, h = static_cast<int>(blockIdx.x) % a.hkv;
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+    const int slot = W == 1 ? wid : 0;
+    const int id = static_cast<int>(blockIdx.x) * R + slot;
+    if (id >= num_rows) return;
+    auto& sh = shared[slot];
+    RowGroup<W> row{sh, W == 1 ? 0 : wid, lane, 0};
+    const int tid = row.warp * 32 + lane;
+    const int t = a.t0 + id / a.hkv, h = id % a.hkv;
+    int r = t;
     if (a.q_indptr) {  // the request that owns row t
-        if (threadIdx.x == 0) sh.req = -1;
-        __syncthreads();
-        for (int r = threadIdx.x; r < a.num_reqs; r += kSelThreads)
-            if (a.q_indptr[r] <= t && t < a.q_indptr[r + 1]) sh.req = r;
-        __syncthreads();
+        if (tid == 0) sh.req = -1;
+        row.sync();
+        for (int i = tid; i < a.num_reqs; i += 32 * W)
+            if (a.q_indptr[i] <= t && t < a.q_indptr[i + 1]) sh.req = i;
+        row.sync();
+        r = sh.req;
+        if (r < 0) return;  // a row behind the last sequence: left as it was
     }
-    const int r = a.q_indptr ? sh.req : t;
-    if (r < 0) return;  // a row behind the last sequence: left as it was
-    const bool report = h == 0 && threadIdx.x == 0;
+    const bool report = h == 0 && tid == 0;
     const Window w = request_window(r, a.seq_lens, a.q_indptr, a.max_len, report, a.err);
     int* out = a.page_ids + (static_cast<int64_t>(t) * a.hkv + h) * a.top;
     if (t - w.q0 >= a.max_q_len) {  // more rows than the caller announced
         if (report) record_error(a.err, MSGL_ERR_BOUNDS, 801);
-        for (int i = threadIdx.x; i < a.top; i += kSelThreads) out[i] = -1;
+        for (int i = tid; i < a.top; i += 32 * W) out[i] = -1;
         return;
     }
     const int pos = w.L - w.qn + (t - w.q0);
     const int seen = pos < 0 ? 0 : pos / kPage + 1;
     if (seen <= a.top) {
-        for (int i = threadIdx.x; i < a.top; i += kSelThreads) out[i] = i < seen ? i : -1;
+        for (int i = tid; i < a.top; i += 32 * W) out[i] = i < seen ? i : -1;
         return;
     }
     const int first = a.sink, last = seen - a.recent;  // candidates; forced pages outside
-    const int need0 = a.top - a.sink - a.recent;
+    const int need = a.top - a.sink - a.recent;
     const int G = a.hq / a.hkv;
-    for (int i = threadIdx.x; i < (seen + 31) / 32; i += kSelThreads) chosen[i] = 0;
+    for (int i = tid; i < a.sink; i += 32 * W) out[i] = i;
+    for (int i = tid; i < a.recent; i += 32 * W) out[a.top - a.recent + i] = last + i;
+    if (need == 0) return;
 
-    // keys, the largest bound magnitude, and the query group's 1-norms
-    const float* srow = a.scores + (static_cast<int64_t>(t - a.t0) * a.hkv + h) * a.stride;
-    const float* mrow = a.mags + (static_cast<int64_t>(max(w.q0, a.t0) - a.t0) * a.hkv + h) * a.stride;
-    float mag = 0.f;
-    for (int j = first + threadIdx.x; j < last; j += kSelThreads) {
-        keys[j] = key_of(srow[j]);
-        mag = fmaxf(mag, mrow[j]);
-    }
-    mag = warp_max(mag);
-    if (lane == 0) sh.mag[warp] = mag;
+    const int64_t srow = (static_cast<int64_t>(t - a.t0) * a.hkv + h) * a.stride;
+    const float* mrow = a.mags + (static_cast<int64_t>(max(w.q0, a.t0) - a.t0) * a.hkv + h) * (a.stride / 16);
     const __nv_bfloat16* qrow = a.q + (static_cast<int64_t>(t) * a.hq + h * G) * kHd;
-    for (int g = warp; g < G; g += kSelWarps) {
-        const uint2 u = *reinterpret_cast<const uint2*>(qrow + g * kHd + 4 * lane);
-        const float v[4] = {bf16lo(u.x), bf16hi(u.x), bf16lo(u.y), bf16hi(u.y)};
-        float n = 0.f;
+    const int base = row.warp * K * 32 + lane;
+    // all loads first: scores, query rows, magnitudes
+    uint32_t key[K];
+    float mag = 0.f;
+    {
+        const float* __restrict__ scores = a.scores + srow;
+        float v[K];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            sh.q[g * kHd + 4 * lane + e] = v[e];
-            n += fabsf(v[e]);
+        for (int i = 0; i < K; ++i) {
+            const int j = base + 32 * i;
+            v[i] = j >= first && j < last ? scores[j] : 0.f;
         }
-        n = warp_sum(n);
-        if (lane == 0) sh.qnorm[g] = n;
+        for (int j = first / 16 + tid; j <= (last - 1) / 16; j += 32 * W) mag = fmaxf(mag, mrow[j]);
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            const int j = base + 32 * i;
+            key[i] = j >= first && j < last ? key_of(v[i]) : 0u;
+        }
     }
-    if (threadIdx.x == 0) sh.band_n = sh.above_n = 0;
-    __syncthreads();
-    if (need0 > 0) {
-        // |fp32 score - exact| <= 2^-13 sum |products| <= 2^-13 |q|_1 max|bound|: two chains of 8
-        // MMA steps of 16 products and one addition round or truncate at most 2^-22 of the partial
-        // sums' magnitude per product (2^-14 in all); the factor 2 is margin.
-        float scale = 0.f;
-        for (int g = 0; g < G; ++g) scale = fmaxf(scale, sh.qnorm[g] != sh.qnorm[g] ? __builtin_huge_valf() : sh.qnorm[g]);
-        mag = 0.f;
-        for (int i = 0; i < kSelWarps; ++i) mag = fmaxf(mag, sh.mag[i]);
-        scale *= mag;
-        const bool bounded = scale < 1e37f;  // else fp32 may have overflowed: all pages again in fp64
-        const float eps = scale * 1.220703125e-4f + 1e-30f;
+    for (int i = lane; i < K; i += 32) picked[slot][row.warp * K + i] = 0u;
+    // |fp32 score - exact| <= 2^-15 sum |products|: a step of an MMA chain adds 16 products and the
+    // partial sum, each cut at worst at one unit (2^-23) of the largest; 8 steps a chain, half the
+    // products in each of two chains and one addition make 2^-15.9. sum |products| <= |q| |max(|lo|,
+    // |hi|)| (2-norms; the margin left covers their own rounding).
+    float norm = 0.f;  // four lanes a head
+    if (lane >> 2 < G) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint4 u = *reinterpret_cast<const uint4*>(qrow + (lane >> 2) * kHd + 32 * i + 8 * (lane & 3));
+            const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) norm += bf16lo(x[e]) * bf16lo(x[e]) + bf16hi(x[e]) * bf16hi(x[e]);
+        }
+    }
+    norm += __shfl_xor_sync(0xffffffffu, norm, 1);
+    norm += __shfl_xor_sync(0xffffffffu, norm, 2);
+    norm = sqrtf(warp_max(norm != norm ? __builtin_huge_valf() : norm));
+    if (tid == 0) sh.n = 0;
+    row.sync();  // the cleared bits and count
+    uint32_t lo = 0xffffffffu, hi = 0u;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+        lo = min(lo, key[i] ? key[i] : 0xffffffffu);
+        hi = max(hi, key[i]);
+    }
+    lo = row.least(lo);
+    hi = row.most(hi);
+    const float scale = norm * __uint_as_float(row.most(__float_as_uint(mag)));
+    const bool bounded = scale < 1e37f;  // else fp32 may have overflowed: all pages again
+    const bool narrow = scale > 1e-20f && scale < 1e37f;
+    const float eps2 = 2.f * (scale * 3.0517578125e-5f + 1e-30f);  // two errors
 
-        int need = need0;
-        const auto approx = [&](auto f) {
-            for (int j = first + threadIdx.x; j < last; j += kSelThreads) f(static_cast<unsigned long long>(keys[j]));
-        };
-        const uint32_t kth = static_cast<uint32_t>(nth_largest(approx, need, sh));
-        // exact k-th largest is within eps of the approximate one, so pages more than 2 eps above
-        // are in, more than 2 eps below are out
-        uint32_t top_key = 0xffffffffu, low_key = 0u;
-        if (bounded) {
-            if (kth == 0xffffffffu) {
-                low_key = kth;
-            } else {
-                const float v = value_of(kth);
-                top_key = key_of(__fadd_ru(v, 2.f * eps));
-                low_key = key_of(__fadd_rd(v, -2.f * eps));
-            }
-        }
-        int above = 0, band = 0;
-        for (int j = first + threadIdx.x; j < last; j += kSelThreads) {
-            const uint32_t k = keys[j];
-            if (k > top_key) {
-                ++above;
-                atomicOr(&chosen[j >> 5], 1u << (j & 31));
-            } else if (k >= low_key) {
-                ++band;
-            }
-        }
-        above = __reduce_add_sync(0xffffffffu, above);
-        band = __reduce_add_sync(0xffffffffu, band);
-        if (lane == 0) {
-            if (above) atomicAdd(&sh.above_n, above);
-            if (band) atomicAdd(&sh.band_n, band);
-        }
-        __syncthreads();
-        const int want = need0 - sh.above_n, nband = sh.band_n;
-        __syncthreads();
-        const auto in_band = [&](int j) { return keys[j] >= low_key && keys[j] <= top_key; };
-        const auto row_of = [&](int j) {
-            int phys = a.page_table[static_cast<int64_t>(r) * a.max_pages + j];
-            if (static_cast<unsigned>(phys) >= static_cast<unsigned>(a.pool_pages)) phys = 0;
-            return a.bounds + (static_cast<int64_t>(phys) * a.hkv + h) * 2 * kHd;
-        };
-        if (nband == want) {
-            for (int j = first + threadIdx.x; j < last; j += kSelThreads)
-                if (in_band(j)) atomicOr(&chosen[j >> 5], 1u << (j & 31));
-        } else if (nband <= kBandCap) {
-            if (threadIdx.x == 0) sh.band_n = 0;
-            __syncthreads();
-            for (int j = first + threadIdx.x; j < last; j += kSelThreads)
-                if (in_band(j)) sh.band_page[atomicAdd(&sh.band_n, 1)] = j;
-            __syncthreads();
-            for (int i = warp; i < nband; i += kSelWarps) {
-                const unsigned long long k = exact_key(row_of(sh.band_page[i]), sh.q, G, lane);
-                if (lane == 0) sh.band_key[i] = k;
-            }
-            __syncthreads();
-            for (int i = threadIdx.x; i < nband; i += kSelThreads) {  // rank by (key, lower page)
-                const unsigned long long k = sh.band_key[i];
-                const int j = sh.band_page[i];
-                int rank = 0;
-                for (int o = 0; o < nband; ++o)
-                    rank += sh.band_key[o] > k || (sh.band_key[o] == k && sh.band_page[o] < j);
-                if (rank < want) atomicOr(&chosen[j >> 5], 1u << (j & 31));
-            }
+    const auto count_from = [&](uint32_t v) {
+        uint32_t c = 0;
+#pragma unroll
+        for (int i = 0; i < K; ++i) c += key[i] >= v;
+        return static_cast<int>(row.sum(c));
+    };
+    // count(key >= lo) = n_lo >= need > n_hi = count(key > hi)
+    int n_lo = last - first, n_hi = 0;
+    while (bounded && lo < hi && n_lo - n_hi > kListGoal) {
+        const uint32_t mid = hi - ((hi - lo) >> 1);
+        const int c = count_from(mid);
+        if (c >= need) {
+            lo = mid;
+            n_lo = c;
         } else {
-            // a wide band (equal pages, huge values): the same search on fp64 keys, computed again
-            // in every pass by a warp per page
-            const auto exact = [&](auto f) {
-                for (int j0 = first + warp * 32; j0 < last; j0 += kSelWarps * 32) {
-                    unsigned m = __ballot_sync(0xffffffffu, j0 + lane < last && in_band(j0 + lane));
-                    while (m) {
-                        const int j = j0 + __ffs(m) - 1;
+            hi = mid - 1;
+            n_hi = c;
+        }
+    }
+    // every key within two errors of the k-th largest lies in [low, high]
+    uint32_t low = lo, high = hi;
+    if (!bounded) {
+        low = 1u;
+        high = 0xffffffffu;
+    } else {
+        if (lo <= kInfKey) low = key_of(__fadd_rd(value_of(lo), -eps2));
+        high = hi <= kInfKey ? key_of(__fadd_ru(value_of(hi), eps2)) : 0xffffffffu;
+    }
+    uint32_t above = 0, inside = 0;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+        above += key[i] > high;
+        inside += key[i] >= low && key[i] <= high;
+    }
+    const uint32_t both = row.sum(above | inside << 16);
+    const int want = need - static_cast<int>(both & 0xffffu), listed = static_cast<int>(both >> 16);
+    const auto bounds_of = [&](int j) {
+        int phys = a.page_table[static_cast<int64_t>(r) * a.max_pages + j];
+        if (static_cast<unsigned>(phys) >= static_cast<unsigned>(a.pool_pages)) phys = 0;  // recorded
+        return a.bounds + (static_cast<int64_t>(phys) * a.hkv + h) * 2 * kHd;
+    };
+    const auto again = [&](const __nv_bfloat16* b) {
+        return narrow ? exact_key<true>(b, qrow, G, lane) : exact_key<false>(b, qrow, G, lane);
+    };
+    if (listed == want) {
+        high = low - 1;  // all of them
+    } else if (listed <= kListCap) {
+        if (inside) {
+            int p = atomicAdd(&sh.n, static_cast<int>(inside));
+#pragma unroll
+            for (int i = 0; i < K; ++i)
+                if (key[i] >= low && key[i] <= high) {
+                    sh.key[p] = key[i];
+                    sh.page[p++] = base + 32 * i;
+                }
+        }
+        row.sync();
+        if (row.warp == 0) {
+            const uint32_t mine = lane < listed ? sh.key[lane] : 0u;
+            const int page = lane < listed ? sh.page[lane] : 0;
+            int more = 0, same = 0;
+#pragma unroll
+            for (int o = 0; o < 32; ++o) {
+                const uint32_t k = __shfl_sync(0xffffffffu, mine, o);
+                more += k > mine;
+                same += k == mine;
+            }
+            // the keys of rank `want` and `want + 1` (if listed)
+            const unsigned is_kth = __ballot_sync(0xffffffffu, more < want && want <= more + same);
+            const unsigned is_next = __ballot_sync(0xffffffffu, mine && more <= want && want < more + same);
+            const uint32_t kth = __shfl_sync(0xffffffffu, mine, __ffs(is_kth) - 1);
+            const uint32_t next = is_next ? __shfl_sync(0xffffffffu, mine, __ffs(is_next) - 1) : 0u;
+            // A score more than two errors above the next one is larger than all from there on, one
+            // more than two errors below the k-th smaller than k others; the rest is open.
+            uint32_t top_key = 0xffffffffu, low_key = 1u;
+            if (bounded) {
+                low_key = kth > kInfKey ? kth : key_of(__fadd_rd(value_of(kth), -eps2));
+                if (next == 0u) top_key = 0u;
+                else if (next <= kInfKey) top_key = key_of(__fadd_ru(value_of(next), eps2));
+            }
+            bool take = mine > top_key && mine >= low_key;
+            const unsigned open = __ballot_sync(0xffffffffu, mine && !take && mine >= low_key);
+            const int left = want - __popc(__ballot_sync(0xffffffffu, take));
+            if (__popc(open) <= left) {
+                take = take || (open >> lane & 1u);
+            } else {  // scored again, four pages at a time
+                unsigned long long exact = 0ull;
+                for (unsigned m = open; m;) {
+                    const int src = group_bit(m, lane);
+                    const unsigned long long k = again(bounds_of(__shfl_sync(0xffffffffu, page, src)));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const unsigned long long ke = __shfl_sync(0xffffffffu, k, 8 * e);
+                        if (m && lane == __ffs(m) - 1) exact = ke;
                         m &= m - 1;
-                        const unsigned long long k = exact_key(row_of(j), sh.q, G, lane);
-                        if (lane == 0) f(k);
                     }
                 }
-            };
-            int eq = want;
-            const unsigned long long edge = nth_largest(exact, eq, sh);
-            // pages above the edge, and the first `eq` pages at it: the ones at it are marked in
-            // the keys (0 = not at the edge) and counted in page order
-            for (int j0 = first + warp * 32; j0 < last; j0 += kSelWarps * 32) {
-                const bool mine = j0 + lane < last && in_band(j0 + lane);
-                unsigned m = __ballot_sync(0xffffffffu, mine);
-                unsigned at = 0;
-                while (m) {
-                    const int b = __ffs(m) - 1;
-                    m &= m - 1;
-                    const unsigned long long k = exact_key(row_of(j0 + b), sh.q, G, lane);
-                    if (k > edge) {
-                        if (lane == 0) atomicOr(&chosen[(j0 + b) >> 5], 1u << ((j0 + b) & 31));
-                    } else if (k == edge) {
-                        at |= 1u << b;
-                    }
+                int rank = 0;  // by (exact key, lower page)
+                for (unsigned m = open; m; m &= m - 1) {
+                    const int o = __ffs(m) - 1;
+                    const unsigned long long k = __shfl_sync(0xffffffffu, exact, o);
+                    const int p = __shfl_sync(0xffffffffu, page, o);
+                    rank += k > exact || (k == exact && p < page);
                 }
-                if (j0 + lane < last) keys[j0 + lane] = (at >> lane) & 1u;
+                take = take || ((open >> lane & 1u) && rank < left);
             }
-            __syncthreads();
-            int taken = 0;
-            for (int j0 = first; j0 < last && taken < eq; j0 += kSelThreads) {
-                const int j = j0 + threadIdx.x;
-                const int one = j < last ? static_cast<int>(keys[j]) : 0;
-                int total;
-                const int before = taken + block_excl_scan(one, sh.scan, total);
-                if (one && before < eq) atomicOr(&chosen[j >> 5], 1u << (j & 31));
-                taken += total;
+            if (take) atomicOr(&picked[slot][page >> 5], 1u << (page & 31));
+        }
+        row.sync();
+    } else {
+        // more than the list holds (equal pages, values beyond fp32): all of them scored again into
+        // the workspace, bisection of those keys
+        unsigned long long* wide = a.wide + srow;
+#pragma unroll 1
+        for (int i = 0; i < K; ++i) {
+            const int j0 = base - lane + 32 * i;
+            const uint32_t k = j0 + lane >= first && j0 + lane < last ? key_of(a.scores[srow + j0 + lane]) : 0u;
+            unsigned m = __ballot_sync(0xffffffffu, k >= low && k <= high);
+            while (m) {  // four pages at a time
+                const int j = j0 + group_bit(m, lane);
+                wide[j] = again(bounds_of(j));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) m &= m - 1;
             }
         }
-        __syncthreads();
-    }
-    // ascending output: sink pages, the chosen ones, the recent pages
-    for (int i = threadIdx.x; i < a.sink; i += kSelThreads) out[i] = i;
-    int at = a.sink;
-    const int words = (seen + 31) / 32;
-    for (int w0 = 0; w0 < words; w0 += kSelThreads) {
-        const int wd = w0 + threadIdx.x;
-        uint32_t bits = wd < words ? chosen[wd] : 0u;
-        int total;
-        int o = at + block_excl_scan(__popc(bits), sh.scan, total);
-        while (bits) {
-            out[o++] = wd * 32 + __ffs(bits) - 1;
-            bits &= bits - 1;
+        row.sync();  // (a warp reads back only what it wrote)
+        const auto each = [&](auto f) {
+#pragma unroll 1
+            for (int i = 0; i < K; ++i) {
+                const int j = base + 32 * i;
+                const uint32_t k = j >= first && j < last ? key_of(a.scores[srow + j]) : 0u;
+                const bool in = k >= low && k <= high;
+                f(i, in ? __ldcg(wide + j) : 0ull, in);
+            }
+        };
+        unsigned long long wlo = ~0ull, whi = 0ull;
+        each([&](int, unsigned long long k, bool in) {
+            if (in) wlo = min(wlo, k);
+            whi = max(whi, k);
+        });
+        wlo = row.template pick64<false>(wlo);
+        whi = row.template pick64<true>(whi);
+        while (wlo < whi) {
+            const unsigned long long mid = whi - ((whi - wlo) >> 1);
+            uint32_t c = 0;
+            each([&](int, unsigned long long k, bool in) { c += in && k >= mid; });
+            if (static_cast<int>(row.sum(c)) >= want) wlo = mid;
+            else whi = mid - 1;
         }
-        at += total;
+        uint32_t more = 0, same = 0;  // above the edge; at it, in this warp
+        each([&](int, unsigned long long k, bool in) {
+            more += in && k > wlo;
+            same += __popc(__ballot_sync(0xffffffffu, in && k == wlo));
+        });
+        const int equal = want - static_cast<int>(row.sum(more));  // taken at the edge, lowest first
+        int rank = static_cast<int>(row.before(same));
+        each([&](int i, unsigned long long k, bool in) {
+            const unsigned e = __ballot_sync(0xffffffffu, in && k == wlo);
+            const bool take = in && (k > wlo || (k == wlo && rank + __popc(e & ((1u << lane) - 1)) < equal));
+            const unsigned bits = __ballot_sync(0xffffffffu, take);
+            if (lane == 0) picked[slot][row.warp * K + i] = bits;
+            rank += __popc(e);
+        });
+        row.sync();
     }
-    for (int i = threadIdx.x; i < a.recent; i += kSelThreads) out[a.top - a.recent + i] = last + i;
+    // ascending output between the sink and the recent pages: lane i writes out word i of the warp
+    uint32_t bits = lane < K ? picked[slot][row.warp * K + lane] : 0u;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+        const uint32_t sure = __ballot_sync(0xffffffffu, key[i] > high);
+        if (lane == i) bits |= sure;
+    }
+    int incl = __popc(bits);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+    }
+    const int mine = __shfl_sync(0xffffffffu, incl, 31);
+    int at = a.sink + static_cast<int>(row.before(mine)) + incl - __popc(bits);
+    for (; bits; bits &= bits - 1) out[at++] = (row.warp * K + lane) * 32 + __ffs(bits) - 1;
 }
 
 // ------------------------------------------------------------------ attention over the lists
@@ -919,14 +1047,15 @@ int check_heads(int hq, int hkv, int head_dim, int page_size) {
 
 int pages_of(int tokens) { return tokens / kPage + (tokens % kPage != 0); }
 
-// Score rows of one launch pair: as many query rows as keep the scores within 64 MB (they are
-// written and read once, from L2), at least 16.
-constexpr int64_t kScoreBytes = int64_t(64) << 20;
+// Query rows of one launch pair: as many as keep the workspace (16 bytes per row, kv head and
+// page) within 128 MB, so that the scores (a quarter of it) stay in L2 until they are read; at
+// least 16.
+constexpr int64_t kSelectBytes = int64_t(128) << 20;
 int slab_rows(int total_q, int stride, int hkv) {
-    const int64_t rows = std::max<int64_t>(16, kScoreBytes / (int64_t(4) * stride * hkv));
+    const int64_t rows = std::max<int64_t>(16, kSelectBytes / (int64_t(16) * stride * hkv));
     return static_cast<int>(std::min<int64_t>(total_q, rows));
 }
-int score_stride(int max_seq_len) { return (pages_of(max_seq_len) + 3) / 4 * 4; }
+int score_stride(int max_seq_len) { return std::max(16, (pages_of(max_seq_len) + 15) / 16 * 16); }
 
 }  // namespace
 }  // namespace msgl
@@ -966,7 +1095,7 @@ int msgl_kv_page_bounds(const void* k_pool, int64_t num_slots, const int* page_t
 size_t msgl_select_pages_workspace_size(int total_q, int max_seq_len, int num_kv_heads) {
     if (total_q <= 0 || max_seq_len <= 0 || num_kv_heads <= 0 || pages_of(max_seq_len) > kMaxPagesPerReq) return 0;
     const int stride = score_stride(max_seq_len);
-    return size_t(2) * slab_rows(total_q, stride, num_kv_heads) * num_kv_heads * stride * sizeof(float);
+    return size_t(16) * slab_rows(total_q, stride, num_kv_heads) * num_kv_heads * stride;
 }
 
 int msgl_select_pages(const void* q, const void* bounds, int64_t num_pages, const int* page_table,
@@ -1014,9 +1143,10 @@ int msgl_select_pages(const void* q, const void* bounds, int64_t num_pages, cons
     a.page_ids = page_ids;
     a.err = device_error_word();
     if (!a.err) return set_error(MSGL_ERR_CUDA, "device error word unavailable");
-    a.stride = std::max(4, score_stride(max_seq_len));
+    a.stride = score_stride(max_seq_len);
     const int slab = slab_rows(total_q, a.stride, num_kv_heads);
-    a.scores = static_cast<float*>(workspace);
+    a.wide = static_cast<unsigned long long*>(workspace);
+    a.scores = reinterpret_cast<float*>(a.wide + int64_t(slab) * num_kv_heads * a.stride);
     a.mags = a.scores + int64_t(slab) * num_kv_heads * a.stride;
 
     const int G = num_q_heads / num_kv_heads;
@@ -1029,10 +1159,19 @@ int msgl_select_pages(const void* q, const void* bounds, int64_t num_pages, cons
     const int64_t sel_blocks = int64_t(slab) * num_kv_heads;
     if (blocks > INT32_MAX || sel_blocks > INT32_MAX)
         return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "select_pages: batch too large");
-    const size_t smem = (size_t(a.stride) + a.stride / 32 + 2) * sizeof(uint32_t);
-    static std::atomic<int> optin[kMaxDevices];
-    cudaError_t e = smem_optin(select_pages_kernel, smem, optin);
-    if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
+    // Up to 1024 pages a warp holds a row; with too few rows to fill the GPU, and for longer
+    // rows, more warps share one.
+    using Select = void (*)(SelectArgs, int);
+    const int pages = pages_of(max_seq_len);
+    const bool many = sel_blocks >= 4 * 148;
+    int warps, rows;  // per row, per CTA
+    Select select;
+    if (pages <= 256 && many) { select = select_pages_kernel<1, 8, 4>; warps = 1; rows = 4; }
+    else if (pages <= 1024 && many) { select = select_pages_kernel<1, 32, 4>; warps = 1; rows = 4; }
+    else if (pages <= 512) { select = select_pages_kernel<4, 4, 1>; warps = 4; rows = 1; }
+    else if (pages <= 2048) { select = select_pages_kernel<8, 8, 1>; warps = 8; rows = 1; }
+    else if (pages <= 8192) { select = select_pages_kernel<16, 16, 1>; warps = 16; rows = 1; }
+    else { select = select_pages_kernel<32, 32, 1>; warps = 32; rows = 1; }
     for (int t0 = 0; t0 < total_q; t0 += slab) {
         a.t0 = t0;
         a.t1 = std::min(total_q, t0 + slab);
@@ -1041,7 +1180,8 @@ int msgl_select_pages(const void* q, const void* bounds, int64_t num_pages, cons
                        tile_rows, tiles, page_tiles);
             MSGL_LAUNCH_CHECK();
         }
-        launch_pdl(select_pages_kernel, dim3((a.t1 - t0) * num_kv_heads), dim3(kSelThreads), smem, stream, a);
+        const int n = (a.t1 - t0) * num_kv_heads;
+        launch_pdl(select, dim3((n + rows - 1) / rows), dim3(32 * warps * rows), 0, stream, a, n);
         MSGL_LAUNCH_CHECK();
     }
     return MSGL_OK;

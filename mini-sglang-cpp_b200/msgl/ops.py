@@ -17,7 +17,9 @@ _SECTIONS = C.c_int * 3
 
 
 def _s():
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream's handle. The raw lookup costs 0.2 us; torch.cuda.current_stream() builds
+    a Stream object (3.3 us)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _p(t):
@@ -29,6 +31,15 @@ def _c(t, dtype=None):
     if dtype is not None:
         assert t.dtype == dtype, f"expected {dtype}, got {t.dtype}"
     return t
+
+
+def _on(dtype, *tensors):
+    """Contiguous tensors of one dtype on the current device (whose stream the call uses)."""
+    dev = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t.get_device() != dev or t.dtype != dtype or not t.is_contiguous():
+            raise ValueError(f"expected a contiguous {dtype} tensor on cuda:{dev}, got {t.dtype} "
+                             f"{tuple(t.shape)} with strides {t.stride()} on {t.device}")
 
 
 # ------------------------------------------------------------------ reference launchers
@@ -118,12 +129,19 @@ def qknorm_rope_store_kv_partials(parts, k_pool, v_pool, positions, slot_mapping
     return q
 
 
-def _mrope_args(positions, sections, interleaved):
-    """Checked [3, T] positions (any row stride), their row stride, and the host section array."""
-    assert positions.is_cuda and positions.dtype == torch.int32, "expected CUDA int32 positions"
-    assert positions.dim() == 2 and positions.shape[0] == 3, "expected positions [3, T]"
-    assert positions.stride(1) == 1 or positions.shape[1] <= 1, "expected contiguous position rows"
-    return positions.stride(0), _SECTIONS(*sections), int(interleaved)
+def _mrope_args(positions, slot_mapping, cos_sin, q_norm, k_norm, k_pool, v_pool, sections, head_dim):
+    """Checked [3, T] positions (any row stride): T, their row stride, the host section array."""
+    _on(torch.int32, slot_mapping)
+    _on(torch.float32, cos_sin)
+    three, T = positions.shape
+    if (three != 3 or positions.dtype != torch.int32 or positions.get_device() != slot_mapping.get_device()
+            or (T > 1 and positions.stride(1) != 1)):
+        raise ValueError("expected int32 positions [3, T] with contiguous rows on the current device")
+    assert slot_mapping.numel() == T, "expected slot_mapping [T]"
+    assert cos_sin.dim() == 2 and cos_sin.shape[1] == head_dim, "expected cos_sin [max_position, D]"
+    assert q_norm.numel() == head_dim and k_norm.numel() == head_dim, "expected norm weights [D]"
+    assert k_pool.numel() == v_pool.numel(), "expected pools of one size"
+    return T, positions.stride(0), _SECTIONS(*sections)
 
 
 def qknorm_mrope_store_kv(qkv, k_pool, v_pool, positions, slot_mapping, cos_sin, q_norm, k_norm,
@@ -131,18 +149,16 @@ def qknorm_mrope_store_kv(qkv, k_pool, v_pool, positions, slot_mapping, cos_sin,
                           out=None):
     """As qknorm_rope_store_kv with positions [3, T] (time, height, width rows) and `sections`, the
     rotary pairs of each axis (sum head_dim / 2): consecutive ranges, or interleaved."""
-    _c(qkv, torch.bfloat16), _c(k_pool, torch.bfloat16), _c(v_pool, torch.bfloat16)
-    _c(slot_mapping, torch.int32), _c(cos_sin, torch.float32)
-    _c(q_norm, torch.bfloat16), _c(k_norm, torch.bfloat16)
-    stride, sec, layout = _mrope_args(positions, sections, interleaved)
-    T = positions.shape[1]
-    assert qkv.numel() == T * (num_q_heads + 2 * num_kv_heads) * head_dim and slot_mapping.numel() == T
     if out is None:
-        out = torch.empty(T, num_q_heads, head_dim, dtype=torch.bfloat16, device=qkv.device)
+        out = torch.empty(positions.shape[1], num_q_heads, head_dim, dtype=torch.bfloat16, device=qkv.device)
+    _on(torch.bfloat16, qkv, k_pool, v_pool, q_norm, k_norm, out)
+    T, stride, sec = _mrope_args(positions, slot_mapping, cos_sin, q_norm, k_norm, k_pool, v_pool, sections, head_dim)
+    assert qkv.numel() == T * (num_q_heads + 2 * num_kv_heads) * head_dim, "expected qkv [T, (Hq + 2 Hkv) D]"
+    assert out.numel() == T * num_q_heads * head_dim, "expected out [T, Hq, D]"
     num_slots = k_pool.numel() // (num_kv_heads * head_dim)
     check(lib().msgl_qknorm_mrope_store_kv(
-        _p(qkv), _p(out), _p(k_pool), _p(v_pool), num_slots, _p(positions), stride, sec, layout,
-        _p(slot_mapping), _p(cos_sin), cos_sin.shape[0], _p(q_norm), _p(k_norm), T, num_q_heads,
+        _p(qkv), _p(out), _p(k_pool), _p(v_pool), num_slots, _p(positions), stride, sec,
+        int(interleaved), _p(slot_mapping), _p(cos_sin), cos_sin.shape[0], _p(q_norm), _p(k_norm), T, num_q_heads,
         num_kv_heads, head_dim, eps, _s()))
     return out
 
@@ -151,20 +167,18 @@ def qknorm_mrope_store_kv_partials(parts, k_pool, v_pool, positions, slot_mappin
                                    k_norm, num_q_heads, num_kv_heads, eps, sections,
                                    interleaved=False, head_dim=128, out=None):
     """As qknorm_mrope_store_kv with the QKV rows the sum of fp32 partials [P, T, (Hq+2Hkv) D]."""
-    _c(parts, torch.float32), _c(k_pool, torch.bfloat16), _c(v_pool, torch.bfloat16)
-    _c(slot_mapping, torch.int32), _c(cos_sin, torch.float32)
-    _c(q_norm, torch.bfloat16), _c(k_norm, torch.bfloat16)
-    stride, sec, layout = _mrope_args(positions, sections, interleaved)
-    T = positions.shape[1]
-    row = T * (num_q_heads + 2 * num_kv_heads) * head_dim
-    nparts = parts.shape[0]
-    assert parts.numel() == nparts * row and slot_mapping.numel() == T
     if out is None:
-        out = torch.empty(T, num_q_heads, head_dim, dtype=torch.bfloat16, device=parts.device)
+        out = torch.empty(positions.shape[1], num_q_heads, head_dim, dtype=torch.bfloat16, device=parts.device)
+    _on(torch.float32, parts)
+    _on(torch.bfloat16, k_pool, v_pool, q_norm, k_norm, out)
+    T, stride, sec = _mrope_args(positions, slot_mapping, cos_sin, q_norm, k_norm, k_pool, v_pool, sections, head_dim)
+    nparts = parts.shape[0]
+    assert parts.numel() == nparts * T * (num_q_heads + 2 * num_kv_heads) * head_dim, "expected parts [P, T, (Hq + 2 Hkv) D]"
+    assert out.numel() == T * num_q_heads * head_dim, "expected out [T, Hq, D]"
     num_slots = k_pool.numel() // (num_kv_heads * head_dim)
     check(lib().msgl_qknorm_mrope_store_kv_partials(
         _p(parts), nparts, _p(out), _p(k_pool), _p(v_pool), num_slots, _p(positions), stride, sec,
-        layout, _p(slot_mapping), _p(cos_sin), cos_sin.shape[0], _p(q_norm), _p(k_norm), T,
+        int(interleaved), _p(slot_mapping), _p(cos_sin), cos_sin.shape[0], _p(q_norm), _p(k_norm), T,
         num_q_heads, num_kv_heads, head_dim, eps, _s()))
     return out
 
@@ -276,13 +290,14 @@ def paged_attention_extend(q, k_pool, v_pool, page_table, seq_lens, q_indptr, ma
 # ------------------------------------------------------------------ page-sparse attention
 def _rows(page_table, seq_lens, q_indptr, max_q_len, total_q):
     """Checked request metadata of the page-sparse calls: the request count."""
-    _c(page_table, torch.int32), _c(seq_lens, torch.int32)
+    _on(torch.int32, page_table, seq_lens)
     B = seq_lens.numel()
     assert page_table.dim() == 2 and page_table.shape[0] == B, "expected a page-table row per request"
     if q_indptr is None:
         assert max_q_len == 1 and total_q in (None, B), "one query row per request without q_indptr"
     else:
-        assert _c(q_indptr, torch.int32).numel() == B + 1, "expected q_indptr [num_reqs + 1]"
+        _on(torch.int32, q_indptr)
+        assert q_indptr.numel() == B + 1, "expected q_indptr [num_reqs + 1]"
     return B
 
 
@@ -290,7 +305,7 @@ def kv_page_bounds_(bounds, k_pool, page_table, seq_lens, num_kv_heads, q_indptr
                     head_dim=128, page_size=16):
     """msgl_kv_page_bounds: smallest / largest key of the pages the last rows of each request
     touch, into bounds [num_pages, Hkv, 2, D] bf16 (in place)."""
-    _c(bounds, torch.bfloat16), _c(k_pool, torch.bfloat16)
+    _on(torch.bfloat16, bounds, k_pool)
     B = _rows(page_table, seq_lens, q_indptr, max_q_len, None)
     num_slots = k_pool.numel() // (num_kv_heads * head_dim)
     assert bounds.numel() * page_size == 2 * k_pool.numel(), "expected bounds [num_pages, Hkv, 2, D]"
@@ -309,7 +324,7 @@ def select_pages(q, bounds, page_table, seq_lens, max_seq_len, top_pages, hq, hk
                  recent_pages=1, q_indptr=None, max_q_len=1, page_size=16, workspace=None, out=None):
     """msgl_select_pages: page ids [total_q, Hkv, top_pages] int32 for query rows q [total_q, Hq, D]
     (rows behind the last request: -1 unless `out` is given)."""
-    _c(q, torch.bfloat16), _c(bounds, torch.bfloat16)
+    _on(torch.bfloat16, q, bounds)
     T = q.numel() // (hq * 128)
     B = _rows(page_table, seq_lens, q_indptr, max_q_len, T)
     if workspace is None:
@@ -318,7 +333,9 @@ def select_pages(q, bounds, page_table, seq_lens, max_seq_len, top_pages, hq, hk
         shape = (T, hkv, top_pages)
         out = (torch.empty(shape, dtype=torch.int32, device=q.device) if q_indptr is None else
                torch.full(shape, -1, dtype=torch.int32, device=q.device))
-    assert _c(out, torch.int32).numel() == T * hkv * top_pages
+    _on(torch.int32, out)
+    _on(torch.uint8, workspace)
+    assert out.numel() == T * hkv * top_pages, "expected out [total_q, Hkv, top_pages]"
     check(lib().msgl_select_pages(_p(q), _p(bounds), bounds.numel() // (hkv * 256), _p(page_table),
                                   page_table.shape[1], _p(seq_lens), _p(q_indptr), B, T, max_q_len,
                                   max_seq_len, hq, hkv, 128, page_size, top_pages, sink_pages,
@@ -330,8 +347,8 @@ def paged_attention_pages(q, k_pool, v_pool, page_table, seq_lens, page_ids, hq,
                           q_indptr=None, max_q_len=1, max_seq_len=None, page_size=16, out=None):
     """msgl_paged_attention_pages: attention of q [total_q, Hq, D] over the pages listed in
     page_ids [total_q, Hkv, top_pages] (select_pages, or lists of the caller's)."""
-    _c(q, torch.bfloat16), _c(k_pool, torch.bfloat16), _c(v_pool, torch.bfloat16)
-    _c(page_ids, torch.int32)
+    _on(torch.bfloat16, q, k_pool, v_pool)
+    _on(torch.int32, page_ids)
     T = q.numel() // (hq * 128)
     B = _rows(page_table, seq_lens, q_indptr, max_q_len, T)
     assert page_ids.dim() == 3 and page_ids.shape[:2] == (T, hkv), "expected page_ids [total_q, Hkv, top]"
@@ -342,12 +359,13 @@ def paged_attention_pages(q, k_pool, v_pool, page_table, seq_lens, page_ids, hq,
         max_seq_len = page_table.shape[1] * page_size
     if out is None:
         out = torch.empty_like(q) if q_indptr is None else torch.zeros_like(q)
+    _on(torch.bfloat16, out)
+    assert out.numel() == q.numel(), "expected out [total_q, Hq, D]"
     num_slots = k_pool.numel() // (hkv * 128)
     check(lib().msgl_paged_attention_pages(_p(q), _p(k_pool), _p(v_pool), num_slots, _p(page_table),
                                            page_table.shape[1], _p(seq_lens), _p(q_indptr), B, T,
                                            max_q_len, max_seq_len, _p(page_ids), page_ids.shape[2],
-                                           hq, hkv, 128, page_size, scale, _p(_c(out, torch.bfloat16)),
-                                           _s()))
+                                           hq, hkv, 128, page_size, scale, _p(out), _s()))
     return out
 
 
@@ -358,24 +376,30 @@ def lora_workspace(num_tokens, K, rank, device="cuda"):
 
 
 def _r(t, dtype):
-    """A 2-D CUDA tensor with contiguous rows: its row stride."""
-    assert t.is_cuda and t.dtype == dtype and t.dim() == 2, f"expected 2-D CUDA {dtype} rows"
-    assert t.stride(1) == 1 or t.shape[1] == 1, "expected contiguous rows"
-    return max(t.stride(0), t.shape[1])
+    """A 2-D tensor with contiguous rows on the current device: its row stride."""
+    if (t.dim() != 2 or t.dtype != dtype or t.get_device() != torch._C._cuda_getDevice()
+            or (t.shape[1] > 1 and t.stride(1) != 1)):
+        raise ValueError(f"expected {dtype} rows [T, n] on the current device, got {t.dtype} "
+                         f"{tuple(t.shape)} with strides {t.stride()} on {t.device}")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
 
 
 def _lora(x, lora_a, lora_b, scales, adapter_ids, q_indptr, max_q_len, workspace):
-    _c(lora_a, torch.bfloat16), _c(lora_b, torch.bfloat16), _c(scales, torch.float32)
-    _c(adapter_ids, torch.int32)
+    _on(torch.bfloat16, lora_a, lora_b)
+    _on(torch.float32, scales)
+    _on(torch.int32, adapter_ids)
     n, R, K = lora_a.shape
-    assert lora_b.shape[0] == n and lora_b.shape[2] == R and scales.numel() == n and x.shape[1] == K
+    assert lora_b.shape[0] == n and lora_b.shape[2] == R and scales.numel() == n and x.shape[1] == K, \
+        "expected lora_a [n, rank, K], lora_b [n, N, rank], scales [n], x [T, K]"
     B = adapter_ids.numel()
     if q_indptr is None:
         assert max_q_len == 1 and B == x.shape[0], "one row per request without q_indptr"
     else:
-        assert _c(q_indptr, torch.int32).numel() == B + 1, "expected q_indptr [num_reqs + 1]"
+        _on(torch.int32, q_indptr)
+        assert q_indptr.numel() == B + 1, "expected q_indptr [num_reqs + 1]"
     if workspace is None:
         workspace = lora_workspace(x.shape[0], K, R, x.device)
+    _on(torch.uint8, workspace)
     return (_p(x), _r(x, torch.bfloat16), _p(lora_a), _p(lora_b), _p(scales), n, _p(adapter_ids),
             _p(q_indptr), B, max_q_len), (x.shape[0], lora_b.shape[1], K, R), workspace
 

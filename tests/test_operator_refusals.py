@@ -84,10 +84,10 @@ def test_select_empty_and_workspace():
     assert select(B=0, T=0) == 0 and select(ip=P, T=0) == 0 and select(ip=P, mq=0) == 0
     assert L.msgl_select_pages_workspace_size(0, 1000, 8) == 0
     assert L.msgl_select_pages_workspace_size(1, 524289, 8) == 0
-    # scores and bound magnitudes of 64 rows x 8 heads x 2048 pages, fp32
-    assert L.msgl_select_pages_workspace_size(64, 32768, 8) == 2 * 64 * 8 * 2048 * 4
-    # bounded for long batches: 64 MB of each
-    assert L.msgl_select_pages_workspace_size(100000, 32768, 8) == 2 * 64 * 2 ** 20
+    # 16 bytes for each of 64 rows x 8 heads x 2048 pages
+    assert L.msgl_select_pages_workspace_size(64, 32768, 8) == 16 * 64 * 8 * 2048
+    # bounded for long batches
+    assert L.msgl_select_pages_workspace_size(100000, 32768, 8) == 128 * 2 ** 20
 
 
 def attend(**k):
