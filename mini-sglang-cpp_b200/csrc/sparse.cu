@@ -17,6 +17,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "tmap.h"
 
 namespace msgl {
 namespace {
@@ -710,17 +711,16 @@ select_pages_kernel(const SelectArgs a, int num_rows) {
 }
 
 // ------------------------------------------------------------------ attention over the lists
-// One CTA per (tile of one request's query rows, kv head): TQ = min(8, 16 / G) rows of a chunk,
-// one row in decode; the 16 MMA rows are tile row x query head. The rows' lists are joined into
-// one ascending list of pages with a mask of the rows that asked for each, so a page that several
-// neighbouring queries chose is loaded once. Four warps take the joined pages in turn, each with
-// a ring of its own (cp.async, 16 bytes a lane), an online softmax, and their partial results are
-// joined at the end.
+// A row's list is read as a set: the listed pages become bits (decode) or row masks (chunks) over
+// the context's pages, and a scan over those gives one ascending list without repeats.
+//
+// A page's 16 keys are the 16 MMA rows and the 8 MMA columns are 8 / G query rows x the G query
+// heads of one kv head: S^T = K Q^T and O^T = V^T P^T, 8 MMAs each per page. With the columns as
+// MMA rows (16 of them) a single token fills at most half of the tile, and a tile of four tokens
+// (G = 4) multiplies pages that only some of them listed: 32 MMAs a page and twice the registers.
 constexpr int kAttWarps = 4;
 constexpr int kAttThreads = kAttWarps * 32;
-constexpr int kAttStages = 3;
 constexpr int kPageBytes = 2 * kPage * kHd * 2;  // K and V of one page and kv head
-constexpr int kAttRing = kAttWarps * kAttStages * kPageBytes;
 
 struct AttArgs {
     const __nv_bfloat16 *q, *k_pool, *v_pool;
@@ -745,122 +745,377 @@ __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// Running state of a warp's online softmax. Lane (g, c) holds dims 16 j + g (+ 8) of columns 2 c and
+// 2 c + 1, the columns' maxima and this lane's part of their sums.
+struct Softmax {
+    float o[8][4];
+    float m[2], l[2];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+        m[0] = m[1] = kNegInf;
+        l[0] = l[1] = 0.f;
+    }
+};
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
 // One page (16 keys) for one warp. K and V tiles: halves of 64 dims, rows of 128 bytes, 16-byte
-// pieces swizzled by the row. lim0 / lim1: last visible offset in the page for MMA rows g / g + 8
-// (< 0: the page is not of that row). With `part`, only rows whose own limit is >= 0 take the new
-// sums (the others' P is zero, but zero times a NaN or infinite value of a page that is not theirs
-// must not reach them), and V rows behind vlim count as zero for the same reason.
-template <bool TWO>
-__device__ __forceinline__ void attend(uint32_t base, const uint32_t (&qa)[8][4], float (&o)[16][4],
-                                       float (&m)[2], float (&l)[2], int lim0, int lim1, bool part,
-                                       int vlim, float sl2e, int lane) {
-    const int mi = lane >> 3, c = lane & 3;
+// pieces swizzled by the row. qb: column g's query as the B operand. lim0 / lim1: last visible
+// offset in the page for columns 2 c / 2 c + 1 (< 0: the page is not of that column). With PART,
+// only columns whose own limit is >= 0 take the new sums (the others' P is zero, but zero times a
+// NaN or infinite value of a page that is not theirs must not reach them), and V rows behind vlim
+// count as zero for the same reason.
+template <bool PART>
+__device__ __forceinline__ void attend(uint32_t base, const uint32_t (&qb)[8][2], Softmax& st,
+                                       int lim0, int lim1, int vlim, float sl2e, int lane) {
+    const int mi = lane >> 3, g = lane >> 2, c = lane & 3;
+    // The asm statements keep their order, so fragments are loaded some steps ahead of the MMAs that
+    // take them: all of K at once, half of V before the softmax and half behind it.
+    uint32_t f[8][4];
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+        const int row = ((mi & 1) << 3) + (lane & 7);
+        const int piece = ((kk & 3) << 1) + (mi >> 1);
+        ldsm_x4(base + ((kk >> 2) << 11) + row * 128 + ((piece ^ (row & 7)) << 4), f[kk][0], f[kk][1], f[kk][2], f[kk][3]);
+    }
     float s[2][4];
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk) {
-        const int row = ((mi >> 1) << 3) + (lane & 7);
-        const int piece = ((kk & 3) << 1) + (mi & 1);
-        uint32_t b0, b1, b2, b3;
-        ldsm_x4(base + ((kk >> 2) << 11) + row * 128 + ((piece ^ (row & 7)) << 4), b0, b1, b2, b3);
-        mma_bf16_16816(s[0], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], b0, b1);
-        mma_bf16_16816(s[1], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], b2, b3);
-    }
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int tk = n * 8 + 2 * c + e;
-            s[n][e] = tk <= lim0 ? s[n][e] * sl2e : kNegInf;
-            if (TWO) s[n][2 + e] = tk <= lim1 ? s[n][2 + e] * sl2e : kNegInf;
-        }
-    float p[2][4];
-#pragma unroll
-    for (int r = 0; r < (TWO ? 2 : 1); ++r) {
-        float mx = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float m_new = fmaxf(m[r], mx);
-        float alpha = 1.f, ref = 0.f;
-        if (m_new != kNegInf) {
-            alpha = exp2f(m[r] - m_new);
-            ref = m_new;
-        }
-        float ps = 0.f;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float v = exp2f(s[n][2 * r + e] - ref);
-                p[n][2 * r + e] = v;
-                ps += v;
-            }
-        l[r] = l[r] * alpha + ps;
-        m[r] = m_new;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            o[j][2 * r] *= alpha;
-            o[j][2 * r + 1] *= alpha;
-        }
-    }
-    // P in bf16, as V is: relative error 2^-9 a weight, averaged over the keys
-    const uint32_t pa0 = pack_bf16x2(p[0][0], p[0][1]);
-    const uint32_t pa2 = pack_bf16x2(p[1][0], p[1][1]);
-    const uint32_t pa1 = TWO ? pack_bf16x2(p[0][2], p[0][3]) : 0u;
-    const uint32_t pa3 = TWO ? pack_bf16x2(p[1][2], p[1][3]) : 0u;
+    for (int kk = 0; kk < 8; ++kk)  // two chains
+        mma_bf16_16816(s[kk & 1], f[kk][0], f[kk][1], f[kk][2], f[kk][3], qb[kk][0], qb[kk][1]);
     const uint32_t vb = base + kPageBytes / 2;
-    // V fragments hold tokens (2c, 2c + 1) and (2c + 8, 2c + 9)
+    const auto load_v = [&](int j) {
+        const int row = ((mi >> 1) << 3) + (lane & 7);
+        const int piece = ((j & 3) << 1) + (mi & 1);
+        ldsm_x4_t(vb + ((j >> 2) << 11) + row * 128 + ((piece ^ (row & 7)) << 4), f[j][0], f[j][1], f[j][2], f[j][3]);
+    };
+#pragma unroll
+    for (int j = 0; j < 4; ++j) load_v(j);
+    // p[e]: key g (e < 2) or g + 8, column 2 c + e % 2
+    float p[4], old[2] = {st.m[0], st.m[1]};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        p[e] = g + (e >> 1) * 8 <= (e & 1 ? lim1 : lim0) ? (s[0][e] + s[1][e]) * sl2e : kNegInf;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        float mx = fmaxf(p[r], p[2 + r]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        st.m[r] = fmaxf(st.m[r], mx);
+    }
+    if (__any_sync(0xffffffffu, st.m[0] != old[0] || st.m[1] != old[1])) {  // a maximum rose: rescale
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const float alpha = st.m[r] == kNegInf ? 1.f : exp2f(old[r] - st.m[r]);
+            st.l[r] *= alpha;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                st.o[j][r] *= alpha;
+                st.o[j][2 + r] *= alpha;
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        p[e] = exp2f(p[e] - (st.m[e & 1] == kNegInf ? 0.f : st.m[e & 1]));
+        st.l[e & 1] += p[e];
+    }
+    // P in bf16, as V is: relative error 2^-8 a weight, averaged over the keys
+    const uint32_t b0 = transpose8x8(pack_bf16x2(p[0], p[1]));
+    const uint32_t b1 = transpose8x8(pack_bf16x2(p[2], p[3]));
+#pragma unroll
+    for (int j = 4; j < 8; ++j) load_v(j);
+    // V fragments hold keys (2c, 2c + 1) and (2c + 8, 2c + 9)
     uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-    if (part) {
+    if (PART) {
         keep0 = (2 * c <= vlim ? 0xffffu : 0u) | (2 * c + 1 <= vlim ? 0xffff0000u : 0u);
         keep1 = (2 * c + 8 <= vlim ? 0xffffu : 0u) | (2 * c + 9 <= vlim ? 0xffff0000u : 0u);
     }
 #pragma unroll
-    for (int j2 = 0; j2 < 8; ++j2) {
-        const int row = ((mi & 1) << 3) + (lane & 7);
-        const int piece = ((j2 & 3) << 1) + (mi >> 1);
-        uint32_t b0, b1, b2, b3;
-        ldsm_x4_t(vb + ((j2 >> 2) << 11) + row * 128 + ((piece ^ (row & 7)) << 4), b0, b1, b2, b3);
-        if (!part) {
-            mma_bf16_16816(o[2 * j2], pa0, pa1, pa2, pa3, b0, b1);
-            mma_bf16_16816(o[2 * j2 + 1], pa0, pa1, pa2, pa3, b2, b3);
+    for (int j = 0; j < 8; ++j) {
+        if (!PART) {
+            mma_bf16_16816(st.o[j], f[j][0], f[j][1], f[j][2], f[j][3], b0, b1);
         } else {
-            float d[2][4];
+            float d[4];
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int e = 0; e < 4; ++e) d[e] = st.o[j][e];
+            mma_bf16_16816(d, f[j][0] & keep0, f[j][1] & keep0, f[j][2] & keep1, f[j][3] & keep1, b0, b1);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) d[n][e] = o[2 * j2 + n][e];
-            mma_bf16_16816(d[0], pa0, pa1, pa2, pa3, b0 & keep0, b1 & keep1);
-            mma_bf16_16816(d[1], pa0, pa1, pa2, pa3, b2 & keep0, b3 & keep1);
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if ((e < 2 ? lim0 : lim1) >= 0) o[2 * j2 + n][e] = d[n][e];
+            for (int e = 0; e < 4; ++e)
+                if ((e & 1 ? lim1 : lim0) >= 0) st.o[j][e] = d[e];
         }
     }
 }
 
-template <bool CHUNK>
-__global__ void __launch_bounds__(kAttThreads, 2)
-attend_pages_kernel(const AttArgs a, int tiles, int words) {
-    constexpr bool TWO = CHUNK;
-    extern __shared__ __align__(128) uint8_t smem[];
-    const int G = a.hq / a.hkv;
-    const int TQ = CHUNK ? min(8, 16 / G) : 1;
-    uint8_t* ring = smem;                                                    // kAttRing
-    uint32_t* bits = reinterpret_cast<uint32_t*>(smem + kAttRing);           // [TQ][words]
-    int* list_phys = reinterpret_cast<int*>(bits + TQ * words);              // [min(TQ top, 32 words)]
-    const int cap = min(TQ * a.top, 32 * words);
-    uint32_t* list_info = reinterpret_cast<uint32_t*>(list_phys + cap);      // page << 8 | row mask
-    __shared__ int scan[32];
+// A warp's state into shared memory: o rows of kPad floats per column, m and l per column.
+constexpr int kPad = kHd + 4;  // the four lanes of a dim fall into different banks
+__device__ __forceinline__ void dump(const Softmax& st, float* o, float* m, float* l, int lane) {
+    const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[(2 * c + (e & 1)) * kPad + 16 * j + g + (e >> 1) * 8] = st.o[j][e];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        float sum = st.l[r];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        if (g == 0) {
+            m[2 * c + r] = st.m[r];
+            l[2 * c + r] = sum;
+        }
+    }
+}
 
+// 8 dims of one column joined over `n` dumped states, `step` columns' worth apart: M and L of the
+// column and its unnormalised values.
+__device__ __forceinline__ void join(const float* o, const float* m, const float* l, int n, int step,
+                                     float& M, float& L, float (&acc)[8]) {
+    M = kNegInf;
+    for (int k = 0; k < n; ++k) M = fmaxf(M, m[k * step]);
+    L = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+    for (int k = 0; k < n; ++k) {
+        const float mk = m[k * step], lk = l[k * step];
+        if (mk == kNegInf && lk == 0.f) continue;  // saw no key
+        const float sc = exp2f(mk - M);
+        L += lk * sc;
+        const float4 u = *reinterpret_cast<const float4*>(o + k * step * kPad);
+        const float4 v = *reinterpret_cast<const float4*>(o + k * step * kPad + 4);
+        acc[0] += u.x * sc; acc[1] += u.y * sc; acc[2] += u.z * sc; acc[3] += u.w * sc;
+        acc[4] += v.x * sc; acc[5] += v.y * sc; acc[6] += v.z * sc; acc[7] += v.w * sc;
+    }
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&v)[8], float f) {
+    return make_uint4(pack_bf16x2(v[0] * f, v[1] * f), pack_bf16x2(v[2] * f, v[3] * f),
+                      pack_bf16x2(v[4] * f, v[5] * f), pack_bf16x2(v[6] * f, v[7] * f));
+}
+
+// ---- single tokens
+// A cluster of up to 8 CTAs (decode_split) per (query row, kv head): each CTA
+// takes a share of the listed pages, its four warps take its pages in turn, every warp with a ring
+// of its own (cp.async, 16 bytes a lane, three pages) and an online softmax. The warps' results are
+// joined in shared memory, the CTAs' through distributed shared memory, each CTA finishing a share
+// of the output: no workspace, one launch, a fixed order.
+constexpr int kDecStages = 3;
+constexpr int kDecRing = kAttWarps * kDecStages * kPageBytes;
+
+__global__ void __launch_bounds__(kAttThreads, 2)
+attend_pages_decode_kernel(const AttArgs a, int words) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t* ring = smem;                                           // kDecRing
+    uint32_t* bits = reinterpret_cast<uint32_t*>(smem + kDecRing);  // [words]
+    int* list_phys = reinterpret_cast<int*>(bits + words);          // [top]
+    int* list_page = list_phys + a.top;                             // [top]
+    __shared__ int scan[32];
+    __shared__ float cm[8], cl[8];  // joined maximum and sum per query head
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int S = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
+    for (int i = threadIdx.x; i < words; i += kAttThreads) bits[i] = 0;
+    pdl_wait();
+    pdl_trigger();
+    const int id = static_cast<int>(blockIdx.x) / S;
+    const int h = id % a.hkv, r = id / a.hkv;
+    const int G = a.hq / a.hkv;
+    const bool report = h == 0 && rank == 0 && threadIdx.x == 0;
+    const Window w = request_window(r, a.seq_lens, a.q_indptr, a.max_len, report, a.err);
+    const bool fits = w.q0 >= 0 && w.qn >= 0 && w.qn <= a.max_q_len && w.q0 + static_cast<int64_t>(w.qn) <= a.total_q;
+    if (report && !fits) record_error(a.err, MSGL_ERR_BOUNDS, 801);
+    if (!fits || w.qn == 0) return;  // the whole cluster
+    const int pos = w.L - 1;
+    const int* ids = a.page_ids + (static_cast<int64_t>(w.q0) * a.hkv + h) * a.top;
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.top; i += kAttThreads) {
+        const int page = ids[i];
+        if (page < 0) continue;
+        if (pos < 0 || page > pos / kPage) {
+            if (rank == 0) record_error(a.err, MSGL_ERR_BOUNDS, 803);
+            continue;
+        }
+        atomicOr(&bits[page >> 5], 1u << (page & 31));
+    }
+    uint32_t qb[8][2];
+    {
+        const __nv_bfloat16* qr = a.q + (static_cast<int64_t>(w.q0) * a.hq + h * G + g) * kHd;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+            qb[kk][0] = g < G ? *reinterpret_cast<const uint32_t*>(qr + 16 * kk + 2 * c) : 0u;
+            qb[kk][1] = g < G ? *reinterpret_cast<const uint32_t*>(qr + 16 * kk + 8 + 2 * c) : 0u;
+        }
+    }
+    __syncthreads();
+    int per = 0;  // set bits of this thread's run of words
+    const int run = (words + kAttThreads - 1) / kAttThreads;
+    const int w_lo = min(words, static_cast<int>(threadIdx.x) * run), w_hi = min(words, w_lo + run);
+    for (int i = w_lo; i < w_hi; ++i) per += __popc(bits[i]);
+    int total;
+    int at = block_excl_scan(per, scan, total);
+    const int lo = static_cast<int>(static_cast<int64_t>(total) * rank / S);       // this CTA's share
+    const int count = static_cast<int>(static_cast<int64_t>(total) * (rank + 1) / S) - lo;
+    for (int i = w_lo; i < w_hi; ++i)
+        for (uint32_t b = bits[i]; b; b &= b - 1, ++at) {
+            if (at < lo || at >= lo + count) continue;
+            const int page = i * 32 + __ffs(b) - 1;
+            int phys = a.page_table[static_cast<int64_t>(r) * a.max_pages + page];
+            if (static_cast<unsigned>(phys) >= static_cast<unsigned>(a.pool_pages)) {
+                record_error(a.err, MSGL_ERR_BOUNDS, 802);
+                phys = 0;
+            }
+            list_phys[at - lo] = phys;
+            list_page[at - lo] = page;
+        }
+    __syncthreads();
+
+    Softmax st;
+    st.clear();
+    const int mine = count > warp ? (count - warp + kAttWarps - 1) / kAttWarps : 0;
+    const uint32_t ring0 = smem_u32(ring) + warp * kDecStages * kPageBytes;
+    const int64_t stride = static_cast<int64_t>(a.hkv) * kHd;
+    const auto issue = [&](int i) {
+        const int e = warp + i * kAttWarps;
+        const uint32_t dst = ring0 + (i % kDecStages) * kPageBytes;
+        const int live = pos - list_page[e] * kPage;  // last row to load: zeros behind it
+        const int64_t off = static_cast<int64_t>(list_phys[e]) * kPage * stride + h * kHd;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            const int row = 2 * x + (lane >> 4), piece = lane & 15;
+            const int64_t src = off + row * stride + piece * 8;
+            const uint32_t d = dst + ((piece >> 3) << 11) + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
+            cp_async16(d, a.k_pool + src, row <= live);
+            cp_async16(d + kPageBytes / 2, a.v_pool + src, row <= live);
+        }
+    };
+    for (int i = 0; i < kDecStages - 1; ++i) {
+        if (i < mine) issue(i);
+        cp_async_commit();
+    }
+    for (int i = 0; i < mine; ++i) {
+        cp_async_wait<kDecStages - 2>();
+        __syncwarp();
+        if (i + kDecStages - 1 < mine) issue(i + kDecStages - 1);
+        cp_async_commit();
+        const int lim = pos - list_page[warp + i * kAttWarps] * kPage;
+        attend<false>(ring0 + (i % kDecStages) * kPageBytes, qb, st, lim, lim, 0, a.sl2e, lane);
+        __syncwarp();
+    }
+
+    // ---- join the warps' results (shared memory over the drained rings)
+    cp_async_wait<0>();
+    __syncthreads();
+    float* mo = reinterpret_cast<float*>(ring);  // [4 warps][8][kPad]
+    float* mm = mo + kAttWarps * 8 * kPad;       // [4][8]
+    float* ml = mm + kAttWarps * 8;
+    float* co = ml + kAttWarps * 8;              // [8][128]: joined, for the cluster
+    dump(st, mo + warp * 8 * kPad, mm + warp * 8, ml + warp * 8, lane);
+    __syncthreads();
+    __nv_bfloat16* out = a.out + (static_cast<int64_t>(w.q0) * a.hq + h * G) * kHd;
+    for (int item = threadIdx.x; item < G * 16; item += kAttThreads) {
+        const int head = item >> 4, d0 = (item & 15) * 8;
+        float M, L, acc[8];
+        join(mo + head * kPad + d0, mm + head, ml + head, kAttWarps, 8, M, L, acc);
+        if (S == 1) {  // an empty list gives a zero row
+            *reinterpret_cast<uint4*>(out + head * kHd + d0) = pack8(acc, L == 0.f ? 0.f : 1.f / L);
+        } else {
+            *reinterpret_cast<float4*>(co + head * kHd + d0) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            *reinterpret_cast<float4*>(co + head * kHd + d0 + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+            if (d0 == 0) {
+                cm[head] = M;
+                cl[head] = L;
+            }
+        }
+    }
+    if (S == 1) return;
+    cluster_sync_all();
+    for (int item = rank + S * threadIdx.x; item < G * 16; item += S * kAttThreads) {
+        const int head = item >> 4, d0 = (item & 15) * 8;
+        float mk[8], lk[8], M = kNegInf;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            mk[k] = k < S ? ld_dsmem_f32(mapa_shared(smem_u32(cm + head), k)) : kNegInf;
+            lk[k] = k < S ? ld_dsmem_f32(mapa_shared(smem_u32(cl + head), k)) : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) M = fmaxf(M, mk[k]);
+        float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, L = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (k >= S) break;
+            const uint32_t src = mapa_shared(smem_u32(co + head * kHd + d0), k);
+            const float4 u = ld_dsmem_v4(src), v = ld_dsmem_v4(src + 16);
+            if (mk[k] == kNegInf && lk[k] == 0.f) continue;
+            const float sc = exp2f(mk[k] - M);
+            L += lk[k] * sc;
+            acc[0] += u.x * sc; acc[1] += u.y * sc; acc[2] += u.z * sc; acc[3] += u.w * sc;
+            acc[4] += v.x * sc; acc[5] += v.y * sc; acc[6] += v.z * sc; acc[7] += v.w * sc;
+        }
+        *reinterpret_cast<uint4*>(out + head * kHd + d0) = pack8(acc, L == 0.f ? 0.f : 1.f / L);
+    }
+    cluster_sync_all();  // no CTA leaves while another reads its shared memory
+}
+
+// ---- chunks
+// One CTA per (tile of one request's query rows, kv head): sixteen warps in RW row groups of TQ =
+// 8 / G rows each (RW from the longest chunk) times 16 / RW page groups, and a producer warp. The
+// rows' lists are joined into one list of pages with a mask of the rows that asked for each, so a
+// page that several neighbouring queries chose crosses from L2 once; a warp attends the pages that
+// its own rows asked for, one in 16 / RW of them. Pages come by TMA (one 3-D box of K, one of V)
+// through a ring shared by the warps, in stages of kStagePages: most warps skip most pages, and a
+// barrier per page cost as much as the pages. Contexts longer than kWin pages are walked in windows
+// of that many.
+//
+// A masked weight is zero, but zero times a NaN or infinite value is NaN. Such values are looked
+// for at the end instead of at every page: a row they reached is NaN from then on, so a tile
+// without NaN or infinite sums was right, and any other is computed again with the masked values
+// kept out (PART of attend).
+constexpr int kChWarps = 16;
+constexpr int kChThreads = (kChWarps + 1) * 32;
+constexpr int kStagePages = 4;
+constexpr int kChStages = 5;
+constexpr int kStageBytes = kStagePages * kPageBytes;
+constexpr int kWin = 2048;
+constexpr int kTileRows = 64;  // mask bits
+constexpr int kChSmem = kChStages * kStageBytes + kWin * (8 + 4 + 2) + 1024;
+
+__global__ void __launch_bounds__(kChThreads, 1)
+attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                          const AttArgs a, int tiles, int row_groups) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    unsigned long long* masks = reinterpret_cast<unsigned long long*>(ring + kChStages * kStageBytes);  // [kWin]
+    int* list_phys = reinterpret_cast<int*>(masks + kWin);                // [kWin]
+    uint16_t* list_page = reinterpret_cast<uint16_t*>(list_phys + kWin);  // [kWin], in the window
+    __shared__ uint64_t full[kChStages], empty[kChStages];
+    __shared__ int scan[32];
+    __shared__ float sm[kChWarps * 8], sl[kChWarps * 8];
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kChStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], kChWarps);
+        }
+        fence_barrier_init();
+        tma_prefetch_desc(&tk);
+        tma_prefetch_desc(&tv);
+    }
     pdl_wait();
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int G = a.hq / a.hkv;
+    const int TQ = 8 / G;
+    const int RW = row_groups, PW = kChWarps / RW, rg = warp % RW, pg = warp / RW;
     int64_t id = blockIdx.x;
     const int h = static_cast<int>(id % a.hkv);
     id /= a.hkv;
@@ -869,167 +1124,142 @@ attend_pages_kernel(const AttArgs a, int tiles, int words) {
     const Window w = request_window(r, a.seq_lens, a.q_indptr, a.max_len, report, a.err);
     const bool fits = w.q0 >= 0 && w.qn >= 0 && w.qn <= a.max_q_len && w.q0 + static_cast<int64_t>(w.qn) <= a.total_q;
     if (report && !fits) record_error(a.err, MSGL_ERR_BOUNDS, 801);
-    const int i0 = tile * TQ;
-    const int rows = min(TQ, w.qn - i0);
+    const int i0 = tile * RW * TQ;
+    const int rows = min(RW * TQ, w.qn - i0);
     if (!fits || rows <= 0) return;
-    const int pos0 = w.L - w.qn + i0;                         // position of the tile's first row
+    const int pos0 = w.L - w.qn + i0;  // position of the tile's first row
 
-    // ---- the rows' lists as bit sets, then one joined list
-    for (int i = threadIdx.x; i < TQ * words; i += kAttThreads) bits[i] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < rows * a.top; i += kAttThreads) {
-        const int row = i / a.top;
-        const int page = a.page_ids[(static_cast<int64_t>(w.q0 + i0 + row) * a.hkv + h) * a.top + (i - row * a.top)];
-        if (page < 0) continue;
-        const int pos = pos0 + row;
-        if (pos < 0 || page > pos / kPage) {
-            record_error(a.err, MSGL_ERR_BOUNDS, 803);
-            continue;
-        }
-        atomicOr(&bits[row * words + (page >> 5)], 1u << (page & 31));
-    }
-    __syncthreads();
-    int count = 0;
-    for (int w0 = 0; w0 < words; w0 += kAttThreads) {
-        const int wd = w0 + threadIdx.x;
-        uint32_t any = 0;
-        if (wd < words)
-            for (int row = 0; row < TQ; ++row) any |= bits[row * words + wd];
-        int total;
-        int at = count + block_excl_scan(__popc(any), scan, total);
-        while (any) {
-            const int b = __ffs(any) - 1;
-            any &= any - 1;
-            uint32_t mask = 0;
-            for (int row = 0; row < TQ; ++row) mask |= ((bits[row * words + wd] >> b) & 1u) << row;
-            const int page = wd * 32 + b;
-            int phys = a.page_table[static_cast<int64_t>(r) * a.max_pages + page];
-            if (static_cast<unsigned>(phys) >= static_cast<unsigned>(a.pool_pages)) {
-                record_error(a.err, MSGL_ERR_BOUNDS, 802);
-                phys = 0;
-            }
-            list_phys[at] = phys;
-            list_info[at] = static_cast<uint32_t>(page) << 8 | mask;
-            ++at;
-        }
-        count += total;
-    }
-    __syncthreads();
-
-    // ---- this warp's pages: warp, warp + 4, ...
-    const int row0 = g / G, row1 = (g + 8) / G;  // tile rows of MMA rows g, g + 8
-    uint32_t qa[8][4];
+    const int wrow = rg * TQ, wrows = max(0, min(TQ, rows - wrow));  // this warp's rows (may be none)
+    const int row0 = 2 * c / G, row1 = (2 * c + 1) / G;              // of columns 2 c, 2 c + 1, in the warp
+    uint32_t qb[8][2];
     {
-        const bool real0 = row0 < rows, real1 = TWO && row1 < rows;
-        const __nv_bfloat16* qr = a.q + (static_cast<int64_t>(w.q0 + i0) * a.hq + h * G) * kHd;
-        const __nv_bfloat16* q0p = qr + (static_cast<int64_t>(row0) * a.hq + g % G) * kHd;
-        const __nv_bfloat16* q1p = qr + (static_cast<int64_t>(row1) * a.hq + (g + 8) % G) * kHd;
+        const bool real = warp < kChWarps && g / G < wrows;
+        const __nv_bfloat16* qr =
+            a.q + (static_cast<int64_t>(w.q0 + i0 + wrow + g / G) * a.hq + h * G + g % G) * kHd;
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {
-            qa[kk][0] = real0 ? *reinterpret_cast<const uint32_t*>(q0p + 16 * kk + 2 * c) : 0u;
-            qa[kk][2] = real0 ? *reinterpret_cast<const uint32_t*>(q0p + 16 * kk + 8 + 2 * c) : 0u;
-            qa[kk][1] = real1 ? *reinterpret_cast<const uint32_t*>(q1p + 16 * kk + 2 * c) : 0u;
-            qa[kk][3] = real1 ? *reinterpret_cast<const uint32_t*>(q1p + 16 * kk + 8 + 2 * c) : 0u;
+            qb[kk][0] = real ? *reinterpret_cast<const uint32_t*>(qr + 16 * kk + 2 * c) : 0u;
+            qb[kk][1] = real ? *reinterpret_cast<const uint32_t*>(qr + 16 * kk + 8 + 2 * c) : 0u;
         }
     }
-    float o[16][4];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    float m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};
-
-    const int mine = count > warp ? (count - warp + kAttWarps - 1) / kAttWarps : 0;
-    const uint32_t ring0 = smem_u32(ring) + warp * kAttStages * kPageBytes;
-    const int64_t stride = static_cast<int64_t>(a.hkv) * kHd;
-    const int last_pos = pos0 + rows - 1;
-    const auto issue = [&](int i) {
-        const int e = warp + i * kAttWarps;
-        const uint32_t dst = ring0 + (i % kAttStages) * kPageBytes;
-        const int live = last_pos - static_cast<int>(list_info[e] >> 8) * kPage;  // last row to load
-        const int64_t off = static_cast<int64_t>(list_phys[e]) * kPage * stride + h * kHd;
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-            const int row = 2 * x + (lane >> 4), piece = lane & 15;
-            const int64_t src = off + row * stride + piece * 8;
-            const uint32_t d = dst + ((piece >> 3) << 11) + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
-            cp_async16(d, a.k_pool + src, row <= live);  // rows nobody sees are zero-filled
-            cp_async16(d + kPageBytes / 2, a.v_pool + src, row <= live);
-        }
-    };
-    for (int i = 0; i < kAttStages - 1; ++i) {
-        if (i < mine) issue(i);
-        cp_async_commit();
-    }
-    for (int i = 0; i < mine; ++i) {
-        cp_async_wait<kAttStages - 2>();
-        __syncwarp();
-        if (i + kAttStages - 1 < mine) issue(i + kAttStages - 1);
-        cp_async_commit();
-        const uint32_t info = list_info[warp + i * kAttWarps];
-        const uint32_t base = ring0 + (i % kAttStages) * kPageBytes;
-        const int rel = pos0 - static_cast<int>(info >> 8) * kPage;  // first row's position in the page
-        const uint32_t mask = info & 0xffu;
-        if (!CHUNK) {
-            attend<false>(base, qa, o, m, l, rel, -1, false, 0, a.sl2e, lane);
-        } else if (rel >= kPage - 1) {  // the page lies before every row
-            const bool all = mask == (1u << rows) - 1u;
-            attend<true>(base, qa, o, m, l, ((mask >> row0) & 1u) ? kPage : -1,
-                         ((mask >> row1) & 1u) ? kPage : -1, !all, kPage, a.sl2e, lane);
-        } else {  // rows end inside the page: one row after the other
-            for (int row = 0; row < rows; ++row) {
-                if (!((mask >> row) & 1u)) continue;
-                attend<true>(base, qa, o, m, l, row0 == row ? rel + row : -1,
-                             row1 == row ? rel + row : -1, true, rel + row, a.sl2e, lane);
+    Softmax st;
+    const uint32_t wmask = warp < kChWarps ? (1u << wrows) - 1u : 0u;
+    const int pages = (pos0 + rows - 1) < 0 ? 0 : (pos0 + rows - 1) / kPage + 1;
+    bool ok = true;
+    int done = 0;  // stages of earlier windows: ring slots and phases run on
+    for (int careful = 0; careful < 2; ++careful) {
+        st.clear();
+        for (int w0 = 0; w0 < pages; w0 += kWin) {
+            for (int i = threadIdx.x; i < kWin; i += kChThreads) masks[i] = 0;
+            __syncthreads();
+            for (int i = threadIdx.x; i < rows * a.top; i += kChThreads) {
+                const int row = i / a.top;
+                const int page =
+                    a.page_ids[(static_cast<int64_t>(w.q0 + i0 + row) * a.hkv + h) * a.top + (i - row * a.top)];
+                if (page < 0) continue;
+                const int pos = pos0 + row;
+                if (pos < 0 || page > pos / kPage) {
+                    if (w0 == 0 && !careful) record_error(a.err, MSGL_ERR_BOUNDS, 803);
+                    continue;
+                }
+                if (page >= w0 && page < w0 + kWin) atomicOr(&masks[page - w0], 1ull << row);
             }
+            __syncthreads();
+            constexpr int kRun = kWin / (kChWarps * 32);
+            const int run0 = static_cast<int>(threadIdx.x) * kRun;  // the producer warp has none
+            int per = 0;
+            if (warp < kChWarps)
+                for (int i = 0; i < kRun; ++i) per += masks[run0 + i] != 0;
+            int count;
+            int at = block_excl_scan(per, scan, count);
+            if (per)
+                for (int i = 0; i < kRun; ++i) {
+                    if (!masks[run0 + i]) continue;
+                    int phys = a.page_table[static_cast<int64_t>(r) * a.max_pages + w0 + run0 + i];
+                    if (static_cast<unsigned>(phys) >= static_cast<unsigned>(a.pool_pages)) {
+                        record_error(a.err, MSGL_ERR_BOUNDS, 802);
+                        phys = 0;
+                    }
+                    list_phys[at] = phys;
+                    list_page[at++] = static_cast<uint16_t>(run0 + i);
+                }
+            __syncthreads();
+
+            const int stages = (count + kStagePages - 1) / kStagePages;
+            if (warp == kChWarps) {
+                if (lane == 0)
+                    for (int i = 0; i < stages; ++i) {
+                        const int n = done + i, s = n % kChStages;
+                        if (n >= kChStages) ok = ok && mbar_wait(&empty[s], (n / kChStages - 1) & 1, a.err, 821);
+                        if (!ok) break;
+                        const int e0 = i * kStagePages, pages_in = min(kStagePages, count - e0);
+                        uint8_t* dst = ring + s * kStageBytes;
+                        mbar_arrive_expect_tx(&full[s], pages_in * kPageBytes);
+                        for (int e = 0; e < pages_in; ++e, dst += kPageBytes) {
+                            const int y = list_phys[e0 + e] * kPage;
+                            tma_load_3d(dst, &tk, &full[s], 0, y, 2 * h);
+                            tma_load_3d(dst + kPageBytes / 2, &tv, &full[s], 0, y, 2 * h);
+                        }
+                    }
+            } else {
+                for (int i = 0, mine = 0; i < stages; ++i) {
+                    const int n = done + i, s = n % kChStages;
+                    // lane e: page e of the stage, and which of this warp's rows want it
+                    const int e = i * kStagePages + lane;
+                    int page = 0;
+                    uint32_t want = 0;
+                    if (lane < kStagePages && e < count) {
+                        page = list_page[e];
+                        want = static_cast<uint32_t>(masks[page] >> wrow) & wmask;
+                    }
+                    unsigned some = __ballot_sync(0xffffffffu, want != 0);
+                    if (ok) ok = mbar_wait(&full[s], (n / kChStages) & 1, a.err, 820);
+                    for (; some; some &= some - 1) {
+                        const int x = __ffs(some) - 1;
+                        if (!ok || mine++ % PW != pg) continue;
+                        const uint32_t mask = __shfl_sync(0xffffffffu, want, x);
+                        const uint32_t base = smem_u32(ring) + s * kStageBytes + x * kPageBytes;
+                        // the first row's position in the page
+                        const int rel = pos0 + wrow - (w0 + __shfl_sync(0xffffffffu, page, x)) * kPage;
+                        if (!careful) {
+                            attend<false>(base, qb, st, ((mask >> row0) & 1u) ? rel + row0 : -1,
+                                          ((mask >> row1) & 1u) ? rel + row1 : -1, 0, a.sl2e, lane);
+                        } else {
+                            // rows that see the whole page go together, one that ends inside it alone
+                            for (uint32_t left = mask; left;) {
+                                const int row = __ffs(left) - 1;
+                                const uint32_t now = rel + row >= kPage - 1 ? left : 1u << row;
+                                left &= ~now;
+                                attend<true>(base, qb, st, ((now >> row0) & 1u) ? rel + row : -1,
+                                             ((now >> row1) & 1u) ? rel + row : -1, rel + row, a.sl2e, lane);
+                            }
+                        }
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&empty[s]);
+                }
+            }
+            done += stages;
+            __syncthreads();
         }
-        __syncwarp();
+        float sum = 0.f;  // NaN where a sum is infinite or NaN
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += 0.f * ((st.o[j][0] + st.o[j][1]) + (st.o[j][2] + st.o[j][3]));
+        if (!__syncthreads_or(sum != sum)) break;
     }
 
-    // ---- join the warps' results (shared memory over the drained rings)
-    float ls[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        ls[u] = l[u] + __shfl_xor_sync(0xffffffffu, l[u], 1);
-        ls[u] += __shfl_xor_sync(0xffffffffu, ls[u], 2);
-    }
-    cp_async_wait<0>();
+    // ---- join the page groups, normalise, store
+    float* mo = reinterpret_cast<float*>(ring);  // [16 warps][8][kPad]
+    if (warp < kChWarps) dump(st, mo + warp * 8 * kPad, sm + warp * 8, sl + warp * 8, lane);
     __syncthreads();
-    constexpr int kRows = TWO ? 16 : 8;
-    float* mo = reinterpret_cast<float*>(ring);          // [4][kRows][128]
-    float* mm = mo + kAttWarps * kRows * kHd;            // [4][kRows]
-    float* ml = mm + kAttWarps * kRows;
-#pragma unroll
-    for (int u = 0; u < (TWO ? 2 : 1); ++u) {
-        const int row = warp * kRows + g + 8 * u;
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-            *reinterpret_cast<float2*>(mo + row * kHd + 8 * j + 2 * c) = make_float2(o[j][2 * u], o[j][2 * u + 1]);
-        if (c == 0) {
-            mm[row] = m[u];
-            ml[row] = ls[u];
-        }
-    }
-    __syncthreads();
-    for (int item = threadIdx.x; item < rows * G * 16; item += kAttThreads) {
-        const int mr = item >> 4, d0 = (item & 15) * 8;
-        float M = kNegInf;
-        for (int k = 0; k < kAttWarps; ++k) M = fmaxf(M, mm[k * kRows + mr]);
-        float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, L = 0.f;
-        for (int k = 0; k < kAttWarps; ++k) {
-            const float mk = mm[k * kRows + mr];
-            if (mk == kNegInf && ml[k * kRows + mr] == 0.f) continue;  // saw no key
-            const float sc = exp2f(mk - M);
-            L += ml[k * kRows + mr] * sc;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] += mo[(k * kRows + mr) * kHd + d0 + e] * sc;
-        }
-        const float inv = L == 0.f ? 0.f : 1.f / L;  // an empty list gives a zero row
-        uint4 u;
-        u.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
-        u.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
-        u.z = pack_bf16x2(acc[4] * inv, acc[5] * inv);
-        u.w = pack_bf16x2(acc[6] * inv, acc[7] * inv);
-        const int tr = mr / G;
-        *reinterpret_cast<uint4*>(a.out + (static_cast<int64_t>(w.q0 + i0 + tr) * a.hq + h * G + mr % G) * kHd + d0) = u;
+    for (int item = threadIdx.x; item < rows * G * 16; item += kChThreads) {
+        const int tr = (item >> 4) / G, head = (item >> 4) % G, d0 = (item & 15) * 8;
+        const int col = tr / TQ * 8 + tr % TQ * G + head;  // in the first page group
+        float M, L, acc[8];
+        join(mo + col * kPad + d0, sm + col, sl + col, PW, RW * 8, M, L, acc);
+        // an empty list gives a zero row
+        *reinterpret_cast<uint4*>(a.out + (static_cast<int64_t>(w.q0 + i0 + tr) * a.hq + h * G + head) * kHd + d0) =
+            pack8(acc, L == 0.f ? 0.f : 1.f / L);
     }
 }
 
@@ -1055,6 +1285,36 @@ int slab_rows(int total_q, int stride, int hkv) {
     const int64_t rows = std::max<int64_t>(16, kSelectBytes / (int64_t(16) * stride * hkv));
     return static_cast<int>(std::min<int64_t>(total_q, rows));
 }
+// CTAs that share a list in decode: a power of two up to the portable cluster size, as many as two
+// CTAs per SM hold, of at least 4 pages (one a warp) each.
+int decode_split(int64_t lists, int top) {
+    int s = 1;
+    while (s < 8 && lists * s * 2 <= 2 * 148 && top >= 8 * s) s *= 2;
+    return s;
+}
+
+// launch_pdl with a thread-block cluster of `size` CTAs.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, int size, size_t smem, cudaStream_t stream,
+                           Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kAttThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    launch_counter().fetch_add(1, std::memory_order_relaxed);
+    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
 int score_stride(int max_seq_len) { return std::max(16, (pages_of(max_seq_len) + 15) / 16 * 16); }
 
 }  // namespace
@@ -1229,19 +1489,37 @@ int msgl_paged_attention_pages(const void* q, const void* k_pool, const void* v_
     a.out = static_cast<__nv_bfloat16*>(out);
     a.err = device_error_word();
     if (!a.err) return set_error(MSGL_ERR_CUDA, "device error word unavailable");
-    const bool chunk = max_q_len > 1;
     const int G = num_q_heads / num_kv_heads;
-    const int TQ = chunk ? std::min(8, 16 / G) : 1;
-    const int tiles = (max_q_len + TQ - 1) / TQ;
+    if (max_q_len > 1) {
+        CUtensorMap tk, tv;  // {64 dims, token rows, head halves}: one page of one kv head a box
+        const uint64_t row = uint64_t(num_kv_heads) * kHd * 2;
+        rc = make_tmap_3d_bf16(&tk, k_pool, 64, num_slots, 2 * num_kv_heads, row, 128, 64, kPage, 2);
+        if (!rc) rc = make_tmap_3d_bf16(&tv, v_pool, 64, num_slots, 2 * num_kv_heads, row, 128, 64, kPage, 2);
+        if (rc) return rc;
+        const int tq = 8 / G;
+        int row_groups = 1;
+        while (row_groups < kChWarps && row_groups * tq < std::min(max_q_len, kTileRows)) row_groups *= 2;
+        const int tiles = (max_q_len + row_groups * tq - 1) / (row_groups * tq);
+        const int64_t blocks = int64_t(num_reqs) * tiles * num_kv_heads;
+        if (blocks > INT32_MAX) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "attention_pages: batch too large");
+        static std::atomic<int> optin[kMaxDevices];
+        cudaError_t e = smem_optin(attend_pages_chunk_kernel, kChSmem, optin);
+        if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
+        launch_pdl(attend_pages_chunk_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kChThreads), kChSmem, stream,
+                   tk, tv, a, tiles, row_groups);
+        MSGL_LAUNCH_CHECK();
+        return MSGL_OK;
+    }
     const int words = pages_of(max_seq_len) / 32 + 1;
-    const size_t smem = kAttRing + size_t(TQ) * words * 4 + size_t(std::min(TQ * top_pages, 32 * words)) * 8;
-    const int64_t blocks = int64_t(num_reqs) * tiles * num_kv_heads;
-    if (blocks > INT32_MAX) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "attention_pages: batch too large");
-    static std::atomic<int> optin[2][kMaxDevices];
-    const auto kern = chunk ? attend_pages_kernel<true> : attend_pages_kernel<false>;
-    cudaError_t e = smem_optin(kern, smem, optin[chunk]);
+    const size_t smem = kDecRing + size_t(words) * 4 + size_t(top_pages) * 8;
+    const int64_t lists = int64_t(num_reqs) * num_kv_heads;
+    if (lists * 16 > INT32_MAX) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "attention_pages: batch too large");
+    const int split = decode_split(lists, top_pages);
+    static std::atomic<int> optin[kMaxDevices];
+    cudaError_t e = smem_optin(attend_pages_decode_kernel, smem, optin);
     if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
-    launch_pdl(kern, dim3(static_cast<unsigned>(blocks)), dim3(kAttThreads), smem, stream, a, tiles, words);
+    e = launch_cluster(attend_pages_decode_kernel, static_cast<unsigned>(lists * split), split, smem, stream, a, words);
+    if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
     MSGL_LAUNCH_CHECK();
     return MSGL_OK;
 }
