@@ -284,8 +284,8 @@ __device__ __forceinline__ unsigned long long key_of(double v) {
     return (b >> 63) ? ~b : b | 0x8000000000000000ull;
 }
 
-// Score key of one page beyond fp32, by each group of eight lanes (every lane of the group gets it;
-// all lanes of the warp call it). bounds_row: lo then hi of the page; q: the group's G query heads.
+// Score key of one page and query head beyond fp32, by each group of eight lanes (every lane of the
+// group gets it; all lanes of the warp call it). bounds_row: lo then hi of the page.
 // A term is q (q > 0 ? hi : lo) plus zero times the other bound (NaN where that is infinite or NaN).
 // With `narrow` (scores well inside the fp32 range) the products of two bf16 values are exact in
 // fp32 and are summed as an unevaluated pair of fp32 values (Knuth's two-sum, about 2^-46 relative),
@@ -293,55 +293,50 @@ __device__ __forceinline__ unsigned long long key_of(double v) {
 // loops stay rolled: few rows come here, and most of what a long body would cost them is fetching it.
 template <bool NARROW>
 __device__ __noinline__ unsigned long long exact_key(const __nv_bfloat16* __restrict__ bounds_row,
-                                                     const __nv_bfloat16* __restrict__ q, int G, int lane) {
+                                                     const __nv_bfloat16* __restrict__ q, int lane) {
     const int d = 16 * (lane & 7);
-    unsigned long long best = 0ull;
+    float sum = 0.f, rest = 0.f;
+    double wide = 0.0;
+    // (sum, rest) += (t, r); the same bits whichever side is which
+    const auto add = [&](float t, float r) {
+        const float n = __fadd_rn(sum, t), z = __fadd_rn(n, -sum);
+        const float err = __fadd_rn(__fadd_rn(sum, -__fadd_rn(n, -z)), __fadd_rn(t, -z));
+        rest = __fadd_rn(__fadd_rn(rest, r), err);
+        sum = n;
+    };
 #pragma unroll 1
-    for (int g = 0; g < G; ++g) {
-        float sum = 0.f, rest = 0.f;
-        double wide = 0.0;
-        // (sum, rest) += (t, r); the same bits whichever side is which
-        const auto add = [&](float t, float r) {
-            const float n = __fadd_rn(sum, t), z = __fadd_rn(n, -sum);
-            const float err = __fadd_rn(__fadd_rn(sum, -__fadd_rn(n, -z)), __fadd_rn(t, -z));
-            rest = __fadd_rn(__fadd_rn(rest, r), err);
-            sum = n;
-        };
-#pragma unroll 1
-        for (int i = 0; i < 16; i += 8) {
-            const uint4 xv = *reinterpret_cast<const uint4*>(q + g * kHd + d + i);
-            const uint4 lv = *reinterpret_cast<const uint4*>(bounds_row + d + i);
-            const uint4 hv = *reinterpret_cast<const uint4*>(bounds_row + kHd + d + i);
-            const uint32_t x[4] = {xv.x, xv.y, xv.z, xv.w};
-            const uint32_t lo[4] = {lv.x, lv.y, lv.z, lv.w};
-            const uint32_t hi[4] = {hv.x, hv.y, hv.z, hv.w};
+    for (int i = 0; i < 16; i += 8) {
+        const uint4 xv = *reinterpret_cast<const uint4*>(q + d + i);
+        const uint4 lv = *reinterpret_cast<const uint4*>(bounds_row + d + i);
+        const uint4 hv = *reinterpret_cast<const uint4*>(bounds_row + kHd + d + i);
+        const uint32_t x[4] = {xv.x, xv.y, xv.z, xv.w};
+        const uint32_t lo[4] = {lv.x, lv.y, lv.z, lv.w};
+        const uint32_t hi[4] = {hv.x, hv.y, hv.z, hv.w};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float f = e & 1 ? bf16hi(x[e >> 1]) : bf16lo(x[e >> 1]);
-                const float l = e & 1 ? bf16hi(lo[e >> 1]) : bf16lo(lo[e >> 1]);
-                const float h = e & 1 ? bf16hi(hi[e >> 1]) : bf16lo(hi[e >> 1]);
-                const float mine = f > 0.f ? h : l, other = __fmul_rn(0.f, f > 0.f ? l : h);
-                if constexpr (NARROW) add(__fmul_rn(f, mine), other);
-                else wide += static_cast<double>(f) * mine + other;
-            }
-        }
-#pragma unroll 1
-        for (int o = 4; o > 0; o >>= 1) {
-            if constexpr (NARROW) {
-                const float t = __shfl_xor_sync(0xffffffffu, sum, o);
-                add(t, __shfl_xor_sync(0xffffffffu, rest, o));
-            } else {
-                wide += __shfl_xor_sync(0xffffffffu, wide, o);
-            }
-        }
-        if constexpr (NARROW) {
-            const float top = __fadd_rn(sum, rest), low = __fadd_rn(rest, -__fadd_rn(top, -sum));
-            best = max(best, static_cast<unsigned long long>(key_of(top)) << 32 | key_of(low));
-        } else {
-            best = max(best, key_of(wide));
+        for (int e = 0; e < 8; ++e) {
+            const float f = e & 1 ? bf16hi(x[e >> 1]) : bf16lo(x[e >> 1]);
+            const float l = e & 1 ? bf16hi(lo[e >> 1]) : bf16lo(lo[e >> 1]);
+            const float h = e & 1 ? bf16hi(hi[e >> 1]) : bf16lo(hi[e >> 1]);
+            const float mine = f > 0.f ? h : l, other = __fmul_rn(0.f, f > 0.f ? l : h);
+            if constexpr (NARROW) add(__fmul_rn(f, mine), other);
+            else wide += static_cast<double>(f) * mine + other;
         }
     }
-    return best;
+#pragma unroll 1
+    for (int o = 4; o > 0; o >>= 1) {
+        if constexpr (NARROW) {
+            const float t = __shfl_xor_sync(0xffffffffu, sum, o);
+            add(t, __shfl_xor_sync(0xffffffffu, rest, o));
+        } else {
+            wide += __shfl_xor_sync(0xffffffffu, wide, o);
+        }
+    }
+    if constexpr (NARROW) {
+        const float top = __fadd_rn(sum, rest), low = __fadd_rn(rest, -__fadd_rn(top, -sum));
+        return static_cast<unsigned long long>(key_of(top)) << 32 | key_of(low);
+    } else {
+        return key_of(wide);
+    }
 }
 
 // Bit number of the lane group's set bit: the group's index (0 .. 3) from the lowest, at most the last.
@@ -366,7 +361,9 @@ struct RowGroup {
         unsigned long long red64[2][32];
         uint32_t key[kListCap];
         int page[kListCap];
-        int n, req;
+        unsigned long long exact[kListCap];  // of the open pages
+        int open[kListCap];
+        int n, req, n_open;
     };
     Shared& sh;
     int warp, lane, turn;
@@ -568,8 +565,9 @@ select_pages_kernel(const SelectArgs a, int num_rows) {
         if (static_cast<unsigned>(phys) >= static_cast<unsigned>(a.pool_pages)) phys = 0;  // recorded
         return a.bounds + (static_cast<int64_t>(phys) * a.hkv + h) * 2 * kHd;
     };
-    const auto again = [&](const __nv_bfloat16* b) {
-        return narrow ? exact_key<true>(b, qrow, G, lane) : exact_key<false>(b, qrow, G, lane);
+    const auto again = [&](int j, int g) {
+        const __nv_bfloat16* b = bounds_of(j);
+        return narrow ? exact_key<true>(b, qrow + g * kHd, lane) : exact_key<false>(b, qrow + g * kHd, lane);
     };
     if (listed == want) {
         high = low - 1;  // all of them
@@ -584,9 +582,11 @@ select_pages_kernel(const SelectArgs a, int num_rows) {
                 }
         }
         row.sync();
+        bool take = false, mine_open = false;
+        int page = 0, left = 0;
         if (row.warp == 0) {
             const uint32_t mine = lane < listed ? sh.key[lane] : 0u;
-            const int page = lane < listed ? sh.page[lane] : 0;
+            page = lane < listed ? sh.page[lane] : 0;
             int more = 0, same = 0;
 #pragma unroll
             for (int o = 0; o < 32; ++o) {
@@ -607,31 +607,42 @@ select_pages_kernel(const SelectArgs a, int num_rows) {
                 if (next == 0u) top_key = 0u;
                 else if (next <= kInfKey) top_key = key_of(__fadd_ru(value_of(next), eps2));
             }
-            bool take = mine > top_key && mine >= low_key;
-            const unsigned open = __ballot_sync(0xffffffffu, mine && !take && mine >= low_key);
-            const int left = want - __popc(__ballot_sync(0xffffffffu, take));
+            take = mine > top_key && mine >= low_key;
+            mine_open = mine && !take && mine >= low_key;
+            const unsigned open = __ballot_sync(0xffffffffu, mine_open);
+            left = want - __popc(__ballot_sync(0xffffffffu, take));
             if (__popc(open) <= left) {
-                take = take || (open >> lane & 1u);
-            } else {  // scored again, four pages at a time
-                unsigned long long exact = 0ull;
-                for (unsigned m = open; m;) {
-                    const int src = group_bit(m, lane);
-                    const unsigned long long k = again(bounds_of(__shfl_sync(0xffffffffu, page, src)));
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const unsigned long long ke = __shfl_sync(0xffffffffu, k, 8 * e);
-                        if (m && lane == __ffs(m) - 1) exact = ke;
-                        m &= m - 1;
-                    }
+                take = take || mine_open;
+                mine_open = false;
+                if (lane == 0) sh.n_open = 0;
+            } else {
+                if (lane == 0) sh.n_open = __popc(open);
+                if (mine_open) {
+                    const int i = __popc(open & ((1u << lane) - 1));
+                    sh.open[i] = page;
+                    sh.exact[i] = 0ull;
                 }
-                int rank = 0;  // by (exact key, lower page)
-                for (unsigned m = open; m; m &= m - 1) {
-                    const int o = __ffs(m) - 1;
-                    const unsigned long long k = __shfl_sync(0xffffffffu, exact, o);
-                    const int p = __shfl_sync(0xffffffffu, page, o);
-                    rank += k > exact || (k == exact && p < page);
-                }
-                take = take || ((open >> lane & 1u) && rank < left);
+            }
+        }
+        row.sync();
+        const int n_open = sh.n_open;
+        if (n_open) {  // scored again: a page and head per group of eight lanes, over all warps
+            for (int i0 = row.warp * 4; i0 < n_open * G; i0 += 4 * W) {
+                const int i = min(i0 + (lane >> 3), n_open * G - 1);
+                const unsigned long long k = again(sh.open[i / G], i % G);
+                if ((lane & 7) == 0) atomicMax(&sh.exact[i / G], k);
+            }
+            row.sync();
+        }
+        if (row.warp == 0) {
+            if (mine_open) {
+                unsigned long long k = 0ull;
+                for (int o = 0; o < n_open; ++o)
+                    if (sh.open[o] == page) k = sh.exact[o];
+                int rank = 0;  // by (score, lower page)
+                for (int o = 0; o < n_open; ++o)
+                    rank += sh.exact[o] > k || (sh.exact[o] == k && sh.open[o] < page);
+                take = rank < left;
             }
             if (take) atomicOr(&picked[slot][page >> 5], 1u << (page & 31));
         }
@@ -647,7 +658,9 @@ select_pages_kernel(const SelectArgs a, int num_rows) {
             unsigned m = __ballot_sync(0xffffffffu, k >= low && k <= high);
             while (m) {  // four pages at a time
                 const int j = j0 + group_bit(m, lane);
-                wide[j] = again(bounds_of(j));
+                unsigned long long k = 0ull;
+                for (int g = 0; g < G; ++g) k = max(k, again(j, g));
+                wide[j] = k;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) m &= m - 1;
             }
@@ -904,7 +917,7 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8], float f) {
 }
 
 // ---- single tokens
-// A cluster of up to 8 CTAs (decode_split) per (query row, kv head): each CTA
+// A cluster of up to 16 CTAs (decode_split) per (query row, kv head): each CTA
 // takes a share of the listed pages, its four warps take its pages in turn, every warp with a ring
 // of its own (cp.async, 16 bytes a lane, three pages) and an online softmax. The warps' results are
 // joined in shared memory, the CTAs' through distributed shared memory, each CTA finishing a share
@@ -966,17 +979,17 @@ attend_pages_decode_kernel(const AttArgs a, int words) {
     const int lo = static_cast<int>(static_cast<int64_t>(total) * rank / S);       // this CTA's share
     const int count = static_cast<int>(static_cast<int64_t>(total) * (rank + 1) / S) - lo;
     for (int i = w_lo; i < w_hi; ++i)
-        for (uint32_t b = bits[i]; b; b &= b - 1, ++at) {
-            if (at < lo || at >= lo + count) continue;
-            const int page = i * 32 + __ffs(b) - 1;
-            int phys = a.page_table[static_cast<int64_t>(r) * a.max_pages + page];
-            if (static_cast<unsigned>(phys) >= static_cast<unsigned>(a.pool_pages)) {
-                record_error(a.err, MSGL_ERR_BOUNDS, 802);
-                phys = 0;
-            }
-            list_phys[at - lo] = phys;
-            list_page[at - lo] = page;
+        for (uint32_t b = bits[i]; b; b &= b - 1, ++at)
+            if (at >= lo && at < lo + count) list_page[at - lo] = i * 32 + __ffs(b) - 1;
+    __syncthreads();
+    for (int i = threadIdx.x; i < count; i += kAttThreads) {  // all in flight together
+        int phys = a.page_table[static_cast<int64_t>(r) * a.max_pages + list_page[i]];
+        if (static_cast<unsigned>(phys) >= static_cast<unsigned>(a.pool_pages)) {
+            record_error(a.err, MSGL_ERR_BOUNDS, 802);
+            phys = 0;
         }
+        list_phys[i] = phys;
+    }
     __syncthreads();
 
     Softmax st;
@@ -1039,29 +1052,28 @@ attend_pages_decode_kernel(const AttArgs a, int words) {
     }
     if (S == 1) return;
     cluster_sync_all();
-    for (int item = rank + S * threadIdx.x; item < G * 16; item += S * kAttThreads) {
-        const int head = item >> 4, d0 = (item & 15) * 8;
-        float mk[8], lk[8], M = kNegInf;
+    // item (column, 8 dims) i of every S, its S parts loaded by as many neighbouring lanes
+    const int part = threadIdx.x % S;
+    for (int i0 = 0; i0 < G * 16; i0 += kAttThreads) {
+        const int item = i0 + threadIdx.x / S * S + rank;
+        const bool live = item < G * 16;
+        const int head = live ? item >> 4 : 0, d0 = live ? (item & 15) * 8 : 0;
+        const uint32_t src = mapa_shared(smem_u32(co + head * kHd + d0), part);
+        const float mk = ld_dsmem_f32(mapa_shared(smem_u32(cm + head), part));
+        const float lk = ld_dsmem_f32(mapa_shared(smem_u32(cl + head), part));
+        const float4 u = ld_dsmem_v4(src), v = ld_dsmem_v4(src + 16);
+        float M = mk;
+        for (int o = 1; o < S; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        // parts that saw no key count nothing (their m may be the -inf that M is too)
+        const float sc = mk == kNegInf && lk == 0.f ? 0.f : exp2f(mk - M);
+        float L = lk * sc, acc[8] = {u.x * sc, u.y * sc, u.z * sc, u.w * sc, v.x * sc, v.y * sc, v.z * sc, v.w * sc};
+        for (int o = 1; o < S; o <<= 1) {
+            L += __shfl_xor_sync(0xffffffffu, L, o);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            mk[k] = k < S ? ld_dsmem_f32(mapa_shared(smem_u32(cm + head), k)) : kNegInf;
-            lk[k] = k < S ? ld_dsmem_f32(mapa_shared(smem_u32(cl + head), k)) : 0.f;
+            for (int e = 0; e < 8; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], o);
         }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) M = fmaxf(M, mk[k]);
-        float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, L = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if (k >= S) break;
-            const uint32_t src = mapa_shared(smem_u32(co + head * kHd + d0), k);
-            const float4 u = ld_dsmem_v4(src), v = ld_dsmem_v4(src + 16);
-            if (mk[k] == kNegInf && lk[k] == 0.f) continue;
-            const float sc = exp2f(mk[k] - M);
-            L += lk[k] * sc;
-            acc[0] += u.x * sc; acc[1] += u.y * sc; acc[2] += u.z * sc; acc[3] += u.w * sc;
-            acc[4] += v.x * sc; acc[5] += v.y * sc; acc[6] += v.z * sc; acc[7] += v.w * sc;
-        }
-        *reinterpret_cast<uint4*>(out + head * kHd + d0) = pack8(acc, L == 0.f ? 0.f : 1.f / L);
+        if (live && part == 0)
+            *reinterpret_cast<uint4*>(out + head * kHd + d0) = pack8(acc, L == 0.f ? 0.f : 1.f / L);
     }
     cluster_sync_all();  // no CTA leaves while another reads its shared memory
 }
@@ -1285,12 +1297,25 @@ int slab_rows(int total_q, int stride, int hkv) {
     const int64_t rows = std::max<int64_t>(16, kSelectBytes / (int64_t(16) * stride * hkv));
     return static_cast<int>(std::min<int64_t>(total_q, rows));
 }
-// CTAs that share a list in decode: a power of two up to the portable cluster size, as many as two
-// CTAs per SM hold, of at least 4 pages (one a warp) each.
+// CTAs that share a list in decode: a power of two up to the largest cluster (16, above the portable
+// 8), as many as two CTAs per SM hold, of at least 4 pages (one a warp) each.
 int decode_split(int64_t lists, int top) {
     int s = 1;
-    while (s < 8 && lists * s * 2 <= 2 * 148 && top >= 8 * s) s *= 2;
+    while (s < 16 && lists * s * 2 <= 2 * 148 && top >= 8 * s) s *= 2;
     return s;
+}
+
+// Opts the decode kernel in to clusters above the portable size, once per device.
+cudaError_t large_clusters() {
+    static std::atomic<bool> done[kMaxDevices];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const bool cached = dev >= 0 && dev < kMaxDevices;
+    if (cached && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+    e = cudaFuncSetAttribute(attend_pages_decode_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && cached) done[dev].store(true, std::memory_order_release);
+    return e;
 }
 
 // launch_pdl with a thread-block cluster of `size` CTAs.
@@ -1517,6 +1542,7 @@ int msgl_paged_attention_pages(const void* q, const void* k_pool, const void* v_
     const int split = decode_split(lists, top_pages);
     static std::atomic<int> optin[kMaxDevices];
     cudaError_t e = smem_optin(attend_pages_decode_kernel, smem, optin);
+    if (e == cudaSuccess && split > 8) e = large_clusters();
     if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
     e = launch_cluster(attend_pages_decode_kernel, static_cast<unsigned>(lists * split), split, smem, stream, a, words);
     if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
