@@ -14,12 +14,15 @@ from ._lib import check, lib
 BF16, F32 = 1, 0
 _DT = {torch.bfloat16: BF16, torch.float32: F32}
 _SECTIONS = C.c_int * 3
+_BF, _F32, _I32, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
+_device = torch._C._cuda_getDevice                 # the current device's index
+_raw_stream = torch._C._cuda_getCurrentRawStream   # its current stream's handle
 
 
 def _s():
     """The current stream's handle. The raw lookup costs 0.2 us; torch.cuda.current_stream() builds
     a Stream object (3.3 us)."""
-    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+    return _raw_stream(_device())
 
 
 def _p(t):
@@ -33,11 +36,10 @@ def _c(t, dtype=None):
     return t
 
 
-def _on(dtype, *tensors):
-    """Contiguous tensors of one dtype on the current device (whose stream the call uses)."""
-    dev = torch._C._cuda_getDevice()
+def _on(dev, dtype, *tensors):
+    """Contiguous tensors of one dtype on the current device `dev` (whose stream the call uses)."""
     for t in tensors:
-        if t.get_device() != dev or t.dtype != dtype or not t.is_contiguous():
+        if t.get_device() != dev or t.dtype is not dtype or not t.is_contiguous():
             raise ValueError(f"expected a contiguous {dtype} tensor on cuda:{dev}, got {t.dtype} "
                              f"{tuple(t.shape)} with strides {t.stride()} on {t.device}")
 
@@ -129,58 +131,49 @@ def qknorm_rope_store_kv_partials(parts, k_pool, v_pool, positions, slot_mapping
     return q
 
 
-def _mrope_args(positions, slot_mapping, cos_sin, q_norm, k_norm, k_pool, v_pool, sections, head_dim):
-    """Checked [3, T] positions (any row stride): T, their row stride, the host section array."""
-    _on(torch.int32, slot_mapping)
-    _on(torch.float32, cos_sin)
+def _mrope(entry, head, x, x_dtype, k_pool, v_pool, positions, slot_mapping, cos_sin, q_norm, k_norm,
+           hq, hkv, eps, sections, interleaved, D, out):
+    dev = _device()
     three, T = positions.shape
-    if (three != 3 or positions.dtype != torch.int32 or positions.get_device() != slot_mapping.get_device()
+    if (three != 3 or positions.dtype is not _I32 or positions.get_device() != dev
             or (T > 1 and positions.stride(1) != 1)):
         raise ValueError("expected int32 positions [3, T] with contiguous rows on the current device")
-    assert slot_mapping.numel() == T, "expected slot_mapping [T]"
-    assert cos_sin.dim() == 2 and cos_sin.shape[1] == head_dim, "expected cos_sin [max_position, D]"
-    assert q_norm.numel() == head_dim and k_norm.numel() == head_dim, "expected norm weights [D]"
-    assert k_pool.numel() == v_pool.numel(), "expected pools of one size"
-    return T, positions.stride(0), _SECTIONS(*sections)
+    if out is None:
+        out = torch.empty(T, hq, D, dtype=_BF, device=x.device)
+    _on(dev, x_dtype, x)
+    _on(dev, _BF, k_pool, v_pool, q_norm, k_norm, out)
+    _on(dev, _I32, slot_mapping)
+    _on(dev, _F32, cos_sin)
+    slots = k_pool.numel()
+    max_position, two = cos_sin.shape
+    assert x.numel() == (head[1] if head[1:] else 1) * T * (hq + 2 * hkv) * D, "expected rows of (Hq + 2 Hkv) D"
+    assert slot_mapping.numel() == T and out.numel() == T * hq * D, "expected slot_mapping [T], out [T, Hq, D]"
+    assert two == q_norm.numel() == k_norm.numel() == D, "expected cos_sin [max_position, D], norm weights [D]"
+    assert v_pool.numel() == slots, "expected pools of one size"
+    check(entry(*head, out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), slots // (hkv * D),
+                positions.data_ptr(), positions.stride(0), _SECTIONS(*sections), interleaved,
+                slot_mapping.data_ptr(), cos_sin.data_ptr(), max_position, q_norm.data_ptr(),
+                k_norm.data_ptr(), T, hq, hkv, D, eps, _raw_stream(dev)))
+    return out
 
 
 def qknorm_mrope_store_kv(qkv, k_pool, v_pool, positions, slot_mapping, cos_sin, q_norm, k_norm,
                           num_q_heads, num_kv_heads, eps, sections, interleaved=False, head_dim=128,
                           out=None):
-    """As qknorm_rope_store_kv with positions [3, T] (time, height, width rows) and `sections`, the
-    rotary pairs of each axis (sum head_dim / 2): consecutive ranges, or interleaved."""
-    if out is None:
-        out = torch.empty(positions.shape[1], num_q_heads, head_dim, dtype=torch.bfloat16, device=qkv.device)
-    _on(torch.bfloat16, qkv, k_pool, v_pool, q_norm, k_norm, out)
-    T, stride, sec = _mrope_args(positions, slot_mapping, cos_sin, q_norm, k_norm, k_pool, v_pool, sections, head_dim)
-    assert qkv.numel() == T * (num_q_heads + 2 * num_kv_heads) * head_dim, "expected qkv [T, (Hq + 2 Hkv) D]"
-    assert out.numel() == T * num_q_heads * head_dim, "expected out [T, Hq, D]"
-    num_slots = k_pool.numel() // (num_kv_heads * head_dim)
-    check(lib().msgl_qknorm_mrope_store_kv(
-        _p(qkv), _p(out), _p(k_pool), _p(v_pool), num_slots, _p(positions), stride, sec,
-        int(interleaved), _p(slot_mapping), _p(cos_sin), cos_sin.shape[0], _p(q_norm), _p(k_norm), T, num_q_heads,
-        num_kv_heads, head_dim, eps, _s()))
-    return out
+    """As qknorm_rope_store_kv with positions [3, T] (time, height, width rows; any row stride) and
+    `sections`, the rotary pairs of each axis (sum head_dim / 2): consecutive ranges, or interleaved."""
+    return _mrope(lib().msgl_qknorm_mrope_store_kv, (qkv.data_ptr(),), qkv, _BF, k_pool, v_pool, positions,
+                  slot_mapping, cos_sin, q_norm, k_norm, num_q_heads, num_kv_heads, eps, sections,
+                  interleaved, head_dim, out)
 
 
 def qknorm_mrope_store_kv_partials(parts, k_pool, v_pool, positions, slot_mapping, cos_sin, q_norm,
                                    k_norm, num_q_heads, num_kv_heads, eps, sections,
                                    interleaved=False, head_dim=128, out=None):
     """As qknorm_mrope_store_kv with the QKV rows the sum of fp32 partials [P, T, (Hq+2Hkv) D]."""
-    if out is None:
-        out = torch.empty(positions.shape[1], num_q_heads, head_dim, dtype=torch.bfloat16, device=parts.device)
-    _on(torch.float32, parts)
-    _on(torch.bfloat16, k_pool, v_pool, q_norm, k_norm, out)
-    T, stride, sec = _mrope_args(positions, slot_mapping, cos_sin, q_norm, k_norm, k_pool, v_pool, sections, head_dim)
-    nparts = parts.shape[0]
-    assert parts.numel() == nparts * T * (num_q_heads + 2 * num_kv_heads) * head_dim, "expected parts [P, T, (Hq + 2 Hkv) D]"
-    assert out.numel() == T * num_q_heads * head_dim, "expected out [T, Hq, D]"
-    num_slots = k_pool.numel() // (num_kv_heads * head_dim)
-    check(lib().msgl_qknorm_mrope_store_kv_partials(
-        _p(parts), nparts, _p(out), _p(k_pool), _p(v_pool), num_slots, _p(positions), stride, sec,
-        int(interleaved), _p(slot_mapping), _p(cos_sin), cos_sin.shape[0], _p(q_norm), _p(k_norm), T,
-        num_q_heads, num_kv_heads, head_dim, eps, _s()))
-    return out
+    return _mrope(lib().msgl_qknorm_mrope_store_kv_partials, (parts.data_ptr(), parts.shape[0]), parts, _F32,
+                  k_pool, v_pool, positions, slot_mapping, cos_sin, q_norm, k_norm, num_q_heads,
+                  num_kv_heads, eps, sections, interleaved, head_dim, out)
 
 
 def decode_advance(next_tokens, input_ids, positions, slot_mapping, page_table, seq_lens,
@@ -288,30 +281,31 @@ def paged_attention_extend(q, k_pool, v_pool, page_table, seq_lens, q_indptr, ma
 
 
 # ------------------------------------------------------------------ page-sparse attention
-def _rows(page_table, seq_lens, q_indptr, max_q_len, total_q):
-    """Checked request metadata of the page-sparse calls: the request count."""
-    _on(torch.int32, page_table, seq_lens)
-    B = seq_lens.numel()
-    assert page_table.dim() == 2 and page_table.shape[0] == B, "expected a page-table row per request"
+def _rows(dev, page_table, seq_lens, q_indptr, max_q_len, total_q):
+    """Checked request metadata of the page-sparse calls: (request count, table width, indptr)."""
+    _on(dev, _I32, page_table, seq_lens)
+    B, width = page_table.shape
+    assert seq_lens.numel() == B, "expected a page-table row per request"
     if q_indptr is None:
-        assert max_q_len == 1 and total_q in (None, B), "one query row per request without q_indptr"
-    else:
-        _on(torch.int32, q_indptr)
-        assert q_indptr.numel() == B + 1, "expected q_indptr [num_reqs + 1]"
-    return B
+        assert max_q_len == 1 and (total_q is None or total_q == B), "one query row per request without q_indptr"
+        return B, width, None
+    _on(dev, _I32, q_indptr)
+    assert q_indptr.numel() == B + 1, "expected q_indptr [num_reqs + 1]"
+    return B, width, q_indptr.data_ptr()
 
 
 def kv_page_bounds_(bounds, k_pool, page_table, seq_lens, num_kv_heads, q_indptr=None, max_q_len=1,
                     head_dim=128, page_size=16):
     """msgl_kv_page_bounds: smallest / largest key of the pages the last rows of each request
     touch, into bounds [num_pages, Hkv, 2, D] bf16 (in place)."""
-    _on(torch.bfloat16, bounds, k_pool)
-    B = _rows(page_table, seq_lens, q_indptr, max_q_len, None)
-    num_slots = k_pool.numel() // (num_kv_heads * head_dim)
-    assert bounds.numel() * page_size == 2 * k_pool.numel(), "expected bounds [num_pages, Hkv, 2, D]"
-    check(lib().msgl_kv_page_bounds(_p(k_pool), num_slots, _p(page_table), page_table.shape[1],
-                                    _p(seq_lens), _p(q_indptr), B, max_q_len, num_kv_heads,
-                                    head_dim, page_size, _p(bounds), _s()))
+    dev = _device()
+    _on(dev, _BF, bounds, k_pool)
+    B, width, indptr = _rows(dev, page_table, seq_lens, q_indptr, max_q_len, None)
+    keys = k_pool.numel()
+    assert bounds.numel() * page_size == 2 * keys, "expected bounds [num_pages, Hkv, 2, D]"
+    check(lib().msgl_kv_page_bounds(k_pool.data_ptr(), keys // (num_kv_heads * head_dim), page_table.data_ptr(),
+                                    width, seq_lens.data_ptr(), indptr, B, max_q_len, num_kv_heads, head_dim,
+                                    page_size, bounds.data_ptr(), _raw_stream(dev)))
     return bounds
 
 
@@ -324,48 +318,48 @@ def select_pages(q, bounds, page_table, seq_lens, max_seq_len, top_pages, hq, hk
                  recent_pages=1, q_indptr=None, max_q_len=1, page_size=16, workspace=None, out=None):
     """msgl_select_pages: page ids [total_q, Hkv, top_pages] int32 for query rows q [total_q, Hq, D]
     (rows behind the last request: -1 unless `out` is given)."""
-    _on(torch.bfloat16, q, bounds)
+    dev = _device()
     T = q.numel() // (hq * 128)
-    B = _rows(page_table, seq_lens, q_indptr, max_q_len, T)
+    B, width, indptr = _rows(dev, page_table, seq_lens, q_indptr, max_q_len, T)
     if workspace is None:
         workspace = select_pages_workspace(T, max_seq_len, hkv, q.device)
     if out is None:
         shape = (T, hkv, top_pages)
-        out = (torch.empty(shape, dtype=torch.int32, device=q.device) if q_indptr is None else
-               torch.full(shape, -1, dtype=torch.int32, device=q.device))
-    _on(torch.int32, out)
-    _on(torch.uint8, workspace)
+        out = (torch.empty(shape, dtype=_I32, device=q.device) if q_indptr is None else
+               torch.full(shape, -1, dtype=_I32, device=q.device))
+    _on(dev, _BF, q, bounds)
+    _on(dev, _I32, out)
+    _on(dev, _U8, workspace)
     assert out.numel() == T * hkv * top_pages, "expected out [total_q, Hkv, top_pages]"
-    check(lib().msgl_select_pages(_p(q), _p(bounds), bounds.numel() // (hkv * 256), _p(page_table),
-                                  page_table.shape[1], _p(seq_lens), _p(q_indptr), B, T, max_q_len,
-                                  max_seq_len, hq, hkv, 128, page_size, top_pages, sink_pages,
-                                  recent_pages, _p(out), _p(workspace), workspace.numel(), _s()))
+    check(lib().msgl_select_pages(q.data_ptr(), bounds.data_ptr(), bounds.numel() // (hkv * 256),
+                                  page_table.data_ptr(), width, seq_lens.data_ptr(), indptr, B, T, max_q_len,
+                                  max_seq_len, hq, hkv, 128, page_size, top_pages, sink_pages, recent_pages,
+                                  out.data_ptr(), workspace.data_ptr(), workspace.numel(), _raw_stream(dev)))
     return out
 
 
-def paged_attention_pages(q, k_pool, v_pool, page_table, seq_lens, page_ids, hq, hkv, scale=None,
+_SCALE = 1.0 / (128 ** 0.5)
+
+
+def paged_attention_pages(q, k_pool, v_pool, page_table, seq_lens, page_ids, hq, hkv, scale=_SCALE,
                           q_indptr=None, max_q_len=1, max_seq_len=None, page_size=16, out=None):
     """msgl_paged_attention_pages: attention of q [total_q, Hq, D] over the pages listed in
     page_ids [total_q, Hkv, top_pages] (select_pages, or lists of the caller's)."""
-    _on(torch.bfloat16, q, k_pool, v_pool)
-    _on(torch.int32, page_ids)
-    T = q.numel() // (hq * 128)
-    B = _rows(page_table, seq_lens, q_indptr, max_q_len, T)
-    assert page_ids.dim() == 3 and page_ids.shape[:2] == (T, hkv), "expected page_ids [total_q, Hkv, top]"
-    assert k_pool.numel() == v_pool.numel(), "expected pools of one size"
-    if scale is None:
-        scale = 1.0 / (128 ** 0.5)
-    if max_seq_len is None:
-        max_seq_len = page_table.shape[1] * page_size
+    dev = _device()
+    n = q.numel()
+    B, width, indptr = _rows(dev, page_table, seq_lens, q_indptr, max_q_len, n // (hq * 128))
     if out is None:
         out = torch.empty_like(q) if q_indptr is None else torch.zeros_like(q)
-    _on(torch.bfloat16, out)
-    assert out.numel() == q.numel(), "expected out [total_q, Hq, D]"
-    num_slots = k_pool.numel() // (hkv * 128)
-    check(lib().msgl_paged_attention_pages(_p(q), _p(k_pool), _p(v_pool), num_slots, _p(page_table),
-                                           page_table.shape[1], _p(seq_lens), _p(q_indptr), B, T,
-                                           max_q_len, max_seq_len, _p(page_ids), page_ids.shape[2],
-                                           hq, hkv, 128, page_size, scale, _p(out), _s()))
+    _on(dev, _BF, q, k_pool, v_pool, out)
+    _on(dev, _I32, page_ids)
+    T, heads, top = page_ids.shape
+    slots = k_pool.numel()
+    assert T * hq * 128 == n == out.numel() and heads == hkv, "expected q / out [total_q, Hq, D], page_ids [total_q, Hkv, top]"
+    assert v_pool.numel() == slots, "expected pools of one size"
+    check(lib().msgl_paged_attention_pages(
+        q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), slots // (hkv * 128), page_table.data_ptr(), width,
+        seq_lens.data_ptr(), indptr, B, T, max_q_len, width * page_size if max_seq_len is None else max_seq_len,
+        page_ids.data_ptr(), top, hq, hkv, 128, page_size, scale, out.data_ptr(), _raw_stream(dev)))
     return out
 
 
@@ -375,60 +369,61 @@ def lora_workspace(num_tokens, K, rank, device="cuda"):
     return torch.empty(max(n, 256), dtype=torch.uint8, device=device)
 
 
-def _r(t, dtype):
-    """A 2-D tensor with contiguous rows on the current device: its row stride."""
-    if (t.dim() != 2 or t.dtype != dtype or t.get_device() != torch._C._cuda_getDevice()
-            or (t.shape[1] > 1 and t.stride(1) != 1)):
-        raise ValueError(f"expected {dtype} rows [T, n] on the current device, got {t.dtype} "
+def _row_stride(dev, t, dtype, rows, cols):
+    """The row stride of [rows, cols] values with contiguous rows on the current device."""
+    if (t.dtype is not dtype or t.shape != (rows, cols) or t.get_device() != dev
+            or (cols > 1 and t.stride(1) != 1)):
+        raise ValueError(f"expected {dtype} rows [{rows}, {cols}] on cuda:{dev}, got {t.dtype} "
                          f"{tuple(t.shape)} with strides {t.stride()} on {t.device}")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    return t.stride(0) if rows > 1 else max(t.stride(0), cols)
 
 
-def _lora(x, lora_a, lora_b, scales, adapter_ids, q_indptr, max_q_len, workspace):
-    _on(torch.bfloat16, lora_a, lora_b)
-    _on(torch.float32, scales)
-    _on(torch.int32, adapter_ids)
+def _lora(entry, x, lora_a, lora_b, scales, adapter_ids, base, q_indptr, max_q_len, workspace, out, out_dtype):
+    dev = _device()
     n, R, K = lora_a.shape
-    assert lora_b.shape[0] == n and lora_b.shape[2] == R and scales.numel() == n and x.shape[1] == K, \
-        "expected lora_a [n, rank, K], lora_b [n, N, rank], scales [n], x [T, K]"
-    B = adapter_ids.numel()
+    n_b, N, R_b = lora_b.shape
+    T, B = x.shape[0], adapter_ids.numel()
+    _on(dev, _BF, lora_a, lora_b)
+    _on(dev, _F32, scales)
+    _on(dev, _I32, adapter_ids)
+    assert n == n_b == scales.numel() and R == R_b, "expected lora_a [n, rank, K], lora_b [n, N, rank], scales [n]"
+    indptr = None
     if q_indptr is None:
-        assert max_q_len == 1 and B == x.shape[0], "one row per request without q_indptr"
+        assert max_q_len == 1 and B == T, "one row per request without q_indptr"
     else:
-        _on(torch.int32, q_indptr)
+        _on(dev, _I32, q_indptr)
         assert q_indptr.numel() == B + 1, "expected q_indptr [num_reqs + 1]"
+        indptr = q_indptr.data_ptr()
     if workspace is None:
-        workspace = lora_workspace(x.shape[0], K, R, x.device)
-    _on(torch.uint8, workspace)
-    return (_p(x), _r(x, torch.bfloat16), _p(lora_a), _p(lora_b), _p(scales), n, _p(adapter_ids),
-            _p(q_indptr), B, max_q_len), (x.shape[0], lora_b.shape[1], K, R), workspace
+        workspace = lora_workspace(T, K, R, x.device)
+    _on(dev, _U8, workspace)
+    check(entry(x.data_ptr(), _row_stride(dev, x, _BF, T, K), lora_a.data_ptr(), lora_b.data_ptr(),
+                scales.data_ptr(), n, adapter_ids.data_ptr(), indptr, B, max_q_len,
+                *((base.data_ptr(), _row_stride(dev, base, _BF, T, N)) if base is not None else ()),
+                out.data_ptr(), _row_stride(dev, out, out_dtype, T, N), T, N, K, R, workspace.data_ptr(),
+                workspace.numel(), _raw_stream(dev)))
+    return out
 
 
 def lora_add(x, lora_a, lora_b, scales, adapter_ids, y, q_indptr=None, max_q_len=1, workspace=None,
              out=None):
     """msgl_lora_add: y + scales[a] * (x A[a]^T) B[a]^T, a = adapter_ids[r] of the request that owns
     the row (negative: y as it is). out may be y (in place); rows of x, y, out may be strided."""
-    head, sizes, workspace = _lora(x, lora_a, lora_b, scales, adapter_ids, q_indptr, max_q_len, workspace)
     if out is None:
         out = torch.empty(y.shape, dtype=y.dtype, device=y.device) if q_indptr is None else y.clone()
-    assert y.shape == out.shape == sizes[:2], "expected y / out [T, N]"
-    check(lib().msgl_lora_add(*head, _p(y), _r(y, torch.bfloat16), _p(out), _r(out, torch.bfloat16),
-                              *sizes, _p(workspace), workspace.numel(), _s()))
-    return out
+    return _lora(lib().msgl_lora_add, x, lora_a, lora_b, scales, adapter_ids, y, q_indptr, max_q_len, workspace,
+                 out, _BF)
 
 
 def lora_partial(x, lora_a, lora_b, scales, adapter_ids, q_indptr=None, max_q_len=1, workspace=None,
                  out=None):
     """msgl_lora_partial: fp32 [T, N] scales[a] * (x A[a]^T) B[a]^T, e.g. into the last slab of the
     partials of linear_partials."""
-    head, sizes, workspace = _lora(x, lora_a, lora_b, scales, adapter_ids, q_indptr, max_q_len, workspace)
     if out is None:
         make = torch.empty if q_indptr is None else torch.zeros
-        out = make(sizes[:2], dtype=torch.float32, device=x.device)
-    assert out.shape == sizes[:2], "expected out [T, N]"
-    check(lib().msgl_lora_partial(*head, _p(out), _r(out, torch.float32), *sizes, _p(workspace),
-                                  workspace.numel(), _s()))
-    return out
+        out = make((x.shape[0], lora_b.shape[1]), dtype=_F32, device=x.device)
+    return _lora(lib().msgl_lora_partial, x, lora_a, lora_b, scales, adapter_ids, None, q_indptr, max_q_len,
+                 workspace, out, _F32)
 
 
 # ------------------------------------------------------------------ GEMMs
