@@ -200,3 +200,22 @@ def test_as_one_more_partial_of_a_projection(cuda):
     v = (x.double() @ w.double().T + d)[:, -hkv * 128:]
     size = (x.double().abs() @ w.double().abs().T + mag)[:, -hkv * 128:]
     assert bool(((vp.double() - v).abs() <= v.abs() * 2 ** -8 + size * 2 * steps(K, R)).all())
+
+
+@pytest.mark.parametrize("partial", [False, True])
+@pytest.mark.parametrize("B,n,R", [(300, 2, 16), (300, 7, 40), (260, 200, 8), (33, 1, 128), (129, 40, 64)])
+def test_many_requests_per_adapter(cuda, partial, B, n, R):
+    """Decode batches with fewer adapters than requests: more than 16 rows of one adapter, adapters
+    that nobody uses, rows without one, an id that does not exist."""
+    from msgl import ops
+    K, N = 1000, 776
+    x, a, b, sc, ids, y, _ = make([1] * B, K, N, R, n, seed=B + n)
+    g = torch.Generator("cuda").manual_seed(7)
+    ids.copy_(torch.randint(-1, max(1, n - 1), (B,), generator=g, device="cuda").int())
+    ids[B // 2] = n  # no such adapter: none
+    d, mag = reference(x, a, b, sc, torch.where(ids < n, ids, -1), [1] * B)
+    if partial:
+        check_partial(ops.lora_partial(x, a, b, sc, ids), d, mag, K, R)
+    else:
+        check_add(ops.lora_add(x, a, b, sc, ids, y), y, d, mag, K, R)
+    assert ops.device_error() == (6, 810)
