@@ -17,8 +17,11 @@
 //  * Longer chunks: `shrink` writes h, `expand` reads it. Both take 64 rows of one request a CTA and
 //    bring what several warps share (A, x, B, h) into shared memory.
 //
-// h is fp32: it enters the second product as a sum of bf16 terms (two terms, 2^-17 relative, for
-// the bf16 result; three, 2^-25, for the fp32 partial), so it is not rounded to bf16.
+// h is summed in fp32. For the fp32 partial it enters the second product as three bf16 terms (2^-25
+// relative). For the bf16 result decode takes two (2^-17), where they cost nothing; chunks round it
+// to bf16, as the projections around it round their activations: h's rounding (2^-9 of each of the
+// rank's terms, of either sign) stays below that of the result, and the MMAs of a second term took
+// as long as the streams (rank 64, 4.5k rows: 53 against 50 us).
 #include <algorithm>
 
 #include "common.cuh"
@@ -313,7 +316,7 @@ lora_small_kernel(const LoraArgs a, int num_reqs, int per) {
 // ------------------------------------------------------------------ chunks
 constexpr int kTile = 64;     // rows a CTA
 constexpr int kBK = 64;       // K columns a stage
-constexpr int kShStages = 4;
+constexpr int sh_stages(int kk) { return kk == 8 ? 4 : 6; }  // of 16 or 24 KB: two CTAs per SM
 constexpr int kNSlice = 256;  // columns of an expand CTA
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
@@ -336,7 +339,7 @@ template <int KK>
 __global__ void __launch_bounds__(kLoraWarps * 32)
 lora_shrink_kernel(const LoraArgs a, int terms) {
     constexpr int R16 = 16 * KK;
-    constexpr int kStage = (kTile + R16) * kBK * 2;
+    constexpr int kStage = (kTile + R16) * kBK * 2, kShStages = sh_stages(KK);
     extern __shared__ __align__(128) uint8_t ring[];
     pdl_wait();
     pdl_trigger();
@@ -432,9 +435,9 @@ lora_shrink_kernel(const LoraArgs a, int terms) {
 // tile next to each other) is loaded before the wait for the previous kernel -- it is a weight, and
 // every kernel before `shrink` has completed once `shrink` runs; h comes behind it.
 template <int KK, bool PARTIAL>
-__global__ void __launch_bounds__(kLoraWarps * 32)
+__global__ void __launch_bounds__(kLoraWarps * 32, KK == 8 ? 3 : 4)
 lora_expand_kernel(const LoraArgs a, int n_slices) {
-    constexpr int R16 = 16 * KK, PIECES = 2 * KK, TERMS = PARTIAL ? 3 : 2;
+    constexpr int R16 = 16 * KK, PIECES = 2 * KK, TERMS = PARTIAL ? 3 : 1;
     constexpr int kSwz = KK == 1 ? 2 : KK == 2 ? 1 : 0, kMask = (PIECES < 8 ? PIECES : 8) - 1;
     extern __shared__ __align__(128) uint8_t smem[];
     const uint32_t bs = smem_u32(smem), hs = bs + kNSlice * R16 * 2;
@@ -498,6 +501,21 @@ lora_expand_kernel(const LoraArgs a, int n_slices) {
     cp_async_wait<0>();
     __syncthreads();
     const int mi = lane >> 3, l7 = lane & 7;
+    uint32_t hf[PARTIAL ? 1 : KK][TERMS][2][4];  // all of h where it is one term
+    const auto load_h = [&](int kk, uint32_t (&f)[TERMS][2][4]) {
+#pragma unroll
+        for (int m = 0; m < TERMS; ++m)
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+                const int row = row0 + mt * 16 + (mi & 1) * 8 + l7;
+                ldsm_x4(hs + m * kTile * R16 * 2 + swizzle(row, 2 * kk + (mi >> 1)), f[m][mt][0], f[m][mt][1],
+                        f[m][mt][2], f[m][mt][3]);
+            }
+    };
+    if (!PARTIAL && some) {
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) load_h(kk, hf[PARTIAL ? 0 : kk]);
+    }
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
         if (!PARTIAL && b < 3) load_y(b + 1);
@@ -515,16 +533,15 @@ lora_expand_kernel(const LoraArgs a, int n_slices) {
                     const int row = (blk0 + b) * 32 + (j + (mi >> 1)) * 8 + l7;
                     ldsm_x4(bs + swizzle(row, 2 * kk + (mi & 1)), w[j][0], w[j][1], w[j + 1][0], w[j + 1][1]);
                 }
+                if (PARTIAL) load_h(kk, hf[0]);
+                const auto& f = hf[PARTIAL ? 0 : kk];
 #pragma unroll
                 for (int m = TERMS - 1; m >= 0; --m)
 #pragma unroll
-                    for (int mt = 0; mt < 2; ++mt) {
-                        const int row = row0 + mt * 16 + (mi & 1) * 8 + l7;
-                        uint32_t h0, h1, h2, h3;
-                        ldsm_x4(hs + m * kTile * R16 * 2 + swizzle(row, 2 * kk + (mi >> 1)), h0, h1, h2, h3);
+                    for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) mma_bf16_16816(acc[mt][j], h0, h1, h2, h3, w[j][0], w[j][1]);
-                    }
+                        for (int j = 0; j < 4; ++j)
+                            mma_bf16_16816(acc[mt][j], f[m][mt][0], f[m][mt][1], f[m][mt][2], f[m][mt][3], w[j][0], w[j][1]);
             }
         }
         const int col = n0 + (blk0 + b) * 32 + 8 * c;
@@ -569,13 +586,13 @@ cudaError_t launch_cluster(void (*kernel)(KArgs...), int64_t grid, int size, siz
 template <int KK, bool PARTIAL>
 cudaError_t launch_chunks(const LoraArgs& a, int64_t row_tiles, int splits, cudaStream_t stream) {
     static std::atomic<int> optin[2][kMaxDevices];
-    const size_t sh = size_t(kShStages) * (kTile + 16 * KK) * kBK * 2;
+    const size_t sh = size_t(sh_stages(KK)) * (kTile + 16 * KK) * kBK * 2;
     cudaError_t e = smem_optin(lora_shrink_kernel<KK>, sh, optin[0]);
     if (e != cudaSuccess) return e;
-    const size_t ex = size_t(kNSlice + (PARTIAL ? 3 : 2) * kTile) * 16 * KK * 2;
+    const size_t ex = size_t(kNSlice + (PARTIAL ? 3 : 1) * kTile) * 16 * KK * 2;
     e = smem_optin(lora_expand_kernel<KK, PARTIAL>, ex, optin[1]);
     if (e != cudaSuccess) return e;
-    e = launch_cluster(lora_shrink_kernel<KK>, row_tiles * splits, splits, sh, stream, a, PARTIAL ? 3 : 2);
+    e = launch_cluster(lora_shrink_kernel<KK>, row_tiles * splits, splits, sh, stream, a, PARTIAL ? 3 : 1);
     if (e != cudaSuccess) return e;
     const int n_slices = (a.N + kNSlice - 1) / kNSlice;
     return launch_pdl(lora_expand_kernel<KK, PARTIAL>, dim3(static_cast<unsigned>(row_tiles * n_slices)),

@@ -3,8 +3,10 @@
 Tolerance per element. The two products accumulate in fp32: each MMA step of 16 products rounds or
 truncates its partial sum by at most 2^-22 of the magnitudes it adds, over K / 16 steps, at most 16
 K-range sums, and (three bf16 terms) 3 rank / 16 steps: (K / 16 + 3 rank / 16 + 20) 2^-22 of
-M = |scale| sum_r |B| sum_k |A| |x|. The bf16 result takes h as two bf16 terms (2^-16 of M: 2^-8 of
-a remainder of at most 2^-8) and rounds once (2^-8 of the value).
+M = |scale| sum_r |B| sum_k |A| |x|. The bf16 result rounds once (2^-8 of the value) and takes h, up
+to 16 rows a request, as two bf16 terms (2^-16 of M: 2^-8 of a remainder of at most 2^-8), in longer
+chunks as one: each of the rank's h off by at most 2^-8 of itself, in all 2^-8 of
+H = |scale| sum_r |B| |h_r|.
 """
 import pytest
 import torch
@@ -29,12 +31,15 @@ def make(lens, K, N, R, n, seed=0, none=()):
 def reference(x, a, b, sc, ids, lens):
     d = torch.zeros(x.shape[0], b.shape[1], dtype=torch.float64, device="cuda")
     mag = torch.zeros_like(d)
+    mag.one_term = torch.zeros_like(d)  # H, where h is one bf16 term
     t = 0
     for r, q in zip(ids.tolist(), lens):
         if r >= 0:
             A, B, X = a[r].double(), b[r].double(), x[t:t + q].double()
             d[t:t + q] = sc[r].double() * (X @ A.T) @ B.T
             mag[t:t + q] = sc[r].double() * (X.abs() @ A.abs().T) @ B.abs().T
+            if max(lens) > 16:
+                mag.one_term[t:t + q] = sc[r].double() * (X @ A.T).abs() @ B.abs().T
         t += q
     return d, mag
 
@@ -49,7 +54,7 @@ def check_partial(p, d, mag, K, R):
 
 def check_add(o, y, d, mag, K, R):
     ref = y.double() + d
-    tol = ref.abs() * 2 ** -8 + mag * (steps(K, R) + 2 ** -16) + y.double().abs() * 2 ** -23
+    tol = ref.abs() * 2 ** -8 + mag * (steps(K, R) + 2 ** -16) + mag.one_term * 2 ** -8 + y.double().abs() * 2 ** -23
     assert bool(((o.double() - ref).abs() <= tol).all())
 
 
