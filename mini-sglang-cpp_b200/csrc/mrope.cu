@@ -46,59 +46,80 @@ __device__ __forceinline__ int axis_of_pair(int d, const MropeArgs& a) {
 // Eight lanes per head, four heads per warp: lane i of a head owns elements [8 i, 8 i + 8) of the
 // first half and their rotate-half partners, so loads and stores are 16 bytes (32 for partials)
 // and the sum of squares takes three shuffles. The token's 64 cosines and sines are gathered once
-// per CTA into shared memory, one element per thread. grid (tokens, head splits).
-template <bool PARTS>
+// per CTA into shared memory, one element per thread, behind the loads of the IT groups of heads that
+// a warp takes. grid (tokens, head splits).
+template <bool PARTS, int IT>
 __global__ void __launch_bounds__(kMropeWarps * 32)
 qknorm_mrope_store_kernel(const MropeArgs a) {
     __shared__ __align__(16) float cs[kHd];  // cos 0..63, sin 0..63
     pdl_wait();
     pdl_trigger();
     const int t = blockIdx.x;
-    {
-        const int d = threadIdx.x & (kHalf - 1);
-        int pos = a.positions[axis_of_pair(d, a) * a.pos_stride + t];
-        if (static_cast<unsigned>(pos) >= static_cast<unsigned>(a.max_position)) {
-            record_error(a.err, MSGL_ERR_BOUNDS, 102);
-            pos = 0;
-        }
-        cs[threadIdx.x] = a.table[static_cast<int64_t>(pos) * kHd + threadIdx.x];
-    }
-    __syncthreads();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int i = lane & 7;
     const int nh = a.hq + 2 * a.hkv;
+    const int h0 = (blockIdx.y * IT * kMropeWarps + warp) * 4 + (lane >> 3);  // then every 16th head
+    int pos = a.positions[axis_of_pair(threadIdx.x & (kHalf - 1), a) * a.pos_stride + t];
     const int64_t slot = a.slots[t];
-    if (slot >= a.num_slots && threadIdx.x == 0 && blockIdx.y == 0)
-        record_error(a.err, MSGL_ERR_BOUNDS, 103);
+    uint4 u[PARTS ? 1 : IT][2];
+    if (!PARTS) {
+#pragma unroll
+        for (int n = 0; n < IT; ++n) {
+            const int h = h0 + n * kMropeWarps * 4;
+            const __nv_bfloat16* src = a.qkv + (static_cast<int64_t>(t) * nh + h) * kHd + 8 * i;
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+                u[n][v] = h < nh ? *reinterpret_cast<const uint4*>(src + v * kHalf) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    if (static_cast<unsigned>(pos) >= static_cast<unsigned>(a.max_position)) {
+        record_error(a.err, MSGL_ERR_BOUNDS, 102);
+        pos = 0;
+    }
+    cs[threadIdx.x] = a.table[static_cast<int64_t>(pos) * kHd + threadIdx.x];
+    if (slot >= a.num_slots && threadIdx.x == 0 && blockIdx.y == 0) record_error(a.err, MSGL_ERR_BOUNDS, 103);
     const bool store = slot >= 0 && slot < a.num_slots;
-    for (int h0 = (blockIdx.y * kMropeWarps + warp) * 4; h0 < nh; h0 += gridDim.y * kMropeWarps * 4) {
-        const int h = h0 + (lane >> 3);
+    if (!PARTS) __syncthreads();
+#pragma unroll
+    for (int n = 0; n < IT; ++n) {
+        const int h = h0 + n * kMropeWarps * 4;
         const bool live = h < nh;
         float x[16];  // elements 8 i + e (e < 8) and 64 + 8 i + (e - 8)
+        if (PARTS) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = 0.f;
-        if (live) {
-            const int64_t row = (static_cast<int64_t>(t) * nh + h) * kHd + 8 * i;
-            if (PARTS) {
+            for (int e = 0; e < 16; ++e) x[e] = 0.f;
+            if (live) {
                 const int64_t stride = static_cast<int64_t>(a.num_tokens) * nh * kHd;
-                for (int p = 0; p < a.nparts; ++p) {  // in part order
-                    const float* src = a.parts + p * stride + row;
+                const float* src = a.parts + (static_cast<int64_t>(t) * nh + h) * kHd + 8 * i;
+                int p = 0;
+                for (; p < a.nparts; p += 3) {  // three parts' loads in flight, added in part order
+                    float4 f[3][4];
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        const float4 f = *reinterpret_cast<const float4*>(src + (v >> 1) * kHalf + (v & 1) * 4);
-                        x[4 * v] += f.x; x[4 * v + 1] += f.y; x[4 * v + 2] += f.z; x[4 * v + 3] += f.w;
+                    for (int q = 0; q < 3; ++q)
+#pragma unroll
+                        for (int v = 0; v < 4; ++v)
+                            f[q][v] = p + q < a.nparts ? *reinterpret_cast<const float4*>(src + (p + q) * stride + (v >> 1) * kHalf + (v & 1) * 4)
+                                                       : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int q = 0; q < 3; ++q) {
+                        if (p + q >= a.nparts) break;
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) {
+                            x[4 * v] += f[q][v].x; x[4 * v + 1] += f[q][v].y;
+                            x[4 * v + 2] += f[q][v].z; x[4 * v + 3] += f[q][v].w;
+                        }
                     }
                 }
-            } else {
+            }
+            if (n == 0) __syncthreads();
+        } else {
 #pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    const uint4 u = *reinterpret_cast<const uint4*>(a.qkv + row + v * kHalf);
-                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            for (int v = 0; v < 2; ++v) {
+                const uint32_t w[4] = {u[n][v].x, u[n][v].y, u[n][v].z, u[n][v].w};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[8 * v + 2 * e] = bf16lo(w[e]);
-                        x[8 * v + 2 * e + 1] = bf16hi(w[e]);
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    x[8 * v + 2 * e] = bf16lo(w[e]);
+                    x[8 * v + 2 * e + 1] = bf16hi(w[e]);
                 }
             }
         }
@@ -108,47 +129,42 @@ qknorm_mrope_store_kernel(const MropeArgs a) {
         ss += __shfl_xor_sync(0xffffffffu, ss, 1);
         ss += __shfl_xor_sync(0xffffffffu, ss, 2);
         ss += __shfl_xor_sync(0xffffffffu, ss, 4);
-        if (!live) continue;
-        __nv_bfloat16* dst;
+        __nv_bfloat16* dst = nullptr;
         if (h < a.hq + a.hkv) {
             const float inv = 1.0f / sqrtf(ss / kHd + a.eps);
             const __nv_bfloat16* w = (h < a.hq ? a.qn : a.kn) + 8 * i;
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
-                const uint4 u = *reinterpret_cast<const uint4*>(w + v * kHalf);
-                const uint32_t ww[4] = {u.x, u.y, u.z, u.w};
+                const uint4 uw = *reinterpret_cast<const uint4*>(w + v * kHalf);
+                const uint32_t ww[4] = {uw.x, uw.y, uw.z, uw.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     x[8 * v + 2 * e] *= inv * bf16lo(ww[e]);
                     x[8 * v + 2 * e + 1] *= inv * bf16hi(ww[e]);
                 }
             }
+            float cv[8], sv[8];
+            *reinterpret_cast<float4*>(cv) = *reinterpret_cast<const float4*>(cs + 8 * i);
+            *reinterpret_cast<float4*>(cv + 4) = *reinterpret_cast<const float4*>(cs + 8 * i + 4);
+            *reinterpret_cast<float4*>(sv) = *reinterpret_cast<const float4*>(cs + kHalf + 8 * i);
+            *reinterpret_cast<float4*>(sv + 4) = *reinterpret_cast<const float4*>(cs + kHalf + 8 * i + 4);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float c = cs[8 * i + e], s = cs[kHalf + 8 * i + e];
                 const float lo = x[e], hi = x[8 + e];
-                x[e] = lo * c - hi * s;
-                x[8 + e] = lo * s + hi * c;
+                x[e] = lo * cv[e] - hi * sv[e];
+                x[8 + e] = lo * sv[e] + hi * cv[e];
             }
-            if (h < a.hq) {
-                dst = a.q_out + (static_cast<int64_t>(t) * a.hq + h) * kHd;
-            } else {
-                if (!store) continue;
-                dst = a.k_pool + (slot * a.hkv + (h - a.hq)) * kHd;
-            }
-        } else {
-            if (!store) continue;
+            if (h < a.hq) dst = a.q_out + (static_cast<int64_t>(t) * a.hq + h) * kHd;
+            else if (store) dst = a.k_pool + (slot * a.hkv + (h - a.hq)) * kHd;
+        } else if (live && store) {
             dst = a.v_pool + (slot * a.hkv + (h - a.hq - a.hkv)) * kHd;
         }
+        if (!dst) continue;
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-            uint4 u;
-            u.x = pack_bf16x2(x[8 * v], x[8 * v + 1]);
-            u.y = pack_bf16x2(x[8 * v + 2], x[8 * v + 3]);
-            u.z = pack_bf16x2(x[8 * v + 4], x[8 * v + 5]);
-            u.w = pack_bf16x2(x[8 * v + 6], x[8 * v + 7]);
-            *reinterpret_cast<uint4*>(dst + v * kHalf + 8 * i) = u;
-        }
+        for (int v = 0; v < 2; ++v)
+            *reinterpret_cast<uint4*>(dst + v * kHalf + 8 * i) =
+                make_uint4(pack_bf16x2(x[8 * v], x[8 * v + 1]), pack_bf16x2(x[8 * v + 2], x[8 * v + 3]),
+                           pack_bf16x2(x[8 * v + 4], x[8 * v + 5]), pack_bf16x2(x[8 * v + 6], x[8 * v + 7]));
     }
 }
 
@@ -178,9 +194,13 @@ int launch_mrope(MropeArgs a, const int* sections, int layout, int head_dim, msg
     a.err = device_error_word();
     if (!a.err) return set_error(MSGL_ERR_CUDA, "device error word unavailable");
     const int nh = a.hq + 2 * a.hkv;
-    const int splits = (nh + 4 * kMropeWarps - 1) / (4 * kMropeWarps);
+    // Many tokens: three groups of heads a warp, so that a thread has 96 bytes in flight and the
+    // table is gathered once for 48 heads; few: one, for more CTAs.
+    const int it = !a.parts && a.num_tokens >= 8 * 148 ? 3 : 1;
+    const int splits = (nh + 4 * kMropeWarps * it - 1) / (4 * kMropeWarps * it);
     if (splits > 65535) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "qknorm_mrope: too many heads");
-    launch_pdl(a.parts ? qknorm_mrope_store_kernel<true> : qknorm_mrope_store_kernel<false>,
+    launch_pdl(a.parts ? qknorm_mrope_store_kernel<true, 1>
+                       : it == 3 ? qknorm_mrope_store_kernel<false, 3> : qknorm_mrope_store_kernel<false, 1>,
                dim3(a.num_tokens, splits), dim3(kMropeWarps * 32), 0, stream, a);
     MSGL_LAUNCH_CHECK();
     return MSGL_OK;

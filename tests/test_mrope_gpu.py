@@ -67,7 +67,7 @@ def check(got, ref, mag):
     assert bool((err <= ref.abs() * 2 ** -8 + mag * 2 ** -17).all()), float((err / mag).max())
 
 
-@pytest.mark.parametrize("T,hq,hkv", [(1, 16, 8), (5, 8, 1), (37, 32, 8), (300, 32, 4), (3, 5, 3)])
+@pytest.mark.parametrize("T,hq,hkv", [(1, 16, 8), (5, 8, 1), (37, 32, 8), (300, 32, 4), (3, 5, 3), (1300, 9, 4)])
 @pytest.mark.parametrize("sections,interleaved", [((24, 20, 20), True), ((16, 24, 24), False),
                                                   ((64, 0, 0), True), ((0, 0, 64), False),
                                                   ((22, 21, 21), True), ((1, 62, 1), False)])
