@@ -47,6 +47,15 @@ __device__ __forceinline__ Window request_window(int r, const int* seq_lens, con
     return w;
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // ------------------------------------------------------------------ bounds
 constexpr int kBoundWarps = 8;
 
@@ -121,7 +130,7 @@ page_bounds_kernel(const __nv_bfloat16* __restrict__ k_pool, int pool_pages,
 }
 
 // ------------------------------------------------------------------ scores
-// Scores of 64 pages (16 a warp) for a tile of one request's query rows. The bounds of 16 pages
+// Scores of `groups` x 64 pages (16 a warp and group) for a tile of one request's query rows. The bounds of 16 pages
 // are the A operand (16 x 256: lo then hi) and stay in registers; the B operand is (min(q, 0),
 // max(q, 0)) of 8 columns = 8 / G tokens x G query heads. Both are loaded straight from global
 // memory as 16-byte pieces: lane (g, c) takes elements 32 i + 8 c .. + 7 of row g, which fixes one
@@ -153,118 +162,156 @@ struct SelectArgs {
     int* err;
 };
 
-template <int G>
-__global__ void __launch_bounds__(kScoreWarps * 32)
-page_scores_kernel(const SelectArgs a, int tile_rows, int tiles, int page_tiles) {
+// Single tokens take `groups` groups of pages one after the other, the next group's page ids loaded
+// ahead, and go through a page's heads first: their bounds are neighbours in memory (64 requests at
+// 4k to 32k: 72 -> 64 us). Chunks take one group for a tile of kScoreCols columns (query rows x G),
+// whose queries lie in shared memory: the loop over them waited for L1 before (PLACEHOLDER).
+constexpr int kScoreCols = 128;
+constexpr int kScorePitch = kHd * 2 + 64;  // bytes a query: two rows of a quarter-warp in other banks
+
+template <int G, bool CHUNK>
+__global__ void __launch_bounds__(kScoreWarps * 32, 4)
+page_scores_kernel(const SelectArgs a, int tiles, int page_tiles, int groups) {
+    constexpr int kRows = CHUNK ? kScoreCols / G : 1;  // query rows of a tile
+    constexpr int TPN = 8 / G;                         // query rows of an 8-column MMA tile
+    __shared__ __align__(16) uint8_t sq[CHUNK ? kScoreCols * kScorePitch : 16];
     pdl_wait();
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     int64_t id = blockIdx.x;
-    const int pt = static_cast<int>(id % page_tiles);
-    id /= page_tiles;
-    const int h = static_cast<int>(id % a.hkv);
-    id /= a.hkv;
+    const int inner = CHUNK ? page_tiles : a.hkv, outer = CHUNK ? a.hkv : page_tiles;
+    const int x = static_cast<int>(id % inner);
+    id /= inner;
+    const int y = static_cast<int>(id % outer);
+    id /= outer;
+    const int h = CHUNK ? y : x, pt = CHUNK ? x : y;
     const int tile = static_cast<int>(id % tiles), r = static_cast<int>(id / tiles);
     const bool report = pt == 0 && h == 0 && tile == 0 && threadIdx.x == 0;
     const Window w = request_window(r, a.seq_lens, a.q_indptr, a.max_len, report, a.err);
     if (report && (w.qn > a.max_q_len || w.qn < 0 || w.q0 < 0 || w.q0 + static_cast<int64_t>(w.qn) > a.total_q))
         record_error(a.err, MSGL_ERR_BOUNDS, 801);
     const int first = max(w.q0, a.t0);  // the request's first row of this launch: holds its mags
-    const int i0 = max(tile * tile_rows, first - w.q0);
-    const int i1 = min(min(w.qn, a.max_q_len), min((tile + 1) * tile_rows, a.t1 - w.q0));
+    const int i0 = max(tile * kRows, first - w.q0);
+    const int i1 = min(min(w.qn, a.max_q_len), min((tile + 1) * kRows, a.t1 - w.q0));
     if (w.q0 < 0 || i0 >= i1) return;
     const int seen = (w.L - w.qn + i1 - 1) >> 4;  // pages before the last row's own page
     const int last = seen + 1 - a.recent;         // pages [sink, last) are scored
     if (seen + 1 <= a.top) return;                // every row of the tile sees all its pages
-    const int pg0 = pt * kScorePages + warp * 16;
-    if (pg0 >= last || pg0 + 16 <= a.sink) return;
+    const int end = min(last, (pt + 1) * groups * kScorePages);
+    int pg0 = pt * groups * kScorePages;
+    if (pg0 >= end || (pt + 1) * groups * kScorePages <= a.sink) return;  // the whole CTA
+    const __nv_bfloat16* q0 = a.q + (static_cast<int64_t>(w.q0 + i0) * a.hq + h * G) * kHd;
+    if (CHUNK) {
+        for (int p = threadIdx.x; p < (i1 - i0) * G * 16; p += kScoreWarps * 32) {
+            const int col = p >> 4, piece = p & 15;
+            cp_async16(smem_u32(sq + col * kScorePitch + piece * 16),
+                       q0 + (static_cast<int64_t>(col / G) * a.hq + col % G) * kHd + piece * 8, true);
+        }
+        cp_async_commit();
+    }
+    pg0 += warp * 16;
+    if (!CHUNK) {
+        pg0 += max(0, (a.sink - pg0) / kScorePages) * kScorePages;  // groups of forced pages only
+        if (pg0 >= end) return;
+    }
 
-    uint32_t af[8][2][4];
+    const int* table = a.page_table + static_cast<int64_t>(r) * a.max_pages;
+    int next[2];  // physical pages of the next group
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int page = pg0 + g + 8 * u;
-        int phys = -1;
-        if (page < last) {
-            phys = a.page_table[static_cast<int64_t>(r) * a.max_pages + page];
-            if (static_cast<unsigned>(phys) >= static_cast<unsigned>(a.pool_pages)) {
+    for (int u = 0; u < 2; ++u) next[u] = pg0 + g + 8 * u < last ? table[pg0 + g + 8 * u] : -1;
+    do {
+        uint32_t af[8][2][4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            int phys = next[u];
+            if (pg0 + g + 8 * u < last && static_cast<unsigned>(phys) >= static_cast<unsigned>(a.pool_pages)) {
                 record_error(a.err, MSGL_ERR_BOUNDS, 802);
                 phys = -1;
             }
+            const __nv_bfloat16* src = a.bounds + (static_cast<int64_t>(max(phys, 0)) * a.hkv + h) * 2 * kHd + 8 * c;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (phys >= 0) v = *reinterpret_cast<const uint4*>(src + 32 * i);
+                af[i][u][0] = v.x; af[i][u][1] = v.y; af[i][u][2] = v.z; af[i][u][3] = v.w;
+            }
         }
-        const __nv_bfloat16* src = a.bounds + (static_cast<int64_t>(max(phys, 0)) * a.hkv + h) * 2 * kHd + 8 * c;
+        if (!CHUNK) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (phys >= 0) v = *reinterpret_cast<const uint4*>(src + 32 * i);
-            af[i][u][0] = v.x; af[i][u][1] = v.y; af[i][u][2] = v.z; af[i][u][3] = v.w;
+            for (int u = 0; u < 2; ++u) {
+                const int page = pg0 + kScorePages + g + 8 * u;
+                next[u] = page < end ? table[page] : -1;
+            }
         }
-    }
-    {   // largest 2-norm of max(|lo|, |hi|) among the 16 pages: what the scores' error scales with
-        float m[2];
+        {   // largest 2-norm of max(|lo|, |hi|) among the 16 pages: what the scores' error scales with
+            float m[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            m[u] = 0.f;
+            for (int u = 0; u < 2; ++u) {
+                m[u] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t x = max_nan2(abs2(af[i][u][e]), abs2(af[4 + i][u][e]));
-                    m[u] += bf16lo(x) * bf16lo(x) + bf16hi(x) * bf16hi(x);
-                }
-            m[u] += __shfl_xor_sync(0xffffffffu, m[u], 1);
-            m[u] += __shfl_xor_sync(0xffffffffu, m[u], 2);
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t v = max_nan2(abs2(af[i][u][e]), abs2(af[4 + i][u][e]));
+                        m[u] += bf16lo(v) * bf16lo(v) + bf16hi(v) * bf16hi(v);
+                    }
+                m[u] += __shfl_xor_sync(0xffffffffu, m[u], 1);
+                m[u] += __shfl_xor_sync(0xffffffffu, m[u], 2);
+            }
+            const float most = sqrtf(warp_max(fmaxf(m[0], m[1])));
+            if (lane == 0 && pg0 < end)
+                a.mags[(static_cast<int64_t>(first - a.t0) * a.hkv + h) * (a.stride / 16) + pg0 / 16] = most;
         }
-        const float most = sqrtf(warp_max(fmaxf(m[0], m[1])));
-        if (lane == 0)
-            a.mags[(static_cast<int64_t>(first - a.t0) * a.hkv + h) * (a.stride / 16) + pg0 / 16] = most;
-    }
+        if (CHUNK) {
+            cp_async_wait<0>();
+            __syncthreads();
+            if (pg0 >= end) return;
+        }
 
-    constexpr int TPN = 8 / G;  // tokens per 8-column tile
-    for (int i = i0; i < i1; i += TPN) {
-        const int tok = i + g / G, head = g % G;
-        const bool live = tok < i1;
-        const __nv_bfloat16* qr =
-            a.q + (static_cast<int64_t>(w.q0 + tok) * a.hq + h * G + head) * kHd + 8 * c;
-        uint32_t qf[4][4];
+        // lane (g, c) stores page g (+ 8) of row i + 2 c / G (of columns 2 c and 2 c + 1 where G = 1)
+        const int tt = 2 * c / G;
+        const bool mine[2] = {(2 * c) % G == 0 && pg0 + g < last, (2 * c) % G == 0 && pg0 + g + 8 < last};
+        const int64_t pitch = static_cast<int64_t>(a.hkv) * a.stride;
+        float* out = a.scores + (w.q0 + i0 + tt - a.t0) * pitch + static_cast<int64_t>(h) * a.stride + pg0 + g;
+        for (int i = 0; i < i1 - i0; i += TPN, out += TPN * pitch) {
+            uint32_t qf[4][4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (live) v = *reinterpret_cast<const uint4*>(qr + 32 * k);
-            qf[k][0] = v.x; qf[k][1] = v.y; qf[k][2] = v.z; qf[k][3] = v.w;
-        }
-        float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const uint32_t n0 = min_nan2(qf[k][2 * s], 0u), n1 = min_nan2(qf[k][2 * s + 1], 0u);
-                const uint32_t p0 = max_nan2(qf[k][2 * s], 0u), p1 = max_nan2(qf[k][2 * s + 1], 0u);
-                mma_bf16_16816(d0, af[k][0][2 * s], af[k][1][2 * s], af[k][0][2 * s + 1],
-                               af[k][1][2 * s + 1], n0, n1);
-                mma_bf16_16816(d1, af[4 + k][0][2 * s], af[4 + k][1][2 * s], af[4 + k][0][2 * s + 1],
-                               af[4 + k][1][2 * s + 1], p0, p1);
+            for (int k = 0; k < 4; ++k) {
+                uint4 v = make_uint4(0, 0, 0, 0);
+                const int col = i * G + g;
+                if (col < (i1 - i0) * G)
+                    v = CHUNK ? *reinterpret_cast<const uint4*>(sq + col * kScorePitch + 16 * c + 64 * k)
+                              : *reinterpret_cast<const uint4*>(q0 + col * kHd + 8 * c + 32 * k);
+                qf[k][0] = v.x; qf[k][1] = v.y; qf[k][2] = v.z; qf[k][3] = v.w;
             }
+            float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int page = pg0 + g + 8 * u;
-            const float v0 = d0[2 * u] + d1[2 * u], v1 = d0[2 * u + 1] + d1[2 * u + 1];
-            if (G == 1) {
+            for (int k = 0; k < 4; ++k)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int tt = i + 2 * c + e;
-                    if (tt < i1 && page < last)
-                        a.scores[(static_cast<int64_t>(w.q0 + tt - a.t0) * a.hkv + h) * a.stride + page] = e ? v1 : v0;
+                for (int s = 0; s < 2; ++s) {
+                    const uint32_t n0 = min_nan2(qf[k][2 * s], 0u), n1 = min_nan2(qf[k][2 * s + 1], 0u);
+                    const uint32_t p0 = max_nan2(qf[k][2 * s], 0u), p1 = max_nan2(qf[k][2 * s + 1], 0u);
+                    mma_bf16_16816(d0, af[k][0][2 * s], af[k][1][2 * s], af[k][0][2 * s + 1],
+                                   af[k][1][2 * s + 1], n0, n1);
+                    mma_bf16_16816(d1, af[4 + k][0][2 * s], af[4 + k][1][2 * s], af[4 + k][0][2 * s + 1],
+                                   af[4 + k][1][2 * s + 1], p0, p1);
                 }
-            } else {
-                float m = max_nan(v0, v1);
-                if (G >= 4) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                if (G >= 8) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                const int tt = i + 2 * c / G;
-                if ((2 * c) % G == 0 && tt < i1 && page < last)
-                    a.scores[(static_cast<int64_t>(w.q0 + tt - a.t0) * a.hkv + h) * a.stride + page] = m;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const float v0 = d0[2 * u] + d1[2 * u], v1 = d0[2 * u + 1] + d1[2 * u + 1];
+                if (G == 1) {
+                    if (mine[u] && i + tt < i1 - i0) out[8 * u] = v0;
+                    if (mine[u] && i + tt + 1 < i1 - i0) out[pitch + 8 * u] = v1;
+                } else {
+                    float m = max_nan(v0, v1);
+                    if (G >= 4) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                    if (G >= 8) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                    if (mine[u] && i + tt < i1 - i0) out[8 * u] = m;
+                }
             }
         }
-    }
+        pg0 += kScorePages;
+    } while (!CHUNK && pg0 < end);
 }
 
 // ------------------------------------------------------------------ selection
@@ -748,15 +795,6 @@ struct AttArgs {
     __nv_bfloat16* out;
     int* err;
 };
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 
 // Running state of a warp's online softmax. Lane (g, c) holds dims 16 j + g (+ 8) of columns 2 c and
 // 2 c + 1, the columns' maxima and this lane's part of their sums.
@@ -1435,12 +1473,24 @@ int msgl_select_pages(const void* q, const void* bounds, int64_t num_pages, cons
     a.mags = a.scores + int64_t(slab) * num_kv_heads * a.stride;
 
     const int G = num_q_heads / num_kv_heads;
-    const auto score = G == 1 ? page_scores_kernel<1> : G == 2 ? page_scores_kernel<2>
-                       : G == 4 ? page_scores_kernel<4> : page_scores_kernel<8>;
-    const int tile_rows = max_q_len == 1 ? 1 : 64;
+    const bool chunk = max_q_len > 1;
+    using Score = void (*)(SelectArgs, int, int, int);
+    const Score score = chunk ? (G == 1   ? Score(page_scores_kernel<1, true>)
+                                 : G == 2 ? Score(page_scores_kernel<2, true>)
+                                 : G == 4 ? Score(page_scores_kernel<4, true>) : Score(page_scores_kernel<8, true>))
+                              : (G == 1   ? Score(page_scores_kernel<1, false>)
+                                 : G == 2 ? Score(page_scores_kernel<2, false>)
+                                 : G == 4 ? Score(page_scores_kernel<4, false>) : Score(page_scores_kernel<8, false>));
+    const int tile_rows = chunk ? kScoreCols / G : 1;
     const int tiles = (max_q_len + tile_rows - 1) / tile_rows;
-    const int page_tiles = (pages_of(max_seq_len) + kScorePages - 1) / kScorePages;
-    const int64_t blocks = int64_t(num_reqs) * tiles * num_kv_heads * page_tiles;
+    // Single tokens: a few groups of pages a warp, whose page ids are loaded a group ahead, as long as
+    // some eight CTAs per SM are left.
+    const int64_t heads = int64_t(num_reqs) * tiles * num_kv_heads;
+    const int all_groups = (pages_of(max_seq_len) + kScorePages - 1) / kScorePages;
+    int groups = 1;
+    while (!chunk && groups < 8 && heads * all_groups >= 16 * 148 * groups) groups *= 2;
+    const int page_tiles = (all_groups + groups - 1) / groups;
+    const int64_t blocks = heads * page_tiles;
     const int64_t sel_blocks = int64_t(slab) * num_kv_heads;
     if (blocks > INT32_MAX || sel_blocks > INT32_MAX)
         return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "select_pages: batch too large");
@@ -1462,7 +1512,7 @@ int msgl_select_pages(const void* q, const void* bounds, int64_t num_pages, cons
         a.t1 = std::min(total_q, t0 + slab);
         if (page_tiles > 0 && pages_of(max_seq_len) > top_pages) {
             launch_pdl(score, dim3(static_cast<unsigned>(blocks)), dim3(kScoreWarps * 32), 0, stream, a,
-                       tile_rows, tiles, page_tiles);
+                       tiles, page_tiles, groups);
             MSGL_LAUNCH_CHECK();
         }
         const int n = (a.t1 - t0) * num_kv_heads;
