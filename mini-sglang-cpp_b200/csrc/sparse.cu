@@ -1124,7 +1124,13 @@ attend_pages_decode_kernel(const AttArgs a, int words) {
 // its own rows asked for, one in 16 / RW of them. Pages come by TMA (one 3-D box of K, one of V)
 // through a ring shared by the warps, in stages of kStagePages: most warps skip most pages, and a
 // barrier per page cost as much as the pages. Contexts longer than kWin pages are walked in windows
-// of that many.
+// of that many. A cluster of CTAs (chunk_split) shares a tile: each takes a share of every window's
+// list, and the partial results are joined through distributed shared memory.
+//
+// Bound by the TMA boxes: without the products the loads alone take 260 of 450 us (1.3k rows of 32
+// heads over 64 pages each, 126k page loads of 8 KB). Slower ways to bring the same pages: cp.async
+// from producer warps 575 us (it shares the path of the fragment loads), bulk copies of single rows
+// 1315 us, tiles of 16 rows on two CTAs per SM 565 us.
 //
 // A masked weight is zero, but zero times a NaN or infinite value is NaN. Such values are looked
 // for at the end instead of at every page: a row they reached is NaN from then on, so a tile
@@ -1166,17 +1172,18 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
     const int G = a.hq / a.hkv;
     const int TQ = 8 / G;
     const int RW = row_groups, PW = kChWarps / RW, rg = warp % RW, pg = warp / RW;
-    int64_t id = blockIdx.x;
+    const int CS = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
+    int64_t id = static_cast<int>(blockIdx.x) / CS;
     const int h = static_cast<int>(id % a.hkv);
     id /= a.hkv;
     const int tile = static_cast<int>(id % tiles), r = static_cast<int>(id / tiles);
-    const bool report = tile == 0 && h == 0 && threadIdx.x == 0;
+    const bool report = tile == 0 && h == 0 && rank == 0 && threadIdx.x == 0;
     const Window w = request_window(r, a.seq_lens, a.q_indptr, a.max_len, report, a.err);
     const bool fits = w.q0 >= 0 && w.qn >= 0 && w.qn <= a.max_q_len && w.q0 + static_cast<int64_t>(w.qn) <= a.total_q;
     if (report && !fits) record_error(a.err, MSGL_ERR_BOUNDS, 801);
     const int i0 = tile * RW * TQ;
     const int rows = min(RW * TQ, w.qn - i0);
-    if (!fits || rows <= 0) return;
+    if (!fits || rows <= 0) return;  // the whole cluster
     const int pos0 = w.L - w.qn + i0;  // position of the tile's first row
 
     const int wrow = rg * TQ, wrows = max(0, min(TQ, rows - wrow));  // this warp's rows (may be none)
@@ -1209,7 +1216,7 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
                 if (page < 0) continue;
                 const int pos = pos0 + row;
                 if (pos < 0 || page > pos / kPage) {
-                    if (w0 == 0 && !careful) record_error(a.err, MSGL_ERR_BOUNDS, 803);
+                    if (w0 == 0 && !careful && rank == 0) record_error(a.err, MSGL_ERR_BOUNDS, 803);
                     continue;
                 }
                 if (page >= w0 && page < w0 + kWin) atomicOr(&masks[page - w0], 1ull << row);
@@ -1220,19 +1227,25 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
             int per = 0;
             if (warp < kChWarps)
                 for (int i = 0; i < kRun; ++i) per += masks[run0 + i] != 0;
-            int count;
-            int at = block_excl_scan(per, scan, count);
+            int total;
+            int at = block_excl_scan(per, scan, total);
+            const int lo = total * rank / CS, count = total * (rank + 1) / CS - lo;  // this CTA's share
+            at -= lo;
             if (per)
                 for (int i = 0; i < kRun; ++i) {
                     if (!masks[run0 + i]) continue;
-                    int phys = a.page_table[static_cast<int64_t>(r) * a.max_pages + w0 + run0 + i];
-                    if (static_cast<unsigned>(phys) >= static_cast<unsigned>(a.pool_pages)) {
-                        record_error(a.err, MSGL_ERR_BOUNDS, 802);
-                        phys = 0;
-                    }
-                    list_phys[at] = phys;
-                    list_page[at++] = static_cast<uint16_t>(run0 + i);
+                    if (at >= 0 && at < count) list_page[at] = static_cast<uint16_t>(run0 + i);
+                    ++at;
                 }
+            __syncthreads();
+            for (int i = threadIdx.x; i < count; i += kChThreads) {  // all in flight together
+                int phys = a.page_table[static_cast<int64_t>(r) * a.max_pages + w0 + list_page[i]];
+                if (static_cast<unsigned>(phys) >= static_cast<unsigned>(a.pool_pages)) {
+                    record_error(a.err, MSGL_ERR_BOUNDS, 802);
+                    phys = 0;
+                }
+                list_phys[i] = phys;
+            }
             __syncthreads();
 
             const int stages = (count + kStagePages - 1) / kStagePages;
@@ -1295,22 +1308,40 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
         float sum = 0.f;  // NaN where a sum is infinite or NaN
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum += 0.f * ((st.o[j][0] + st.o[j][1]) + (st.o[j][2] + st.o[j][3]));
-        if (!__syncthreads_or(sum != sum)) break;
+        if (!__syncthreads_or(sum != sum)) break;  // each CTA for itself
     }
 
-    // ---- join the page groups, normalise, store
+    // ---- join the page groups and the cluster's shares, normalise, store
     float* mo = reinterpret_cast<float*>(ring);  // [16 warps][8][kPad]
     if (warp < kChWarps) dump(st, mo + warp * 8 * kPad, sm + warp * 8, sl + warp * 8, lane);
-    __syncthreads();
-    for (int item = threadIdx.x; item < rows * G * 16; item += kChThreads) {
+    __syncwarp();
+    cluster_sync_all();
+    for (int item = rank * kChThreads + threadIdx.x; item < rows * G * 16; item += CS * kChThreads) {
         const int tr = (item >> 4) / G, head = (item >> 4) % G, d0 = (item & 15) * 8;
         const int col = tr / TQ * 8 + tr % TQ * G + head;  // in the first page group
-        float M, L, acc[8];
-        join(mo + col * kPad + d0, sm + col, sl + col, PW, RW * 8, M, L, acc);
+        float M = kNegInf, L = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int p = 0; p < PW; ++p)
+            for (int k = 0; k < CS; ++k)
+                M = fmaxf(M, ld_dsmem_f32(mapa_shared(smem_u32(sm + col + p * RW * 8), k)));
+        for (int p = 0; p < PW; ++p)
+            for (int k = 0; k < CS; ++k) {
+                const int at = col + p * RW * 8;
+                const float mk = ld_dsmem_f32(mapa_shared(smem_u32(sm + at), k));
+                const float lk = ld_dsmem_f32(mapa_shared(smem_u32(sl + at), k));
+                const uint32_t src = mapa_shared(smem_u32(mo + at * kPad + d0), k);
+                const float4 u = ld_dsmem_v4(src), v = ld_dsmem_v4(src + 16);
+                if (mk == kNegInf && lk == 0.f) continue;  // saw no key
+                const float sc = exp2f(mk - M);
+                L += lk * sc;
+                acc[0] += u.x * sc; acc[1] += u.y * sc; acc[2] += u.z * sc; acc[3] += u.w * sc;
+                acc[4] += v.x * sc; acc[5] += v.y * sc; acc[6] += v.z * sc; acc[7] += v.w * sc;
+            }
         // an empty list gives a zero row
         *reinterpret_cast<uint4*>(a.out + (static_cast<int64_t>(w.q0 + i0 + tr) * a.hq + h * G + head) * kHd + d0) =
             pack8(acc, L == 0.f ? 0.f : 1.f / L);
     }
+    __syncwarp();
+    cluster_sync_all();  // no CTA leaves while another reads its shared memory
 }
 
 // ------------------------------------------------------------------ host checks
@@ -1343,6 +1374,20 @@ int decode_split(int64_t lists, int top) {
     return s;
 }
 
+// CTAs that share a tile of a chunk (up to 4): one SM holds one, and the rounds of 148 should be full.
+// A share costs a list and a join of its own, so it has to gain a sixth: 16 tiles take 159 us alone,
+// 69 in fours; 64 tiles 85 and 61 in twos; 256 tiles 148 and 182 in twos.
+int chunk_split(int64_t tiles) {
+    const auto fill = [&](int s) {
+        const int64_t ctas = tiles * s, rounds = (ctas + 147) / 148;
+        return static_cast<double>(ctas) / (148 * rounds);
+    };
+    int best = 1;
+    for (int s = 2; s <= 4; s *= 2)
+        if (fill(s) > 1.17 * fill(best)) best = s;
+    return best;
+}
+
 // Opts the decode kernel in to clusters above the portable size, once per device.
 cudaError_t large_clusters() {
     static std::atomic<bool> done[kMaxDevices];
@@ -1358,11 +1403,11 @@ cudaError_t large_clusters() {
 
 // launch_pdl with a thread-block cluster of `size` CTAs.
 template <typename... KArgs, typename... Args>
-cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, int size, size_t smem, cudaStream_t stream,
+cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, int threads, int size, size_t smem, cudaStream_t stream,
                            Args&&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kAttThreads);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -1576,12 +1621,16 @@ int msgl_paged_attention_pages(const void* q, const void* k_pool, const void* v_
         while (row_groups < kChWarps && row_groups * tq < std::min(max_q_len, kTileRows)) row_groups *= 2;
         const int tiles = (max_q_len + row_groups * tq - 1) / (row_groups * tq);
         const int64_t blocks = int64_t(num_reqs) * tiles * num_kv_heads;
-        if (blocks > INT32_MAX) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "attention_pages: batch too large");
+        // tiles that hold rows: every request ends with a part of one
+        const int64_t held = (total_q / (row_groups * tq) + (num_reqs + 1) / 2) * num_kv_heads;
+        const int split = chunk_split(std::min(blocks, std::max<int64_t>(1, held)));
+        if (blocks * split > INT32_MAX) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "attention_pages: batch too large");
         static std::atomic<int> optin[kMaxDevices];
         cudaError_t e = smem_optin(attend_pages_chunk_kernel, kChSmem, optin);
+        if (e == cudaSuccess)
+            e = launch_cluster(attend_pages_chunk_kernel, static_cast<unsigned>(blocks * split), kChThreads, split,
+                               kChSmem, stream, tk, tv, a, tiles, row_groups);
         if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
-        launch_pdl(attend_pages_chunk_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kChThreads), kChSmem, stream,
-                   tk, tv, a, tiles, row_groups);
         MSGL_LAUNCH_CHECK();
         return MSGL_OK;
     }
@@ -1594,7 +1643,7 @@ int msgl_paged_attention_pages(const void* q, const void* k_pool, const void* v_
     cudaError_t e = smem_optin(attend_pages_decode_kernel, smem, optin);
     if (e == cudaSuccess && split > 8) e = large_clusters();
     if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
-    e = launch_cluster(attend_pages_decode_kernel, static_cast<unsigned>(lists * split), split, smem, stream, a, words);
+    e = launch_cluster(attend_pages_decode_kernel, static_cast<unsigned>(lists * split), kAttThreads, split, smem, stream, a, words);
     if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
     MSGL_LAUNCH_CHECK();
     return MSGL_OK;
