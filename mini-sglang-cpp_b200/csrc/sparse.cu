@@ -954,17 +954,22 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8], float f) {
                       pack_bf16x2(v[4] * f, v[5] * f), pack_bf16x2(v[6] * f, v[7] * f));
 }
 
-// ---- single tokens
+// ---- single rows: decode, and short chunks
+// Lists attended one by one, also in chunks whose tiles would be half empty or too few (kRowsAlone
+// rows a request, kTotalAlone rows in all): selection and attention of 8 requests x 5 / 33 / 65 rows (32
+// heads, 64 of 512 pages) take 34 / 119 / 213 us this way and 61 / 150 / 197 in tiles, of 1 x 129 / 513
+// rows 85 / 245 and 114 / 193.
 // A cluster of up to 16 CTAs (decode_split) per (query row, kv head): each CTA
 // takes a share of the listed pages, its four warps take its pages in turn, every warp with a ring
 // of its own (cp.async, 16 bytes a lane, three pages) and an online softmax. The warps' results are
 // joined in shared memory, the CTAs' through distributed shared memory, each CTA finishing a share
 // of the output: no workspace, one launch, a fixed order.
+constexpr int kRowsAlone = 32, kTotalAlone = 256;
 constexpr int kDecStages = 3;
 constexpr int kDecRing = kAttWarps * kDecStages * kPageBytes;
 
 __global__ void __launch_bounds__(kAttThreads, 2)
-attend_pages_decode_kernel(const AttArgs a, int words) {
+attend_pages_decode_kernel(const AttArgs a, int num_reqs, int words) {
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* ring = smem;                                           // kDecRing
     uint32_t* bits = reinterpret_cast<uint32_t*>(smem + kDecRing);  // [words]
@@ -972,6 +977,7 @@ attend_pages_decode_kernel(const AttArgs a, int words) {
     int* list_page = list_phys + a.top;                             // [top]
     __shared__ int scan[32];
     __shared__ float cm[8], cl[8];  // joined maximum and sum per query head
+    __shared__ int owner;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int S = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
@@ -979,15 +985,25 @@ attend_pages_decode_kernel(const AttArgs a, int words) {
     pdl_wait();
     pdl_trigger();
     const int id = static_cast<int>(blockIdx.x) / S;
-    const int h = id % a.hkv, r = id / a.hkv;
+    const int h = id % a.hkv, t = id / a.hkv;
     const int G = a.hq / a.hkv;
+    int r = t;
+    if (a.q_indptr) {  // the request that owns row t
+        if (threadIdx.x == 0) owner = -1;
+        __syncthreads();
+        for (int i = threadIdx.x; i < num_reqs; i += kAttThreads)
+            if (a.q_indptr[i] <= t && t < a.q_indptr[i + 1]) owner = i;
+        __syncthreads();
+        r = owner;
+        if (r < 0) return;  // a row behind the last request: left as it was (the whole cluster)
+    }
     const bool report = h == 0 && rank == 0 && threadIdx.x == 0;
     const Window w = request_window(r, a.seq_lens, a.q_indptr, a.max_len, report, a.err);
-    const bool fits = w.q0 >= 0 && w.qn >= 0 && w.qn <= a.max_q_len && w.q0 + static_cast<int64_t>(w.qn) <= a.total_q;
+    const bool fits = w.q0 >= 0 && w.qn <= a.max_q_len && w.q0 + static_cast<int64_t>(w.qn) <= a.total_q;
     if (report && !fits) record_error(a.err, MSGL_ERR_BOUNDS, 801);
-    if (!fits || w.qn == 0) return;  // the whole cluster
-    const int pos = w.L - 1;
-    const int* ids = a.page_ids + (static_cast<int64_t>(w.q0) * a.hkv + h) * a.top;
+    if (!fits) return;  // the whole cluster
+    const int pos = w.L - w.qn + (t - w.q0);
+    const int* ids = a.page_ids + (static_cast<int64_t>(t) * a.hkv + h) * a.top;
     __syncthreads();
     for (int i = threadIdx.x; i < a.top; i += kAttThreads) {
         const int page = ids[i];
@@ -1000,7 +1016,7 @@ attend_pages_decode_kernel(const AttArgs a, int words) {
     }
     uint32_t qb[8][2];
     {
-        const __nv_bfloat16* qr = a.q + (static_cast<int64_t>(w.q0) * a.hq + h * G + g) * kHd;
+        const __nv_bfloat16* qr = a.q + (static_cast<int64_t>(t) * a.hq + h * G + g) * kHd;
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {
             qb[kk][0] = g < G ? *reinterpret_cast<const uint32_t*>(qr + 16 * kk + 2 * c) : 0u;
@@ -1072,7 +1088,7 @@ attend_pages_decode_kernel(const AttArgs a, int words) {
     float* co = ml + kAttWarps * 8;              // [8][128]: joined, for the cluster
     dump(st, mo + warp * 8 * kPad, mm + warp * 8, ml + warp * 8, lane);
     __syncthreads();
-    __nv_bfloat16* out = a.out + (static_cast<int64_t>(w.q0) * a.hq + h * G) * kHd;
+    __nv_bfloat16* out = a.out + (static_cast<int64_t>(t) * a.hq + h * G) * kHd;
     for (int item = threadIdx.x; item < G * 16; item += kAttThreads) {
         const int head = item >> 4, d0 = (item & 15) * 8;
         float M, L, acc[8];
@@ -1375,8 +1391,8 @@ int decode_split(int64_t lists, int top) {
 }
 
 // CTAs that share a tile of a chunk (up to 4): one SM holds one, and the rounds of 148 should be full.
-// A share costs a list and a join of its own, so it has to gain a sixth: 16 tiles take 159 us alone,
-// 69 in fours; 64 tiles 85 and 61 in twos; 256 tiles 148 and 182 in twos.
+// A share costs a list and a join of its own, so it has to gain a sixth: 16 tiles of 64 rows take 159
+// us alone, 69 in fours; 344 tiles 604 and 589 in twos; 256 tiles 148 and 182 in twos.
 int chunk_split(int64_t tiles) {
     const auto fill = [&](int s) {
         const int64_t ctas = tiles * s, rounds = (ctas + 147) / 148;
@@ -1610,7 +1626,7 @@ int msgl_paged_attention_pages(const void* q, const void* k_pool, const void* v_
     a.err = device_error_word();
     if (!a.err) return set_error(MSGL_ERR_CUDA, "device error word unavailable");
     const int G = num_q_heads / num_kv_heads;
-    if (max_q_len > 1) {
+    if (max_q_len > kRowsAlone && total_q > kTotalAlone) {
         CUtensorMap tk, tv;  // {64 dims, token rows, head halves}: one page of one kv head a box
         const uint64_t row = uint64_t(num_kv_heads) * kHd * 2;
         rc = make_tmap_3d_bf16(&tk, k_pool, 64, num_slots, 2 * num_kv_heads, row, 128, 64, kPage, 2);
@@ -1636,14 +1652,14 @@ int msgl_paged_attention_pages(const void* q, const void* k_pool, const void* v_
     }
     const int words = pages_of(max_seq_len) / 32 + 1;
     const size_t smem = kDecRing + size_t(words) * 4 + size_t(top_pages) * 8;
-    const int64_t lists = int64_t(num_reqs) * num_kv_heads;
+    const int64_t lists = int64_t(total_q) * num_kv_heads;
     if (lists * 16 > INT32_MAX) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "attention_pages: batch too large");
     const int split = decode_split(lists, top_pages);
     static std::atomic<int> optin[kMaxDevices];
     cudaError_t e = smem_optin(attend_pages_decode_kernel, smem, optin);
     if (e == cudaSuccess && split > 8) e = large_clusters();
     if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
-    e = launch_cluster(attend_pages_decode_kernel, static_cast<unsigned>(lists * split), kAttThreads, split, smem, stream, a, words);
+    e = launch_cluster(attend_pages_decode_kernel, static_cast<unsigned>(lists * split), kAttThreads, split, smem, stream, a, num_reqs, words);
     if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
     MSGL_LAUNCH_CHECK();
     return MSGL_OK;

@@ -248,7 +248,8 @@ def test_selection_in_several_passes(cuda):
 @pytest.mark.parametrize("lens,q_lens,hq,hkv,top", [
     ([1], [1], 8, 8, 1), ([17, 16, 0, 1, 900], [1] * 5, 16, 8, 8), ([3000, 200], [1, 1], 8, 1, 70),
     ([700, 130, 90], [70, 33, 1], 8, 4, 9), ([300, 40], [300, 0], 4, 4, 6), ([600, 21], [90, 21], 16, 2, 12),
-    ([520], [45], 32, 8, 10)])
+    ([520], [45], 32, 8, 10), ([900, 330, 50], [300, 70, 3], 8, 4, 20), ([700], [280], 16, 2, 9),
+    ([400, 300], [200, 120], 4, 4, 7), ([500, 600], [260, 33], 8, 1, 11)])
 def test_attention_over_selected_pages(cuda, lens, q_lens, hq, hkv, top):
     from msgl import ops
     b = Batch(lens, q_lens, hq, hkv, seed=top + 1)
@@ -260,7 +261,7 @@ def test_attention_over_selected_pages(cuda, lens, q_lens, hq, hkv, top):
     assert ops.device_error() == (0, 0)
 
 
-@pytest.mark.parametrize("q_lens", [[1, 1, 1], [40, 7, 90]])
+@pytest.mark.parametrize("q_lens", [[1, 1, 1], [40, 7, 90], [220, 33, 40]])
 @pytest.mark.parametrize("hq,hkv", [(8, 8), (8, 4), (16, 4), (16, 2)])
 def test_attention_over_any_lists(cuda, q_lens, hq, hkv):
     """Lists of the caller's: unsorted, with repeats and gaps, empty rows, different per row; other
@@ -304,17 +305,20 @@ def test_attention_over_any_lists(cuda, q_lens, hq, hkv):
     assert ops.device_error() == (0, 0)
 
 
-def test_rows_do_not_see_later_tokens(cuda):
-    """NaN and infinite keys and values of a chunk's later tokens do not reach the earlier rows."""
+@pytest.mark.parametrize("m", [40, 300])
+def test_rows_do_not_see_later_tokens(cuda, m):
+    """NaN and infinite keys and values of a chunk's later tokens do not reach the earlier rows, row by
+    row and in tiles of rows."""
     from msgl import ops
-    b = Batch([210], [40], 8, 2, seed=12)
+    n = 170 + m
+    b = Batch([n], [m], 8, 2, seed=12)
     b.all_bounds(ops)
     ids = b.select(ops, 6, 1, 2)
     clean = b.attend(ops, ids)
     for bad in (float("nan"), INF):
-        for cut in (171, 175, 176, 190, 209):  # positions from `cut` on hold bad values
+        for cut in (171, 175, 176, 190, n - 1):  # positions from `cut` on hold bad values
             k, v = b.k.clone(), b.v.clone()
-            keys = torch.arange(cut, 210, device="cuda")
+            keys = torch.arange(cut, n, device="cuda")
             slots = b.page_table[0, keys // PAGE].long() * PAGE + keys % PAGE
             b.k[slots], b.v[slots] = bad, bad
             got = b.attend(ops, ids)
@@ -341,19 +345,21 @@ def test_listed_pages_behind_the_row_and_bad_page_table(cuda):
     assert ops.device_error() == (6, 802)
 
 
-def test_contexts_and_rows_outside_what_was_announced(cuda):
+@pytest.mark.parametrize("first,second", [(20, 12), (400, 40)])
+def test_contexts_and_rows_outside_what_was_announced(cuda, first, second):
     from msgl import ops
-    b = Batch([200, 150], [20, 12], 8, 2, seed=14)
+    b = Batch([first + 180, second + 138], [first, second], 8, 2, seed=14)
     b.all_bounds(ops)
     ids = b.select(ops, 4, 1, 1)
-    b.kw = dict(q_indptr=b.indptr, max_q_len=12)  # request 0 has 20 rows
+    b.kw = dict(q_indptr=b.indptr, max_q_len=second)  # request 0 has `first` rows
     got = b.select(ops, 4, 1, 1)
     assert ops.device_error() == (6, 801)
-    assert torch.equal(got[:12], ids[:12]) and torch.equal(got[20:], ids[20:]) and bool((got[12:20] == -1).all())
+    assert torch.equal(got[:second], ids[:second]) and torch.equal(got[first:], ids[first:])
+    assert bool((got[second:first] == -1).all())
     out = b.attend(ops, ids)
-    assert ops.device_error() == (6, 801) and bool((out[:20] == 0).all()) and not bool((out[20:] == 0).any())
+    assert ops.device_error() == (6, 801) and bool((out[:first] == 0).all()) and not bool((out[first:] == 0).any())
     b.seq_lens[1] = 10 ** 6
-    b.kw = dict(q_indptr=b.indptr, max_q_len=20)
+    b.kw = dict(q_indptr=b.indptr, max_q_len=first)
     b.select(ops, 4, 1, 1)
     assert ops.device_error() == (6, 800)
     b.attend(ops, ids)
@@ -362,19 +368,21 @@ def test_contexts_and_rows_outside_what_was_announced(cuda):
     assert ops.device_error() == (6, 800)
 
 
-def test_rows_behind_the_last_request_stay(cuda):
+@pytest.mark.parametrize("first", [20, 330])
+def test_rows_behind_the_last_request_stay(cuda, first):
     from msgl import ops
-    b = Batch([200, 40], [20, 3], 8, 2, seed=15)
+    b = Batch([first + 180, 40], [first, 3], 8, 2, seed=15)
     b.all_bounds(ops)
     ids0 = b.select(ops, 4, 1, 1)
     out0 = b.attend(ops, ids0)
     b.q = torch.cat([b.q, torch.full((5, 8, D), float("nan"), device="cuda").bfloat16()])
-    ids = torch.full((28, 2, 4), 77, dtype=torch.int32, device="cuda")
-    out = torch.full((28, 8, D), 3.0, device="cuda").bfloat16()
+    n = first + 3
+    ids = torch.full((n + 5, 2, 4), 77, dtype=torch.int32, device="cuda")
+    out = torch.full((n + 5, 8, D), 3.0, device="cuda").bfloat16()
     b.select(ops, 4, 1, 1, out=ids)
-    assert torch.equal(ids[:23], ids0) and bool((ids[23:] == 77).all())
+    assert torch.equal(ids[:n], ids0) and bool((ids[n:] == 77).all())
     b.attend(ops, ids, out=out)
-    assert torch.equal(out[:23], out0) and bool((out[23:] == 3).all())
+    assert torch.equal(out[:n], out0) and bool((out[n:] == 3).all())
     assert ops.device_error() == (0, 0)
 
 
@@ -498,3 +506,15 @@ def test_full_lists_equal_dense_attention(cuda):
     dense = ops.paged_attention_extend(b.q, b.k, b.v, b.page_table, b.seq_lens, b.indptr, 77, 16, 4)
     ref, tol = b.ref_attend(ids)
     close(out, ref, tol), close(dense.view_as(out), ref, tol)
+
+
+def test_chunk_contexts_longer_than_a_window(cuda):
+    """Tiles whose context spans several windows of 2048 pages, with lists that touch some of them."""
+    from msgl import ops
+    b = Batch([100000], [270], 4, 1, seed=21)
+    g = torch.Generator().manual_seed(4)
+    ids = torch.randint(0, 6232, (270, 1, 12), generator=g).int()
+    ids[::3, 0, :6] = torch.tensor([0, 2047, 2048, 4095, 4096, 6231], dtype=torch.int32)
+    ids[5:40, 0] = torch.randint(2048, 4096, (35, 12), generator=g).int()
+    close(b.attend(ops, ids.cuda()), *b.ref_attend(ids))
+    assert ops.device_error() == (0, 0)
