@@ -165,7 +165,7 @@ struct SelectArgs {
 // Single tokens take `groups` groups of pages one after the other, the next group's page ids loaded
 // ahead, and go through a page's heads first: their bounds are neighbours in memory (64 requests at
 // 4k to 32k: 72 -> 64 us). Chunks take one group for a tile of kScoreCols columns (query rows x G),
-// whose queries lie in shared memory: the loop over them waited for L1 before (PLACEHOLDER).
+// whose queries lie in shared memory: the loop over them waited for L1 before (1.3k rows 113 -> 90 us).
 constexpr int kScoreCols = 128;
 constexpr int kScorePitch = kHd * 2 + 64;  // bytes a query: two rows of a quarter-warp in other banks
 
