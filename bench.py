@@ -288,6 +288,11 @@ def reference_workload(name):
 def run_reference_arm(args, rank):
     if rank != 0:
         return 0
+    from oracle import REF_SO
+    if not os.path.exists(REF_SO):
+        print(json.dumps({"impl": "reference",
+                          "unavailable": "oracle/_ref is not built (needs the reference sources)"}), flush=True)
+        return 0
     if args.workload != "qwen3-8b-decode":
         vals = []
         for i in range(args.warmup + args.steps):
@@ -591,11 +596,15 @@ def run_ours(args, rank, world, local_rank):
     achieved = unique_bytes / (attn_ms * 1e-3) / 1e9
 
     if rank == 0:
-        cpu = CpuReference()
-        cpu.sample()
-        cpu_val, sample = cpu.sample()
-        cpu.close()
-        cores = cpu.threads
+        try:
+            cpu = CpuReference()
+            cpu.sample()
+            cpu_val, sample = cpu.sample()
+            cpu.close()
+            cpu_baseline = {"value": cpu_val, "unit": UNIT, "cores": cpu.threads, "kind": "reference",
+                            "sample": sample}
+        except FileNotFoundError:
+            cpu_baseline = {"unavailable": "oracle/_ref is not built (needs the reference sources)"}
         line = {
             "metric": METRIC, "value": BATCH / (ms * 1e-3), "unit": UNIT,
             "n_gpus": world, "steps": args.steps, "warmup": args.warmup, "ms_per_step": ms,
@@ -618,8 +627,7 @@ def run_ours(args, rank, world, local_rank):
                          "per_request_bytes_per_launch": per_request_bytes,
                          "launch_ms": attn_ms,
                          "peak_source": "MEASURED_PEAKS.json hbm_gbs" if "hbm_gbs" in peaks else "fallback"},
-            "cpu_baseline": {"value": cpu_val, "unit": UNIT, "cores": cores, "kind": "reference",
-                             "sample": sample},
+            "cpu_baseline": cpu_baseline,
             "clocks": clk.summary(),
             "gpu_launches": launches_per_step * args.steps,
             "gpu_launches_per_step": launches_per_step,
