@@ -297,7 +297,7 @@ lora_small_kernel(const LoraArgs a, int num_reqs, int per) {
         if (!GROUPED) break;
         __syncthreads();  // list, red
     }
-    if (GROUPED && (PARTIAL || a.out != a.y || a.ldo != a.ldy)) {  // this cluster's share of the rows without one
+    if (GROUPED && (PARTIAL || a.out != a.y)) {  // this cluster's share of the rows without one
         for (int r = id; r < num_reqs; r += a.num_adapters * per) {
             const int own = a.ids[r];
             if (own >= 0 && own < a.num_adapters) continue;
@@ -447,7 +447,10 @@ lora_expand_kernel(const LoraArgs a, int n_slices) {
     id /= n_slices;
     const int tile = static_cast<int>(id % a.tiles), r = static_cast<int>(id / a.tiles);
     const LoraTile lt = lora_tile(a, r, tile, kTile, false);
-    if (lt.rows <= 0) return;
+    if (lt.rows <= 0) {
+        pdl_wait();  // no grid may end before its predecessor
+        return;
+    }
     const bool some = lt.adapter >= 0;
     const int n0 = ns * kNSlice;
     const auto swizzle = [](int row, int piece) {
@@ -464,6 +467,7 @@ lora_expand_kernel(const LoraArgs a, int n_slices) {
     }
     pdl_wait();
     pdl_trigger();
+    if (!PARTIAL && !some && a.out == a.y) return;  // in place: nothing to add
     if (some) {
 #pragma unroll
         for (int m = 0; m < TERMS; ++m)
@@ -636,6 +640,8 @@ int launch_lora(LoraArgs a, int num_reqs, bool partial, void* workspace, size_t 
     const int64_t ow = partial ? 4 : 8;  // elements per 16 bytes of out
     if (a.ldx < a.K || a.ldx % 8 || a.ldo < a.N || a.ldo % ow || (!partial && (a.ldy < a.N || a.ldy % 8)))
         return set_error(MSGL_ERR_INVALID_ARG, "lora: row strides must cover the row and keep it 16-byte aligned");
+    if (!partial && a.out == a.y && a.ldo != a.ldy)
+        return set_error(MSGL_ERR_INVALID_ARG, "lora: out in place of y needs y's row stride");
     if (!a.x || !a.ids || !a.out || (!partial && !a.y) || (a.num_adapters && (!a.a || !a.b || !a.scales)))
         return set_error(MSGL_ERR_INVALID_ARG, "lora: null pointer");
     if (!aligned16(a.x) || !aligned16(a.a) || !aligned16(a.b) || !aligned16(a.y) || !aligned16(a.out))
@@ -645,6 +651,7 @@ int launch_lora(LoraArgs a, int num_reqs, bool partial, void* workspace, size_t 
         return set_error(MSGL_ERR_WORKSPACE, "lora: workspace missing, unaligned or too small");
     a.err = device_error_word();
     if (!a.err) return set_error(MSGL_ERR_CUDA, "device error word unavailable");
+    a.max_q_len = std::min(a.max_q_len, a.T);  // no request can own more rows
     a.h = static_cast<__nv_bfloat16*>(workspace);
     a.tiles = (a.max_q_len + kTile - 1) / kTile;
     if (int64_t(num_reqs) * a.tiles * std::max(8, (a.N + kNSlice - 1) / kNSlice) > INT32_MAX)

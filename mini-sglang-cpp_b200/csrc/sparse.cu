@@ -1517,7 +1517,7 @@ int msgl_select_pages(const void* q, const void* bounds, int64_t num_pages, cons
     a.q_indptr = q_indptr;
     a.num_reqs = num_reqs;
     a.total_q = total_q;
-    a.max_q_len = max_q_len;
+    a.max_q_len = max_q_len = std::min(max_q_len, total_q);  // no request can own more rows
     a.max_len = max_seq_len;
     a.hq = num_q_heads;
     a.hkv = num_kv_heads;
@@ -1615,7 +1615,7 @@ int msgl_paged_attention_pages(const void* q, const void* k_pool, const void* v_
     a.seq_lens = seq_lens;
     a.q_indptr = q_indptr;
     a.total_q = total_q;
-    a.max_q_len = max_q_len;
+    a.max_q_len = max_q_len = std::min(max_q_len, total_q);  // no request can own more rows
     a.max_len = max_seq_len;
     a.page_ids = page_ids;
     a.top = top_pages;

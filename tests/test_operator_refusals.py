@@ -135,7 +135,8 @@ def test_lora(partial, bad, rc):
 
 
 def test_lora_y_and_empty():
-    assert lora(y=None) == INVALID and lora(ldy=120) == INVALID and lora(ldy=129) == INVALID and lora(y=P + 2) == INVALID
+    assert lora(ldo=136) == INVALID  # in place with another stride
+    assert lora(y=None, out=P) == INVALID and lora(ldy=120) == INVALID and lora(ldy=129) == INVALID and lora(y=P + 2) == INVALID
     for partial in (False, True):
         assert lora(partial, T=0, B=0) == 0 and lora(partial, ip=P, mq=0) == 0 and lora(partial, ip=P, B=0) == 0
     assert msgl.lib().msgl_lora_workspace_size(0, 64, 16) == 0

@@ -518,3 +518,51 @@ def test_chunk_contexts_longer_than_a_window(cuda):
     ids[5:40, 0] = torch.randint(2048, 4096, (35, 12), generator=g).int()
     close(b.attend(ops, ids.cuda()), *b.ref_attend(ids))
     assert ops.device_error() == (0, 0)
+
+
+def test_largest_context_and_list(cuda):
+    from msgl import ops
+    b = Batch([524288, 40], [1, 1], 2, 1, seed=22)
+    b.all_bounds(ops)
+    ids = b.select(ops, 1024, 3, 5)
+    assert torch.equal(ids.cpu(), b.ref_select(1024, 3, 5))
+    close(b.attend(ops, ids), *b.ref_attend(ids))
+    assert ops.device_error() == (0, 0)
+
+
+@pytest.mark.parametrize("m", [1, 700])
+def test_nan_queries(cuda, m):
+    """A row of NaN ties all its pages (the lowest are taken) and gives NaN; its neighbours' lists stay
+    and their outputs stay right (in tiles not bit for bit: where a tile's joined list is cut into
+    shares follows from all of its rows' lists)."""
+    from msgl import ops
+    b = Batch([9000, 9000], [m, m], 8, 2, seed=23)
+    b.all_bounds(ops)
+    ids0 = b.select(ops, 10, 1, 2)
+    out0 = b.attend(ops, ids0)
+    b.q[0, :4] = float("nan")
+    ids = b.select(ops, 10, 1, 2)
+    last = (9000 - m) // PAGE
+    assert ids[0, 0].tolist() == list(range(8)) + [last - 1, last]
+    ids0[0, 0] = ids[0, 0]
+    assert torch.equal(ids, ids0)
+    out = b.attend(ops, ids)
+    assert bool(out[0, :4].isnan().all())
+    ref, tol = b.ref_attend(ids)
+    close(out[1:], ref[1:], tol[1:]), close(out[0, 4:], ref[0, 4:], tol[0, 4:]), close(out0[1:], ref[1:], tol[1:])
+
+
+def test_tensors_elsewhere_are_refused(cuda):
+    from msgl import ops
+    b = Batch([40], [1], 4, 2, seed=24)
+    with pytest.raises(ValueError):
+        ops.kv_page_bounds_(b.bounds, b.k.cpu(), b.page_table, b.seq_lens, 2)
+    with pytest.raises(ValueError):
+        ops.kv_page_bounds_(b.bounds, b.k, b.page_table, b.seq_lens.long(), 2)
+    with pytest.raises(ValueError):
+        ops.select_pages(b.q.transpose(1, 2), b.bounds, b.page_table, b.seq_lens, 40, 2, 4, 2)
+    with pytest.raises(AssertionError):
+        ops.select_pages(b.q, b.bounds, b.page_table, b.seq_lens, 40, 2, 4, 2, max_q_len=2)
+    with pytest.raises(ValueError):
+        ops.paged_attention_pages(b.q, b.k, b.v.cpu(), b.page_table, b.seq_lens,
+                                  torch.zeros(1, 2, 1, dtype=torch.int32, device="cuda"), 4, 2)
