@@ -1146,7 +1146,8 @@ attend_pages_decode_kernel(const AttArgs a, int num_reqs, int words) {
 // Bound by the TMA boxes: without the products the loads alone take 260 of 450 us (1.3k rows of 32
 // heads over 64 pages each, 126k page loads of 8 KB). Slower ways to bring the same pages: cp.async
 // from producer warps 575 us (it shares the path of the fragment loads), bulk copies of single rows
-// 1315 us, tiles of 16 rows on two CTAs per SM 565 us.
+// 1315 us, K by TMA and V by cp.async 497 us, tiles of 16 rows on two CTAs per SM 565 us. Stages of
+// 2 / 4 / 6 / 10 pages (of 20 in the ring): selection and attention 661 / 586 / 571 / 568 us.
 //
 // A masked weight is zero, but zero times a NaN or infinite value is NaN. Such values are looked
 // for at the end instead of at every page: a row they reached is NaN from then on, so a tile
@@ -1154,8 +1155,8 @@ attend_pages_decode_kernel(const AttArgs a, int num_reqs, int words) {
 // kept out (PART of attend).
 constexpr int kChWarps = 16;
 constexpr int kChThreads = (kChWarps + 1) * 32;
-constexpr int kStagePages = 4;
-constexpr int kChStages = 5;
+constexpr int kStagePages = 6;
+constexpr int kChStages = 3;
 constexpr int kStageBytes = kStagePages * kPageBytes;
 constexpr int kWin = 2048;
 constexpr int kTileRows = 64;  // mask bits
@@ -1549,7 +1550,7 @@ int msgl_select_pages(const void* q, const void* bounds, int64_t num_pages, cons
     const int64_t heads = int64_t(num_reqs) * tiles * num_kv_heads;
     const int all_groups = (pages_of(max_seq_len) + kScorePages - 1) / kScorePages;
     int groups = 1;
-    while (!chunk && groups < 8 && heads * all_groups >= 16 * 148 * groups) groups *= 2;
+    while (!chunk && groups < 8 && heads * all_groups >= 32 * 148 * groups) groups *= 2;
     const int page_tiles = (all_groups + groups - 1) / groups;
     const int64_t blocks = heads * page_tiles;
     const int64_t sel_blocks = int64_t(slab) * num_kv_heads;
