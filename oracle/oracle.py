@@ -37,7 +37,7 @@ def build(with_ref: bool | None = None, reference_src: str | None = None) -> Non
     src = reference_src if reference_src is not None else REFERENCE_SRC
     targets, extra = ["oracle"], []
     if with_ref is None:
-        with_ref = bool(src) and os.path.isdir(src)
+        with_ref = bool(src) and os.path.isdir(os.path.join(src, "src"))
     if with_ref:
         targets.append("ref")
         extra = [f"REF={src}", f"JSON_INC={json_include_dir()}"]
