@@ -316,7 +316,7 @@ lora_small_kernel(const LoraArgs a, int num_reqs, int per) {
 // ------------------------------------------------------------------ chunks
 constexpr int kTile = 64;     // rows a CTA
 constexpr int kBK = 64;       // K columns a stage
-constexpr int sh_stages(int kk) { return kk == 8 ? 4 : 6; }  // of 16 or 24 KB: two CTAs per SM
+constexpr int sh_stages(int kk) { return kk == 8 ? 4 : 5; }  // of 16 or 24 KB: two CTAs per SM
 constexpr int kNSlice = 256;  // columns of an expand CTA
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {

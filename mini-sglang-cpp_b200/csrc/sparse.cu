@@ -1143,7 +1143,7 @@ attend_pages_decode_kernel(const AttArgs a, int num_reqs, int words) {
 // of that many. A cluster of CTAs (chunk_split) shares a tile: each takes a share of every window's
 // list, and the partial results are joined through distributed shared memory.
 //
-// Bound by the TMA boxes: without the products the loads alone take 260 of 450 us (1.3k rows of 32
+// Bound by the TMA boxes: without the products the loads alone take 260 of 435 us (1.3k rows of 32
 // heads over 64 pages each, 126k page loads of 8 KB). Slower ways to bring the same pages: cp.async
 // from producer warps 575 us (it shares the path of the fragment loads), bulk copies of single rows
 // 1315 us, K by TMA and V by cp.async 497 us, tiles of 16 rows on two CTAs per SM 565 us. Stages of
@@ -1557,7 +1557,10 @@ int msgl_select_pages(const void* q, const void* bounds, int64_t num_pages, cons
     if (blocks > INT32_MAX || sel_blocks > INT32_MAX)
         return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "select_pages: batch too large");
     // Up to 1024 pages a warp holds a row; with too few rows to fill the GPU, and for longer
-    // rows, more warps share one.
+    // rows, more warps share one. Few warps that hold many scores beat many that hold few, whose
+    // counts meet at a barrier in every step: 8192 pages, one request, 8 warps 27.5 us for
+    // selection and attention, 16 warps 29.2; 2048 pages, 64 requests, 4 warps 173, 8 warps 175,
+    // 16 warps 186. At 512 pages the order turns: 4 warps 15.2 us, 2 warps 16.6.
     using Select = void (*)(SelectArgs, int);
     const int pages = pages_of(max_seq_len);
     const bool many = sel_blocks >= 4 * 148;
@@ -1566,8 +1569,8 @@ int msgl_select_pages(const void* q, const void* bounds, int64_t num_pages, cons
     if (pages <= 256 && many) { select = select_pages_kernel<1, 8, 4>; warps = 1; rows = 4; }
     else if (pages <= 1024 && many) { select = select_pages_kernel<1, 32, 4>; warps = 1; rows = 4; }
     else if (pages <= 512) { select = select_pages_kernel<4, 4, 1>; warps = 4; rows = 1; }
-    else if (pages <= 2048) { select = select_pages_kernel<8, 8, 1>; warps = 8; rows = 1; }
-    else if (pages <= 8192) { select = select_pages_kernel<16, 16, 1>; warps = 16; rows = 1; }
+    else if (pages <= 2048) { select = select_pages_kernel<4, 16, 1>; warps = 4; rows = 1; }
+    else if (pages <= 8192) { select = select_pages_kernel<8, 32, 1>; warps = 8; rows = 1; }
     else { select = select_pages_kernel<32, 32, 1>; warps = 32; rows = 1; }
     for (int t0 = 0; t0 < total_q; t0 += slab) {
         a.t0 = t0;
