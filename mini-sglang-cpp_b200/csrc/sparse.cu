@@ -816,12 +816,15 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 }
 
 // One page (16 keys) for one warp. K and V tiles: halves of 64 dims, rows of 128 bytes, 16-byte
-// pieces swizzled by the row. qb: column g's query as the B operand. lim0 / lim1: last visible
+// pieces swizzled by the row; with PADDED rows of kPadRow bytes, 16 more than they hold, which sets
+// the rows of a fragment 16 bytes apart in the banks as well. qb: column g's query as the B operand. lim0 / lim1: last visible
 // offset in the page for columns 2 c / 2 c + 1 (< 0: the page is not of that column). With PART,
 // only columns whose own limit is >= 0 take the new sums (the others' P is zero, but zero times a
 // NaN or infinite value of a page that is not theirs must not reach them), and V rows behind vlim
 // count as zero for the same reason.
-template <bool PART>
+constexpr int kPadRow = kHd * 2 + 16;
+constexpr int kPadTile = kPage * kPadRow;
+template <bool PART, bool PADDED>
 __device__ __forceinline__ void attend(uint32_t base, const uint32_t (&qb)[8][2], Softmax& st,
                                        int lim0, int lim1, int vlim, float sl2e, int lane) {
     const int mi = lane >> 3, g = lane >> 2, c = lane & 3;
@@ -832,7 +835,9 @@ __device__ __forceinline__ void attend(uint32_t base, const uint32_t (&qb)[8][2]
     for (int kk = 0; kk < 8; ++kk) {
         const int row = ((mi & 1) << 3) + (lane & 7);
         const int piece = ((kk & 3) << 1) + (mi >> 1);
-        ldsm_x4(base + ((kk >> 2) << 11) + row * 128 + ((piece ^ (row & 7)) << 4), f[kk][0], f[kk][1], f[kk][2], f[kk][3]);
+        const uint32_t at = PADDED ? row * kPadRow + ((2 * kk + (mi >> 1)) << 4)
+                                   : ((kk >> 2) << 11) + row * 128 + ((piece ^ (row & 7)) << 4);
+        ldsm_x4(base + at, f[kk][0], f[kk][1], f[kk][2], f[kk][3]);
     }
     float s[2][4];
 #pragma unroll
@@ -842,11 +847,13 @@ __device__ __forceinline__ void attend(uint32_t base, const uint32_t (&qb)[8][2]
 #pragma unroll
     for (int kk = 0; kk < 8; ++kk)  // two chains
         mma_bf16_16816(s[kk & 1], f[kk][0], f[kk][1], f[kk][2], f[kk][3], qb[kk][0], qb[kk][1]);
-    const uint32_t vb = base + kPageBytes / 2;
+    const uint32_t vb = base + (PADDED ? kPadTile : kPageBytes / 2);
     const auto load_v = [&](int j) {
         const int row = ((mi >> 1) << 3) + (lane & 7);
         const int piece = ((j & 3) << 1) + (mi & 1);
-        ldsm_x4_t(vb + ((j >> 2) << 11) + row * 128 + ((piece ^ (row & 7)) << 4), f[j][0], f[j][1], f[j][2], f[j][3]);
+        const uint32_t at = PADDED ? row * kPadRow + ((2 * j + (mi & 1)) << 4)
+                                   : ((j >> 2) << 11) + row * 128 + ((piece ^ (row & 7)) << 4);
+        ldsm_x4_t(vb + at, f[j][0], f[j][1], f[j][2], f[j][3]);
     };
 #pragma unroll
     for (int j = 0; j < 4; ++j) load_v(j);
@@ -1075,7 +1082,7 @@ attend_pages_decode_kernel(const AttArgs a, int num_reqs, int words) {
         if (i + kDecStages - 1 < mine) issue(i + kDecStages - 1);
         cp_async_commit();
         const int lim = pos - list_page[warp + i * kAttWarps] * kPage;
-        attend<false>(ring0 + (i % kDecStages) * kPageBytes, qb, st, lim, lim, 0, a.sl2e, lane);
+        attend<false, false>(ring0 + (i % kDecStages) * kPageBytes, qb, st, lim, lim, 0, a.sl2e, lane);
         __syncwarp();
     }
 
@@ -1157,7 +1164,7 @@ constexpr int kChWarps = 16;
 constexpr int kChThreads = (kChWarps + 1) * 32;
 constexpr int kStagePages = 6;
 constexpr int kChStages = 3;
-constexpr int kStageBytes = kStagePages * kPageBytes;
+constexpr int kStageBytes = kStagePages * 2 * kPadTile;
 constexpr int kWin = 2048;
 constexpr int kTileRows = 64;  // mask bits
 constexpr int kChSmem = kChStages * kStageBytes + kWin * (8 + 4 + 2) + 1024;
@@ -1274,11 +1281,11 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
                         if (!ok) break;
                         const int e0 = i * kStagePages, pages_in = min(kStagePages, count - e0);
                         uint8_t* dst = ring + s * kStageBytes;
-                        mbar_arrive_expect_tx(&full[s], pages_in * kPageBytes);
-                        for (int e = 0; e < pages_in; ++e, dst += kPageBytes) {
+                        mbar_arrive_expect_tx(&full[s], pages_in * 2 * kPadTile);
+                        for (int e = 0; e < pages_in; ++e, dst += 2 * kPadTile) {
                             const int y = list_phys[e0 + e] * kPage;
-                            tma_load_3d(dst, &tk, &full[s], 0, y, 2 * h);
-                            tma_load_3d(dst + kPageBytes / 2, &tv, &full[s], 0, y, 2 * h);
+                            tma_load_3d(dst, &tk, &full[s], 0, h, y);
+                            tma_load_3d(dst + kPadTile, &tv, &full[s], 0, h, y);
                         }
                     }
             } else {
@@ -1298,11 +1305,11 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
                         const int x = __ffs(some) - 1;
                         if (!ok || mine++ % PW != pg) continue;
                         const uint32_t mask = __shfl_sync(0xffffffffu, want, x);
-                        const uint32_t base = smem_u32(ring) + s * kStageBytes + x * kPageBytes;
+                        const uint32_t base = smem_u32(ring) + s * kStageBytes + x * 2 * kPadTile;
                         // the first row's position in the page
                         const int rel = pos0 + wrow - (w0 + __shfl_sync(0xffffffffu, page, x)) * kPage;
                         if (!careful) {
-                            attend<false>(base, qb, st, ((mask >> row0) & 1u) ? rel + row0 : -1,
+                            attend<false, true>(base, qb, st, ((mask >> row0) & 1u) ? rel + row0 : -1,
                                           ((mask >> row1) & 1u) ? rel + row1 : -1, 0, a.sl2e, lane);
                         } else {
                             // rows that see the whole page go together, one that ends inside it alone
@@ -1310,7 +1317,7 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
                                 const int row = __ffs(left) - 1;
                                 const uint32_t now = rel + row >= kPage - 1 ? left : 1u << row;
                                 left &= ~now;
-                                attend<true>(base, qb, st, ((now >> row0) & 1u) ? rel + row : -1,
+                                attend<true, true>(base, qb, st, ((now >> row0) & 1u) ? rel + row : -1,
                                              ((now >> row1) & 1u) ? rel + row : -1, rel + row, a.sl2e, lane);
                             }
                         }
@@ -1631,10 +1638,10 @@ int msgl_paged_attention_pages(const void* q, const void* k_pool, const void* v_
     if (!a.err) return set_error(MSGL_ERR_CUDA, "device error word unavailable");
     const int G = num_q_heads / num_kv_heads;
     if (max_q_len > kRowsAlone && total_q > kTotalAlone) {
-        CUtensorMap tk, tv;  // {64 dims, token rows, head halves}: one page of one kv head a box
+        CUtensorMap tk, tv;  // {dims, kv heads, token rows}: one page of one kv head a box, its rows padded
         const uint64_t row = uint64_t(num_kv_heads) * kHd * 2;
-        rc = make_tmap_3d_bf16(&tk, k_pool, 64, num_slots, 2 * num_kv_heads, row, 128, 64, kPage, 2);
-        if (!rc) rc = make_tmap_3d_bf16(&tv, v_pool, 64, num_slots, 2 * num_kv_heads, row, 128, 64, kPage, 2);
+        rc = make_tmap_3d_bf16(&tk, k_pool, kHd, num_kv_heads, num_slots, kHd * 2, row, kPadRow / 2, 1, kPage, false);
+        if (!rc) rc = make_tmap_3d_bf16(&tv, v_pool, kHd, num_kv_heads, num_slots, kHd * 2, row, kPadRow / 2, 1, kPage, false);
         if (rc) return rc;
         const int tq = 8 / G;
         int row_groups = 1;
