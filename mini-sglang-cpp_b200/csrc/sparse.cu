@@ -829,31 +829,38 @@ __device__ __forceinline__ void attend(uint32_t base, const uint32_t (&qb)[8][2]
                                        int lim0, int lim1, int vlim, float sl2e, int lane) {
     const int mi = lane >> 3, g = lane >> 2, c = lane & 3;
     // The asm statements keep their order, so fragments are loaded some steps ahead of the MMAs that
-    // take them: all of K at once, half of V before the softmax and half behind it.
-    uint32_t f[8][4];
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk) {
+    // take them: kAhead of K, then half of V before the softmax and the rest behind it.
+    constexpr int kAhead = PADDED ? 6 : 8;  // chunks have 96 registers a thread
+    uint32_t f[kAhead][4];
+    const auto load_k = [&](int kk) {
         const int row = ((mi & 1) << 3) + (lane & 7);
         const int piece = ((kk & 3) << 1) + (mi >> 1);
         const uint32_t at = PADDED ? row * kPadRow + ((2 * kk + (mi >> 1)) << 4)
                                    : ((kk >> 2) << 11) + row * 128 + ((piece ^ (row & 7)) << 4);
-        ldsm_x4(base + at, f[kk][0], f[kk][1], f[kk][2], f[kk][3]);
-    }
+        uint32_t(&x)[4] = f[kk % kAhead];
+        ldsm_x4(base + at, x[0], x[1], x[2], x[3]);
+    };
+#pragma unroll
+    for (int kk = 0; kk < kAhead; ++kk) load_k(kk);
     float s[2][4];
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk)  // two chains
-        mma_bf16_16816(s[kk & 1], f[kk][0], f[kk][1], f[kk][2], f[kk][3], qb[kk][0], qb[kk][1]);
+    for (int kk = 0; kk < 8; ++kk) {  // two chains
+        const uint32_t(&x)[4] = f[kk % kAhead];
+        mma_bf16_16816(s[kk & 1], x[0], x[1], x[2], x[3], qb[kk][0], qb[kk][1]);
+        if (kk + kAhead < 8) load_k(kk + kAhead);
+    }
     const uint32_t vb = base + (PADDED ? kPadTile : kPageBytes / 2);
     const auto load_v = [&](int j) {
         const int row = ((mi >> 1) << 3) + (lane & 7);
         const int piece = ((j & 3) << 1) + (mi & 1);
         const uint32_t at = PADDED ? row * kPadRow + ((2 * j + (mi & 1)) << 4)
                                    : ((j >> 2) << 11) + row * 128 + ((piece ^ (row & 7)) << 4);
-        ldsm_x4_t(vb + at, f[j][0], f[j][1], f[j][2], f[j][3]);
+        uint32_t(&x)[4] = f[j % kAhead];
+        ldsm_x4_t(vb + at, x[0], x[1], x[2], x[3]);
     };
 #pragma unroll
     for (int j = 0; j < 4; ++j) load_v(j);
@@ -891,7 +898,7 @@ __device__ __forceinline__ void attend(uint32_t base, const uint32_t (&qb)[8][2]
     const uint32_t b0 = transpose8x8(pack_bf16x2(p[0], p[1]));
     const uint32_t b1 = transpose8x8(pack_bf16x2(p[2], p[3]));
 #pragma unroll
-    for (int j = 4; j < 8; ++j) load_v(j);
+    for (int j = 4; j < kAhead; ++j) load_v(j);
     // V fragments hold keys (2c, 2c + 1) and (2c + 8, 2c + 9)
     uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
     if (PART) {
@@ -900,17 +907,19 @@ __device__ __forceinline__ void attend(uint32_t base, const uint32_t (&qb)[8][2]
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
+        const uint32_t(&x)[4] = f[j % kAhead];
         if (!PART) {
-            mma_bf16_16816(st.o[j], f[j][0], f[j][1], f[j][2], f[j][3], b0, b1);
+            mma_bf16_16816(st.o[j], x[0], x[1], x[2], x[3], b0, b1);
         } else {
             float d[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) d[e] = st.o[j][e];
-            mma_bf16_16816(d, f[j][0] & keep0, f[j][1] & keep0, f[j][2] & keep1, f[j][3] & keep1, b0, b1);
+            mma_bf16_16816(d, x[0] & keep0, x[1] & keep0, x[2] & keep1, x[3] & keep1, b0, b1);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if ((e & 1 ? lim1 : lim0) >= 0) st.o[j][e] = d[e];
         }
+        if (j + kAhead < 8) load_v(j + kAhead);
     }
 }
 
@@ -1160,6 +1169,23 @@ attend_pages_decode_kernel(const AttArgs a, int num_reqs, int words) {
 // for at the end instead of at every page: a row they reached is NaN from then on, so a tile
 // without NaN or infinite sums was right, and any other is computed again with the masked values
 // kept out (PART of attend).
+struct Careful {
+    Softmax st;
+    uint32_t qb[8][2];
+};
+// Not inlined, and with copies of the state: inlined it costs the loop of ordinary pages 10% (spills).
+__device__ __noinline__ void attend_careful(Careful* x, uint32_t base, uint32_t mask, int rel, int row0, int row1,
+                                            float sl2e, int lane) {
+    // rows that see the whole page go together, one that ends inside it alone
+    for (uint32_t left = mask; left;) {
+        const int row = __ffs(left) - 1;
+        const uint32_t now = rel + row >= kPage - 1 ? left : 1u << row;
+        left &= ~now;
+        attend<true, true>(base, x->qb, x->st, ((now >> row0) & 1u) ? rel + row : -1,
+                           ((now >> row1) & 1u) ? rel + row : -1, rel + row, sl2e, lane);
+    }
+}
+
 constexpr int kChWarps = 16;
 constexpr int kChThreads = (kChWarps + 1) * 32;
 constexpr int kStagePages = 6;
@@ -1174,8 +1200,8 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
                           const AttArgs a, int tiles, int row_groups) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    unsigned long long* masks = reinterpret_cast<unsigned long long*>(ring + kChStages * kStageBytes);  // [kWin]
-    int* list_phys = reinterpret_cast<int*>(masks + kWin);                // [kWin]
+    uint32_t* masks = reinterpret_cast<uint32_t*>(ring + kChStages * kStageBytes);  // [2][kWin]: rows 0-31, 32-63
+    int* list_phys = reinterpret_cast<int*>(masks + 2 * kWin);            // [kWin]
     uint16_t* list_page = reinterpret_cast<uint16_t*>(list_phys + kWin);  // [kWin], in the window
     __shared__ uint64_t full[kChStages], empty[kChStages];
     __shared__ int scan[32];
@@ -1190,11 +1216,12 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
         tma_prefetch_desc(&tk);
         tma_prefetch_desc(&tv);
     }
+    for (int i = threadIdx.x; i < 2 * kWin; i += kChThreads) masks[i] = 0;
     pdl_wait();
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int G = a.hq / a.hkv;
-    const int TQ = 8 / G;
+    const int lgG = 31 - __clz(G), TQ = 8 >> lgG;
     const int RW = row_groups, PW = kChWarps / RW, rg = warp % RW, pg = warp / RW;
     const int CS = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
     int64_t id = static_cast<int>(blockIdx.x) / CS;
@@ -1211,12 +1238,12 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
     const int pos0 = w.L - w.qn + i0;  // position of the tile's first row
 
     const int wrow = rg * TQ, wrows = max(0, min(TQ, rows - wrow));  // this warp's rows (may be none)
-    const int row0 = 2 * c / G, row1 = (2 * c + 1) / G;              // of columns 2 c, 2 c + 1, in the warp
+    const int row0 = (2 * c) >> lgG, row1 = (2 * c + 1) >> lgG;              // of columns 2 c, 2 c + 1, in the warp
     uint32_t qb[8][2];
     {
-        const bool real = warp < kChWarps && g / G < wrows;
+        const bool real = warp < kChWarps && (g >> lgG) < wrows;
         const __nv_bfloat16* qr =
-            a.q + (static_cast<int64_t>(w.q0 + i0 + wrow + g / G) * a.hq + h * G + g % G) * kHd;
+            a.q + (static_cast<int64_t>(w.q0 + i0 + wrow + (g >> lgG)) * a.hq + h * G + (g & (G - 1))) * kHd;
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {
             qb[kk][0] = real ? *reinterpret_cast<const uint32_t*>(qr + 16 * kk + 2 * c) : 0u;
@@ -1231,63 +1258,85 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
     for (int careful = 0; careful < 2; ++careful) {
         st.clear();
         for (int w0 = 0; w0 < pages; w0 += kWin) {
-            for (int i = threadIdx.x; i < kWin; i += kChThreads) masks[i] = 0;
-            __syncthreads();
-            for (int i = threadIdx.x; i < rows * a.top; i += kChThreads) {
-                const int row = i / a.top;
-                const int page =
-                    a.page_ids[(static_cast<int64_t>(w.q0 + i0 + row) * a.hkv + h) * a.top + (i - row * a.top)];
-                if (page < 0) continue;
-                const int pos = pos0 + row;
-                if (pos < 0 || page > pos / kPage) {
-                    if (w0 == 0 && !careful && rank == 0) record_error(a.err, MSGL_ERR_BOUNDS, 803);
-                    continue;
-                }
-                if (page >= w0 && page < w0 + kWin) atomicOr(&masks[page - w0], 1ull << row);
-            }
-            __syncthreads();
+            // Loads first, each kind together: the table of this thread's run of pages, then ids by fours.
             constexpr int kRun = kWin / (kChWarps * 32);
             const int run0 = static_cast<int>(threadIdx.x) * kRun;  // the producer warp has none
+            int phys[kRun];
+#pragma unroll
+            for (int e = 0; e < kRun; ++e)
+                phys[e] = warp < kChWarps && w0 + run0 + e < pages
+                              ? a.page_table[static_cast<int64_t>(r) * a.max_pages + w0 + run0 + e] : 0;
+            __syncthreads();  // masks are zero
+            const int* ids = a.page_ids + (static_cast<int64_t>(w.q0 + i0) * a.hkv + h) * a.top;
+            const int step_row = kChThreads / a.top, step_at = kChThreads % a.top;
+            int row = threadIdx.x / a.top, at = threadIdx.x % a.top;
+            while (row < rows) {
+                int page[4], of[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    page[e] = row < rows ? ids[static_cast<int64_t>(row) * a.hkv * a.top + at] : -1;
+                    of[e] = row;
+                    row += step_row;
+                    at += step_at;
+                    if (at >= a.top) {
+                        at -= a.top;
+                        ++row;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (page[e] < 0) continue;
+                    const int pos = pos0 + of[e];
+                    if (pos < 0 || page[e] > pos / kPage) {
+                        if (w0 == 0 && !careful && rank == 0) record_error(a.err, MSGL_ERR_BOUNDS, 803);
+                        continue;
+                    }
+                    if (page[e] >= w0 && page[e] < w0 + kWin)
+                        atomicOr(&masks[(of[e] >> 5) * kWin + page[e] - w0], 1u << (of[e] & 31));
+                }
+            }
+            __syncthreads();
+            uint32_t any[kRun];
             int per = 0;
-            if (warp < kChWarps)
-                for (int i = 0; i < kRun; ++i) per += masks[run0 + i] != 0;
+#pragma unroll
+            for (int e = 0; e < kRun; ++e) {
+                any[e] = warp < kChWarps ? masks[run0 + e] | masks[kWin + run0 + e] : 0u;
+                per += any[e] != 0;
+            }
             int total;
-            int at = block_excl_scan(per, scan, total);
+            at = block_excl_scan(per, scan, total);
             const int lo = total * rank / CS, count = total * (rank + 1) / CS - lo;  // this CTA's share
             at -= lo;
-            if (per)
-                for (int i = 0; i < kRun; ++i) {
-                    if (!masks[run0 + i]) continue;
-                    if (at >= 0 && at < count) list_page[at] = static_cast<uint16_t>(run0 + i);
-                    ++at;
+#pragma unroll
+            for (int e = 0; e < kRun; ++e) {
+                if (!any[e]) continue;
+                if (at >= 0 && at < count) {
+                    if (static_cast<unsigned>(phys[e]) >= static_cast<unsigned>(a.pool_pages)) {
+                        record_error(a.err, MSGL_ERR_BOUNDS, 802);
+                        phys[e] = 0;
+                    }
+                    list_page[at] = static_cast<uint16_t>(run0 + e);
+                    list_phys[at] = phys[e];
                 }
-            __syncthreads();
-            for (int i = threadIdx.x; i < count; i += kChThreads) {  // all in flight together
-                int phys = a.page_table[static_cast<int64_t>(r) * a.max_pages + w0 + list_page[i]];
-                if (static_cast<unsigned>(phys) >= static_cast<unsigned>(a.pool_pages)) {
-                    record_error(a.err, MSGL_ERR_BOUNDS, 802);
-                    phys = 0;
-                }
-                list_phys[i] = phys;
+                ++at;
             }
             __syncthreads();
 
             const int stages = (count + kStagePages - 1) / kStagePages;
             if (warp == kChWarps) {
-                if (lane == 0)
-                    for (int i = 0; i < stages; ++i) {
-                        const int n = done + i, s = n % kChStages;
-                        if (n >= kChStages) ok = ok && mbar_wait(&empty[s], (n / kChStages - 1) & 1, a.err, 821);
-                        if (!ok) break;
-                        const int e0 = i * kStagePages, pages_in = min(kStagePages, count - e0);
-                        uint8_t* dst = ring + s * kStageBytes;
-                        mbar_arrive_expect_tx(&full[s], pages_in * 2 * kPadTile);
-                        for (int e = 0; e < pages_in; ++e, dst += 2 * kPadTile) {
-                            const int y = list_phys[e0 + e] * kPage;
-                            tma_load_3d(dst, &tk, &full[s], 0, h, y);
-                            tma_load_3d(dst + kPadTile, &tv, &full[s], 0, h, y);
-                        }
-                    }
+                for (int i = 0; i < stages; ++i) {  // lane l loads K (even) or V of page l / 2
+                    const int n = done + i, s = n % kChStages;
+                    const int e0 = i * kStagePages, pages_in = min(kStagePages, count - e0);
+                    const int y = lane < 2 * pages_in ? list_phys[e0 + lane / 2] * kPage : 0;
+                    if (n >= kChStages)
+                        ok = ok && __all_sync(0xffffffffu, mbar_wait(&empty[s], (n / kChStages - 1) & 1, a.err, 821));
+                    if (!ok) break;
+                    if (lane == 0) mbar_arrive_expect_tx(&full[s], pages_in * 2 * kPadTile);
+                    __syncwarp();
+                    if (lane < 2 * pages_in)
+                        tma_load_3d(ring + s * kStageBytes + lane * kPadTile, lane & 1 ? &tv : &tk, &full[s], 0, h, y);
+                    __syncwarp();
+                }
             } else {
                 for (int i = 0, mine = 0; i < stages; ++i) {
                     const int n = done + i, s = n % kChStages;
@@ -1297,10 +1346,10 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
                     uint32_t want = 0;
                     if (lane < kStagePages && e < count) {
                         page = list_page[e];
-                        want = static_cast<uint32_t>(masks[page] >> wrow) & wmask;
+                        want = (masks[(wrow >> 5) * kWin + page] >> (wrow & 31)) & wmask;
                     }
                     unsigned some = __ballot_sync(0xffffffffu, want != 0);
-                    if (ok) ok = mbar_wait(&full[s], (n / kChStages) & 1, a.err, 820);
+                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (n / kChStages) & 1, a.err, 820));
                     for (; some; some &= some - 1) {
                         const int x = __ffs(some) - 1;
                         if (!ok || mine++ % PW != pg) continue;
@@ -1312,14 +1361,12 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
                             attend<false, true>(base, qb, st, ((mask >> row0) & 1u) ? rel + row0 : -1,
                                           ((mask >> row1) & 1u) ? rel + row1 : -1, 0, a.sl2e, lane);
                         } else {
-                            // rows that see the whole page go together, one that ends inside it alone
-                            for (uint32_t left = mask; left;) {
-                                const int row = __ffs(left) - 1;
-                                const uint32_t now = rel + row >= kPage - 1 ? left : 1u << row;
-                                left &= ~now;
-                                attend<true, true>(base, qb, st, ((now >> row0) & 1u) ? rel + row : -1,
-                                             ((now >> row1) & 1u) ? rel + row : -1, rel + row, a.sl2e, lane);
-                            }
+                            Careful x;
+                            x.st = st;
+#pragma unroll
+                            for (int kk = 0; kk < 8; ++kk) x.qb[kk][0] = qb[kk][0], x.qb[kk][1] = qb[kk][1];
+                            attend_careful(&x, base, mask, rel, row0, row1, a.sl2e, lane);
+                            st = x.st;
                         }
                     }
                     __syncwarp();
@@ -1328,6 +1375,7 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
             }
             done += stages;
             __syncthreads();
+            for (int i = threadIdx.x; i < 2 * kWin; i += kChThreads) masks[i] = 0;  // of the next window
         }
         float sum = 0.f;  // NaN where a sum is infinite or NaN
 #pragma unroll
@@ -1341,25 +1389,38 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
     __syncwarp();
     cluster_sync_all();
     for (int item = rank * kChThreads + threadIdx.x; item < rows * G * 16; item += CS * kChThreads) {
-        const int tr = (item >> 4) / G, head = (item >> 4) % G, d0 = (item & 15) * 8;
-        const int col = tr / TQ * 8 + tr % TQ * G + head;  // in the first page group
+        const int tr = item >> (4 + lgG), head = (item >> 4) & (G - 1), d0 = (item & 15) * 8;
+        const int col = item >> 4;  // in the first page group: eight a warp, a row's heads together
         float M = kNegInf, L = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (int p = 0; p < PW; ++p)
-            for (int k = 0; k < CS; ++k)
-                M = fmaxf(M, ld_dsmem_f32(mapa_shared(smem_u32(sm + col + p * RW * 8), k)));
-        for (int p = 0; p < PW; ++p)
-            for (int k = 0; k < CS; ++k) {
-                const int at = col + p * RW * 8;
-                const float mk = ld_dsmem_f32(mapa_shared(smem_u32(sm + at), k));
-                const float lk = ld_dsmem_f32(mapa_shared(smem_u32(sl + at), k));
-                const uint32_t src = mapa_shared(smem_u32(mo + at * kPad + d0), k);
-                const float4 u = ld_dsmem_v4(src), v = ld_dsmem_v4(src + 16);
-                if (mk == kNegInf && lk == 0.f) continue;  // saw no key
-                const float sc = exp2f(mk - M);
-                L += lk * sc;
-                acc[0] += u.x * sc; acc[1] += u.y * sc; acc[2] += u.z * sc; acc[3] += u.w * sc;
-                acc[4] += v.x * sc; acc[5] += v.y * sc; acc[6] += v.z * sc; acc[7] += v.w * sc;
+        // part p: page group p / CS of CTA p % CS, four loaded together
+        const int parts = PW * CS, lgCS = 31 - __clz(CS);
+        const auto slot = [&](int p) { return col + (p >> lgCS) * RW * 8; };
+#pragma unroll 4
+        for (int p = 0; p < parts; ++p) M = fmaxf(M, ld_dsmem_f32(mapa_shared(smem_u32(sm + slot(p)), p & (CS - 1))));
+        for (int p0 = 0; p0 < parts; p0 += 4) {
+            float mk[4], lk[4];
+            float4 u[4], v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int p = p0 + e;
+                mk[e] = kNegInf;
+                lk[e] = 0.f;
+                if (p >= parts) continue;
+                mk[e] = ld_dsmem_f32(mapa_shared(smem_u32(sm + slot(p)), p & (CS - 1)));
+                lk[e] = ld_dsmem_f32(mapa_shared(smem_u32(sl + slot(p)), p & (CS - 1)));
+                const uint32_t src = mapa_shared(smem_u32(mo + slot(p) * kPad + d0), p & (CS - 1));
+                u[e] = ld_dsmem_v4(src);
+                v[e] = ld_dsmem_v4(src + 16);
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (mk[e] == kNegInf && lk[e] == 0.f) continue;  // saw no key
+                const float sc = exp2f(mk[e] - M);
+                L += lk[e] * sc;
+                acc[0] += u[e].x * sc; acc[1] += u[e].y * sc; acc[2] += u[e].z * sc; acc[3] += u[e].w * sc;
+                acc[4] += v[e].x * sc; acc[5] += v[e].y * sc; acc[6] += v[e].z * sc; acc[7] += v[e].w * sc;
+            }
+        }
         // an empty list gives a zero row
         *reinterpret_cast<uint4*>(a.out + (static_cast<int64_t>(w.q0 + i0 + tr) * a.hq + h * G + head) * kHd + d0) =
             pack8(acc, L == 0.f ? 0.f : 1.f / L);
