@@ -15,6 +15,7 @@
 // MMAs in fp32, and where the error bound leaves open which page is the k-th, the pages in question
 // are scored again to 2^-46 or better.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "tmap.h"
@@ -1169,26 +1170,9 @@ attend_pages_decode_kernel(const AttArgs a, int num_reqs, int words) {
 // for at the end instead of at every page: a row they reached is NaN from then on, so a tile
 // without NaN or infinite sums was right, and any other is computed again with the masked values
 // kept out (PART of attend).
-struct Careful {
-    Softmax st;
-    uint32_t qb[8][2];
-};
-// Not inlined, and with copies of the state: inlined it costs the loop of ordinary pages 10% (spills).
-__device__ __noinline__ void attend_careful(Careful* x, uint32_t base, uint32_t mask, int rel, int row0, int row1,
-                                            float sl2e, int lane) {
-    // rows that see the whole page go together, one that ends inside it alone
-    for (uint32_t left = mask; left;) {
-        const int row = __ffs(left) - 1;
-        const uint32_t now = rel + row >= kPage - 1 ? left : 1u << row;
-        left &= ~now;
-        attend<true, true>(base, x->qb, x->st, ((now >> row0) & 1u) ? rel + row : -1,
-                           ((now >> row1) & 1u) ? rel + row : -1, rel + row, sl2e, lane);
-    }
-}
-
 constexpr int kChWarps = 16;
 constexpr int kChThreads = (kChWarps + 1) * 32;
-constexpr int kStagePages = 6;
+constexpr int kStagePages = 7;
 constexpr int kChStages = 3;
 constexpr int kStageBytes = kStagePages * 2 * kPadTile;
 constexpr int kWin = 2048;
@@ -1255,7 +1239,10 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
     const int pages = (pos0 + rows - 1) < 0 ? 0 : (pos0 + rows - 1) / kPage + 1;
     bool ok = true;
     int done = 0;  // stages of earlier windows: ring slots and phases run on
-    for (int careful = 0; careful < 2; ++careful) {
+    // One pass over the pages; true where a sum of this CTA is infinite or NaN. Two copies, so that the
+    // registers of the careful one are not those of the other.
+    const auto walk = [&](auto careful) {
+        constexpr bool kCareful = decltype(careful)::value;
         st.clear();
         for (int w0 = 0; w0 < pages; w0 += kWin) {
             // Loads first, each kind together: the table of this thread's run of pages, then ids by fours.
@@ -1288,7 +1275,7 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
                     if (page[e] < 0) continue;
                     const int pos = pos0 + of[e];
                     if (pos < 0 || page[e] > pos / kPage) {
-                        if (w0 == 0 && !careful && rank == 0) record_error(a.err, MSGL_ERR_BOUNDS, 803);
+                        if (w0 == 0 && !kCareful && rank == 0) record_error(a.err, MSGL_ERR_BOUNDS, 803);
                         continue;
                     }
                     if (page[e] >= w0 && page[e] < w0 + kWin)
@@ -1352,21 +1339,23 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
                     if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (n / kChStages) & 1, a.err, 820));
                     for (; some; some &= some - 1) {
                         const int x = __ffs(some) - 1;
-                        if (!ok || mine++ % PW != pg) continue;
+                        if (!ok || (mine++ & (PW - 1)) != pg) continue;
                         const uint32_t mask = __shfl_sync(0xffffffffu, want, x);
                         const uint32_t base = smem_u32(ring) + s * kStageBytes + x * 2 * kPadTile;
                         // the first row's position in the page
                         const int rel = pos0 + wrow - (w0 + __shfl_sync(0xffffffffu, page, x)) * kPage;
-                        if (!careful) {
+                        if constexpr (!kCareful) {
                             attend<false, true>(base, qb, st, ((mask >> row0) & 1u) ? rel + row0 : -1,
                                           ((mask >> row1) & 1u) ? rel + row1 : -1, 0, a.sl2e, lane);
                         } else {
-                            Careful x;
-                            x.st = st;
-#pragma unroll
-                            for (int kk = 0; kk < 8; ++kk) x.qb[kk][0] = qb[kk][0], x.qb[kk][1] = qb[kk][1];
-                            attend_careful(&x, base, mask, rel, row0, row1, a.sl2e, lane);
-                            st = x.st;
+                            // rows that see the whole page go together, one that ends inside it alone
+                            for (uint32_t left = mask; left;) {
+                                const int row = __ffs(left) - 1;
+                                const uint32_t now = rel + row >= kPage - 1 ? left : 1u << row;
+                                left &= ~now;
+                                attend<true, true>(base, qb, st, ((now >> row0) & 1u) ? rel + row : -1,
+                                                   ((now >> row1) & 1u) ? rel + row : -1, rel + row, a.sl2e, lane);
+                            }
                         }
                     }
                     __syncwarp();
@@ -1380,8 +1369,9 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
         float sum = 0.f;  // NaN where a sum is infinite or NaN
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum += 0.f * ((st.o[j][0] + st.o[j][1]) + (st.o[j][2] + st.o[j][3]));
-        if (!__syncthreads_or(sum != sum)) break;  // each CTA for itself
-    }
+        return __syncthreads_or(sum != sum) != 0;
+    };
+    if (walk(std::false_type{})) walk(std::true_type{});  // each CTA for itself
 
     // ---- join the page groups and the cluster's shares, normalise, store
     float* mo = reinterpret_cast<float*>(ring);  // [16 warps][8][kPad]
