@@ -924,14 +924,8 @@ __device__ __forceinline__ void attend(uint32_t base, const uint32_t (&qb)[8][2]
     }
 }
 
-// A warp's state into shared memory: o rows of kPad floats per column, m and l per column.
-constexpr int kPad = kHd + 4;  // the four lanes of a dim fall into different banks
-__device__ __forceinline__ void dump(const Softmax& st, float* o, float* m, float* l, int lane) {
+__device__ __forceinline__ void dump_sums(const Softmax& st, float* m, float* l, int lane) {
     const int g = lane >> 2, c = lane & 3;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[(2 * c + (e & 1)) * kPad + 16 * j + g + (e >> 1) * 8] = st.o[j][e];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         float sum = st.l[r];
@@ -943,6 +937,17 @@ __device__ __forceinline__ void dump(const Softmax& st, float* o, float* m, floa
             l[2 * c + r] = sum;
         }
     }
+}
+
+// A warp's state into shared memory: o rows of kPad floats per column, m and l per column.
+constexpr int kPad = kHd + 4;  // the four lanes of a dim fall into different banks
+__device__ __forceinline__ void dump(const Softmax& st, float* o, float* m, float* l, int lane) {
+    const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[(2 * c + (e & 1)) * kPad + 16 * j + g + (e >> 1) * 8] = st.o[j][e];
+    dump_sums(st, m, l, lane);
 }
 
 // 8 dims of one column joined over `n` dumped states, `step` columns' worth apart: M and L of the
@@ -1253,12 +1258,11 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
             for (int e = 0; e < kRun; ++e)
                 phys[e] = warp < kChWarps && w0 + run0 + e < pages
                               ? a.page_table[static_cast<int64_t>(r) * a.max_pages + w0 + run0 + e] : 0;
-            __syncthreads();  // masks are zero
             const int* ids = a.page_ids + (static_cast<int64_t>(w.q0 + i0) * a.hkv + h) * a.top;
             const int step_row = kChThreads / a.top, step_at = kChThreads % a.top;
             int row = threadIdx.x / a.top, at = threadIdx.x % a.top;
-            while (row < rows) {
-                int page[4], of[4];
+            int page[4], of[4];
+            const auto load = [&] {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     page[e] = row < rows ? ids[static_cast<int64_t>(row) * a.hkv * a.top + at] : -1;
@@ -1270,6 +1274,10 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
                         ++row;
                     }
                 }
+            };
+            load();
+            __syncthreads();  // masks are zero
+            for (;;) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if (page[e] < 0) continue;
@@ -1281,6 +1289,8 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
                     if (page[e] >= w0 && page[e] < w0 + kWin)
                         atomicOr(&masks[(of[e] >> 5) * kWin + page[e] - w0], 1u << (of[e] & 31));
                 }
+                if (row >= rows) break;
+                load();
             }
             __syncthreads();
             uint32_t any[kRun];
@@ -1374,46 +1384,72 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
     if (walk(std::false_type{})) walk(std::true_type{});  // each CTA for itself
 
     // ---- join the page groups and the cluster's shares, normalise, store
-    float* mo = reinterpret_cast<float*>(ring);  // [16 warps][8][kPad]
-    if (warp < kChWarps) dump(st, mo + warp * 8 * kPad, sm + warp * 8, sl + warp * 8, lane);
+    // A warp's state lies lane by lane, 16 bytes per 16 dims. The PW x CS warps of a row group each join
+    // and store a share of the 128 dims, as MMA tiles.
+    float4* mo = reinterpret_cast<float4*>(ring);  // [16 warps][8][32 lanes]
+    if (warp < kChWarps) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            mo[(warp * 8 + j) * 32 + lane] = make_float4(st.o[j][0], st.o[j][1], st.o[j][2], st.o[j][3]);
+        dump_sums(st, sm + warp * 8, sl + warp * 8, lane);
+    }
     __syncwarp();
     cluster_sync_all();
-    for (int item = rank * kChThreads + threadIdx.x; item < rows * G * 16; item += CS * kChThreads) {
-        const int tr = item >> (4 + lgG), head = (item >> 4) & (G - 1), d0 = (item & 15) * 8;
-        const int col = item >> 4;  // in the first page group: eight a warp, a row's heads together
-        float M = kNegInf, L = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        // part p: page group p / CS of CTA p % CS, four loaded together
-        const int parts = PW * CS, lgCS = 31 - __clz(CS);
-        const auto slot = [&](int p) { return col + (p >> lgCS) * RW * 8; };
+    const int parts = PW * CS, lgCS = 31 - __clz(CS);  // part p: page group p / CS of CTA p % CS
+    const int self = pg * CS + rank, j0 = 8 * self / parts, j1 = 8 * (self + 1) / parts;
+    if (warp < kChWarps && j0 < j1) {
+        const auto at = [&](const void* x, int p) { return mapa_shared(smem_u32(x), p & (CS - 1)); };
+        float M[2] = {kNegInf, kNegInf}, L[2] = {0.f, 0.f};
 #pragma unroll 4
-        for (int p = 0; p < parts; ++p) M = fmaxf(M, ld_dsmem_f32(mapa_shared(smem_u32(sm + slot(p)), p & (CS - 1))));
-        for (int p0 = 0; p0 < parts; p0 += 4) {
-            float mk[4], lk[4];
-            float4 u[4], v[4];
+        for (int p = 0; p < parts; ++p) {
+            const int col = ((p >> lgCS) * RW + rg) * 8 + 2 * c;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int p = p0 + e;
-                mk[e] = kNegInf;
-                lk[e] = 0.f;
-                if (p >= parts) continue;
-                mk[e] = ld_dsmem_f32(mapa_shared(smem_u32(sm + slot(p)), p & (CS - 1)));
-                lk[e] = ld_dsmem_f32(mapa_shared(smem_u32(sl + slot(p)), p & (CS - 1)));
-                const uint32_t src = mapa_shared(smem_u32(mo + slot(p) * kPad + d0), p & (CS - 1));
-                u[e] = ld_dsmem_v4(src);
-                v[e] = ld_dsmem_v4(src + 16);
+            for (int k = 0; k < 2; ++k) M[k] = fmaxf(M[k], ld_dsmem_f32(at(sm + col + k, p)));
+        }
+        const int tr = wrow + (g >> lgG);  // of column g, which this lane stores
+        uint32_t* out = reinterpret_cast<uint32_t*>(
+            a.out + (static_cast<int64_t>(w.q0 + i0 + tr) * a.hq + h * G + (g & (G - 1))) * kHd);
+        float acc[8][4];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) acc[x][0] = acc[x][1] = acc[x][2] = acc[x][3] = 0.f;
+        for (int p = 0; p < parts; ++p) {  // a part's loads together
+            const int from = (p >> lgCS) * RW + rg, col = from * 8 + 2 * c;
+            float mk[2], lk[2];
+            float4 o[8];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                mk[k] = ld_dsmem_f32(at(sm + col + k, p));
+                lk[k] = ld_dsmem_f32(at(sl + col + k, p));
             }
+            const uint32_t src = at(mo + (from * 8 + j0) * 32 + lane, p);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (mk[e] == kNegInf && lk[e] == 0.f) continue;  // saw no key
-                const float sc = exp2f(mk[e] - M);
-                L += lk[e] * sc;
-                acc[0] += u[e].x * sc; acc[1] += u[e].y * sc; acc[2] += u[e].z * sc; acc[3] += u[e].w * sc;
-                acc[4] += v[e].x * sc; acc[5] += v[e].y * sc; acc[6] += v[e].z * sc; acc[7] += v[e].w * sc;
+            for (int x = 0; x < 8; ++x)
+                if (j0 + x < j1) o[x] = ld_dsmem_v4(src + x * 32 * 16);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                if (mk[k] == kNegInf && lk[k] == 0.f) continue;  // saw no key
+                const float sc = exp2f(mk[k] - M[k]);
+                L[k] += lk[k] * sc;
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    if (j0 + x >= j1) continue;
+                    acc[x][k] += (k ? o[x].y : o[x].x) * sc;
+                    acc[x][2 + k] += (k ? o[x].w : o[x].z) * sc;
+                }
             }
         }
         // an empty list gives a zero row
-        *reinterpret_cast<uint4*>(a.out + (static_cast<int64_t>(w.q0 + i0 + tr) * a.hq + h * G + head) * kHd + d0) =
-            pack8(acc, L == 0.f ? 0.f : 1.f / L);
+        const float f0 = L[0] == 0.f ? 0.f : 1.f / L[0], f1 = L[1] == 0.f ? 0.f : 1.f / L[1];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            if (j0 + x >= j1) break;
+            const uint32_t lo = transpose8x8(pack_bf16x2(acc[x][0] * f0, acc[x][1] * f1));
+            const uint32_t hi = transpose8x8(pack_bf16x2(acc[x][2] * f0, acc[x][3] * f1));
+            if (tr < rows) {  // dims 16 j + 2 c, + 1 and those 8 further of column g
+                out[8 * (j0 + x) + c] = lo;
+                out[8 * (j0 + x) + 4 + c] = hi;
+            }
+        }
     }
     __syncwarp();
     cluster_sync_all();  // no CTA leaves while another reads its shared memory
