@@ -978,9 +978,9 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8], float f) {
 
 // ---- single rows: decode, and short chunks
 // Lists attended one by one, also in chunks whose tiles would be half empty or too few (kRowsAlone
-// rows a request, kTotalAlone rows in all): selection and attention of 8 requests x 5 / 33 / 65 rows (32
-// heads, 64 of 512 pages) take 34 / 119 / 213 us this way and 61 / 150 / 197 in tiles, of 1 x 129 / 513
-// rows 85 / 245 and 114 / 193.
+// rows a request, kTotalAlone rows in all): selection and attention of 8 requests x 17 / 33 / 65 rows (32
+// heads, 64 of 512 pages) take 84 / 119 / 213 us this way and 88 / 130 / 161 in tiles, of 1 x 129 / 513
+// rows 86 / 245 and 93 / 158.
 // A cluster of up to 16 CTAs (decode_split) per (query row, kv head): each CTA
 // takes a share of the listed pages, its four warps take its pages in turn, every warp with a ring
 // of its own (cp.async, 16 bytes a lane, three pages) and an online softmax. The warps' results are
@@ -1165,11 +1165,15 @@ attend_pages_decode_kernel(const AttArgs a, int num_reqs, int words) {
 // of that many. A cluster of CTAs (chunk_split) shares a tile: each takes a share of every window's
 // list, and the partial results are joined through distributed shared memory.
 //
-// Bound by the TMA boxes: without the products the loads alone take 260 of 435 us (1.3k rows of 32
-// heads over 64 pages each, 126k page loads of 8 KB). Slower ways to bring the same pages: cp.async
-// from producer warps 575 us (it shares the path of the fragment loads), bulk copies of single rows
-// 1315 us, K by TMA and V by cp.async 497 us, tiles of 16 rows on two CTAs per SM 565 us. Stages of
-// 2 / 4 / 6 / 10 pages (of 20 in the ring): selection and attention 661 / 586 / 571 / 568 us.
+// Bound by shared memory: a warp's fragments of a page are 8 KB, 64 cycles of its port, and 5.3 of the
+// 16 row groups want a page; with the write of the page 410 cycles, of 525 that a page takes (1.3k
+// rows of 32 heads over 64 pages each, 126k page loads: 335 us; a CTA's list and join are 10 of 65 us).
+// A box is 16 rows of kPadRow bytes, wider than the tensor's rows: the rest is filled with zeros, which
+// pads the rows. Boxes of swizzled half rows of 128 bytes took 225 cycles of the copy engine each and
+// 30 us more in all. Slower ways to bring the same pages: cp.async from producer warps (it shares the
+// path of the fragment loads), bulk copies of single rows, K by TMA and V by cp.async, tiles of 16
+// rows on two CTAs per SM; 16 warps, the last to leave a stage filling it again, in place of the
+// producer: 554 against 528 us.
 //
 // A masked weight is zero, but zero times a NaN or infinite value is NaN. Such values are looked
 // for at the end instead of at every page: a row they reached is NaN from then on, so a tile
@@ -1486,16 +1490,18 @@ int decode_split(int64_t lists, int top) {
 }
 
 // CTAs that share a tile of a chunk (up to 4): one SM holds one, and the rounds of 148 should be full.
-// A share costs a list and a join of its own, so it has to gain a sixth: 16 tiles of 64 rows take 159
-// us alone, 69 in fours; 344 tiles 604 and 589 in twos; 256 tiles 148 and 182 in twos.
+// A share costs a list and a join of its own, about a tenth of a tile's time in twos and a third in
+// fours. Selection and attention with tiles alone / in twos / in fours: 16 tiles 121 / 80 / 57 us, 136
+// tiles 158 / 170 / 207, 344 tiles 487 / 478 / 600.
 int chunk_split(int64_t tiles) {
-    const auto fill = [&](int s) {
-        const int64_t ctas = tiles * s, rounds = (ctas + 147) / 148;
-        return static_cast<double>(ctas) / (148 * rounds);
-    };
+    const double gain[3] = {1.0, 0.9, 0.63};
     int best = 1;
-    for (int s = 2; s <= 4; s *= 2)
-        if (fill(s) > 1.17 * fill(best)) best = s;
+    double most = 0.0;
+    for (int k = 0; k < 3; ++k) {
+        const int64_t ctas = tiles << k, rounds = (ctas + 147) / 148;
+        const double v = gain[k] * static_cast<double>(ctas) / static_cast<double>(148 * rounds);
+        if (v > most) most = v, best = 1 << k;
+    }
     return best;
 }
 
