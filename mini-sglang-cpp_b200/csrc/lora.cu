@@ -353,6 +353,7 @@ lora_shrink_kernel(const LoraArgs a, int terms) {
     const int s_lo = static_cast<int>(static_cast<int64_t>(steps) * rank_c / S);
     const int s_n = static_cast<int>(static_cast<int64_t>(steps) * (rank_c + 1) / S) - s_lo;
     const __nv_bfloat16* wa = a.a + static_cast<int64_t>(lt.adapter) * a.R * a.K;
+    const float scale = a.scales[lt.adapter];
     const auto issue = [&](int i) {
         const uint32_t dst = smem_u32(ring) + (i % kShStages) * kStage;
         const int k0 = (s_lo + i) * kBK;
@@ -408,7 +409,6 @@ lora_shrink_kernel(const LoraArgs a, int terms) {
         *reinterpret_cast<float2*>(p + 8 * R16) = make_float2(acc[j][2], acc[j][3]);
     }
     cluster_sync_all();
-    const float scale = a.scales[lt.adapter];
     for (int i = rank_c + S * static_cast<int>(threadIdx.x); i < lt.rows * R16 / 4; i += S * kLoraWarps * 32) {
         const uint32_t src = smem_u32(sums + 4 * i);
         float v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -432,8 +432,8 @@ lora_shrink_kernel(const LoraArgs a, int terms) {
 
 // One CTA per 64 rows and 256 columns; four warps of 32 rows x 128 columns, in blocks of 32 columns
 // whose MMA column tiles interleave as in lora_small_kernel. B (rows of R16, its rows of a column
-// tile next to each other) is loaded before the wait for the previous kernel -- it is a weight, and
-// every kernel before `shrink` has completed once `shrink` runs; h comes behind it.
+// tile next to each other) and the first block of y are loaded before the wait for the previous kernel:
+// every kernel before `shrink` has completed once `shrink` runs. h comes behind it.
 template <int KK, bool PARTIAL>
 __global__ void __launch_bounds__(kLoraWarps * 32, KK == 8 ? 3 : 4)
 lora_expand_kernel(const LoraArgs a, int n_slices) {
@@ -465,20 +465,6 @@ lora_expand_kernel(const LoraArgs a, int n_slices) {
             cp_async16(bs + swizzle(row, piece), wb + (in ? static_cast<int64_t>(n0 + n) * a.R + piece * 8 : 0), in);
         }
     }
-    pdl_wait();
-    pdl_trigger();
-    if (!PARTIAL && !some && a.out == a.y) return;  // in place: nothing to add
-    if (some) {
-#pragma unroll
-        for (int m = 0; m < TERMS; ++m)
-            for (int p = threadIdx.x; p < kTile * PIECES; p += kLoraWarps * 32) {
-                const int row = p / PIECES, piece = p % PIECES;
-                const bool in = row < lt.rows;
-                cp_async16(hs + m * kTile * R16 * 2 + swizzle(row, piece),
-                           a.h + h_terms(a.T, R16, m) + (in ? static_cast<int64_t>(lt.t0 + row) * R16 + piece * 8 : 0), in);
-            }
-    }
-    cp_async_commit();
     const int row0 = (warp & 1) * 32, blk0 = (warp >> 1) * 4;
     bool live[2][2];
     int64_t t[2][2];
@@ -502,6 +488,20 @@ lora_expand_kernel(const LoraArgs a, int n_slices) {
                                        : make_uint4(0, 0, 0, 0);
     };
     if (!PARTIAL) load_y(0);
+    pdl_wait();
+    pdl_trigger();
+    if (!PARTIAL && !some && a.out == a.y) return;  // in place: nothing to add
+    if (some) {
+#pragma unroll
+        for (int m = 0; m < TERMS; ++m)
+            for (int p = threadIdx.x; p < kTile * PIECES; p += kLoraWarps * 32) {
+                const int row = p / PIECES, piece = p % PIECES;
+                const bool in = row < lt.rows;
+                cp_async16(hs + m * kTile * R16 * 2 + swizzle(row, piece),
+                           a.h + h_terms(a.T, R16, m) + (in ? static_cast<int64_t>(lt.t0 + row) * R16 + piece * 8 : 0), in);
+            }
+    }
+    cp_async_commit();
     cp_async_wait<0>();
     __syncthreads();
     const int mi = lane >> 3, l7 = lane & 7;
