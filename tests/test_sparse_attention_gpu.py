@@ -261,6 +261,19 @@ def test_attention_over_selected_pages(cuda, lens, q_lens, hq, hkv, top):
     assert ops.device_error() == (0, 0)
 
 
+@pytest.mark.parametrize("n,m,hq,hkv", [(900, 800, 8, 1), (500, 400, 8, 8), (600, 512, 16, 16), (700, 290, 4, 4)])
+def test_tiles_shared_by_ctas(cuda, n, m, hq, hkv):
+    """Tiles of one CTA, of two and of four, with one and two groups of pages among a CTA's warps."""
+    from msgl import ops
+    b = Batch([n], [m], hq, hkv, seed=31)
+    b.all_bounds(ops)
+    ids = b.select(ops, 9, 1, 1)
+    out = b.attend(ops, ids)
+    close(out, *b.ref_attend(ids))
+    assert torch.equal(out, b.attend(ops, ids))
+    assert ops.device_error() == (0, 0)
+
+
 @pytest.mark.parametrize("q_lens", [[1, 1, 1], [40, 7, 90], [220, 33, 40]])
 @pytest.mark.parametrize("hq,hkv", [(8, 8), (8, 4), (16, 4), (16, 2)])
 def test_attention_over_any_lists(cuda, q_lens, hq, hkv):
