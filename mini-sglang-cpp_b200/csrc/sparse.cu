@@ -1497,9 +1497,9 @@ int check_heads(int hq, int hkv, int head_dim, int page_size) {
 int pages_of(int tokens) { return tokens / kPage + (tokens % kPage != 0); }
 
 // Query rows of one launch pair: as many as keep the workspace (16 bytes per row, kv head and
-// page) within 128 MB, so that the scores (a quarter of it) stay in L2 until they are read; at
-// least 16.
-constexpr int64_t kSelectBytes = int64_t(128) << 20;
+// page) within 256 MB, so that the scores (a quarter of it) stay in L2 until they are read; at
+// least 16. (1.3k rows of 1024 pages: 479 us in two passes of 128 MB, 465 in one.)
+constexpr int64_t kSelectBytes = int64_t(256) << 20;
 int slab_rows(int total_q, int stride, int hkv) {
     const int64_t rows = std::max<int64_t>(16, kSelectBytes / (int64_t(16) * stride * hkv));
     return static_cast<int>(std::min<int64_t>(total_q, rows));

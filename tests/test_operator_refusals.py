@@ -87,7 +87,7 @@ def test_select_empty_and_workspace():
     # 16 bytes for each of 64 rows x 8 heads x 2048 pages
     assert L.msgl_select_pages_workspace_size(64, 32768, 8) == 16 * 64 * 8 * 2048
     # bounded for long batches
-    assert L.msgl_select_pages_workspace_size(100000, 32768, 8) == 128 * 2 ** 20
+    assert L.msgl_select_pages_workspace_size(100000, 32768, 8) == 256 * 2 ** 20
 
 
 def attend(**k):

@@ -225,11 +225,11 @@ def test_selection_ties_and_extremes(cuda, kind, pages, q_len):
 
 
 def test_selection_in_several_passes(cuda):
-    """More query rows than one pass holds (128 MB: 512 rows of 2048 pages, 8 heads)."""
+    """More query rows than one pass holds (256 MB: 1024 rows of 2048 pages, 8 heads)."""
     from msgl import ops
     b = Batch([32768], [1500], 8, 8, seed=5)
     b.all_bounds(ops)
-    assert ops.select_pages_workspace(1500, 32768, 8).numel() == 128 * 2 ** 20
+    assert ops.select_pages_workspace(1500, 32768, 8).numel() == 256 * 2 ** 20
     ids = b.select(ops, 20, 1, 1).cpu()
     # every row by a product per head in 64 bits
     pos = 32768 - 1500 + torch.arange(1500, device="cuda")
