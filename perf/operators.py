@@ -34,18 +34,13 @@ def _device():
     return "cuda" if torch.cuda.is_available() else "cpu"
 
 
-_loaded = None
-
-
 def _ops():
-    """msgl.ops, imported once as a program does."""
-    global _loaded
-    if _loaded is None:
-        root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-        sys.path.insert(0, os.path.join(root, "mini-sglang-cpp_b200"))
-        from msgl import ops
-        _loaded = ops
-    return _loaded
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    path = os.path.join(root, "mini-sglang-cpp_b200")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from msgl import ops
+    return ops
 
 
 # ------------------------------------------------------------------ cases
