@@ -157,7 +157,7 @@ struct SelectArgs {
     int t0, t1;        // query rows of this launch
     int stride;        // pages per score row
     float* scores;             // [rows][Hkv][stride]
-    float* mags;               // [rows][Hkv][stride / 16]: in the request's first row
+    float* mags;               // [rows][Hkv][stride / 16]: in the request's first row of the launch
     unsigned long long* wide;  // [rows][Hkv][stride]: keys beyond fp32 where many scores are close
     int* page_ids;
     int* err;
@@ -204,6 +204,11 @@ page_scores_kernel(const SelectArgs a, int tiles, int page_tiles, int groups) {
     if (w.q0 < 0 || i0 >= i1) return;
     const int seen = (w.L - w.qn + i1 - 1) >> 4;  // pages before the last row's own page
     const int last = seen + 1 - a.recent;         // pages [sink, last) are scored
+    // Pages up to those that the request's last row of this launch scores take part in the magnitudes:
+    // every tile then finds the same for a group of pages that its own end cuts, and whichever of them
+    // stores it last, no row works with a smaller one than its pages have.
+    const int rows_end = min(min(w.qn, a.max_q_len), a.t1 - w.q0);
+    const int cover = ((w.L - w.qn + rows_end - 1) >> 4) + 1 - a.recent;
     if (seen + 1 <= a.top) return;                // every row of the tile sees all its pages
     const int end = min(last, (pt + 1) * groups * kScorePages);
     int pg0 = pt * groups * kScorePages;
@@ -226,13 +231,13 @@ page_scores_kernel(const SelectArgs a, int tiles, int page_tiles, int groups) {
     const int* table = a.page_table + static_cast<int64_t>(r) * a.max_pages;
     int next[2];  // physical pages of the next group
 #pragma unroll
-    for (int u = 0; u < 2; ++u) next[u] = pg0 + g + 8 * u < last ? table[pg0 + g + 8 * u] : -1;
+    for (int u = 0; u < 2; ++u) next[u] = pg0 + g + 8 * u < cover ? table[pg0 + g + 8 * u] : -1;
     do {
         uint32_t af[8][2][4];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             int phys = next[u];
-            if (pg0 + g + 8 * u < last && static_cast<unsigned>(phys) >= static_cast<unsigned>(a.pool_pages)) {
+            if (pg0 + g + 8 * u < cover && static_cast<unsigned>(phys) >= static_cast<unsigned>(a.pool_pages)) {
                 record_error(a.err, MSGL_ERR_BOUNDS, 802);
                 phys = -1;
             }
@@ -248,7 +253,7 @@ page_scores_kernel(const SelectArgs a, int tiles, int page_tiles, int groups) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int page = pg0 + kScorePages + g + 8 * u;
-                next[u] = page < end ? table[page] : -1;
+                next[u] = page < end ? table[page] : -1;  // (one row: cover is last)
             }
         }
         {   // largest 2-norm of max(|lo|, |hi|) among the 16 pages: what the scores' error scales with

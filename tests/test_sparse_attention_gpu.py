@@ -224,6 +224,30 @@ def test_selection_ties_and_extremes(cuda, kind, pages, q_len):
     assert ops.device_error() == (0, 0)
 
 
+@pytest.mark.parametrize("times", [1e3, 1e36])
+@pytest.mark.parametrize("n,m,hq,hkv", [(3200, 330, 8, 2), (16384, 512, 8, 2), (5000, 700, 4, 4), (3200, 300, 8, 1)])
+def test_large_bounds_at_the_newest_pages(cuda, times, n, m, hq, hkv):
+    """Near scores of a few pages whose bounds are much larger than the others', behind what the chunk's
+    earlier rows see: their rows tell them apart by their own magnitude, whichever tile of rows was
+    scored last."""
+    from msgl import ops
+    b = Batch([n], [m], hq, hkv, seed=33)
+    b.all_bounds(ops)
+    pages = b.page_table[0].long()
+    end = (n - 1) // PAGE + 1
+    # one element apart by a last place of a small bound
+    large = pages[end - 18:end - 3]
+    b.bounds[large] = (b.bounds[pages[0]].float() * times).bfloat16()
+    last_place = torch.randint(0, 128, (15, hkv, 1), generator=b.g, device="cuda") / 128
+    b.bounds[large, :, :, 17] = (times / 131072 * (1 + last_place)).bfloat16()
+    if times > 1e30:
+        b.q.mul_(1e3)  # products beyond fp32
+    ref = b.ref_select(6, 1, 2)
+    for _ in range(5):
+        assert torch.equal(b.select(ops, 6, 1, 2).cpu(), ref)
+    assert ops.device_error() == (0, 0)
+
+
 def test_selection_in_several_passes(cuda):
     """More query rows than one pass holds (256 MB: 1024 rows of 2048 pages, 8 heads)."""
     from msgl import ops
