@@ -48,6 +48,12 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
     return *reinterpret_cast<uint32_t*>(&h);
 }
 
+// Two bf16 values, zero where infinite or NaN.
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {
+    const uint32_t a = w & 0x7fff7fffu, most = 0x7f7f7f7fu;
+    return w & __hle2_mask(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&most));
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

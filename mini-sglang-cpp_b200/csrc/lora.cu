@@ -17,11 +17,11 @@
 //  * Longer chunks: `shrink` writes h, `expand` reads it. Both take 64 rows of one request a CTA and
 //    bring what several warps share (A, x, B, h) into shared memory.
 //
-// h is summed in fp32. For the fp32 partial it enters the second product as three bf16 terms (2^-25
-// relative). For the bf16 result decode takes two (2^-17), where they cost nothing; chunks round it
-// to bf16, as the projections around it round their activations: h's rounding (2^-9 of each of the
-// rank's terms, of either sign) stays below that of the result, and the MMAs of a second term took
-// as long as the streams (rank 64, 4.5k rows: 53 against 50 us).
+// h is summed in fp32. For the fp32 partial it enters the second product as three bf16 terms (what is
+// left of h: 2^-24 of it), for the bf16 result as two (2^-16). One term (2^-8 of each of the rank's h)
+// is not enough: the result is off by as much of sum |B h|, which where those terms cancel, or cancel
+// y, is far more than the rounding of the result itself. (4.5k rows, 4096 -> 6144, on the device: 43 us
+// with one term and 50 with two at rank 64, 65 and 79 at rank 128, no difference at rank 16.)
 #include <algorithm>
 
 #include "common.cuh"
@@ -437,7 +437,7 @@ lora_shrink_kernel(const LoraArgs a, int terms) {
 template <int KK, bool PARTIAL>
 __global__ void __launch_bounds__(kLoraWarps * 32, KK == 8 ? 3 : 4)
 lora_expand_kernel(const LoraArgs a, int n_slices) {
-    constexpr int R16 = 16 * KK, PIECES = 2 * KK, TERMS = PARTIAL ? 3 : 1;
+    constexpr int R16 = 16 * KK, PIECES = 2 * KK, TERMS = PARTIAL ? 3 : 2;
     constexpr int kSwz = KK == 1 ? 2 : KK == 2 ? 1 : 0, kMask = (PIECES < 8 ? PIECES : 8) - 1;
     extern __shared__ __align__(128) uint8_t smem[];
     const uint32_t bs = smem_u32(smem), hs = bs + kNSlice * R16 * 2;
@@ -505,7 +505,8 @@ lora_expand_kernel(const LoraArgs a, int n_slices) {
     cp_async_wait<0>();
     __syncthreads();
     const int mi = lane >> 3, l7 = lane & 7;
-    uint32_t hf[PARTIAL ? 1 : KK][TERMS][2][4];  // all of h where it is one term
+    constexpr bool kHold = !PARTIAL && KK <= 2;  // all of h in registers (of more ranks: 488 bytes spill, 50 -> 52 us)
+    uint32_t hf[kHold ? KK : 1][TERMS][2][4];
     const auto load_h = [&](int kk, uint32_t (&f)[TERMS][2][4]) {
 #pragma unroll
         for (int m = 0; m < TERMS; ++m)
@@ -516,9 +517,9 @@ lora_expand_kernel(const LoraArgs a, int n_slices) {
                         f[m][mt][2], f[m][mt][3]);
             }
     };
-    if (!PARTIAL && some) {
+    if (kHold && some) {
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) load_h(kk, hf[PARTIAL ? 0 : kk]);
+        for (int kk = 0; kk < KK; ++kk) load_h(kk, hf[kHold ? kk : 0]);
     }
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
@@ -537,15 +538,21 @@ lora_expand_kernel(const LoraArgs a, int n_slices) {
                     const int row = (blk0 + b) * 32 + (j + (mi >> 1)) * 8 + l7;
                     ldsm_x4(bs + swizzle(row, 2 * kk + (mi & 1)), w[j][0], w[j][1], w[j + 1][0], w[j + 1][1]);
                 }
-                if (PARTIAL) load_h(kk, hf[0]);
-                const auto& f = hf[PARTIAL ? 0 : kk];
+                if (!kHold) load_h(kk, hf[0]);
+                const auto& f = hf[kHold ? kk : 0];
+                // What is left of an h that is a bf16 value is zero, and zero times an infinite weight
+                // would be NaN: those take part through the first term alone.
+                uint32_t wf[4][2];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) wf[j][0] = finite2(w[j][0]), wf[j][1] = finite2(w[j][1]);
 #pragma unroll
                 for (int m = TERMS - 1; m >= 0; --m)
 #pragma unroll
                     for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            mma_bf16_16816(acc[mt][j], f[m][mt][0], f[m][mt][1], f[m][mt][2], f[m][mt][3], w[j][0], w[j][1]);
+                            mma_bf16_16816(acc[mt][j], f[m][mt][0], f[m][mt][1], f[m][mt][2], f[m][mt][3],
+                                           m ? wf[j][0] : w[j][0], m ? wf[j][1] : w[j][1]);
             }
         }
         const int col = n0 + (blk0 + b) * 32 + 8 * c;
@@ -593,10 +600,10 @@ cudaError_t launch_chunks(const LoraArgs& a, int64_t row_tiles, int splits, cuda
     const size_t sh = size_t(sh_stages(KK)) * (kTile + 16 * KK) * kBK * 2;
     cudaError_t e = smem_optin(lora_shrink_kernel<KK>, sh, optin[0]);
     if (e != cudaSuccess) return e;
-    const size_t ex = size_t(kNSlice + (PARTIAL ? 3 : 1) * kTile) * 16 * KK * 2;
+    const size_t ex = size_t(kNSlice + (PARTIAL ? 3 : 2) * kTile) * 16 * KK * 2;
     e = smem_optin(lora_expand_kernel<KK, PARTIAL>, ex, optin[1]);
     if (e != cudaSuccess) return e;
-    e = launch_cluster(lora_shrink_kernel<KK>, row_tiles * splits, splits, sh, stream, a, PARTIAL ? 3 : 1);
+    e = launch_cluster(lora_shrink_kernel<KK>, row_tiles * splits, splits, sh, stream, a, PARTIAL ? 3 : 2);
     if (e != cudaSuccess) return e;
     const int n_slices = (a.N + kNSlice - 1) / kNSlice;
     return launch_pdl(lora_expand_kernel<KK, PARTIAL>, dim3(static_cast<unsigned>(row_tiles * n_slices)),

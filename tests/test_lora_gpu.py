@@ -95,6 +95,28 @@ def test_against_formula(cuda, lens, K, N, R, n, none):
     assert ops.device_error() == (0, 0)
 
 
+@pytest.mark.parametrize("lens", [[1] * 20, [9, 16], [17, 40], [90, 200, 1]])
+@pytest.mark.parametrize("R", [16, 24, 64, 128])
+def test_cancelling_ranks(cuda, lens, R):
+    """Ranks in pairs whose terms nearly cancel, and cancel y: what h is rounded by shows in the result.
+    Two bf16 terms leave 2^-16 of each h, 2^-16 of H in all, however many rows a request has."""
+    from msgl import ops
+    K, N = 64, 264
+    x, a, b, sc, ids, _, indptr = make(lens, K, N, R, 3, seed=R)
+    a[:, 1::2] = (a[:, ::2].float() * (1 + 2 ** -6)).bfloat16()
+    b[:, :, 1::2] = -b[:, :, ::2]
+    d, mag = reference(x, a, b, sc, ids, lens)
+    H = torch.cat([sc[r].double() * (X @ a[r].double().T).abs() @ b[r].double().abs().T
+                   for r, X in zip(ids.tolist(), x.double().split(lens))])
+    y = (-d).bfloat16()
+    for _y in (torch.zeros_like(y), y):
+        ref = _y.double() + d
+        out = ops.lora_add(x, a, b, sc, ids, _y, q_indptr=indptr, max_q_len=max(lens))
+        tol = ref.abs() * 2 ** -8 + mag * steps(K, R) + H * 2 ** -16 + _y.double().abs() * 2 ** -23
+        assert bool(((out.double() - ref).abs() <= tol).all()), float(((out.double() - ref).abs() / tol).max())
+    assert ops.device_error() == (0, 0)
+
+
 def test_strided_rows_and_rows_behind_the_last_request(cuda):
     """A column range of a fused projection, x as a column range, and padding rows."""
     from msgl import ops
