@@ -505,7 +505,7 @@ lora_expand_kernel(const LoraArgs a, int n_slices) {
     cp_async_wait<0>();
     __syncthreads();
     const int mi = lane >> 3, l7 = lane & 7;
-    constexpr bool kHold = !PARTIAL && KK <= 2;  // all of h in registers (of more ranks: 488 bytes spill, 50 -> 52 us)
+    constexpr bool kHold = !PARTIAL && KK <= 2;  // h in registers; of 64 ranks that leaves three CTAs an SM: 50 -> 52 us
     uint32_t hf[kHold ? KK : 1][TERMS][2][4];
     const auto load_h = [&](int kk, uint32_t (&f)[TERMS][2][4]) {
 #pragma unroll
