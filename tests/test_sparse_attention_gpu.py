@@ -285,6 +285,53 @@ def test_attention_over_selected_pages(cuda, lens, q_lens, hq, hkv, top):
     assert ops.device_error() == (0, 0)
 
 
+@pytest.mark.parametrize("m", [1, 30, 300])
+@pytest.mark.parametrize("hq,hkv", [(4, 4), (8, 2), (8, 1)])
+def test_cancelling_values(cuda, m, hq, hkv):
+    """Values that nearly cancel over keys of much the same weight: what the weights are rounded by
+    shows in the result. Two bf16 terms leave 2^-16 of each; fp32 scores and exp2 as above (size +
+    2^-18), and the sums over n keys are off by at most 2^-22 of their magnitude a step of 16 products,
+    two such steps (terms) a page, and as much again for the joins of up to 64 parts."""
+    from msgl import ops
+    n, top = 400 + m, 6
+    b = Batch([n], [m], hq, hkv, seed=35)
+    b.q.mul_(0.125)
+    slots = (b.page_table[0].long()[:, None] * PAGE + torch.arange(PAGE, device="cuda")).view(-1)[:n]
+    v = b.v[slots]
+    v[1::2] = -v[:n // 2 * 2:2]
+    b.v[slots] = v
+    b.all_bounds(ops)
+    ids = b.select(ops, top, 1, 2)
+    ref, tol = b.ref_attend(ids)
+    weight = (tol - ref.abs() * 2 ** -8)                 # (2^-8 + size + 2^-18) sum p |v|
+    keys = b.k[slots].view(n, hkv, D).double().abs()
+    size = max(float((b.q[:, h * hq // hkv:(h + 1) * hq // hkv].double().abs() @ keys[:, h].T).amax())
+               for h in range(hkv)) * D ** -0.5 * 2 ** -18
+    fine = (2 ** -16 + size + 2 ** -18 + (2 * top + 64) * 2 ** -22) / 2 ** -8
+    close(b.attend(ops, ids), ref, ref.abs() * 2 ** -8 + weight * fine)
+    assert ops.device_error() == (0, 0)
+
+
+@pytest.mark.parametrize("m", [1, 30, 300])
+def test_infinite_values_that_rows_see(cuda, m):
+    """An infinite value gives infinities of its sign in its dimension to every row that lists its page,
+    and nothing to the others."""
+    from msgl import ops
+    n = 200 + m
+    b = Batch([n], [m], 8, 2, seed=36)
+    ids = torch.tensor([0, 3, 5], dtype=torch.int32, device="cuda").repeat(m, 2, 1)
+    ids[1::2, :, 1] = 4
+    slot = int(b.page_table[0, 3]) * PAGE + 7
+    ref, tol = b.ref_attend(ids)
+    b.v[slot, 9], b.v[slot, 128 + 40] = INF, -INF
+    out = b.attend(ops, ids).double()
+    hit = torch.arange(m, device="cuda") % 2 == 0
+    assert bool((out[hit, :4, 9] == INF).all()) and bool((out[hit, 4:, 40] == -INF).all())
+    at = torch.zeros_like(out, dtype=torch.bool)
+    at[hit, :4, 9], at[hit, 4:, 40] = True, True
+    close(out[~at], ref[~at], tol[~at])
+
+
 @pytest.mark.parametrize("n,m,hq,hkv", [(900, 800, 8, 1), (500, 400, 8, 8), (600, 512, 16, 16), (700, 290, 4, 4)])
 def test_tiles_shared_by_ctas(cuda, n, m, hq, hkv):
     """Tiles of one CTA, of two and of four, with one and two groups of pages among a CTA's warps."""
