@@ -16,6 +16,7 @@
 #include <utility>
 
 #include "../../include/msgl_kernels.h"
+#include "raise_limit.h"
 
 namespace msgl {
 
@@ -488,23 +489,17 @@ cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t s
 // ------------------------------------------------------------ dynamic shared memory opt-in
 // cudaFuncSetAttribute(MaxDynamicSharedMemorySize) applies to the CURRENT device only, so a
 // process that drives several GPUs must opt a kernel in on each of them. `done` (one static
-// array per kernel) records per device the largest size already granted; the check is a
-// lock-free load, and two host threads racing on a first call both set the same attribute.
+// array per kernel) records per device the largest size already granted.
 constexpr int kMaxDevices = 64;
 template <typename... KArgs>
 cudaError_t smem_optin(void (*kernel)(KArgs...), size_t bytes, std::atomic<int> (&done)[kMaxDevices]) {
     int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+    const cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    const int want = static_cast<int>(bytes);
-    const bool cached = dev >= 0 && dev < kMaxDevices;
-    if (cached && done[dev].load(std::memory_order_acquire) >= want) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, want);
-    if (e == cudaSuccess && cached) {
-        int prev = done[dev].load(std::memory_order_relaxed);
-        while (prev < want && !done[dev].compare_exchange_weak(prev, want)) {
-        }
-    }
-    return e;
+    const auto set = [&](int want) {
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, want);
+    };
+    if (dev < 0 || dev >= kMaxDevices) return set(static_cast<int>(bytes));
+    return raise_limit(done[dev], static_cast<int>(bytes), set);
 }
 }  // namespace msgl
