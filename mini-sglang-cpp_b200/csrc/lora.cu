@@ -210,7 +210,7 @@ lora_small_kernel(const LoraArgs a, int num_reqs, int per) {
                 *reinterpret_cast<float2*>(p + 8 * R16) = make_float2(acc[j][2], acc[j][3]);
             }
             // the sums of the last 16 rows have been read by every CTA
-            if (waiting) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+            if (waiting) cluster_wait();
             __syncthreads();
             for (int i = threadIdx.x; i < rows * R16; i += kLoraWarps * 32) {
                 float v = 0.f;
@@ -218,7 +218,6 @@ lora_small_kernel(const LoraArgs a, int num_reqs, int per) {
                 for (int w = 0; w < kLoraWarps; ++w) v += red[w * 16 * R16 + i];
                 part[i] = v;
             }
-            __syncwarp();
             cluster_sync_all();
             const float scale = a.scales[adapter];
             for (int i = threadIdx.x; i < rows * R16; i += kLoraWarps * 32) {
@@ -230,8 +229,7 @@ lora_small_kernel(const LoraArgs a, int num_reqs, int per) {
                 for (int k = 0; k < 8; ++k) sum += v[k];  // in rank order
                 red[i] = sum * scale;
             }
-            __syncwarp();
-            asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for above or at the end
+            cluster_arrive();  // waited for above or at the end
             waiting = true;
             __syncthreads();
 #pragma unroll
@@ -309,8 +307,7 @@ lora_small_kernel(const LoraArgs a, int num_reqs, int per) {
             }
         }
     }
-    __syncwarp();
-    if (waiting) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (waiting) cluster_wait();
 }
 
 // ------------------------------------------------------------------ chunks

@@ -1435,7 +1435,6 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
             mo[(warp * 8 + j) * 32 + lane] = make_float4(st.o[j][0], st.o[j][1], st.o[j][2], st.o[j][3]);
         dump_sums(st, sm + warp * 8, sl + warp * 8, lane);
     }
-    __syncwarp();
     cluster_sync_all();
     const int parts = PW * CS, lgCS = 31 - __clz(CS);  // part p: page group p / CS of CTA p % CS
     const int self = pg * CS + rank, j0 = 8 * self / parts, j1 = 8 * (self + 1) / parts;
@@ -1493,7 +1492,6 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
             }
         }
     }
-    __syncwarp();
     cluster_sync_all();  // no CTA leaves while another reads its shared memory
 }
 
