@@ -21,7 +21,9 @@
 // left of h: 2^-24 of it), for the bf16 result as two (2^-16). One term (2^-8 of each of the rank's h)
 // is not enough: the result is off by as much of sum |B h|, which where those terms cancel, or cancel
 // y, is far more than the rounding of the result itself. (4.5k rows, 4096 -> 6144, on the device: 43 us
-// with one term and 50 with two at rank 64, 65 and 79 at rank 128, no difference at rank 16.)
+// with one term and 50 with two at rank 64, 65 and 79 at rank 128, no difference at rank 16.) The terms
+// behind the first take infinite and NaN weights as zero: what is left of an h that is a bf16 value is
+// zero, and zero times an infinite weight would be NaN.
 #include <algorithm>
 
 #include "common.cuh"
@@ -237,7 +239,8 @@ lora_small_kernel(const LoraArgs a, int num_reqs, int per) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (live[u]) f = *reinterpret_cast<const float4*>(red + (g + 8 * u) * R16 + 16 * kk + 4 * c);
+                    if (live[u] && 16 * kk + 4 * c < a.R)  // behind the rank: zero times x, NaN where that is infinite
+                        f = *reinterpret_cast<const float4*>(red + (g + 8 * u) * R16 + 16 * kk + 4 * c);
                     float v[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
                     for (int m = 0; m < TERMS; ++m) {
@@ -279,7 +282,8 @@ lora_small_kernel(const LoraArgs a, int num_reqs, int per) {
 #pragma unroll
                             for (int m = TERMS - 1; m >= 0; --m)
                                 mma_bf16_16816(acc[j], ha[kk][m][0], ha[kk][m][1], ha[kk][m][2], ha[kk][m][3],
-                                               bf[p][j][kk].x, bf[p][j][kk].y);
+                                               m ? finite2(bf[p][j][kk].x) : bf[p][j][kk].x,
+                                               m ? finite2(bf[p][j][kk].y) : bf[p][j][kk].y);
                 }
                 const int col = (blk0 + p) * 32 + 8 * c;
                 if (col >= a.N) continue;
@@ -325,7 +329,8 @@ __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// h terms in the workspace: [term][T][R16] bf16, zero behind the rank.
+// h terms in the workspace: [term][T][R16] bf16, zero behind the rank (where the sums are zero times x,
+// NaN where that is infinite).
 __host__ __device__ constexpr int64_t h_terms(int64_t T, int r16, int term) { return term * T * r16; }
 
 // A cluster of S CTAs (K ranges) per 64 rows; four warps of 16 rows times all ranks. x and A tiles
@@ -415,7 +420,7 @@ lora_shrink_kernel(const LoraArgs a, int terms) {
             v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] *= scale;
+        for (int e = 0; e < 4; ++e) v[e] = 4 * i % R16 < a.R ? v[e] * scale : 0.f;
         __nv_bfloat16* dst = a.h + static_cast<int64_t>(lt.t0) * R16 + 4 * i;
         for (int m = 0; m < terms; ++m) {
             const uint2 u = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
@@ -537,8 +542,6 @@ lora_expand_kernel(const LoraArgs a, int n_slices) {
                 }
                 if (!kHold) load_h(kk, hf[0]);
                 const auto& f = hf[kHold ? kk : 0];
-                // What is left of an h that is a bf16 value is zero, and zero times an infinite weight
-                // would be NaN: those take part through the first term alone.
                 uint32_t wf[4][2];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) wf[j][0] = finite2(w[j][0]), wf[j][1] = finite2(w[j][1]);

@@ -160,6 +160,37 @@ def test_a_row_does_not_reach_another(cuda, lens):
     assert bool(got[lens[0]:lens[0] + lens[1]].isnan().all())
 
 
+@pytest.mark.parametrize("lens", [[1], [1] * 20, [3, 16, 1], [20, 70]])
+@pytest.mark.parametrize("R", [8, 16, 24, 40, 72])
+def test_infinities_are_those_of_the_formula(cuda, lens, R):
+    """An infinite element of x, then an infinite weight: infinities of the formula's sign where the formula
+    has them, at ranks that end inside the MMA's 16 and at full ones, and finite values elsewhere."""
+    from msgl import ops
+    K, N, n = 64, 136, 2
+    x, a, b, sc, ids, y, indptr = make(lens, K, N, R, n, seed=R)
+    T = sum(lens)
+    x.fill_(1.0), a.fill_(2.0 ** -6), sc.fill_(1.0)
+    b.copy_(b.abs() + 2.0 ** -7)
+    b[:, 5::7] *= -1
+    kws = [dict(q_indptr=indptr, max_q_len=max(lens))] + ([{}] if max(lens) == 1 else [])
+    for kind in ("x", "weight"):
+        if kind == "x":
+            x[T // 2, 9] = float("inf")
+        else:
+            x.fill_(1.0)  # every h is 1: nothing is left of it behind its first term
+            b[:, 3, R - 1], b[:, 12, 0] = float("inf"), float("-inf")
+        d, mag = reference(x, a, b, sc, ids, lens)
+        ref = y.double() + d
+        assert bool(ref.isinf().any()) and not bool(ref.isnan().any())
+        fin = ref.isfinite()
+        for kw in kws:
+            o, p = ops.lora_add(x, a, b, sc, ids, y, **kw).double(), ops.lora_partial(x, a, b, sc, ids, **kw).double()
+            assert torch.equal(o[~fin], ref[~fin]) and torch.equal(p[~fin], d[~fin])
+            assert bool(((o - ref).abs()[fin] <= (ref.abs() * 2 ** -8 + mag * (steps(K, R) + 2 ** -16))[fin]).all())
+            assert bool(((p - d).abs()[fin] <= (mag * steps(K, R))[fin]).all())
+    assert ops.device_error() == (0, 0)
+
+
 def test_bad_ids_and_rows_are_recorded(cuda):
     from msgl import ops
     lens = [4, 6]
