@@ -314,7 +314,8 @@ MSGL_API int msgl_kv_page_bounds(const void* k_pool, int64_t num_slots, const in
  * lower page, NaN scores rank highest.
  * page_ids [total_q, Hkv, top_pages] int32: logical pages (page-table columns), ascending, filled
  * up with -1. top_pages <= 1024. The workspace (msgl_select_pages_workspace_size, 16-byte aligned)
- * needs no clearing; calls that overlap on the GPU need one each. */
+ * needs no clearing and serves every call with no more rows, heads and context than it was sized for;
+ * calls that overlap on the GPU need one each. */
 MSGL_API size_t msgl_select_pages_workspace_size(int total_q, int max_seq_len, int num_kv_heads);
 MSGL_API int msgl_select_pages(const void* q, const void* bounds, int64_t num_pages,
                                const int* page_table, int max_pages, const int* seq_lens,

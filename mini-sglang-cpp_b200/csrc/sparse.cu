@@ -1615,8 +1615,9 @@ int msgl_kv_page_bounds(const void* k_pool, int64_t num_slots, const int* page_t
 
 size_t msgl_select_pages_workspace_size(int total_q, int max_seq_len, int num_kv_heads) {
     if (total_q <= 0 || max_seq_len <= 0 || num_kv_heads <= 0 || pages_of(max_seq_len) > kMaxPagesPerReq) return 0;
-    const int stride = score_stride(max_seq_len);
-    return size_t(16) * slab_rows(total_q, stride, num_kv_heads) * num_kv_heads * stride;
+    // never less for fewer rows or a shorter context: one allocation serves all calls below its own
+    const int64_t row = int64_t(16) * num_kv_heads * score_stride(max_seq_len);
+    return static_cast<size_t>(std::min(total_q * row, std::max(kSelectBytes, 16 * row)));
 }
 
 int msgl_select_pages(const void* q, const void* bounds, int64_t num_pages, const int* page_table,

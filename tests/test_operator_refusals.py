@@ -90,6 +90,19 @@ def test_select_empty_and_workspace():
     assert L.msgl_select_pages_workspace_size(100000, 32768, 8) == 256 * 2 ** 20
 
 
+def test_select_workspace_serves_smaller_calls():
+    size = msgl.lib().msgl_select_pages_workspace_size
+    rows, contexts, heads = (1, 15, 16, 17, 300, 4096, 100000), (1, 300, 32768, 50000, 131072, 131088, 200000, 524288), (1, 3, 8, 64)
+    for T in rows:
+        for L in contexts:
+            for h in heads:
+                n = size(T, L, h)
+                assert all(size(t, l, g) <= n for t in rows if t <= T for l in contexts if l <= L for g in heads if g <= h), (T, L, h)
+                # 16 bytes per row of a pass, head and page of the context; 16 rows a pass or more
+                pages = max(16, -(-L // 256) * 16)
+                assert n >= 16 * min(T, max(16, 2 ** 28 // (16 * pages * h))) * h * pages
+
+
 def attend(**k):
     a = dict(q=P, k=P, v=P, slots=64, pt=P, mp=64, sl=P, ip=None, B=2, T=2, mq=1, L=1000, ids=P, top=8, hq=8, hkv=2,
              d=128, page=16, out=P)
