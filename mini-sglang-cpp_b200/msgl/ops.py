@@ -370,12 +370,13 @@ def lora_workspace(num_tokens, K, rank, device="cuda"):
 
 
 def _row_stride(dev, t, dtype, rows, cols):
-    """The row stride of [rows, cols] values with contiguous rows on the current device."""
+    """The row stride of [rows, cols] values with contiguous rows on the current device (of a single row:
+    its length, whatever the tensor that it was cut from has)."""
     if (t.dtype is not dtype or t.shape != (rows, cols) or t.get_device() != dev
             or (cols > 1 and t.stride(1) != 1)):
         raise ValueError(f"expected {dtype} rows [{rows}, {cols}] on cuda:{dev}, got {t.dtype} "
                          f"{tuple(t.shape)} with strides {t.stride()} on {t.device}")
-    return t.stride(0) if rows > 1 else max(t.stride(0), cols)
+    return t.stride(0) if rows > 1 else cols
 
 
 def _lora(entry, x, lora_a, lora_b, scales, adapter_ids, base, q_indptr, max_q_len, workspace, out, out_dtype):

@@ -142,6 +142,21 @@ def test_strided_rows_and_rows_behind_the_last_request(cuda):
     assert ops.device_error() == (0, 0)
 
 
+def test_one_row_of_a_tensor_of_any_width(cuda):
+    from msgl import ops
+    K, N, R = 1000, 264, 16
+    x, a, b, sc, ids, y, _ = make([1], K, N, R, 2, seed=3)
+    wide = [torch.zeros(3, n + 3, dtype=t.dtype, device="cuda") for t, n in ((x, K), (y, N), (y.float(), N))]
+    wide[0][:1, :K], wide[1][:1, :N] = x, y
+    x1, y1 = wide[0][:1, :K], wide[1][:1, :N]
+    d, mag = reference(x, a, b, sc, ids, [1])
+    check_partial(ops.lora_partial(x1, a, b, sc, ids, out=wide[2][:1, :N]), d, mag, K, R)
+    assert ops.lora_add(x1, a, b, sc, ids, y1, out=y1) is y1
+    check_add(y1, y, d, mag, K, R)
+    assert all(bool((w[1:] == 0).all()) and bool((w[0, -3:] == 0).all()) for w in wide)
+    assert ops.device_error() == (0, 0)
+
+
 @pytest.mark.parametrize("lens", [[1, 1, 1], [20, 40, 70]])
 def test_a_row_does_not_reach_another(cuda, lens):
     """NaN and infinite rows, adapters and weights of others change nothing for a request."""
