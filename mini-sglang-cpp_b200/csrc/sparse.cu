@@ -1194,11 +1194,11 @@ attend_pages_decode_kernel(const AttArgs a, int num_reqs, int words) {
 
 // ---- chunks
 // One CTA per (tile of one request's query rows, kv head): sixteen warps in RW row groups of TQ =
-// 8 / G rows each (RW from the longest chunk) times 16 / RW page groups, and a producer warp. The
-// rows' lists are joined into one list of pages with a mask of the rows that asked for each, so a
-// page that several neighbouring queries chose crosses from L2 once; a warp attends the pages that
-// its own rows asked for, one in 16 / RW of them. Pages come by TMA (one 3-D box of K, one of V)
-// through a ring shared by the warps, in stages of kStagePages: most warps skip most pages, and a
+// 8 / G rows each (8 for G = 1, where that is 64 rows, else 16) times 16 / RW page groups, and a
+// producer warp. The rows' lists are joined into one list of pages with a mask of the rows that asked
+// for each, so a page that several neighbouring queries chose crosses from L2 once; a warp attends the
+// pages that its own rows asked for, one in 16 / RW of them. Pages come by TMA (one 3-D box of K, one of
+// V) through a ring shared by the warps, in stages of kStagePages: most warps skip most pages, and a
 // barrier per page cost as much as the pages. Contexts longer than kWin pages are walked in windows
 // of that many. A cluster of CTAs (chunk_split) shares a tile: each takes a share of every window's
 // list, and the partial results are joined through distributed shared memory.
@@ -1774,8 +1774,7 @@ int msgl_paged_attention_pages(const void* q, const void* k_pool, const void* v_
         if (!rc) rc = make_tmap_3d_bf16(&tv, v_pool, kHd, num_kv_heads, num_slots, kHd * 2, row, kPadRow / 2, 1, kPage, false);
         if (rc) return rc;
         const int tq = 8 / G;
-        int row_groups = 1;
-        while (row_groups < kChWarps && row_groups * tq < std::min(max_q_len, kTileRows)) row_groups *= 2;
+        const int row_groups = std::min(kChWarps, kTileRows / tq);
         const int tiles = (max_q_len + row_groups * tq - 1) / (row_groups * tq);
         const int64_t blocks = int64_t(num_reqs) * tiles * num_kv_heads;
         // tiles that hold rows: every request ends with a part of one
