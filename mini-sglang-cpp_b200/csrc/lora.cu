@@ -320,15 +320,6 @@ constexpr int kBK = 64;       // K columns a stage
 constexpr int sh_stages(int kk) { return kk == 8 ? 4 : 5; }  // of 16 or 24 KB: two CTAs per SM
 constexpr int kNSlice = 256;  // columns of an expand CTA
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // h terms in the workspace: [term][T][R16] bf16, zero behind the rank (where the sums are zero times x,
 // NaN where that is infinite).
 __host__ __device__ constexpr int64_t h_terms(int64_t T, int r16, int term) { return term * T * r16; }
@@ -569,30 +560,7 @@ lora_expand_kernel(const LoraArgs a, int n_slices) {
     }
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 int rank16(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
-
-template <typename... KArgs, typename... Args>
-cudaError_t launch_cluster(void (*kernel)(KArgs...), int64_t grid, int size, size_t smem, cudaStream_t stream,
-                           Args&&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(grid));
-    cfg.blockDim = dim3(kLoraWarps * 32);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = size;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    launch_counter().fetch_add(1, std::memory_order_relaxed);
-    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
-}
 
 template <int KK, bool PARTIAL>
 cudaError_t launch_chunks(const LoraArgs& a, int64_t row_tiles, int splits, cudaStream_t stream) {
@@ -603,7 +571,7 @@ cudaError_t launch_chunks(const LoraArgs& a, int64_t row_tiles, int splits, cuda
     const size_t ex = size_t(kNSlice + (PARTIAL ? 3 : 2) * kTile) * 16 * KK * 2;
     e = smem_optin(lora_expand_kernel<KK, PARTIAL>, ex, optin[1]);
     if (e != cudaSuccess) return e;
-    e = launch_cluster(lora_shrink_kernel<KK>, row_tiles * splits, splits, sh, stream, a, PARTIAL ? 3 : 2);
+    e = launch_cluster(lora_shrink_kernel<KK>, row_tiles * splits, kLoraWarps * 32, splits, sh, stream, a, PARTIAL ? 3 : 2);
     if (e != cudaSuccess) return e;
     const int n_slices = (a.N + kNSlice - 1) / kNSlice;
     return launch_pdl(lora_expand_kernel<KK, PARTIAL>, dim3(static_cast<unsigned>(row_tiles * n_slices)),
@@ -625,7 +593,7 @@ cudaError_t launch_rank(const LoraArgs& a, int num_reqs, bool partial, cudaStrea
         }
         const auto kern = partial ? (grouped ? lora_small_kernel<KK, true, true> : lora_small_kernel<KK, true, false>)
                                   : (grouped ? lora_small_kernel<KK, false, true> : lora_small_kernel<KK, false, false>);
-        return launch_cluster(kern, clusters * size, size, 0, stream, a, num_reqs, per);
+        return launch_cluster(kern, clusters * size, kLoraWarps * 32, size, 0, stream, a, num_reqs, per);
     }
     // K ranges: about three CTAs per SM, ranges of at least 256 columns
     const int64_t row_tiles = int64_t(num_reqs) * a.tiles;

@@ -168,8 +168,6 @@ qknorm_mrope_store_kernel(const MropeArgs a) {
     }
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 int launch_mrope(MropeArgs a, const int* sections, int layout, int head_dim, msgl_stream_t stream) {
     if (head_dim != kHd) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "qknorm_mrope: head_dim != 128");
     if (a.num_tokens < 0 || a.hq <= 0 || a.hkv <= 0 || a.max_position <= 0 || a.num_slots < 0 || !sections)

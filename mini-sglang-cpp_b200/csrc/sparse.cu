@@ -48,15 +48,6 @@ __device__ __forceinline__ Window request_window(int r, const int* seq_lens, con
     return w;
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // ------------------------------------------------------------------ bounds
 constexpr int kBoundWarps = 8;
 
@@ -1496,8 +1487,6 @@ attend_pages_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
 }
 
 // ------------------------------------------------------------------ host checks
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 int check_heads(int hq, int hkv, int head_dim, int page_size) {
     if (head_dim != kHd) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "sparse attention: head_dim must be 128");
     if (page_size != kPage) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "sparse attention: page_size must be 16");
@@ -1552,28 +1541,6 @@ cudaError_t large_clusters() {
     e = cudaFuncSetAttribute(attend_pages_decode_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e == cudaSuccess && cached) done[dev].store(true, std::memory_order_release);
     return e;
-}
-
-// launch_pdl with a thread-block cluster of `size` CTAs.
-template <typename... KArgs, typename... Args>
-cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, int threads, int size, size_t smem, cudaStream_t stream,
-                           Args&&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = size;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    launch_counter().fetch_add(1, std::memory_order_relaxed);
-    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
 int score_stride(int max_seq_len) { return std::max(16, (pages_of(max_seq_len) + 15) / 16 * 16); }
@@ -1784,7 +1751,7 @@ int msgl_paged_attention_pages(const void* q, const void* k_pool, const void* v_
         static std::atomic<int> optin[kMaxDevices];
         cudaError_t e = smem_optin(attend_pages_chunk_kernel, kChSmem, optin);
         if (e == cudaSuccess)
-            e = launch_cluster(attend_pages_chunk_kernel, static_cast<unsigned>(blocks * split), kChThreads, split,
+            e = launch_cluster(attend_pages_chunk_kernel, blocks * split, kChThreads, split,
                                kChSmem, stream, tk, tv, a, tiles, row_groups);
         if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
         MSGL_LAUNCH_CHECK();
@@ -1799,7 +1766,7 @@ int msgl_paged_attention_pages(const void* q, const void* k_pool, const void* v_
     cudaError_t e = smem_optin(attend_pages_decode_kernel, smem, optin);
     if (e == cudaSuccess && split > 8) e = large_clusters();
     if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
-    e = launch_cluster(attend_pages_decode_kernel, static_cast<unsigned>(lists * split), kAttThreads, split, smem, stream, a, num_reqs, words);
+    e = launch_cluster(attend_pages_decode_kernel, lists * split, kAttThreads, split, smem, stream, a, num_reqs, words);
     if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
     MSGL_LAUNCH_CHECK();
     return MSGL_OK;
