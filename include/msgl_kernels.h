@@ -290,6 +290,9 @@ MSGL_API int msgl_paged_attention_extend(const void* q, const void* k_pool, cons
  * request r owns query rows [q_indptr[r], q_indptr[r+1]) of total_q rows, row i of an n-row
  * request at position seq_lens[r] - n + i (q_indptr NULL: one row per request, max_q_len 1);
  * max_q_len bounds the rows per request, max_seq_len (<= 524288, <= max_pages * 16) the contexts.
+ * Selection and attention choose their form by max_q_len: give the long chunks and the single tokens of a
+ * mixed batch in calls of their own (127 single tokens and a chunk of 512 rows, 32 / 8 heads, 64 of 256
+ * pages: attention 577 us in one call, 204 in two).
  * Rows behind the last request are left as they were. Recorded as MSGL_ERR_BOUNDS in the device
  * error word: a context outside [0, max_seq_len] (clamped, site 800), a request with more than
  * max_q_len rows or rows outside total_q (site 801: its extra rows get empty lists, attention
@@ -374,13 +377,17 @@ MSGL_API int msgl_gemm_bf16_partials(const void* x, const void* w, float* parts,
  *                      requests without an adapter are copied (out may be y itself);
  *   msgl_lora_partial  part[t] = scales[a] * lora_b[a] (lora_a[a] x[t]) (zero without an adapter),
  *                      fp32: the split-K partial behind those of msgl_gemm_bf16_partials.
+ * x is multiplied by lora_a in fp32; what the second product takes of that is 2^-16 off at most (partial:
+ * 2^-24), relative to each of the rank's values.
  * x [num_tokens, K], y / out / part [num_tokens, N] with row strides ldx, ldy, ldo, ldp in elements
  * (rows 16-byte aligned), so that a column range of a fused projection can be given. K, N, rank
  * multiples of 8, rank <= 128. Rows behind the last request are left as they were. Recorded as
  * MSGL_ERR_BOUNDS: an adapter id >= num_adapters (treated as none, site 810), a request with more
  * than max_q_len rows or rows outside num_tokens (skipped, site 811). The workspace
  * (msgl_lora_workspace_size, 16-byte aligned) needs no clearing; calls that overlap on the GPU need
- * one each. */
+ * one each. The form is chosen by max_q_len (up to 16 rows a request, or longer chunks): give the two
+ * kinds of a mixed batch in calls of their own (127 single tokens on 48 adapters and a chunk of 512 rows,
+ * 4096 -> 6144, rank 16: 92 us in one call, 26 in two). */
 MSGL_API size_t msgl_lora_workspace_size(int num_tokens, int K, int rank);
 MSGL_API int msgl_lora_add(const void* x, int64_t ldx, const void* lora_a, const void* lora_b,
                            const float* scales, int num_adapters, const int* adapter_ids,

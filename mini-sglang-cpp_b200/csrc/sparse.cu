@@ -902,7 +902,7 @@ __device__ __forceinline__ void attend(uint32_t base, const uint32_t (&qb)[8][2]
     }
     // P as two bf16 terms, which leaves 2^-16 of a weight out. One term leaves 2^-8 of each, which where
     // the values cancel is far more than the rounding of the result. (Selection and attention of 1.3k rows
-    // of 64 pages: 464 us with one term, 494 with two; 64 requests 168.5 and 169.9.)
+    // of 64 pages: 460 us with one term, 494 with two; 64 requests 169.3 and 170.4.)
     const uint32_t h0 = pack_bf16x2(p[0], p[1]), h1 = pack_bf16x2(p[2], p[3]);
     const uint32_t b0 = transpose8x8(h0), b1 = transpose8x8(h1);
     const uint32_t r0 = transpose8x8(pack_bf16x2(p[0] - bf16lo(h0), p[1] - bf16hi(h0)));
@@ -990,10 +990,11 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8], float f) {
 }
 
 // ---- single rows: decode, and short chunks
-// Lists attended one by one, also in chunks whose tiles would be half empty or too few (kRowsAlone
-// rows a request, kTotalAlone rows in all): selection and attention of 8 requests x 17 / 33 / 65 rows (32
-// heads, 64 of 512 pages) take 84 / 119 / 213 us this way and 88 / 130 / 161 in tiles, of 1 x 129 / 513
-// rows 86 / 245 and 93 / 158.
+// Lists attended one by one, also in chunks whose tiles would be half empty or too few (at most kRowsAlone
+// rows a request, or kTotalAlone rows in all). Selection and attention, 64 of 512 pages, 32 / 8 heads: 8
+// requests x 17 / 33 / 48 / 65 rows take 96 / 158 / 215 / 283 us this way and 96 / 164 / 168 / 222 in tiles,
+// one of 129 / 257 / 513 rows 88 / 143 / 270 and 99 / 101 / 169. The rows at which the two cross move
+// with the query group: 8 x 33 rows take 170 and 179 at 64 / 8 heads, 146 and 104 at 16 / 8.
 // A cluster of up to 16 CTAs (decode_split) per (query row, kv head): each CTA
 // takes a share of the listed pages, its four warps take its pages in turn, every warp with a ring
 // of its own (cp.async, 16 bytes a lane, three pages) and an online softmax. The warps' results are
@@ -1195,11 +1196,12 @@ attend_pages_decode_kernel(const AttArgs a, int num_reqs, int words) {
 // list, and the partial results are joined through distributed shared memory.
 //
 // Bound by shared memory: a warp's fragments of a page are 8 KB, 64 cycles of its port, and 5.3 of the
-// 16 row groups want a page; with the write of the page 410 cycles, of 525 that a page takes (1.3k
-// rows of 32 heads over 64 pages each, 126k page loads: 335 us; a CTA's list and join are 10 of 65 us).
+// 16 row groups want a page; with the write of the page 410 cycles, of some 580 that a page takes (1.3k
+// rows of 32 heads over 64 pages each, 126k page loads: 371 us; a CTA's list and join are 8 of 70 us). With
+// one bf16 term of P it was 525, and 338 us.
 // A box is 16 rows of kPadRow bytes, wider than the tensor's rows: the rest is filled with zeros, which
 // pads the rows. Boxes of swizzled half rows of 128 bytes took 225 cycles of the copy engine each and
-// 30 us more in all. Slower ways to bring the same pages: cp.async from producer warps (it shares the
+// 36 us more in all. Slower ways to bring the same pages: cp.async from producer warps (it shares the
 // path of the fragment loads), bulk copies of single rows, K by TMA and V by cp.async, tiles of 16
 // rows on two CTAs per SM; 16 warps, the last to leave a stage filling it again, in place of the
 // producer: 554 against 528 us.
@@ -1500,7 +1502,7 @@ int pages_of(int tokens) { return tokens / kPage + (tokens % kPage != 0); }
 
 // Query rows of one launch pair: as many as keep the workspace (16 bytes per row, kv head and
 // page) within 256 MB, so that the scores (a quarter of it) stay in L2 until they are read; at
-// least 16. (1.3k rows of 1024 pages: 479 us in two passes of 128 MB, 465 in one.)
+// least 16. (1.3k rows of 1024 pages: 509 us in two passes of 128 MB, 494 in one.)
 constexpr int64_t kSelectBytes = int64_t(256) << 20;
 int slab_rows(int total_q, int stride, int hkv) {
     const int64_t rows = std::max<int64_t>(16, kSelectBytes / (int64_t(16) * stride * hkv));
@@ -1516,8 +1518,8 @@ int decode_split(int64_t lists, int top) {
 
 // CTAs that share a tile of a chunk (up to 4): one SM holds one, and the rounds of 148 should be full.
 // A share costs a list and a join of its own, about a tenth of a tile's time in twos and a third in
-// fours. Selection and attention with tiles alone / in twos / in fours: 16 tiles 121 / 80 / 57 us, 136
-// tiles 158 / 170 / 207, 344 tiles 487 / 478 / 600.
+// fours. Selection and attention with tiles alone / in twos / in fours: 16 tiles 135 / 86 / 62 us, 136
+// tiles 169 / 182 / 222, 344 tiles 508 / 494 / 621.
 int chunk_split(int64_t tiles) {
     const double gain[3] = {1.0, 0.9, 0.63};
     int best = 1;
@@ -1662,9 +1664,9 @@ int msgl_select_pages(const void* q, const void* bounds, int64_t num_pages, cons
         return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "select_pages: batch too large");
     // Up to 1024 pages a warp holds a row; with too few rows to fill the GPU, and for longer
     // rows, more warps share one. Few warps that hold many scores beat many that hold few, whose
-    // counts meet at a barrier in every step: 8192 pages, one request, 8 warps 27.5 us for
-    // selection and attention, 16 warps 29.2; 2048 pages, 64 requests, 4 warps 173, 8 warps 175,
-    // 16 warps 186. At 512 pages the order turns: 4 warps 15.2 us, 2 warps 16.6.
+    // counts meet at a barrier in every step: 8192 pages, one request, 8 warps 27.0 us for
+    // selection and attention, 16 warps 28.4; 2048 pages, 64 requests, 4 warps 170, 8 warps 172,
+    // 16 warps 183. At 512 pages the order turns: 4 warps 14.7 us, 2 warps 15.0.
     using Select = void (*)(SelectArgs, int);
     const int pages = pages_of(max_seq_len);
     const bool many = sel_blocks >= 4 * 148;
