@@ -398,7 +398,7 @@ def _run_attend(st):
         ops = _ops()
         if "ws" not in st:  # the workspace and the output buffer that a serving loop keeps
             T = st["q"].shape[0]
-            st["ws"] = ops.attention_kv8_workspace(case["reqs"], T, st["max_q"], st["max_seq"], hq, hkv)
+            st["ws"] = ops.attention_kv8_workspace(case["reqs"], st["max_q"], hq, hkv)
             st["out"] = torch.empty(T, hq, HD, dtype=torch.bfloat16, device=st["q"].device)
         return ops.paged_attention_kv8(st["q"], st["kv8"], st["scales"], st["page_table"], st["seq_lens"], st["max_seq"],
                                        hq, hkv, q_indptr=st["indptr"], max_q_len=st["max_q"], workspace=st["ws"],
