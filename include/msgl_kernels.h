@@ -182,6 +182,34 @@ MSGL_API int msgl_sample(const float* logits, int num_rows, int vocab, const flo
                          const int* top_k, const float* top_p, uint64_t seed, uint64_t step,
                          int* out, msgl_stream_t stream);
 
+/* Probabilities of fp32 logits [num_rows, vocab] (row strides ldx, ldp in elements; probs may be
+ * logits with the same stride): probs[r] = softmax(logits[r] / temperature[r]) in fp32
+ * (temperature [num_rows] device, NULL: 1). A row with temperature <= 0 gets 1 at the first index
+ * of its maximum and 0 elsewhere (the greedy row of msgl_sample). A row without any logit above
+ * -inf gives zeros, one with a NaN or +inf gives NaN. vocab <= 327680. */
+MSGL_API int msgl_token_probs(const float* logits, int64_t ldx, int num_rows, int vocab,
+                              const float* temperature, float* probs, int64_t ldp,
+                              msgl_stream_t stream);
+/* Verification of drafted tokens (speculative sampling; no counterpart in the reference). Request r
+ * drafted k = draft_indptr[r+1] - draft_indptr[r] tokens, 0 <= k <= max_drafts: draft i is token
+ * draft_tokens[draft_indptr[r] + i], proposed with the probabilities draft_probs[draft_indptr[r] + i]
+ * [vocab]; the target gave k + 1 rows, target_probs[draft_indptr[r] + r + i] [vocab] behind i accepted
+ * drafts (fp32, row strides ldp, ldq). draft_probs NULL: each draft was certain.
+ *   Draft i is accepted while uniforms[draft_indptr[r] + i] * q(x) < p(x).
+ *   With n accepted drafts the next token is the first v whose running sum of w passes
+ *   last_uniforms[r] * sum(w): w = max(p_n - q_n, 0) of draft n's rows (p_n where that is 0
+ *   throughout), or w = p_k where all were accepted.
+ * Products, sums and comparisons in 64 bits; uniforms in [0, 1). accepted[r] = n; tokens[r]
+ * [max_drafts + 1] = the n drafts, the next token, then -1. Recorded as MSGL_ERR_BOUNDS: a draft
+ * range outside [0, num_drafts] or longer than max_drafts (n = 0, tokens -1, site 920), a drafted
+ * token outside the vocabulary (rejected, site 921), weights without a positive finite sum (next
+ * token -1, site 922). */
+MSGL_API int msgl_verify_drafts(const float* target_probs, int64_t ldp, const float* draft_probs,
+                                int64_t ldq, const int* draft_tokens, const int* draft_indptr,
+                                const float* uniforms, const float* last_uniforms, int num_reqs,
+                                int num_drafts, int max_drafts, int vocab, int* accepted,
+                                int* tokens, msgl_stream_t stream);
+
 /* ---------------------------------------------------------------- batch metadata */
 /* Advances a decode batch on the device (the decode branch of Scheduler::step's host flatten,
  * src/scheduler/scheduler.cpp:83-106, with KVCachePool::allocate, src/cache/kvcache.cpp:21-28,
@@ -206,6 +234,27 @@ MSGL_API int msgl_decode_advance_masked(const int* next_tokens, int* input_ids, 
                                         int* seq_lens, const int* free_pages, int* free_top,
                                         const int* finished, int num_reqs, int page_size,
                                         msgl_stream_t stream);
+/* Tables of a step of any rows per request (chunks, drafted tokens, none) from the requests' lengths,
+ * with the page pool's bookkeeping (KVCachePool::allocate / free, src/cache/kvcache.cpp:21-32) on the
+ * device. Request r keeps kept_lens[r] tokens whose keys and values are stored and adds new_lens[r]:
+ *   seq_lens = kept + new; its pages = ceil(seq_lens / page_size);
+ *   a request that holds more pages (held_pages[r]) gives the last ones back: columns held - 1 down
+ *   to `pages` are pushed onto free_pages[0 .. *free_top) (capacity free_capacity), requests in order;
+ *   then a request that holds fewer takes the others, columns ascending, popped from the top,
+ *   requests in order; held_pages[r] = pages;
+ *   q_indptr [num_reqs + 1] = running sum of new_lens; last_idx[r] = its last row, -1 without rows;
+ *   row i of request r: positions = kept + i, slot_mapping = its slot in the page pool; rows behind the
+ *   last request, up to num_tokens: position 0, slot -1 (a padding token).
+ * So kept = accepted length drops rejected drafts, kept = new = 0 frees a finished request. Columns
+ * given back keep their entries. All-or-nothing: with a stack that runs out (MSGL_ERR_WORKSPACE,
+ * site 710) or over (site 713), lengths below 0 or above max_pages (site 711), more rows than
+ * num_tokens (site 712) nothing is written. All arrays are device int32; page_table is
+ * [num_reqs, max_pages]; num_tokens <= 2^20. Outputs must not be inputs. */
+MSGL_API int msgl_step_tables(const int* kept_lens, const int* new_lens, int* page_table,
+                              int max_pages, int* held_pages, int* free_pages, int free_capacity,
+                              int* free_top, int num_reqs, int num_tokens, int page_size,
+                              int* seq_lens, int* q_indptr, int* positions, int* slot_mapping,
+                              int* last_idx, msgl_stream_t stream);
 /* The finish rule of Scheduler::step (scheduler.cpp:126-131) with the SamplingParams of
  * include/minisgl/core/types.h:12-20, on the device, for one decode step: for every request not
  * yet finished, token_out[r] = next_tokens[r], generated[r] += 1, and finished[r] = 1 once
@@ -338,6 +387,70 @@ MSGL_API int msgl_paged_attention_pages(const void* q, const void* k_pool, const
                                         const int* page_ids, int top_pages, int num_q_heads,
                                         int num_kv_heads, int head_dim, int page_size, float scale,
                                         void* out, msgl_stream_t stream);
+
+/* ---------------------------------------------------------------- 8-bit key / value pool */
+/* A page pool in 8 bits (no counterpart in the reference): half the bytes of the bf16 pools. Common to
+ * the calls: head_dim 128, page_size 16; request r owns rows [q_indptr[r], q_indptr[r+1]), row i of an
+ * n-row request at position seq_lens[r] - n + i (q_indptr NULL: one row per request, max_q_len 1);
+ * page_table [num_reqs, max_pages]; rows behind the last request are left as they were.
+ *   kv8    [num_pages, Hkv, 4096] e4m3 codes of a page and kv head: key of token t, dimension d at
+ *          d / 64 * 1024 + t * 64 + d % 64, its value at
+ *          2048 + d / 4 * 64 + t % 8 / 2 * 16 + d % 4 * 4 + t / 8 * 2 + t % 2;
+ *   scales [num_pages, Hkv, 2] exponents of keys and values, 127 added;
+ * both bytes, 16-byte aligned. A value is code * 2^(scale - 127).
+ *
+ * Append: msgl_qknorm_rope_store_kv (positions index cos_sin_cache [max_position, 128]) with keys and
+ * values quantised into the pages that each request's rows reach. Of each page, kv head and kind the
+ * exponent is the smallest e >= -96 with max |value| <= 448 * 2^e over the values that the page holds
+ * (the tokens before the context's end), codes are the nearest e4m3 values, ties to even; earlier
+ * tokens' values are rounded again where the exponent grows (which changes those that become
+ * subnormal) and the page's slots behind the context's end become 0. NaN and infinities are stored as
+ * NaN and do not count for the exponent. Slots behind the kept tokens are not read: a rejected draft
+ * leaves nothing but the rounding of earlier values that it made subnormal. Two requests of one call
+ * must not reach the same page.
+ * Recorded as MSGL_ERR_BOUNDS: a context outside [rows, max_pages * 16] (site 910) or more than
+ * max_q_len rows or rows outside num_tokens (site 911; the request's keys and values are skipped), a
+ * position outside the table (counts as 0, site 912), a page outside the pool (skipped, site 913). */
+MSGL_API int msgl_qknorm_rope_store_kv8(const void* qkv, void* q_out, void* kv8, void* scales,
+                                        int64_t num_pages, const int* positions,
+                                        const int* page_table, int max_pages, const int* seq_lens,
+                                        const int* q_indptr, int num_reqs, int max_q_len,
+                                        const float* cos_sin_cache, int max_position,
+                                        const void* q_norm_w, const void* k_norm_w,
+                                        int num_tokens, int num_q_heads, int num_kv_heads,
+                                        int head_dim, int page_size, float eps,
+                                        msgl_stream_t stream);
+/* The same, with the QKV row the sum (in p order) of fp32 split-K partials
+ * parts [nparts][T][(Hq + 2 Hkv) D] (msgl_gemm_bf16_partials, msgl_lora_partial). */
+MSGL_API int msgl_qknorm_rope_store_kv8_partials(const float* parts, int nparts, void* q_out,
+                                                 void* kv8, void* scales, int64_t num_pages,
+                                                 const int* positions, const int* page_table,
+                                                 int max_pages, const int* seq_lens,
+                                                 const int* q_indptr, int num_reqs, int max_q_len,
+                                                 const float* cos_sin_cache, int max_position,
+                                                 const void* q_norm_w, const void* k_norm_w,
+                                                 int num_tokens, int num_q_heads,
+                                                 int num_kv_heads, int head_dim, int page_size,
+                                                 float eps, msgl_stream_t stream);
+/* Attention over the 8-bit pool: single tokens, drafted rows and chunks. q / out [total_q, Hq, 128]
+ * bf16, Hq / Hkv in {1, 2, 4, 8}; each row attends the keys up to its own position (a row before the
+ * context's first token, or of an empty context, gives zeros); keys and values behind it do not reach
+ * it whatever they hold. A row with a NaN or an infinity in its query gives NaN. max_q_len bounds the
+ * rows per request, max_seq_len (<= max_pages * 16) the contexts. Recorded as MSGL_ERR_BOUNDS: a
+ * context outside [0, max_seq_len] (clamped, site 900), a request with more than max_q_len rows or
+ * rows outside total_q (skipped, site 901), a page outside the pool (page 0 in its place, site 902).
+ * The workspace (msgl_paged_attention_kv8_workspace_size, 16-byte aligned) is zero-filled once before
+ * its first use and left zero-filled where it counts; it serves every call with no more requests and
+ * rows a request of the same head counts; calls that overlap on the GPU need one each. */
+MSGL_API size_t msgl_paged_attention_kv8_workspace_size(int num_reqs, int max_q_len, int num_q_heads,
+                                                        int num_kv_heads);
+MSGL_API int msgl_paged_attention_kv8(const void* q, const void* kv8, const void* scales,
+                                      int64_t num_pages, const int* page_table, int max_pages,
+                                      const int* seq_lens, const int* q_indptr, int num_reqs,
+                                      int total_q, int max_q_len, int max_seq_len, int num_q_heads,
+                                      int num_kv_heads, int head_dim, int page_size, float scale,
+                                      void* out, void* workspace, size_t workspace_bytes,
+                                      msgl_stream_t stream);
 
 /* ---------------------------------------------------------------- tcgen05 GEMMs */
 /* Linear::forward (layer.cpp:122-143): y[M,N] = x[M,K] * W[N,K]^T, W in the reference's

@@ -11,6 +11,9 @@
 //                          the same with finished requests held in place, and the stop rules
 //                          (max_tokens, stop ids, ignore_eos) applied on the device.
 //
+//  * msgl_step_tables      a step of any rows per request (chunks, drafted tokens, none): pages
+//                          given back and taken, page table, row ranges, positions and slots.
+//
 // One CTA of up to 1024 threads walks the requests in blocks of blockDim; a block-wide scan
 // gives each request that starts a new page its rank among this step's allocations, so pages
 // leave the free stack in request order, as the host pool hands them out. The step is
@@ -116,6 +119,202 @@ __global__ void decode_finish_kernel(const int* __restrict__ next_tokens, int* _
     if (stop) finished[r] = 1;
 }
 
+// ------------------------------------------------------------------ step tables
+// seq = kept + new, pages = ceil(seq / page). Requests that hold more pages than that give the others
+// back (rejected drafts, finished requests), then requests that hold fewer take theirs; both in request
+// order. A request's pages go back last column first, so that the next to be taken are in the order in
+// which they were held. Latency bound: a scan of the requests, then one gather per row.
+//
+// One cluster. Its first CTA does what hangs on the order: three scans over the requests (pages given
+// back, pages taken, rows) in one pass, then pages and rows are dealt to the threads by their place in
+// the scans, so that one long prompt among single tokens costs no serial walk. All CTAs fill positions
+// and slots. (A cluster of eight from 2048 rows on.)
+constexpr int kStepThreads = 1024;
+
+struct StepArgs {
+    const int *kept, *add;
+    int* table;
+    int width;
+    int* held;
+    int* free_pages;
+    int capacity;
+    int* free_top;
+    int B, tokens, page;
+    int *seq_lens, *indptr, *positions, *slots, *last;
+    int* err;
+};
+
+// First index i of ends[0 .. n) (ascending) with ends[i] > x; n if there is none.
+__device__ __forceinline__ int first_above(const int* ends, int n, int x) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (ends[mid] > x) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(kStepThreads)
+step_tables_kernel(const StepArgs a) {
+    __shared__ int give_end[kStepThreads], take_end[kStepThreads], row_end[kStepThreads + 1];
+    __shared__ int s_need[kStepThreads], s_kept[kStepThreads];
+    __shared__ int warp_sums[3][32];
+    __shared__ int bad;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = cluster_ctarank(), size = cluster_nctarank();
+    if (tid == 0) bad = 0;
+    pdl_wait();
+    pdl_trigger();
+    if (rank == 0) {
+        const int blocks = (a.B + kStepThreads - 1) / kStepThreads;
+        int give_all, take_all, rows_all;
+        // Requests [r0, r0 + 1024): inclusive sums of pages given, taken and rows into shared memory.
+        auto load = [&](int r0) {
+            const int r = r0 + tid;
+            int k = 0, n = 0, h = 0, need = 0;
+            if (r < a.B) {
+                k = a.kept[r];
+                n = a.add[r];
+                h = a.held[r];
+                if (k < 0 || n < 0 || h < 0 || h > a.width ||
+                    static_cast<int64_t>(k) + n > static_cast<int64_t>(a.width) * a.page) {
+                    atomicOr(&bad, 2);
+                    k = n = h = 0;
+                } else if (n > a.tokens) {
+                    atomicOr(&bad, 4);
+                    k = n = h = 0;
+                }
+                need = (k + n + a.page - 1) / a.page;
+            }
+            int x[3] = {max(h - need, 0), max(need - h, 0), n};
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+                for (int v = 0; v < 3; ++v) {
+                    const int y = __shfl_up_sync(0xffffffffu, x[v], o);
+                    if (lane >= o) x[v] += y;
+                }
+            __syncthreads();  // the sums of the block before are no longer read
+            if (lane == 31)
+#pragma unroll
+                for (int v = 0; v < 3; ++v) warp_sums[v][warp] = x[v];
+            __syncthreads();
+            if (warp < 3) {
+                int t = warp_sums[warp][lane];
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int y = __shfl_up_sync(0xffffffffu, t, o);
+                    if (lane >= o) t += y;
+                }
+                warp_sums[warp][lane] = t;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int v = 0; v < 3; ++v) x[v] += warp ? warp_sums[v][warp - 1] : 0;
+            give_end[tid] = x[0];
+            take_end[tid] = x[1];
+            row_end[tid] = x[2];
+            s_need[tid] = need;
+            s_kept[tid] = k;
+            give_all = warp_sums[0][31];
+            take_all = warp_sums[1][31];
+            rows_all = warp_sums[2][31];
+            __syncthreads();
+        };
+        // pass 1: totals, every check; nothing is written
+        const int top0 = *a.free_top;
+        int64_t gives = 0, takes = 0, rows = 0;
+        for (int blk = 0; blk < blocks; ++blk) {
+            load(blk * kStepThreads);
+            gives += give_all;
+            takes += take_all;
+            rows += rows_all;
+        }
+        if (tid == 0) {
+            if (rows > a.tokens) bad |= 4;
+            if (top0 < 0 || top0 + gives > a.capacity) bad |= 8;
+            if (top0 + gives < takes) bad |= 1;
+            if (bad)
+                record_error(a.err, bad & 2 ? MSGL_ERR_BOUNDS : bad & 4 ? MSGL_ERR_BOUNDS
+                                    : bad & 8 ? MSGL_ERR_BOUNDS : MSGL_ERR_WORKSPACE,
+                             bad & 2 ? 711 : bad & 4 ? 712 : bad & 8 ? 713 : 710);
+        }
+        __syncthreads();
+        if (!bad) {
+            // pass 2: pages back onto the stack
+            int top = top0;
+            for (int blk = 0; blk < blocks && gives; ++blk) {
+                if (blocks > 1) load(blk * kStepThreads);
+                const int n = min(kStepThreads, a.B - blk * kStepThreads);
+                for (int i = tid; i < give_all; i += kStepThreads) {
+                    const int q = first_above(give_end, n, i);
+                    const int c = s_need[q] + (give_end[q] - 1 - i);  // the last column first
+                    a.free_pages[top + i] = a.table[static_cast<int64_t>(blk * kStepThreads + q) * a.width + c];
+                }
+                top += give_all;
+            }
+            __syncthreads();
+            // pass 3: pages taken, the requests' outputs
+            int row0 = 0;
+            for (int blk = 0; blk < blocks; ++blk) {
+                if (blocks > 1) load(blk * kStepThreads);
+                const int r0 = blk * kStepThreads, n = min(kStepThreads, a.B - r0);
+                for (int i = tid; i < take_all; i += kStepThreads) {
+                    const int q = first_above(take_end, n, i);
+                    const int c = s_need[q] - (take_end[q] - i);
+                    a.table[static_cast<int64_t>(r0 + q) * a.width + c] = a.free_pages[top - 1 - i];
+                }
+                if (tid < n) {
+                    const int end = row_end[tid], begin = tid ? row_end[tid - 1] : 0;
+                    a.seq_lens[r0 + tid] = s_kept[tid] + end - begin;
+                    a.held[r0 + tid] = s_need[tid];
+                    a.indptr[r0 + tid + 1] = row0 + end;
+                    a.last[r0 + tid] = end > begin ? row0 + end - 1 : -1;
+                }
+                top -= take_all;
+                row0 += rows_all;
+            }
+            if (tid == 0) {
+                a.indptr[0] = 0;
+                *a.free_top = top;
+            }
+        }
+    }
+    __syncthreads();
+    cluster_sync_all();  // the tables of the first CTA, and whether it wrote them
+    int failed = bad;
+    if (rank != 0) failed = __float_as_int(ld_dsmem_f32(mapa_shared(smem_u32(&bad), 0)));
+    if (!failed) {
+        // rows' request: ends and kept lengths in shared memory where they fit
+        const int* ends = a.indptr + 1;
+        const int* kept = a.kept;
+        __syncthreads();
+        if (a.B <= kStepThreads) {
+            if (tid < a.B) {
+                row_end[tid + 1] = ends[tid];
+                s_kept[tid] = kept[tid];
+            }
+            if (tid == 0) row_end[0] = 0;
+            __syncthreads();
+            ends = row_end + 1;
+            kept = s_kept;
+        }
+        const int total = ends[a.B - 1];
+        for (int i = rank * kStepThreads + tid; i < a.tokens; i += size * kStepThreads) {
+            int pos = 0, slot = -1;
+            if (i < total) {
+                const int r = first_above(ends, a.B, i);
+                pos = kept[r] + i - (r ? ends[r - 1] : 0);
+                slot = a.table[static_cast<int64_t>(r) * a.width + pos / a.page] * a.page + pos % a.page;
+            }
+            a.positions[i] = pos;
+            a.slots[i] = slot;
+        }
+    }
+    cluster_sync_all();  // the first CTA's shared memory was read
+}
+
 }  // namespace
 }  // namespace msgl
 
@@ -158,6 +357,31 @@ int msgl_decode_advance_masked(const int* next_tokens, int* input_ids, int* posi
     launch_pdl(decode_advance_kernel, dim3(1), dim3(threads), 0, stream, next_tokens, input_ids,
                positions, slot_mapping, page_table, max_pages, seq_lens, free_pages, free_top,
                num_reqs, page_size, finished, err);
+    MSGL_LAUNCH_CHECK();
+    return MSGL_OK;
+}
+
+int msgl_step_tables(const int* kept_lens, const int* new_lens, int* page_table, int max_pages, int* held_pages,
+                     int* free_pages, int free_capacity, int* free_top, int num_reqs, int num_tokens,
+                     int page_size, int* seq_lens, int* q_indptr, int* positions, int* slot_mapping,
+                     int* last_idx, msgl_stream_t stream) {
+    if (num_reqs < 0 || num_tokens < 0 || max_pages <= 0 || page_size <= 0 || free_capacity < 0)
+        return set_error(MSGL_ERR_INVALID_ARG, "step_tables: bad sizes");
+    if (num_tokens > 1 << 20 || static_cast<int64_t>(num_reqs) * max_pages > INT32_MAX ||
+        static_cast<int64_t>(max_pages) * page_size > INT32_MAX)
+        return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "step_tables: more than 2^20 rows, 2^31 page-table entries or 2^31 tokens a request");
+    if (num_reqs == 0) return MSGL_OK;
+    if (!kept_lens || !new_lens || !page_table || !held_pages || !free_pages || !free_top || !seq_lens ||
+        !q_indptr || !last_idx || (num_tokens > 0 && (!positions || !slot_mapping)))
+        return set_error(MSGL_ERR_INVALID_ARG, "step_tables: null pointer");
+    if (seq_lens == kept_lens || seq_lens == new_lens)
+        return set_error(MSGL_ERR_INVALID_ARG, "step_tables: seq_lens must not be an input");
+    StepArgs a = {kept_lens, new_lens, page_table, max_pages, held_pages, free_pages, free_capacity, free_top,
+                  num_reqs, num_tokens, page_size, seq_lens, q_indptr, positions, slot_mapping, last_idx,
+                  device_error_word()};
+    if (!a.err) return set_error(MSGL_ERR_CUDA, "device error word unavailable");
+    const int size = num_tokens > 2 * kStepThreads ? 8 : 1;
+    launch_cluster(step_tables_kernel, size, kStepThreads, size, 0, stream, a);
     MSGL_LAUNCH_CHECK();
     return MSGL_OK;
 }

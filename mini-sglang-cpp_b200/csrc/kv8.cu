@@ -1,0 +1,1058 @@
+// kv8.cu -- append to the 8-bit key / value pool, and attention of single tokens and drafted rows over it.
+//
+//  * msgl_qknorm_rope_store_kv8 (+ _partials)  QK-norm + rotation + quantised append
+//  * msgl_paged_attention_kv8                  attention (long chunks: kv8_chunk.cu)
+//
+// Format and conversions: kv8.cuh.
+#include <algorithm>
+
+#include "kv8.cuh"
+#include "kv8_args.h"
+
+namespace msgl {
+namespace {
+
+constexpr int kPage = kKv8Page;
+constexpr int kHd = kKv8Head;
+constexpr int kHalf = kHd / 2;
+constexpr float kNegInf = -__builtin_huge_valf();
+
+// ------------------------------------------------------------------ append
+// One warp per touched page, kv head and kind (keys, values): it brings the page's 16 x 128 values together
+// in registers (earlier tokens from their codes, new ones from the projection, zeros behind the context's
+// end), takes the largest magnitude, and writes codes and exponent. So the scale is that of the values
+// which the page holds now (a rejected draft does not keep it up), and old codes are only rounded again
+// where they become subnormal: e4m3 times a power of two is e4m3. NaN and infinities
+// are stored as NaN and do not count for the scale, so they stay where they are.
+// Lane 8 c + i: dimensions [8 i, 8 i + 8) of both halves (rotate-half partners) of the tokens 2 c, 2 c + 1,
+// 8 + 2 c, 9 + 2 c: rows are 256-byte reads and the value units 16-byte writes.
+// Query heads: eight lanes a head, as in the bf16 append.
+constexpr int kStoreWarps = 4;
+
+struct StoreArgs {
+    const __nv_bfloat16* qkv;
+    const float* parts;
+    int nparts;
+    __nv_bfloat16* q_out;
+    uint8_t *kv8, *scales;
+    int64_t num_pages;
+    const int *positions, *page_table;
+    int max_pages;
+    const int *seq_lens, *q_indptr;
+    int num_reqs, max_q_len;
+    const float* table;
+    int max_position;
+    const __nv_bfloat16 *qn, *kn;
+    int num_tokens, hq, hkv;
+    float eps;
+    int page_tasks;    // pages a request may touch
+    int kv_blocks;     // blocks of the append; the others take query heads
+    int q_blocks;      // of a token
+    int* err;
+};
+
+// 16 values of a head row: elements 8 i + e (e < 8) and 64 + 8 i + (e - 8), bf16 or summed in part order.
+template <bool PARTS>
+__device__ __forceinline__ void load_head(const StoreArgs& a, int64_t row, int head, int i, float (&x)[16]) {
+    const int nh = a.hq + 2 * a.hkv;
+    const int64_t at = (row * nh + head) * kHd + 8 * i;
+    if (PARTS) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = 0.f;
+        const int64_t stride = static_cast<int64_t>(a.num_tokens) * nh * kHd;
+        for (int p = 0; p < a.nparts; ++p) {
+            const float4* src = reinterpret_cast<const float4*>(a.parts + p * stride + at);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const float4 f = src[(v >> 1) * (kHalf / 4) + (v & 1)];
+                x[4 * v] += f.x; x[4 * v + 1] += f.y; x[4 * v + 2] += f.z; x[4 * v + 3] += f.w;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+            const uint4 u = *reinterpret_cast<const uint4*>(a.qkv + at + v * kHalf);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[8 * v + 2 * e] = bf16lo(w[e]);
+                x[8 * v + 2 * e + 1] = bf16hi(w[e]);
+            }
+        }
+    }
+}
+
+// x = x / sqrt(mean(x^2) + eps) * w, then the rotate-half pairs (8 i + e, 64 + 8 i + e) turned by the angle of
+// table row `turn`. The eight lanes of a head call it together.
+__device__ __forceinline__ void norm_turn(float (&x)[16], const __nv_bfloat16* w, const float* turn, int i, float eps) {
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) ss += x[e] * x[e];
+    ss += __shfl_xor_sync(0xffffffffu, ss, 1);
+    ss += __shfl_xor_sync(0xffffffffu, ss, 2);
+    ss += __shfl_xor_sync(0xffffffffu, ss, 4);
+    float inv = 1.0f / sqrtf(ss / kHd + eps);
+    if (__any_sync(0xffffffffu, ss > 3.4e38f)) {  // squares beyond fp32: the sum once more, of x 2^-70
+        float s2 = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float y = x[e] * 0x1p-70f;
+            s2 += y * y;
+        }
+        s2 += __shfl_xor_sync(0xffffffffu, s2, 1);
+        s2 += __shfl_xor_sync(0xffffffffu, s2, 2);
+        s2 += __shfl_xor_sync(0xffffffffu, s2, 4);
+        if (ss > 3.4e38f) inv = 0x1p-70f / sqrtf(s2 / kHd);
+    }
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+        const uint4 u = *reinterpret_cast<const uint4*>(w + 8 * i + v * kHalf);
+        const uint32_t ww[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[8 * v + 2 * e] *= inv * bf16lo(ww[e]);
+            x[8 * v + 2 * e + 1] *= inv * bf16hi(ww[e]);
+        }
+    }
+    float c[8], s[8];
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+        *reinterpret_cast<float4*>(c + 4 * v) = *reinterpret_cast<const float4*>(turn + 8 * i + 4 * v);
+        *reinterpret_cast<float4*>(s + 4 * v) = *reinterpret_cast<const float4*>(turn + kHalf + 8 * i + 4 * v);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float lo = x[e], hi = x[8 + e];
+        x[e] = lo * c[e] - hi * s[e];
+        x[8 + e] = lo * s[e] + hi * c[e];
+    }
+}
+
+__device__ __forceinline__ const float* turn_row(const StoreArgs& a, int64_t row) {
+    int pos = a.positions[row];
+    if (static_cast<unsigned>(pos) >= static_cast<unsigned>(a.max_position)) {
+        record_error(a.err, MSGL_ERR_BOUNDS, 912);
+        pos = 0;
+    }
+    return a.table + static_cast<int64_t>(pos) * kHd;
+}
+
+template <bool PARTS>
+__device__ __forceinline__ void append_page(const StoreArgs& a, int task, int lane) {
+    const int kind = task & 1;  // 0 keys, 1 values
+    task >>= 1;
+    const int h = task % a.hkv;
+    task /= a.hkv;
+    const int r = task / a.page_tasks, nth = task % a.page_tasks;
+    int L = a.seq_lens[r];
+    const int q0 = a.q_indptr ? a.q_indptr[r] : r;
+    const int n = a.q_indptr ? a.q_indptr[r + 1] - q0 : 1;
+    const bool first = lane == 0 && nth == 0 && h == 0 && kind == 0;
+    if (L < 0 || L > a.max_pages * static_cast<int64_t>(kPage) || n < 0 || n > L) {
+        if (first && n != 0) record_error(a.err, MSGL_ERR_BOUNDS, 910);
+        return;
+    }
+    if (n == 0) return;
+    if (n > a.max_q_len || q0 < 0 || q0 > a.num_tokens - n) {
+        if (first) record_error(a.err, MSGL_ERR_BOUNDS, 911);
+        return;
+    }
+    const int begin = L - n;  // tokens before it are held already
+    const int page = begin / kPage + nth;
+    if (page * kPage >= L) return;
+    const int phys = a.page_table[static_cast<int64_t>(r) * a.max_pages + page];
+    if (phys < 0 || phys >= a.num_pages) {
+        if (lane == 0) record_error(a.err, MSGL_ERR_BOUNDS, 913);
+        return;
+    }
+    const int64_t block = static_cast<int64_t>(phys) * a.hkv + h;
+    uint8_t* codes = a.kv8 + block * kKv8Bytes + kind * kKv8Values;
+    const int c = lane >> 3, i = lane & 7;
+    float x[4][16];
+    const int old = begin - page * kPage;  // tokens of the page that are held already, if positive
+    if (old > 0) {
+        const float s = kv8_power(a.scales[2 * block + kind]);
+        if (kind == 0) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    const uint2 u = *reinterpret_cast<const uint2*>(codes + v * 1024 + ((e >> 1) * 8 + 2 * c + (e & 1)) * 64 + 8 * i);
+                    const uint32_t w[2] = {u.x, u.y};
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const float2 f = __half22float2(__nv_cvt_fp8x2_to_halfraw2(w[b >> 1] >> ((b & 1) * 16) & 0xffff, __NV_E4M3));
+                        x[e][8 * v + 2 * b] = f.x * s;
+                        x[e][8 * v + 2 * b + 1] = f.y * s;
+                    }
+                }
+        } else {
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {  // dimensions 64 (v / 2) + 8 i + 4 (v % 2) + j
+                const uint4 u = *reinterpret_cast<const uint4*>(codes + ((v >> 1) * 16 + 2 * i + (v & 1)) * 64 + c * 16);
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const float2 f = __half22float2(__nv_cvt_fp8x2_to_halfraw2(w[j] >> (b * 16) & 0xffff, __NV_E4M3));
+                        x[2 * b][4 * v + j] = f.x * s;
+                        x[2 * b + 1][4 * v + j] = f.y * s;
+                    }
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int t = (e >> 1) * 8 + 2 * c + (e & 1);
+        const bool live = t >= old && page * kPage + t < L;
+        const int64_t row = q0 + (live ? page * kPage + t - begin : n - 1);
+        if (__any_sync(0xffffffffu, live)) {  // lanes of other tokens work on the request's last row
+            float y[16];
+            load_head<PARTS>(a, row, a.hq + kind * a.hkv + h, i, y);
+            if (kind == 0) norm_turn(y, a.kn, turn_row(a, row), i, a.eps);
+#pragma unroll
+            for (int d = 0; d < 16; ++d) x[e][d] = live ? y[d] : t < old ? x[e][d] : 0.f;
+        } else if (t >= old) {
+#pragma unroll
+            for (int d = 0; d < 16; ++d) x[e][d] = 0.f;
+        }
+    }
+    float amax = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int d = 0; d < 16; ++d) {
+            if (fabsf(x[e][d]) < __builtin_huge_valf()) amax = fmaxf(amax, fabsf(x[e][d]));
+            else x[e][d] = __int_as_float(0x7fffffff);
+        }
+    amax = warp_max(amax);
+    const int stored = kv8_exponent(amax);
+    const float inv = kv8_inverse(stored);
+    if (kind == 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                uint32_t w[4];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) w[b] = e4m3_codes2(x[e][8 * v + 2 * b] * inv, x[e][8 * v + 2 * b + 1] * inv);
+                *reinterpret_cast<uint2*>(codes + v * 1024 + ((e >> 1) * 8 + 2 * c + (e & 1)) * 64 + 8 * i) =
+                    make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+            }
+    } else {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                w[j] = e4m3_codes2(x[0][4 * v + j] * inv, x[1][4 * v + j] * inv) |
+                       e4m3_codes2(x[2][4 * v + j] * inv, x[3][4 * v + j] * inv) << 16;
+            *reinterpret_cast<uint4*>(codes + ((v >> 1) * 16 + 2 * i + (v & 1)) * 64 + c * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    if (lane == 0) a.scales[2 * block + kind] = static_cast<uint8_t>(stored);
+}
+
+template <bool PARTS>
+__global__ void __launch_bounds__(kStoreWarps * 32)
+qknorm_rope_store_kv8_kernel(const StoreArgs a) {
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (static_cast<int>(blockIdx.x) < a.kv_blocks) {
+        const int task = blockIdx.x * kStoreWarps + warp;
+        if (task < a.num_reqs * a.page_tasks * a.hkv * 2) append_page<PARTS>(a, task, lane);
+        return;
+    }
+    const int b = blockIdx.x - a.kv_blocks;
+    const int64_t t = b / a.q_blocks;
+    if (a.q_indptr && (t < a.q_indptr[0] || t >= a.q_indptr[a.num_reqs])) return;  // no request's row
+    const int h = ((b % a.q_blocks) * kStoreWarps + warp) * 4 + (lane >> 3), i = lane & 7;
+    const bool live = h < a.hq;
+    float x[16];
+    load_head<PARTS>(a, t, live ? h : 0, i, x);
+    norm_turn(x, a.qn, turn_row(a, t), i, a.eps);
+    if (!live) return;
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+        *reinterpret_cast<uint4*>(a.q_out + (t * a.hq + h) * kHd + v * kHalf + 8 * i) =
+            make_uint4(pack_bf16x2(x[8 * v], x[8 * v + 1]), pack_bf16x2(x[8 * v + 2], x[8 * v + 3]),
+                       pack_bf16x2(x[8 * v + 4], x[8 * v + 5]), pack_bf16x2(x[8 * v + 6], x[8 * v + 7]));
+}
+
+int launch_store(StoreArgs a, int head_dim, int page_size, msgl_stream_t stream) {
+    if (head_dim != kHd) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "store_kv8: head_dim must be 128");
+    if (page_size != kPage) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "store_kv8: page_size must be 16");
+    if (a.num_tokens < 0 || a.num_reqs < 0 || a.max_q_len < 0 || a.hq <= 0 || a.hkv <= 0 || a.max_position <= 0 ||
+        a.num_pages <= 0 || a.max_pages <= 0 || a.max_pages > INT32_MAX / kPage)
+        return set_error(MSGL_ERR_INVALID_ARG, "store_kv8: bad sizes");
+    if (!a.q_indptr && (a.max_q_len != 1 || a.num_tokens != a.num_reqs))
+        return set_error(MSGL_ERR_INVALID_ARG, "store_kv8: one row per request without q_indptr");
+    if (a.num_tokens == 0 || a.num_reqs == 0 || a.max_q_len == 0) return MSGL_OK;
+    if ((!a.qkv && !a.parts) || !a.q_out || !a.kv8 || !a.scales || !a.positions || !a.page_table || !a.seq_lens ||
+        !a.table || !a.qn || !a.kn)
+        return set_error(MSGL_ERR_INVALID_ARG, "store_kv8: null pointer");
+    if (!aligned16(a.qkv) || !aligned16(a.parts) || !aligned16(a.q_out) || !aligned16(a.kv8) || !aligned16(a.qn) ||
+        !aligned16(a.kn) || !aligned16(a.table))
+        return set_error(MSGL_ERR_INVALID_ARG, "store_kv8: rows must be 16-byte aligned");
+    const int64_t rows = std::min(a.max_q_len, a.num_tokens);
+    a.page_tasks = static_cast<int>((rows + kPage - 2) / kPage + 1);
+    a.q_blocks = (a.hq + 4 * kStoreWarps - 1) / (4 * kStoreWarps);
+    const int64_t tasks = static_cast<int64_t>(a.num_reqs) * a.page_tasks * a.hkv * 2;
+    const int64_t kv = (tasks + kStoreWarps - 1) / kStoreWarps;
+    const int64_t grid = kv + static_cast<int64_t>(a.num_tokens) * a.q_blocks;
+    if (tasks > INT32_MAX / 2 || grid > INT32_MAX)
+        return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "store_kv8: too many rows, requests or heads");
+    a.kv_blocks = static_cast<int>(kv);
+    a.err = device_error_word();
+    if (!a.err) return set_error(MSGL_ERR_CUDA, "device error word unavailable");
+    launch_pdl(a.parts ? qknorm_rope_store_kv8_kernel<true> : qknorm_rope_store_kv8_kernel<false>,
+               dim3(static_cast<unsigned>(grid)), dim3(kStoreWarps * 32), 0, stream, a);
+    MSGL_LAUNCH_CHECK();
+    return MSGL_OK;
+}
+
+// ------------------------------------------------------------------ attention of few rows
+// The rows of a kv head (query row x head of its group, R <= 16 TILES of them) against its pages. MMAs
+// m16n8k16 in f16: S = Q K^T with the rows as M and the 16 keys of a page as two N tiles, then
+// O^T += V^T P^T with 16 dimensions as M, 8 rows as N and the page's keys as K, where S's accumulators are
+// P^T's fragments as they stand. Codes are exact in f16; q is scaled by a power of two per row, which keeps
+// it to 2^-25 of the row's largest value; a page's scales enter the exponent,
+//   s = (q . k) 2^(q + k exponents) scale log2(e) + (exponent of v),  p = 2^(s - m) <= 2^8 in f16,
+// so that O needs no scaling by page, and l adds p 2^-(exponent of v). HBM bound: 4 KB a page and head,
+// 24 to 32 MMAs, 64 conversions.
+//
+// The pages of all (request, row block, kv head) items in a row are dealt to the CTAs in equal parts
+// (ragged contexts cost no tail); where an item is shared, its CTAs leave partial sums in the workspace
+// and the last of them to arrive joins them in order. In a CTA the pages of an item go around 8 / TILES
+// streams of warps, each with a ring of 4 KB stages that one lane fills by bulk copies across items.
+constexpr int kWarps = 8;
+constexpr int kAttThreads = kWarps * 32;
+constexpr int kPitch = kHd + 4;  // floats of a row in the joining buffer
+
+template <int NT, int TILES>
+struct RowsShape {
+    static constexpr int kStreams = kWarps / TILES;
+    static constexpr int kCtas = NT == 1 ? 2 : 1;                 // per SM
+    static constexpr int kStages = NT == 1 ? 18 : 36;             // of a CTA
+    static constexpr int kRing = kStages / kStreams;              // of a stream
+    static constexpr int kRows = NT * 8 * TILES;
+    static constexpr size_t kJoin = static_cast<size_t>(kWarps) * NT * 8 * (kPitch + 2) * 4;
+    static constexpr size_t kSmem = static_cast<size_t>(kRing) * kStreams * kKv8Bytes + kJoin;
+};
+
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ int64_t larger(int64_t a, int64_t b) { return a > b ? a : b; }
+__device__ __forceinline__ int64_t smaller(int64_t a, int64_t b) { return a < b ? a : b; }
+
+// One item's rows as a CTA sees them.
+struct Item {
+    int r, rb, h;       // request, row block, kv head
+    int L, n, q0;       // context, rows of the request, first of them
+    int row0;           // first query row of the block (of the request)
+    int rows;           // live MMA rows: query rows x group
+    int pages;          // 0 .. last visible page
+};
+
+// Context and rows of request r; n = 0 where it is skipped.
+__device__ __forceinline__ void request_rows(const Kv8AttnArgs& a, int r, bool report, int& L, int& n, int& q0) {
+    L = a.seq_lens[r];
+    q0 = a.q_indptr ? a.q_indptr[r] : r;
+    n = a.q_indptr ? a.q_indptr[r + 1] - q0 : 1;
+    if (n < 0 || n > a.max_q_len || q0 < 0 || (n > 0 && q0 > a.total_q - n)) {
+        if (report) record_error(a.err, MSGL_ERR_BOUNDS, 901);
+        n = 0;
+    }
+    if (n > 0 && (L < 0 || L > a.max_len)) {
+        if (report) record_error(a.err, MSGL_ERR_BOUNDS, 900);
+        L = L < 0 ? 0 : a.max_len;
+    }
+}
+
+// Pages that the rows [row0, row0 + count) of a request see.
+__device__ __forceinline__ int visible_pages(int L, int n, int row0, int count) {
+    const int last = L - n + min(n, row0 + count) - 1;
+    return row0 < n && last >= 0 ? last / kPage + 1 : 0;
+}
+
+// Pages of one head of all row blocks of a request.
+__device__ __forceinline__ int64_t request_pages(int L, int n, int per_block) {
+    int64_t s = 0;
+    for (int row0 = 0; row0 < n; row0 += per_block) s += visible_pages(L, n, row0, per_block);
+    return s;
+}
+
+template <int NT>
+struct RowState {
+    uint32_t q[8][NT == 1 ? 2 : 4];  // Q fragments: k step, a0 a2 (a1 a3)
+    float qs[NT];                    // 2^(q exponent) scale log2(e)
+    int lim[NT];                     // last visible key of rows g (and 8 + g); -1: no such row
+    float m[NT], l[NT];
+    float o[8][NT][4];
+};
+
+// Bytes of a word of codes that are NaN, as 0x80 each.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// NaN values at keys that only some rows see: those rows' sums become NaN. nan[v]: bytes of the lane's value
+// words (4 dimensions x 4 tokens) that hold NaN, 0x80 each.
+template <int NT>
+__device__ __forceinline__ void spread_nan(RowState<NT>& st, const uint32_t (&nan)[16], int key0, int lane) {
+    const int c = lane & 3;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+        uint32_t tok = 0;  // tokens of the page
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (nan[v] & (0x80u << (8 * e))) tok |= 1u << ((e >> 1) * 8 + 2 * c + (e & 1));
+        tok |= __shfl_xor_sync(0xffffffffu, tok, 1);
+        tok |= __shfl_xor_sync(0xffffffffu, tok, 2);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const int lim = __shfl_sync(0xffffffffu, st.lim[t], (2 * c + b) * 4);  // of row 8 t + 2 c + b
+                const int seen = min(16, lim - key0 + 1);
+                const uint32_t vis = seen <= 0 ? 0u : (1u << seen) - 1u;
+                // tile (v / 4, (v % 4) / 2): dimension rows g (even v) and 8 + g (odd v)
+                if (tok & vis) st.o[v >> 1][t][(v & 1) * 2 + b] = __int_as_float(0x7fffffff);
+            }
+    }
+}
+
+// One page: EDGE where some live row does not see all of its keys.
+template <int NT, bool EDGE>
+__device__ __forceinline__ void attend_page8(const uint8_t* page, uint32_t scale2, RowState<NT>& st, int key0, int min_lim,
+                                             int lane) {
+    const int g = lane >> 2, c = lane & 3;
+    float s[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[t][e] = 0.f;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        uint4 u[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) u[t] = *reinterpret_cast<const uint4*>(page + half * 1024 + (t * 8 + g) * 64 + c * 16);
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                uint32_t b0, b1;
+                e4m3x4_to_half(w == 0 ? u[t].x : w == 1 ? u[t].y : w == 2 ? u[t].z : u[t].w, b0, b1);
+                const uint32_t* q = st.q[half * 4 + w];
+                mma_f16_16816(s[t], q[0], NT == 1 ? 0u : q[NT == 1 ? 0 : 2], q[1], NT == 1 ? 0u : q[NT == 1 ? 0 : 3], b0, b1);
+            }
+    }
+    const float kscale = kv8_power(scale2 & 0xff);
+    const int vstored = (scale2 >> 8) & 0xff;
+    const float vexp = static_cast<float>(vstored - 127), vinv = kv8_inverse(vstored);
+    float p[NT][4];
+    bool moved = false;
+    float alpha[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const float f = st.qs[t] * kscale;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float x = fmaf(s[e >> 1][2 * t + (e & 1)], f, vexp);
+            p[t][e] = EDGE && key0 + (e >> 1) * 8 + 2 * c + (e & 1) > st.lim[t] ? kNegInf : x;
+        }
+        float mx = fmaxf(fmaxf(p[t][0], p[t][1]), fmaxf(p[t][2], p[t][3]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        // The maximum moves only where it grows by more than 8: p stays below 2^8, which f16 holds as well.
+        const bool move = mx > st.m[t] + 8.f || st.m[t] == kNegInf;
+        const float next = move ? fmaxf(mx, st.m[t]) : st.m[t];
+        alpha[t] = 1.f;
+        if (move && next != kNegInf) {
+            alpha[t] = exp2f(st.m[t] - next);
+            moved = true;
+        }
+        st.m[t] = next;
+        const float base = next == kNegInf ? 0.f : next;
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            p[t][e] = exp2f(p[t][e] - base);
+            sum += p[t][e];
+        }
+        st.l[t] = fmaf(sum, vinv, st.l[t] * alpha[t]);
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const float a0 = __shfl_sync(0xffffffffu, alpha[t], (2 * c) * 4);
+            const float a1 = __shfl_sync(0xffffffffu, alpha[t], (2 * c + 1) * 4);
+#pragma unroll
+            for (int v = 0; v < 8; ++v) {
+                st.o[v][t][0] *= a0;
+                st.o[v][t][1] *= a1;
+                st.o[v][t][2] *= a0;
+                st.o[v][t][3] *= a1;
+            }
+        }
+    }
+    uint32_t pb[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        pb[t][0] = pack_half2(p[t][0], p[t][1]);
+        pb[t][1] = pack_half2(p[t][2], p[t][3]);
+    }
+    uint32_t hidden = 0;  // 0x80 in the bytes of tokens that some live row does not see
+    if (EDGE)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (key0 + (e >> 1) * 8 + 2 * c + (e & 1) > min_lim) hidden |= 0x80u << (8 * e);
+    uint32_t nan[EDGE ? 16 : 1], any = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint4 u = *reinterpret_cast<const uint4*>(page + kKv8Values + ((g + 8 * i) * 4 + c) * 16);
+        uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (EDGE) {
+                const uint32_t bad = nan_codes(w[j]) & hidden;
+                nan[EDGE ? 4 * i + j : 0] = bad;
+                any |= bad;
+                w[j] &= ~((bad >> 7) * 0xffu);
+            }
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+            uint32_t a0, a1, a2, a3;
+            e4m3x4_to_half(w[2 * jj], a0, a2);
+            e4m3x4_to_half(w[2 * jj + 1], a1, a3);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) mma_f16_16816(st.o[2 * i + jj][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
+        }
+    }
+    if (EDGE)
+        if (__any_sync(0xffffffffu, any != 0)) spread_nan<NT>(st, reinterpret_cast<uint32_t(&)[16]>(nan), key0, lane);
+}
+
+// Q rows of a tile into fragments. Row m of the block: query row m / group, head m % group.
+template <int NT>
+__device__ __forceinline__ void load_rows(const Kv8AttnArgs& a, const Item& it, int tile, RowState<NT>& st, int lane) {
+    const int g = lane >> 2, c = lane & 3, group = a.hq / a.hkv;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int m = tile * NT * 8 + t * 8 + g;
+        const bool live = m < it.rows;
+        const int i = it.row0 + (live ? m / group : 0);
+        st.lim[t] = live ? it.L - it.n + i : -1;
+        const __nv_bfloat16* src = a.q + (static_cast<int64_t>(it.q0 + i) * a.hq + it.h * group + (live ? m % group : 0)) * kHd;
+        uint4 u[4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+            u[v] = live ? *reinterpret_cast<const uint4*>(src + (v >> 1) * kHalf + 16 * c + (v & 1) * 8) : make_uint4(0, 0, 0, 0);
+        float amax = 0.f;
+        bool bad = false;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            const uint32_t w[4] = {u[v].x, u[v].y, u[v].z, u[v].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = fmaxf(fabsf(bf16lo(w[e])), fabsf(bf16hi(w[e])));
+                amax = fmaxf(amax, x);
+                bad |= finite2(w[e]) != w[e];
+            }
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const uint32_t bads = __ballot_sync(0xffffffffu, bad) >> (4 * g) & 0xfu;
+        const int stored = max(1, min(253, static_cast<int>(__float_as_uint(amax) >> 23)));
+        const float inv = kv8_inverse(stored);
+        // a row with an infinity or a NaN has no defined logit: NaN throughout
+        st.qs[t] = bads ? __int_as_float(0x7fffffff) : kv8_power(stored) * a.sl2e;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            const uint32_t w[4] = {u[v].x, u[v].y, u[v].z, u[v].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {  // word 2 (v % 2) + e / 2 of the 16 bytes of codes, its bytes 2 (e % 2)
+                const uint32_t f = bads ? 0u : pack_half2(bf16lo(w[e]) * inv, bf16hi(w[e]) * inv);
+                st.q[(v >> 1) * 4 + (v & 1) * 2 + (e >> 1)][(NT == 1 ? 0 : 2 * t) + (e & 1)] = f;
+            }
+        }
+        st.m[t] = kNegInf;
+        st.l[t] = 0.f;
+    }
+#pragma unroll
+    for (int v = 0; v < 8; ++v)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) st.o[v][t][e] = 0.f;
+}
+
+template <int NT, int TILES>
+__global__ void __launch_bounds__(kAttThreads, RowsShape<NT, TILES>::kCtas)
+attend_rows_kernel(const Kv8AttnArgs a) {
+    using S = RowsShape<NT, TILES>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    float* join = reinterpret_cast<float*>(smem + S::kRing * S::kStreams * kKv8Bytes);
+    float* join_ml = join + kWarps * NT * 8 * kPitch;  // [warp][row]{m, l}
+    __shared__ uint64_t full[S::kStages], empty[S::kStages];
+    __shared__ uint32_t stage_scale[S::kStages];
+    __shared__ int64_t warp_sums[kWarps];
+    __shared__ int64_t s_total, s_before;
+    __shared__ int s_first, s_flag;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int stream = warp % S::kStreams, tile = warp / S::kStreams;
+    const int group = a.hq / a.hkv;
+    if (tid == 0) {
+        for (int i = 0; i < S::kStages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], TILES);
+        }
+        fence_barrier_init();
+        s_first = -1;
+    }
+    pdl_wait();
+    pdl_trigger();
+    // total pages of all items
+    const int per_block = S::kRows / group;  // query rows of a block
+    int64_t mine = 0;
+    for (int r = tid; r < a.num_reqs; r += kAttThreads) {
+        int L, n, q0;
+        request_rows(a, r, blockIdx.x == 0, L, n, q0);
+        mine += request_pages(L, n, per_block) * a.hkv;
+        // rows before the context's first token, and rows of an empty context: zeros
+        if (r % gridDim.x == blockIdx.x && n > L)
+            for (int64_t i = static_cast<int64_t>(q0) * a.hq * kHd; i < static_cast<int64_t>(q0 + min(n, n - L)) * a.hq * kHd; i += 8)
+                *reinterpret_cast<uint4*>(a.out + i) = make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) warp_sums[warp] = mine;
+    __syncthreads();
+    if (tid == 0) {
+        int64_t t = 0;
+        for (int w = 0; w < kWarps; ++w) t += warp_sums[w];
+        s_total = t;
+    }
+    __syncthreads();
+    const int64_t total = s_total;
+    const int64_t per = larger((total + gridDim.x - 1) / gridDim.x, a.min_pages);
+    const int64_t begin = per * blockIdx.x, end = min(total, begin + per);
+    if (begin >= end) return;
+    // the request of the first page: blocks of requests scanned until their sum passes `begin`
+    int64_t base = 0;
+    for (int r0 = 0; r0 < a.num_reqs; r0 += kAttThreads) {
+        const int r = r0 + tid;
+        int64_t w = 0;
+        if (r < a.num_reqs) {
+            int L, n, q0;
+            request_rows(a, r, false, L, n, q0);
+            w = request_pages(L, n, per_block) * a.hkv;
+        }
+        int64_t x = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 31) warp_sums[warp] = x;
+        __syncthreads();
+        int64_t ahead = base;
+        for (int v = 0; v < kWarps; ++v) {
+            if (v < warp) ahead += warp_sums[v];
+            base += warp_sums[v];
+        }
+        if (w > 0 && begin >= ahead + x - w && begin < ahead + x) {
+            s_first = r;
+            s_before = ahead + x - w;
+        }
+        __syncthreads();
+        if (s_first >= 0) break;
+    }
+
+    // A walk over the items from the one that holds `begin`: position of the item's first page in the row
+    // of all pages, and the item. Used twice a warp: by the filling of the ring and by its use.
+    struct Walk {
+        Item it;
+        int64_t first;
+    };
+    auto set_block = [&](Walk& w) {
+        w.it.row0 = w.it.rb * per_block;
+        w.it.rows = min(per_block, w.it.n - w.it.row0) * group;
+        w.it.pages = visible_pages(w.it.L, w.it.n, w.it.row0, per_block);
+    };
+    auto next = [&](Walk& w) {  // to the next item with any page (order: request, row block, head)
+        w.first += w.it.pages;
+        if (++w.it.h < a.hkv) return;
+        w.it.h = 0;
+        do {
+            if ((w.it.rb + 1) * per_block < w.it.n) {
+                ++w.it.rb;
+            } else {
+                w.it.rb = 0;
+                do {
+                    if (++w.it.r >= a.num_reqs) return;
+                    request_rows(a, w.it.r, false, w.it.L, w.it.n, w.it.q0);
+                } while (w.it.n <= 0);
+            }
+            set_block(w);
+        } while (w.it.pages == 0);
+    };
+    Walk use;
+    use.it.r = s_first;
+    use.it.rb = use.it.h = 0;
+    use.first = s_before;
+    request_rows(a, use.it.r, false, use.it.L, use.it.n, use.it.q0);
+    set_block(use);
+    while (use.it.pages == 0 || use.first + use.it.pages <= begin) next(use);
+
+    // ---------------- filling: the stream's first warp, a lane per page id read ahead
+    Walk fill = use;
+    int fill_page = 0, fill_end = 0;      // next page of this stream and end of the CTA's pages in the item
+    int ids = 0, ids_at = 32;             // lane j: physical page (or -1) and scales of the j-th page from here
+    uint32_t sc = 0;
+    int filled = 0;
+    auto fill_item = [&]() {
+        fill_page = static_cast<int>(larger(0, begin - fill.first)) + stream;
+        fill_end = static_cast<int>(smaller(fill.it.pages, end - fill.first));
+        ids_at = 32;
+    };
+    auto fill_one = [&]() {  // issues the stream's next page, if there is one
+        while (fill_page >= fill_end) {
+            if (fill.first + fill.it.pages >= end) return;
+            next(fill);
+            fill_item();
+        }
+        if (ids_at == 32) {
+            const int p = fill_page + lane * S::kStreams;
+            ids = 0;
+            sc = 0;
+            if (p < fill_end) {
+                ids = a.page_table[static_cast<int64_t>(fill.it.r) * a.max_pages + p];
+                if (ids < 0 || ids >= a.num_pages) {
+                    record_error(a.err, MSGL_ERR_BOUNDS, 902);
+                    ids = 0;
+                }
+                sc = *reinterpret_cast<const uint16_t*>(a.scales + (static_cast<int64_t>(ids) * a.hkv + fill.it.h) * 2);
+            }
+            ids_at = 0;
+        }
+        const int id = __shfl_sync(0xffffffffu, ids, ids_at);
+        const uint32_t scale2 = __shfl_sync(0xffffffffu, sc, ids_at);
+        const int st = stream * S::kRing + filled % S::kRing;
+        if (TILES > 1 && filled >= S::kRing) mbar_wait(&empty[st], (filled / S::kRing - 1) & 1, a.err, 903);
+        if (lane == 0) {
+            stage_scale[st] = scale2;
+            mbar_arrive_expect_tx(&full[st], kKv8Bytes);
+            bulk_load(smem + st * kKv8Bytes, a.kv8 + (static_cast<int64_t>(id) * a.hkv + fill.it.h) * kKv8Bytes, kKv8Bytes, &full[st]);
+        }
+        __syncwarp();
+        ++ids_at;
+        ++filled;
+        fill_page += S::kStreams;
+    };
+    if (tile == 0) {
+        fill_item();
+        for (int i = 0; i < S::kRing; ++i) fill_one();
+    }
+
+    RowState<NT> st;
+    int used = 0;
+    bool ok = true;
+    while (true) {
+        load_rows<NT>(a, use.it, tile, st, lane);
+        int min_lim = use.it.L - use.it.n + use.it.row0;  // the block's first query row
+        const int p0 = static_cast<int>(larger(0, begin - use.first));
+        const int p1 = static_cast<int>(smaller(use.it.pages, end - use.first));
+        for (int p = p0 + stream; p < p1; p += S::kStreams) {
+            const int sg = stream * S::kRing + used % S::kRing;
+            ok = ok && mbar_wait(&full[sg], (used / S::kRing) & 1, a.err, 904);
+            const uint8_t* page = smem + sg * kKv8Bytes;
+            const uint32_t scale2 = stage_scale[sg];
+            if (__all_sync(0xffffffffu, ok)) {
+                if (p * kPage + kPage - 1 > min_lim) attend_page8<NT, true>(page, scale2, st, p * kPage, min_lim, lane);
+                else attend_page8<NT, false>(page, scale2, st, p * kPage, min_lim, lane);
+            }
+            __syncwarp();
+            if (TILES > 1 && lane == 0) mbar_arrive(&empty[sg]);
+            ++used;
+            if (tile == 0) fill_one();
+        }
+        // ---------------- join the streams: unnormalised sums and (m, l) of each warp through shared memory
+        const int g = lane >> 2, c = lane & 3;
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float l = st.l[t];
+            l += __shfl_xor_sync(0xffffffffu, l, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
+            if (c == 0) {
+                join_ml[(warp * NT * 8 + t * 8 + g) * 2] = st.m[t];
+                join_ml[(warp * NT * 8 + t * 8 + g) * 2 + 1] = l;
+            }
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    join[(warp * NT * 8 + t * 8 + 2 * c + (e & 1)) * kPitch + 4 * (g + 8 * (v >> 1)) + 2 * (v & 1) + (e >> 1)] = st.o[v][t][e];
+        }
+        __syncthreads();
+        const int a0 = static_cast<int>(use.first / per), a1 = static_cast<int>((use.first + use.it.pages - 1) / per);
+        const bool whole = a0 == a1;
+        // a CTA takes part in at most one item that it did not begin and one that it does not end
+        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (static_cast<int>(blockIdx.x) != a0 ? 0 : 1);
+        for (int i = tid; i < use.it.rows * (kHd / 4); i += kAttThreads) {
+            const int m = i / (kHd / 4), d = i % (kHd / 4) * 4;
+            const int t0 = m / (NT * 8), mr = m % (NT * 8);
+            float M = kNegInf;
+            for (int s = 0; s < S::kStreams; ++s) M = fmaxf(M, join_ml[((t0 * S::kStreams + s) * NT * 8 + mr) * 2]);
+            float l = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int s = 0; s < S::kStreams; ++s) {
+                const int w = (t0 * S::kStreams + s) * NT * 8 + mr;
+                const float ms = join_ml[2 * w];
+                // a stream without a visible key has l = 0 (or NaN where a NaN was seen)
+                const float f = ms == kNegInf ? 1.f : exp2f(ms - M);
+                const float4 x = *reinterpret_cast<const float4*>(join + w * kPitch + d);
+                l += join_ml[2 * w + 1] * f;
+                o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
+            }
+            if (whole) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                uint2 u = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+                *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(use.it.q0 + use.it.row0 + m / group) * a.hq + use.it.h * group + m % group) * kHd + d) = u;
+            } else {
+                *reinterpret_cast<float4*>(a.ws_o + (slot * S::kRows + m) * kHd + d) = o;
+                if (d == 0) {
+                    a.ws_ml[(slot * S::kRows + m) * 2] = M;
+                    a.ws_ml[(slot * S::kRows + m) * 2 + 1] = l;
+                }
+            }
+        }
+        if (!whole) {
+            __threadfence();
+            __syncthreads();
+            int* count = a.ws_count + (static_cast<int64_t>(use.it.r) * a.row_blocks + use.it.rb) * a.hkv + use.it.h;
+            if (tid == 0) s_flag = atomicAdd(count, 1) == a1 - a0;
+            __syncthreads();
+            if (s_flag) {
+                __threadfence();
+                for (int i = tid; i < use.it.rows * (kHd / 4); i += kAttThreads) {
+                    const int m = i / (kHd / 4), d = i % (kHd / 4) * 4;
+                    float M = kNegInf, l = 0.f;
+                    for (int b = a0; b <= a1; ++b) M = fmaxf(M, __ldcg(a.ws_ml + ((2 * static_cast<int64_t>(b) + (b == a0)) * S::kRows + m) * 2));
+                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                    for (int b = a0; b <= a1; ++b) {
+                        const int64_t w = (2 * static_cast<int64_t>(b) + (b == a0)) * S::kRows + m;
+                        const float ms = __ldcg(a.ws_ml + 2 * w);
+                        const float f = ms == kNegInf ? 1.f : exp2f(ms - M);
+                        const float4 x = __ldcg(reinterpret_cast<const float4*>(a.ws_o + w * kHd + d));
+                        l += __ldcg(a.ws_ml + 2 * w + 1) * f;
+                        o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
+                    }
+                    const float inv = l == 0.f ? 0.f : 1.f / l;
+                    uint2 u = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+                    *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(use.it.q0 + use.it.row0 + m / group) * a.hq + use.it.h * group + m % group) * kHd + d) = u;
+                }
+                if (tid == 0) *count = 0;
+            }
+        }
+        if (use.first + use.it.pages >= end) break;
+        next(use);
+    }
+}
+
+// ------------------------------------------------------------------ host side
+// Counters of every (request, row block, kv head), then the partial sums of two items a CTA.
+struct RowsPlan {
+    int nt, tiles, rows, row_blocks, grid;
+    size_t off_o, off_ml, bytes;
+};
+
+RowsPlan plan_rows(int num_reqs, int max_q_len, int hq, int hkv) {
+    RowsPlan p{};
+    const int group = hq / hkv;
+    const int64_t rows = static_cast<int64_t>(max_q_len) * group;
+    p.nt = rows <= 8 ? 1 : 2;
+    p.tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    p.rows = 8 * p.nt * p.tiles;
+    p.row_blocks = std::max(1, (max_q_len + p.rows / group - 1) / (p.rows / group));
+    p.grid = 148 * (p.nt == 1 ? 2 : 1);
+    const size_t count = (static_cast<size_t>(num_reqs) * p.row_blocks * hkv * 4 + 255) / 256 * 256;
+    p.off_o = count;
+    p.off_ml = count + static_cast<size_t>(p.grid) * 2 * p.rows * kHd * 4;
+    p.bytes = p.off_ml + static_cast<size_t>(p.grid) * 2 * p.rows * 8;
+    return p;
+}
+
+template <int NT, int TILES>
+int launch_rows(const Kv8AttnArgs& a, int grid, msgl_stream_t stream) {
+    using S = RowsShape<NT, TILES>;
+    static std::atomic<int> optin[kMaxDevices];
+    const cudaError_t e = smem_optin(attend_rows_kernel<NT, TILES>, S::kSmem, optin);
+    if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
+    launch_pdl(attend_rows_kernel<NT, TILES>, dim3(grid), dim3(kAttThreads), S::kSmem, stream, a);
+    MSGL_LAUNCH_CHECK();
+    return MSGL_OK;
+}
+
+int check_attend(int num_reqs, int total_q, int max_q_len, int max_seq_len, int hq, int hkv, int head_dim, int page_size) {
+    if (head_dim != kHd) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "attention_kv8: head_dim must be 128");
+    if (page_size != kPage) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "attention_kv8: page_size must be 16");
+    if (num_reqs < 0 || total_q < 0 || max_q_len < 0 || max_seq_len < 0 || hq <= 0 || hkv <= 0 || hq % hkv)
+        return set_error(MSGL_ERR_INVALID_ARG, "attention_kv8: bad sizes or Hq % Hkv != 0");
+    const int group = hq / hkv;
+    if (group > 8 || (group & (group - 1)))
+        return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "attention_kv8: Hq / Hkv must be 1, 2, 4 or 8");
+    if (num_reqs > 65535 || hkv > 1024 || total_q > 1 << 24)
+        return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "attention_kv8: too many requests, heads or rows");
+    return MSGL_OK;
+}
+
+}  // namespace
+}  // namespace msgl
+
+using namespace msgl;
+
+extern "C" {
+
+int msgl_qknorm_rope_store_kv8(const void* qkv, void* q_out, void* kv8, void* scales, int64_t num_pages,
+                               const int* positions, const int* page_table, int max_pages, const int* seq_lens,
+                               const int* q_indptr, int num_reqs, int max_q_len, const float* cos_sin_cache,
+                               int max_position, const void* q_norm_w, const void* k_norm_w, int num_tokens,
+                               int num_q_heads, int num_kv_heads, int head_dim, int page_size, float eps,
+                               msgl_stream_t stream) {
+    StoreArgs a = {};
+    a.qkv = static_cast<const __nv_bfloat16*>(qkv);
+    a.q_out = static_cast<__nv_bfloat16*>(q_out);
+    a.kv8 = static_cast<uint8_t*>(kv8);
+    a.scales = static_cast<uint8_t*>(scales);
+    a.num_pages = num_pages;
+    a.positions = positions;
+    a.page_table = page_table;
+    a.max_pages = max_pages;
+    a.seq_lens = seq_lens;
+    a.q_indptr = q_indptr;
+    a.num_reqs = num_reqs;
+    a.max_q_len = max_q_len;
+    a.table = cos_sin_cache;
+    a.max_position = max_position;
+    a.qn = static_cast<const __nv_bfloat16*>(q_norm_w);
+    a.kn = static_cast<const __nv_bfloat16*>(k_norm_w);
+    a.num_tokens = num_tokens;
+    a.hq = num_q_heads;
+    a.hkv = num_kv_heads;
+    a.eps = eps;
+    return launch_store(a, head_dim, page_size, stream);
+}
+
+int msgl_qknorm_rope_store_kv8_partials(const float* parts, int nparts, void* q_out, void* kv8, void* scales,
+                                        int64_t num_pages, const int* positions, const int* page_table,
+                                        int max_pages, const int* seq_lens, const int* q_indptr, int num_reqs,
+                                        int max_q_len, const float* cos_sin_cache, int max_position,
+                                        const void* q_norm_w, const void* k_norm_w, int num_tokens,
+                                        int num_q_heads, int num_kv_heads, int head_dim, int page_size,
+                                        float eps, msgl_stream_t stream) {
+    if (!parts || nparts < 1 || nparts > 64)
+        return set_error(MSGL_ERR_INVALID_ARG, "store_kv8_partials: parts / nparts in [1, 64]");
+    StoreArgs a = {};
+    a.parts = parts;
+    a.nparts = nparts;
+    a.q_out = static_cast<__nv_bfloat16*>(q_out);
+    a.kv8 = static_cast<uint8_t*>(kv8);
+    a.scales = static_cast<uint8_t*>(scales);
+    a.num_pages = num_pages;
+    a.positions = positions;
+    a.page_table = page_table;
+    a.max_pages = max_pages;
+    a.seq_lens = seq_lens;
+    a.q_indptr = q_indptr;
+    a.num_reqs = num_reqs;
+    a.max_q_len = max_q_len;
+    a.table = cos_sin_cache;
+    a.max_position = max_position;
+    a.qn = static_cast<const __nv_bfloat16*>(q_norm_w);
+    a.kn = static_cast<const __nv_bfloat16*>(k_norm_w);
+    a.num_tokens = num_tokens;
+    a.hq = num_q_heads;
+    a.hkv = num_kv_heads;
+    a.eps = eps;
+    return launch_store(a, head_dim, page_size, stream);
+}
+
+size_t msgl_paged_attention_kv8_workspace_size(int num_reqs, int max_q_len, int num_q_heads, int num_kv_heads) {
+    if (num_reqs <= 0 || max_q_len <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads ||
+        num_q_heads / num_kv_heads > 8 || num_reqs > 65535 || num_kv_heads > 1024)
+        return 0;
+    // the largest of the forms that this call or a smaller one may take
+    const int group = num_q_heads / num_kv_heads;
+    size_t most = plan_rows(num_reqs, max_q_len, num_q_heads, num_kv_heads).bytes;
+    for (int rows = 8; rows <= 32; rows *= 2)
+        most = std::max(most, plan_rows(num_reqs, std::min(max_q_len, rows / group), num_q_heads, num_kv_heads).bytes);
+    return most;
+}
+
+int msgl_paged_attention_kv8(const void* q, const void* kv8, const void* scales, int64_t num_pages,
+                             const int* page_table, int max_pages, const int* seq_lens, const int* q_indptr,
+                             int num_reqs, int total_q, int max_q_len, int max_seq_len, int num_q_heads,
+                             int num_kv_heads, int head_dim, int page_size, float scale, void* out,
+                             void* workspace, size_t workspace_bytes, msgl_stream_t stream) {
+    int rc = check_attend(num_reqs, total_q, max_q_len, max_seq_len, num_q_heads, num_kv_heads, head_dim, page_size);
+    if (rc) return rc;
+    if (num_pages <= 0 || num_pages > INT32_MAX || max_pages <= 0 || max_seq_len > static_cast<int64_t>(max_pages) * kPage)
+        return set_error(MSGL_ERR_INVALID_ARG, "attention_kv8: bad pool or page-table width");
+    if (!q_indptr && (max_q_len != 1 || total_q != num_reqs))
+        return set_error(MSGL_ERR_INVALID_ARG, "attention_kv8: one row per request without q_indptr");
+    if (num_reqs == 0 || total_q == 0 || max_q_len == 0) return MSGL_OK;
+    if (!q || !kv8 || !scales || !page_table || !seq_lens || !out)
+        return set_error(MSGL_ERR_INVALID_ARG, "attention_kv8: null pointer");
+    if (!aligned16(q) || !aligned16(kv8) || !aligned16(out) || (reinterpret_cast<uintptr_t>(scales) & 1))
+        return set_error(MSGL_ERR_INVALID_ARG, "attention_kv8: q, kv8 and out must be 16-byte aligned, scales 2-byte");
+    Kv8AttnArgs a = {};
+    a.q = static_cast<const __nv_bfloat16*>(q);
+    a.kv8 = static_cast<const uint8_t*>(kv8);
+    a.scales = static_cast<const uint8_t*>(scales);
+    a.num_pages = num_pages;
+    a.page_table = page_table;
+    a.max_pages = max_pages;
+    a.max_len = max_seq_len;
+    a.seq_lens = seq_lens;
+    a.q_indptr = q_indptr;
+    a.num_reqs = num_reqs;
+    a.total_q = total_q;
+    a.max_q_len = std::min(max_q_len, total_q);
+    a.hq = num_q_heads;
+    a.hkv = num_kv_heads;
+    a.sl2e = scale * 1.4426950408889634f;
+    a.out = static_cast<__nv_bfloat16*>(out);
+    const RowsPlan p = plan_rows(num_reqs, a.max_q_len, num_q_heads, num_kv_heads);
+    if (!workspace || workspace_bytes < p.bytes || !aligned16(workspace))
+        return set_error(MSGL_ERR_WORKSPACE, "attention_kv8: workspace missing, too small or not 16-byte aligned");
+    a.err = device_error_word();
+    if (!a.err) return set_error(MSGL_ERR_CUDA, "device error word unavailable");
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    a.ws_count = reinterpret_cast<int*>(ws);
+    a.ws_o = reinterpret_cast<float*>(ws + p.off_o);
+    a.ws_ml = reinterpret_cast<float*>(ws + p.off_ml);
+    a.row_blocks = p.row_blocks;
+    a.min_pages = 8;
+    if (p.nt == 1) return launch_rows<1, 1>(a, p.grid, stream);
+    if (p.tiles == 1) return launch_rows<2, 1>(a, p.grid, stream);
+    if (p.tiles == 2) return launch_rows<2, 2>(a, p.grid, stream);
+    return launch_rows<2, 4>(a, p.grid, stream);
+}
+
+}  // extern "C"

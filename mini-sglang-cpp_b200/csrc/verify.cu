@@ -1,0 +1,446 @@
+// verify.cu -- probabilities of logits, and the verification of drafted tokens against them.
+//
+//  * msgl_token_probs    p = softmax(logits / temperature) per row, one-hot where greedy
+//  * msgl_verify_drafts  speculative sampling (Leviathan, Kalman, Matias, "Fast inference from
+//                        transformers via speculative decoding", ICML 2023): draft i with target
+//                        probability p and draft probability q is accepted iff u q < p; the token behind
+//                        the accepted ones is drawn from max(p - q, 0) of the first rejected draft's rows,
+//                        or from the target's last row. With given uniform numbers nothing is random.
+//
+// Comparisons and running sums that decide a token are in 64 bits: of 150k borders in [0, 1), fp32 sums
+// put one in thirty uniform numbers on the wrong side, 64-bit sums one in 10^9.
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace msgl {
+namespace {
+
+constexpr int kProbThreads = 512;
+constexpr int kProbValues = 40;  // of a row, per thread, in registers
+constexpr int kMaxCluster = 16;
+constexpr float kNegInf = -__builtin_huge_valf();
+
+__device__ __forceinline__ double ld_dsmem_f64(uint32_t addr) {
+    double v;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+// Larger float -> larger key, NaN above all; then the smaller index.
+__device__ __forceinline__ unsigned long long argmax_key(float v, uint32_t i) {
+    const uint32_t u = v != v ? 0x7fffffffu : __float_as_uint(v);
+    const uint32_t k = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    return (static_cast<unsigned long long>(k) << 32) | (0xffffffffu - i);
+}
+
+// ------------------------------------------------------------------ probabilities
+// A row is read once and written once: the cluster's threads hold it in registers (VEC consecutive
+// values at a time), each CTA takes the maximum and the sum of its own part, and one exchange through
+// distributed shared memory joins them: p = exp(x - m_cta) * (exp(m_cta - m) / sum). HBM bound.
+template <int VEC>
+__global__ void __launch_bounds__(kProbThreads)
+token_probs_kernel(const float* logits, int64_t ldx, const float* __restrict__ temperature, float* probs,
+                   int64_t ldp, int vocab, int part) {
+    constexpr int kVecs = kProbValues / VEC;
+    __shared__ float red[kProbThreads / 32];
+    __shared__ unsigned long long red_key[kProbThreads / 32];
+    __shared__ __align__(8) float mine[2];  // the CTA's maximum and sum, read by the cluster
+    __shared__ unsigned long long mine_key;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = cluster_ctarank(), size = cluster_nctarank();
+    pdl_wait();
+    pdl_trigger();
+    const int64_t row = cluster_id_x();
+    const float* x = logits + row * ldx;
+    const float T = temperature ? temperature[row] : 1.f;
+    const int begin = rank * part, end = min(vocab, begin + part);  // a multiple of VEC but for the row's end
+    float v[kProbValues];
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+        const int i = begin + (k * kProbThreads + tid) * VEC;
+        if (VEC == 4) {
+            const float4 f = i < end ? *reinterpret_cast<const float4*>(x + i) : make_float4(kNegInf, kNegInf, kNegInf, kNegInf);
+            v[4 * k] = f.x; v[4 * k + 1] = f.y; v[4 * k + 2] = f.z; v[4 * k + 3] = f.w;
+        } else {
+            v[k] = i < end ? x[i] : kNegInf;
+        }
+    }
+    if (!(T <= 0.f)) {
+        const float c = fminf(1.4426950408889634f / T, 3.0e38f);
+        float m = kNegInf;
+#pragma unroll
+        for (int e = 0; e < kProbValues; ++e) m = fmaxf(m, v[e]);
+        m = warp_max(m);
+        if (lane == 0) red[warp] = m;
+        __syncthreads();
+        m = kNegInf;
+#pragma unroll
+        for (int w = 0; w < kProbThreads / 32; ++w) m = fmaxf(m, red[w]);
+        // a part without a finite value adds nothing (NaN still does)
+        const float base = m == kNegInf ? 0.f : m;
+        float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < kProbValues; ++e) {
+            v[e] = exp2f((v[e] - base) * c);
+            s4[e & 3] += v[e];
+        }
+        float s = warp_sum((s4[0] + s4[1]) + (s4[2] + s4[3]));
+        __syncthreads();
+        if (lane == 0) red[warp] = s;
+        __syncthreads();
+        s = 0.f;
+#pragma unroll
+        for (int w = 0; w < kProbThreads / 32; ++w) s += red[w];
+        if (tid == 0) {
+            mine[0] = m;
+            mine[1] = s;
+        }
+        cluster_sync_all();
+        // lane q: CTA q's maximum and sum
+        float mq = kNegInf, sq = 0.f;
+        if (lane < size) {
+            mq = ld_dsmem_f32(mapa_shared(smem_u32(&mine[0]), lane));
+            sq = ld_dsmem_f32(mapa_shared(smem_u32(&mine[1]), lane));
+        }
+        const float M = warp_max(mq);
+        const float S = warp_sum(mq == kNegInf ? sq : sq * exp2f((mq - M) * c));
+        cluster_arrive();  // this CTA's peers are read; waited for at the end
+        // a row without any finite logit: S = 0, zeros (S is NaN where a logit is NaN or +inf)
+        const float f = S == 0.f ? 0.f : (m == kNegInf ? 1.f : exp2f((m - M) * c)) / S;
+#pragma unroll
+        for (int e = 0; e < kProbValues; ++e) v[e] *= f;
+    } else {
+        unsigned long long best = 0;
+#pragma unroll
+        for (int e = 0; e < kProbValues; ++e) {
+            const int i = begin + ((e / VEC) * kProbThreads + tid) * VEC + e % VEC;
+            const unsigned long long key = argmax_key(v[e], i);
+            if (i < end && key > best) best = key;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const unsigned long long y = __shfl_xor_sync(0xffffffffu, best, o);
+            best = y > best ? y : best;
+        }
+        if (lane == 0) red_key[warp] = best;
+        __syncthreads();
+        best = 0;
+#pragma unroll
+        for (int w = 0; w < kProbThreads / 32; ++w) best = red_key[w] > best ? red_key[w] : best;
+        if (tid == 0) mine_key = best;
+        cluster_sync_all();
+        for (int q = 0; q < size; ++q) {
+            const unsigned long long y = __double_as_longlong(ld_dsmem_f64(mapa_shared(smem_u32(&mine_key), q)));
+            best = y > best ? y : best;
+        }
+        cluster_arrive();
+        const int top = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best));
+#pragma unroll
+        for (int e = 0; e < kProbValues; ++e)
+            v[e] = begin + ((e / VEC) * kProbThreads + tid) * VEC + e % VEC == top ? 1.f : 0.f;
+    }
+    float* p = probs + row * ldp;
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+        const int i = begin + (k * kProbThreads + tid) * VEC;
+        if (i >= end) continue;
+        if (VEC == 4) *reinterpret_cast<float4*>(p + i) = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+        else p[i] = v[k];
+    }
+    cluster_wait();  // no CTA leaves while its shared memory may be read
+}
+
+// ------------------------------------------------------------------ verification
+// One cluster per request. Every CTA finds the first rejected draft (two loads a draft) and takes one
+// range of the vocabulary of that draft's rows; its warps take consecutive parts of the range and sum
+// their weights. One exchange of the CTAs' sums gives every CTA the total and what lies before it; the
+// warp whose part holds u * total walks that part again, 128 values at a time. HBM bound for many
+// requests, a chain of four latencies (drafts, rows, exchange, walk) for one.
+constexpr int kVerThreads = 512;
+constexpr int kVerWarps = kVerThreads / 32;
+
+struct VerifyArgs {
+    const float* p;
+    int64_t ldp;
+    const float* q;  // null: draft i has probability 1 for its token
+    int64_t ldq;
+    const int *drafts, *indptr;
+    const float *u, *u_last;
+    int num_drafts, max_drafts, vocab, part;
+    int *accepted, *tokens;
+    int* err;
+};
+
+__device__ __forceinline__ double warp_sum64(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// Weight of a token: p - q where positive (NaN: none).
+__device__ __forceinline__ double rest_of(float p, float q) {
+    const double w = static_cast<double>(p) - static_cast<double>(q);
+    return w > 0.0 ? w : 0.0;
+}
+
+template <int VEC>
+__device__ __forceinline__ void load_values(const float* row, int i, int end, float (&v)[4]) {
+    if (VEC == 4) {
+        const float4 f = i < end ? __ldg(reinterpret_cast<const float4*>(row + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = i + e < end ? __ldg(row + i + e) : 0.f;
+    }
+}
+
+template <int VEC>
+__global__ void __launch_bounds__(kVerThreads)
+verify_drafts_kernel(const VerifyArgs a) {
+    __shared__ double warp_rest[kVerWarps], warp_all[kVerWarps];
+    __shared__ __align__(8) double mine[2];  // sums of max(p - q, 0) and of p over this CTA's range
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = cluster_ctarank(), size = cluster_nctarank();
+    pdl_wait();
+    pdl_trigger();
+    const int r = cluster_id_x();
+    const int d0 = a.indptr[r], k = a.indptr[r + 1] - d0;
+    int* out = a.tokens + static_cast<int64_t>(r) * (a.max_drafts + 1);
+    if (d0 < 0 || k < 0 || k > a.max_drafts || d0 > a.num_drafts - k) {  // the same for the whole cluster
+        if (rank == 0) {
+            for (int i = tid; i <= a.max_drafts; i += kVerThreads) out[i] = -1;
+            if (tid == 0) {
+                a.accepted[r] = 0;
+                record_error(a.err, MSGL_ERR_BOUNDS, 920);
+            }
+        }
+        return;
+    }
+    const float* p0 = a.p + (static_cast<int64_t>(d0) + r) * a.ldp;
+    // the first rejected draft, by every warp for itself
+    int n = k;
+    for (int b = 0; b < k && n == k; b += 32) {
+        const int i = b + lane;
+        bool rejected = false;
+        if (i < k) {
+            const int x = a.drafts[d0 + i];
+            rejected = true;
+            if (x >= 0 && x < a.vocab) {
+                const float px = __ldg(p0 + i * a.ldp + x);
+                const float qx = a.q ? __ldg(a.q + (static_cast<int64_t>(d0) + i) * a.ldq + x) : 1.f;
+                rejected = !(static_cast<double>(a.u[d0 + i]) * static_cast<double>(qx) < static_cast<double>(px));
+            } else if (rank == 0 && warp == 0) {
+                record_error(a.err, MSGL_ERR_BOUNDS, 921);
+            }
+        }
+        const uint32_t any = __ballot_sync(0xffffffffu, rejected);
+        if (any) n = b + __ffs(any) - 1;
+    }
+    const float* prow = p0 + n * a.ldp;
+    const float* qrow = n < k && a.q ? a.q + (static_cast<int64_t>(d0) + n) * a.ldq : nullptr;
+    const int point = n < k && !a.q ? a.drafts[d0 + n] : -1;  // weight of this token: p - 1 <= 0
+    // this warp's part of the CTA's range
+    const int begin = min(a.vocab, rank * a.part), end = min(a.vocab, begin + a.part);
+    const int share = (a.part / 128 + kVerWarps - 1) / kVerWarps * 128;
+    const int w0 = min(end, begin + warp * share), w1 = min(end, w0 + share);
+    double rest = 0.0, all = 0.0;
+#pragma unroll 4
+    for (int i = w0 + lane * 4; i < w1; i += 128) {
+        float pv[4], qv[4] = {0.f, 0.f, 0.f, 0.f};
+        load_values<VEC>(prow, i, w1, pv);
+        if (qrow) load_values<VEC>(qrow, i, w1, qv);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (i + e == point) qv[e] = 1.f;
+            rest += rest_of(pv[e], qv[e]);
+            all += rest_of(pv[e], 0.f);
+        }
+    }
+    rest = warp_sum64(rest);
+    all = warp_sum64(all);
+    if (lane == 0) {
+        warp_rest[warp] = rest;
+        warp_all[warp] = all;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        double s = 0.0, t = 0.0;
+        for (int w = 0; w < kVerWarps; ++w) {
+            s += warp_rest[w];
+            t += warp_all[w];
+        }
+        mine[0] = s;
+        mine[1] = t;
+    }
+    cluster_sync_all();
+    double total[2] = {0.0, 0.0}, before[2] = {0.0, 0.0}, here[2] = {0.0, 0.0};
+    int last_part[2] = {-1, -1};  // last CTA with any weight
+    for (int c = 0; c < size; ++c)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const double s = ld_dsmem_f64(mapa_shared(smem_u32(&mine[j]), c));
+            if (c == rank) {
+                before[j] = total[j];
+                here[j] = s;
+            }
+            total[j] += s;
+            if (s > 0.0) last_part[j] = c;
+        }
+    cluster_arrive();
+    // where p <= q everywhere (rounding), the target's own row
+    const int j = total[0] > 0.0 ? 0 : 1;
+    const double* parts = j == 0 ? warp_rest : warp_all;
+    const bool fine = total[j] > 0.0 && total[j] < __longlong_as_double(0x7ff0000000000000ll);
+    double goal = static_cast<double>(a.u_last[r]) * total[j];
+    if (!(goal >= 0.0)) goal = 0.0;
+    if (rank == 0) {
+        for (int i = tid; i <= a.max_drafts; i += kVerThreads)
+            if (i != n || !fine) out[i] = i < n ? a.drafts[d0 + i] : -1;
+        if (tid == 0) {
+            a.accepted[r] = n;
+            if (!fine) record_error(a.err, MSGL_ERR_BOUNDS, 922);
+        }
+    }
+    // The first place whose running sum passes the goal lies in this CTA (in the last one with any
+    // weight where u is 1 or more).
+    const bool holds = here[j] > 0.0 && before[j] <= goal && (goal < before[j] + here[j] || rank == last_part[j]);
+    if (fine && holds) {
+        double sum = before[j];
+        int pick = -1, last = -1;
+        for (int w = 0; w < kVerWarps; ++w) {
+            if (parts[w] > 0.0) last = w;
+            if (pick < 0 && goal < sum + parts[w]) pick = w;
+            if (pick < 0) sum += parts[w];
+        }
+        if (pick < 0) {  // the sums over warps and over CTAs round differently
+            pick = last;
+            sum -= parts[last];
+        }
+        if (warp == pick) {
+            int found = -1, weighty = -1;  // weighty: the last token with any weight
+            for (int b = w0; b < w1 && found < 0; b += 128) {
+                const int i = b + lane * 4;
+                float pv[4], qv[4] = {0.f, 0.f, 0.f, 0.f};
+                load_values<VEC>(prow, i, w1, pv);
+                if (qrow && j == 0) load_values<VEC>(qrow, i, w1, qv);
+                double wv[4], own = 0.0;
+                int mine_last = -1;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (i + e == point && j == 0) qv[e] = 1.f;
+                    wv[e] = rest_of(pv[e], qv[e]);
+                    own += wv[e];
+                    if (wv[e] > 0.0) mine_last = i + e;
+                }
+                double upto = own;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double y = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += y;
+                }
+                weighty = max(weighty, __reduce_max_sync(0xffffffffu, mine_last));
+                const uint32_t passed = __ballot_sync(0xffffffffu, own > 0.0 && goal < sum + upto);
+                if (passed) {
+                    const int lead = __ffs(passed) - 1;
+                    int at = -1;
+                    double c = sum + upto - own;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        c += wv[e];
+                        if (at < 0 && wv[e] > 0.0 && goal < c) at = i + e;
+                    }
+                    if (at < 0) at = mine_last;
+                    found = __shfl_sync(0xffffffffu, at, lead);
+                }
+                sum += __shfl_sync(0xffffffffu, upto, 31);
+            }
+            if (lane == 0) out[n] = found >= 0 ? found : weighty;
+        }
+    }
+    cluster_wait();
+}
+
+// CTAs of a row or request: a power of two, enough for `fit`, doubled while the GPU has room.
+int cluster_size(int64_t rows, int fit) {
+    int c = 1;
+    while (c < fit) c *= 2;
+    while (c < kMaxCluster && rows * c < 148) c *= 2;
+    return c;
+}
+
+template <typename... K>
+cudaError_t allow_large_clusters(void (*kernel)(K...), std::atomic<int> (&done)[kMaxDevices]) {
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const auto set = [&](int want) {
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, want);
+    };
+    if (dev < 0 || dev >= kMaxDevices) return set(1);
+    return raise_limit(done[dev], 1, set);
+}
+
+}  // namespace
+}  // namespace msgl
+
+using namespace msgl;
+
+extern "C" {
+
+int msgl_token_probs(const float* logits, int64_t ldx, int num_rows, int vocab, const float* temperature,
+                     float* probs, int64_t ldp, msgl_stream_t stream) {
+    if (num_rows < 0 || vocab <= 0 || ldx < vocab || ldp < vocab)
+        return set_error(MSGL_ERR_INVALID_ARG, "token_probs: bad sizes");
+    constexpr int kPer = kProbThreads * kProbValues;
+    if (vocab > kPer * kMaxCluster)
+        return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "token_probs: vocab above 327680");
+    if (num_rows > INT32_MAX / kMaxCluster) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "token_probs: too many rows");
+    if (num_rows == 0) return MSGL_OK;
+    if (!logits || !probs) return set_error(MSGL_ERR_INVALID_ARG, "token_probs: null pointer");
+    if (logits == probs && ldx != ldp) return set_error(MSGL_ERR_INVALID_ARG, "token_probs: in place with another stride");
+    const bool vec = vocab % 4 == 0 && ldx % 4 == 0 && ldp % 4 == 0 && aligned16(logits) && aligned16(probs);
+    const int size = cluster_size(num_rows, (vocab + kPer - 1) / kPer);
+    const int part = ((vocab + size - 1) / size + 3) / 4 * 4;
+    static std::atomic<int> large4[kMaxDevices], large1[kMaxDevices];
+    const cudaError_t e = size <= 8 ? cudaSuccess
+                          : vec ? allow_large_clusters(token_probs_kernel<4>, large4)
+                                : allow_large_clusters(token_probs_kernel<1>, large1);
+    if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
+    launch_cluster(vec ? token_probs_kernel<4> : token_probs_kernel<1>, static_cast<int64_t>(num_rows) * size,
+                   kProbThreads, size, 0, stream, logits, ldx, temperature, probs, ldp, vocab, part);
+    MSGL_LAUNCH_CHECK();
+    return MSGL_OK;
+}
+
+int msgl_verify_drafts(const float* target_probs, int64_t ldp, const float* draft_probs, int64_t ldq,
+                       const int* draft_tokens, const int* draft_indptr, const float* uniforms,
+                       const float* last_uniforms, int num_reqs, int num_drafts, int max_drafts, int vocab,
+                       int* accepted, int* tokens, msgl_stream_t stream) {
+    if (num_reqs < 0 || num_drafts < 0 || max_drafts < 0 || vocab <= 0 || ldp < vocab || (draft_probs && ldq < vocab))
+        return set_error(MSGL_ERR_INVALID_ARG, "verify_drafts: bad sizes");
+    if (vocab > 1 << 30 || num_reqs > INT32_MAX / kMaxCluster || max_drafts > 1 << 20)
+        return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "verify_drafts: too many requests, drafts or tokens");
+    if (num_reqs == 0) return MSGL_OK;
+    if (!target_probs || !draft_indptr || !last_uniforms || !accepted || !tokens ||
+        (num_drafts > 0 && (!draft_tokens || !uniforms)))
+        return set_error(MSGL_ERR_INVALID_ARG, "verify_drafts: null pointer");
+    const bool vec = vocab % 4 == 0 && ldp % 4 == 0 && aligned16(target_probs) &&
+                     (!draft_probs || (ldq % 4 == 0 && aligned16(draft_probs)));
+    const int size = cluster_size(num_reqs, 1);
+    const int part = ((vocab + size - 1) / size + 127) / 128 * 128;
+    static std::atomic<int> large4[kMaxDevices], large1[kMaxDevices];
+    const cudaError_t e = size <= 8 ? cudaSuccess
+                          : vec ? allow_large_clusters(verify_drafts_kernel<4>, large4)
+                                : allow_large_clusters(verify_drafts_kernel<1>, large1);
+    if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
+    const VerifyArgs a = {target_probs, ldp, draft_probs, ldq, draft_tokens, draft_indptr, uniforms, last_uniforms,
+                          num_drafts, max_drafts, vocab, part, accepted, tokens, device_error_word()};
+    if (!a.err) return set_error(MSGL_ERR_CUDA, "device error word unavailable");
+    launch_cluster(vec ? verify_drafts_kernel<4> : verify_drafts_kernel<1>, static_cast<int64_t>(num_reqs) * size,
+                   kVerThreads, size, 0, stream, a);
+    MSGL_LAUNCH_CHECK();
+    return MSGL_OK;
+}
+
+}  // extern "C"

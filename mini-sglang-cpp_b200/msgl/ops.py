@@ -6,6 +6,7 @@ current torch stream. No function here computes anything itself.
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import torch
 
@@ -188,6 +189,79 @@ def decode_advance(next_tokens, input_ids, positions, slot_mapping, page_table, 
                                     _p(seq_lens), _p(free_pages), _p(free_top), B, page_size, _s()))
 
 
+class StepTables(NamedTuple):
+    """What step_tables writes (device int32)."""
+    seq_lens: torch.Tensor      # [B]
+    q_indptr: torch.Tensor      # [B + 1]
+    positions: torch.Tensor     # [T]
+    slot_mapping: torch.Tensor  # [T]
+    last_idx: torch.Tensor      # [B]
+
+
+def step_tables_buffers(num_reqs, num_tokens, device="cuda"):
+    """Buffers that step_tables fills, for up to num_tokens rows (kept from step to step)."""
+    return StepTables(*(torch.empty(n, dtype=_I32, device=device)
+                        for n in (num_reqs, num_reqs + 1, num_tokens, num_tokens, num_reqs)))
+
+
+def step_tables(kept_lens, new_lens, page_table, held_pages, free_pages, free_top, num_tokens=None, page_size=16,
+                out=None):
+    """msgl_step_tables: the tables of a step that keeps kept_lens[r] tokens of each request and adds new_lens[r],
+    its pages taken from and given back to the free stack. page_table [B, width], held_pages [B], free_pages
+    (the stack's whole buffer) and free_top [1] are updated in place; rows up to num_tokens are padding."""
+    dev = _device()
+    B, width = page_table.shape
+    if out is None:
+        out = step_tables_buffers(B, num_tokens, page_table.device)
+    T = out.positions.numel()
+    _on(dev, _I32, kept_lens, new_lens, page_table, held_pages, free_pages, free_top, *out)
+    assert kept_lens.numel() == new_lens.numel() == held_pages.numel() == B and free_top.numel() == 1, "expected lengths [B], free_top [1]"
+    assert (out.seq_lens.numel() == out.last_idx.numel() == B and out.q_indptr.numel() == B + 1
+            and out.slot_mapping.numel() == T and num_tokens in (None, T)), "expected step_tables_buffers(B, num_tokens)"
+    check(lib().msgl_step_tables(kept_lens.data_ptr(), new_lens.data_ptr(), page_table.data_ptr(), width,
+                                 held_pages.data_ptr(), free_pages.data_ptr(), free_pages.numel(), free_top.data_ptr(),
+                                 B, T, page_size, *[t.data_ptr() for t in out], _raw_stream(dev)))
+    return out
+
+
+def token_probs(logits, temperature=None, out=None):
+    """msgl_token_probs: softmax(logits / temperature) of fp32 rows [T, V] (rows may be strided; out may be
+    logits); temperature [T] or None, <= 0: one at the first maximum."""
+    dev = _device()
+    T, V = logits.shape
+    if out is None:
+        out = torch.empty((T, V), dtype=_F32, device=logits.device)
+    if temperature is not None:
+        _on(dev, _F32, temperature)
+        assert temperature.numel() == T, "expected a temperature per row"
+    check(lib().msgl_token_probs(logits.data_ptr(), _row_stride(dev, logits, _F32, T, V), T, V, _p(temperature),
+                                 out.data_ptr(), _row_stride(dev, out, _F32, T, V), _raw_stream(dev)))
+    return out
+
+
+def verify_drafts(target_probs, draft_probs, draft_tokens, draft_indptr, uniforms, last_uniforms, max_drafts, out=None):
+    """msgl_verify_drafts: (accepted [B], tokens [B, max_drafts + 1]) int32 from fp32 target_probs
+    [drafts + B, V], draft_probs [drafts, V] (None: certain drafts), draft_tokens [drafts], draft_indptr [B + 1],
+    uniforms [drafts], last_uniforms [B]. out: the two outputs."""
+    dev = _device()
+    B, n = last_uniforms.numel(), draft_tokens.numel()
+    rows, V = target_probs.shape
+    if out is None:
+        out = (torch.empty(B, dtype=_I32, device=target_probs.device),
+               torch.empty(B, max_drafts + 1, dtype=_I32, device=target_probs.device))
+    accepted, tokens = out
+    _on(dev, _I32, draft_tokens, draft_indptr, accepted, tokens)
+    _on(dev, _F32, uniforms, last_uniforms)
+    assert rows == n + B and draft_indptr.numel() == B + 1 and uniforms.numel() == n, "expected target rows [drafts + B, V], draft_indptr [B + 1], uniforms [drafts]"
+    assert accepted.numel() == B and tokens.shape == (B, max_drafts + 1), "expected out ([B], [B, max_drafts + 1])"
+    q, ldq = (None, 0) if draft_probs is None else (draft_probs.data_ptr(), _row_stride(dev, draft_probs, _F32, n, V))
+    check(lib().msgl_verify_drafts(target_probs.data_ptr(), _row_stride(dev, target_probs, _F32, rows, V), q, ldq,
+                                   draft_tokens.data_ptr(), draft_indptr.data_ptr(), uniforms.data_ptr(),
+                                   last_uniforms.data_ptr(), B, n, max_drafts, V, accepted.data_ptr(),
+                                   tokens.data_ptr(), _raw_stream(dev)))
+    return out
+
+
 def sample(logits, temperature, top_k, top_p, seed=0, step=0, out=None):
     """msgl_sample: one token id per row of fp32 logits [B, V] (per-row parameters, device)."""
     _c(logits, torch.float32), _c(temperature, torch.float32), _c(top_k, torch.int32)
@@ -360,6 +434,88 @@ def paged_attention_pages(q, k_pool, v_pool, page_table, seq_lens, page_ids, hq,
         q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), slots // (hkv * 128), page_table.data_ptr(), width,
         seq_lens.data_ptr(), indptr, B, T, max_q_len, width * page_size if max_seq_len is None else max_seq_len,
         page_ids.data_ptr(), top, hq, hkv, 128, page_size, scale, out.data_ptr(), _raw_stream(dev)))
+    return out
+
+
+# ------------------------------------------------------------------ 8-bit key / value pool
+def kv8_pool(num_pages, num_kv_heads, device="cuda"):
+    """An empty 8-bit page pool: codes [num_pages, Hkv, 4096] and scales [num_pages, Hkv, 2] (uint8)."""
+    return (torch.zeros(num_pages, num_kv_heads, 4096, dtype=_U8, device=device),
+            torch.zeros(num_pages, num_kv_heads, 2, dtype=_U8, device=device))
+
+
+def _kv8_pool(dev, kv8, scales, hkv):
+    _on(dev, _U8, kv8, scales)
+    pages = kv8.numel() // (hkv * 4096)
+    assert kv8.numel() == pages * hkv * 4096 and scales.numel() == pages * hkv * 2, "expected kv8 [num_pages, Hkv, 4096], scales [num_pages, Hkv, 2]"
+    return pages
+
+
+def _store_kv8(entry, head, x, x_dtype, kv8, scales, positions, page_table, seq_lens, cos_sin, q_norm, k_norm, hq, hkv,
+               eps, q_indptr, max_q_len, D, page_size, out):
+    dev = _device()
+    T = positions.numel()
+    B, width, indptr = _rows(dev, page_table, seq_lens, q_indptr, max_q_len, T)
+    if out is None:
+        shape = (T, hq, D)
+        out = (torch.empty if q_indptr is None else torch.zeros)(shape, dtype=_BF, device=x.device)
+    _on(dev, x_dtype, x)
+    _on(dev, _BF, q_norm, k_norm, out)
+    _on(dev, _I32, positions)
+    _on(dev, _F32, cos_sin)
+    pages = _kv8_pool(dev, kv8, scales, hkv)
+    max_position, two = cos_sin.shape
+    assert x.numel() == (head[1] if head[1:] else 1) * T * (hq + 2 * hkv) * D, "expected rows of (Hq + 2 Hkv) D"
+    assert out.numel() == T * hq * D, "expected out [T, Hq, D]"
+    assert two == q_norm.numel() == k_norm.numel() == D, "expected cos_sin [max_position, D], norm weights [D]"
+    check(entry(*head, out.data_ptr(), kv8.data_ptr(), scales.data_ptr(), pages, positions.data_ptr(),
+                page_table.data_ptr(), width, seq_lens.data_ptr(), indptr, B, max_q_len, cos_sin.data_ptr(),
+                max_position, q_norm.data_ptr(), k_norm.data_ptr(), T, hq, hkv, D, page_size, eps, _raw_stream(dev)))
+    return out
+
+
+def qknorm_rope_store_kv8(qkv, kv8, scales, positions, page_table, seq_lens, cos_sin, q_norm, k_norm, num_q_heads,
+                          num_kv_heads, eps, q_indptr=None, max_q_len=1, head_dim=128, page_size=16, out=None):
+    """msgl_qknorm_rope_store_kv8: as qknorm_rope_store_kv, with keys and values quantised into the pages of
+    each request's context (page_table, seq_lens, q_indptr as in the attention over the pool)."""
+    return _store_kv8(lib().msgl_qknorm_rope_store_kv8, (qkv.data_ptr(),), qkv, _BF, kv8, scales, positions,
+                      page_table, seq_lens, cos_sin, q_norm, k_norm, num_q_heads, num_kv_heads, eps, q_indptr,
+                      max_q_len, head_dim, page_size, out)
+
+
+def qknorm_rope_store_kv8_partials(parts, kv8, scales, positions, page_table, seq_lens, cos_sin, q_norm, k_norm,
+                                   num_q_heads, num_kv_heads, eps, q_indptr=None, max_q_len=1, head_dim=128,
+                                   page_size=16, out=None):
+    """As qknorm_rope_store_kv8 with the QKV rows the sum of fp32 partials [P, T, (Hq+2Hkv) D]."""
+    return _store_kv8(lib().msgl_qknorm_rope_store_kv8_partials, (parts.data_ptr(), parts.shape[0]), parts, _F32, kv8,
+                      scales, positions, page_table, seq_lens, cos_sin, q_norm, k_norm, num_q_heads, num_kv_heads,
+                      eps, q_indptr, max_q_len, head_dim, page_size, out)
+
+
+def attention_kv8_workspace(num_reqs, max_q_len, hq, hkv, device="cuda"):
+    n = lib().msgl_paged_attention_kv8_workspace_size(num_reqs, max_q_len, hq, hkv)
+    return torch.zeros(max(n, 256), dtype=_U8, device=device)
+
+
+def paged_attention_kv8(q, kv8, scales, page_table, seq_lens, max_seq_len, hq, hkv, scale=_SCALE, q_indptr=None,
+                        max_q_len=1, page_size=16, workspace=None, out=None):
+    """msgl_paged_attention_kv8: attention of q [total_q, Hq, D] over the 8-bit pool, each row up to its position."""
+    dev = _device()
+    n = q.numel()
+    T = n // (hq * 128)
+    B, width, indptr = _rows(dev, page_table, seq_lens, q_indptr, max_q_len, T)
+    if workspace is None:
+        workspace = attention_kv8_workspace(B, max_q_len, hq, hkv, q.device)
+    if out is None:
+        out = torch.empty_like(q) if q_indptr is None else torch.zeros_like(q)
+    _on(dev, _BF, q, out)
+    _on(dev, _U8, workspace)
+    pages = _kv8_pool(dev, kv8, scales, hkv)
+    assert T * hq * 128 == n == out.numel(), "expected q / out [total_q, Hq, D]"
+    check(lib().msgl_paged_attention_kv8(
+        q.data_ptr(), kv8.data_ptr(), scales.data_ptr(), pages, page_table.data_ptr(), width, seq_lens.data_ptr(),
+        indptr, B, T, max_q_len, max_seq_len, hq, hkv, 128, page_size, scale, out.data_ptr(), workspace.data_ptr(),
+        workspace.numel(), _raw_stream(dev)))
     return out
 
 
