@@ -7,7 +7,6 @@
 #include <algorithm>
 
 #include "kv8.cuh"
-#include "kv8_args.h"
 
 namespace msgl {
 namespace {
@@ -1049,6 +1048,7 @@ int msgl_paged_attention_kv8(const void* q, const void* kv8, const void* scales,
     a.ws_ml = reinterpret_cast<float*>(ws + p.off_ml);
     a.row_blocks = p.row_blocks;
     a.min_pages = 8;
+    if (a.max_q_len * (num_q_heads / num_kv_heads) > 64) return launch_attend_chunk(a, stream);
     if (p.nt == 1) return launch_rows<1, 1>(a, p.grid, stream);
     if (p.tiles == 1) return launch_rows<2, 1>(a, p.grid, stream);
     if (p.tiles == 2) return launch_rows<2, 2>(a, p.grid, stream);

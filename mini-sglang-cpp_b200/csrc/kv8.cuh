@@ -13,8 +13,11 @@
 #include <cuda_fp8.h>
 
 #include "common.cuh"
+#include "kv8_args.h"
 
 namespace msgl {
+// Attention of chunks (kv8_chunk.cu): more than 64 rows x heads of a group.
+int launch_attend_chunk(const Kv8AttnArgs& a, msgl_stream_t stream);
 
 constexpr int kKv8Page = 16;
 constexpr int kKv8Head = 128;
