@@ -313,32 +313,29 @@ int launch_store(StoreArgs a, int head_dim, int page_size, msgl_stream_t stream)
 }
 
 // ------------------------------------------------------------------ attention of few rows
-// The rows of a kv head (query row x head of its group, R <= 16 TILES of them) against its pages. MMAs
+// The rows of a kv head (query row x head of its group, at most 8 NT of them) against its pages. MMAs
 // m16n8k16 in f16: S = Q K^T with the rows as M and the 16 keys of a page as two N tiles, then
 // O^T += V^T P^T with 16 dimensions as M, 8 rows as N and the page's keys as K, where S's accumulators are
 // P^T's fragments as they stand. Codes are exact in f16; q is scaled by a power of two per row, which keeps
 // it to 2^-25 of the row's largest value; a page's scales enter the exponent,
 //   s = (q . k) 2^(q + k exponents) scale log2(e) + (exponent of v),  p = 2^(s - m) <= 2^8 in f16,
 // so that O needs no scaling by page, and l adds p 2^-(exponent of v). HBM bound: 4 KB a page and head,
-// 24 to 32 MMAs, 64 conversions.
+// 24 or 32 MMAs, 64 conversions.
 //
-// The pages of all (request, row block, kv head) items in a row are dealt to the CTAs in equal parts
-// (ragged contexts cost no tail); where an item is shared, its CTAs leave partial sums in the workspace
-// and the last of them to arrive joins them in order. In a CTA the pages of an item go around 8 / TILES
-// streams of warps, each with a ring of 4 KB stages that one lane fills by bulk copies across items.
+// In a CTA the pages of an item go around the warps, each with a ring of 4 KB stages that one lane fills by
+// bulk copies across items. Where an item is shared by CTAs they leave partial sums in the workspace and
+// the last of them to arrive joins them in order.
 constexpr int kWarps = 8;
 constexpr int kAttThreads = kWarps * 32;
 constexpr int kPitch = kHd + 4;  // floats of a row in the joining buffer
 
-template <int NT, int TILES>
+template <int NT>
 struct RowsShape {
-    static constexpr int kStreams = kWarps / TILES;
-    static constexpr int kCtas = NT == 1 ? 2 : 1;                 // per SM
-    static constexpr int kStages = NT == 1 ? 18 : 36;             // of a CTA
-    static constexpr int kRing = kStages / kStreams;              // of a stream
-    static constexpr int kRows = NT * 8 * TILES;
-    static constexpr size_t kJoin = static_cast<size_t>(kWarps) * NT * 8 * (kPitch + 2) * 4;
-    static constexpr size_t kSmem = static_cast<size_t>(kRing) * kStreams * kKv8Bytes + kJoin;
+    static constexpr int kCtas = NT == 1 ? 2 : 1;  // per SM
+    static constexpr int kRing = NT == 1 ? 2 : 4;  // stages of a warp
+    static constexpr int kRows = NT * 8;
+    static constexpr size_t kJoin = static_cast<size_t>(kWarps) * kRows * (kPitch + 2) * 4;
+    static constexpr size_t kSmem = static_cast<size_t>(kRing) * kWarps * kKv8Bytes + kJoin;
 };
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -355,46 +352,6 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-__device__ __forceinline__ int64_t larger(int64_t a, int64_t b) { return a > b ? a : b; }
-__device__ __forceinline__ int64_t smaller(int64_t a, int64_t b) { return a < b ? a : b; }
-
-// One item's rows as a CTA sees them.
-struct Item {
-    int r, rb, h;       // request, row block, kv head
-    int L, n, q0;       // context, rows of the request, first of them
-    int row0;           // first query row of the block (of the request)
-    int rows;           // live MMA rows: query rows x group
-    int pages;          // 0 .. last visible page
-};
-
-// Context and rows of request r; n = 0 where it is skipped.
-__device__ __forceinline__ void request_rows(const Kv8AttnArgs& a, int r, bool report, int& L, int& n, int& q0) {
-    L = a.seq_lens[r];
-    q0 = a.q_indptr ? a.q_indptr[r] : r;
-    n = a.q_indptr ? a.q_indptr[r + 1] - q0 : 1;
-    if (n < 0 || n > a.max_q_len || q0 < 0 || (n > 0 && q0 > a.total_q - n)) {
-        if (report) record_error(a.err, MSGL_ERR_BOUNDS, 901);
-        n = 0;
-    }
-    if (n > 0 && (L < 0 || L > a.max_len)) {
-        if (report) record_error(a.err, MSGL_ERR_BOUNDS, 900);
-        L = L < 0 ? 0 : a.max_len;
-    }
-}
-
-// Pages that the rows [row0, row0 + count) of a request see.
-__device__ __forceinline__ int visible_pages(int L, int n, int row0, int count) {
-    const int last = L - n + min(n, row0 + count) - 1;
-    return row0 < n && last >= 0 ? last / kPage + 1 : 0;
-}
-
-// Pages of one head of all row blocks of a request.
-__device__ __forceinline__ int64_t request_pages(int L, int n, int per_block) {
-    int64_t s = 0;
-    for (int row0 = 0; row0 < n; row0 += per_block) s += visible_pages(L, n, row0, per_block);
-    return s;
-}
-
 template <int NT>
 struct RowState {
     uint32_t q[8][NT == 1 ? 2 : 4];  // Q fragments: k step, a0 a2 (a1 a3)
@@ -403,9 +360,6 @@ struct RowState {
     float m[NT], l[NT];
     float o[8][NT][4];
 };
-
-// Bytes of a word of codes that are NaN, as 0x80 each.
-__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
 // NaN values at keys that only some rows see: those rows' sums become NaN. nan[v]: bytes of the lane's value
 // words (4 dimensions x 4 tokens) that hold NaN, 0x80 each.
@@ -544,14 +498,14 @@ __device__ __forceinline__ void attend_page8(const uint8_t* page, uint32_t scale
         if (__any_sync(0xffffffffu, any != 0)) spread_nan<NT>(st, reinterpret_cast<uint32_t(&)[16]>(nan), key0, lane);
 }
 
-// Q rows of a tile into fragments. Row m of the block: query row m / group, head m % group.
+// Q rows of an item into fragments. Row m: query row m / group, head m % group.
 template <int NT>
-__device__ __forceinline__ void load_rows(const Kv8AttnArgs& a, const Item& it, int tile, RowState<NT>& st, int lane) {
+__device__ __forceinline__ void load_rows(const Kv8AttnArgs& a, const Kv8Item& it, RowState<NT>& st, int lane) {
     const int g = lane >> 2, c = lane & 3, group = a.hq / a.hkv;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const int m = tile * NT * 8 + t * 8 + g;
-        const bool live = m < it.rows;
+        const int m = t * 8 + g;
+        const bool live = m < it.rows * group;
         const int i = it.row0 + (live ? m / group : 0);
         st.lim[t] = live ? it.L - it.n + i : -1;
         const __nv_bfloat16* src = a.q + (static_cast<int64_t>(it.q0 + i) * a.hq + it.h * group + (live ? m % group : 0)) * kHd;
@@ -598,144 +552,48 @@ __device__ __forceinline__ void load_rows(const Kv8AttnArgs& a, const Item& it, 
             for (int e = 0; e < 4; ++e) st.o[v][t][e] = 0.f;
 }
 
-template <int NT, int TILES>
-__global__ void __launch_bounds__(kAttThreads, RowsShape<NT, TILES>::kCtas)
+template <int NT>
+__global__ void __launch_bounds__(kAttThreads, RowsShape<NT>::kCtas)
 attend_rows_kernel(const Kv8AttnArgs a) {
-    using S = RowsShape<NT, TILES>;
+    using S = RowsShape<NT>;
     extern __shared__ __align__(128) uint8_t smem[];
-    float* join = reinterpret_cast<float*>(smem + S::kRing * S::kStreams * kKv8Bytes);
-    float* join_ml = join + kWarps * NT * 8 * kPitch;  // [warp][row]{m, l}
-    __shared__ uint64_t full[S::kStages], empty[S::kStages];
-    __shared__ uint32_t stage_scale[S::kStages];
-    __shared__ int64_t warp_sums[kWarps];
-    __shared__ int64_t s_total, s_before;
-    __shared__ int s_first, s_flag;
+    float* join = reinterpret_cast<float*>(smem + S::kRing * kWarps * kKv8Bytes);  // [warp][row][kPitch]
+    float* join_ml = join + kWarps * S::kRows * kPitch;                            // [warp][row]{m, l}
+    __shared__ uint64_t full[S::kRing * kWarps];
+    __shared__ Kv8Scan<kAttThreads> scan;
+    __shared__ int s_flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int stream = warp % S::kStreams, tile = warp / S::kStreams;
     const int group = a.hq / a.hkv;
     if (tid == 0) {
-        for (int i = 0; i < S::kStages; ++i) {
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], TILES);
-        }
+        for (int i = 0; i < S::kRing * kWarps; ++i) mbar_init(&full[i], 1);
         fence_barrier_init();
-        s_first = -1;
     }
     pdl_wait();
     pdl_trigger();
-    // total pages of all items
     const int per_block = S::kRows / group;  // query rows of a block
-    int64_t mine = 0;
-    for (int r = tid; r < a.num_reqs; r += kAttThreads) {
-        int L, n, q0;
-        request_rows(a, r, blockIdx.x == 0, L, n, q0);
-        mine += request_pages(L, n, per_block) * a.hkv;
-        // rows before the context's first token, and rows of an empty context: zeros
-        if (r % gridDim.x == blockIdx.x && n > L)
-            for (int64_t i = static_cast<int64_t>(q0) * a.hq * kHd; i < static_cast<int64_t>(q0 + min(n, n - L)) * a.hq * kHd; i += 8)
-                *reinterpret_cast<uint4*>(a.out + i) = make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if (lane == 0) warp_sums[warp] = mine;
-    __syncthreads();
-    if (tid == 0) {
-        int64_t t = 0;
-        for (int w = 0; w < kWarps; ++w) t += warp_sums[w];
-        s_total = t;
-    }
-    __syncthreads();
-    const int64_t total = s_total;
-    const int64_t per = larger((total + gridDim.x - 1) / gridDim.x, a.min_pages);
-    const int64_t begin = per * blockIdx.x, end = min(total, begin + per);
-    if (begin >= end) return;
-    // the request of the first page: blocks of requests scanned until their sum passes `begin`
-    int64_t base = 0;
-    for (int r0 = 0; r0 < a.num_reqs; r0 += kAttThreads) {
-        const int r = r0 + tid;
-        int64_t w = 0;
-        if (r < a.num_reqs) {
-            int L, n, q0;
-            request_rows(a, r, false, L, n, q0);
-            w = request_pages(L, n, per_block) * a.hkv;
-        }
-        int64_t x = w;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
-        }
-        __syncthreads();
-        if (lane == 31) warp_sums[warp] = x;
-        __syncthreads();
-        int64_t ahead = base;
-        for (int v = 0; v < kWarps; ++v) {
-            if (v < warp) ahead += warp_sums[v];
-            base += warp_sums[v];
-        }
-        if (w > 0 && begin >= ahead + x - w && begin < ahead + x) {
-            s_first = r;
-            s_before = ahead + x - w;
-        }
-        __syncthreads();
-        if (s_first >= 0) break;
-    }
+    int64_t per, begin, end;
+    Kv8Walk<kPage> use;
+    if (!kv8_part<kAttThreads, kPage>(a, per_block, scan, per, begin, end, use)) return;
 
-    // A walk over the items from the one that holds `begin`: position of the item's first page in the row
-    // of all pages, and the item. Used twice a warp: by the filling of the ring and by its use.
-    struct Walk {
-        Item it;
-        int64_t first;
-    };
-    auto set_block = [&](Walk& w) {
-        w.it.row0 = w.it.rb * per_block;
-        w.it.rows = min(per_block, w.it.n - w.it.row0) * group;
-        w.it.pages = visible_pages(w.it.L, w.it.n, w.it.row0, per_block);
-    };
-    auto next = [&](Walk& w) {  // to the next item with any page (order: request, row block, head)
-        w.first += w.it.pages;
-        if (++w.it.h < a.hkv) return;
-        w.it.h = 0;
-        do {
-            if ((w.it.rb + 1) * per_block < w.it.n) {
-                ++w.it.rb;
-            } else {
-                w.it.rb = 0;
-                do {
-                    if (++w.it.r >= a.num_reqs) return;
-                    request_rows(a, w.it.r, false, w.it.L, w.it.n, w.it.q0);
-                } while (w.it.n <= 0);
-            }
-            set_block(w);
-        } while (w.it.pages == 0);
-    };
-    Walk use;
-    use.it.r = s_first;
-    use.it.rb = use.it.h = 0;
-    use.first = s_before;
-    request_rows(a, use.it.r, false, use.it.L, use.it.n, use.it.q0);
-    set_block(use);
-    while (use.it.pages == 0 || use.first + use.it.pages <= begin) next(use);
-
-    // ---------------- filling: the stream's first warp, a lane per page id read ahead
-    Walk fill = use;
-    int fill_page = 0, fill_end = 0;      // next page of this stream and end of the CTA's pages in the item
-    int ids = 0, ids_at = 32;             // lane j: physical page (or -1) and scales of the j-th page from here
-    uint32_t sc = 0;
+    // ---------------- filling: a lane per page id read ahead
+    Kv8Walk<kPage> fill = use;
+    int fill_page = 0, fill_end = 0;  // this warp's next page and the end of the CTA's pages in the item
+    int ids = 0, ids_at = 32;         // lane j: physical page of the j-th page from here, and its scales
+    uint32_t sc = 0, scales[S::kRing];
     int filled = 0;
     auto fill_item = [&]() {
-        fill_page = static_cast<int>(larger(0, begin - fill.first)) + stream;
-        fill_end = static_cast<int>(smaller(fill.it.pages, end - fill.first));
+        fill_page = static_cast<int>(larger(0, begin - fill.first)) + warp;
+        fill_end = static_cast<int>(smaller(fill.it.units, end - fill.first));
         ids_at = 32;
     };
-    auto fill_one = [&]() {  // issues the stream's next page, if there is one
+    auto fill_one = [&](int stage) {  // issues the warp's next page, if there is one; returns its scales
         while (fill_page >= fill_end) {
-            if (fill.first + fill.it.pages >= end) return;
-            next(fill);
+            if (fill.first + fill.it.units >= end) return 0u;
+            fill.next(a, per_block);
             fill_item();
         }
         if (ids_at == 32) {
-            const int p = fill_page + lane * S::kStreams;
+            const int p = fill_page + lane * kWarps;
             ids = 0;
             sc = 0;
             if (p < fill_end) {
@@ -750,46 +608,46 @@ attend_rows_kernel(const Kv8AttnArgs a) {
         }
         const int id = __shfl_sync(0xffffffffu, ids, ids_at);
         const uint32_t scale2 = __shfl_sync(0xffffffffu, sc, ids_at);
-        const int st = stream * S::kRing + filled % S::kRing;
-        if (TILES > 1 && filled >= S::kRing) mbar_wait(&empty[st], (filled / S::kRing - 1) & 1, a.err, 903);
+        const int st = warp * S::kRing + stage;
         if (lane == 0) {
-            stage_scale[st] = scale2;
             mbar_arrive_expect_tx(&full[st], kKv8Bytes);
             bulk_load(smem + st * kKv8Bytes, a.kv8 + (static_cast<int64_t>(id) * a.hkv + fill.it.h) * kKv8Bytes, kKv8Bytes, &full[st]);
         }
-        __syncwarp();
         ++ids_at;
         ++filled;
-        fill_page += S::kStreams;
+        fill_page += kWarps;
+        return scale2;
     };
-    if (tile == 0) {
-        fill_item();
-        for (int i = 0; i < S::kRing; ++i) fill_one();
-    }
+    fill_item();
+#pragma unroll
+    for (int i = 0; i < S::kRing; ++i) scales[i] = fill_one(i);
 
     RowState<NT> st;
     int used = 0;
     bool ok = true;
     while (true) {
-        load_rows<NT>(a, use.it, tile, st, lane);
-        int min_lim = use.it.L - use.it.n + use.it.row0;  // the block's first query row
-        const int p0 = static_cast<int>(larger(0, begin - use.first));
-        const int p1 = static_cast<int>(smaller(use.it.pages, end - use.first));
-        for (int p = p0 + stream; p < p1; p += S::kStreams) {
-            const int sg = stream * S::kRing + used % S::kRing;
+        load_rows<NT>(a, use.it, st, lane);
+        const int min_lim = use.it.L - use.it.n + use.it.row0;  // last key of the block's first query row
+        const int p1 = static_cast<int>(smaller(use.it.units, end - use.first));
+        for (int p = static_cast<int>(larger(0, begin - use.first)) + warp; p < p1; p += kWarps) {
+            const int stage = used % S::kRing;
+            const int sg = warp * S::kRing + stage;
+            uint32_t scale2 = scales[0];
+#pragma unroll
+            for (int i = 1; i < S::kRing; ++i) scale2 = stage == i ? scales[i] : scale2;
             ok = ok && mbar_wait(&full[sg], (used / S::kRing) & 1, a.err, 904);
             const uint8_t* page = smem + sg * kKv8Bytes;
-            const uint32_t scale2 = stage_scale[sg];
             if (__all_sync(0xffffffffu, ok)) {
                 if (p * kPage + kPage - 1 > min_lim) attend_page8<NT, true>(page, scale2, st, p * kPage, min_lim, lane);
                 else attend_page8<NT, false>(page, scale2, st, p * kPage, min_lim, lane);
             }
             __syncwarp();
-            if (TILES > 1 && lane == 0) mbar_arrive(&empty[sg]);
             ++used;
-            if (tile == 0) fill_one();
+            scale2 = fill_one(stage);
+#pragma unroll
+            for (int i = 0; i < S::kRing; ++i) scales[i] = stage == i ? scale2 : scales[i];
         }
-        // ---------------- join the streams: unnormalised sums and (m, l) of each warp through shared memory
+        // ---------------- join the warps: unnormalised sums and (m, l) of each through shared memory
         const int g = lane >> 2, c = lane & 3;
         __syncthreads();
 #pragma unroll
@@ -798,40 +656,36 @@ attend_rows_kernel(const Kv8AttnArgs a) {
             l += __shfl_xor_sync(0xffffffffu, l, 1);
             l += __shfl_xor_sync(0xffffffffu, l, 2);
             if (c == 0) {
-                join_ml[(warp * NT * 8 + t * 8 + g) * 2] = st.m[t];
-                join_ml[(warp * NT * 8 + t * 8 + g) * 2 + 1] = l;
+                join_ml[(warp * S::kRows + t * 8 + g) * 2] = st.m[t];
+                join_ml[(warp * S::kRows + t * 8 + g) * 2 + 1] = l;
             }
 #pragma unroll
             for (int v = 0; v < 8; ++v)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    join[(warp * NT * 8 + t * 8 + 2 * c + (e & 1)) * kPitch + 4 * (g + 8 * (v >> 1)) + 2 * (v & 1) + (e >> 1)] = st.o[v][t][e];
+                    join[(warp * S::kRows + t * 8 + 2 * c + (e & 1)) * kPitch + 4 * (g + 8 * (v >> 1)) + 2 * (v & 1) + (e >> 1)] = st.o[v][t][e];
         }
         __syncthreads();
-        const int a0 = static_cast<int>(use.first / per), a1 = static_cast<int>((use.first + use.it.pages - 1) / per);
-        const bool whole = a0 == a1;
+        const int64_t a0 = use.first / per, a1 = (use.first + use.it.units - 1) / per;
         // a CTA takes part in at most one item that it did not begin and one that it does not end
-        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (static_cast<int>(blockIdx.x) != a0 ? 0 : 1);
-        for (int i = tid; i < use.it.rows * (kHd / 4); i += kAttThreads) {
+        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (blockIdx.x == a0);
+        for (int i = tid; i < use.it.rows * group * (kHd / 4); i += kAttThreads) {
             const int m = i / (kHd / 4), d = i % (kHd / 4) * 4;
-            const int t0 = m / (NT * 8), mr = m % (NT * 8);
             float M = kNegInf;
-            for (int s = 0; s < S::kStreams; ++s) M = fmaxf(M, join_ml[((t0 * S::kStreams + s) * NT * 8 + mr) * 2]);
+            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, join_ml[(w * S::kRows + m) * 2]);
             float l = 0.f;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int s = 0; s < S::kStreams; ++s) {
-                const int w = (t0 * S::kStreams + s) * NT * 8 + mr;
-                const float ms = join_ml[2 * w];
-                // a stream without a visible key has l = 0 (or NaN where a NaN was seen)
-                const float f = ms == kNegInf ? 1.f : exp2f(ms - M);
-                const float4 x = *reinterpret_cast<const float4*>(join + w * kPitch + d);
-                l += join_ml[2 * w + 1] * f;
+            for (int w = 0; w < kWarps; ++w) {
+                const float ms = join_ml[(w * S::kRows + m) * 2];
+                const float f = ms == kNegInf ? 1.f : exp2_ftz(ms - M);  // as in kv8_join
+                const float4 x = *reinterpret_cast<const float4*>(join + (w * S::kRows + m) * kPitch + d);
+                l += join_ml[(w * S::kRows + m) * 2 + 1] * f;
                 o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
             }
-            if (whole) {
+            if (a0 == a1) {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
-                uint2 u = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-                *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(use.it.q0 + use.it.row0 + m / group) * a.hq + use.it.h * group + m % group) * kHd + d) = u;
+                *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(use.it.q0 + use.it.row0 + m / group) * a.hq + use.it.h * group + m % group) * kHd + d) =
+                    make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
             } else {
                 *reinterpret_cast<float4*>(a.ws_o + (slot * S::kRows + m) * kHd + d) = o;
                 if (d == 0) {
@@ -840,44 +694,28 @@ attend_rows_kernel(const Kv8AttnArgs a) {
                 }
             }
         }
-        if (!whole) {
+        if (a0 != a1) {
             __threadfence();
             __syncthreads();
             int* count = a.ws_count + (static_cast<int64_t>(use.it.r) * a.row_blocks + use.it.rb) * a.hkv + use.it.h;
-            if (tid == 0) s_flag = atomicAdd(count, 1) == a1 - a0;
+            if (tid == 0) s_flag = atomicAdd(count, 1) == static_cast<int>(a1 - a0);
             __syncthreads();
             if (s_flag) {
                 __threadfence();
-                for (int i = tid; i < use.it.rows * (kHd / 4); i += kAttThreads) {
-                    const int m = i / (kHd / 4), d = i % (kHd / 4) * 4;
-                    float M = kNegInf, l = 0.f;
-                    for (int b = a0; b <= a1; ++b) M = fmaxf(M, __ldcg(a.ws_ml + ((2 * static_cast<int64_t>(b) + (b == a0)) * S::kRows + m) * 2));
-                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                    for (int b = a0; b <= a1; ++b) {
-                        const int64_t w = (2 * static_cast<int64_t>(b) + (b == a0)) * S::kRows + m;
-                        const float ms = __ldcg(a.ws_ml + 2 * w);
-                        const float f = ms == kNegInf ? 1.f : exp2f(ms - M);
-                        const float4 x = __ldcg(reinterpret_cast<const float4*>(a.ws_o + w * kHd + d));
-                        l += __ldcg(a.ws_ml + 2 * w + 1) * f;
-                        o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
-                    }
-                    const float inv = l == 0.f ? 0.f : 1.f / l;
-                    uint2 u = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-                    *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(use.it.q0 + use.it.row0 + m / group) * a.hq + use.it.h * group + m % group) * kHd + d) = u;
-                }
+                kv8_join<S::kRows>(a, use.it, group, a0, a1, tid, kAttThreads);
                 if (tid == 0) *count = 0;
             }
         }
-        if (use.first + use.it.pages >= end) break;
-        next(use);
+        if (use.first + use.it.units >= end) break;
+        use.next(a, per_block);
     }
 }
 
 // ------------------------------------------------------------------ host side
 // Counters of every (request, row block, kv head), then the partial sums of two items a CTA.
 struct RowsPlan {
-    int nt, tiles, rows, row_blocks, grid;
+    int rows;  // of a block: MMA rows
+    int row_blocks, grid;
     size_t off_o, off_ml, bytes;
 };
 
@@ -885,11 +723,9 @@ RowsPlan plan_rows(int num_reqs, int max_q_len, int hq, int hkv) {
     RowsPlan p{};
     const int group = hq / hkv;
     const int64_t rows = static_cast<int64_t>(max_q_len) * group;
-    p.nt = rows <= 8 ? 1 : 2;
-    p.tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    p.rows = 8 * p.nt * p.tiles;
-    p.row_blocks = std::max(1, (max_q_len + p.rows / group - 1) / (p.rows / group));
-    p.grid = 148 * (p.nt == 1 ? 2 : 1);
+    p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 128 ? 128 : 256;
+    p.row_blocks = (max_q_len + p.rows / group - 1) / (p.rows / group);
+    p.grid = 148 * (p.rows == 8 ? 2 : 1);
     const size_t count = (static_cast<size_t>(num_reqs) * p.row_blocks * hkv * 4 + 255) / 256 * 256;
     p.off_o = count;
     p.off_ml = count + static_cast<size_t>(p.grid) * 2 * p.rows * kHd * 4;
@@ -897,13 +733,13 @@ RowsPlan plan_rows(int num_reqs, int max_q_len, int hq, int hkv) {
     return p;
 }
 
-template <int NT, int TILES>
+template <int NT>
 int launch_rows(const Kv8AttnArgs& a, int grid, msgl_stream_t stream) {
-    using S = RowsShape<NT, TILES>;
+    using S = RowsShape<NT>;
     static std::atomic<int> optin[kMaxDevices];
-    const cudaError_t e = smem_optin(attend_rows_kernel<NT, TILES>, S::kSmem, optin);
+    const cudaError_t e = smem_optin(attend_rows_kernel<NT>, S::kSmem, optin);
     if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
-    launch_pdl(attend_rows_kernel<NT, TILES>, dim3(grid), dim3(kAttThreads), S::kSmem, stream, a);
+    launch_pdl(attend_rows_kernel<NT>, dim3(grid), dim3(kAttThreads), S::kSmem, stream, a);
     MSGL_LAUNCH_CHECK();
     return MSGL_OK;
 }
@@ -999,7 +835,7 @@ size_t msgl_paged_attention_kv8_workspace_size(int num_reqs, int max_q_len, int 
     // the largest of the forms that this call or a smaller one may take
     const int group = num_q_heads / num_kv_heads;
     size_t most = plan_rows(num_reqs, max_q_len, num_q_heads, num_kv_heads).bytes;
-    for (int rows = 8; rows <= 32; rows *= 2)
+    for (int rows : {8, 16, 128})
         most = std::max(most, plan_rows(num_reqs, std::min(max_q_len, rows / group), num_q_heads, num_kv_heads).bytes);
     return most;
 }
@@ -1047,12 +883,12 @@ int msgl_paged_attention_kv8(const void* q, const void* kv8, const void* scales,
     a.ws_o = reinterpret_cast<float*>(ws + p.off_o);
     a.ws_ml = reinterpret_cast<float*>(ws + p.off_ml);
     a.row_blocks = p.row_blocks;
-    a.min_pages = 8;
-    if (a.max_q_len * (num_q_heads / num_kv_heads) > 64) return launch_attend_chunk(a, stream);
-    if (p.nt == 1) return launch_rows<1, 1>(a, p.grid, stream);
-    if (p.tiles == 1) return launch_rows<2, 1>(a, p.grid, stream);
-    if (p.tiles == 2) return launch_rows<2, 2>(a, p.grid, stream);
-    return launch_rows<2, 4>(a, p.grid, stream);
+    if (p.rows <= 16) {
+        a.min_units = 8;  // a page for each warp
+        return p.rows == 8 ? launch_rows<1>(a, p.grid, stream) : launch_rows<2>(a, p.grid, stream);
+    }
+    a.min_units = 4;
+    return launch_attend_tiles(a, p.rows == 128, p.grid, stream);
 }
 
 }  // extern "C"

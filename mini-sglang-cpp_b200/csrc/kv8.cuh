@@ -16,8 +16,8 @@
 #include "kv8_args.h"
 
 namespace msgl {
-// Attention of chunks (kv8_chunk.cu): more than 64 rows x heads of a group.
-int launch_attend_chunk(const Kv8AttnArgs& a, msgl_stream_t stream);
+// Attention of more than 16 rows x heads of a group (kv8_tiles.cu).
+int launch_attend_tiles(const Kv8AttnArgs& a, bool few, int grid, msgl_stream_t stream);
 
 constexpr int kKv8Page = 16;
 constexpr int kKv8Head = 128;
@@ -51,6 +51,179 @@ __device__ __forceinline__ void e4m3x4_to_half(uint32_t w, uint32_t& lo, uint32_
 // Codes of x0 (low byte) and x1, rounded to nearest even; |x| <= 448 or NaN.
 __device__ __forceinline__ uint32_t e4m3_codes2(float x0, float x1) {
     return __nv_cvt_float2_to_fp8x2(make_float2(x0, x1), __NV_SATFINITE, __NV_E4M3);
+}
+
+__device__ __forceinline__ float exp2_ftz(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Bytes of a word of codes that are NaN, as 0x80 each.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+__device__ __forceinline__ int64_t larger(int64_t a, int64_t b) { return a > b ? a : b; }
+__device__ __forceinline__ int64_t smaller(int64_t a, int64_t b) { return a < b ? a : b; }
+
+// ------------------------------------------------------------------ attention: the row of all work
+// An item is a block of query rows of a request on a kv head; its units are the UNIT-key pieces that any of
+// the rows sees. All items' units in a row (request, row block, head) are dealt to the CTAs in equal
+// parts, so that ragged contexts and causal chunks leave no tail.
+struct Kv8Item {
+    int r, rb, h;
+    int L, n, q0;    // context, rows of the request, first of them
+    int row0, rows;  // query rows of the block, within the request
+    int units;
+};
+
+// Context and rows of request r; n = 0 where it is skipped.
+__device__ __forceinline__ void kv8_request(const Kv8AttnArgs& a, int r, bool report, int& L, int& n, int& q0) {
+    L = a.seq_lens[r];
+    q0 = a.q_indptr ? a.q_indptr[r] : r;
+    n = a.q_indptr ? a.q_indptr[r + 1] - q0 : 1;
+    if (n < 0 || n > a.max_q_len || q0 < 0 || (n > 0 && q0 > a.total_q - n)) {
+        if (report) record_error(a.err, MSGL_ERR_BOUNDS, 901);
+        n = 0;
+    }
+    if (n > 0 && (L < 0 || L > a.max_len)) {
+        if (report) record_error(a.err, MSGL_ERR_BOUNDS, 900);
+        L = L < 0 ? 0 : a.max_len;
+    }
+}
+
+// Units that the rows [row0, row0 + count) of a request see.
+template <int UNIT>
+__device__ __forceinline__ int kv8_units(int L, int n, int row0, int count) {
+    const int last = L - n + min(n, row0 + count) - 1;
+    return row0 < n && last >= 0 ? last / UNIT + 1 : 0;
+}
+
+template <int UNIT>
+struct Kv8Walk {
+    Kv8Item it;
+    int64_t first;  // place of the item's first unit
+
+    __device__ __forceinline__ void set_block(int per_block) {
+        it.row0 = it.rb * per_block;
+        it.rows = min(per_block, it.n - it.row0);
+        it.units = kv8_units<UNIT>(it.L, it.n, it.row0, per_block);
+    }
+    __device__ __forceinline__ void next(const Kv8AttnArgs& a, int per_block) {  // to the next item with any unit
+        first += it.units;
+        if (++it.h < a.hkv) return;
+        it.h = 0;
+        do {
+            if ((it.rb + 1) * per_block < it.n) {
+                ++it.rb;
+            } else {
+                it.rb = 0;
+                do {
+                    if (++it.r >= a.num_reqs) return;
+                    kv8_request(a, it.r, false, it.L, it.n, it.q0);
+                } while (it.n <= 0);
+            }
+            set_block(per_block);
+        } while (it.units == 0);
+    }
+};
+
+// Scratch of kv8_part.
+template <int THREADS>
+struct Kv8Scan {
+    int64_t warp_sums[THREADS / 32], before;
+    int first;
+};
+
+// Zeros for the first `rows` query rows from q0 on.
+__device__ __forceinline__ void zero_rows(const Kv8AttnArgs& a, int q0, int rows) {
+    const int64_t from = static_cast<int64_t>(q0) * a.hq * kKv8Head, to = from + static_cast<int64_t>(rows) * a.hq * kKv8Head;
+    for (int64_t i = from; i < to; i += 8) *reinterpret_cast<uint4*>(a.out + i) = make_uint4(0, 0, 0, 0);
+}
+
+// This CTA's part [begin, end) of all units and the item that holds its first; false where there is none. Rows
+// before their context's first token get zeros on the way. Every thread of the block calls it.
+template <int THREADS, int UNIT>
+__device__ __forceinline__ bool kv8_part(const Kv8AttnArgs& a, int per_block, Kv8Scan<THREADS>& sh, int64_t& per, int64_t& begin,
+                                         int64_t& end, Kv8Walk<UNIT>& walk) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto weight = [&](int r, bool report) {
+        int L, n, q0;
+        kv8_request(a, r, report, L, n, q0);
+        int64_t s = 0;
+        for (int row0 = 0; row0 < n; row0 += per_block) s += kv8_units<UNIT>(L, n, row0, per_block);
+        if (report && n > L) zero_rows(a, q0, n - L);
+        return s * a.hkv;
+    };
+    int64_t mine = 0;
+    for (int r = tid; r < a.num_reqs; r += THREADS) mine += weight(r, blockIdx.x == 0);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) sh.warp_sums[warp] = mine;
+    if (tid == 0) sh.first = -1;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) total += sh.warp_sums[w];
+    per = larger((total + gridDim.x - 1) / gridDim.x, a.min_units);
+    begin = per * blockIdx.x;
+    end = smaller(total, begin + per);
+    if (begin >= end) return false;
+    int64_t base = 0;
+    for (int r0 = 0; r0 < a.num_reqs; r0 += THREADS) {  // blocks of requests, until their sum passes `begin`
+        const int r = r0 + tid;
+        const int64_t w = r < a.num_reqs ? weight(r, false) : 0;
+        int64_t x = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 31) sh.warp_sums[warp] = x;
+        __syncthreads();
+        int64_t ahead = base;
+        for (int v = 0; v < THREADS / 32; ++v) {
+            if (v < warp) ahead += sh.warp_sums[v];
+            base += sh.warp_sums[v];
+        }
+        if (w > 0 && begin >= ahead + x - w && begin < ahead + x) {
+            sh.first = r;
+            sh.before = ahead + x - w;
+        }
+        __syncthreads();
+        if (sh.first >= 0) break;
+    }
+    walk.it.r = sh.first;
+    walk.it.rb = walk.it.h = 0;
+    walk.first = sh.before;
+    kv8_request(a, walk.it.r, false, walk.it.L, walk.it.n, walk.it.q0);
+    walk.set_block(per_block);
+    while (walk.it.units == 0 || walk.first + walk.it.units <= begin) walk.next(a, per_block);
+    return true;
+}
+
+// Joins the partial sums of an item that the CTAs a0 .. a1 share, in their order: rows (query row x head of the
+// group) x 128 values by `threads` threads. ROWS: rows of a slot.
+template <int ROWS>
+__device__ __forceinline__ void kv8_join(const Kv8AttnArgs& a, const Kv8Item& it, int group, int64_t a0, int64_t a1, int tid, int threads) {
+    for (int i = tid; i < it.rows * group * (kKv8Head / 4); i += threads) {
+        const int m = i / (kKv8Head / 4), d = i % (kKv8Head / 4) * 4;
+        float M = -__builtin_huge_valf(), l = 0.f;
+#pragma unroll 4
+        for (int64_t b = a0; b <= a1; ++b) M = fmaxf(M, __ldcg(a.ws_ml + ((2 * b + (b == a0)) * ROWS + m) * 2));
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int64_t b = a0; b <= a1; ++b) {
+            const int64_t w = (2 * b + (b == a0)) * ROWS + m;
+            const float ms = __ldcg(a.ws_ml + 2 * w);
+            // a part without a visible key has l = 0 (or NaN where a NaN was seen)
+            const float f = ms == -__builtin_huge_valf() ? 1.f : exp2_ftz(ms - M);
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(a.ws_o + w * kKv8Head + d));
+            l += __ldcg(a.ws_ml + 2 * w + 1) * f;
+            o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(it.q0 + it.row0 + m / group) * a.hq + it.h * group + m % group) * kKv8Head + d) =
+            make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+    }
 }
 
 }  // namespace msgl

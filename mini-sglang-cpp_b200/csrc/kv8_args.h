@@ -17,7 +17,7 @@ struct Kv8AttnArgs {
     float *ws_o, *ws_ml;
     int* ws_count;
     int row_blocks;  // of a request, at most
-    int min_pages;   // of a CTA, at least
+    int min_units;   // of a CTA, at least
     int* err;
 };
 }  // namespace msgl

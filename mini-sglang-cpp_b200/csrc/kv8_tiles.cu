@@ -1,0 +1,687 @@
+// kv8_tiles.cu -- attention of many rows (chunks, drafted rows) over the 8-bit key / value pool, on tcgen05.
+//
+// Persistent: each CTA takes an equal part of the steps (64 keys) of all items (block of query rows x kv head;
+// rows = query rows x the group's heads); items shared by CTAs are joined through the workspace by the last
+// CTA to arrive. Codes are converted to f16 (exactly) into the operands' canonical tiles, q is scaled to f16
+// by a power of two per row (2^-25 of its largest value). A page's scales enter the exponent:
+// s = (q . k) 2^(q + k exponents) scale log2(e) + (exponent of v), p = 2^(s - m) <= 2^8 in f16, so that O needs
+// no scaling by page, and l adds p 2^-(exponent of v).
+//
+// Two streams of 128 MMA rows each:
+//   FEW = false  blocks of 256 rows: the streams are its halves, and both take every step;
+//   FEW = true   blocks of up to 128 rows: both streams hold them and take every other step, joined at the
+//                item's end, so that one's softmax runs while the other's MMAs do.
+// Warps:
+//   0-3, 4-7   softmax of stream 0 / 1: a thread per row. S from tensor memory, p as f16 pairs over the first
+//              half of S, l and m in registers; O in tensor memory is rescaled only where the maximum grew by
+//              more than 8;
+//   8-11       conversion of a step's four pages: keys [64][128], values [128][64], both K-major (the keys of a
+//              page in the order in which the pool stores their values);
+//   12, 13     one lane each issues a stream's MMAs: PV(i), then S(i + 2). S has two buffers of 64 columns, so that
+//              the next S is there before the softmax of a step ends; while one stream waits for a hand-over
+//              (100 to 400 clocks each) the other's MMAs run;
+//   14         page ids and scales, a bulk copy of 4 KB a page into a ring of two steps (loads by the
+//              converting warps held them up for half of their time).
+// Tensor memory: two S buffers a stream and O: 2 x (128 + 128) columns.
+//
+// Bound: chunks by the MMAs (4 x 128 FLOP a row and key), then by the softmax's and the conversion's
+// instructions; few rows by HBM (4 KB a page and head).
+#include <algorithm>
+
+#include "kv8.cuh"
+
+namespace msgl {
+namespace {
+
+constexpr int kPage = kKv8Page;
+constexpr int kHd = kKv8Head;
+constexpr int kStep = 64;                      // keys
+constexpr int kPages = kStep / kPage;          // of a step
+constexpr int kRows = 128;                     // of a stream
+constexpr int kQTile = 2 * kRows * 128;        // [2 halves of the dimensions][128 rows][64 f16]
+constexpr int kKTile = 2 * kStep * 128;        // [2 halves of the dimensions][64 keys][64 f16]
+constexpr int kVTile = kHd * 128;              // [128 dimensions][64 keys f16]
+constexpr int kStages = 4;                     // of keys and of values
+constexpr int kRaw = 2;                        // steps of codes
+constexpr int kInfo = 8;                       // steps whose scales are kept (a softmax is behind by fewer)
+constexpr int kThreads = 512;
+constexpr size_t kSmem = 1024 + 2 * kQTile + kStages * (kKTile + kVTile) + kRaw * kPages * kKv8Bytes;
+constexpr float kNegInf = -__builtin_huge_valf();
+
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {  // A, B f16 K-major, D fp32
+    return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+__device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ bool elect_lane() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
+}
+__device__ __forceinline__ void named_barrier(int id, int threads) {
+    __syncwarp();
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// Waits of a whole warp: even lanes for the use-th completion of a, odd ones for that of b.
+__device__ __forceinline__ bool wait_two(uint64_t* a, int use_a, uint64_t* b, int use_b, int* err, int site) {
+    const bool odd = threadIdx.x & 1;
+    return __all_sync(0xffffffffu, mbar_wait(odd ? b : a, (odd ? use_b : use_a) & 1, err, site));
+}
+__device__ __forceinline__ bool wait_one(uint64_t* a, int use, int* err, int site) {
+    return __all_sync(0xffffffffu, mbar_wait(a, use & 1, err, site));
+}
+
+// Token of a page at place i of its order.
+__host__ __device__ constexpr int token_at(int i) { return (i % 4 / 2) * 8 + (i / 4) * 2 + i % 2; }
+
+// Scales of a page: keys' factor, values' exponent and inverse factor.
+struct PageScale {
+    float k, v_exp, v_inv, pad;
+};
+
+struct Shared {
+    uint64_t raw_full[kRaw], raw_empty[kRaw], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], info_full[kInfo];
+    uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2][2];  // stream, parity of its steps
+    PageScale info[kInfo][kPages];
+    int nan_seen[kInfo];  // by item in turn: a value hidden from some of its rows was NaN
+    uint32_t tmem;
+    int last;
+    union {
+        Kv8Scan<kThreads> scan;  // before the walk
+        float2 ml[kRows];        // stream 1's (m, l), FEW
+    };
+};
+
+// Two fp32 values in a register pair.
+__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+    return v;
+}
+__device__ __forceinline__ uint64_t pair(float v) { return pair(__float_as_uint(v), __float_as_uint(v)); }
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// One step of a row: 64 S columns into pairs of p. EDGE: keys behind `lim` do not count. The factor of a page
+// is positive (qs is), so the page's largest logit comes from its largest product.
+template <bool EDGE>
+__device__ __forceinline__ void softmax_step(uint32_t (&s)[64], uint32_t (&out)[32], const PageScale* info, float qs, int key0,
+                                             int lim, float& m, float& l, float& alpha) {
+    float mx = kNegInf;
+#pragma unroll
+    for (int p = 0; p < kPages; ++p) {
+        float pm[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+#pragma unroll
+        for (int i = 0; i < kPage; ++i) {
+            uint32_t& x = s[p * kPage + i];
+            if (EDGE && key0 + p * kPage + token_at(i) > lim) x = 0xff800000u;
+            pm[i & 3] = fmaxf(pm[i & 3], __uint_as_float(x));
+        }
+        mx = fmaxf(mx, fmaf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), qs * info[p].k, info[p].v_exp));
+    }
+    // The maximum moves only where it grows by more than 8: p stays below 2^8, which f16 holds as well.
+    const float next = m == kNegInf || mx > m + 8.f ? fmaxf(m, mx) : m;
+    const float base = next == kNegInf ? 0.f : next;
+    alpha = next == m ? 1.f : exp2_ftz(m - next);
+    float sum = 0.f;
+#pragma unroll
+    for (int p = 0; p < kPages; ++p) {
+        const uint64_t f = pair(qs * info[p].k), v = pair(info[p].v_exp - base);
+        uint64_t part[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < kPage; i += 2) {
+            const int c = p * kPage + i;
+            float x, y;
+            unpair(fma2(pair(s[c], s[c + 1]), f, v), x, y);
+            x = exp2_ftz(x);
+            y = exp2_ftz(y);
+            part[i / 2 & 1] = add2(part[i / 2 & 1], pair(__float_as_uint(x), __float_as_uint(y)));
+            out[c / 2] = half2_of(x, y);
+        }
+        float a, b;
+        unpair(add2(part[0], part[1]), a, b);
+        sum = fmaf(a + b, info[p].v_inv, sum);
+    }
+    l = fmaf(l, alpha, sum);
+    m = next;
+}
+
+// 32 consecutive columns of this thread's lane.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    __syncwarp();
+    uint32_t lo[16], hi[16];
+    tmem_ld16(taddr, lo);
+    tmem_ld16(taddr + 16, hi);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        r[e] = lo[e];
+        r[16 + e] = hi[e];
+    }
+}
+
+// Stages of keys and values. FEW: two for each stream, so that a stream meets every phase of its barriers (one
+// that skipped a phase would take the one before for it); else all for both. n: steps taken before.
+template <bool FEW>
+__device__ __forceinline__ int stage_of(int t, int n) { return FEW ? 2 * t + n % 2 : n % kStages; }
+template <bool FEW>
+__device__ __forceinline__ int use_of(int n) { return FEW ? n / 2 : n / kStages; }
+
+// A CTA's steps of an item: [u0, u1) of its units. Of them, a stream's own ones are first, first + stride, ...
+template <bool FEW>
+struct Share {
+    int u0, u1;
+    __device__ __forceinline__ Share(const Kv8Walk<kStep>& w, int64_t begin, int64_t end)
+        : u0(static_cast<int>(larger(0, begin - w.first))), u1(static_cast<int>(smaller(w.it.units, end - w.first))) {}
+    // number of stream t's steps
+    __device__ __forceinline__ int own(const Kv8Item& it, int per_stream, int t) const {
+        if (FEW) return (u1 - u0 + 1 - t) / 2;
+        return max(0, min(u1, kv8_units<kStep>(it.L, it.n, it.row0 + t * per_stream, min(per_stream, it.rows - t * per_stream))) - u0);
+    }
+    __device__ __forceinline__ int step(int t, int i) const { return FEW ? u0 + t + 2 * i : u0 + i; }
+};
+
+template <bool FEW>
+__global__ void __launch_bounds__(kThreads, 1)
+attend_tiles_kernel(const Kv8AttnArgs a) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ Shared sh;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sQ = smem;                       // a tile per stream; FEW: stream 1's sums between two items
+    uint8_t* sK = sQ + 2 * kQTile;            // [kStages]
+    uint8_t* sV = sK + kStages * kKTile;      // [kStages]
+    uint8_t* sRaw = sV + kStages * kVTile;    // [kRaw][kPages]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int group = a.hq / a.hkv, per_stream = kRows / group, per_block = FEW ? per_stream : 2 * per_stream;
+    if (tid == 0) {
+        for (int i = 0; i < kRaw; ++i) {
+            mbar_init(&sh.raw_full[i], 1);
+            mbar_init(&sh.raw_empty[i], 4);
+        }
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&sh.k_full[i], 4);
+            mbar_init(&sh.k_empty[i], FEW ? 1 : 2);
+            mbar_init(&sh.v_full[i], 4);
+            mbar_init(&sh.v_empty[i], FEW ? 1 : 2);
+        }
+        for (int i = 0; i < kInfo; ++i) {
+            mbar_init(&sh.info_full[i], 1);
+            sh.nan_seen[i] = 0;
+        }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&sh.q_full[t], 4);
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&sh.s_full[t][b], 1);
+                mbar_init(&sh.p_full[t][b], 4);
+                mbar_init(&sh.o_done[t][b], 1);
+            }
+        }
+        fence_barrier_init();
+    }
+    pdl_wait();
+    pdl_trigger();
+    int64_t per, begin, end;
+    Kv8Walk<kStep> walk;
+    if (!kv8_part<kThreads, kStep>(a, per_block, sh.scan, per, begin, end, walk)) return;
+    if (warp == 12) {
+        tmem_alloc(&sh.tmem, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    // Every role walks the CTA's items by itself: `count` steps of the items before this one, the `item`-th item.
+    int count = 0, item = 0;
+    bool ok = true;
+    auto last_item = [&]() { return walk.first + walk.it.units >= end; };
+
+    if (warp < 8) {
+        // ---------------- softmax of stream t: a thread per row
+        const int t = warp >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t tS = tmem + t * 128 + lanes, tO = tmem + 256 + t * 128 + lanes;
+        int done = 0;  // steps of this stream
+        while (true) {
+            const Share<FEW> share(walk, begin, end);
+            const Kv8Item& it = walk.it;
+            const int i_row = it.row0 + (FEW ? 0 : t * per_stream) + row / group;
+            const bool live = i_row < it.row0 + it.rows;
+            const int lim = live ? it.L - it.n + i_row : -1;
+            const int first_lim = it.L - it.n + it.row0;                                   // last key of the block's first row
+            const int stream_first = first_lim + (FEW ? 0 : t * per_stream);               // of the stream's
+            const int64_t at = (static_cast<int64_t>(it.q0 + (live ? i_row : 0)) * a.hq + it.h * group + row % group) * kHd;
+            const int own = share.own(it, per_stream, t);
+            float qs = 0.f, m = kNegInf, l = 0.f;
+            if (own > 0 && ok) {
+                const uint4* src = reinterpret_cast<const uint4*>(a.q + at);
+                float amax = 0.f;
+                bool bad = false;
+                uint4 u[16];
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    u[v] = live ? src[v] : make_uint4(0, 0, 0, 0);
+                    const uint32_t w[4] = {u[v].x, u[v].y, u[v].z, u[v].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        amax = fmaxf(amax, fmaxf(fabsf(bf16lo(w[e])), fabsf(bf16hi(w[e]))));
+                        bad |= finite2(w[e]) != w[e];
+                    }
+                }
+                const int stored = max(1, min(253, static_cast<int>(__float_as_uint(amax) >> 23)));
+                const float inv = a.sl2e < 0.f ? -kv8_inverse(stored) : kv8_inverse(stored);
+                // a row with an infinity or a NaN has no defined logit: NaN throughout
+                qs = bad ? __int_as_float(0x7fffffff) : kv8_power(stored) * fabsf(a.sl2e);
+                uint8_t* dst = sQ + t * kQTile + row * 128;
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const uint32_t w[4] = {u[v].x, u[v].y, u[v].z, u[v].w};
+                    uint32_t f[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) f[e] = bad ? 0u : half2_of(bf16lo(w[e]) * inv, bf16hi(w[e]) * inv);
+                    *reinterpret_cast<uint4*>(dst + (v >> 3) * (kQTile / 2) + (((v & 7) ^ (row & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.q_full[t]);
+            }
+            for (int i = 0; i < own && ok; ++i, ++done) {
+                const int b = done & 1, u = share.step(t, i), c = count + u - share.u0;
+                // S first: with it the step's scales are the next ones to come, if they are not there
+                ok = wait_one(&sh.s_full[t][b], done >> 1, a.err, 906) && wait_one(&sh.info_full[c % kInfo], c / kInfo, a.err, 906);
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t s[64], pairs[32];
+                tmem_ld64(tS + b * 64, s);
+                tmem_ld_wait();
+                const PageScale* info = sh.info[c % kInfo];
+                float alpha;
+                if ((u + 1) * kStep - 1 > stream_first) softmax_step<true>(s, pairs, info, qs, u * kStep, lim, m, l, alpha);
+                else softmax_step<false>(s, pairs, info, qs, u * kStep, lim, m, l, alpha);
+                tmem_st32(tS + b * 64, pairs);
+                if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                    // O *= alpha once the step before has landed, and before this one is issued
+                    ok = wait_one(&sh.o_done[t][b ^ 1], (done - 1) >> 1, a.err, 907);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int part = 0; part < 4; ++part) {
+                        uint32_t o[32];
+                        tmem_ld32(tO + part * 32, o);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                        tmem_st32(tO + part * 32, o);
+                    }
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.p_full[t][b]);
+            }
+            if (own > 0 && ok) ok = wait_one(&sh.o_done[t][(done - 1) & 1], (done - 1) >> 1, a.err, 907);
+            tc_fence_after();
+            const bool nan_seen = *reinterpret_cast<volatile int*>(&sh.nan_seen[item % kInfo]) != 0;
+            // the row's sums, 32 dimensions at a time
+            auto sums = [&](int part, uint32_t (&o)[32]) {
+                if (own > 0 && ok) {
+                    tmem_ld32(tO + part * 32, o);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0u;
+                }
+                if (nan_seen) {  // NaN values between the block's first row and this one: their dimensions are NaN
+                    uint32_t gone = 0;
+                    for (int k = max(first_lim + 1, share.u0 * kStep); k <= min(lim, share.u1 * kStep - 1); ++k) {
+                        int page = a.page_table[static_cast<int64_t>(it.r) * a.max_pages + k / kPage];
+                        if (page < 0 || page >= a.num_pages) page = 0;
+                        const int tk = k % kPage;
+                        const uint8_t* v = a.kv8 + (static_cast<int64_t>(page) * a.hkv + it.h) * kKv8Bytes + kKv8Values + part * 512 +
+                                           tk % 8 / 2 * 16 + tk / 8 * 2 + tk % 2;
+#pragma unroll 1
+                        for (int d = 0; d < 32; ++d)
+                            if ((v[d / 4 * 64 + d % 4 * 4] & 0x7f) == 0x7f) gone |= 1u << d;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (gone >> e & 1) o[e] = 0x7fffffffu;
+                }
+            };
+            float scale0 = 1.f, scale1 = 0.f;  // FEW: factors of the streams' sums
+            float* other = reinterpret_cast<float*>(sQ);  // FEW: stream 1's sums [dimension][row]
+            if (FEW) {
+                named_barrier(1, 256);  // both streams are done with Q
+                if (t == 1) {
+                    sh.ml[row] = make_float2(m, l);
+                    if (own > 0) {
+#pragma unroll 1
+                        for (int part = 0; part < 4; ++part) {
+                            uint32_t o[32];
+                            sums(part, o);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) other[(part * 32 + e) * kRows + row] = __uint_as_float(o[e]);
+                        }
+                    }
+                }
+                named_barrier(1, 256);
+                if (t == 0 && share.own(it, per_stream, 1) > 0) {
+                    const float2 x = sh.ml[row];
+                    const float M = fmaxf(m, x.x);
+                    scale0 = m == kNegInf ? 1.f : exp2_ftz(m - M);
+                    scale1 = x.x == kNegInf ? 1.f : exp2_ftz(x.x - M);
+                    l = l * scale0 + x.y * scale1;
+                    m = M;
+                }
+            }
+            const bool joins = FEW && share.own(it, per_stream, 1) > 0;
+            const int64_t a0 = walk.first / per, a1 = (walk.first + it.units - 1) / per;
+            // a CTA takes part in at most one item that it did not begin and one that it does not end
+            const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (blockIdx.x == a0);
+            constexpr int kSlotRows = FEW ? kRows : 2 * kRows;
+            const int slot_row = FEW ? row : t * kRows + row;
+            if (!FEW || t == 0) {
+                const float inv = a0 != a1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+                if (a0 != a1 && live) *reinterpret_cast<float2*>(a.ws_ml + (slot * kSlotRows + slot_row) * 2) = make_float2(m, l);
+#pragma unroll 1
+                for (int part = 0; part < 4; ++part) {
+                    uint32_t o[32];
+                    sums(part, o);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        float x = __uint_as_float(o[e]);
+                        if (joins) x = x * scale0 + other[(part * 32 + e) * kRows + row] * scale1;
+                        o[e] = __float_as_uint(x * inv);
+                    }
+                    if (!live) continue;
+                    if (a0 != a1) {
+                        float4* dst = reinterpret_cast<float4*>(a.ws_o + (slot * kSlotRows + slot_row) * kHd + part * 32);
+#pragma unroll
+                        for (int c = 0; c < 8; ++c)
+                            dst[c] = make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]), __uint_as_float(o[4 * c + 2]),
+                                                 __uint_as_float(o[4 * c + 3]));
+                    } else {
+                        uint4* dst = reinterpret_cast<uint4*>(a.out + at + part * 32);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                w[e] = pack_bf16x2(__uint_as_float(o[8 * c + 2 * e]), __uint_as_float(o[8 * c + 2 * e + 1]));
+                            dst[c] = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                }
+            }
+            if (a0 != a1) {
+                __threadfence();
+                named_barrier(1, 256);
+                int* arrived = a.ws_count + (static_cast<int64_t>(it.r) * a.row_blocks + it.rb) * a.hkv + it.h;
+                if (tid == 0) sh.last = atomicAdd(arrived, 1) == static_cast<int>(a1 - a0);
+                named_barrier(1, 256);
+                if (sh.last) {
+                    __threadfence();
+                    kv8_join<kSlotRows>(a, it, group, a0, a1, tid, 256);
+                    if (tid == 0) *arrived = 0;
+                }
+            } else if (FEW) {
+                named_barrier(1, 256);  // stream 1's sums were read: Q may come
+            }
+            tc_fence_before();
+            count += share.u1 - share.u0;
+            ++item;
+            if (last_item()) break;
+            walk.next(a, per_block);
+        }
+    } else if (warp < 12) {
+        // ---------------- keys and values of each step into f16 tiles
+        const int cw = warp - 8, ct = tid - 256;
+        // keys: half of the dimensions, token, 16 dimensions of it; the row is the token's place
+        const int k_half = ct >> 6, k_tok = (ct >> 2) & 15, k_c = ct & 3;
+        const int k_place = k_tok % 8 / 2 * 4 + k_tok / 8 * 2 + k_tok % 2;
+        // values: 8 keys of a page (half v_b), group of four dimensions, page v_page or v_page + 2: eight lanes store
+        // to eight different 16-byte columns, and load with two to a bank
+        const int v_b = lane & 1, v_dq = (lane >> 1 & 1) | (lane >> 3) << 1 | cw << 3, v_page = lane >> 2 & 1;
+        int c = 0, taken[2] = {0, 0};
+        while (ok) {
+            const Share<FEW> share(walk, begin, end);
+            const Kv8Item& it = walk.it;
+            const int first_lim = it.L - it.n + it.row0, last_lim = first_lim + it.rows - 1;
+            for (int u = share.u0; u < share.u1 && ok; ++u, ++c) {
+                const int raw = c % kRaw, t = FEW ? (u - share.u0) & 1 : 0;
+                const int st = stage_of<FEW>(t, taken[t]), use = use_of<FEW>(taken[t]);
+                ++taken[t];
+                ok = wait_two(&sh.raw_full[raw], c / kRaw, use == 0 ? &sh.raw_full[raw] : &sh.k_empty[st],
+                              use == 0 ? c / kRaw : use - 1, a.err, 908);
+                if (!ok) break;
+                const uint8_t* src = sRaw + raw * kPages * kKv8Bytes;
+                {
+                    uint4 w[kPages];
+#pragma unroll
+                    for (int i = 0; i < kPages; ++i) w[i] = *reinterpret_cast<const uint4*>(src + i * kKv8Bytes + k_half * 1024 + k_tok * 64 + k_c * 16);
+                    uint8_t* kd = sK + st * kKTile + k_half * (kKTile / 2);
+#pragma unroll
+                    for (int i = 0; i < kPages; ++i) {
+                        const int row = i * kPage + k_place;
+                        uint32_t f[8];
+                        e4m3x4_to_half(w[i].x, f[0], f[1]);
+                        e4m3x4_to_half(w[i].y, f[2], f[3]);
+                        e4m3x4_to_half(w[i].z, f[4], f[5]);
+                        e4m3x4_to_half(w[i].w, f[6], f[7]);
+                        *reinterpret_cast<uint4*>(kd + row * 128 + (((2 * k_c) ^ (row & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
+                        *reinterpret_cast<uint4*>(kd + row * 128 + (((2 * k_c + 1) ^ (row & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
+                    }
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.k_full[st]);
+                uint4 w[2][2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+                        w[i][x] = *reinterpret_cast<const uint4*>(src + (v_page + 2 * i) * kKv8Bytes + kKv8Values + v_dq * 64 + v_b * 32 + x * 16);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.raw_empty[raw]);
+                if ((u + 1) * kStep - 1 > first_lim) {  // some row does not see all of the step
+                    bool any = false;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const int key = u * kStep + (v_page + 2 * i) * kPage;
+                            uint32_t hidden = 0, seen = 0;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int k = key + (e >> 1) * 8 + (2 * v_b + x) * 2 + (e & 1);
+                                if (k > first_lim) hidden |= 0x80u << (8 * e);
+                                if (k <= last_lim) seen |= 0x80u << (8 * e);
+                            }
+                            uint32_t y[4] = {w[i][x].x, w[i][x].y, w[i][x].z, w[i][x].w};
+#pragma unroll
+                            for (int d = 0; d < 4; ++d) {
+                                const uint32_t bad = nan_codes(y[d]) & hidden;
+                                any |= (bad & seen) != 0;
+                                y[d] &= ~((bad >> 7) * 0xffu);
+                            }
+                            w[i][x] = make_uint4(y[0], y[1], y[2], y[3]);
+                        }
+                    if (any) *reinterpret_cast<volatile int*>(&sh.nan_seen[item % kInfo]) = 1;
+                    __threadfence_block();
+                }
+                if (use > 0) ok = wait_one(&sh.v_empty[st], use - 1, a.err, 909);
+                if (!ok) break;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t w0[4] = {w[i][0].x, w[i][0].y, w[i][0].z, w[i][0].w};
+                    const uint32_t w1[4] = {w[i][1].x, w[i][1].y, w[i][1].z, w[i][1].w};
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int dim = v_dq * 4 + x;
+                        uint32_t f[4];
+                        e4m3x4_to_half(w0[x], f[0], f[1]);
+                        e4m3x4_to_half(w1[x], f[2], f[3]);
+                        *reinterpret_cast<uint4*>(sV + st * kVTile + dim * 128 + (((2 * (v_page + 2 * i) + v_b) ^ (dim & 7)) << 4)) =
+                            make_uint4(f[0], f[1], f[2], f[3]);
+                    }
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.v_full[st]);
+            }
+            ++item;
+            if (last_item()) break;
+            walk.next(a, per_block);
+        }
+    } else if (warp < 14) {
+        // ---------------- MMAs of stream t: the warp waits together, one lane issues (descriptors stay uniform)
+        constexpr uint32_t id_s = idesc_f16(kRows, kStep), id_o = idesc_f16(kRows, kHd);
+        const int t = warp - 12;
+        const bool lead = elect_lane();
+        const uint64_t dQ = umma_desc_sw128(smem_u32(sQ + t * kQTile)), dK = umma_desc_sw128(smem_u32(sK)), dV = umma_desc_sw128(smem_u32(sV));
+        const uint32_t tS = tmem + t * 128, tO = tmem + 256 + t * 128;
+        int s_count = 0, p_count = 0, loaded = 0;  // S and PV issued so far, items in which the stream had any
+        while (ok) {
+            const Share<FEW> share(walk, begin, end);
+            const int own = share.own(walk.it, per_stream, t);
+            auto issue_s = [&](int i) {  // S of the i-th own step into its buffer, which p of two steps before has left
+                if (i >= own || !ok) return;
+                const int n = FEW ? s_count : count + i, st = stage_of<FEW>(t, n), use = use_of<FEW>(n), b = s_count & 1;
+                if (i == 0) ok = wait_one(&sh.q_full[t], loaded, a.err, 905);
+                ok = ok && wait_two(&sh.k_full[st], use, s_count < 2 ? &sh.k_full[st] : &sh.o_done[t][b],
+                                    s_count < 2 ? use : (s_count - 2) >> 1, a.err, 908);
+                if (!ok) return;
+                tc_fence_after();
+                if (lead) {
+                    const uint64_t k = dK + (st * kKTile >> 4);
+#pragma unroll
+                    for (int x = 0; x < 8; ++x)  // 16 dimensions: 32 bytes; the second 64 lie in the other half tile
+                        umma_bf16(tS + b * 64, dQ + (((x >> 2) * (kQTile / 2) + (x & 3) * 32) >> 4),
+                                  k + (((x >> 2) * (kKTile / 2) + (x & 3) * 32) >> 4), id_s, x > 0 ? 1u : 0u);
+                    umma_commit(&sh.s_full[t][b]);
+                    umma_commit(&sh.k_empty[st]);
+                }
+                __syncwarp();
+                ++s_count;
+            };
+            issue_s(0);
+            issue_s(1);
+            for (int i = 0; i < own && ok; ++i) {
+                const int n = FEW ? p_count : count + i, st = stage_of<FEW>(t, n), b = p_count & 1;
+                ok = wait_two(&sh.v_full[st], use_of<FEW>(n), &sh.p_full[t][b], p_count >> 1, a.err, 909);
+                if (!ok) break;
+                tc_fence_after();
+                if (lead) {
+                    const uint64_t v = dV + (st * kVTile >> 4);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)  // 16 keys: 8 columns of p
+                        umma_bf16_ta(tO, tS + b * 64 + x * 8, v + (x * 32 >> 4), id_o, (i > 0 || x > 0) ? 1u : 0u);
+                    umma_commit(&sh.o_done[t][b]);
+                    umma_commit(&sh.v_empty[st]);
+                }
+                __syncwarp();
+                ++p_count;
+                issue_s(i + 2);
+            }
+            // steps that only the other stream sees: their stages are free as far as this one goes
+            if (!FEW)
+                for (int u = share.u0 + own; u < share.u1 && ok; ++u) {
+                    const int c = count + u - share.u0, st = c % kStages;
+                    ok = wait_two(&sh.k_full[st], c / kStages, &sh.v_full[st], c / kStages, a.err, 908);
+                    if (ok && lead) {
+                        mbar_arrive(&sh.k_empty[st]);
+                        mbar_arrive(&sh.v_empty[st]);
+                    }
+                    __syncwarp();
+                }
+            count += share.u1 - share.u0;
+            if (own > 0) ++loaded;
+            if (last_item()) break;
+            walk.next(a, per_block);
+        }
+    } else if (warp == 14) {
+        // ---------------- codes and scales of each step
+        int c = 0;
+        while (ok) {
+            const Share<FEW> share(walk, begin, end);
+            const Kv8Item& it = walk.it;
+            const int seen = (it.L - it.n + it.row0 + it.rows - 1) / kPage + 1;  // pages that any row sees
+            const int* table = a.page_table + static_cast<int64_t>(it.r) * a.max_pages;
+            auto page_id = [&](int u) {  // lane 4 s + p: page p of step u + s; -1 behind the CTA's part
+                const int p = u * kPages + lane;
+                return p < min(seen, share.u1 * kPages) ? table[p] : -1;
+            };
+            int ids = page_id(share.u0), ids_next = -1;
+            uint32_t sc = 0x7f7f;
+            for (int u = share.u0; u < share.u1 && ok; ++u, ++c) {
+                const int at = (u - share.u0) % 8 * kPages;
+                if (at == 0) {
+                    if (u > share.u0) ids = ids_next;
+                    ids_next = page_id(u + 8);
+                    const bool none = (u * kPages + lane) >= min(seen, share.u1 * kPages);
+                    if (!none && (ids < 0 || ids >= a.num_pages)) {
+                        record_error(a.err, MSGL_ERR_BOUNDS, 902);
+                        ids = 0;
+                    }
+                    sc = none ? 0x7f7fu : *reinterpret_cast<const uint16_t*>(a.scales + (static_cast<int64_t>(ids) * a.hkv + it.h) * 2);
+                    if (none) ids = -1;
+                }
+                const int raw = c % kRaw;
+                if (u == share.u0 && lane == 0) sh.nan_seen[item % kInfo] = 0;  // last of an item that is done
+                if (c >= kRaw) ok = wait_one(&sh.raw_empty[raw], c / kRaw - 1, a.err, 908);
+                if (!ok) break;
+                const int pages = min(kPages, seen - u * kPages);
+                if (lane == 0) mbar_arrive_expect_tx(&sh.raw_full[raw], pages * kKv8Bytes);
+                __syncwarp();
+                if (lane >= at && lane < at + kPages) {
+                    if (lane < at + pages)
+                        bulk_load(sRaw + (raw * kPages + lane - at) * kKv8Bytes, a.kv8 + (static_cast<int64_t>(ids) * a.hkv + it.h) * kKv8Bytes,
+                                  kKv8Bytes, &sh.raw_full[raw]);
+                    const int ve = sc >> 8;
+                    sh.info[c % kInfo][lane - at] = {kv8_power(sc & 0xff), static_cast<float>(ve - 127), kv8_inverse(ve), 0.f};
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.info_full[c % kInfo]);
+            }
+            ++item;
+            if (last_item()) break;
+            walk.next(a, per_block);
+        }
+    }
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <bool FEW>
+int launch(const Kv8AttnArgs& a, int grid, msgl_stream_t stream) {
+    static std::atomic<int> optin[kMaxDevices];
+    const cudaError_t e = smem_optin(attend_tiles_kernel<FEW>, kSmem, optin);
+    if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
+    launch_pdl(attend_tiles_kernel<FEW>, dim3(grid), dim3(kThreads), kSmem, stream, a);
+    MSGL_LAUNCH_CHECK();
+    return MSGL_OK;
+}
+
+}  // namespace
+
+int launch_attend_tiles(const Kv8AttnArgs& a, bool few, int grid, msgl_stream_t stream) {
+    return few ? launch<true>(a, grid, stream) : launch<false>(a, grid, stream);
+}
+
+}  // namespace msgl
