@@ -439,10 +439,10 @@ MSGL_API int msgl_qknorm_rope_store_kv8_partials(const float* parts, int nparts,
  * rows per request, max_seq_len (<= max_pages * 16) the contexts. Recorded as MSGL_ERR_BOUNDS: a
  * context outside [0, max_seq_len] (clamped, site 900), a request with more than max_q_len rows or
  * rows outside total_q (skipped, site 901), a page outside the pool (page 0 in its place, site 902).
- * The workspace (msgl_paged_attention_kv8_workspace_size, 16-byte aligned) is zero-filled once before
- * its first use and left zero-filled where it counts; it serves every call with no more requests and
- * rows a request of the same head counts; calls that overlap on the GPU need one each. */
-MSGL_API size_t msgl_paged_attention_kv8_workspace_size(int num_reqs, int max_q_len, int num_q_heads,
+ * The workspace (msgl_paged_attention_kv8_workspace_size, 16-byte aligned) needs no clearing and serves
+ * every call with no more rows a request of the same head counts, whatever their number and contexts;
+ * calls that overlap on the GPU need one each. */
+MSGL_API size_t msgl_paged_attention_kv8_workspace_size(int max_q_len, int num_q_heads,
                                                         int num_kv_heads);
 MSGL_API int msgl_paged_attention_kv8(const void* q, const void* kv8, const void* scales,
                                       int64_t num_pages, const int* page_table, int max_pages,

@@ -323,8 +323,7 @@ int launch_store(StoreArgs a, int head_dim, int page_size, msgl_stream_t stream)
 // 24 or 32 MMAs, 64 conversions.
 //
 // In a CTA the pages of an item go around the warps, each with a ring of 4 KB stages that one lane fills by
-// bulk copies across items. Where an item is shared by CTAs they leave partial sums in the workspace and
-// the last of them to arrive joins them in order.
+// bulk copies across items. Where an item is shared by CTAs they leave partial sums in the workspace.
 constexpr int kWarps = 8;
 constexpr int kAttThreads = kWarps * 32;
 constexpr int kPitch = kHd + 4;  // floats of a row in the joining buffer
@@ -561,7 +560,6 @@ attend_rows_kernel(const Kv8AttnArgs a) {
     float* join_ml = join + kWarps * S::kRows * kPitch;                            // [warp][row]{m, l}
     __shared__ uint64_t full[S::kRing * kWarps];
     __shared__ Kv8Scan<kAttThreads> scan;
-    __shared__ int s_flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int group = a.hq / a.hkv;
     if (tid == 0) {
@@ -677,7 +675,8 @@ attend_rows_kernel(const Kv8AttnArgs a) {
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int w = 0; w < kWarps; ++w) {
                 const float ms = join_ml[(w * S::kRows + m) * 2];
-                const float f = ms == kNegInf ? 1.f : exp2_ftz(ms - M);  // as in kv8_join
+                // a warp without a visible key has l = 0 (or NaN where a NaN was seen)
+                const float f = ms == kNegInf ? 1.f : exp2_ftz(ms - M);
                 const float4 x = *reinterpret_cast<const float4*>(join + (w * S::kRows + m) * kPitch + d);
                 l += join_ml[(w * S::kRows + m) * 2 + 1] * f;
                 o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
@@ -694,41 +693,74 @@ attend_rows_kernel(const Kv8AttnArgs a) {
                 }
             }
         }
-        if (a0 != a1) {
-            __threadfence();
-            __syncthreads();
-            int* count = a.ws_count + (static_cast<int64_t>(use.it.r) * a.row_blocks + use.it.rb) * a.hkv + use.it.h;
-            if (tid == 0) s_flag = atomicAdd(count, 1) == static_cast<int>(a1 - a0);
-            __syncthreads();
-            if (s_flag) {
-                __threadfence();
-                kv8_join<S::kRows>(a, use.it, group, a0, a1, tid, kAttThreads);
-                if (tid == 0) *count = 0;
-            }
-        }
         if (use.first + use.it.units >= end) break;
         use.next(a, per_block);
     }
 }
 
+// ------------------------------------------------------------------ joining
+// Partial sums of the items that CTAs share, in the CTAs' order. Block (b, y): the item that CTA b goes on with, if
+// the CTA before it is the first; rows 8 y .. 8 y + 7 of every gridDim.y x 8, a warp per row, a lane per four dimensions,
+// eight parts' loads in flight. A kernel of its own: the last CTA of an item to arrive took XX us for 19 parts of 2
+// rows and 30 us for five of 256.
+constexpr int kJoinWarps = 8;
+
+__global__ void __launch_bounds__(kJoinWarps * 32)
+join_shared_kernel(const Kv8AttnArgs a, int slot_rows) {
+    pdl_wait();
+    pdl_trigger();
+    const Kv8Shared s = a.ws_shared[blockIdx.x + 1];
+    if (s.last < s.first || s.first != static_cast<int>(blockIdx.x)) return;
+    const int lane = threadIdx.x & 31, group = a.hq / a.hkv;
+    for (int m = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); m < s.rows; m += gridDim.y * kJoinWarps) {
+        float M = kNegInf, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int b0 = s.first; b0 <= s.last; b0 += 8) {
+            float2 ml[8];
+            float4 x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int b = b0 + i;
+                const int64_t w = (2 * static_cast<int64_t>(b) + (b == s.first)) * slot_rows + m;
+                ml[i] = b <= s.last ? __ldcg(reinterpret_cast<const float2*>(a.ws_ml) + w) : make_float2(kNegInf, 0.f);
+                x[i] = b <= s.last ? __ldcg(reinterpret_cast<const float4*>(a.ws_o + w * kHd) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            float next = M;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) next = fmaxf(next, ml[i].x);
+            const float f0 = M == kNegInf ? 1.f : exp2_ftz(M - next);
+            l *= f0;
+            o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
+            M = next;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                // a part without a visible key has l = 0 (or NaN where a NaN was seen)
+                const float f = ml[i].x == kNegInf ? 1.f : exp2_ftz(ml[i].x - M);
+                l += ml[i].y * f;
+                o.x += x[i].x * f; o.y += x[i].y * f; o.z += x[i].z * f; o.w += x[i].w * f;
+            }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        *reinterpret_cast<uint2*>(a.out + ((s.q_row + m / group) * a.hq + s.h * group + m % group) * kHd + lane * 4) =
+            make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+    }
+}
+
 // ------------------------------------------------------------------ host side
-// Counters of every (request, row block, kv head), then the partial sums of two items a CTA.
+// What each CTA goes on with, then the partial sums of two items a CTA.
 struct RowsPlan {
     int rows;  // of a block: MMA rows
-    int row_blocks, grid;
+    int grid;
     size_t off_o, off_ml, bytes;
 };
 
-RowsPlan plan_rows(int num_reqs, int max_q_len, int hq, int hkv) {
+RowsPlan plan_rows(int max_q_len, int hq, int hkv) {
     RowsPlan p{};
-    const int group = hq / hkv;
-    const int64_t rows = static_cast<int64_t>(max_q_len) * group;
+    const int64_t rows = static_cast<int64_t>(max_q_len) * (hq / hkv);
     p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 128 ? 128 : 256;
-    p.row_blocks = (max_q_len + p.rows / group - 1) / (p.rows / group);
     p.grid = 148 * (p.rows == 8 ? 2 : 1);
-    const size_t count = (static_cast<size_t>(num_reqs) * p.row_blocks * hkv * 4 + 255) / 256 * 256;
-    p.off_o = count;
-    p.off_ml = count + static_cast<size_t>(p.grid) * 2 * p.rows * kHd * 4;
+    p.off_o = (p.grid * sizeof(Kv8Shared) + 255) / 256 * 256;
+    p.off_ml = p.off_o + static_cast<size_t>(p.grid) * 2 * p.rows * kHd * 4;
     p.bytes = p.off_ml + static_cast<size_t>(p.grid) * 2 * p.rows * 8;
     return p;
 }
@@ -828,15 +860,15 @@ int msgl_qknorm_rope_store_kv8_partials(const float* parts, int nparts, void* q_
     return launch_store(a, head_dim, page_size, stream);
 }
 
-size_t msgl_paged_attention_kv8_workspace_size(int num_reqs, int max_q_len, int num_q_heads, int num_kv_heads) {
-    if (num_reqs <= 0 || max_q_len <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads ||
-        num_q_heads / num_kv_heads > 8 || num_reqs > 65535 || num_kv_heads > 1024)
+size_t msgl_paged_attention_kv8_workspace_size(int max_q_len, int num_q_heads, int num_kv_heads) {
+    if (max_q_len <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads ||
+        num_q_heads / num_kv_heads > 8)
         return 0;
     // the largest of the forms that this call or a smaller one may take
     const int group = num_q_heads / num_kv_heads;
-    size_t most = plan_rows(num_reqs, max_q_len, num_q_heads, num_kv_heads).bytes;
+    size_t most = plan_rows(max_q_len, num_q_heads, num_kv_heads).bytes;
     for (int rows : {8, 16, 128})
-        most = std::max(most, plan_rows(num_reqs, std::min(max_q_len, rows / group), num_q_heads, num_kv_heads).bytes);
+        most = std::max(most, plan_rows(std::min(max_q_len, rows / group), num_q_heads, num_kv_heads).bytes);
     return most;
 }
 
@@ -873,22 +905,22 @@ int msgl_paged_attention_kv8(const void* q, const void* kv8, const void* scales,
     a.hkv = num_kv_heads;
     a.sl2e = scale * 1.4426950408889634f;
     a.out = static_cast<__nv_bfloat16*>(out);
-    const RowsPlan p = plan_rows(num_reqs, a.max_q_len, num_q_heads, num_kv_heads);
+    const RowsPlan p = plan_rows(a.max_q_len, num_q_heads, num_kv_heads);
     if (!workspace || workspace_bytes < p.bytes || !aligned16(workspace))
         return set_error(MSGL_ERR_WORKSPACE, "attention_kv8: workspace missing, too small or not 16-byte aligned");
     a.err = device_error_word();
     if (!a.err) return set_error(MSGL_ERR_CUDA, "device error word unavailable");
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    a.ws_count = reinterpret_cast<int*>(ws);
+    a.ws_shared = reinterpret_cast<Kv8Shared*>(ws);
     a.ws_o = reinterpret_cast<float*>(ws + p.off_o);
     a.ws_ml = reinterpret_cast<float*>(ws + p.off_ml);
-    a.row_blocks = p.row_blocks;
-    if (p.rows <= 16) {
-        a.min_units = 8;  // a page for each warp
-        return p.rows == 8 ? launch_rows<1>(a, p.grid, stream) : launch_rows<2>(a, p.grid, stream);
-    }
-    a.min_units = 4;
-    return launch_attend_tiles(a, p.rows == 128, p.grid, stream);
+    a.min_units = p.rows <= 16 ? kWarps : 4;  // a page for each warp, or 256 keys
+    rc = p.rows == 8 ? launch_rows<1>(a, p.grid, stream) : p.rows == 16 ? launch_rows<2>(a, p.grid, stream)
+                                                          : launch_attend_tiles(a, p.rows == 128, p.grid, stream);
+    if (rc) return rc;
+    launch_pdl(join_shared_kernel, dim3(p.grid - 1, std::min(p.rows / kJoinWarps, 8)), dim3(kJoinWarps * 32), 0, stream, a, p.rows);
+    MSGL_LAUNCH_CHECK();
+    return MSGL_OK;
 }
 
 }  // extern "C"

@@ -16,7 +16,8 @@
 #include "kv8_args.h"
 
 namespace msgl {
-// Attention of more than 16 rows x heads of a group (kv8_tiles.cu).
+// Attention of more than 16 rows x heads of a group (kv8_tiles.cu). Items that CTAs share are left as partial sums:
+// CTA b's in slot 2 b where it goes on with an item, in slot 2 b + 1 where it leaves one to the next.
 int launch_attend_tiles(const Kv8AttnArgs& a, bool few, int grid, msgl_stream_t stream);
 
 constexpr int kKv8Page = 16;
@@ -139,7 +140,8 @@ __device__ __forceinline__ void zero_rows(const Kv8AttnArgs& a, int q0, int rows
 }
 
 // This CTA's part [begin, end) of all units and the item that holds its first; false where there is none. Rows
-// before their context's first token get zeros on the way. Every thread of the block calls it.
+// before their context's first token get zeros on the way, and the workspace is told of an item that the CTA before
+// began. Every thread of the block calls it.
 template <int THREADS, int UNIT>
 __device__ __forceinline__ bool kv8_part(const Kv8AttnArgs& a, int per_block, Kv8Scan<THREADS>& sh, int64_t& per, int64_t& begin,
                                          int64_t& end, Kv8Walk<UNIT>& walk) {
@@ -165,7 +167,10 @@ __device__ __forceinline__ bool kv8_part(const Kv8AttnArgs& a, int per_block, Kv
     per = larger((total + gridDim.x - 1) / gridDim.x, a.min_units);
     begin = per * blockIdx.x;
     end = smaller(total, begin + per);
-    if (begin >= end) return false;
+    if (begin >= end) {
+        if (tid == 0) a.ws_shared[blockIdx.x] = {0, -1, 0, 0, 0};
+        return false;
+    }
     int64_t base = 0;
     for (int r0 = 0; r0 < a.num_reqs; r0 += THREADS) {  // blocks of requests, until their sum passes `begin`
         const int r = r0 + tid;
@@ -197,33 +202,14 @@ __device__ __forceinline__ bool kv8_part(const Kv8AttnArgs& a, int per_block, Kv
     kv8_request(a, walk.it.r, false, walk.it.L, walk.it.n, walk.it.q0);
     walk.set_block(per_block);
     while (walk.it.units == 0 || walk.first + walk.it.units <= begin) walk.next(a, per_block);
-    return true;
-}
-
-// Joins the partial sums of an item that the CTAs a0 .. a1 share, in their order: rows (query row x head of the
-// group) x 128 values by `threads` threads. ROWS: rows of a slot.
-template <int ROWS>
-__device__ __forceinline__ void kv8_join(const Kv8AttnArgs& a, const Kv8Item& it, int group, int64_t a0, int64_t a1, int tid, int threads) {
-    for (int i = tid; i < it.rows * group * (kKv8Head / 4); i += threads) {
-        const int m = i / (kKv8Head / 4), d = i % (kKv8Head / 4) * 4;
-        float M = -__builtin_huge_valf(), l = 0.f;
-#pragma unroll 4
-        for (int64_t b = a0; b <= a1; ++b) M = fmaxf(M, __ldcg(a.ws_ml + ((2 * b + (b == a0)) * ROWS + m) * 2));
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int64_t b = a0; b <= a1; ++b) {
-            const int64_t w = (2 * b + (b == a0)) * ROWS + m;
-            const float ms = __ldcg(a.ws_ml + 2 * w);
-            // a part without a visible key has l = 0 (or NaN where a NaN was seen)
-            const float f = ms == -__builtin_huge_valf() ? 1.f : exp2_ftz(ms - M);
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(a.ws_o + w * kKv8Head + d));
-            l += __ldcg(a.ws_ml + 2 * w + 1) * f;
-            o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
-        }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(it.q0 + it.row0 + m / group) * a.hq + it.h * group + m % group) * kKv8Head + d) =
-            make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+    if (tid == 0) {
+        const Kv8Item& it = walk.it;
+        const int a0 = static_cast<int>(walk.first / per), a1 = static_cast<int>((walk.first + it.units - 1) / per);
+        const int group = a.hq / a.hkv;
+        if (walk.first < begin) a.ws_shared[blockIdx.x] = {a0, a1, it.q0 + static_cast<int64_t>(it.row0), it.h, it.rows * group};
+        else a.ws_shared[blockIdx.x] = {0, -1, 0, 0, 0};
     }
+    return true;
 }
 
 }  // namespace msgl

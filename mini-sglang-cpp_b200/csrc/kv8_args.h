@@ -4,6 +4,13 @@
 #include <stdint.h>
 
 namespace msgl {
+// An item that several CTAs share: CTAs first .. last; query row of out, kv head, rows x heads of the group.
+struct Kv8Shared {
+    int first, last;
+    int64_t q_row;
+    int h, rows;
+};
+
 struct Kv8AttnArgs {
     const __nv_bfloat16* q;
     const uint8_t *kv8, *scales;
@@ -15,8 +22,7 @@ struct Kv8AttnArgs {
     float sl2e;  // scale * log2(e)
     __nv_bfloat16* out;
     float *ws_o, *ws_ml;
-    int* ws_count;
-    int row_blocks;  // of a request, at most
+    struct Kv8Shared* ws_shared;  // by CTA: the item that it goes on with from the CTA before
     int min_units;   // of a CTA, at least
     int* err;
 };

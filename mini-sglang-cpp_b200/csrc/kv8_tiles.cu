@@ -1,8 +1,7 @@
 // kv8_tiles.cu -- attention of many rows (chunks, drafted rows) over the 8-bit key / value pool, on tcgen05.
 //
 // Persistent: each CTA takes an equal part of the steps (64 keys) of all items (block of query rows x kv head;
-// rows = query rows x the group's heads); items shared by CTAs are joined through the workspace by the last
-// CTA to arrive. Codes are converted to f16 (exactly) into the operands' canonical tiles, q is scaled to f16
+// rows = query rows x the group's heads); of items shared by CTAs they leave partial sums. Codes are converted to f16 (exactly) into the operands' canonical tiles, q is scaled to f16
 // by a power of two per row (2^-25 of its largest value). A page's scales enter the exponent:
 // s = (q . k) 2^(q + k exponents) scale log2(e) + (exponent of v), p = 2^(s - m) <= 2^8 in f16, so that O needs
 // no scaling by page, and l adds p 2^-(exponent of v).
@@ -89,7 +88,6 @@ struct Shared {
     PageScale info[kInfo][kPages];
     int nan_seen[kInfo];  // by item in turn: a value hidden from some of its rows was NaN
     uint32_t tmem;
-    int last;
     union {
         Kv8Scan<kThreads> scan;  // before the walk
         float2 ml[kRows];        // stream 1's (m, l), FEW
@@ -426,18 +424,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                     }
                 }
             }
-            if (a0 != a1) {
-                __threadfence();
-                named_barrier(1, 256);
-                int* arrived = a.ws_count + (static_cast<int64_t>(it.r) * a.row_blocks + it.rb) * a.hkv + it.h;
-                if (tid == 0) sh.last = atomicAdd(arrived, 1) == static_cast<int>(a1 - a0);
-                named_barrier(1, 256);
-                if (sh.last) {
-                    __threadfence();
-                    kv8_join<kSlotRows>(a, it, group, a0, a1, tid, 256);
-                    if (tid == 0) *arrived = 0;
-                }
-            } else if (FEW) {
+            if (FEW) {
                 named_barrier(1, 256);  // stream 1's sums were read: Q may come
             }
             tc_fence_before();

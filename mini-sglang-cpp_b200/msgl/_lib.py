@@ -44,7 +44,7 @@ SIGNATURES = {
     "msgl_step_tables": (I, [P, P, P, I, P, P, I, P, I, I, I, P, P, P, P, P, P]),
     "msgl_qknorm_rope_store_kv8": (I, [P, P, P, P, I64, P, P, I, P, P, I, I, P, I, P, P, I, I, I, I, I, F, P]),
     "msgl_qknorm_rope_store_kv8_partials": (I, [P, I, P, P, P, I64, P, P, I, P, P, I, I, P, I, P, P, I, I, I, I, I, F, P]),
-    "msgl_paged_attention_kv8_workspace_size": (SZ, [I, I, I, I]),
+    "msgl_paged_attention_kv8_workspace_size": (SZ, [I, I, I]),
     "msgl_paged_attention_kv8": (I, [P, P, P, I64, P, I, P, P, I, I, I, I, I, I, I, I, F, P, P, SZ, P]),
     "msgl_token_probs": (I, [P, I64, I, I, P, P, I64, P]),
     "msgl_verify_drafts": (I, [P, I64, P, I64, P, P, P, P, I, I, I, I, P, P, P]),

@@ -493,8 +493,9 @@ def qknorm_rope_store_kv8_partials(parts, kv8, scales, positions, page_table, se
 
 
 def attention_kv8_workspace(num_reqs, max_q_len, hq, hkv, device="cuda"):
-    n = lib().msgl_paged_attention_kv8_workspace_size(num_reqs, max_q_len, hq, hkv)
-    return torch.zeros(max(n, 256), dtype=_U8, device=device)
+    """A workspace for every call with no more rows a request of these heads (its size does not hang on num_reqs)."""
+    n = lib().msgl_paged_attention_kv8_workspace_size(max_q_len, hq, hkv)
+    return torch.empty(max(n, 256), dtype=_U8, device=device)
 
 
 def paged_attention_kv8(q, kv8, scales, page_table, seq_lens, max_seq_len, hq, hkv, scale=_SCALE, q_indptr=None,
