@@ -14,8 +14,8 @@
 //   0-3, 4-7   softmax of stream 0 / 1: a thread per row. S from tensor memory, p as f16 pairs over the first
 //              half of S, l and m in registers; O in tensor memory is rescaled only where the maximum grew by
 //              more than 8;
-//   8-11       conversion of a step's four pages: keys [64][128], values [128][64], both K-major (the keys of a
-//              page in the order in which the pool stores their values);
+//   8, 9       conversion of a step's keys to [64][128], 10, 11 of its values to [128][64], both K-major (the keys
+//              of a page in the order in which the pool stores their values);
 //   12, 13     one lane each issues a stream's MMAs: PV(i), then S(i + 2). S has two buffers of 64 columns, so that
 //              the next S is there before the softmax of a step ends; while one stream waits for a hand-over
 //              (100 to 400 clocks each) the other's MMAs run;
@@ -83,7 +83,7 @@ struct PageScale {
 };
 
 struct Shared {
-    uint64_t raw_full[kRaw], raw_empty[kRaw], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], info_full[kInfo];
+    uint64_t raw_full[kRaw], raw_empty[kRaw], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
     uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2][2];  // stream, parity of its steps
     PageScale info[kInfo][kPages];
     int nan_seen[kInfo];  // by item in turn: a value hidden from some of its rows was NaN
@@ -115,37 +115,49 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return d;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // One step of a row: 64 S columns into pairs of p. EDGE: keys behind `lim` do not count. The factor of a page
 // is positive (qs is), so the page's largest logit comes from its largest product.
 template <bool EDGE>
 __device__ __forceinline__ void softmax_step(uint32_t (&s)[64], uint32_t (&out)[32], const PageScale* info, float qs, int key0,
                                              int lim, float& m, float& l, float& alpha) {
-    float mx = kNegInf;
+    float f[kPages], v_exp[kPages], v_inv[kPages], mx[kPages];
 #pragma unroll
     for (int p = 0; p < kPages; ++p) {
-        float pm[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+        const float4 sc = *reinterpret_cast<const float4*>(&info[p]);
+        f[p] = qs * sc.x;
+        v_exp[p] = sc.y;
+        v_inv[p] = sc.z;
+        float x[kPage];
 #pragma unroll
         for (int i = 0; i < kPage; ++i) {
-            uint32_t& x = s[p * kPage + i];
-            if (EDGE && key0 + p * kPage + token_at(i) > lim) x = 0xff800000u;
-            pm[i & 3] = fmaxf(pm[i & 3], __uint_as_float(x));
+            if (EDGE && key0 + p * kPage + token_at(i) > lim) s[p * kPage + i] = 0xff800000u;
+            x[i] = __uint_as_float(s[p * kPage + i]);
         }
-        mx = fmaxf(mx, fmaf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), qs * info[p].k, info[p].v_exp));
+        const float a = max3(max3(max3(x[0], x[1], x[2]), x[3], x[4]), x[5], x[6]);
+        const float b = max3(max3(max3(x[7], x[8], x[9]), x[10], x[11]), x[12], x[13]);
+        mx[p] = fmaf(fmaxf(max3(a, b, x[14]), x[15]), f[p], v_exp[p]);
     }
+    const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
     // The maximum moves only where it grows by more than 8: p stays below 2^8, which f16 holds as well.
-    const float next = m == kNegInf || mx > m + 8.f ? fmaxf(m, mx) : m;
+    const float next = m == kNegInf || top > m + 8.f ? fmaxf(m, top) : m;
     const float base = next == kNegInf ? 0.f : next;
     alpha = next == m ? 1.f : exp2_ftz(m - next);
     float sum = 0.f;
 #pragma unroll
     for (int p = 0; p < kPages; ++p) {
-        const uint64_t f = pair(qs * info[p].k), v = pair(info[p].v_exp - base);
+        const uint64_t f2 = pair(f[p]), v2 = pair(v_exp[p] - base);
         uint64_t part[2] = {0, 0};
 #pragma unroll
         for (int i = 0; i < kPage; i += 2) {
             const int c = p * kPage + i;
             float x, y;
-            unpair(fma2(pair(s[c], s[c + 1]), f, v), x, y);
+            unpair(fma2(pair(s[c], s[c + 1]), f2, v2), x, y);
             x = exp2_ftz(x);
             y = exp2_ftz(y);
             part[i / 2 & 1] = add2(part[i / 2 & 1], pair(__float_as_uint(x), __float_as_uint(y)));
@@ -153,7 +165,7 @@ __device__ __forceinline__ void softmax_step(uint32_t (&s)[64], uint32_t (&out)[
         }
         float a, b;
         unpair(add2(part[0], part[1]), a, b);
-        sum = fmaf(a + b, info[p].v_inv, sum);
+        sum = fmaf(a + b, v_inv[p], sum);
     }
     l = fmaf(l, alpha, sum);
     m = next;
@@ -212,15 +224,12 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
             mbar_init(&sh.raw_empty[i], 4);
         }
         for (int i = 0; i < kStages; ++i) {
-            mbar_init(&sh.k_full[i], 4);
+            mbar_init(&sh.k_full[i], 2);
             mbar_init(&sh.k_empty[i], FEW ? 1 : 2);
-            mbar_init(&sh.v_full[i], 4);
+            mbar_init(&sh.v_full[i], 2);
             mbar_init(&sh.v_empty[i], FEW ? 1 : 2);
         }
-        for (int i = 0; i < kInfo; ++i) {
-            mbar_init(&sh.info_full[i], 1);
-            sh.nan_seen[i] = 0;
-        }
+        for (int i = 0; i < kInfo; ++i) sh.nan_seen[i] = 0;
         for (int t = 0; t < 2; ++t) {
             mbar_init(&sh.q_full[t], 4);
             for (int b = 0; b < 2; ++b) {
@@ -300,8 +309,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
             }
             for (int i = 0; i < own && ok; ++i, ++done) {
                 const int b = done & 1, u = share.step(t, i), c = count + u - share.u0;
-                // S first: with it the step's scales are the next ones to come, if they are not there
-                ok = wait_one(&sh.s_full[t][b], done >> 1, a.err, 906) && wait_one(&sh.info_full[c % kInfo], c / kInfo, a.err, 906);
+                ok = wait_one(&sh.s_full[t][b], done >> 1, a.err, 906);
                 if (!ok) break;
                 tc_fence_after();
                 uint32_t s[64], pairs[32];
@@ -434,14 +442,14 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
             walk.next(a, per_block);
         }
     } else if (warp < 12) {
-        // ---------------- keys and values of each step into f16 tiles
-        const int cw = warp - 8, ct = tid - 256;
-        // keys: half of the dimensions, token, 16 dimensions of it; the row is the token's place
-        const int k_half = ct >> 6, k_tok = (ct >> 2) & 15, k_c = ct & 3;
-        const int k_place = k_tok % 8 / 2 * 4 + k_tok / 8 * 2 + k_tok % 2;
+        // ---------------- each step into f16 tiles: keys by warps 8 and 9, values by 10 and 11
+        const int ct = tid & 63;
+        const bool keys = warp < 10;
+        // keys: the page, half of the dimensions, token, 16 dimensions of it; the row is the token's place
+        const int k_tok = ct >> 2, k_c = ct & 3, k_place = k_tok % 8 / 2 * 4 + k_tok / 8 * 2 + k_tok % 2;
         // values: 8 keys of a page (half v_b), group of four dimensions, page v_page or v_page + 2: eight lanes store
         // to eight different 16-byte columns, and load with two to a bank
-        const int v_b = lane & 1, v_dq = (lane >> 1 & 1) | (lane >> 3) << 1 | cw << 3, v_page = lane >> 2 & 1;
+        const int v_b = lane & 1, v_dq = (lane >> 1 & 1) | (lane >> 3) << 1 | (warp & 1) << 4, v_page = lane >> 2 & 1;
         int c = 0, taken[2] = {0, 0};
         while (ok) {
             const Share<FEW> share(walk, begin, end);
@@ -451,45 +459,53 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 const int raw = c % kRaw, t = FEW ? (u - share.u0) & 1 : 0;
                 const int st = stage_of<FEW>(t, taken[t]), use = use_of<FEW>(taken[t]);
                 ++taken[t];
-                ok = wait_two(&sh.raw_full[raw], c / kRaw, use == 0 ? &sh.raw_full[raw] : &sh.k_empty[st],
-                              use == 0 ? c / kRaw : use - 1, a.err, 908);
+                uint64_t* empty = keys ? &sh.k_empty[st] : &sh.v_empty[st];
+                ok = wait_two(&sh.raw_full[raw], c / kRaw, use == 0 ? &sh.raw_full[raw] : empty, use == 0 ? c / kRaw : use - 1, a.err, 908);
                 if (!ok) break;
                 const uint8_t* src = sRaw + raw * kPages * kKv8Bytes;
-                {
-                    uint4 w[kPages];
+                if (keys) {
+                    uint4 w[kPages][2];
 #pragma unroll
-                    for (int i = 0; i < kPages; ++i) w[i] = *reinterpret_cast<const uint4*>(src + i * kKv8Bytes + k_half * 1024 + k_tok * 64 + k_c * 16);
-                    uint8_t* kd = sK + st * kKTile + k_half * (kKTile / 2);
+                    for (int i = 0; i < kPages; ++i)
 #pragma unroll
-                    for (int i = 0; i < kPages; ++i) {
-                        const int row = i * kPage + k_place;
-                        uint32_t f[8];
-                        e4m3x4_to_half(w[i].x, f[0], f[1]);
-                        e4m3x4_to_half(w[i].y, f[2], f[3]);
-                        e4m3x4_to_half(w[i].z, f[4], f[5]);
-                        e4m3x4_to_half(w[i].w, f[6], f[7]);
-                        *reinterpret_cast<uint4*>(kd + row * 128 + (((2 * k_c) ^ (row & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
-                        *reinterpret_cast<uint4*>(kd + row * 128 + (((2 * k_c + 1) ^ (row & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
-                    }
+                        for (int x = 0; x < 2; ++x) w[i][x] = *reinterpret_cast<const uint4*>(src + i * kKv8Bytes + x * 1024 + k_tok * 64 + k_c * 16);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.raw_empty[raw]);
+                    uint8_t* kd = sK + st * kKTile;
+#pragma unroll
+                    for (int i = 0; i < kPages; ++i)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const int row = i * kPage + k_place;
+                            uint32_t f[8];
+                            e4m3x4_to_half(w[i][x].x, f[0], f[1]);
+                            e4m3x4_to_half(w[i][x].y, f[2], f[3]);
+                            e4m3x4_to_half(w[i][x].z, f[4], f[5]);
+                            e4m3x4_to_half(w[i][x].w, f[6], f[7]);
+                            uint8_t* dst = kd + x * (kKTile / 2) + row * 128;
+                            *reinterpret_cast<uint4*>(dst + (((2 * k_c) ^ (row & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
+                            *reinterpret_cast<uint4*>(dst + (((2 * k_c + 1) ^ (row & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
+                        }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.k_full[st]);
+                    continue;
                 }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.k_full[st]);
-                uint4 w[2][2];
+                uint4 w[4][2];  // pages v_page + 2 (i / 2), groups v_dq + 8 (i % 2)
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
-                        w[i][x] = *reinterpret_cast<const uint4*>(src + (v_page + 2 * i) * kKv8Bytes + kKv8Values + v_dq * 64 + v_b * 32 + x * 16);
+                        w[i][x] = *reinterpret_cast<const uint4*>(src + (v_page + 2 * (i >> 1)) * kKv8Bytes + kKv8Values + (v_dq + 8 * (i & 1)) * 64 + v_b * 32 + x * 16);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.raw_empty[raw]);
                 if ((u + 1) * kStep - 1 > first_lim) {  // some row does not see all of the step
                     bool any = false;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                    for (int i = 0; i < 4; ++i)
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            const int key = u * kStep + (v_page + 2 * i) * kPage;
+                            const int key = u * kStep + (v_page + 2 * (i >> 1)) * kPage;
                             uint32_t hidden = 0, seen = 0;
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
@@ -509,19 +525,17 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                     if (any) *reinterpret_cast<volatile int*>(&sh.nan_seen[item % kInfo]) = 1;
                     __threadfence_block();
                 }
-                if (use > 0) ok = wait_one(&sh.v_empty[st], use - 1, a.err, 909);
-                if (!ok) break;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < 4; ++i) {
                     const uint32_t w0[4] = {w[i][0].x, w[i][0].y, w[i][0].z, w[i][0].w};
                     const uint32_t w1[4] = {w[i][1].x, w[i][1].y, w[i][1].z, w[i][1].w};
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        const int dim = v_dq * 4 + x;
+                        const int dim = (v_dq + 8 * (i & 1)) * 4 + x;
                         uint32_t f[4];
                         e4m3x4_to_half(w0[x], f[0], f[1]);
                         e4m3x4_to_half(w1[x], f[2], f[3]);
-                        *reinterpret_cast<uint4*>(sV + st * kVTile + dim * 128 + (((2 * (v_page + 2 * i) + v_b) ^ (dim & 7)) << 4)) =
+                        *reinterpret_cast<uint4*>(sV + st * kVTile + dim * 128 + (((2 * (v_page + 2 * (i >> 1)) + v_b) ^ (dim & 7)) << 4)) =
                             make_uint4(f[0], f[1], f[2], f[3]);
                     }
                 }
@@ -631,17 +645,17 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 if (c >= kRaw) ok = wait_one(&sh.raw_empty[raw], c / kRaw - 1, a.err, 908);
                 if (!ok) break;
                 const int pages = min(kPages, seen - u * kPages);
-                if (lane == 0) mbar_arrive_expect_tx(&sh.raw_full[raw], pages * kKv8Bytes);
-                __syncwarp();
+                // the scales go ahead of the barrier that the conversion, the MMAs and so the softmax wait for
                 if (lane >= at && lane < at + kPages) {
-                    if (lane < at + pages)
-                        bulk_load(sRaw + (raw * kPages + lane - at) * kKv8Bytes, a.kv8 + (static_cast<int64_t>(ids) * a.hkv + it.h) * kKv8Bytes,
-                                  kKv8Bytes, &sh.raw_full[raw]);
                     const int ve = sc >> 8;
                     sh.info[c % kInfo][lane - at] = {kv8_power(sc & 0xff), static_cast<float>(ve - 127), kv8_inverse(ve), 0.f};
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.info_full[c % kInfo]);
+                if (lane == 0) mbar_arrive_expect_tx(&sh.raw_full[raw], pages * kKv8Bytes);
+                __syncwarp();
+                if (lane >= at && lane < at + pages)
+                    bulk_load(sRaw + (raw * kPages + lane - at) * kKv8Bytes, a.kv8 + (static_cast<int64_t>(ids) * a.hkv + it.h) * kKv8Bytes,
+                              kKv8Bytes, &sh.raw_full[raw]);
             }
             ++item;
             if (last_item()) break;
