@@ -139,7 +139,7 @@ struct StepArgs {
     int* free_pages;
     int capacity;
     int* free_top;
-    int B, tokens, page;
+    int B, tokens, page, shift;  // page = 2^shift, or shift < 0
     int *seq_lens, *indptr, *positions, *slots, *last;
     int* err;
 };
@@ -306,7 +306,8 @@ step_tables_kernel(const StepArgs a) {
             if (i < total) {
                 const int r = first_above(ends, a.B, i);
                 pos = kept[r] + i - (r ? ends[r - 1] : 0);
-                slot = a.table[static_cast<int64_t>(r) * a.width + pos / a.page] * a.page + pos % a.page;
+                const int column = a.shift >= 0 ? pos >> a.shift : pos / a.page;
+                slot = a.table[static_cast<int64_t>(r) * a.width + column] * a.page + pos - column * a.page;
             }
             a.positions[i] = pos;
             a.slots[i] = slot;
@@ -376,8 +377,11 @@ int msgl_step_tables(const int* kept_lens, const int* new_lens, int* page_table,
         return set_error(MSGL_ERR_INVALID_ARG, "step_tables: null pointer");
     if (seq_lens == kept_lens || seq_lens == new_lens)
         return set_error(MSGL_ERR_INVALID_ARG, "step_tables: seq_lens must not be an input");
+    int shift = -1;
+    if ((page_size & (page_size - 1)) == 0)
+        for (shift = 0; 1 << shift < page_size;) ++shift;
     StepArgs a = {kept_lens, new_lens, page_table, max_pages, held_pages, free_pages, free_capacity, free_top,
-                  num_reqs, num_tokens, page_size, seq_lens, q_indptr, positions, slot_mapping, last_idx,
+                  num_reqs, num_tokens, page_size, shift, seq_lens, q_indptr, positions, slot_mapping, last_idx,
                   device_error_word()};
     if (!a.err) return set_error(MSGL_ERR_CUDA, "device error word unavailable");
     const int size = num_tokens > 2 * kStepThreads ? 8 : 1;

@@ -37,9 +37,39 @@ __device__ __forceinline__ unsigned long long argmax_key(float v, uint32_t i) {
 // ------------------------------------------------------------------ probabilities
 // A row is read once and written once: the cluster's threads hold it in registers (VEC consecutive
 // values at a time), each CTA takes the maximum and the sum of its own part, and one exchange through
-// distributed shared memory joins them: p = exp(x - m_cta) * (exp(m_cta - m) / sum). HBM bound.
+// distributed shared memory joins them: p = exp(x - m_cta) * (exp(m_cta - m) / sum). HBM bound; two CTAs an
+// SM, so that one's loads run while the other exchanges (320 rows of 151936: one CTA 137 us, two XX).
 template <int VEC>
-__global__ void __launch_bounds__(kProbThreads)
+__device__ __forceinline__ void greedy_row(const float* x, float* p, int begin, int end, int size, unsigned long long* red,
+                                           unsigned long long* mine) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    unsigned long long best = 0;
+    for (int i = begin + tid; i < end; i += kProbThreads) {
+        const unsigned long long key = argmax_key(x[i], i);
+        best = key > best ? key : best;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const unsigned long long y = __shfl_xor_sync(0xffffffffu, best, o);
+        best = y > best ? y : best;
+    }
+    if (lane == 0) red[tid >> 5] = best;
+    __syncthreads();
+    for (int w = 0; w < kProbThreads / 32; ++w) best = red[w] > best ? red[w] : best;
+    if (tid == 0) *mine = best;
+    cluster_sync_all();
+    for (int q = 0; q < size; ++q) {
+        const unsigned long long y = __double_as_longlong(ld_dsmem_f64(mapa_shared(smem_u32(mine), q)));
+        best = y > best ? y : best;
+    }
+    cluster_arrive();
+    const int top = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best));
+    for (int i = begin + tid; i < end; i += kProbThreads) p[i] = i == top ? 1.f : 0.f;
+    cluster_wait();  // no CTA leaves while its shared memory may be read
+}
+
+template <int VEC>
+__global__ void __launch_bounds__(kProbThreads, 2)
 token_probs_kernel(const float* logits, int64_t ldx, const float* __restrict__ temperature, float* probs,
                    int64_t ldp, int vocab, int part) {
     constexpr int kVecs = kProbValues / VEC;
@@ -53,100 +83,67 @@ token_probs_kernel(const float* logits, int64_t ldx, const float* __restrict__ t
     pdl_trigger();
     const int64_t row = cluster_id_x();
     const float* x = logits + row * ldx;
+    float* p = probs + row * ldp;
     const float T = temperature ? temperature[row] : 1.f;
     const int begin = rank * part, end = min(vocab, begin + part);  // a multiple of VEC but for the row's end
+    if (T <= 0.f) {  // the whole cluster
+        greedy_row<VEC>(x, p, begin, end, size, red_key, &mine_key);
+        return;
+    }
     float v[kProbValues];
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
         const int i = begin + (k * kProbThreads + tid) * VEC;
         if (VEC == 4) {
-            const float4 f = i < end ? *reinterpret_cast<const float4*>(x + i) : make_float4(kNegInf, kNegInf, kNegInf, kNegInf);
+            const float4 f = i < end ? __ldcs(reinterpret_cast<const float4*>(x + i)) : make_float4(kNegInf, kNegInf, kNegInf, kNegInf);
             v[4 * k] = f.x; v[4 * k + 1] = f.y; v[4 * k + 2] = f.z; v[4 * k + 3] = f.w;
         } else {
-            v[k] = i < end ? x[i] : kNegInf;
+            v[k] = i < end ? __ldcs(x + i) : kNegInf;
         }
     }
-    if (!(T <= 0.f)) {
-        const float c = fminf(1.4426950408889634f / T, 3.0e38f);
-        float m = kNegInf;
+    const float c = fminf(1.4426950408889634f / T, 3.0e38f);
+    float m = kNegInf;
 #pragma unroll
-        for (int e = 0; e < kProbValues; ++e) m = fmaxf(m, v[e]);
-        m = warp_max(m);
-        if (lane == 0) red[warp] = m;
-        __syncthreads();
-        m = kNegInf;
+    for (int e = 0; e < kProbValues; ++e) m = fmaxf(m, v[e]);
+    m = warp_max(m);
+    if (lane == 0) red[warp] = m;
+    __syncthreads();
+    m = warp_max(red[lane & (kProbThreads / 32 - 1)]);
+    // a part without a finite value adds nothing (NaN still does)
+    const float base = m == kNegInf ? 0.f : m;
+    float s4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < kProbThreads / 32; ++w) m = fmaxf(m, red[w]);
-        // a part without a finite value adds nothing (NaN still does)
-        const float base = m == kNegInf ? 0.f : m;
-        float s4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < kProbValues; ++e) {
-            v[e] = exp2f((v[e] - base) * c);
-            s4[e & 3] += v[e];
-        }
-        float s = warp_sum((s4[0] + s4[1]) + (s4[2] + s4[3]));
-        __syncthreads();
-        if (lane == 0) red[warp] = s;
-        __syncthreads();
-        s = 0.f;
-#pragma unroll
-        for (int w = 0; w < kProbThreads / 32; ++w) s += red[w];
-        if (tid == 0) {
-            mine[0] = m;
-            mine[1] = s;
-        }
-        cluster_sync_all();
-        // lane q: CTA q's maximum and sum
-        float mq = kNegInf, sq = 0.f;
-        if (lane < size) {
-            mq = ld_dsmem_f32(mapa_shared(smem_u32(&mine[0]), lane));
-            sq = ld_dsmem_f32(mapa_shared(smem_u32(&mine[1]), lane));
-        }
-        const float M = warp_max(mq);
-        const float S = warp_sum(mq == kNegInf ? sq : sq * exp2f((mq - M) * c));
-        cluster_arrive();  // this CTA's peers are read; waited for at the end
-        // a row without any finite logit: S = 0, zeros (S is NaN where a logit is NaN or +inf)
-        const float f = S == 0.f ? 0.f : (m == kNegInf ? 1.f : exp2f((m - M) * c)) / S;
-#pragma unroll
-        for (int e = 0; e < kProbValues; ++e) v[e] *= f;
-    } else {
-        unsigned long long best = 0;
-#pragma unroll
-        for (int e = 0; e < kProbValues; ++e) {
-            const int i = begin + ((e / VEC) * kProbThreads + tid) * VEC + e % VEC;
-            const unsigned long long key = argmax_key(v[e], i);
-            if (i < end && key > best) best = key;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const unsigned long long y = __shfl_xor_sync(0xffffffffu, best, o);
-            best = y > best ? y : best;
-        }
-        if (lane == 0) red_key[warp] = best;
-        __syncthreads();
-        best = 0;
-#pragma unroll
-        for (int w = 0; w < kProbThreads / 32; ++w) best = red_key[w] > best ? red_key[w] : best;
-        if (tid == 0) mine_key = best;
-        cluster_sync_all();
-        for (int q = 0; q < size; ++q) {
-            const unsigned long long y = __double_as_longlong(ld_dsmem_f64(mapa_shared(smem_u32(&mine_key), q)));
-            best = y > best ? y : best;
-        }
-        cluster_arrive();
-        const int top = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best));
-#pragma unroll
-        for (int e = 0; e < kProbValues; ++e)
-            v[e] = begin + ((e / VEC) * kProbThreads + tid) * VEC + e % VEC == top ? 1.f : 0.f;
+    for (int e = 0; e < kProbValues; ++e) {
+        v[e] = exp2f((v[e] - base) * c);
+        s4[e & 3] += v[e];
     }
-    float* p = probs + row * ldp;
+    float s = warp_sum((s4[0] + s4[1]) + (s4[2] + s4[3]));
+    __syncthreads();
+    if (lane == 0) red[warp] = s;
+    __syncthreads();
+    s = warp_sum(lane < kProbThreads / 32 ? red[lane] : 0.f);
+    if (tid == 0) {
+        mine[0] = m;
+        mine[1] = s;
+    }
+    cluster_sync_all();
+    // lane q: CTA q's maximum and sum
+    float mq = kNegInf, sq = 0.f;
+    if (lane < size) {
+        mq = ld_dsmem_f32(mapa_shared(smem_u32(&mine[0]), lane));
+        sq = ld_dsmem_f32(mapa_shared(smem_u32(&mine[1]), lane));
+    }
+    const float M = warp_max(mq);
+    const float S = warp_sum(mq == kNegInf ? sq : sq * exp2f((mq - M) * c));
+    cluster_arrive();  // this CTA's peers are read; waited for at the end
+    // a row without any logit above -inf: S = 0, zeros (S is NaN where a logit is NaN or +inf)
+    const float f = S == 0.f ? 0.f : (m == kNegInf ? 1.f : exp2f((m - M) * c)) / S;
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
         const int i = begin + (k * kProbThreads + tid) * VEC;
         if (i >= end) continue;
-        if (VEC == 4) *reinterpret_cast<float4*>(p + i) = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-        else p[i] = v[k];
+        if (VEC == 4) __stcs(reinterpret_cast<float4*>(p + i), make_float4(v[4 * k] * f, v[4 * k + 1] * f, v[4 * k + 2] * f, v[4 * k + 3] * f));
+        else __stcs(p + i, v[k] * f);
     }
     cluster_wait();  // no CTA leaves while its shared memory may be read
 }
@@ -198,8 +195,8 @@ __device__ __forceinline__ void load_values(const float* row, int i, int end, fl
 template <int VEC>
 __global__ void __launch_bounds__(kVerThreads)
 verify_drafts_kernel(const VerifyArgs a) {
-    __shared__ double warp_rest[kVerWarps], warp_all[kVerWarps];
-    __shared__ __align__(8) double mine[2];  // sums of max(p - q, 0) and of p over this CTA's range
+    __shared__ double parts[kVerWarps];
+    __shared__ __align__(8) double mine[2];  // sum of this CTA's weights, in either turn
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = cluster_ctarank(), size = cluster_nctarank();
     pdl_wait();
@@ -244,55 +241,51 @@ verify_drafts_kernel(const VerifyArgs a) {
     const int begin = min(a.vocab, rank * a.part), end = min(a.vocab, begin + a.part);
     const int share = (a.part / 128 + kVerWarps - 1) / kVerWarps * 128;
     const int w0 = min(end, begin + warp * share), w1 = min(end, w0 + share);
-    double rest = 0.0, all = 0.0;
+    // sum of the weights of [w0, w1), the warp's; FALL: of the target's row alone
+    auto weigh = [&](bool fall) {
+        double sum = 0.0;
 #pragma unroll 4
-    for (int i = w0 + lane * 4; i < w1; i += 128) {
-        float pv[4], qv[4] = {0.f, 0.f, 0.f, 0.f};
-        load_values<VEC>(prow, i, w1, pv);
-        if (qrow) load_values<VEC>(qrow, i, w1, qv);
+        for (int i = w0 + lane * 4; i < w1; i += 128) {
+            float pv[4], qv[4] = {0.f, 0.f, 0.f, 0.f};
+            load_values<VEC>(prow, i, w1, pv);
+            if (qrow && !fall) load_values<VEC>(qrow, i, w1, qv);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (i + e == point) qv[e] = 1.f;
-            rest += rest_of(pv[e], qv[e]);
-            all += rest_of(pv[e], 0.f);
-        }
-    }
-    rest = warp_sum64(rest);
-    all = warp_sum64(all);
-    if (lane == 0) {
-        warp_rest[warp] = rest;
-        warp_all[warp] = all;
-    }
-    __syncthreads();
-    if (tid == 0) {
-        double s = 0.0, t = 0.0;
-        for (int w = 0; w < kVerWarps; ++w) {
-            s += warp_rest[w];
-            t += warp_all[w];
-        }
-        mine[0] = s;
-        mine[1] = t;
-    }
-    cluster_sync_all();
-    double total[2] = {0.0, 0.0}, before[2] = {0.0, 0.0}, here[2] = {0.0, 0.0};
-    int last_part[2] = {-1, -1};  // last CTA with any weight
-    for (int c = 0; c < size; ++c)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const double s = ld_dsmem_f64(mapa_shared(smem_u32(&mine[j]), c));
-            if (c == rank) {
-                before[j] = total[j];
-                here[j] = s;
+            for (int e = 0; e < 4; ++e) {
+                if (i + e == point && !fall) qv[e] = 1.f;
+                sum += rest_of(pv[e], qv[e]);
             }
-            total[j] += s;
-            if (s > 0.0) last_part[j] = c;
         }
+        return warp_sum64(sum);
+    };
+    double total = 0.0, before = 0.0, here = 0.0;
+    int last_part = -1;  // last CTA with any weight
+    bool fall = false;
+    for (int turn = 0; turn < 2; ++turn) {  // where p <= q everywhere (rounding), once more over the target's own row
+        fall = turn == 1;
+        const double sum = weigh(fall);
+        if (lane == 0) parts[warp] = sum;
+        __syncthreads();
+        if (tid == 0) {
+            double s = 0.0;
+            for (int w = 0; w < kVerWarps; ++w) s += parts[w];
+            mine[turn] = s;
+        }
+        cluster_sync_all();
+        total = 0.0;
+        for (int c = 0; c < size; ++c) {
+            const double s = ld_dsmem_f64(mapa_shared(smem_u32(&mine[turn]), c));
+            if (c == rank) {
+                before = total;
+                here = s;
+            }
+            total += s;
+            if (s > 0.0) last_part = c;
+        }
+        if (total > 0.0 || (!qrow && point < 0)) break;
+    }
     cluster_arrive();
-    // where p <= q everywhere (rounding), the target's own row
-    const int j = total[0] > 0.0 ? 0 : 1;
-    const double* parts = j == 0 ? warp_rest : warp_all;
-    const bool fine = total[j] > 0.0 && total[j] < __longlong_as_double(0x7ff0000000000000ll);
-    double goal = static_cast<double>(a.u_last[r]) * total[j];
+    const bool fine = total > 0.0 && total < __longlong_as_double(0x7ff0000000000000ll);
+    double goal = static_cast<double>(a.u_last[r]) * total;
     if (!(goal >= 0.0)) goal = 0.0;
     if (rank == 0) {
         for (int i = tid; i <= a.max_drafts; i += kVerThreads)
@@ -304,9 +297,9 @@ verify_drafts_kernel(const VerifyArgs a) {
     }
     // The first place whose running sum passes the goal lies in this CTA (in the last one with any
     // weight where u is 1 or more).
-    const bool holds = here[j] > 0.0 && before[j] <= goal && (goal < before[j] + here[j] || rank == last_part[j]);
+    const bool holds = here > 0.0 && before <= goal && (goal < before + here || rank == last_part);
     if (fine && holds) {
-        double sum = before[j];
+        double sum = before;
         int pick = -1, last = -1;
         for (int w = 0; w < kVerWarps; ++w) {
             if (parts[w] > 0.0) last = w;
@@ -323,12 +316,12 @@ verify_drafts_kernel(const VerifyArgs a) {
                 const int i = b + lane * 4;
                 float pv[4], qv[4] = {0.f, 0.f, 0.f, 0.f};
                 load_values<VEC>(prow, i, w1, pv);
-                if (qrow && j == 0) load_values<VEC>(qrow, i, w1, qv);
+                if (qrow && !fall) load_values<VEC>(qrow, i, w1, qv);
                 double wv[4], own = 0.0;
                 int mine_last = -1;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if (i + e == point && j == 0) qv[e] = 1.f;
+                    if (i + e == point && !fall) qv[e] = 1.f;
                     wv[e] = rest_of(pv[e], qv[e]);
                     own += wv[e];
                     if (wv[e] > 0.0) mine_last = i + e;
