@@ -17,16 +17,21 @@ constexpr int kHalf = kHd / 2;
 constexpr float kNegInf = -__builtin_huge_valf();
 
 // ------------------------------------------------------------------ append
-// One warp per touched page, kv head and kind (keys, values): it brings the page's 16 x 128 values together
+// Two warps per touched page, kv head and kind (keys, values): they bring the page's 16 x 128 values together
 // in registers (earlier tokens from their codes, new ones from the projection, zeros behind the context's
-// end), takes the largest magnitude, and writes codes and exponent. So the scale is that of the values
+// end), take the largest magnitude, and write codes and exponent. So the scale is that of the values
 // which the page holds now (a rejected draft does not keep it up), and old codes are only rounded again
-// where they become subnormal: e4m3 times a power of two is e4m3. NaN and infinities
-// are stored as NaN and do not count for the scale, so they stay where they are.
-// Lane 8 c + i: dimensions [8 i, 8 i + 8) of both halves (rotate-half partners) of the tokens 2 c, 2 c + 1,
-// 8 + 2 c, 9 + 2 c: rows are 256-byte reads and the value units 16-byte writes.
+// where they become subnormal: e4m3 times a power of two is e4m3. NaN and infinities are stored as NaN
+// and do not count for the scale, so they stay where they are. HBM bound.
+// Lane 8 c + i: dimensions 8 i .. 8 i + 7 of one or both halves (keys: rotate-half partners) of the tokens 2 c, 2 c + 1
+// and / or 8 + 2 c, 9 + 2 c: rows are read in pieces of 128 bytes, value units written in 16. Keys are split over the
+// warps by tokens, values by dimensions; with one warp and 64 values a lane the kernel needed 162 registers and 8.5k
+// tokens took 79 us, so 50 (24 of them the append, 29 the query heads by themselves).
 // Query heads: eight lanes a head, as in the bf16 append.
 constexpr int kStoreWarps = 4;
+
+// Token of a page at place i of its values' order.
+__device__ __forceinline__ int token_at(int i) { return (i % 4 / 2) * 8 + (i / 4) * 2 + i % 2; }
 
 struct StoreArgs {
     const __nv_bfloat16* qkv;
@@ -46,36 +51,49 @@ struct StoreArgs {
     float eps;
     int page_tasks;    // pages a request may touch
     int kv_blocks;     // blocks of the append; the others take query heads
-    int q_blocks;      // of a token
+    int q_groups;      // of 16 query heads, of a token
     int* err;
 };
 
-// 16 values of a head row: elements 8 i + e (e < 8) and 64 + 8 i + (e - 8), bf16 or summed in part order.
-template <bool PARTS>
-__device__ __forceinline__ void load_head(const StoreArgs& a, int64_t row, int head, int i, float (&x)[16]) {
-    const int nh = a.hq + 2 * a.hkv;
-    const int64_t at = (row * nh + head) * kHd + 8 * i;
-    if (PARTS) {
+// 16 values of a head row: elements 8 i + e (e < 8) and 64 + 8 i + (e - 8), bf16 (their 32 bytes first, so that several
+// rows' loads are in flight) or summed in part order.
+__device__ __forceinline__ void load_raw(const StoreArgs& a, int64_t row, int head, int i, uint4 (&u)[2]) {
+    const __nv_bfloat16* src = a.qkv + (row * (a.hq + 2 * a.hkv) + head) * kHd + 8 * i;
+    u[0] = *reinterpret_cast<const uint4*>(src);
+    u[1] = *reinterpret_cast<const uint4*>(src + kHalf);
+}
+__device__ __forceinline__ void raw_values(const uint4 (&u)[2], float (&x)[16]) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = 0.f;
-        const int64_t stride = static_cast<int64_t>(a.num_tokens) * nh * kHd;
-        for (int p = 0; p < a.nparts; ++p) {
-            const float4* src = reinterpret_cast<const float4*>(a.parts + p * stride + at);
+    for (int v = 0; v < 2; ++v) {
+        const uint32_t w[4] = {u[v].x, u[v].y, u[v].z, u[v].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[8 * v + 2 * e] = bf16lo(w[e]);
+            x[8 * v + 2 * e + 1] = bf16hi(w[e]);
+        }
+    }
+}
+__device__ __forceinline__ void sum_parts(const StoreArgs& a, int64_t row, int head, int i, float (&x)[16]) {
+    const int nh = a.hq + 2 * a.hkv;
+    const int64_t stride = static_cast<int64_t>(a.num_tokens) * nh * kHd;
+    const float* at = a.parts + (row * nh + head) * kHd + 8 * i;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = 0.f;
+    for (int p = 0; p < a.nparts; p += 3) {  // three parts' loads in flight, added in part order
+        float4 f[3][4];
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+                f[q][v] = p + q < a.nparts ? *reinterpret_cast<const float4*>(at + (p + q) * stride + (v >> 1) * kHalf + (v & 1) * 4)
+                                           : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+            if (p + q >= a.nparts) break;
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-                const float4 f = src[(v >> 1) * (kHalf / 4) + (v & 1)];
-                x[4 * v] += f.x; x[4 * v + 1] += f.y; x[4 * v + 2] += f.z; x[4 * v + 3] += f.w;
-            }
-        }
-    } else {
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-            const uint4 u = *reinterpret_cast<const uint4*>(a.qkv + at + v * kHalf);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[8 * v + 2 * e] = bf16lo(w[e]);
-                x[8 * v + 2 * e + 1] = bf16hi(w[e]);
+                x[4 * v] += f[q][v].x; x[4 * v + 1] += f[q][v].y;
+                x[4 * v + 2] += f[q][v].z; x[4 * v + 3] += f[q][v].w;
             }
         }
     }
@@ -136,148 +154,242 @@ __device__ __forceinline__ const float* turn_row(const StoreArgs& a, int64_t row
     return a.table + static_cast<int64_t>(pos) * kHd;
 }
 
-template <bool PARTS>
-__device__ __forceinline__ void append_page(const StoreArgs& a, int task, int lane) {
-    const int kind = task & 1;  // 0 keys, 1 values
+// The page of a task: its place in the pool, and which of its tokens are held already (t < old), new, or behind the
+// context's end (pos >= L).
+struct PageTask {
+    int64_t block;  // page and head
+    int kind, h, page, old, begin, L, q0, n;
+
+    __device__ __forceinline__ bool live(int t) const { return t >= old && page * kPage + t < L; }
+    // row of a new token; of the others the request's last one, so that all lanes work on something
+    __device__ __forceinline__ int64_t row(int t) const { return q0 + (live(t) ? page * kPage + t - begin : n - 1); }
+};
+
+__device__ __forceinline__ bool find_page(const StoreArgs& a, int task, bool report, PageTask& p) {
+    p.kind = task & 1;  // 0 keys, 1 values
     task >>= 1;
-    const int h = task % a.hkv;
+    p.h = task % a.hkv;
     task /= a.hkv;
     const int r = task / a.page_tasks, nth = task % a.page_tasks;
-    int L = a.seq_lens[r];
-    const int q0 = a.q_indptr ? a.q_indptr[r] : r;
-    const int n = a.q_indptr ? a.q_indptr[r + 1] - q0 : 1;
-    const bool first = lane == 0 && nth == 0 && h == 0 && kind == 0;
-    if (L < 0 || L > a.max_pages * static_cast<int64_t>(kPage) || n < 0 || n > L) {
-        if (first && n != 0) record_error(a.err, MSGL_ERR_BOUNDS, 910);
-        return;
+    p.L = a.seq_lens[r];
+    p.q0 = a.q_indptr ? a.q_indptr[r] : r;
+    p.n = a.q_indptr ? a.q_indptr[r + 1] - p.q0 : 1;
+    const bool first = report && nth == 0 && p.h == 0 && p.kind == 0;
+    if (p.L < 0 || p.L > a.max_pages * static_cast<int64_t>(kPage) || p.n < 0 || p.n > p.L) {
+        if (first && p.n != 0) record_error(a.err, MSGL_ERR_BOUNDS, 910);
+        return false;
     }
-    if (n == 0) return;
-    if (n > a.max_q_len || q0 < 0 || q0 > a.num_tokens - n) {
+    if (p.n == 0) return false;
+    if (p.n > a.max_q_len || p.q0 < 0 || p.q0 > a.num_tokens - p.n) {
         if (first) record_error(a.err, MSGL_ERR_BOUNDS, 911);
-        return;
+        return false;
     }
-    const int begin = L - n;  // tokens before it are held already
-    const int page = begin / kPage + nth;
-    if (page * kPage >= L) return;
-    const int phys = a.page_table[static_cast<int64_t>(r) * a.max_pages + page];
+    p.begin = p.L - p.n;
+    p.page = p.begin / kPage + nth;
+    if (p.page * kPage >= p.L) return false;
+    const int phys = a.page_table[static_cast<int64_t>(r) * a.max_pages + p.page];
     if (phys < 0 || phys >= a.num_pages) {
-        if (lane == 0) record_error(a.err, MSGL_ERR_BOUNDS, 913);
-        return;
+        if (report) record_error(a.err, MSGL_ERR_BOUNDS, 913);
+        return false;
     }
-    const int64_t block = static_cast<int64_t>(phys) * a.hkv + h;
-    uint8_t* codes = a.kv8 + block * kKv8Bytes + kind * kKv8Values;
-    const int c = lane >> 3, i = lane & 7;
-    float x[4][16];
-    const int old = begin - page * kPage;  // tokens of the page that are held already, if positive
-    if (old > 0) {
-        const float s = kv8_power(a.scales[2 * block + kind]);
-        if (kind == 0) {
+    p.block = static_cast<int64_t>(phys) * a.hkv + p.h;
+    p.old = p.begin - p.page * kPage;
+    return true;
+}
+
+// The exponent of the page's values, of which the two warps of a pair hold 32 a lane each; NaN and infinities become
+// NaN and do not count.
+__device__ __forceinline__ int page_exponent(float (&x)[32], float* maxima, int warp, int lane) {
+    float amax = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < 32; ++e) {
+        if (fabsf(x[e]) < __builtin_huge_valf()) amax = fmaxf(amax, fabsf(x[e]));
+        else x[e] = __int_as_float(0x7fffffff);
+    }
+    amax = warp_max(amax);
+    if (lane == 0) maxima[warp] = amax;
+    __syncwarp();
+    asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp >> 1)) : "memory");
+    return kv8_exponent(fmaxf(maxima[warp & ~1], maxima[warp | 1]));
+}
+
+// Keys: this warp's tokens are t0 + 2 c and t0 + 2 c + 1, t0 = 0 or 8.
+template <bool PARTS>
+__device__ __forceinline__ void append_keys(const StoreArgs& a, const PageTask& p, float* maxima, int warp, int lane) {
+    uint8_t* codes = a.kv8 + p.block * kKv8Bytes;
+    const int c = lane >> 3, i = lane & 7, t0 = (warp & 1) * 8 + 2 * c;
+    float x[32];  // token t0 + e: [16 e, 16 e + 16)
+    uint4 raw[2][2];
+    bool some[2];  // some lane's token is a new one
 #pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    const uint2 u = *reinterpret_cast<const uint2*>(codes + v * 1024 + ((e >> 1) * 8 + 2 * c + (e & 1)) * 64 + 8 * i);
-                    const uint32_t w[2] = {u.x, u.y};
+    for (int e = 0; e < 2; ++e) {
+        some[e] = __any_sync(0xffffffffu, p.live(t0 + e));
+        if (some[e] && !PARTS) load_raw(a, p.row(t0 + e), a.hq + p.h, i, raw[e]);
+    }
+    if (p.old > 0) {
+        const float s = kv8_power(a.scales[2 * p.block]);
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        const float2 f = __half22float2(__nv_cvt_fp8x2_to_halfraw2(w[b >> 1] >> ((b & 1) * 16) & 0xffff, __NV_E4M3));
-                        x[e][8 * v + 2 * b] = f.x * s;
-                        x[e][8 * v + 2 * b + 1] = f.y * s;
-                    }
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                const uint2 u = *reinterpret_cast<const uint2*>(codes + v * 1024 + (t0 + e) * 64 + 8 * i);
+                const uint32_t w[2] = {u.x, u.y};
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const float2 f = __half22float2(__nv_cvt_fp8x2_to_halfraw2(w[b >> 1] >> ((b & 1) * 16) & 0xffff, __NV_E4M3));
+                    x[16 * e + 8 * v + 2 * b] = f.x * s;
+                    x[16 * e + 8 * v + 2 * b + 1] = f.y * s;
                 }
-        } else {
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {  // dimensions 64 (v / 2) + 8 i + 4 (v % 2) + j
-                const uint4 u = *reinterpret_cast<const uint4*>(codes + ((v >> 1) * 16 + 2 * i + (v & 1)) * 64 + c * 16);
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const float2 f = __half22float2(__nv_cvt_fp8x2_to_halfraw2(w[j] >> (b * 16) & 0xffff, __NV_E4M3));
-                        x[2 * b][4 * v + j] = f.x * s;
-                        x[2 * b + 1][4 * v + j] = f.y * s;
-                    }
             }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int t = t0 + e;
+        if (some[e]) {
+            float y[16];
+            const int64_t row = p.row(t);
+            if (PARTS) sum_parts(a, row, a.hq + p.h, i, y);
+            else raw_values(raw[e], y);
+            norm_turn(y, a.kn, turn_row(a, row), i, a.eps);
+#pragma unroll
+            for (int d = 0; d < 16; ++d) x[16 * e + d] = p.live(t) ? y[d] : t < p.old ? x[16 * e + d] : 0.f;
+        } else if (t >= p.old) {
+#pragma unroll
+            for (int d = 0; d < 16; ++d) x[16 * e + d] = 0.f;
         }
+    }
+    const int stored = page_exponent(x, maxima, warp, lane);
+    const float inv = kv8_inverse(stored);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+            uint32_t w[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) w[b] = e4m3_codes2(x[16 * e + 8 * v + 2 * b] * inv, x[16 * e + 8 * v + 2 * b + 1] * inv);
+            *reinterpret_cast<uint2*>(codes + v * 1024 + (t0 + e) * 64 + 8 * i) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+        }
+    if ((warp & 1) == 0 && lane == 0) a.scales[2 * p.block] = static_cast<uint8_t>(stored);
+}
+
+// Values: this warp's dimensions are half + 8 i .. + 7, half = 0 or 64; of the tokens 2 c, 2 c + 1, 8 + 2 c, 9 + 2 c.
+template <bool PARTS>
+__device__ __forceinline__ void append_values(const StoreArgs& a, const PageTask& p, float* maxima, int warp, int lane) {
+    const int c = lane >> 3, i = lane & 7, half = (warp & 1) * kHalf;
+    uint8_t* codes = a.kv8 + p.block * kKv8Bytes + kKv8Values + (half / 4 + 2 * i) * 64 + c * 16;  // a unit, and one 64 further
+    const int head = a.hq + a.hkv + p.h, nh = a.hq + 2 * a.hkv;
+    float x[32];  // token e, dimension d: 8 e + d
+    uint4 raw[4], held[2];
+    bool some[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int t = token_at(4 * c + e);
+        some[e] = __any_sync(0xffffffffu, p.live(t));
+        if (some[e] && !PARTS) raw[e] = *reinterpret_cast<const uint4*>(a.qkv + (p.row(t) * nh + head) * kHd + half + 8 * i);
+    }
+    float s = 0.f;
+    if (p.old > 0) {
+        s = kv8_power(a.scales[2 * p.block + 1]);
+#pragma unroll
+        for (int v = 0; v < 2; ++v) held[v] = *reinterpret_cast<const uint4*>(codes + v * 64);
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const int t = (e >> 1) * 8 + 2 * c + (e & 1);
-        const bool live = t >= old && page * kPage + t < L;
-        const int64_t row = q0 + (live ? page * kPage + t - begin : n - 1);
-        if (__any_sync(0xffffffffu, live)) {  // lanes of other tokens work on the request's last row
-            float y[16];
-            load_head<PARTS>(a, row, a.hq + kind * a.hkv + h, i, y);
-            if (kind == 0) norm_turn(y, a.kn, turn_row(a, row), i, a.eps);
+        const int t = token_at(4 * c + e);
+        float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (some[e]) {
+            if (PARTS) {
+                const int64_t stride = static_cast<int64_t>(a.num_tokens) * nh * kHd;
+                const float* at = a.parts + (p.row(t) * nh + head) * kHd + half + 8 * i;
+#pragma unroll 3
+                for (int q = 0; q < a.nparts; ++q)
 #pragma unroll
-            for (int d = 0; d < 16; ++d) x[e][d] = live ? y[d] : t < old ? x[e][d] : 0.f;
-        } else if (t >= old) {
+                    for (int v = 0; v < 2; ++v) {
+                        const float4 f = *reinterpret_cast<const float4*>(at + q * stride + 4 * v);
+                        y[4 * v] += f.x; y[4 * v + 1] += f.y; y[4 * v + 2] += f.z; y[4 * v + 3] += f.w;
+                    }
+            } else {
+                const uint32_t w[4] = {raw[e].x, raw[e].y, raw[e].z, raw[e].w};
 #pragma unroll
-            for (int d = 0; d < 16; ++d) x[e][d] = 0.f;
-        }
-    }
-    float amax = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int d = 0; d < 16; ++d) {
-            if (fabsf(x[e][d]) < __builtin_huge_valf()) amax = fmaxf(amax, fabsf(x[e][d]));
-            else x[e][d] = __int_as_float(0x7fffffff);
-        }
-    amax = warp_max(amax);
-    const int stored = kv8_exponent(amax);
-    const float inv = kv8_inverse(stored);
-    if (kind == 0) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
-                uint32_t w[4];
-#pragma unroll
-                for (int b = 0; b < 4; ++b) w[b] = e4m3_codes2(x[e][8 * v + 2 * b] * inv, x[e][8 * v + 2 * b + 1] * inv);
-                *reinterpret_cast<uint2*>(codes + v * 1024 + ((e >> 1) * 8 + 2 * c + (e & 1)) * 64 + 8 * i) =
-                    make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+                for (int d = 0; d < 4; ++d) {
+                    y[2 * d] = bf16lo(w[d]);
+                    y[2 * d + 1] = bf16hi(w[d]);
+                }
             }
-    } else {
+        }
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            uint32_t w[4];
+        for (int d = 0; d < 8; ++d) x[8 * e + d] = p.live(t) ? y[d] : 0.f;
+        if (p.old > 0 && t < p.old) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                w[j] = e4m3_codes2(x[0][4 * v + j] * inv, x[1][4 * v + j] * inv) |
-                       e4m3_codes2(x[2][4 * v + j] * inv, x[3][4 * v + j] * inv) << 16;
-            *reinterpret_cast<uint4*>(codes + ((v >> 1) * 16 + 2 * i + (v & 1)) * 64 + c * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int d = 0; d < 8; ++d) {  // unit d / 4, its dimension d % 4: word d % 4, byte e
+                const uint4& u = held[d >> 2];
+                const uint32_t w = (d & 3) == 0 ? u.x : (d & 3) == 1 ? u.y : (d & 3) == 2 ? u.z : u.w;
+                x[8 * e + d] = __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<uint8_t>(w >> (8 * e)), __NV_E4M3))) * s;
+            }
         }
     }
-    if (lane == 0) a.scales[2 * block + kind] = static_cast<uint8_t>(stored);
+    const int stored = page_exponent(x, maxima, warp, lane);
+    const float inv = kv8_inverse(stored);
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+        uint32_t w[4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+            w[d] = e4m3_codes2(x[4 * v + d] * inv, x[8 + 4 * v + d] * inv) |
+                   e4m3_codes2(x[16 + 4 * v + d] * inv, x[24 + 4 * v + d] * inv) << 16;
+        *reinterpret_cast<uint4*>(codes + v * 64) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if ((warp & 1) == 0 && lane == 0) a.scales[2 * p.block + 1] = static_cast<uint8_t>(stored);
 }
 
-template <bool PARTS>
-__global__ void __launch_bounds__(kStoreWarps * 32)
+template <bool PARTS, int IT>
+__global__ void __launch_bounds__(kStoreWarps * 32, PARTS ? 4 : 8)
 qknorm_rope_store_kv8_kernel(const StoreArgs a) {
     pdl_wait();
     pdl_trigger();
+    __shared__ float maxima[kStoreWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (static_cast<int>(blockIdx.x) < a.kv_blocks) {
-        const int task = blockIdx.x * kStoreWarps + warp;
-        if (task < a.num_reqs * a.page_tasks * a.hkv * 2) append_page<PARTS>(a, task, lane);
+        const int task = blockIdx.x * (kStoreWarps / 2) + (warp >> 1);
+        PageTask p;
+        if (task >= a.num_reqs * a.page_tasks * a.hkv * 2 || !find_page(a, task, lane == 0 && (warp & 1) == 0, p)) return;
+        if (p.kind == 0) append_keys<PARTS>(a, p, maxima, warp, lane);
+        else append_values<PARTS>(a, p, maxima, warp, lane);
         return;
     }
-    const int b = blockIdx.x - a.kv_blocks;
-    const int64_t t = b / a.q_blocks;
-    if (a.q_indptr && (t < a.q_indptr[0] || t >= a.q_indptr[a.num_reqs])) return;  // no request's row
-    const int h = ((b % a.q_blocks) * kStoreWarps + warp) * 4 + (lane >> 3), i = lane & 7;
-    const bool live = h < a.hq;
-    float x[16];
-    load_head<PARTS>(a, t, live ? h : 0, i, x);
-    norm_turn(x, a.qn, turn_row(a, t), i, a.eps);
-    if (!live) return;
+    // query heads: a warp takes four of 16 heads of a token, IT such groups in a row with their loads in flight together
+    const int i = lane & 7;
+    const int64_t first = a.q_indptr ? a.q_indptr[0] : 0, last = a.q_indptr ? a.q_indptr[a.num_reqs] : a.num_tokens;
+    const int64_t g0 = static_cast<int64_t>(blockIdx.x - a.kv_blocks) * IT;
+    uint4 raw[PARTS ? 1 : IT][2];
+    const float* turn[IT];
+    int64_t token[IT];
+    int head[IT];
 #pragma unroll
-    for (int v = 0; v < 2; ++v)
-        *reinterpret_cast<uint4*>(a.q_out + (t * a.hq + h) * kHd + v * kHalf + 8 * i) =
-            make_uint4(pack_bf16x2(x[8 * v], x[8 * v + 1]), pack_bf16x2(x[8 * v + 2], x[8 * v + 3]),
-                       pack_bf16x2(x[8 * v + 4], x[8 * v + 5]), pack_bf16x2(x[8 * v + 6], x[8 * v + 7]));
+    for (int k = 0; k < IT; ++k) {
+        token[k] = (g0 + k) / a.q_groups;
+        head[k] = static_cast<int>((g0 + k) % a.q_groups) * 16 + warp * 4 + (lane >> 3);
+        if (token[k] < first || token[k] >= last || token[k] >= a.num_tokens) token[k] = -1;  // no request's row
+        if (token[k] < 0) continue;
+        if (!PARTS) load_raw(a, token[k], min(head[k], a.hq - 1), i, raw[PARTS ? 0 : k]);
+        turn[k] = turn_row(a, token[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < IT; ++k) {
+        if (token[k] < 0) continue;
+        float x[16];
+        if (PARTS) sum_parts(a, token[k], min(head[k], a.hq - 1), i, x);
+        else raw_values(raw[PARTS ? 0 : k], x);
+        norm_turn(x, a.qn, turn[k], i, a.eps);
+        if (head[k] < a.hq) {
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+                *reinterpret_cast<uint4*>(a.q_out + (token[k] * a.hq + head[k]) * kHd + v * kHalf + 8 * i) =
+                    make_uint4(pack_bf16x2(x[8 * v], x[8 * v + 1]), pack_bf16x2(x[8 * v + 2], x[8 * v + 3]),
+                               pack_bf16x2(x[8 * v + 4], x[8 * v + 5]), pack_bf16x2(x[8 * v + 6], x[8 * v + 7]));
+        }
+        __syncwarp();
+    }
 }
 
 int launch_store(StoreArgs a, int head_dim, int page_size, msgl_stream_t stream) {
@@ -297,16 +409,19 @@ int launch_store(StoreArgs a, int head_dim, int page_size, msgl_stream_t stream)
         return set_error(MSGL_ERR_INVALID_ARG, "store_kv8: rows must be 16-byte aligned");
     const int64_t rows = std::min(a.max_q_len, a.num_tokens);
     a.page_tasks = static_cast<int>((rows + kPage - 2) / kPage + 1);
-    a.q_blocks = (a.hq + 4 * kStoreWarps - 1) / (4 * kStoreWarps);
+    // Many tokens: four groups of query heads a warp, so that a block's loads cover its latency; few: one, for more blocks.
+    const int it = !a.parts && a.num_tokens >= 8 * 148 ? 4 : 1;
+    a.q_groups = (a.hq + 15) / 16;
     const int64_t tasks = static_cast<int64_t>(a.num_reqs) * a.page_tasks * a.hkv * 2;
-    const int64_t kv = (tasks + kStoreWarps - 1) / kStoreWarps;
-    const int64_t grid = kv + static_cast<int64_t>(a.num_tokens) * a.q_blocks;
+    const int64_t kv = (tasks + kStoreWarps / 2 - 1) / (kStoreWarps / 2);
+    const int64_t grid = kv + (static_cast<int64_t>(a.num_tokens) * a.q_groups + it - 1) / it;
     if (tasks > INT32_MAX / 2 || grid > INT32_MAX)
         return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "store_kv8: too many rows, requests or heads");
     a.kv_blocks = static_cast<int>(kv);
     a.err = device_error_word();
     if (!a.err) return set_error(MSGL_ERR_CUDA, "device error word unavailable");
-    launch_pdl(a.parts ? qknorm_rope_store_kv8_kernel<true> : qknorm_rope_store_kv8_kernel<false>,
+    launch_pdl(a.parts ? qknorm_rope_store_kv8_kernel<true, 1>
+                       : it == 4 ? qknorm_rope_store_kv8_kernel<false, 4> : qknorm_rope_store_kv8_kernel<false, 1>,
                dim3(static_cast<unsigned>(grid)), dim3(kStoreWarps * 32), 0, stream, a);
     MSGL_LAUNCH_CHECK();
     return MSGL_OK;

@@ -17,7 +17,7 @@ namespace msgl {
 namespace {
 
 constexpr int kProbThreads = 512;
-constexpr int kProbValues = 40;  // of a row, per thread, in registers
+constexpr int kProbPart = 20480;  // values of a row that a CTA holds, at most (80 KB, and as much for the next row)
 constexpr int kMaxCluster = 16;
 constexpr float kNegInf = -__builtin_huge_valf();
 
@@ -35,115 +35,141 @@ __device__ __forceinline__ unsigned long long argmax_key(float v, uint32_t i) {
 }
 
 // ------------------------------------------------------------------ probabilities
-// A row is read once and written once: the cluster's threads hold it in registers (VEC consecutive
-// values at a time), each CTA takes the maximum and the sum of its own part, and one exchange through
-// distributed shared memory joins them: p = exp(x - m_cta) * (exp(m_cta - m) / sum). HBM bound; two CTAs an
-// SM, so that one's loads run while the other exchanges (320 rows of 151936: one CTA 137 us, two XX).
+// A row is read once and written once: a cluster's CTAs hold it in shared memory, each takes the maximum and the sum
+// of its own part, and one exchange through distributed shared memory joins them:
+// p = exp(x - m_thread) * (exp(m_thread - m) / sum). HBM bound; up to three CTAs an SM, so that one's loads run while
+// the others reduce, exchange and store. 320 rows of 151936: 88 us, 4.4 TB/s. The parts in registers: 97 us with two
+// CTAs an SM, 137 with one; clusters that walk the rows with the next row's loads in flight (one CTA an SM, and 15
+// clusters of 8 are all that the GPU holds then) 122; clusters of 16: 165.
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 template <int VEC>
-__device__ __forceinline__ void greedy_row(const float* x, float* p, int begin, int end, int size, unsigned long long* red,
-                                           unsigned long long* mine) {
-    const int tid = threadIdx.x, lane = tid & 31;
-    unsigned long long best = 0;
-    for (int i = begin + tid; i < end; i += kProbThreads) {
-        const unsigned long long key = argmax_key(x[i], i);
-        best = key > best ? key : best;
+__device__ __forceinline__ void copy_async(float* dst, const float* src) {
+    if (VEC == 4) cp_async16(smem_u32(dst), src, true);
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+template <int VEC>
+__device__ __forceinline__ void read_part(const float* src, float (&v)[VEC]) {
+    if (VEC == 4) {
+        const float4 f = *reinterpret_cast<const float4*>(src);
+        v[0] = f.x; v[1 % VEC] = f.y; v[2 % VEC] = f.z; v[3 % VEC] = f.w;
+    } else {
+        v[0] = *src;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const unsigned long long y = __shfl_xor_sync(0xffffffffu, best, o);
-        best = y > best ? y : best;
-    }
-    if (lane == 0) red[tid >> 5] = best;
-    __syncthreads();
-    for (int w = 0; w < kProbThreads / 32; ++w) best = red[w] > best ? red[w] : best;
-    if (tid == 0) *mine = best;
-    cluster_sync_all();
-    for (int q = 0; q < size; ++q) {
-        const unsigned long long y = __double_as_longlong(ld_dsmem_f64(mapa_shared(smem_u32(mine), q)));
-        best = y > best ? y : best;
-    }
-    cluster_arrive();
-    const int top = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best));
-    for (int i = begin + tid; i < end; i += kProbThreads) p[i] = i == top ? 1.f : 0.f;
-    cluster_wait();  // no CTA leaves while its shared memory may be read
+}
+// Maximum m and sum s = sum exp2((x - m) c) of a warp's 32 such pairs, in every lane.
+__device__ __forceinline__ void join_pairs(float& m, float& s, float c) {
+    const float all = warp_max(m);
+    s = warp_sum(m == kNegInf ? s : s * exp2_approx((m - all) * c));
+    m = all;
 }
 
 template <int VEC>
-__global__ void __launch_bounds__(kProbThreads, 2)
+__device__ __forceinline__ void write_part(float* dst, const float (&v)[VEC]) {
+    if (VEC == 4) *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1 % VEC], v[2 % VEC], v[3 % VEC]);
+    else *dst = v[0];
+}
+
+template <int VEC>
+__global__ void __launch_bounds__(kProbThreads, 3)
 token_probs_kernel(const float* logits, int64_t ldx, const float* __restrict__ temperature, float* probs,
                    int64_t ldp, int vocab, int part) {
-    constexpr int kVecs = kProbValues / VEC;
-    __shared__ float red[kProbThreads / 32];
-    __shared__ unsigned long long red_key[kProbThreads / 32];
-    __shared__ __align__(8) float mine[2];  // the CTA's maximum and sum, read by the cluster
-    __shared__ unsigned long long mine_key;
+    extern __shared__ __align__(16) float here[];
+    __shared__ float2 red[kProbThreads / 32];
+    __shared__ float2 mine;  // the CTA's maximum and sum, read by the cluster
+    __shared__ unsigned long long red_key[kProbThreads / 32], mine_key;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = cluster_ctarank(), size = cluster_nctarank();
+    const int begin = rank * part, count = min(vocab, begin + part) - begin;  // a multiple of VEC but for the row's end
     pdl_wait();
     pdl_trigger();
     const int64_t row = cluster_id_x();
-    const float* x = logits + row * ldx;
-    float* p = probs + row * ldp;
+    const float* x = logits + row * ldx + begin;
+    float* p = probs + row * ldp + begin;
+    // all loads in flight together; a thread works on what it loaded
+    for (int i = tid * VEC; i < count; i += kProbThreads * VEC) copy_async<VEC>(here + i, x + i);
+    cp_async_commit();
     const float T = temperature ? temperature[row] : 1.f;
-    const int begin = rank * part, end = min(vocab, begin + part);  // a multiple of VEC but for the row's end
+    cp_async_wait<0>();
     if (T <= 0.f) {  // the whole cluster
-        greedy_row<VEC>(x, p, begin, end, size, red_key, &mine_key);
+        unsigned long long best = 0;
+        for (int k = tid * VEC; k < count; k += kProbThreads * VEC)
+            for (int i = k; i < k + VEC; ++i) {
+                const unsigned long long key = argmax_key(here[i], begin + i);
+                best = key > best ? key : best;
+            }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const unsigned long long y = __shfl_xor_sync(0xffffffffu, best, o);
+            best = y > best ? y : best;
+        }
+        if (lane == 0) red_key[warp] = best;
+        __syncthreads();
+        for (int w = 0; w < kProbThreads / 32; ++w) best = red_key[w] > best ? red_key[w] : best;
+        if (tid == 0) mine_key = best;
+        cluster_sync_all();
+        for (int q = 0; q < size; ++q) {
+            const unsigned long long y = __double_as_longlong(ld_dsmem_f64(mapa_shared(smem_u32(&mine_key), q)));
+            best = y > best ? y : best;
+        }
+        cluster_arrive();
+        const int top = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best)) - begin;
+        for (int k = tid * VEC; k < count; k += kProbThreads * VEC)
+            for (int i = k; i < k + VEC; ++i) p[i] = i == top ? 1.f : 0.f;
+        cluster_wait();  // no CTA leaves while its shared memory may be read
         return;
     }
-    float v[kProbValues];
-#pragma unroll
-    for (int k = 0; k < kVecs; ++k) {
-        const int i = begin + (k * kProbThreads + tid) * VEC;
-        if (VEC == 4) {
-            const float4 f = i < end ? __ldcs(reinterpret_cast<const float4*>(x + i)) : make_float4(kNegInf, kNegInf, kNegInf, kNegInf);
-            v[4 * k] = f.x; v[4 * k + 1] = f.y; v[4 * k + 2] = f.z; v[4 * k + 3] = f.w;
-        } else {
-            v[k] = i < end ? __ldcs(x + i) : kNegInf;
-        }
-    }
     const float c = fminf(1.4426950408889634f / T, 3.0e38f);
-    float m = kNegInf;
+    // Each thread against its own maximum: one reduction of (maximum, sum) pairs, and exponentials ahead of it.
+    float own = kNegInf;
+#pragma unroll 4
+    for (int i = tid * VEC; i < count; i += kProbThreads * VEC) {
+        float v[VEC];
+        read_part<VEC>(here + i, v);
 #pragma unroll
-    for (int e = 0; e < kProbValues; ++e) m = fmaxf(m, v[e]);
-    m = warp_max(m);
-    if (lane == 0) red[warp] = m;
-    __syncthreads();
-    m = warp_max(red[lane & (kProbThreads / 32 - 1)]);
-    // a part without a finite value adds nothing (NaN still does)
-    const float base = m == kNegInf ? 0.f : m;
-    float s4[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int e = 0; e < VEC; ++e) own = fmaxf(own, v[e]);
+    }
+    const float base = own == kNegInf ? 0.f : own;  // values without a finite one add nothing (NaN still does)
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll 4
+    for (int i = tid * VEC; i < count; i += kProbThreads * VEC) {
+        float v[VEC];
+        read_part<VEC>(here + i, v);
 #pragma unroll
-    for (int e = 0; e < kProbValues; ++e) {
-        v[e] = exp2f((v[e] - base) * c);
-        s4[e & 3] += v[e];
+        for (int e = 0; e < VEC; ++e) {
+            v[e] = exp2_approx((v[e] - base) * c);
+            (e & 1 ? s1 : s0) += v[e];
+        }
+        write_part<VEC>(here + i, v);
     }
-    float s = warp_sum((s4[0] + s4[1]) + (s4[2] + s4[3]));
+    float m = own, s = s0 + s1;
+    join_pairs(m, s, c);
+    if (lane == 0) red[warp] = make_float2(m, s);
     __syncthreads();
-    if (lane == 0) red[warp] = s;
-    __syncthreads();
-    s = warp_sum(lane < kProbThreads / 32 ? red[lane] : 0.f);
-    if (tid == 0) {
-        mine[0] = m;
-        mine[1] = s;
-    }
+    m = lane < kProbThreads / 32 ? red[lane].x : kNegInf;
+    s = lane < kProbThreads / 32 ? red[lane].y : 0.f;
+    join_pairs(m, s, c);
+    if (tid == 0) mine = make_float2(m, s);
     cluster_sync_all();
-    // lane q: CTA q's maximum and sum
-    float mq = kNegInf, sq = 0.f;
+    m = kNegInf;  // lane q: CTA q's maximum and sum
+    s = 0.f;
     if (lane < size) {
-        mq = ld_dsmem_f32(mapa_shared(smem_u32(&mine[0]), lane));
-        sq = ld_dsmem_f32(mapa_shared(smem_u32(&mine[1]), lane));
+        m = ld_dsmem_f32(mapa_shared(smem_u32(&mine.x), lane));
+        s = ld_dsmem_f32(mapa_shared(smem_u32(&mine.y), lane));
     }
-    const float M = warp_max(mq);
-    const float S = warp_sum(mq == kNegInf ? sq : sq * exp2f((mq - M) * c));
     cluster_arrive();  // this CTA's peers are read; waited for at the end
+    join_pairs(m, s, c);
     // a row without any logit above -inf: S = 0, zeros (S is NaN where a logit is NaN or +inf)
-    const float f = S == 0.f ? 0.f : (m == kNegInf ? 1.f : exp2f((m - M) * c)) / S;
-#pragma unroll
-    for (int k = 0; k < kVecs; ++k) {
-        const int i = begin + (k * kProbThreads + tid) * VEC;
-        if (i >= end) continue;
-        if (VEC == 4) __stcs(reinterpret_cast<float4*>(p + i), make_float4(v[4 * k] * f, v[4 * k + 1] * f, v[4 * k + 2] * f, v[4 * k + 3] * f));
-        else __stcs(p + i, v[k] * f);
+    const float f = s == 0.f ? 0.f : (own == kNegInf ? 1.f : exp2_approx((own - m) * c)) / s;
+#pragma unroll 4
+    for (int i = tid * VEC; i < count; i += kProbThreads * VEC) {
+        float v[VEC];
+        read_part<VEC>(here + i, v);
+        if (VEC == 4) __stcs(reinterpret_cast<float4*>(p + i), make_float4(v[0] * f, v[1 % VEC] * f, v[2 % VEC] * f, v[3 % VEC] * f));
+        else __stcs(p + i, v[0] * f);
     }
     cluster_wait();  // no CTA leaves while its shared memory may be read
 }
@@ -385,7 +411,7 @@ int msgl_token_probs(const float* logits, int64_t ldx, int num_rows, int vocab, 
                      float* probs, int64_t ldp, msgl_stream_t stream) {
     if (num_rows < 0 || vocab <= 0 || ldx < vocab || ldp < vocab)
         return set_error(MSGL_ERR_INVALID_ARG, "token_probs: bad sizes");
-    constexpr int kPer = kProbThreads * kProbValues;
+    constexpr int kPer = kProbPart;
     if (vocab > kPer * kMaxCluster)
         return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "token_probs: vocab above 327680");
     if (num_rows > INT32_MAX / kMaxCluster) return set_error(MSGL_ERR_UNSUPPORTED_SHAPE, "token_probs: too many rows");
@@ -395,13 +421,13 @@ int msgl_token_probs(const float* logits, int64_t ldx, int num_rows, int vocab, 
     const bool vec = vocab % 4 == 0 && ldx % 4 == 0 && ldp % 4 == 0 && aligned16(logits) && aligned16(probs);
     const int size = cluster_size(num_rows, (vocab + kPer - 1) / kPer);
     const int part = ((vocab + size - 1) / size + 3) / 4 * 4;
-    static std::atomic<int> large4[kMaxDevices], large1[kMaxDevices];
-    const cudaError_t e = size <= 8 ? cudaSuccess
-                          : vec ? allow_large_clusters(token_probs_kernel<4>, large4)
-                                : allow_large_clusters(token_probs_kernel<1>, large1);
+    const auto kernel = vec ? token_probs_kernel<4> : token_probs_kernel<1>;
+    static std::atomic<int> large[2][kMaxDevices], room[2][kMaxDevices];
+    cudaError_t e = smem_optin(kernel, kPer * sizeof(float), room[vec]);
+    if (e == cudaSuccess && size > 8) e = allow_large_clusters(kernel, large[vec]);
     if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
-    launch_cluster(vec ? token_probs_kernel<4> : token_probs_kernel<1>, static_cast<int64_t>(num_rows) * size,
-                   kProbThreads, size, 0, stream, logits, ldx, temperature, probs, ldp, vocab, part);
+    launch_cluster(kernel, static_cast<int64_t>(num_rows) * size, kProbThreads, size, part * sizeof(float), stream, logits, ldx,
+                   temperature, probs, ldp, vocab, part);
     MSGL_LAUNCH_CHECK();
     return MSGL_OK;
 }
