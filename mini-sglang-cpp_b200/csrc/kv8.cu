@@ -437,10 +437,11 @@ int launch_store(StoreArgs a, int head_dim, int page_size, msgl_stream_t stream)
 // so that O needs no scaling by page, and l adds p 2^-(exponent of v). HBM bound: 4 KB a page and head,
 // 24 or 32 MMAs, 64 conversions.
 //
-// In a CTA the pages of an item go around the warps, each with a ring of 4 KB stages that one lane fills by
-// bulk copies across items. Where an item is shared by CTAs they leave partial sums in the workspace.
-constexpr int kWarps = 8;
-constexpr int kAttThreads = kWarps * 32;
+// In a CTA the pages of an item go around the warps, each with a ring of 4 KB stages that a warp of its own
+// fills by bulk copies, across items. Where an item is shared by CTAs they leave partial sums in the workspace.
+constexpr int kWarps = 7;                        // that attend (eight warps in all: 128 registers a thread at two CTAs an SM)
+constexpr int kBatch = 32 / kWarps * kWarps;     // pages whose ids are read together
+constexpr int kAttThreads = kWarps * 32;        // that attend; one warp more copies
 constexpr int kPitch = kHd + 4;  // floats of a row in the joining buffer
 
 template <int NT>
@@ -666,19 +667,29 @@ __device__ __forceinline__ void load_rows(const Kv8AttnArgs& a, const Kv8Item& i
             for (int e = 0; e < 4; ++e) st.o[v][t][e] = 0.f;
 }
 
+// The attending warps.
+__device__ __forceinline__ void attending_barrier() {
+    __syncwarp();
+    asm volatile("bar.sync 1, %0;" ::"n"(kAttThreads) : "memory");
+}
+
 template <int NT>
-__global__ void __launch_bounds__(kAttThreads, RowsShape<NT>::kCtas)
+__global__ void __launch_bounds__(kAttThreads + 32, RowsShape<NT>::kCtas)
 attend_rows_kernel(const Kv8AttnArgs a) {
     using S = RowsShape<NT>;
     extern __shared__ __align__(128) uint8_t smem[];
     float* join = reinterpret_cast<float*>(smem + S::kRing * kWarps * kKv8Bytes);  // [warp][row][kPitch]
     float* join_ml = join + kWarps * S::kRows * kPitch;                            // [warp][row]{m, l}
-    __shared__ uint64_t full[S::kRing * kWarps];
-    __shared__ Kv8Scan<kAttThreads> scan;
+    __shared__ uint64_t full[S::kRing * kWarps], empty[S::kRing * kWarps];
+    __shared__ uint32_t stage_scales[S::kRing * kWarps];
+    __shared__ Kv8Scan<kAttThreads + 32> scan;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int group = a.hq / a.hkv;
     if (tid == 0) {
-        for (int i = 0; i < S::kRing * kWarps; ++i) mbar_init(&full[i], 1);
+        for (int i = 0; i < S::kRing * kWarps; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
         fence_barrier_init();
     }
     pdl_wait();
@@ -686,54 +697,47 @@ attend_rows_kernel(const Kv8AttnArgs a) {
     const int per_block = S::kRows / group;  // query rows of a block
     int64_t per, begin, end;
     Kv8Walk<kPage> use;
-    if (!kv8_part<kAttThreads, kPage>(a, per_block, scan, per, begin, end, use)) return;
+    if (!kv8_part<kAttThreads + 32, kPage>(a, per_block, scan, per, begin, end, use)) return;
 
-    // ---------------- filling: a lane per page id read ahead
-    Kv8Walk<kPage> fill = use;
-    int fill_page = 0, fill_end = 0;  // this warp's next page and the end of the CTA's pages in the item
-    int ids = 0, ids_at = 32;         // lane j: physical page of the j-th page from here, and its scales
-    uint32_t sc = 0, scales[S::kRing];
-    int filled = 0;
-    auto fill_item = [&]() {
-        fill_page = static_cast<int>(larger(0, begin - fill.first)) + warp;
-        fill_end = static_cast<int>(smaller(fill.it.units, end - fill.first));
-        ids_at = 32;
-    };
-    auto fill_one = [&](int stage) {  // issues the warp's next page, if there is one; returns its scales
-        while (fill_page >= fill_end) {
-            if (fill.first + fill.it.units >= end) return 0u;
-            fill.next(a, per_block);
-            fill_item();
-        }
-        if (ids_at == 32) {
-            const int p = fill_page + lane * kWarps;
-            ids = 0;
-            sc = 0;
-            if (p < fill_end) {
-                ids = a.page_table[static_cast<int64_t>(fill.it.r) * a.max_pages + p];
-                if (ids < 0 || ids >= a.num_pages) {
+    if (warp == kWarps) {
+        // ---------------- copies: lane l takes pages l, kBatch + l, ... of an item's part, for warp l % kWarps
+        int filled = 0;  // pages that this warp got before this item
+        bool ok = true;
+        while (__all_sync(0xffffffffu, ok)) {
+            const int p0 = static_cast<int>(larger(0, begin - use.first)), p1 = static_cast<int>(smaller(use.it.units, end - use.first));
+            const int* table = a.page_table + static_cast<int64_t>(use.it.r) * a.max_pages;
+            const int w = lane % kWarps;
+            int next = lane < kBatch && p0 + lane < p1 ? table[p0 + lane] : 0;
+            for (int base = p0; base < p1; base += kBatch) {
+                const int p = lane < kBatch ? base + lane : p1;
+                int id = next;
+                next = p + kBatch < p1 ? table[p + kBatch] : 0;
+                if (id < 0 || id >= a.num_pages) {
                     record_error(a.err, MSGL_ERR_BOUNDS, 902);
-                    ids = 0;
+                    id = 0;
                 }
-                sc = *reinterpret_cast<const uint16_t*>(a.scales + (static_cast<int64_t>(ids) * a.hkv + fill.it.h) * 2);
-            }
-            ids_at = 0;
-        }
-        const int id = __shfl_sync(0xffffffffu, ids, ids_at);
-        const uint32_t scale2 = __shfl_sync(0xffffffffu, sc, ids_at);
-        const int st = warp * S::kRing + stage;
-        if (lane == 0) {
-            mbar_arrive_expect_tx(&full[st], kKv8Bytes);
-            bulk_load(smem + st * kKv8Bytes, a.kv8 + (static_cast<int64_t>(id) * a.hkv + fill.it.h) * kKv8Bytes, kKv8Bytes, &full[st]);
-        }
-        ++ids_at;
-        ++filled;
-        fill_page += kWarps;
-        return scale2;
-    };
-    fill_item();
+                const int64_t block = static_cast<int64_t>(id) * a.hkv + use.it.h;
+                const uint32_t sc = p < p1 ? *reinterpret_cast<const uint16_t*>(a.scales + block * 2) : 0u;
+                const int n = filled + (p - p0) / kWarps, st = w * S::kRing + n % S::kRing;
 #pragma unroll
-    for (int i = 0; i < S::kRing; ++i) scales[i] = fill_one(i);
+                for (int round = 0; round < kBatch / kWarps; ++round) {
+                    if (lane / kWarps == round && p < p1) {
+                        if (n >= S::kRing) ok = ok && mbar_wait(&empty[st], (n / S::kRing - 1) & 1, a.err, 903);
+                        if (ok) {
+                            stage_scales[st] = sc;
+                            mbar_arrive_expect_tx(&full[st], kKv8Bytes);
+                            bulk_load(smem + st * kKv8Bytes, a.kv8 + block * kKv8Bytes, kKv8Bytes, &full[st]);
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+            filled += (p1 - p0 - w + kWarps - 1) / kWarps;
+            if (use.first + use.it.units >= end) break;
+            use.next(a, per_block);
+        }
+        return;
+    }
 
     RowState<NT> st;
     int used = 0;
@@ -743,26 +747,21 @@ attend_rows_kernel(const Kv8AttnArgs a) {
         const int min_lim = use.it.L - use.it.n + use.it.row0;  // last key of the block's first query row
         const int p1 = static_cast<int>(smaller(use.it.units, end - use.first));
         for (int p = static_cast<int>(larger(0, begin - use.first)) + warp; p < p1; p += kWarps) {
-            const int stage = used % S::kRing;
-            const int sg = warp * S::kRing + stage;
-            uint32_t scale2 = scales[0];
-#pragma unroll
-            for (int i = 1; i < S::kRing; ++i) scale2 = stage == i ? scales[i] : scale2;
+            const int sg = warp * S::kRing + used % S::kRing;
             ok = ok && mbar_wait(&full[sg], (used / S::kRing) & 1, a.err, 904);
             const uint8_t* page = smem + sg * kKv8Bytes;
             if (__all_sync(0xffffffffu, ok)) {
+                const uint32_t scale2 = stage_scales[sg];
                 if (p * kPage + kPage - 1 > min_lim) attend_page8<NT, true>(page, scale2, st, p * kPage, min_lim, lane);
                 else attend_page8<NT, false>(page, scale2, st, p * kPage, min_lim, lane);
             }
             __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[sg]);
             ++used;
-            scale2 = fill_one(stage);
-#pragma unroll
-            for (int i = 0; i < S::kRing; ++i) scales[i] = stage == i ? scale2 : scales[i];
         }
         // ---------------- join the warps: unnormalised sums and (m, l) of each through shared memory
         const int g = lane >> 2, c = lane & 3;
-        __syncthreads();
+        attending_barrier();
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             float l = st.l[t];
@@ -778,7 +777,7 @@ attend_rows_kernel(const Kv8AttnArgs a) {
                 for (int e = 0; e < 4; ++e)
                     join[(warp * S::kRows + t * 8 + 2 * c + (e & 1)) * kPitch + 4 * (g + 8 * (v >> 1)) + 2 * (v & 1) + (e >> 1)] = st.o[v][t][e];
         }
-        __syncthreads();
+        attending_barrier();
         const int64_t a0 = use.first / per, a1 = (use.first + use.it.units - 1) / per;
         // a CTA takes part in at most one item that it did not begin and one that it does not end
         const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (blockIdx.x == a0);
@@ -886,7 +885,7 @@ int launch_rows(const Kv8AttnArgs& a, int grid, msgl_stream_t stream) {
     static std::atomic<int> optin[kMaxDevices];
     const cudaError_t e = smem_optin(attend_rows_kernel<NT>, S::kSmem, optin);
     if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
-    launch_pdl(attend_rows_kernel<NT>, dim3(grid), dim3(kAttThreads), S::kSmem, stream, a);
+    launch_pdl(attend_rows_kernel<NT>, dim3(grid), dim3(kAttThreads + 32), S::kSmem, stream, a);
     MSGL_LAUNCH_CHECK();
     return MSGL_OK;
 }
