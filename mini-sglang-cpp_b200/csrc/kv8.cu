@@ -871,7 +871,7 @@ struct RowsPlan {
 RowsPlan plan_rows(int max_q_len, int hq, int hkv) {
     RowsPlan p{};
     const int64_t rows = static_cast<int64_t>(max_q_len) * (hq / hkv);
-    p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 128 ? 128 : 256;
+    p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
     p.grid = 148 * (p.rows == 8 ? 2 : 1);
     p.off_o = (p.grid * sizeof(Kv8Shared) + 255) / 256 * 256;
     p.off_ml = p.off_o + static_cast<size_t>(p.grid) * 2 * p.rows * kHd * 4;
@@ -981,7 +981,7 @@ size_t msgl_paged_attention_kv8_workspace_size(int max_q_len, int num_q_heads, i
     // the largest of the forms that this call or a smaller one may take
     const int group = num_q_heads / num_kv_heads;
     size_t most = plan_rows(max_q_len, num_q_heads, num_kv_heads).bytes;
-    for (int rows : {8, 16, 128})
+    for (int rows : {8, 16, 64, 128})
         most = std::max(most, plan_rows(std::min(max_q_len, rows / group), num_q_heads, num_kv_heads).bytes);
     return most;
 }
@@ -1030,7 +1030,7 @@ int msgl_paged_attention_kv8(const void* q, const void* kv8, const void* scales,
     a.ws_ml = reinterpret_cast<float*>(ws + p.off_ml);
     a.min_units = p.rows <= 16 ? kWarps : 4;  // a page for each warp, or 256 keys
     rc = p.rows == 8 ? launch_rows<1>(a, p.grid, stream) : p.rows == 16 ? launch_rows<2>(a, p.grid, stream)
-                                                          : launch_attend_tiles(a, p.rows == 128, p.grid, stream);
+                                                          : launch_attend_tiles(a, p.rows, p.grid, stream);
     if (rc) return rc;
     launch_pdl(join_shared_kernel, dim3(p.grid - 1, std::min(p.rows / kJoinWarps, 8)), dim3(kJoinWarps * 32), 0, stream, a, p.rows);
     MSGL_LAUNCH_CHECK();

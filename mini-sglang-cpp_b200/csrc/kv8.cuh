@@ -18,7 +18,8 @@
 namespace msgl {
 // Attention of more than 16 rows x heads of a group (kv8_tiles.cu). Items that CTAs share are left as partial sums:
 // CTA b's in slot 2 b where it goes on with an item, in slot 2 b + 1 where it leaves one to the next.
-int launch_attend_tiles(const Kv8AttnArgs& a, bool few, int grid, msgl_stream_t stream);
+// rows: of a block, 64, 128 or 256.
+int launch_attend_tiles(const Kv8AttnArgs& a, int rows, int grid, msgl_stream_t stream);
 
 constexpr int kKv8Page = 16;
 constexpr int kKv8Head = 128;

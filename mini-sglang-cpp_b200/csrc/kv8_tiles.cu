@@ -40,11 +40,27 @@ constexpr int kRows = 128;                     // of a stream
 constexpr int kQTile = 2 * kRows * 128;        // [2 halves of the dimensions][128 rows][64 f16]
 constexpr int kKTile = 2 * kStep * 128;        // [2 halves of the dimensions][64 keys][64 f16]
 constexpr int kVTile = kHd * 128;              // [128 dimensions][64 keys f16]
-constexpr int kStages = 4;                     // of keys and of values
-constexpr int kRaw = 2;                        // steps of codes
 constexpr int kInfo = 8;                       // steps whose scales are kept (a softmax is behind by fewer)
 constexpr int kThreads = 512;
-constexpr size_t kSmem = 1024 + 2 * kQTile + kStages * (kKTile + kVTile) + kRaw * kPages * kKv8Bytes;
+
+// The forms by the rows of a block. 256: the streams are its halves, and both take every step. 128, 64: both streams
+// hold the block and take every other step, joined at the item's end, so that one's softmax runs while the
+// other's MMAs do. With 64 rows half of the softmax warps would have none: they convert (the conversion of
+// four warps is what bounds few rows: 24 requests x 48 rows 145 us, with eight warps XX).
+template <int ROWS>
+struct Form {
+    static constexpr bool kFew = ROWS <= 128;
+    static constexpr int kSoftmaxWarps = ROWS == 64 ? 2 : 4;    // of a stream
+    static constexpr int kConvertWarps = ROWS == 64 ? 4 : 2;    // of keys, and as many of values
+    static constexpr int kStages = 4;                           // of keys and of values
+    static constexpr int kRaw = ROWS == 64 ? 3 : 2;             // steps of codes
+    static constexpr int kQTiles = ROWS == 64 ? 1 : 2;          // 64 rows: both streams read one
+    static constexpr size_t kSmem = 1024 + kQTiles * kQTile + kStages * (kKTile + kVTile) + kRaw * kPages * kKv8Bytes;
+    // Stages of keys and values. Few rows: two for each stream, so that a stream meets every phase of its barriers (one
+    // that skipped a phase would take the one before for it); else all for both. n: steps taken before.
+    __device__ static int stage(int t, int n) { return kFew ? 2 * t + n % 2 : n % kStages; }
+    __device__ static int use(int n) { return kFew ? n / 2 : n / kStages; }
+};
 constexpr float kNegInf = -__builtin_huge_valf();
 
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {  // A, B f16 K-major, D fp32
@@ -83,7 +99,7 @@ struct PageScale {
 };
 
 struct Shared {
-    uint64_t raw_full[kRaw], raw_empty[kRaw], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
+    uint64_t raw_full[3], raw_empty[3], k_full[4], k_empty[4], v_full[4], v_empty[4];
     uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2][2];  // stream, parity of its steps
     PageScale info[kInfo][kPages];
     int nan_seen[kInfo];  // by item in turn: a value hidden from some of its rows was NaN
@@ -185,13 +201,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
     }
 }
 
-// Stages of keys and values. FEW: two for each stream, so that a stream meets every phase of its barriers (one
-// that skipped a phase would take the one before for it); else all for both. n: steps taken before.
-template <bool FEW>
-__device__ __forceinline__ int stage_of(int t, int n) { return FEW ? 2 * t + n % 2 : n % kStages; }
-template <bool FEW>
-__device__ __forceinline__ int use_of(int n) { return FEW ? n / 2 : n / kStages; }
-
 // A CTA's steps of an item: [u0, u1) of its units. Of them, a stream's own ones are first, first + stride, ...
 template <bool FEW>
 struct Share {
@@ -206,35 +215,37 @@ struct Share {
     __device__ __forceinline__ int step(int t, int i) const { return FEW ? u0 + t + 2 * i : u0 + i; }
 };
 
-template <bool FEW>
+template <int ROWS>
 __global__ void __launch_bounds__(kThreads, 1)
 attend_tiles_kernel(const Kv8AttnArgs a) {
+    using F = Form<ROWS>;
+    constexpr bool FEW = F::kFew;
     extern __shared__ uint8_t smem_raw[];
     __shared__ Shared sh;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sQ = smem;                       // a tile per stream; FEW: stream 1's sums between two items
-    uint8_t* sK = sQ + 2 * kQTile;            // [kStages]
-    uint8_t* sV = sK + kStages * kKTile;      // [kStages]
-    uint8_t* sRaw = sV + kStages * kVTile;    // [kRaw][kPages]
+    uint8_t* sK = sQ + F::kQTiles * kQTile;         // [kStages]
+    uint8_t* sV = sK + F::kStages * kKTile;         // [kStages]
+    uint8_t* sRaw = sV + F::kStages * kVTile;       // [kRaw][kPages]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int group = a.hq / a.hkv, per_stream = kRows / group, per_block = FEW ? per_stream : 2 * per_stream;
+    const int group = a.hq / a.hkv, per_block = ROWS / group, per_stream = FEW ? per_block : per_block / 2;
     if (tid == 0) {
-        for (int i = 0; i < kRaw; ++i) {
+        for (int i = 0; i < F::kRaw; ++i) {
             mbar_init(&sh.raw_full[i], 1);
-            mbar_init(&sh.raw_empty[i], 4);
+            mbar_init(&sh.raw_empty[i], 2 * F::kConvertWarps);
         }
-        for (int i = 0; i < kStages; ++i) {
-            mbar_init(&sh.k_full[i], 2);
+        for (int i = 0; i < F::kStages; ++i) {
+            mbar_init(&sh.k_full[i], F::kConvertWarps);
             mbar_init(&sh.k_empty[i], FEW ? 1 : 2);
-            mbar_init(&sh.v_full[i], 2);
+            mbar_init(&sh.v_full[i], F::kConvertWarps);
             mbar_init(&sh.v_empty[i], FEW ? 1 : 2);
         }
         for (int i = 0; i < kInfo; ++i) sh.nan_seen[i] = 0;
         for (int t = 0; t < 2; ++t) {
-            mbar_init(&sh.q_full[t], 4);
+            mbar_init(&sh.q_full[t], F::kSoftmaxWarps);
             for (int b = 0; b < 2; ++b) {
                 mbar_init(&sh.s_full[t][b], 1);
-                mbar_init(&sh.p_full[t][b], 4);
+                mbar_init(&sh.p_full[t][b], F::kSoftmaxWarps);
                 mbar_init(&sh.o_done[t][b], 1);
             }
         }
@@ -258,7 +269,8 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
     bool ok = true;
     auto last_item = [&]() { return walk.first + walk.it.units >= end; };
 
-    if (warp < 8) {
+    constexpr int kSoftmaxThreads = 2 * F::kSoftmaxWarps * 32;
+    if (warp < 8 && (warp & 3) < F::kSoftmaxWarps) {
         // ---------------- softmax of stream t: a thread per row
         const int t = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -294,9 +306,9 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 const float inv = a.sl2e < 0.f ? -kv8_inverse(stored) : kv8_inverse(stored);
                 // a row with an infinity or a NaN has no defined logit: NaN throughout
                 qs = bad ? __int_as_float(0x7fffffff) : kv8_power(stored) * fabsf(a.sl2e);
-                uint8_t* dst = sQ + t * kQTile + row * 128;
+                uint8_t* dst = sQ + (F::kQTiles == 1 ? 0 : t * kQTile) + row * 128;
 #pragma unroll
-                for (int v = 0; v < 16; ++v) {
+                for (int v = 0; v < (F::kQTiles == 1 && t == 1 ? 0 : 16); ++v) {
                     const uint32_t w[4] = {u[v].x, u[v].y, u[v].z, u[v].w};
                     uint32_t f[4];
 #pragma unroll
@@ -305,7 +317,11 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 }
                 fence_proxy_async();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.q_full[t]);
+                if (lane == 0 && F::kQTiles == 2) mbar_arrive(&sh.q_full[t]);
+                if (lane == 0 && F::kQTiles == 1 && t == 0) {  // one tile for both
+                    mbar_arrive(&sh.q_full[0]);
+                    mbar_arrive(&sh.q_full[1]);
+                }
             }
             for (int i = 0; i < own && ok; ++i, ++done) {
                 const int b = done & 1, u = share.step(t, i), c = count + u - share.u0;
@@ -370,7 +386,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
             float scale0 = 1.f, scale1 = 0.f;  // FEW: factors of the streams' sums
             float* other = reinterpret_cast<float*>(sQ);  // FEW: stream 1's sums [dimension][row]
             if (FEW) {
-                named_barrier(1, 256);  // both streams are done with Q
+                named_barrier(1, kSoftmaxThreads);  // both streams are done with Q
                 if (t == 1) {
                     sh.ml[row] = make_float2(m, l);
                     if (own > 0) {
@@ -379,11 +395,11 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                             uint32_t o[32];
                             sums(part, o);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) other[(part * 32 + e) * kRows + row] = __uint_as_float(o[e]);
+                            for (int e = 0; e < 32; ++e) other[(part * 32 + e) * ROWS + row] = __uint_as_float(o[e]);
                         }
                     }
                 }
-                named_barrier(1, 256);
+                named_barrier(1, kSoftmaxThreads);
                 if (t == 0 && share.own(it, per_stream, 1) > 0) {
                     const float2 x = sh.ml[row];
                     const float M = fmaxf(m, x.x);
@@ -397,11 +413,10 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
             const int64_t a0 = walk.first / per, a1 = (walk.first + it.units - 1) / per;
             // a CTA takes part in at most one item that it did not begin and one that it does not end
             const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (blockIdx.x == a0);
-            constexpr int kSlotRows = FEW ? kRows : 2 * kRows;
             const int slot_row = FEW ? row : t * kRows + row;
             if (!FEW || t == 0) {
                 const float inv = a0 != a1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-                if (a0 != a1 && live) *reinterpret_cast<float2*>(a.ws_ml + (slot * kSlotRows + slot_row) * 2) = make_float2(m, l);
+                if (a0 != a1 && live) *reinterpret_cast<float2*>(a.ws_ml + (slot * ROWS + slot_row) * 2) = make_float2(m, l);
 #pragma unroll 1
                 for (int part = 0; part < 4; ++part) {
                     uint32_t o[32];
@@ -409,12 +424,12 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
                         float x = __uint_as_float(o[e]);
-                        if (joins) x = x * scale0 + other[(part * 32 + e) * kRows + row] * scale1;
+                        if (joins) x = x * scale0 + other[(part * 32 + e) * ROWS + row] * scale1;
                         o[e] = __float_as_uint(x * inv);
                     }
                     if (!live) continue;
                     if (a0 != a1) {
-                        float4* dst = reinterpret_cast<float4*>(a.ws_o + (slot * kSlotRows + slot_row) * kHd + part * 32);
+                        float4* dst = reinterpret_cast<float4*>(a.ws_o + (slot * ROWS + slot_row) * kHd + part * 32);
 #pragma unroll
                         for (int c = 0; c < 8; ++c)
                             dst[c] = make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]), __uint_as_float(o[4 * c + 2]),
@@ -433,7 +448,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 }
             }
             if (FEW) {
-                named_barrier(1, 256);  // stream 1's sums were read: Q may come
+                named_barrier(1, kSoftmaxThreads);  // stream 1's sums were read: Q may come
             }
             tc_fence_before();
             count += share.u1 - share.u0;
@@ -442,47 +457,54 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
             walk.next(a, per_block);
         }
     } else if (warp < 12) {
-        // ---------------- each step into f16 tiles: keys by warps 8 and 9, values by 10 and 11
-        const int ct = tid & 63;
-        const bool keys = warp < 10;
-        // keys: the page, half of the dimensions, token, 16 dimensions of it; the row is the token's place
-        const int k_tok = ct >> 2, k_c = ct & 3, k_place = k_tok % 8 / 2 * 4 + k_tok / 8 * 2 + k_tok % 2;
+        // ---------------- each step into f16 tiles: keys by one team of warps, values by the other
+        constexpr int kTeam = F::kConvertWarps;
+        // 64 rows: warps 2, 3, 6, 7 and 8 .. 11; else the latter
+        const int cw = kTeam == 2 ? warp - 8 : warp >= 8 ? warp - 4 : (warp & 1) + (warp >> 2) * 2, ct = (cw & (kTeam - 1)) * 32 + lane;
+        const bool keys = cw < kTeam;
+        constexpr int kUnits = 8 / kTeam;  // 16-byte units of keys of a thread and two pages, pairs of units of values of a thread
+        // keys: token, 16 dimensions of a half; the row is the token's place. Team of 4: a half of the dimensions each
+        const int k_tok = (ct >> 2) & 15, k_c = ct & 3, k_half = kTeam == 4 ? ct >> 6 : 0, k_place = k_tok % 8 / 2 * 4 + k_tok / 8 * 2 + k_tok % 2;
         // values: 8 keys of a page (half v_b), group of four dimensions, page v_page or v_page + 2: eight lanes store
         // to eight different 16-byte columns, and load with two to a bank
-        const int v_b = lane & 1, v_dq = (lane >> 1 & 1) | (lane >> 3) << 1 | (warp & 1) << 4, v_page = lane >> 2 & 1;
+        const int v_b = lane & 1, v_page = lane >> 2 & 1;
+        const int v_dq = (lane >> 1 & 1) | (lane >> 3) << 1 | (cw & (kTeam - 1)) << (kTeam == 4 ? 3 : 4);
+        constexpr int kGroups = kUnits / 2;  // of dimensions, 8 apart
         int c = 0, taken[2] = {0, 0};
         while (ok) {
             const Share<FEW> share(walk, begin, end);
             const Kv8Item& it = walk.it;
             const int first_lim = it.L - it.n + it.row0, last_lim = first_lim + it.rows - 1;
             for (int u = share.u0; u < share.u1 && ok; ++u, ++c) {
-                const int raw = c % kRaw, t = FEW ? (u - share.u0) & 1 : 0;
-                const int st = stage_of<FEW>(t, taken[t]), use = use_of<FEW>(taken[t]);
+                const int raw = c % F::kRaw, t = FEW ? (u - share.u0) & 1 : 0;
+                const int st = F::stage(t, taken[t]), use = F::use(taken[t]);
                 ++taken[t];
                 uint64_t* empty = keys ? &sh.k_empty[st] : &sh.v_empty[st];
-                ok = wait_two(&sh.raw_full[raw], c / kRaw, use == 0 ? &sh.raw_full[raw] : empty, use == 0 ? c / kRaw : use - 1, a.err, 908);
+                ok = wait_two(&sh.raw_full[raw], c / F::kRaw, use == 0 ? &sh.raw_full[raw] : empty, use == 0 ? c / F::kRaw : use - 1, a.err, 908);
                 if (!ok) break;
                 const uint8_t* src = sRaw + raw * kPages * kKv8Bytes;
                 if (keys) {
-                    uint4 w[kPages][2];
+                    constexpr int kHalves = 2 / (kTeam / 2);
+                    uint4 w[kPages][kHalves];
 #pragma unroll
                     for (int i = 0; i < kPages; ++i)
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) w[i][x] = *reinterpret_cast<const uint4*>(src + i * kKv8Bytes + x * 1024 + k_tok * 64 + k_c * 16);
+                        for (int x = 0; x < kHalves; ++x)
+                            w[i][x] = *reinterpret_cast<const uint4*>(src + i * kKv8Bytes + (k_half + x) * 1024 + k_tok * 64 + k_c * 16);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh.raw_empty[raw]);
                     uint8_t* kd = sK + st * kKTile;
 #pragma unroll
                     for (int i = 0; i < kPages; ++i)
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
+                        for (int x = 0; x < kHalves; ++x) {
                             const int row = i * kPage + k_place;
                             uint32_t f[8];
                             e4m3x4_to_half(w[i][x].x, f[0], f[1]);
                             e4m3x4_to_half(w[i][x].y, f[2], f[3]);
                             e4m3x4_to_half(w[i][x].z, f[4], f[5]);
                             e4m3x4_to_half(w[i][x].w, f[6], f[7]);
-                            uint8_t* dst = kd + x * (kKTile / 2) + row * 128;
+                            uint8_t* dst = kd + (k_half + x) * (kKTile / 2) + row * 128;
                             *reinterpret_cast<uint4*>(dst + (((2 * k_c) ^ (row & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
                             *reinterpret_cast<uint4*>(dst + (((2 * k_c + 1) ^ (row & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
                         }
@@ -491,21 +513,21 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                     if (lane == 0) mbar_arrive(&sh.k_full[st]);
                     continue;
                 }
-                uint4 w[4][2];  // pages v_page + 2 (i / 2), groups v_dq + 8 (i % 2)
+                uint4 w[kUnits][2];  // pages v_page + 2 (i / kGroups), groups v_dq + 8 (i % kGroups)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < kUnits; ++i)
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
-                        w[i][x] = *reinterpret_cast<const uint4*>(src + (v_page + 2 * (i >> 1)) * kKv8Bytes + kKv8Values + (v_dq + 8 * (i & 1)) * 64 + v_b * 32 + x * 16);
+                        w[i][x] = *reinterpret_cast<const uint4*>(src + (v_page + 2 * (i / kGroups)) * kKv8Bytes + kKv8Values + (v_dq + 8 * (i % kGroups)) * 64 + v_b * 32 + x * 16);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.raw_empty[raw]);
                 if ((u + 1) * kStep - 1 > first_lim) {  // some row does not see all of the step
                     bool any = false;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                    for (int i = 0; i < kUnits; ++i)
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            const int key = u * kStep + (v_page + 2 * (i >> 1)) * kPage;
+                            const int key = u * kStep + (v_page + 2 * (i / kGroups)) * kPage;
                             uint32_t hidden = 0, seen = 0;
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
@@ -526,16 +548,16 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                     __threadfence_block();
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < kUnits; ++i) {
                     const uint32_t w0[4] = {w[i][0].x, w[i][0].y, w[i][0].z, w[i][0].w};
                     const uint32_t w1[4] = {w[i][1].x, w[i][1].y, w[i][1].z, w[i][1].w};
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        const int dim = (v_dq + 8 * (i & 1)) * 4 + x;
+                        const int dim = (v_dq + 8 * (i % kGroups)) * 4 + x;
                         uint32_t f[4];
                         e4m3x4_to_half(w0[x], f[0], f[1]);
                         e4m3x4_to_half(w1[x], f[2], f[3]);
-                        *reinterpret_cast<uint4*>(sV + st * kVTile + dim * 128 + (((2 * (v_page + 2 * (i >> 1)) + v_b) ^ (dim & 7)) << 4)) =
+                        *reinterpret_cast<uint4*>(sV + st * kVTile + dim * 128 + (((2 * (v_page + 2 * (i / kGroups)) + v_b) ^ (dim & 7)) << 4)) =
                             make_uint4(f[0], f[1], f[2], f[3]);
                     }
                 }
@@ -552,15 +574,17 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
         constexpr uint32_t id_s = idesc_f16(kRows, kStep), id_o = idesc_f16(kRows, kHd);
         const int t = warp - 12;
         const bool lead = elect_lane();
-        const uint64_t dQ = umma_desc_sw128(smem_u32(sQ + t * kQTile)), dK = umma_desc_sw128(smem_u32(sK)), dV = umma_desc_sw128(smem_u32(sV));
+        const uint64_t dQ = umma_desc_sw128(smem_u32(sQ + (F::kQTiles == 1 ? 0 : t * kQTile))), dK = umma_desc_sw128(smem_u32(sK)), dV = umma_desc_sw128(smem_u32(sV));
         const uint32_t tS = tmem + t * 128, tO = tmem + 256 + t * 128;
         int s_count = 0, p_count = 0, loaded = 0;  // S and PV issued so far, items in which the stream had any
         while (ok) {
             const Share<FEW> share(walk, begin, end);
             const int own = share.own(walk.it, per_stream, t);
+            // one tile of Q for both streams: every phase of its barrier is met
+            if (F::kQTiles == 1 && own == 0) ok = wait_one(&sh.q_full[t], loaded, a.err, 905);
             auto issue_s = [&](int i) {  // S of the i-th own step into its buffer, which p of two steps before has left
                 if (i >= own || !ok) return;
-                const int n = FEW ? s_count : count + i, st = stage_of<FEW>(t, n), use = use_of<FEW>(n), b = s_count & 1;
+                const int n = FEW ? s_count : count + i, st = F::stage(t, n), use = F::use(n), b = s_count & 1;
                 if (i == 0) ok = wait_one(&sh.q_full[t], loaded, a.err, 905);
                 ok = ok && wait_two(&sh.k_full[st], use, s_count < 2 ? &sh.k_full[st] : &sh.o_done[t][b],
                                     s_count < 2 ? use : (s_count - 2) >> 1, a.err, 908);
@@ -581,8 +605,8 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
             issue_s(0);
             issue_s(1);
             for (int i = 0; i < own && ok; ++i) {
-                const int n = FEW ? p_count : count + i, st = stage_of<FEW>(t, n), b = p_count & 1;
-                ok = wait_two(&sh.v_full[st], use_of<FEW>(n), &sh.p_full[t][b], p_count >> 1, a.err, 909);
+                const int n = FEW ? p_count : count + i, st = F::stage(t, n), b = p_count & 1;
+                ok = wait_two(&sh.v_full[st], F::use(n), &sh.p_full[t][b], p_count >> 1, a.err, 909);
                 if (!ok) break;
                 tc_fence_after();
                 if (lead) {
@@ -600,8 +624,8 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
             // steps that only the other stream sees: their stages are free as far as this one goes
             if (!FEW)
                 for (int u = share.u0 + own; u < share.u1 && ok; ++u) {
-                    const int c = count + u - share.u0, st = c % kStages;
-                    ok = wait_two(&sh.k_full[st], c / kStages, &sh.v_full[st], c / kStages, a.err, 908);
+                    const int c = count + u - share.u0, st = F::stage(0, c);
+                    ok = wait_two(&sh.k_full[st], F::use(c), &sh.v_full[st], F::use(c), a.err, 908);
                     if (ok && lead) {
                         mbar_arrive(&sh.k_empty[st]);
                         mbar_arrive(&sh.v_empty[st]);
@@ -609,7 +633,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                     __syncwarp();
                 }
             count += share.u1 - share.u0;
-            if (own > 0) ++loaded;
+            if (own > 0 || F::kQTiles == 1) ++loaded;
             if (last_item()) break;
             walk.next(a, per_block);
         }
@@ -640,9 +664,9 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                     sc = none ? 0x7f7fu : *reinterpret_cast<const uint16_t*>(a.scales + (static_cast<int64_t>(ids) * a.hkv + it.h) * 2);
                     if (none) ids = -1;
                 }
-                const int raw = c % kRaw;
+                const int raw = c % F::kRaw;
                 if (u == share.u0 && lane == 0) sh.nan_seen[item % kInfo] = 0;  // last of an item that is done
-                if (c >= kRaw) ok = wait_one(&sh.raw_empty[raw], c / kRaw - 1, a.err, 908);
+                if (c >= F::kRaw) ok = wait_one(&sh.raw_empty[raw], c / F::kRaw - 1, a.err, 908);
                 if (!ok) break;
                 const int pages = min(kPages, seen - u * kPages);
                 // the scales go ahead of the barrier that the conversion, the MMAs and so the softmax wait for
@@ -669,20 +693,20 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
     }
 }
 
-template <bool FEW>
+template <int ROWS>
 int launch(const Kv8AttnArgs& a, int grid, msgl_stream_t stream) {
     static std::atomic<int> optin[kMaxDevices];
-    const cudaError_t e = smem_optin(attend_tiles_kernel<FEW>, kSmem, optin);
+    const cudaError_t e = smem_optin(attend_tiles_kernel<ROWS>, Form<ROWS>::kSmem, optin);
     if (e != cudaSuccess) return set_error(MSGL_ERR_CUDA, cudaGetErrorString(e));
-    launch_pdl(attend_tiles_kernel<FEW>, dim3(grid), dim3(kThreads), kSmem, stream, a);
+    launch_pdl(attend_tiles_kernel<ROWS>, dim3(grid), dim3(kThreads), Form<ROWS>::kSmem, stream, a);
     MSGL_LAUNCH_CHECK();
     return MSGL_OK;
 }
 
 }  // namespace
 
-int launch_attend_tiles(const Kv8AttnArgs& a, bool few, int grid, msgl_stream_t stream) {
-    return few ? launch<true>(a, grid, stream) : launch<false>(a, grid, stream);
+int launch_attend_tiles(const Kv8AttnArgs& a, int rows, int grid, msgl_stream_t stream) {
+    return rows <= 64 ? launch<64>(a, grid, stream) : rows <= 128 ? launch<128>(a, grid, stream) : launch<256>(a, grid, stream);
 }
 
 }  // namespace msgl
