@@ -40,7 +40,9 @@ constexpr int kRows = 128;                     // of a stream
 constexpr int kQTile = 2 * kRows * 128;        // [2 halves of the dimensions][128 rows][64 f16]
 constexpr int kKTile = 2 * kStep * 128;        // [2 halves of the dimensions][64 keys][64 f16]
 constexpr int kVTile = kHd * 128;              // [128 dimensions][64 keys f16]
-constexpr int kInfo = 8;                       // steps whose scales are kept (a softmax is behind by fewer)
+// Steps whose scales are kept. Step c + 8's are written once codes c + 5 (kRaw = 3) were read, hence values c + 4 laid
+// down, hence PV of step c done.
+constexpr int kInfo = 8;
 constexpr int kThreads = 512;
 
 // The forms by the rows of a block. 256: the streams are its halves, and both take every step. 128, 64: both streams
@@ -645,41 +647,32 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
             const Kv8Item& it = walk.it;
             const int seen = (it.L - it.n + it.row0 + it.rows - 1) / kPage + 1;  // pages that any row sees
             const int* table = a.page_table + static_cast<int64_t>(it.r) * a.max_pages;
-            auto page_id = [&](int u) {  // lane 4 s + p: page p of step u + s; -1 behind the CTA's part
-                const int p = u * kPages + lane;
-                return p < min(seen, share.u1 * kPages) ? table[p] : -1;
-            };
-            int ids = page_id(share.u0), ids_next = -1;
-            uint32_t sc = 0x7f7f;
-            for (int u = share.u0; u < share.u1 && ok; ++u, ++c) {
-                const int at = (u - share.u0) % 8 * kPages;
-                if (at == 0) {
-                    if (u > share.u0) ids = ids_next;
-                    ids_next = page_id(u + 8);
-                    const bool none = (u * kPages + lane) >= min(seen, share.u1 * kPages);
-                    if (!none && (ids < 0 || ids >= a.num_pages)) {
-                        record_error(a.err, MSGL_ERR_BOUNDS, 902);
-                        ids = 0;
-                    }
-                    sc = none ? 0x7f7fu : *reinterpret_cast<const uint16_t*>(a.scales + (static_cast<int64_t>(ids) * a.hkv + it.h) * 2);
-                    if (none) ids = -1;
+            const int pages = min(seen, share.u1 * kPages);
+            // eight steps at a time: lane 4 s + p has page p of the s-th, the next eight's ids on their way
+            int next = share.u0 * kPages + lane < pages ? table[share.u0 * kPages + lane] : 0;
+            if (lane == 0) sh.nan_seen[item % kInfo] = 0;  // last of an item that is done
+            for (int u0 = share.u0; u0 < share.u1 && ok; u0 += 8) {
+                const int page = u0 * kPages + lane;
+                int id = next;
+                next = page + 32 < pages ? table[page + 32] : 0;
+                if (id < 0 || id >= a.num_pages) {
+                    record_error(a.err, MSGL_ERR_BOUNDS, 902);
+                    id = 0;
                 }
-                const int raw = c % F::kRaw;
-                if (u == share.u0 && lane == 0) sh.nan_seen[item % kInfo] = 0;  // last of an item that is done
-                if (c >= F::kRaw) ok = wait_one(&sh.raw_empty[raw], c / F::kRaw - 1, a.err, 908);
-                if (!ok) break;
-                const int pages = min(kPages, seen - u * kPages);
-                // the scales go ahead of the barrier that the conversion, the MMAs and so the softmax wait for
-                if (lane >= at && lane < at + kPages) {
-                    const int ve = sc >> 8;
-                    sh.info[c % kInfo][lane - at] = {kv8_power(sc & 0xff), static_cast<float>(ve - 127), kv8_inverse(ve), 0.f};
+                const int64_t block = static_cast<int64_t>(id) * a.hkv + it.h;
+                const uint32_t sc = page < pages ? *reinterpret_cast<const uint16_t*>(a.scales + block * 2) : 0x7f7fu;
+                const PageScale scale = {kv8_power(sc & 0xff), static_cast<float>(static_cast<int>(sc >> 8) - 127), kv8_inverse(sc >> 8), 0.f};
+                const uint8_t* codes = a.kv8 + block * kKv8Bytes;
+                for (int s = 0; s < 8 && u0 + s < share.u1; ++s, ++c) {
+                    const int raw = c % F::kRaw;
+                    if (c >= F::kRaw) ok = ok && wait_one(&sh.raw_empty[raw], c / F::kRaw - 1, a.err, 908);
+                    if (!ok) break;
+                    // the scales go ahead of the barrier that the conversion, the MMAs and so the softmax wait for
+                    if (lane >> 2 == s) sh.info[c % kInfo][lane & 3] = scale;
+                    __syncwarp();
+                    if (lane >> 2 == s && page < pages) bulk_load(sRaw + (raw * kPages + (lane & 3)) * kKv8Bytes, codes, kKv8Bytes, &sh.raw_full[raw]);
+                    if (lane == 0) mbar_arrive_expect_tx(&sh.raw_full[raw], min(kPages, pages - (u0 + s) * kPages) * kKv8Bytes);
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive_expect_tx(&sh.raw_full[raw], pages * kKv8Bytes);
-                __syncwarp();
-                if (lane >= at && lane < at + pages)
-                    bulk_load(sRaw + (raw * kPages + lane - at) * kKv8Bytes, a.kv8 + (static_cast<int64_t>(ids) * a.hkv + it.h) * kKv8Bytes,
-                              kKv8Bytes, &sh.raw_full[raw]);
             }
             ++item;
             if (last_item()) break;
