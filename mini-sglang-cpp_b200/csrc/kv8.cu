@@ -814,19 +814,27 @@ attend_rows_kernel(const Kv8AttnArgs a) {
 
 // ------------------------------------------------------------------ joining
 // Partial sums of the items that CTAs share, in the CTAs' order. Block (b, y): the item that CTA b goes on with, if
-// the CTA before it is the first; rows 8 y .. 8 y + 7 of every gridDim.y x 8, a warp per row, a lane per four dimensions,
-// eight parts' loads in flight. A kernel of its own: the last CTA of an item to arrive took XX us for 19 parts of 2
-// rows and 30 us for five of 256.
+// the CTA before it is the first; eight parts' loads in flight. A kernel of its own: where the last CTA of an item to
+// arrive joined it, one request at 4k took 20.5 us for 18.0 and 256 rows at 8k 133 for 75.
+// COLUMNS false (few rows, row after row): a warp per row, rows 8 y .. 8 y + 7 of every gridDim.y x 8, a lane per four
+// dimensions. COLUMNS true (four dimensions of all rows after each other): a lane per row, of 32 y .. 32 y + 31, four
+// such columns a warp; with row after row 256 rows' stores took 18 us a part (2048 rows of a prompt: 231 us, so XX).
 constexpr int kJoinWarps = 8;
 
+template <bool COLUMNS>
 __global__ void __launch_bounds__(kJoinWarps * 32)
 join_shared_kernel(const Kv8AttnArgs a, int slot_rows) {
     pdl_wait();
     pdl_trigger();
     const Kv8Shared s = a.ws_shared[blockIdx.x + 1];
     if (s.last < s.first || s.first != static_cast<int>(blockIdx.x)) return;
-    const int lane = threadIdx.x & 31, group = a.hq / a.hkv;
-    for (int m = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); m < s.rows; m += gridDim.y * kJoinWarps) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = a.hq / a.hkv;
+    const int turns = COLUMNS ? kHd / 4 / kJoinWarps : (s.rows + gridDim.y * kJoinWarps - 1) / (gridDim.y * kJoinWarps);
+    for (int turn = 0; turn < turns; ++turn) {
+        const int m = COLUMNS ? blockIdx.y * 32 + lane : (turn * gridDim.y + blockIdx.y) * kJoinWarps + warp;
+        const int column = COLUMNS ? turn * kJoinWarps + warp : lane;  // four dimensions
+        if (m >= s.rows) continue;
+        const int64_t at = COLUMNS ? static_cast<int64_t>(column) * slot_rows + m : static_cast<int64_t>(m) * (kHd / 4) + column;
         float M = kNegInf, l = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int b0 = s.first; b0 <= s.last; b0 += 8) {
@@ -835,9 +843,9 @@ join_shared_kernel(const Kv8AttnArgs a, int slot_rows) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int b = b0 + i;
-                const int64_t w = (2 * static_cast<int64_t>(b) + (b == s.first)) * slot_rows + m;
-                ml[i] = b <= s.last ? __ldcg(reinterpret_cast<const float2*>(a.ws_ml) + w) : make_float2(kNegInf, 0.f);
-                x[i] = b <= s.last ? __ldcg(reinterpret_cast<const float4*>(a.ws_o + w * kHd) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const int64_t slot = 2 * static_cast<int64_t>(b) + (b == s.first);
+                ml[i] = b <= s.last ? __ldcg(reinterpret_cast<const float2*>(a.ws_ml) + slot * slot_rows + m) : make_float2(kNegInf, 0.f);
+                x[i] = b <= s.last ? __ldcg(reinterpret_cast<const float4*>(a.ws_o) + slot * slot_rows * (kHd / 4) + at) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
             float next = M;
 #pragma unroll
@@ -855,7 +863,7 @@ join_shared_kernel(const Kv8AttnArgs a, int slot_rows) {
             }
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        *reinterpret_cast<uint2*>(a.out + ((s.q_row + m / group) * a.hq + s.h * group + m % group) * kHd + lane * 4) =
+        *reinterpret_cast<uint2*>(a.out + ((s.q_row + m / group) * a.hq + s.h * group + m % group) * kHd + column * 4) =
             make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
     }
 }
@@ -1032,7 +1040,9 @@ int msgl_paged_attention_kv8(const void* q, const void* kv8, const void* scales,
     rc = p.rows == 8 ? launch_rows<1>(a, p.grid, stream) : p.rows == 16 ? launch_rows<2>(a, p.grid, stream)
                                                           : launch_attend_tiles(a, p.rows, p.grid, stream);
     if (rc) return rc;
-    launch_pdl(join_shared_kernel, dim3(p.grid - 1, std::min(p.rows / kJoinWarps, 8)), dim3(kJoinWarps * 32), 0, stream, a, p.rows);
+    const bool columns = p.rows > 16;
+    launch_pdl(columns ? join_shared_kernel<true> : join_shared_kernel<false>, dim3(p.grid - 1, columns ? p.rows / 32 : p.rows / kJoinWarps),
+               dim3(kJoinWarps * 32), 0, stream, a, p.rows);
     MSGL_LAUNCH_CHECK();
     return MSGL_OK;
 }

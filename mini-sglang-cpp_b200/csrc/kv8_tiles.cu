@@ -431,10 +431,11 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                     }
                     if (!live) continue;
                     if (a0 != a1) {
-                        float4* dst = reinterpret_cast<float4*>(a.ws_o + (slot * ROWS + slot_row) * kHd + part * 32);
+                        // [group of four dimensions][row]: a warp's stores are next to each other
+                        float4* dst = reinterpret_cast<float4*>(a.ws_o + slot * ROWS * kHd) + part * 8 * ROWS + slot_row;
 #pragma unroll
                         for (int c = 0; c < 8; ++c)
-                            dst[c] = make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]), __uint_as_float(o[4 * c + 2]),
+                            dst[c * ROWS] = make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]), __uint_as_float(o[4 * c + 2]),
                                                  __uint_as_float(o[4 * c + 3]));
                     } else {
                         uint4* dst = reinterpret_cast<uint4*>(a.out + at + part * 32);
