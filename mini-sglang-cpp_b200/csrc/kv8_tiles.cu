@@ -83,10 +83,13 @@ __device__ __forceinline__ void named_barrier(int id, int threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
-// Waits of a whole warp: even lanes for the use-th completion of a, odd ones for that of b.
+// Waits of a whole warp: even lanes for the use-th completion of a, odd ones for that of b. A vote orders no memory:
+// the warp barrier behind it is what lets each lane see what the other half waited for.
 __device__ __forceinline__ bool wait_two(uint64_t* a, int use_a, uint64_t* b, int use_b, int* err, int site) {
     const bool odd = threadIdx.x & 1;
-    return __all_sync(0xffffffffu, mbar_wait(odd ? b : a, (odd ? use_b : use_a) & 1, err, site));
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(odd ? b : a, (odd ? use_b : use_a) & 1, err, site));
+    __syncwarp();
+    return ok;
 }
 __device__ __forceinline__ bool wait_one(uint64_t* a, int use, int* err, int site) {
     return __all_sync(0xffffffffu, mbar_wait(a, use & 1, err, site));
@@ -189,13 +192,22 @@ __device__ __forceinline__ void softmax_step(uint32_t (&s)[64], uint32_t (&out)[
     m = next;
 }
 
+// Waits for the loads that write r: no use of r moves ahead of it.
+template <int N>
+__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[N]) {
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < N; ++e) asm volatile("" : "+r"(r[e]));
+}
+
 // 32 consecutive columns of this thread's lane.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
     __syncwarp();
     uint32_t lo[16], hi[16];
     tmem_ld16(taddr, lo);
     tmem_ld16(taddr + 16, hi);
-    tmem_ld_wait();
+    tmem_loaded(lo);
+    tmem_loaded(hi);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
         r[e] = lo[e];
@@ -203,12 +215,16 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
     }
 }
 
+// Of an item, in steps (Q loaded, the pipeline filled and emptied, sums stored): four prompts of 2048 328 us with 3, 234 with
+// 6, 222 with 10.
+constexpr int kItemCost = 10;
+using Walk = Kv8Walk<kStep, kItemCost>;
+
 // A CTA's steps of an item: [u0, u1) of its units. Of them, a stream's own ones are first, first + stride, ...
 template <bool FEW>
 struct Share {
     int u0, u1;
-    __device__ __forceinline__ Share(const Kv8Walk<kStep>& w, int64_t begin, int64_t end)
-        : u0(static_cast<int>(larger(0, begin - w.first))), u1(static_cast<int>(smaller(w.it.units, end - w.first))) {}
+    __device__ __forceinline__ explicit Share(const Walk& w) : u0(w.u0()), u1(w.u1()) {}
     // number of stream t's steps
     __device__ __forceinline__ int own(const Kv8Item& it, int per_stream, int t) const {
         if (FEW) return (u1 - u0 + 1 - t) / 2;
@@ -255,9 +271,8 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
     }
     pdl_wait();
     pdl_trigger();
-    int64_t per, begin, end;
-    Kv8Walk<kStep> walk;
-    if (!kv8_part<kThreads, kStep>(a, per_block, sh.scan, per, begin, end, walk)) return;
+    Walk walk;
+    if (!kv8_part(a, per_block, sh.scan, walk)) return;
     if (warp == 12) {
         tmem_alloc(&sh.tmem, 512);
         tmem_relinquish();
@@ -269,7 +284,6 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
     // Every role walks the CTA's items by itself: `count` steps of the items before this one, the `item`-th item.
     int count = 0, item = 0;
     bool ok = true;
-    auto last_item = [&]() { return walk.first + walk.it.units >= end; };
 
     constexpr int kSoftmaxThreads = 2 * F::kSoftmaxWarps * 32;
     if (warp < 8 && (warp & 3) < F::kSoftmaxWarps) {
@@ -279,7 +293,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
         const uint32_t tS = tmem + t * 128 + lanes, tO = tmem + 256 + t * 128 + lanes;
         int done = 0;  // steps of this stream
         while (true) {
-            const Share<FEW> share(walk, begin, end);
+            const Share<FEW> share(walk);
             const Kv8Item& it = walk.it;
             const int i_row = it.row0 + (FEW ? 0 : t * per_stream) + row / group;
             const bool live = i_row < it.row0 + it.rows;
@@ -332,7 +346,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 tc_fence_after();
                 uint32_t s[64], pairs[32];
                 tmem_ld64(tS + b * 64, s);
-                tmem_ld_wait();
+                tmem_loaded(s);
                 const PageScale* info = sh.info[c % kInfo];
                 float alpha;
                 if ((u + 1) * kStep - 1 > stream_first) softmax_step<true>(s, pairs, info, qs, u * kStep, lim, m, l, alpha);
@@ -412,9 +426,9 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 }
             }
             const bool joins = FEW && share.own(it, per_stream, 1) > 0;
-            const int64_t a0 = walk.first / per, a1 = (walk.first + it.units - 1) / per;
+            const int a0 = walk.cta0(), a1 = walk.cta1();
             // a CTA takes part in at most one item that it did not begin and one that it does not end
-            const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (blockIdx.x == a0);
+            const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (static_cast<int>(blockIdx.x) == a0);
             const int slot_row = FEW ? row : t * kRows + row;
             if (!FEW || t == 0) {
                 const float inv = a0 != a1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
@@ -456,8 +470,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
             tc_fence_before();
             count += share.u1 - share.u0;
             ++item;
-            if (last_item()) break;
-            walk.next(a, per_block);
+            if (!walk.next(a, per_block)) break;
         }
     } else if (warp < 12) {
         // ---------------- each step into f16 tiles: keys by one team of warps, values by the other
@@ -475,7 +488,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
         constexpr int kGroups = kUnits / 2;  // of dimensions, 8 apart
         int c = 0, taken[2] = {0, 0};
         while (ok) {
-            const Share<FEW> share(walk, begin, end);
+            const Share<FEW> share(walk);
             const Kv8Item& it = walk.it;
             const int first_lim = it.L - it.n + it.row0, last_lim = first_lim + it.rows - 1;
             for (int u = share.u0; u < share.u1 && ok; ++u, ++c) {
@@ -486,6 +499,8 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 ok = wait_two(&sh.raw_full[raw], c / F::kRaw, use == 0 ? &sh.raw_full[raw] : empty, use == 0 ? c / F::kRaw : use - 1, a.err, 908);
                 if (!ok) break;
                 const uint8_t* src = sRaw + raw * kPages * kKv8Bytes;
+                // The fence before a slot is given back puts its reads ahead of the copy that overwrites it: without, that copy
+                // overtook loads on their way (giving it back after the conversion instead: chunks 557 us, so 440).
                 if (keys) {
                     constexpr int kHalves = 2 / (kTeam / 2);
                     uint4 w[kPages][kHalves];
@@ -494,6 +509,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
 #pragma unroll
                         for (int x = 0; x < kHalves; ++x)
                             w[i][x] = *reinterpret_cast<const uint4*>(src + i * kKv8Bytes + (k_half + x) * 1024 + k_tok * 64 + k_c * 16);
+                    fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh.raw_empty[raw]);
                     uint8_t* kd = sK + st * kKTile;
@@ -522,6 +538,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
                         w[i][x] = *reinterpret_cast<const uint4*>(src + (v_page + 2 * (i / kGroups)) * kKv8Bytes + kKv8Values + (v_dq + 8 * (i % kGroups)) * 64 + v_b * 32 + x * 16);
+                fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.raw_empty[raw]);
                 if ((u + 1) * kStep - 1 > first_lim) {  // some row does not see all of the step
@@ -569,8 +586,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 if (lane == 0) mbar_arrive(&sh.v_full[st]);
             }
             ++item;
-            if (last_item()) break;
-            walk.next(a, per_block);
+            if (!walk.next(a, per_block)) break;
         }
     } else if (warp < 14) {
         // ---------------- MMAs of stream t: the warp waits together, one lane issues (descriptors stay uniform)
@@ -581,7 +597,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
         const uint32_t tS = tmem + t * 128, tO = tmem + 256 + t * 128;
         int s_count = 0, p_count = 0, loaded = 0;  // S and PV issued so far, items in which the stream had any
         while (ok) {
-            const Share<FEW> share(walk, begin, end);
+            const Share<FEW> share(walk);
             const int own = share.own(walk.it, per_stream, t);
             // one tile of Q for both streams: every phase of its barrier is met
             if (F::kQTiles == 1 && own == 0) ok = wait_one(&sh.q_full[t], loaded, a.err, 905);
@@ -637,14 +653,13 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 }
             count += share.u1 - share.u0;
             if (own > 0 || F::kQTiles == 1) ++loaded;
-            if (last_item()) break;
-            walk.next(a, per_block);
+            if (!walk.next(a, per_block)) break;
         }
     } else if (warp == 14) {
         // ---------------- codes and scales of each step
         int c = 0;
         while (ok) {
-            const Share<FEW> share(walk, begin, end);
+            const Share<FEW> share(walk);
             const Kv8Item& it = walk.it;
             const int seen = (it.L - it.n + it.row0 + it.rows - 1) / kPage + 1;  // pages that any row sees
             const int* table = a.page_table + static_cast<int64_t>(it.r) * a.max_pages;
@@ -671,13 +686,14 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                     // the scales go ahead of the barrier that the conversion, the MMAs and so the softmax wait for
                     if (lane >> 2 == s) sh.info[c % kInfo][lane & 3] = scale;
                     __syncwarp();
-                    if (lane >> 2 == s && page < pages) bulk_load(sRaw + (raw * kPages + (lane & 3)) * kKv8Bytes, codes, kKv8Bytes, &sh.raw_full[raw]);
+                    // the bytes are expected before any of them comes
                     if (lane == 0) mbar_arrive_expect_tx(&sh.raw_full[raw], min(kPages, pages - (u0 + s) * kPages) * kKv8Bytes);
+                    __syncwarp();
+                    if (lane >> 2 == s && page < pages) bulk_load(sRaw + (raw * kPages + (lane & 3)) * kKv8Bytes, codes, kKv8Bytes, &sh.raw_full[raw]);
                 }
             }
             ++item;
-            if (last_item()) break;
-            walk.next(a, per_block);
+            if (!walk.next(a, per_block)) break;
         }
     }
     __syncthreads();

@@ -354,6 +354,16 @@ def test_chunks(cuda, lens, rows, hq, hkv):
     assert ops.device_error() == (0, 0)
 
 
+@pytest.mark.parametrize("lens,rows,hq,hkv", [([1500, 1100], [1100, 333], 32, 8), ([2048], [2048], 32, 8), ([2000] * 24, [6] * 24, 8, 1),
+                                              ([1000] * 9, [30] * 9, 16, 4), ([900] * 30, [1] * 30, 32, 8)])
+def test_the_same_call_again_gives_the_same_bits(cuda, lens, rows, hq, hkv):
+    """No part of a result hangs on which warp or copy came first."""
+    a = Attend(lens, rows, hq, hkv, seed=5)
+    first = a.call()
+    for _ in range(40):
+        assert torch.equal(a.call(), first)
+
+
 @pytest.mark.parametrize("rows", [[1, 1, 1], [6, 6, 6], [70, 33, 90]])
 def test_values_behind_a_row_do_not_reach_it(cuda, rows):
     """NaN keys and values in tokens that only later rows see, and in all slots behind the context (Attend)."""
