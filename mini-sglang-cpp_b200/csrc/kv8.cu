@@ -734,6 +734,9 @@ attend_rows_kernel(const Kv8AttnArgs a) {
             }
             filled += (p1 - p0 - w + kWarps - 1) / kWarps;
         } while (__all_sync(0xffffffffu, ok) && use.next(a, per_block));
+        // after a wait that ran out: no copy is left on its way into the block's shared memory
+        if (lane < kWarps)
+            for (int i = max(0, filled - S::kRing); i < filled; ++i) mbar_wait(&full[lane * S::kRing + i % S::kRing], (i / S::kRing) & 1, a.err, 904);
         return;
     }
 

@@ -695,6 +695,8 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
             ++item;
             if (!walk.next(a, per_block)) break;
         }
+        // after a wait that ran out: no copy is left on its way into the block's shared memory
+        for (int i = max(0, c - F::kRaw); i < c; ++i) wait_one(&sh.raw_full[i % F::kRaw], i / F::kRaw, a.err, 908);
     }
     __syncthreads();
     if (warp == 12) {
