@@ -37,12 +37,9 @@ constexpr int kHd = kKv8Head;
 constexpr int kStep = 64;                      // keys
 constexpr int kPages = kStep / kPage;          // of a step
 constexpr int kRows = 128;                     // of a stream
-constexpr int kQTile = 2 * kRows * 128;        // [2 halves of the dimensions][128 rows][64 f16]
 constexpr int kKTile = 2 * kStep * 128;        // [2 halves of the dimensions][64 keys][64 f16]
 constexpr int kVTile = kHd * 128;              // [128 dimensions][64 keys f16]
-// Steps whose scales are kept. Step c + 8's are written once codes c + 5 (kRaw = 3) were read, hence values c + 4 laid
-// down, hence PV of step c done.
-constexpr int kInfo = 8;
+constexpr int kItems = 16;  // items whose NaN are kept; the copies are ahead by fewer than ten (of one step each)
 constexpr int kThreads = 512;
 
 // The forms by the rows of a block. 256: the streams are its halves, and both take every step. 128, 64: both streams
@@ -53,15 +50,23 @@ template <int ROWS>
 struct Form {
     static constexpr bool kFew = ROWS <= 128;
     static constexpr int kSoftmaxWarps = ROWS == 64 ? 2 : 4;    // of a stream
-    static constexpr int kConvertWarps = ROWS == 64 ? 4 : 2;    // of keys, and as many of values
+    static constexpr int kConvertWarps = 2;                     // of keys, and as many of values
+    static constexpr int kTeams = ROWS == 64 ? 2 : 1;           // of them: one, or one for each stream
     static constexpr int kStages = 4;                           // of keys and of values
-    static constexpr int kRaw = ROWS == 64 ? 3 : 2;             // steps of codes
-    static constexpr int kQTiles = ROWS == 64 ? 1 : 2;          // 64 rows: both streams read one
-    static constexpr size_t kSmem = 1024 + kQTiles * kQTile + kStages * (kKTile + kVTile) + kRaw * kPages * kKv8Bytes;
+    static constexpr int kRaw = ROWS == 64 ? 4 : 2;             // steps of codes
+    // Steps whose scales are kept: more than the copies are ahead of a softmax (by the slots of codes, the stages and two).
+    static constexpr int kInfo = ROWS == 64 ? 16 : 8;
+    static constexpr int kQHalf = (ROWS == 64 ? 64 : kRows) * 128;  // 64 dimensions of a tile of Q: [rows][64 f16]
+    static constexpr int kQTiles = ROWS == 64 ? 1 : 2;
+    static constexpr int kQ = 2 * kQTiles * kQHalf;
+    static constexpr size_t kSmem = 1024 + kQ + kStages * (kKTile + kVTile) + kRaw * kPages * kKv8Bytes;
+    static constexpr int kJoinDims = kQ / 4 / ROWS < kHd ? kQ / 4 / ROWS : kHd;  // of stream 1's sums that the place of Q holds
     // Stages of keys and values. Few rows: two for each stream, so that a stream meets every phase of its barriers (one
     // that skipped a phase would take the one before for it); else all for both. n: steps taken before.
     __device__ static int stage(int t, int n) { return kFew ? 2 * t + n % 2 : n % kStages; }
     __device__ static int use(int n) { return kFew ? n / 2 : n / kStages; }
+    // Slots of codes: of each team its own, for the same reason.
+    __device__ static int slot(int t, int n) { return kTeams == 2 ? 2 * t + n % 2 : n % 2; }
 };
 constexpr float kNegInf = -__builtin_huge_valf();
 
@@ -103,15 +108,16 @@ struct PageScale {
     float k, v_exp, v_inv, pad;
 };
 
+template <int ROWS>
 struct Shared {
-    uint64_t raw_full[3], raw_empty[3], k_full[4], k_empty[4], v_full[4], v_empty[4];
+    uint64_t raw_full[Form<ROWS>::kRaw], raw_empty[Form<ROWS>::kRaw], k_full[4], k_empty[4], v_full[4], v_empty[4];
     uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2][2];  // stream, parity of its steps
-    PageScale info[kInfo][kPages];
-    int nan_seen[kInfo];  // by item in turn: a value hidden from some of its rows was NaN
+    PageScale info[Form<ROWS>::kInfo][kPages];
+    int nan_seen[kItems];  // by item in turn: a value hidden from some of its rows was NaN
     uint32_t tmem;
     union {
         Kv8Scan<kThreads> scan;  // before the walk
-        float2 ml[kRows];        // stream 1's (m, l), FEW
+        float2 ml[Form<ROWS>::kFew ? ROWS : 1];  // stream 1's (m, l)
     };
 };
 
@@ -239,11 +245,11 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
     using F = Form<ROWS>;
     constexpr bool FEW = F::kFew;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ Shared sh;
+    __shared__ Shared<ROWS> sh;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* sQ = smem;                       // a tile per stream; FEW: stream 1's sums between two items
-    uint8_t* sK = sQ + F::kQTiles * kQTile;         // [kStages]
-    uint8_t* sV = sK + F::kStages * kKTile;         // [kStages]
+    uint8_t* sK = smem;                             // [kStages]
+    uint8_t* sQ = sK + F::kStages * kKTile;         // a tile per stream, or one; FEW: stream 1's sums between two items
+    uint8_t* sV = sQ + F::kQ;                       // [kStages]
     uint8_t* sRaw = sV + F::kStages * kVTile;       // [kRaw][kPages]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int group = a.hq / a.hkv, per_block = ROWS / group, per_stream = FEW ? per_block : per_block / 2;
@@ -258,7 +264,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
             mbar_init(&sh.v_full[i], F::kConvertWarps);
             mbar_init(&sh.v_empty[i], FEW ? 1 : 2);
         }
-        for (int i = 0; i < kInfo; ++i) sh.nan_seen[i] = 0;
+        for (int i = 0; i < kItems; ++i) sh.nan_seen[i] = 0;
         for (int t = 0; t < 2; ++t) {
             mbar_init(&sh.q_full[t], F::kSoftmaxWarps);
             for (int b = 0; b < 2; ++b) {
@@ -286,9 +292,9 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
     bool ok = true;
 
     constexpr int kSoftmaxThreads = 2 * F::kSoftmaxWarps * 32;
-    if (warp < 8 && (warp & 3) < F::kSoftmaxWarps) {
+    if (warp < 8 && (ROWS > 64 || warp < 2 || warp > 5)) {
         // ---------------- softmax of stream t: a thread per row
-        const int t = warp >> 2, row = (warp & 3) * 32 + lane;
+        const int t = warp >> 2, row = (warp & (F::kSoftmaxWarps - 1)) * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + t * 128 + lanes, tO = tmem + 256 + t * 128 + lanes;
         int done = 0;  // steps of this stream
@@ -322,14 +328,14 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 const float inv = a.sl2e < 0.f ? -kv8_inverse(stored) : kv8_inverse(stored);
                 // a row with an infinity or a NaN has no defined logit: NaN throughout
                 qs = bad ? __int_as_float(0x7fffffff) : kv8_power(stored) * fabsf(a.sl2e);
-                uint8_t* dst = sQ + (F::kQTiles == 1 ? 0 : t * kQTile) + row * 128;
+                uint8_t* dst = sQ + (F::kQTiles == 1 ? 0 : t * 2 * F::kQHalf) + row * 128;
 #pragma unroll
                 for (int v = 0; v < (F::kQTiles == 1 && t == 1 ? 0 : 16); ++v) {
                     const uint32_t w[4] = {u[v].x, u[v].y, u[v].z, u[v].w};
                     uint32_t f[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) f[e] = bad ? 0u : half2_of(bf16lo(w[e]) * inv, bf16hi(w[e]) * inv);
-                    *reinterpret_cast<uint4*>(dst + (v >> 3) * (kQTile / 2) + (((v & 7) ^ (row & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
+                    *reinterpret_cast<uint4*>(dst + (v >> 3) * F::kQHalf + (((v & 7) ^ (row & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
                 }
                 fence_proxy_async();
                 __syncwarp();
@@ -347,7 +353,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 uint32_t s[64], pairs[32];
                 tmem_ld64(tS + b * 64, s);
                 tmem_loaded(s);
-                const PageScale* info = sh.info[c % kInfo];
+                const PageScale* info = sh.info[c % F::kInfo];
                 float alpha;
                 if ((u + 1) * kStep - 1 > stream_first) softmax_step<true>(s, pairs, info, qs, u * kStep, lim, m, l, alpha);
                 else softmax_step<false>(s, pairs, info, qs, u * kStep, lim, m, l, alpha);
@@ -373,7 +379,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
             }
             if (own > 0 && ok) ok = wait_one(&sh.o_done[t][(done - 1) & 1], (done - 1) >> 1, a.err, 907);
             tc_fence_after();
-            const bool nan_seen = *reinterpret_cast<volatile int*>(&sh.nan_seen[item % kInfo]) != 0;
+            const bool nan_seen = *reinterpret_cast<volatile int*>(&sh.nan_seen[item % kItems]) != 0;
             // the row's sums, 32 dimensions at a time
             auto sums = [&](int part, uint32_t (&o)[32]) {
                 if (own > 0 && ok) {
@@ -401,71 +407,76 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
             };
             float scale0 = 1.f, scale1 = 0.f;  // FEW: factors of the streams' sums
             float* other = reinterpret_cast<float*>(sQ);  // FEW: stream 1's sums [dimension][row]
-            if (FEW) {
-                named_barrier(1, kSoftmaxThreads);  // both streams are done with Q
-                if (t == 1) {
-                    sh.ml[row] = make_float2(m, l);
-                    if (own > 0) {
-#pragma unroll 1
-                        for (int part = 0; part < 4; ++part) {
-                            uint32_t o[32];
-                            sums(part, o);
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) other[(part * 32 + e) * ROWS + row] = __uint_as_float(o[e]);
-                        }
-                    }
-                }
-                named_barrier(1, kSoftmaxThreads);
-                if (t == 0 && share.own(it, per_stream, 1) > 0) {
-                    const float2 x = sh.ml[row];
-                    const float M = fmaxf(m, x.x);
-                    scale0 = m == kNegInf ? 1.f : exp2_ftz(m - M);
-                    scale1 = x.x == kNegInf ? 1.f : exp2_ftz(x.x - M);
-                    l = l * scale0 + x.y * scale1;
-                    m = M;
-                }
-            }
             const bool joins = FEW && share.own(it, per_stream, 1) > 0;
             const int a0 = walk.cta0(), a1 = walk.cta1();
             // a CTA takes part in at most one item that it did not begin and one that it does not end
             const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (static_cast<int>(blockIdx.x) == a0);
             const int slot_row = FEW ? row : t * kRows + row;
-            if (!FEW || t == 0) {
+            auto store = [&](int part) {
+                uint32_t o[32];
+                sums(part, o);
                 const float inv = a0 != a1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-                if (a0 != a1 && live) *reinterpret_cast<float2*>(a.ws_ml + (slot * ROWS + slot_row) * 2) = make_float2(m, l);
-#pragma unroll 1
-                for (int part = 0; part < 4; ++part) {
-                    uint32_t o[32];
-                    sums(part, o);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        float x = __uint_as_float(o[e]);
-                        if (joins) x = x * scale0 + other[(part * 32 + e) * ROWS + row] * scale1;
-                        o[e] = __float_as_uint(x * inv);
-                    }
-                    if (!live) continue;
-                    if (a0 != a1) {
-                        // [group of four dimensions][row]: a warp's stores are next to each other
-                        float4* dst = reinterpret_cast<float4*>(a.ws_o + slot * ROWS * kHd) + part * 8 * ROWS + slot_row;
+                for (int e = 0; e < 32; ++e) {
+                    float x = __uint_as_float(o[e]);
+                    if (joins) x = x * scale0 + other[(part * 32 + e) % F::kJoinDims * ROWS + row] * scale1;
+                    o[e] = __float_as_uint(x * inv);
+                }
+                if (live && a0 != a1) {
+                    // [group of four dimensions][row]: a warp's stores are next to each other
+                    float4* dst = reinterpret_cast<float4*>(a.ws_o + slot * ROWS * kHd) + part * 8 * ROWS + slot_row;
 #pragma unroll
-                        for (int c = 0; c < 8; ++c)
-                            dst[c * ROWS] = make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]), __uint_as_float(o[4 * c + 2]),
-                                                 __uint_as_float(o[4 * c + 3]));
-                    } else {
-                        uint4* dst = reinterpret_cast<uint4*>(a.out + at + part * 32);
+                    for (int c = 0; c < 8; ++c)
+                        dst[c * ROWS] = make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]), __uint_as_float(o[4 * c + 2]),
+                                                    __uint_as_float(o[4 * c + 3]));
+                } else if (live) {
+                    uint4* dst = reinterpret_cast<uint4*>(a.out + at + part * 32);
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            uint32_t w[4];
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t w[4];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                w[e] = pack_bf16x2(__uint_as_float(o[8 * c + 2 * e]), __uint_as_float(o[8 * c + 2 * e + 1]));
-                            dst[c] = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
+                        for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(__uint_as_float(o[8 * c + 2 * e]), __uint_as_float(o[8 * c + 2 * e + 1]));
+                        dst[c] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                 }
-            }
+            };
             if (FEW) {
-                named_barrier(1, kSoftmaxThreads);  // stream 1's sums were read: Q may come
+                constexpr int kParts = F::kJoinDims / 32;  // at a time
+                named_barrier(1, kSoftmaxThreads);  // both streams are done with Q
+                if (t == 1) sh.ml[row] = make_float2(m, l);
+#pragma unroll 1
+                for (int part0 = 0; part0 < 4; part0 += kParts) {
+                    if (t == 1 && own > 0) {
+#pragma unroll 1
+                        for (int part = part0; part < part0 + kParts; ++part) {
+                            uint32_t o[32];
+                            sums(part, o);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) other[((part - part0) * 32 + e) * ROWS + row] = __uint_as_float(o[e]);
+                        }
+                    }
+                    named_barrier(1, kSoftmaxThreads);
+                    if (t == 0) {
+                        if (part0 == 0) {
+                            if (joins) {
+                                const float2 x = sh.ml[row];
+                                const float M = fmaxf(m, x.x);
+                                scale0 = m == kNegInf ? 1.f : exp2_ftz(m - M);
+                                scale1 = x.x == kNegInf ? 1.f : exp2_ftz(x.x - M);
+                                l = l * scale0 + x.y * scale1;
+                                m = M;
+                            }
+                            if (a0 != a1 && live) *reinterpret_cast<float2*>(a.ws_ml + (slot * ROWS + slot_row) * 2) = make_float2(m, l);
+                        }
+#pragma unroll 1
+                        for (int part = part0; part < part0 + kParts; ++part) store(part);
+                    }
+                    named_barrier(1, kSoftmaxThreads);  // stream 1's sums were read: the next ones or Q may come
+                }
+            } else {
+                if (a0 != a1 && live) *reinterpret_cast<float2*>(a.ws_ml + (slot * ROWS + slot_row) * 2) = make_float2(m, l);
+#pragma unroll 1
+                for (int part = 0; part < 4; ++part) store(part);
             }
             tc_fence_before();
             count += share.u1 - share.u0;
@@ -474,41 +485,37 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
         }
     } else if (warp < 12) {
         // ---------------- each step into f16 tiles: keys by one team of warps, values by the other
-        constexpr int kTeam = F::kConvertWarps;
-        // 64 rows: warps 2, 3, 6, 7 and 8 .. 11; else the latter
-        const int cw = kTeam == 2 ? warp - 8 : warp >= 8 ? warp - 4 : (warp & 1) + (warp >> 2) * 2, ct = (cw & (kTeam - 1)) * 32 + lane;
-        const bool keys = cw < kTeam;
-        constexpr int kUnits = 8 / kTeam;  // 16-byte units of keys of a thread and two pages, pairs of units of values of a thread
-        // keys: token, 16 dimensions of a half; the row is the token's place. Team of 4: a half of the dimensions each
-        const int k_tok = (ct >> 2) & 15, k_c = ct & 3, k_half = kTeam == 4 ? ct >> 6 : 0, k_place = k_tok % 8 / 2 * 4 + k_tok / 8 * 2 + k_tok % 2;
-        // values: 8 keys of a page (half v_b), group of four dimensions, page v_page or v_page + 2: eight lanes store
-        // to eight different 16-byte columns, and load with two to a bank
-        const int v_b = lane & 1, v_page = lane >> 2 & 1;
-        const int v_dq = (lane >> 1 & 1) | (lane >> 3) << 1 | (cw & (kTeam - 1)) << (kTeam == 4 ? 3 : 4);
-        constexpr int kGroups = kUnits / 2;  // of dimensions, 8 apart
-        int c = 0, taken[2] = {0, 0};
+        // 64 rows: stream 0's are warps 2 .. 5, stream 1's 8 .. 11; else the latter for both
+        const int cw = warp < 8 ? warp - 2 : warp - 8, ct = (cw & 1) * 32 + lane, mine = warp < 8 ? 0 : 1;
+        const bool keys = cw < 2;
+        // keys: token, 16 dimensions of each half; the row is the token's place
+        const int k_tok = ct >> 2, k_c = ct & 3, k_place = k_tok % 8 / 2 * 4 + k_tok / 8 * 2 + k_tok % 2;
+        // values: 8 keys of a page (half v_b), groups of four dimensions v_dq and v_dq + 8, pages v_page and v_page + 2:
+        // eight lanes store to eight different 16-byte columns, and load with two to a bank
+        const int v_b = lane & 1, v_page = lane >> 2 & 1, v_dq = (lane >> 1 & 1) | (lane >> 3) << 1 | (cw & 1) << 4;
+        constexpr int kUnits = 4;
+        int count = 0, taken[2] = {0, 0};
         while (ok) {
             const Share<FEW> share(walk);
             const Kv8Item& it = walk.it;
             const int first_lim = it.L - it.n + it.row0, last_lim = first_lim + it.rows - 1;
-            for (int u = share.u0; u < share.u1 && ok; ++u, ++c) {
-                const int raw = c % F::kRaw, t = FEW ? (u - share.u0) & 1 : 0;
-                const int st = F::stage(t, taken[t]), use = F::use(taken[t]);
+            for (int u = share.u0 + (F::kTeams == 2 ? mine : 0); u < share.u1 && ok; u += F::kTeams) {
+                const int t = FEW ? (u - share.u0) & 1 : 0, n = F::kTeams == 2 ? taken[t] : count + u - share.u0;
+                const int raw = F::slot(t, n), st = F::stage(t, taken[t]), use = F::use(taken[t]);
                 ++taken[t];
                 uint64_t* empty = keys ? &sh.k_empty[st] : &sh.v_empty[st];
-                ok = wait_two(&sh.raw_full[raw], c / F::kRaw, use == 0 ? &sh.raw_full[raw] : empty, use == 0 ? c / F::kRaw : use - 1, a.err, 908);
+                ok = wait_two(&sh.raw_full[raw], n / 2, use == 0 ? &sh.raw_full[raw] : empty, use == 0 ? n / 2 : use - 1, a.err, 908);
                 if (!ok) break;
                 const uint8_t* src = sRaw + raw * kPages * kKv8Bytes;
                 // The fence before a slot is given back puts its reads ahead of the copy that overwrites it: without, that copy
                 // overtook loads on their way (giving it back after the conversion instead: chunks 557 us, so 440).
                 if (keys) {
-                    constexpr int kHalves = 2 / (kTeam / 2);
-                    uint4 w[kPages][kHalves];
+                    uint4 w[kPages][2];
 #pragma unroll
                     for (int i = 0; i < kPages; ++i)
 #pragma unroll
-                        for (int x = 0; x < kHalves; ++x)
-                            w[i][x] = *reinterpret_cast<const uint4*>(src + i * kKv8Bytes + (k_half + x) * 1024 + k_tok * 64 + k_c * 16);
+                        for (int x = 0; x < 2; ++x)
+                            w[i][x] = *reinterpret_cast<const uint4*>(src + i * kKv8Bytes + x * 1024 + k_tok * 64 + k_c * 16);
                     fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh.raw_empty[raw]);
@@ -516,14 +523,14 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
 #pragma unroll
                     for (int i = 0; i < kPages; ++i)
 #pragma unroll
-                        for (int x = 0; x < kHalves; ++x) {
+                        for (int x = 0; x < 2; ++x) {
                             const int row = i * kPage + k_place;
                             uint32_t f[8];
                             e4m3x4_to_half(w[i][x].x, f[0], f[1]);
                             e4m3x4_to_half(w[i][x].y, f[2], f[3]);
                             e4m3x4_to_half(w[i][x].z, f[4], f[5]);
                             e4m3x4_to_half(w[i][x].w, f[6], f[7]);
-                            uint8_t* dst = kd + (k_half + x) * (kKTile / 2) + row * 128;
+                            uint8_t* dst = kd + x * (kKTile / 2) + row * 128;
                             *reinterpret_cast<uint4*>(dst + (((2 * k_c) ^ (row & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
                             *reinterpret_cast<uint4*>(dst + (((2 * k_c + 1) ^ (row & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
                         }
@@ -532,12 +539,12 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                     if (lane == 0) mbar_arrive(&sh.k_full[st]);
                     continue;
                 }
-                uint4 w[kUnits][2];  // pages v_page + 2 (i / kGroups), groups v_dq + 8 (i % kGroups)
+                uint4 w[kUnits][2];  // pages v_page + 2 (i / 2), groups v_dq + 8 (i % 2)
 #pragma unroll
                 for (int i = 0; i < kUnits; ++i)
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
-                        w[i][x] = *reinterpret_cast<const uint4*>(src + (v_page + 2 * (i / kGroups)) * kKv8Bytes + kKv8Values + (v_dq + 8 * (i % kGroups)) * 64 + v_b * 32 + x * 16);
+                        w[i][x] = *reinterpret_cast<const uint4*>(src + (v_page + 2 * (i / 2)) * kKv8Bytes + kKv8Values + (v_dq + 8 * (i % 2)) * 64 + v_b * 32 + x * 16);
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.raw_empty[raw]);
@@ -547,7 +554,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                     for (int i = 0; i < kUnits; ++i)
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            const int key = u * kStep + (v_page + 2 * (i / kGroups)) * kPage;
+                            const int key = u * kStep + (v_page + 2 * (i / 2)) * kPage;
                             uint32_t hidden = 0, seen = 0;
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
@@ -564,7 +571,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                             }
                             w[i][x] = make_uint4(y[0], y[1], y[2], y[3]);
                         }
-                    if (any) *reinterpret_cast<volatile int*>(&sh.nan_seen[item % kInfo]) = 1;
+                    if (any) *reinterpret_cast<volatile int*>(&sh.nan_seen[item % kItems]) = 1;
                     __threadfence_block();
                 }
 #pragma unroll
@@ -573,11 +580,11 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                     const uint32_t w1[4] = {w[i][1].x, w[i][1].y, w[i][1].z, w[i][1].w};
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        const int dim = (v_dq + 8 * (i % kGroups)) * 4 + x;
+                        const int dim = (v_dq + 8 * (i % 2)) * 4 + x;
                         uint32_t f[4];
                         e4m3x4_to_half(w0[x], f[0], f[1]);
                         e4m3x4_to_half(w1[x], f[2], f[3]);
-                        *reinterpret_cast<uint4*>(sV + st * kVTile + dim * 128 + (((2 * (v_page + 2 * (i / kGroups)) + v_b) ^ (dim & 7)) << 4)) =
+                        *reinterpret_cast<uint4*>(sV + st * kVTile + dim * 128 + (((2 * (v_page + 2 * (i / 2)) + v_b) ^ (dim & 7)) << 4)) =
                             make_uint4(f[0], f[1], f[2], f[3]);
                     }
                 }
@@ -585,6 +592,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.v_full[st]);
             }
+            count += share.u1 - share.u0;
             ++item;
             if (!walk.next(a, per_block)) break;
         }
@@ -593,7 +601,8 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
         constexpr uint32_t id_s = idesc_f16(kRows, kStep), id_o = idesc_f16(kRows, kHd);
         const int t = warp - 12;
         const bool lead = elect_lane();
-        const uint64_t dQ = umma_desc_sw128(smem_u32(sQ + (F::kQTiles == 1 ? 0 : t * kQTile))), dK = umma_desc_sw128(smem_u32(sK)), dV = umma_desc_sw128(smem_u32(sV));
+        // 64 rows: MMA rows 64 t and on are theirs, the others' sums nobody reads (whatever lies there in shared memory)
+        const uint64_t dQ = umma_desc_sw128(smem_u32(F::kQTiles == 1 ? sQ - t * F::kQHalf : sQ + t * 2 * F::kQHalf)), dK = umma_desc_sw128(smem_u32(sK)), dV = umma_desc_sw128(smem_u32(sV));
         const uint32_t tS = tmem + t * 128, tO = tmem + 256 + t * 128;
         int s_count = 0, p_count = 0, loaded = 0;  // S and PV issued so far, items in which the stream had any
         while (ok) {
@@ -613,7 +622,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                     const uint64_t k = dK + (st * kKTile >> 4);
 #pragma unroll
                     for (int x = 0; x < 8; ++x)  // 16 dimensions: 32 bytes; the second 64 lie in the other half tile
-                        umma_bf16(tS + b * 64, dQ + (((x >> 2) * (kQTile / 2) + (x & 3) * 32) >> 4),
+                        umma_bf16(tS + b * 64, dQ + (((x >> 2) * F::kQHalf + (x & 3) * 32) >> 4),
                                   k + (((x >> 2) * (kKTile / 2) + (x & 3) * 32) >> 4), id_s, x > 0 ? 1u : 0u);
                     umma_commit(&sh.s_full[t][b]);
                     umma_commit(&sh.k_empty[st]);
@@ -657,7 +666,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
         }
     } else if (warp == 14) {
         // ---------------- codes and scales of each step
-        int c = 0;
+        int c = 0, filled[2] = {0, 0};  // steps; of a team
         while (ok) {
             const Share<FEW> share(walk);
             const Kv8Item& it = walk.it;
@@ -666,7 +675,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
             const int pages = min(seen, share.u1 * kPages);
             // eight steps at a time: lane 4 s + p has page p of the s-th, the next eight's ids on their way
             int next = share.u0 * kPages + lane < pages ? table[share.u0 * kPages + lane] : 0;
-            if (lane == 0) sh.nan_seen[item % kInfo] = 0;  // last of an item that is done
+            if (lane == 0) sh.nan_seen[item % kItems] = 0;  // last of an item that is done
             for (int u0 = share.u0; u0 < share.u1 && ok; u0 += 8) {
                 const int page = u0 * kPages + lane;
                 int id = next;
@@ -680,11 +689,12 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 const PageScale scale = {kv8_power(sc & 0xff), static_cast<float>(static_cast<int>(sc >> 8) - 127), kv8_inverse(sc >> 8), 0.f};
                 const uint8_t* codes = a.kv8 + block * kKv8Bytes;
                 for (int s = 0; s < 8 && u0 + s < share.u1; ++s, ++c) {
-                    const int raw = c % F::kRaw;
-                    if (c >= F::kRaw) ok = ok && wait_one(&sh.raw_empty[raw], c / F::kRaw - 1, a.err, 908);
+                    const int t = F::kTeams == 2 ? (u0 + s - share.u0) & 1 : 0, n = filled[t], raw = F::slot(t, n);
+                    if (n >= 2) ok = ok && wait_one(&sh.raw_empty[raw], n / 2 - 1, a.err, 908);
                     if (!ok) break;
+                    ++filled[t];
                     // the scales go ahead of the barrier that the conversion, the MMAs and so the softmax wait for
-                    if (lane >> 2 == s) sh.info[c % kInfo][lane & 3] = scale;
+                    if (lane >> 2 == s) sh.info[c % F::kInfo][lane & 3] = scale;
                     __syncwarp();
                     // the bytes are expected before any of them comes
                     if (lane == 0) mbar_arrive_expect_tx(&sh.raw_full[raw], min(kPages, pages - (u0 + s) * kPages) * kKv8Bytes);
@@ -696,7 +706,8 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
             if (!walk.next(a, per_block)) break;
         }
         // after a wait that ran out: no copy is left on its way into the block's shared memory
-        for (int i = max(0, c - F::kRaw); i < c; ++i) wait_one(&sh.raw_full[i % F::kRaw], i / F::kRaw, a.err, 908);
+        for (int t = 0; t < F::kTeams; ++t)
+            for (int n = max(0, filled[t] - 2); n < filled[t]; ++n) wait_one(&sh.raw_full[F::slot(t, n)], n / 2, a.err, 908);
     }
     __syncthreads();
     if (warp == 12) {
