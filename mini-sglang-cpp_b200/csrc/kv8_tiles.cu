@@ -504,7 +504,11 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 const int raw = F::slot(t, n), st = F::stage(t, taken[t]), use = F::use(taken[t]);
                 ++taken[t];
                 uint64_t* empty = keys ? &sh.k_empty[st] : &sh.v_empty[st];
-                ok = wait_two(&sh.raw_full[raw], n / 2, use == 0 ? &sh.raw_full[raw] : empty, use == 0 ? n / 2 : use - 1, a.err, 908);
+                // With a team for each stream the codes are read as soon as they are there, ahead of their tile (their slots then come
+                // back earlier: 24 requests x 6 drafted rows 111 us, so 107). One team has not the registers (chunks 431 us, so 440).
+                constexpr bool kAhead = F::kTeams == 2;
+                const bool both = !kAhead && use > 0;
+                ok = wait_two(&sh.raw_full[raw], n / 2, both ? empty : &sh.raw_full[raw], both ? use - 1 : n / 2, a.err, 908);
                 if (!ok) break;
                 const uint8_t* src = sRaw + raw * kPages * kKv8Bytes;
                 // The fence before a slot is given back puts its reads ahead of the copy that overwrites it: without, that copy
@@ -519,6 +523,8 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                     fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh.raw_empty[raw]);
+                    if (kAhead && use > 0) ok = wait_one(empty, use - 1, a.err, 908);
+                    if (!ok) break;
                     uint8_t* kd = sK + st * kKTile;
 #pragma unroll
                     for (int i = 0; i < kPages; ++i)
@@ -574,6 +580,8 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                     if (any) *reinterpret_cast<volatile int*>(&sh.nan_seen[item % kItems]) = 1;
                     __threadfence_block();
                 }
+                if (kAhead && use > 0) ok = wait_one(empty, use - 1, a.err, 908);
+                if (!ok) break;
 #pragma unroll
                 for (int i = 0; i < kUnits; ++i) {
                     const uint32_t w0[4] = {w[i][0].x, w[i][0].y, w[i][0].z, w[i][0].w};
