@@ -818,7 +818,7 @@ attend_rows_kernel(const Kv8AttnArgs a) {
 // arrive joined it, one request at 4k took 20.5 us for 18.0 and 256 rows at 8k 133 for 75.
 // COLUMNS false (few rows, row after row): a warp per row, rows 8 y .. 8 y + 7 of every gridDim.y x 8, a lane per four
 // dimensions. COLUMNS true (four dimensions of all rows after each other): a lane per row, of 32 y .. 32 y + 31, four
-// such columns a warp; with row after row 256 rows' stores took 18 us a part (2048 rows of a prompt: 231 us, so XX).
+// such columns a warp; with row after row 256 rows' stores took 18 us a part.
 constexpr int kJoinWarps = 8;
 
 template <bool COLUMNS>

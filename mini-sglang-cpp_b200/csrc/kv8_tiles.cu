@@ -1,30 +1,33 @@
 // kv8_tiles.cu -- attention of many rows (chunks, drafted rows) over the 8-bit key / value pool, on tcgen05.
 //
 // Persistent: each CTA takes an equal part of the steps (64 keys) of all items (block of query rows x kv head;
-// rows = query rows x the group's heads); of items shared by CTAs they leave partial sums. Codes are converted to f16 (exactly) into the operands' canonical tiles, q is scaled to f16
-// by a power of two per row (2^-25 of its largest value). A page's scales enter the exponent:
-// s = (q . k) 2^(q + k exponents) scale log2(e) + (exponent of v), p = 2^(s - m) <= 2^8 in f16, so that O needs
-// no scaling by page, and l adds p 2^-(exponent of v).
+// rows = query rows x the group's heads); of items shared by CTAs they leave partial sums. Codes are converted to
+// f16 (exactly) into the operands' canonical tiles, q is scaled to f16 by a power of two per row (2^-25 of its
+// largest value). A page's scales enter the exponent: s = (q . k) 2^(q + k exponents) scale log2(e) + (exponent of v),
+// p = 2^(s - m) <= 2^8 in f16 (2^-11 of each), so that O needs no scaling by page, and l adds p 2^-(exponent of v).
 //
-// Two streams of 128 MMA rows each:
+// Two streams of up to 128 MMA rows each:
 //   FEW = false  blocks of 256 rows: the streams are its halves, and both take every step;
 //   FEW = true   blocks of up to 128 rows: both streams hold them and take every other step, joined at the
 //                item's end, so that one's softmax runs while the other's MMAs do.
-// Warps:
-//   0-3, 4-7   softmax of stream 0 / 1: a thread per row. S from tensor memory, p as f16 pairs over the first
-//              half of S, l and m in registers; O in tensor memory is rescaled only where the maximum grew by
+// Warps (those of 64 rows in brackets):
+//   0-3, 4-7   [0, 1, 6, 7] softmax of stream 0 / 1: a thread per row. S from tensor memory, p as f16 pairs over the
+//              first half of S, l and m in registers; O in tensor memory is rescaled only where the maximum grew by
 //              more than 8;
-//   8, 9       conversion of a step's keys to [64][128], 10, 11 of its values to [128][64], both K-major (the keys
-//              of a page in the order in which the pool stores their values);
+//   8, 9       [2, 3 of stream 0, 8, 9 of stream 1] conversion of a step's keys to [64][128],
+//   10, 11     [4, 5; 10, 11] of its values to [128][64], both K-major (the keys of a page in the order in which the
+//              pool stores their values);
 //   12, 13     one lane each issues a stream's MMAs: PV(i), then S(i + 2). S has two buffers of 64 columns, so that
 //              the next S is there before the softmax of a step ends; while one stream waits for a hand-over
 //              (100 to 400 clocks each) the other's MMAs run;
-//   14         page ids and scales, a bulk copy of 4 KB a page into a ring of two steps (loads by the
-//              converting warps held them up for half of their time).
+//   14         page ids and scales, a bulk copy of 4 KB a page into a ring of two steps [two of each stream] (loads by
+//              the converting warps held them up for half of their time).
 // Tensor memory: two S buffers a stream and O: 2 x (128 + 128) columns.
 //
-// Bound: chunks by the MMAs (4 x 128 FLOP a row and key), then by the softmax's and the conversion's
-// instructions; few rows by HBM (4 KB a page and head).
+// Bound: chunks by the softmax, whose two warps a scheduler take 1560 clocks a step (1024 of them exponentials) of
+// 2500, ahead of the MMAs' 1024; few rows by the chain from a step's copy over its conversion to its softmax, 1500
+// clocks a step where HBM would allow 700. Measured: two chunks of 2048 rows over 6k to 8k tokens, 32 / 8 heads, 430 us
+// (865 TFLOP/s); 24 requests x 6 rows over 5k to 20k tokens, 32 / 4 heads, 107 us (2.9 TB/s).
 #include <algorithm>
 
 #include "kv8.cuh"
@@ -44,8 +47,10 @@ constexpr int kThreads = 512;
 
 // The forms by the rows of a block. 256: the streams are its halves, and both take every step. 128, 64: both streams
 // hold the block and take every other step, joined at the item's end, so that one's softmax runs while the
-// other's MMAs do. With 64 rows half of the softmax warps would have none: they convert (the conversion of
-// four warps is what bounds few rows: 24 requests x 48 rows 145 us, with eight warps XX).
+// other's MMAs do. With 64 rows half of the softmax warps would have none: they convert, a team for each stream (one
+// team of eight warps took as long for a step as four for their own; 24 requests x 48 rows 145 us with four
+// warps, 123 with eight as one team, 111 as two). 32 requests over 4096 tokens: 64 rows 112 us, 68 (as 128) 133,
+// 128 rows 130, 132 (as 256) 172, 256 rows 180.
 template <int ROWS>
 struct Form {
     static constexpr bool kFew = ROWS <= 128;
