@@ -142,8 +142,9 @@ struct Kv8Walk {
 // Scratch of kv8_part.
 template <int THREADS>
 struct Kv8Scan {
-    int64_t warp_sums[THREADS / 32], before;
-    int first;
+    int64_t sums[THREADS / 32], first_sums[THREADS / 32], before;
+    Kv8Item item;
+    int found;
 };
 
 // Zeros for the first `rows` query rows from q0 on.
@@ -162,58 +163,69 @@ __device__ __forceinline__ bool kv8_part(const Kv8AttnArgs& a, int per_block, Kv
         const int units = kv8_units<UNIT>(L, n, row0, per_block);
         return units ? static_cast<int64_t>(units + COST) * a.hkv : 0;
     };
-    auto weight = [&](int r, bool report) {
-        int L, n, q0;
-        kv8_request(a, r, report, L, n, q0);
+    auto weight = [&](int r, bool report, Kv8Item& it) {  // and the request's context and rows
+        kv8_request(a, r, report, it.L, it.n, it.q0);
         int64_t s = 0;
-        for (int row0 = 0; row0 < n; row0 += per_block) s += block_weight(L, n, row0);
-        if (report && n > L) zero_rows(a, q0, n - L);
+        for (int row0 = 0; row0 < it.n; row0 += per_block) s += block_weight(it.L, it.n, row0);
+        if (report && it.n > it.L) zero_rows(a, it.q0, it.n - it.L);
         return s;
     };
-    int64_t mine = 0;
-    for (int r = tid; r < a.num_reqs; r += THREADS) mine += weight(r, blockIdx.x == 0);
+    // A thread has the weight of one request of the first THREADS, which is all that most calls have.
+    Kv8Item own{};
+    const int64_t first_weight = tid < a.num_reqs ? weight(tid, blockIdx.x == 0, own) : 0;
+    int64_t mine = first_weight, upto = first_weight;  // of all its requests; inclusive sum of a warp's first ones
+    for (int r = tid + THREADS; r < a.num_reqs; r += THREADS) {
+        Kv8Item other;
+        mine += weight(r, blockIdx.x == 0, other);
+    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if (lane == 0) sh.warp_sums[warp] = mine;
-    if (tid == 0) sh.first = -1;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+        mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    }
+    if (lane == 0) sh.sums[warp] = mine;
+    if (lane == 31) sh.first_sums[warp] = upto;
+    if (tid == 0) sh.found = 0;
     __syncthreads();
     int64_t total = 0;
 #pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) total += sh.warp_sums[w];
+    for (int w = 0; w < THREADS / 32; ++w) total += sh.sums[w];
     const int64_t per = larger((total + gridDim.x - 1) / gridDim.x, a.min_units), begin = per * blockIdx.x, end = smaller(total, begin + per);
     walk.per = per;
     walk.begin = begin;
     walk.end = end;
     bool any = begin < end;
     if (any) {
-        int64_t base = 0;
+        int64_t base = 0, w = first_weight;
         for (int r0 = 0; r0 < a.num_reqs; r0 += THREADS) {  // blocks of requests, until their sum passes `begin`
             const int r = r0 + tid;
-            const int64_t w = r < a.num_reqs ? weight(r, false) : 0;
-            int64_t x = w;
+            if (r0 > 0) {
+                w = upto = r < a.num_reqs ? weight(r, false, own) : 0;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= o) x += y;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += y;
+                }
+                if (lane == 31) sh.first_sums[warp] = upto;
+                __syncthreads();
             }
-            __syncthreads();
-            if (lane == 31) sh.warp_sums[warp] = x;
-            __syncthreads();
-            int64_t ahead = base;
+            int64_t ahead = base + upto - w;
             for (int v = 0; v < THREADS / 32; ++v) {
-                if (v < warp) ahead += sh.warp_sums[v];
-                base += sh.warp_sums[v];
+                if (v < warp) ahead += sh.first_sums[v];
+                base += sh.first_sums[v];
             }
-            if (w > 0 && begin >= ahead + x - w && begin < ahead + x) {
-                sh.first = r;
-                sh.before = ahead + x - w;
+            if (w > 0 && begin >= ahead && begin < ahead + w) {
+                own.r = r;
+                sh.item = own;
+                sh.before = ahead;
+                sh.found = 1;
             }
             __syncthreads();
-            if (sh.first >= 0) break;
+            if (sh.found) break;
         }
         // in the request: the row block, then the head
-        walk.it.r = sh.first;
-        kv8_request(a, walk.it.r, false, walk.it.L, walk.it.n, walk.it.q0);
+        walk.it = sh.item;
         int64_t at = sh.before;
         int rb = 0;
         for (int64_t w; (w = block_weight(walk.it.L, walk.it.n, rb * per_block)) <= begin - at; ++rb) at += w;
