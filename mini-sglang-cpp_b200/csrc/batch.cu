@@ -128,7 +128,8 @@ __global__ void decode_finish_kernel(const int* __restrict__ next_tokens, int* _
 // One cluster. Its first CTA does what hangs on the order: three scans over the requests (pages given
 // back, pages taken, rows) in one pass, then pages and rows are dealt to the threads by their place in
 // the scans, so that one long prompt among single tokens costs no serial walk. All CTAs fill positions
-// and slots. (A cluster of eight from 2048 rows on.)
+// and slots: one up to 2048 rows, else eight (64 requests x 16 rows 9.6 us, with eight 10.8; x 33 rows 10.2, with one 11.2;
+// 32k rows 12.0, with one 27.5).
 constexpr int kStepThreads = 1024;
 
 struct StepArgs {

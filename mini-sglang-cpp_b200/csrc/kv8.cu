@@ -1,7 +1,7 @@
 // kv8.cu -- append to the 8-bit key / value pool, and attention of single tokens and drafted rows over it.
 //
 //  * msgl_qknorm_rope_store_kv8 (+ _partials)  QK-norm + rotation + quantised append
-//  * msgl_paged_attention_kv8                  attention (long chunks: kv8_chunk.cu)
+//  * msgl_paged_attention_kv8                  attention (more than 16 rows x heads: kv8_tiles.cu)
 //
 // Format and conversions: kv8.cuh.
 #include <algorithm>
@@ -409,8 +409,9 @@ int launch_store(StoreArgs a, int head_dim, int page_size, msgl_stream_t stream)
         return set_error(MSGL_ERR_INVALID_ARG, "store_kv8: rows must be 16-byte aligned");
     const int64_t rows = std::min(a.max_q_len, a.num_tokens);
     a.page_tasks = static_cast<int>((rows + kPage - 2) / kPage + 1);
-    // Many tokens: four groups of query heads a warp, so that a block's loads cover its latency; few: one, for more blocks.
-    const int it = !a.parts && a.num_tokens >= 8 * 148 ? 4 : 1;
+    // Groups of query heads a warp: four, so that its loads cover their latency (256 tokens 5.3 us, with one 7.1, 8.2k 50 and 54);
+    // of partials one, whose sums have loads enough.
+    const int it = a.parts ? 1 : 4;
     a.q_groups = (a.hq + 15) / 16;
     const int64_t tasks = static_cast<int64_t>(a.num_reqs) * a.page_tasks * a.hkv * 2;
     const int64_t kv = (tasks + kStoreWarps / 2 - 1) / (kStoreWarps / 2);
@@ -420,8 +421,7 @@ int launch_store(StoreArgs a, int head_dim, int page_size, msgl_stream_t stream)
     a.kv_blocks = static_cast<int>(kv);
     a.err = device_error_word();
     if (!a.err) return set_error(MSGL_ERR_CUDA, "device error word unavailable");
-    launch_pdl(a.parts ? qknorm_rope_store_kv8_kernel<true, 1>
-                       : it == 4 ? qknorm_rope_store_kv8_kernel<false, 4> : qknorm_rope_store_kv8_kernel<false, 1>,
+    launch_pdl(a.parts ? qknorm_rope_store_kv8_kernel<true, 1> : qknorm_rope_store_kv8_kernel<false, 4>,
                dim3(static_cast<unsigned>(grid)), dim3(kStoreWarps * 32), 0, stream, a);
     MSGL_LAUNCH_CHECK();
     return MSGL_OK;
@@ -816,60 +816,91 @@ attend_rows_kernel(const Kv8AttnArgs a) {
 // Partial sums of the items that CTAs share, in the CTAs' order. Block (b, y): the item that CTA b goes on with, if
 // the CTA before it is the first; eight parts' loads in flight. A kernel of its own: where the last CTA of an item to
 // arrive joined it, one request at 4k took 20.5 us for 18.0 and 256 rows at 8k 133 for 75.
-// COLUMNS false (few rows, row after row): a warp per row, rows 8 y .. 8 y + 7 of every gridDim.y x 8, a lane per four
-// dimensions. COLUMNS true (four dimensions of all rows after each other): a lane per row, of 32 y .. 32 y + 31, four
-// such columns a warp; with row after row 256 rows' stores took 18 us a part.
+// COLUMNS false (up to 16 rows, row after row): a lane per four dimensions, rows 4 y .. 4 y + 3, two warps a row or
+// four where there are only two, each with its share of the parts, which add up through shared memory (one request
+// at 4k is 37 parts of two rows: a warp per row took 3.6 us more; blocks of two rows cost 64 requests 1.2 us, as most
+// items have few parts). COLUMNS true (four dimensions of all rows after each other): a lane per row, of 32 y ..
+// 32 y + 31, four such columns a warp; with row after row 256 rows' stores took 18 us a part.
 constexpr int kJoinWarps = 8;
+constexpr int kJoinRows = 4;  // COLUMNS false
+
+// Unnormalised sums over parts, relative to the maximum M.
+struct JoinSum {
+    float M, l;
+    float4 o;
+    __device__ __forceinline__ void scale(float f) {
+        l *= f;
+        o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+    }
+    __device__ __forceinline__ void add(float f, float l1, const float4& x) {
+        l += l1 * f;
+        o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
+    }
+};
 
 template <bool COLUMNS>
 __global__ void __launch_bounds__(kJoinWarps * 32)
 join_shared_kernel(const Kv8AttnArgs a, int slot_rows) {
+    __shared__ JoinSum split_sums[COLUMNS ? 1 : kJoinWarps][32];
     pdl_wait();
     pdl_trigger();
     const Kv8Shared s = a.ws_shared[blockIdx.x + 1];
     if (s.last < s.first || s.first != static_cast<int>(blockIdx.x)) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = a.hq / a.hkv;
-    const int turns = COLUMNS ? kHd / 4 / kJoinWarps : (s.rows + gridDim.y * kJoinWarps - 1) / (gridDim.y * kJoinWarps);
-    for (int turn = 0; turn < turns; ++turn) {
-        const int m = COLUMNS ? blockIdx.y * 32 + lane : (turn * gridDim.y + blockIdx.y) * kJoinWarps + warp;
+    const int row0 = blockIdx.y * (COLUMNS ? 32 : kJoinRows);
+    if (row0 >= s.rows) return;
+    const int at_once = s.rows - row0 > kJoinRows / 2 ? kJoinRows : kJoinRows / 2, step = COLUMNS ? 1 : kJoinWarps / at_once;
+    const int split = COLUMNS ? 0 : warp / at_once;
+    for (int turn = 0; turn < (COLUMNS ? kHd / 4 / kJoinWarps : 1); ++turn) {
+        const int m = row0 + (COLUMNS ? lane : warp % at_once);
         const int column = COLUMNS ? turn * kJoinWarps + warp : lane;  // four dimensions
-        if (m >= s.rows) continue;
+        if (COLUMNS && m >= s.rows) continue;
+        const bool live = m < s.rows;
         const int64_t at = COLUMNS ? static_cast<int64_t>(column) * slot_rows + m : static_cast<int64_t>(m) * (kHd / 4) + column;
-        float M = kNegInf, l = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int b0 = s.first; b0 <= s.last; b0 += 8) {
+        JoinSum sum = {kNegInf, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+        for (int b0 = s.first + split; live && b0 <= s.last; b0 += 8 * step) {
             float2 ml[8];
             float4 x[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int b = b0 + i;
+                const int b = b0 + i * step;
                 const int64_t slot = 2 * static_cast<int64_t>(b) + (b == s.first);
                 ml[i] = b <= s.last ? __ldcg(reinterpret_cast<const float2*>(a.ws_ml) + slot * slot_rows + m) : make_float2(kNegInf, 0.f);
                 x[i] = b <= s.last ? __ldcg(reinterpret_cast<const float4*>(a.ws_o) + slot * slot_rows * (kHd / 4) + at) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            float next = M;
+            float next = sum.M;
 #pragma unroll
             for (int i = 0; i < 8; ++i) next = fmaxf(next, ml[i].x);
-            const float f0 = M == kNegInf ? 1.f : exp2_ftz(M - next);
-            l *= f0;
-            o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
-            M = next;
+            sum.scale(sum.M == kNegInf ? 1.f : exp2_ftz(sum.M - next));
+            sum.M = next;
+            // a part without a visible key has l = 0 (or NaN where a NaN was seen)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                // a part without a visible key has l = 0 (or NaN where a NaN was seen)
-                const float f = ml[i].x == kNegInf ? 1.f : exp2_ftz(ml[i].x - M);
-                l += ml[i].y * f;
-                o.x += x[i].x * f; o.y += x[i].y * f; o.z += x[i].z * f; o.w += x[i].w * f;
+            for (int i = 0; i < 8; ++i) sum.add(ml[i].x == kNegInf ? 1.f : exp2_ftz(ml[i].x - next), ml[i].y, x[i]);
+        }
+        if (!COLUMNS) {
+            split_sums[COLUMNS ? 0 : warp][lane] = sum;
+            __syncthreads();
+            if (split > 0) return;
+            for (int i = 1; i < step; ++i) {
+                const JoinSum& y = split_sums[COLUMNS ? 0 : i * at_once + warp][lane];
+                const float next = fmaxf(sum.M, y.M);
+                sum.scale(sum.M == kNegInf ? 1.f : exp2_ftz(sum.M - next));
+                sum.add(y.M == kNegInf ? 1.f : exp2_ftz(y.M - next), y.l, y.o);
+                sum.M = next;
             }
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (!live) continue;
+        const float inv = sum.l == 0.f ? 0.f : 1.f / sum.l;
         *reinterpret_cast<uint2*>(a.out + ((s.q_row + m / group) * a.hq + s.h * group + m % group) * kHd + column * 4) =
-            make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+            make_uint2(pack_bf16x2(sum.o.x * inv, sum.o.y * inv), pack_bf16x2(sum.o.z * inv, sum.o.w * inv));
     }
 }
 
 // ------------------------------------------------------------------ host side
-// What each CTA goes on with, then the partial sums of two items a CTA.
+// The form by the rows of a block: the query rows of a request x the heads of a group, as long as one block holds them all
+// and so reads the keys once (32 requests over 4096 tokens, 32 / 8 heads: 8 rows 54 us, 16 rows 67, 20 rows, the
+// first on tcgen05, 110 as up to 64; larger ones in kv8_tiles.cu).
+// Workspace: what each CTA goes on with, then the partial sums of two items a CTA.
 struct RowsPlan {
     int rows;  // of a block: MMA rows
     int grid;
@@ -1041,7 +1072,7 @@ int msgl_paged_attention_kv8(const void* q, const void* kv8, const void* scales,
                                                           : launch_attend_tiles(a, p.rows, p.grid, stream);
     if (rc) return rc;
     const bool columns = p.rows > 16;
-    launch_pdl(columns ? join_shared_kernel<true> : join_shared_kernel<false>, dim3(p.grid - 1, columns ? p.rows / 32 : p.rows / kJoinWarps),
+    launch_pdl(columns ? join_shared_kernel<true> : join_shared_kernel<false>, dim3(p.grid - 1, columns ? p.rows / 32 : p.rows / kJoinRows),
                dim3(kJoinWarps * 32), 0, stream, a, p.rows);
     MSGL_LAUNCH_CHECK();
     return MSGL_OK;

@@ -17,7 +17,7 @@ namespace msgl {
 namespace {
 
 constexpr int kProbThreads = 512;
-constexpr int kProbPart = 20480;  // values of a row that a CTA holds, at most (80 KB, and as much for the next row)
+constexpr int kProbPart = 20480;  // values of a row that a CTA holds, at most (80 KB)
 constexpr int kMaxCluster = 16;
 constexpr float kNegInf = -__builtin_huge_valf();
 
@@ -380,11 +380,13 @@ verify_drafts_kernel(const VerifyArgs a) {
     cluster_wait();
 }
 
-// CTAs of a row or request: a power of two, enough for `fit`, doubled while the GPU has room.
+// CTAs of a row or request: a power of two, enough for `fit`, doubled while the GPU has room; 16 only where all of them
+// run at once: they find places more slowly (16 rows of probabilities 10.3 us as clusters of 8, 13.0 of 16; but 4 rows 10.0
+// and 7.2, one request's verification 11.5 and 7.5).
 int cluster_size(int64_t rows, int fit) {
     int c = 1;
     while (c < fit) c *= 2;
-    while (c < kMaxCluster && rows * c < 148) c *= 2;
+    while (c < kMaxCluster && rows * c < 148 && (c < 8 || rows * 16 <= 148)) c *= 2;
     return c;
 }
 
@@ -446,7 +448,8 @@ int msgl_verify_drafts(const float* target_probs, int64_t ldp, const float* draf
         return set_error(MSGL_ERR_INVALID_ARG, "verify_drafts: null pointer");
     const bool vec = vocab % 4 == 0 && ldp % 4 == 0 && aligned16(target_probs) &&
                      (!draft_probs || (ldq % 4 == 0 && aligned16(draft_probs)));
-    const int size = cluster_size(num_reqs, 1);
+    // four at least, for an even load of many requests: 256 81 us, with one each 107, with eight 99
+    const int size = cluster_size(num_reqs, 4);
     const int part = ((vocab + size - 1) / size + 127) / 128 * 128;
     static std::atomic<int> large4[kMaxDevices], large1[kMaxDevices];
     const cudaError_t e = size <= 8 ? cudaSuccess
