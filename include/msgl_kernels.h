@@ -441,7 +441,9 @@ MSGL_API int msgl_qknorm_rope_store_kv8_partials(const float* parts, int nparts,
  * rows outside total_q (skipped, site 901), a page outside the pool (page 0 in its place, site 902).
  * The workspace (msgl_paged_attention_kv8_workspace_size, 16-byte aligned) needs no clearing and serves
  * every call with no more rows a request of the same head counts, whatever their number and contexts;
- * calls that overlap on the GPU need one each. */
+ * calls that overlap on the GPU need one each. The form is chosen by max_q_len: give the chunks and the
+ * single tokens of a mixed batch in calls of their own (127 tokens over 2048 and a chunk of 512 rows over
+ * 4096, 32 / 8 heads: 380 us in one call, 165 in two). */
 MSGL_API size_t msgl_paged_attention_kv8_workspace_size(int max_q_len, int num_q_heads,
                                                         int num_kv_heads);
 MSGL_API int msgl_paged_attention_kv8(const void* q, const void* kv8, const void* scales,
