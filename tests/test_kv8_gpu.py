@@ -508,3 +508,63 @@ def test_workspace_serves_smaller_calls(cuda):
     for lens, rows in (([700, 20], [100, 3]), ([900] * 5, [1] * 5), ([50, 1200, 8], [8, 8, 8]), ([2000], [17])):
         a = Attend(lens, rows, 8, 2, seed=len(lens))
         a.check(a.call(workspace=ws))
+
+
+def test_many_short_requests_of_several_rows(cuda):
+    """Many items a CTA, short ones, in every tile form; a NaN that only later rows see in each of them."""
+    keys, values = places()
+    for rows, hq, hkv in ((9, 4, 2), (20, 16, 8), (70, 4, 2), (40, 16, 2)):
+        g = torch.Generator().manual_seed(rows)
+        lens = torch.randint(rows, rows + 50, (90,), generator=g).tolist()
+        a = Attend(lens, [rows] * 90, hq, hkv, seed=rows)
+        for r, n in enumerate(lens):
+            if r % 3 == 0:
+                a.kv8[int(a.table[r, (n - 2) // PAGE]), r % hkv, values[(n - 2) % PAGE, r % D]] = 0x7f
+        a.check(a.call())
+
+
+def test_pool_beyond_2_gib(cuda):
+    """Pages whose offsets pass 32 bits: the same bits as from a small pool."""
+    from msgl import ops
+    pages, hq, hkv = 70000, 16, 8  # 2.3 GB
+    far = torch.zeros(pages, hkv, 4096, dtype=torch.uint8, device="cuda")
+    far_scales = torch.zeros(pages, hkv, 2, dtype=torch.uint8, device="cuda")
+    for rows in (1, 8, 20, 60, 200):
+        a = Attend([400, 310], [rows] * 2, hq, hkv, seed=rows)
+        near = a.call()
+        n = len(a.kv8)
+        far[pages - n:], far_scales[pages - n:] = a.kv8, a.scales
+        a.kv8, a.scales, a.table = far, far_scales, a.table + (pages - n)
+        assert torch.equal(a.call(), near)
+    b = Append([100, 0], [30, 50], hq, hkv)
+    n, before = len(b.kv8), (b.kv8.clone(), b.scales.clone())
+    far[pages - n:], far_scales[pages - n:] = before
+    b.call()
+    want = b.kv8, b.scales
+    b.kv8, b.scales, b.table = far, far_scales, b.table + (pages - n)
+    b.call()
+    assert torch.equal(far[pages - n:], want[0]) and torch.equal(far_scales[pages - n:], want[1])
+    assert ops.device_error() == (0, 0)
+
+
+@pytest.mark.parametrize("rows", [1, 6, 40, 150])
+def test_two_streams_and_padding_rows(cuda, rows):
+    """Two calls at once, each with its workspace, on a stream of its own; rows behind the last request keep what they held."""
+    from msgl import ops
+    calls = [Attend([3000, 500, 1200], [rows] * 3, 16, 4, seed=21), Attend([900, 2500], [rows] * 2, 16, 4, seed=22)]
+    want = [a.call() for a in calls]
+    runs = []
+    torch.cuda.synchronize()
+    for a in calls:
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            q = torch.cat([a.q, torch.full((5, 16, D), float("nan"), device="cuda").bfloat16()])
+            runs.append((s, a, q, ints(a.lens), torch.full_like(q, 7.0), ops.attention_kv8_workspace(3, rows, 16, 4)))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, a, q, seq, out, ws in runs:
+            with torch.cuda.stream(s):
+                ops.paged_attention_kv8(q, a.kv8, a.scales, a.table, seq, max(a.lens), 16, 4, q_indptr=a.indptr, max_q_len=rows, workspace=ws, out=out)
+    torch.cuda.synchronize()
+    for (s, a, q, seq, out, ws), w in zip(runs, want):
+        assert torch.equal(out[:a.T], w) and bool((out[a.T:] == 7).all())
