@@ -26,8 +26,8 @@
 //
 // Bound: chunks by the softmax, whose two warps a scheduler take 1560 clocks a step (1024 of them exponentials) of
 // 2500, ahead of the MMAs' 1024; few rows by the chain from a step's copy over its conversion to its softmax, 1500
-// clocks a step where HBM would allow 700. Measured: two chunks of 2048 rows over 6k to 8k tokens, 32 / 8 heads, 430 us
-// (865 TFLOP/s); 24 requests x 6 rows over 5k to 20k tokens, 32 / 4 heads, 107 us (2.9 TB/s).
+// clocks a step where HBM would allow 700. Measured: two chunks of 2048 rows over 6k to 8k tokens, 32 / 8 heads, 424 us
+// (900 TFLOP/s); 24 requests x 6 rows over 5k to 20k tokens, 32 / 4 heads, 104 us (3.0 TB/s).
 #include <algorithm>
 
 #include "kv8.cuh"
@@ -519,34 +519,46 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 // The fence before a slot is given back puts its reads ahead of the copy that overwrites it: without, that copy
                 // overtook loads on their way (giving it back after the conversion instead: chunks 557 us, so 440).
                 if (keys) {
-                    uint4 w[kPages][2];
+                    const uint8_t* ks = src + k_tok * 64 + k_c * 16;
+                    uint8_t* kd = sK + st * kKTile + k_place * 128;
+                    const int to[2] = {((2 * k_c) ^ (k_place & 7)) << 4, ((2 * k_c + 1) ^ (k_place & 7)) << 4};
+                    auto codes = [&](int i, int x) { return *reinterpret_cast<const uint4*>(ks + i * kKv8Bytes + x * 1024); };
+                    auto convert = [&](int i, int x, const uint4& v) {
+                        uint32_t f[8];
+                        e4m3x4_to_half(v.x, f[0], f[1]);
+                        e4m3x4_to_half(v.y, f[2], f[3]);
+                        e4m3x4_to_half(v.z, f[4], f[5]);
+                        e4m3x4_to_half(v.w, f[6], f[7]);
+                        uint8_t* dst = kd + x * (kKTile / 2) + i * (kPage * 128);
+                        *reinterpret_cast<uint4*>(dst + to[0]) = make_uint4(f[0], f[1], f[2], f[3]);
+                        *reinterpret_cast<uint4*>(dst + to[1]) = make_uint4(f[4], f[5], f[6], f[7]);
+                    };
+                    // 128 rows: all codes first, so that their slot comes back early (130 us for 142, where two steps are all that
+                    // is on its way); else two pages at a time, less code at once (24 x 6 rows 107 us, so 104).
+                    if constexpr (ROWS == 128) {
+                        uint4 w[kPages][2];
 #pragma unroll
-                    for (int i = 0; i < kPages; ++i)
+                        for (int i = 0; i < kPages; ++i)
 #pragma unroll
-                        for (int x = 0; x < 2; ++x)
-                            w[i][x] = *reinterpret_cast<const uint4*>(src + i * kKv8Bytes + x * 1024 + k_tok * 64 + k_c * 16);
+                            for (int x = 0; x < 2; ++x) w[i][x] = codes(i, x);
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.raw_empty[raw]);
+#pragma unroll
+                        for (int i = 0; i < kPages; ++i)
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) convert(i, x, w[i][x]);
+                    } else {
+                        if (kAhead && use > 0) ok = wait_one(empty, use - 1, a.err, 908);
+                        if (!ok) break;
+#pragma unroll 2
+                        for (int i = 0; i < kPages; ++i)
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) convert(i, x, codes(i, x));
+                    }
                     fence_proxy_async();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.raw_empty[raw]);
-                    if (kAhead && use > 0) ok = wait_one(empty, use - 1, a.err, 908);
-                    if (!ok) break;
-                    uint8_t* kd = sK + st * kKTile;
-#pragma unroll
-                    for (int i = 0; i < kPages; ++i)
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const int row = i * kPage + k_place;
-                            uint32_t f[8];
-                            e4m3x4_to_half(w[i][x].x, f[0], f[1]);
-                            e4m3x4_to_half(w[i][x].y, f[2], f[3]);
-                            e4m3x4_to_half(w[i][x].z, f[4], f[5]);
-                            e4m3x4_to_half(w[i][x].w, f[6], f[7]);
-                            uint8_t* dst = kd + x * (kKTile / 2) + row * 128;
-                            *reinterpret_cast<uint4*>(dst + (((2 * k_c) ^ (row & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
-                            *reinterpret_cast<uint4*>(dst + (((2 * k_c + 1) ^ (row & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
-                        }
-                    fence_proxy_async();
-                    __syncwarp();
+                    if (ROWS != 128 && lane == 0) mbar_arrive(&sh.raw_empty[raw]);
                     if (lane == 0) mbar_arrive(&sh.k_full[st]);
                     continue;
                 }
