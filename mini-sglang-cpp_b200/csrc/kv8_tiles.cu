@@ -26,8 +26,8 @@
 //
 // Bound: chunks by the softmax, whose two warps a scheduler take 1560 clocks a step (1024 of them exponentials) of
 // 2500, ahead of the MMAs' 1024; few rows by the chain from a step's copy over its conversion to its softmax, 1500
-// clocks a step where HBM would allow 700. Measured: two chunks of 2048 rows over 6k to 8k tokens, 32 / 8 heads, 424 us
-// (900 TFLOP/s); 24 requests x 6 rows over 5k to 20k tokens, 32 / 4 heads, 104 us (3.0 TB/s).
+// clocks a step where HBM would allow 700. Measured: two chunks of 2048 rows over 6k to 8k tokens, 32 / 8 heads, 416 us
+// (920 TFLOP/s); 24 requests x 6 rows over 5k to 20k tokens, 32 / 4 heads, 104 us (3.0 TB/s).
 #include <algorithm>
 
 #include "kv8.cuh"
@@ -171,33 +171,52 @@ __device__ __forceinline__ void softmax_step(uint32_t (&s)[64], uint32_t (&out)[
             if (EDGE && key0 + p * kPage + token_at(i) > lim) s[p * kPage + i] = 0xff800000u;
             x[i] = __uint_as_float(s[p * kPage + i]);
         }
-        const float a = max3(max3(max3(x[0], x[1], x[2]), x[3], x[4]), x[5], x[6]);
-        const float b = max3(max3(max3(x[7], x[8], x[9]), x[10], x[11]), x[12], x[13]);
-        mx[p] = fmaf(fmaxf(max3(a, b, x[14]), x[15]), f[p], v_exp[p]);
+        const float a = max3(x[0], x[1], x[2]), b = max3(x[3], x[4], x[5]), c = max3(x[6], x[7], x[8]);
+        const float d = max3(x[9], x[10], x[11]), e = max3(x[12], x[13], x[14]);
+        mx[p] = fmaf(fmaxf(max3(a, b, c), max3(d, e, x[15])), f[p], v_exp[p]);
     }
     const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
     // The maximum moves only where it grows by more than 8: p stays below 2^8, which f16 holds as well.
     const float next = m == kNegInf || top > m + 8.f ? fmaxf(m, top) : m;
     const float base = next == kNegInf ? 0.f : next;
     alpha = next == m ? 1.f : exp2_ftz(m - next);
+    // Of each turn: the sums and f16 of the page before, this page's exponentials, the next one's exponents. The warp barrier
+    // keeps the turns apart for the compiler (chunks 424 us, so 416).
     float sum = 0.f;
+    uint64_t z[8], e[8];
 #pragma unroll
-    for (int p = 0; p < kPages; ++p) {
-        const uint64_t f2 = pair(f[p]), v2 = pair(v_exp[p] - base);
-        uint64_t part[2] = {0, 0};
+    for (int k = -1; k <= kPages; ++k) {
+        if (k >= 1) {  // the page before
+            const int p = k - 1;
+            uint64_t part[2] = {0, 0};
 #pragma unroll
-        for (int i = 0; i < kPage; i += 2) {
-            const int c = p * kPage + i;
-            float x, y;
-            unpair(fma2(pair(s[c], s[c + 1]), f2, v2), x, y);
-            x = exp2_ftz(x);
-            y = exp2_ftz(y);
-            part[i / 2 & 1] = add2(part[i / 2 & 1], pair(__float_as_uint(x), __float_as_uint(y)));
-            out[c / 2] = half2_of(x, y);
+            for (int i = 0; i < 8; ++i) {
+                float a, b;
+                part[i & 1] = add2(part[i & 1], e[i]);
+                unpair(e[i], a, b);
+                out[p * 8 + i] = half2_of(a, b);
+            }
+            float a, b;
+            unpair(add2(part[0], part[1]), a, b);
+            sum = fmaf(a + b, v_inv[p], sum);
         }
-        float a, b;
-        unpair(add2(part[0], part[1]), a, b);
-        sum = fmaf(a + b, v_inv[p], sum);
+        if (k >= 0 && k < kPages) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float x, y;
+                unpair(z[i], x, y);
+                x = exp2_ftz(x);
+                y = exp2_ftz(y);
+                e[i] = pair(__float_as_uint(x), __float_as_uint(y));
+            }
+        }
+        if (k + 1 < kPages) {
+            const int p = k + 1;
+            const uint64_t f2 = pair(f[p]), v2 = pair(v_exp[p] - base);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[i] = fma2(pair(s[p * 16 + 2 * i], s[p * 16 + 2 * i + 1]), f2, v2);
+        }
+        __syncwarp();
     }
     l = fmaf(l, alpha, sum);
     m = next;
