@@ -26,7 +26,7 @@ constexpr float kNegInf = -__builtin_huge_valf();
 // Lane 8 c + i: dimensions 8 i .. 8 i + 7 of one or both halves (keys: rotate-half partners) of the tokens 2 c, 2 c + 1
 // and / or 8 + 2 c, 9 + 2 c: rows are read in pieces of 128 bytes, value units written in 16. Keys are split over the
 // warps by tokens, values by dimensions; with one warp and 64 values a lane the kernel needed 162 registers and 8.5k
-// tokens took 79 us, so 50 (24 of them the append, 29 the query heads by themselves).
+// tokens took 79 us, so 50 (24 of them the append, 29 the query heads by themselves; 52 with near_middle below).
 // Query heads: eight lanes a head, as in the bf16 append.
 constexpr int kStoreWarps = 4;
 
@@ -145,6 +145,144 @@ __device__ __forceinline__ void norm_turn(float (&x)[16], const __nv_bfloat16* w
     }
 }
 
+// A value as h + l, and exact sums and products of fp32 values as such.
+struct Two {
+    float h, l;
+};
+__device__ __forceinline__ Two two_sum(float a, float b) {
+    const float s = __fadd_rn(a, b), t = __fsub_rn(s, a);
+    return {s, __fadd_rn(__fsub_rn(a, __fsub_rn(s, t)), __fsub_rn(b, t))};
+}
+__device__ __forceinline__ Two two_product(float a, float b) {
+    const float p = __fmul_rn(a, b);
+    return {p, fmaf(a, b, -p)};
+}
+
+// h + l rounded to the odd neighbour unless it is exact: rounding that to fewer bits is then right.
+__device__ __forceinline__ float odd_sum(float h, float l) {
+    const Two s = two_sum(h, l);
+    const uint32_t u = __float_as_uint(s.h);
+    if (!(fabsf(s.l) > 0.f) || (u & 1)) return s.h;
+    return __uint_as_float((s.l > 0.f) == (s.h > 0.f) ? u + 1 : u - 1);
+}
+
+// norm_turn of a key, rounded once at the end.
+__device__ __forceinline__ void norm_turn_exactly(float (&x)[16], const __nv_bfloat16* w, const float* turn, int i, float eps) {
+    Two part[4];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const Two p = two_product(x[e], x[e]), t = two_sum(e < 4 ? 0.f : part[e & 3].h, p.h);
+        part[e & 3] = {t.h, (e < 4 ? 0.f : part[e & 3].l) + (t.l + p.l)};
+    }
+    const Two s0 = two_sum(part[0].h, part[1].h), s1 = two_sum(part[2].h, part[3].h), all = two_sum(s0.h, s1.h);
+    Two ss = {all.h, (part[0].l + part[1].l) + (part[2].l + part[3].l) + (s0.l + s1.l) + all.l};
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+        const float h = __shfl_xor_sync(0xffffffffu, ss.h, o), l = __shfl_xor_sync(0xffffffffu, ss.l, o);
+        const Two t = two_sum(ss.h, h);
+        ss = {t.h, ss.l + l + t.l};
+    }
+    // 1 / sqrt(mean + eps): the fp32 value, and a step of Newton's method for the rest
+    const Two m = two_sum(ss.h / kHd, eps), v = two_sum(m.h, m.l + ss.l / kHd);
+    Two inv = {1.0f / sqrtf(v.h), 0.f};
+    const Two square = two_product(inv.h, inv.h);
+    inv.l = 0.5f * inv.h * (fmaf(-v.h, square.h, 1.f) - fmaf(v.h, square.l, v.l * square.h));
+    if (__any_sync(0xffffffffu, ss.h > 3.4e38f)) {  // squares beyond fp32: the sum once more, of x 2^-70
+        float s2 = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float y = x[e] * 0x1p-70f;
+            s2 += y * y;
+        }
+        s2 += __shfl_xor_sync(0xffffffffu, s2, 1);
+        s2 += __shfl_xor_sync(0xffffffffu, s2, 2);
+        s2 += __shfl_xor_sync(0xffffffffu, s2, 4);
+        if (ss.h > 3.4e38f) inv = {0x1p-70f / sqrtf(s2 / kHd), 0.f};
+    }
+    auto normed = [&](float y, float weight) {
+        Two g = two_product(inv.h, weight);
+        g.l = fmaf(inv.l, weight, g.l);
+        Two z = two_product(y, g.h);
+        z.l = fmaf(y, g.l, z.l);
+        return z;
+    };
+#pragma unroll
+    for (int v4 = 0; v4 < 2; ++v4) {
+        const float4 c4 = *reinterpret_cast<const float4*>(turn + 8 * i + 4 * v4), s4 = *reinterpret_cast<const float4*>(turn + kHalf + 8 * i + 4 * v4);
+        const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+        const uint2 w0 = *reinterpret_cast<const uint2*>(w + 8 * i + 4 * v4), w1 = *reinterpret_cast<const uint2*>(w + kHalf + 8 * i + 4 * v4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t a = e < 2 ? w0.x : w0.y, b = e < 2 ? w1.x : w1.y;
+            const Two lo = normed(x[4 * v4 + e], e & 1 ? bf16hi(a) : bf16lo(a)), hi = normed(x[8 + 4 * v4 + e], e & 1 ? bf16hi(b) : bf16lo(b));
+            auto turned = [&](const Two& y, float f, const Two& z, float g) {  // y f + z g
+                const Two p = two_product(y.h, f), q = two_product(z.h, g), t = two_sum(p.h, q.h);
+                return odd_sum(t.h, t.l + (p.l + q.l) + fmaf(y.l, f, z.l * g));
+            };
+            x[4 * v4 + e] = turned(lo, c[e], hi, -s[e]);
+            x[8 + 4 * v4 + e] = turned(lo, s[e], hi, c[e]);
+        }
+    }
+}
+
+// Where each step is rounded to fp32, a value that is within some 2^-23 of the middle of two codes may end on the wrong side:
+// one of 10^6. Tokens with a value that close (6 of its units; the bits behind the code tell) are computed again, exactly
+// but for one rounding, which is 1% of the warps' tokens: 8.5k tokens 52 us for 50, 240 rows behind 6 partials 9.3 for 8.8.
+// (All of them so: 60 and 14.3.) What is left, one of 10^7, are codes below 2^-6, whose middles lie elsewhere.
+__device__ __forceinline__ bool near_middle(float code) { return ((__float_as_uint(code) - 0x80000u + 6u) & 0xfffffu) <= 12u; }
+
+// 4 N values of a head row as sums of partials, to the odd neighbour: N float4 at at + step * v, three parts' loads in flight.
+template <int N>
+__device__ __forceinline__ void sum_exactly(const float* at, const int (&step)[N], int64_t stride, int nparts, float* x) {
+    float l[4 * N];
+#pragma unroll
+    for (int e = 0; e < 4 * N; ++e) x[e] = l[e] = 0.f;
+    for (int p = 0; p < nparts; p += 3) {
+        float4 f[3][N];
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+#pragma unroll
+            for (int v = 0; v < N; ++v)
+                f[q][v] = p + q < nparts ? *reinterpret_cast<const float4*>(at + (p + q) * stride + step[v]) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+#pragma unroll
+            for (int v = 0; v < N; ++v) {
+                const float y[4] = {f[q][v].x, f[q][v].y, f[q][v].z, f[q][v].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float z = __fsub_rn(y[e], l[4 * v + e]), t = __fadd_rn(x[4 * v + e], z);  // Kahan
+                    l[4 * v + e] = __fsub_rn(__fsub_rn(t, x[4 * v + e]), z);
+                    x[4 * v + e] = t;
+                }
+            }
+    }
+#pragma unroll
+    for (int e = 0; e < 4 * N; ++e) x[e] = odd_sum(x[e], -l[e]);
+}
+template <bool PARTS>
+__device__ __noinline__ void key_exactly(const void* src, int64_t stride, int nparts, const __nv_bfloat16* w, const float* turn, int i, float eps, float* y) {
+    float x[16];
+    if (PARTS) {
+        const int step[4] = {0, 4, kHalf, kHalf + 4};
+        sum_exactly<4>(static_cast<const float*>(src), step, stride, nparts, x);
+    } else {
+        const __nv_bfloat16* raw = static_cast<const __nv_bfloat16*>(src);
+        const uint4 u[2] = {*reinterpret_cast<const uint4*>(raw), *reinterpret_cast<const uint4*>(raw + kHalf)};
+        raw_values(u, x);
+    }
+    norm_turn_exactly(x, w, turn, i, eps);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) y[e] = fabsf(x[e]) < __builtin_huge_valf() ? x[e] : __int_as_float(0x7fffffff);
+}
+__device__ __noinline__ void values_exactly(const float* src, int64_t stride, int nparts, float* y) {
+    float x[8];
+    const int step[2] = {0, 4};
+    sum_exactly<2>(src, step, stride, nparts, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = fabsf(x[e]) < __builtin_huge_valf() ? x[e] : __int_as_float(0x7fffffff);
+}
+
 __device__ __forceinline__ const float* turn_row(const StoreArgs& a, int64_t row) {
     int pos = a.positions[row];
     if (static_cast<unsigned>(pos) >= static_cast<unsigned>(a.max_position)) {
@@ -261,6 +399,22 @@ __device__ __forceinline__ void append_keys(const StoreArgs& a, const PageTask& 
     const int stored = page_exponent(x, maxima, warp, lane);
     const float inv = kv8_inverse(stored);
 #pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        bool near = false;
+#pragma unroll
+        for (int d = 0; d < 16; ++d) near |= near_middle(x[16 * e + d] * inv);
+        if (some[e] && __any_sync(0xffffffffu, near)) {
+            const int nh = a.hq + 2 * a.hkv;
+            const int64_t row = p.row(t0 + e), at = (row * nh + a.hq + p.h) * kHd + 8 * i;
+            float y[16];
+            key_exactly<PARTS>(PARTS ? static_cast<const void*>(a.parts + at) : a.qkv + at, static_cast<int64_t>(a.num_tokens) * nh * kHd, a.nparts, a.kn,
+                               turn_row(a, row), i, a.eps, y);
+#pragma unroll
+            for (int d = 0; d < 16; ++d)
+                if (p.live(t0 + e)) x[16 * e + d] = y[d];
+        }
+    }
+#pragma unroll
     for (int e = 0; e < 2; ++e)
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
@@ -330,6 +484,21 @@ __device__ __forceinline__ void append_values(const StoreArgs& a, const PageTask
     }
     const int stored = page_exponent(x, maxima, warp, lane);
     const float inv = kv8_inverse(stored);
+    if (PARTS)  // (the others are bf16 as they stand)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int t = token_at(4 * c + e);
+            bool near = false;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) near |= near_middle(x[8 * e + d] * inv);
+            if (near && p.live(t)) {
+                float y[8];
+                values_exactly(a.parts + (p.row(t) * nh + head) * kHd + half + 8 * i, static_cast<int64_t>(a.num_tokens) * nh * kHd, a.nparts, y);
+#pragma unroll
+                for (int d = 0; d < 8; ++d) x[8 * e + d] = y[d];
+            }
+        }
+    __syncwarp();
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
         uint32_t w[4];
@@ -409,7 +578,7 @@ int launch_store(StoreArgs a, int head_dim, int page_size, msgl_stream_t stream)
         return set_error(MSGL_ERR_INVALID_ARG, "store_kv8: rows must be 16-byte aligned");
     const int64_t rows = std::min(a.max_q_len, a.num_tokens);
     a.page_tasks = static_cast<int>((rows + kPage - 2) / kPage + 1);
-    // Groups of query heads a warp: four, so that its loads cover their latency (256 tokens 5.3 us, with one 7.1, 8.2k 50 and 54);
+    // Groups of query heads a warp: four, so that its loads cover their latency (8.2k tokens 50 us, with one 54);
     // of partials one, whose sums have loads enough.
     const int it = a.parts ? 1 : 4;
     a.q_groups = (a.hq + 15) / 16;
