@@ -154,7 +154,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // One step of a row: 64 S columns into pairs of p. EDGE: keys behind `lim` do not count. The factor of a page
-// is positive (qs is), so the page's largest logit comes from its largest product.
+// is positive, so the page's largest logit comes from its largest product, and a masked one stays -inf: where the scales'
+// product underflows (a row of zeros over keys of zeros, scale 0) it is the smallest normal number in its place, which
+// makes logits of at most 2^-109 of the products.
 template <bool EDGE>
 __device__ __forceinline__ void softmax_step(uint32_t (&s)[64], uint32_t (&out)[32], const PageScale* info, float qs, int key0,
                                              int lim, float& m, float& l, float& alpha) {
@@ -162,7 +164,7 @@ __device__ __forceinline__ void softmax_step(uint32_t (&s)[64], uint32_t (&out)[
 #pragma unroll
     for (int p = 0; p < kPages; ++p) {
         const float4 sc = *reinterpret_cast<const float4*>(&info[p]);
-        f[p] = qs * sc.x;
+        f[p] = fmaxf(qs * sc.x, 0x1p-126f);
         v_exp[p] = sc.y;
         v_inv[p] = sc.z;
         float x[kPage];
@@ -350,8 +352,10 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 }
                 const int stored = max(1, min(253, static_cast<int>(__float_as_uint(amax) >> 23)));
                 const float inv = a.sl2e < 0.f ? -kv8_inverse(stored) : kv8_inverse(stored);
-                // a row with an infinity or a NaN has no defined logit: NaN throughout
-                qs = bad ? __int_as_float(0x7fffffff) : kv8_power(stored) * fabsf(a.sl2e);
+                // a row (or a scale) with an infinity or a NaN has no defined logit: NaN throughout, by its sum of weights
+                bad |= !(fabsf(a.sl2e) < __builtin_huge_valf());
+                qs = bad ? 0.f : kv8_power(stored) * fabsf(a.sl2e);
+                if (bad) l = __int_as_float(0x7fffffff);
                 uint8_t* dst = sQ + (F::kQTiles == 1 ? 0 : t * 2 * F::kQHalf) + row * 128;
 #pragma unroll
                 for (int v = 0; v < (F::kQTiles == 1 && t == 1 ? 0 : 16); ++v) {

@@ -1,0 +1,62 @@
+"""Attention over the 8-bit pool where factors underflow, against softmax in 64 bits
+(Attend.check of test_kv8_gpu.py and its tolerances: half a bf16 step, 2^-11 of each weight, fp32 logits)."""
+import pytest
+import torch
+
+from kv8_plain import D, PAGE, fill
+from test_kv8_gpu import Attend
+
+pytestmark = pytest.mark.gpu
+# rows of a request with 4 heads a group: warp MMAs of 8 and 16 rows, tcgen05 of 64, 128 and 256
+ROWS = [1, 2, 4, 6, 16, 30, 40, 150]
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_zero_queries_over_zero_keys(cuda, rows):
+    """Every logit is 0: the mean of the values that a row sees, the last pages' masked keys among them."""
+    a = Attend([rows + 75, rows, rows + 16], [rows] * 3, 8, 2, seed=rows)
+    pages = torch.arange(len(a.kv8), device="cuda")
+    fill(a.kv8, a.scales, pages, 0, torch.zeros(len(pages), 2, PAGE, D, device="cuda"))
+    for r, n in enumerate(a.lens):
+        a.hide(r, n)
+    a.q.zero_()
+    a.check(a.call())
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_some_zero_queries(cuda, rows):
+    """Zero rows among others, keys of any size."""
+    a = Attend([rows + 75, rows], [rows] * 2, 8, 2, seed=rows + 1)
+    pages = torch.arange(len(a.kv8), device="cuda")
+    keys = torch.randn(len(pages), 2, PAGE, D, generator=a.g, device="cuda", dtype=torch.float64)
+    fill(a.kv8, a.scales, pages, 0, keys * 2.0 ** torch.randint(-70, 2, (len(pages), 2, 1, 1), generator=a.g, device="cuda"))
+    for r, n in enumerate(a.lens):
+        a.hide(r, n)
+    a.q[::2, 1] = 0
+    a.q[0] = 0
+    a.check(a.call())
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_scale_zero(cuda, rows):
+    a = Attend([rows + 75, rows], [rows] * 2, 8, 2, seed=rows + 2)
+    a.check(a.call(scale=0.0), scale=0.0)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_scale_nan(cuda, rows):
+    a = Attend([rows + 75], [rows], 8, 2, seed=rows + 2)
+    assert bool(torch.isnan(a.call(scale=float("nan"))).all())
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_a_pool_that_was_only_cleared(cuda, rows):
+    """Zero codes and zero scale bytes (kv8_pool): zeros, whatever the query."""
+    from msgl import ops
+    a = Attend([rows + 75, rows], [rows] * 2, 8, 2, seed=rows + 3)
+    a.kv8, a.scales = ops.kv8_pool(len(a.kv8), 2)
+    for zero in (False, True):
+        if zero:
+            a.q.zero_()
+        out = a.call(out=torch.full_like(a.q, 7.0))
+        assert bool((out == 0).all())
