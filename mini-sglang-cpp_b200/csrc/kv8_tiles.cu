@@ -355,7 +355,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 // a row (or a scale) with an infinity or a NaN has no defined logit: NaN throughout, by its sum of weights
                 bad |= !(fabsf(a.sl2e) < __builtin_huge_valf());
                 qs = bad ? 0.f : kv8_power(stored) * fabsf(a.sl2e);
-                if (bad) l = __int_as_float(0x7fffffff);
+                if (bad && lim >= 0) l = __int_as_float(0x7fffffff);  // (a row before the context's first token sees nothing: zeros)
                 uint8_t* dst = sQ + (F::kQTiles == 1 ? 0 : t * 2 * F::kQHalf) + row * 128;
 #pragma unroll
                 for (int v = 0; v < (F::kQTiles == 1 && t == 1 ? 0 : 16); ++v) {

@@ -1,5 +1,7 @@
 """Attention over the 8-bit pool where factors underflow, against softmax in 64 bits
 (Attend.check of test_kv8_gpu.py and its tolerances: half a bf16 step, 2^-11 of each weight, fp32 logits)."""
+import math
+
 import pytest
 import torch
 
@@ -7,6 +9,7 @@ from kv8_plain import D, PAGE, fill
 from test_kv8_gpu import Attend
 
 pytestmark = pytest.mark.gpu
+NAN = float("nan")
 # rows of a request with 4 heads a group: warp MMAs of 8 and 16 rows, tcgen05 of 64, 128 and 256
 ROWS = [1, 2, 4, 6, 16, 30, 40, 150]
 
@@ -46,7 +49,7 @@ def test_scale_zero(cuda, rows):
 @pytest.mark.parametrize("rows", ROWS)
 def test_scale_nan(cuda, rows):
     a = Attend([rows + 75], [rows], 8, 2, seed=rows + 2)
-    assert bool(torch.isnan(a.call(scale=float("nan"))).all())
+    assert bool(torch.isnan(a.call(scale=NAN)).all())
 
 
 @pytest.mark.parametrize("rows", ROWS)
@@ -60,3 +63,18 @@ def test_a_pool_that_was_only_cleared(cuda, rows):
             a.q.zero_()
         out = a.call(out=torch.full_like(a.q, 7.0))
         assert bool((out == 0).all())
+
+
+@pytest.mark.parametrize("rows", [2, 6, 30, 80])
+@pytest.mark.parametrize("what", [NAN, math.inf])
+def test_bad_queries_before_the_context(cuda, rows, what):
+    """A row before its context's first token gives zeros whatever its query holds, and a NaN or infinite query of
+    another row gives NaN, on every call."""
+    kept = 4 if rows > 6 else 1
+    a = Attend([rows - kept, 90], [rows, rows], 8, 2, seed=rows + 5)
+    a.q[0, 1, 3], a.q[kept, 2, 5], a.q[2 * rows - 1, 7, 9] = what, what, what
+    for _ in range(20):
+        out = a.call(out=torch.full_like(a.q, 7.0))
+        assert bool((out[:kept] == 0).all())
+        bad = torch.isnan(out).all(-1)
+        assert bool(bad[kept, 2]) and bool(bad[2 * rows - 1, 7]) and int(bad.sum()) == 2 and int(torch.isnan(out).sum()) == 2 * D
