@@ -397,7 +397,8 @@ MSGL_API int msgl_paged_attention_pages(const void* q, const void* k_pool, const
  *          d / 64 * 1024 + t * 64 + d % 64, its value at
  *          2048 + d / 4 * 64 + t % 8 / 2 * 16 + d % 4 * 4 + t / 8 * 2 + t % 2;
  *   scales [num_pages, Hkv, 2] exponents of keys and values, 127 added;
- * both bytes, 16-byte aligned. A value is code * 2^(scale - 127).
+ * both bytes, 16-byte aligned. A value is code * 2^(scale - 127), scale in [31, 247] as the append stores
+ * it; pages that were only cleared (codes and scales of 0) hold zeros.
  *
  * Append: msgl_qknorm_rope_store_kv (positions index cos_sin_cache [max_position, 128]) with keys and
  * values quantised into the pages that each request's rows reach. Of each page, kv head and kind the

@@ -698,7 +698,7 @@ __device__ __forceinline__ void attend_page8(const uint8_t* page, uint32_t scale
             }
     }
     const float kscale = kv8_power(scale2 & 0xff);
-    const int vstored = (scale2 >> 8) & 0xff;
+    const int vstored = kv8_value_exponent(scale2);
     const float vexp = static_cast<float>(vstored - 127), vinv = kv8_inverse(vstored);
     float p[NT][4];
     bool moved = false;

@@ -37,6 +37,10 @@ __device__ __forceinline__ int kv8_exponent(float amax) {
 __device__ __forceinline__ float kv8_power(int stored) { return __uint_as_float(static_cast<uint32_t>(stored) << 23); }
 // 2^-(stored - 127), stored in [1, 253]
 __device__ __forceinline__ float kv8_inverse(int stored) { return __uint_as_float(static_cast<uint32_t>(254 - stored) << 23); }
+// The values' stored exponent of a page's two scale bytes, as the attention takes it. The append stores none below the
+// floor; a page that was only cleared (codes of 0, scale bytes of 0) counts as zeros at the floor: with 2^-127 its keys' weights
+// would not fit the sum.
+__device__ __forceinline__ int kv8_value_exponent(uint32_t scale2) { return max(kKv8Floor, static_cast<int>(scale2 >> 8 & 0xff)); }
 
 // Two e4m3 codes (the low 16 bits) as two halves, exactly.
 __device__ __forceinline__ uint32_t e4m3_to_half2(uint32_t codes) {

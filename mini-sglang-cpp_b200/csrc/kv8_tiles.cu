@@ -734,7 +734,8 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 }
                 const int64_t block = static_cast<int64_t>(id) * a.hkv + it.h;
                 const uint32_t sc = page < pages ? *reinterpret_cast<const uint16_t*>(a.scales + block * 2) : 0x7f7fu;
-                const PageScale scale = {kv8_power(sc & 0xff), static_cast<float>(static_cast<int>(sc >> 8) - 127), kv8_inverse(sc >> 8), 0.f};
+                const int v_stored = kv8_value_exponent(sc);
+                const PageScale scale = {kv8_power(sc & 0xff), static_cast<float>(v_stored - 127), kv8_inverse(v_stored), 0.f};
                 const uint8_t* codes = a.kv8 + block * kKv8Bytes;
                 for (int s = 0; s < 8 && u0 + s < share.u1; ++s, ++c) {
                     const int t = F::kTeams == 2 ? (u0 + s - share.u0) & 1 : 0, n = filled[t], raw = F::slot(t, n);

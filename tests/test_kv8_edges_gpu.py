@@ -78,3 +78,13 @@ def test_bad_queries_before_the_context(cuda, rows, what):
         assert bool((out[:kept] == 0).all())
         bad = torch.isnan(out).all(-1)
         assert bool(bad[kept, 2]) and bool(bad[2 * rows - 1, 7]) and int(bad.sum()) == 2 and int(torch.isnan(out).sum()) == 2 * D
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_pages_that_were_only_cleared(cuda, rows):
+    """Such pages among others: their keys count with logit 0, their values are 0."""
+    a = Attend([rows + 700, rows + 40], [rows] * 2, 8, 2, seed=rows + 4)
+    for r, column in ((0, 0), (0, 17), (0, 39), (1, 1)):
+        page = int(a.table[r, column])
+        a.kv8[page], a.scales[page] = 0, 0
+    a.check(a.call())
