@@ -602,8 +602,8 @@ int launch_store(StoreArgs a, int head_dim, int page_size, msgl_stream_t stream)
 // O^T += V^T P^T with 16 dimensions as M, 8 rows as N and the page's keys as K, where S's accumulators are
 // P^T's fragments as they stand. Codes are exact in f16; q is scaled by a power of two per row, which keeps
 // it to 2^-25 of the row's largest value; a page's scales enter the exponent,
-//   s = (q . k) 2^(q + k exponents) scale log2(e) + (exponent of v),  p = 2^(s - m) <= 2^8 in f16,
-// so that O needs no scaling by page, and l adds p 2^-(exponent of v). HBM bound: 4 KB a page and head,
+//   s = (q . k) 2^(q + k exponents) scale log2(e) + (exponent of v),  p = 2^(s - m + 11) in f16 (kv8.cuh),
+// so that O needs no scaling by page, and l adds p 2^-(11 + exponent of v). HBM bound: 4 KB a page and head,
 // 24 or 32 MMAs, 64 conversions.
 //
 // In a CTA the pages of an item go around the warps, each with a ring of 4 KB stages that a warp of its own
@@ -699,7 +699,7 @@ __device__ __forceinline__ void attend_page8(const uint8_t* page, uint32_t scale
     }
     const float kscale = kv8_power(scale2 & 0xff);
     const int vstored = kv8_value_exponent(scale2);
-    const float vexp = static_cast<float>(vstored - 127), vinv = kv8_inverse(vstored);
+    const float vexp = static_cast<float>(vstored - 127), vinv = kv8_inverse(vstored) * kKv8Unlift;
     float p[NT][4];
     bool moved = false;
     float alpha[NT];
@@ -714,8 +714,7 @@ __device__ __forceinline__ void attend_page8(const uint8_t* page, uint32_t scale
         float mx = fmaxf(fmaxf(p[t][0], p[t][1]), fmaxf(p[t][2], p[t][3]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        // The maximum moves only where it grows by more than 8: p stays below 2^8, which f16 holds as well.
-        const bool move = mx > st.m[t] + 8.f || st.m[t] == kNegInf;
+        const bool move = mx > st.m[t] + kKv8Lag || st.m[t] == kNegInf;
         const float next = move ? fmaxf(mx, st.m[t]) : st.m[t];
         alpha[t] = 1.f;
         if (move && next != kNegInf) {
@@ -723,7 +722,7 @@ __device__ __forceinline__ void attend_page8(const uint8_t* page, uint32_t scale
             moved = true;
         }
         st.m[t] = next;
-        const float base = next == kNegInf ? 0.f : next;
+        const float base = next == kNegInf ? 0.f : next - kKv8Lift;
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -749,8 +748,8 @@ __device__ __forceinline__ void attend_page8(const uint8_t* page, uint32_t scale
     uint32_t pb[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        pb[t][0] = pack_half2(p[t][0], p[t][1]);
-        pb[t][1] = pack_half2(p[t][2], p[t][3]);
+        pb[t][0] = half2_weights(p[t][0], p[t][1]);
+        pb[t][1] = half2_weights(p[t][2], p[t][3]);
     }
     uint32_t hidden = 0;  // 0x80 in the bytes of tokens that some live row does not see
     if (EDGE)
@@ -967,7 +966,7 @@ attend_rows_kernel(const Kv8AttnArgs a) {
                 o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
             }
             if (a0 == a1) {
-                const float inv = l == 0.f ? 0.f : 1.f / l;
+                const float inv = l == 0.f ? 0.f : kKv8Unlift / l;
                 *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(use.it.q0 + use.it.row0 + m / group) * a.hq + use.it.h * group + m % group) * kHd + d) =
                     make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
             } else {
@@ -1059,7 +1058,7 @@ join_shared_kernel(const Kv8AttnArgs a, int slot_rows) {
             }
         }
         if (!live) continue;
-        const float inv = sum.l == 0.f ? 0.f : 1.f / sum.l;
+        const float inv = sum.l == 0.f ? 0.f : kKv8Unlift / sum.l;
         *reinterpret_cast<uint2*>(a.out + ((s.q_row + m / group) * a.hq + s.h * group + m % group) * kHd + column * 4) =
             make_uint2(pack_bf16x2(sum.o.x * inv, sum.o.y * inv), pack_bf16x2(sum.o.z * inv, sum.o.w * inv));
     }

@@ -64,6 +64,19 @@ __device__ __forceinline__ float exp2_ftz(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Weights of the attention, in f16: p = 2^(s - m + kKv8Lift), s with the exponent of the page's values, m the row's running
+// maximum, which moves only where it grows by more than kKv8Lag, so that p <= 2^15. f16 rounds each weight by 2^-12 of itself
+// at most (a code carries a rounding of 2^-4 already) down to 2^-25 of the row's largest and flushes below 2^-36: behind a key
+// that takes nearly all of the weight, or in pages whose values are that much smaller, the others still count. With
+// p = 2^(s - m) <= 2^8 that began at 2^-14 (keys 20 octaves below a sink came out 3% off, 25 octaves lost). The sums of weights
+// stay in fp32, of 2^-kKv8Lift p.
+constexpr float kKv8Lift = 11.f, kKv8Lag = 4.f, kKv8Unlift = 0x1p-11f;
+// Two weights; where logits of millions differ by their own rounding, the largest f16 value.
+__device__ __forceinline__ uint32_t half2_weights(float lo, float hi) {
+    uint32_t h;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(hi), "f"(lo));
+    return h;
+}
 // Bytes of a word of codes that are NaN, as 0x80 each.
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 __device__ __forceinline__ int64_t larger(int64_t a, int64_t b) { return a > b ? a : b; }

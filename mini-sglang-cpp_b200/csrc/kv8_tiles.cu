@@ -4,7 +4,7 @@
 // rows = query rows x the group's heads); of items shared by CTAs they leave partial sums. Codes are converted to
 // f16 (exactly) into the operands' canonical tiles, q is scaled to f16 by a power of two per row (2^-25 of its
 // largest value). A page's scales enter the exponent: s = (q . k) 2^(q + k exponents) scale log2(e) + (exponent of v),
-// p = 2^(s - m) <= 2^8 in f16 (2^-11 of each), so that O needs no scaling by page, and l adds p 2^-(exponent of v).
+// p = 2^(s - m + 11) in f16 (kv8.cuh), so that O needs no scaling by page, and l adds p 2^-(11 + exponent of v).
 //
 // Two streams of up to 128 MMA rows each:
 //   FEW = false  blocks of 256 rows: the streams are its halves, and both take every step;
@@ -13,7 +13,7 @@
 // Warps (those of 64 rows in brackets):
 //   0-3, 4-7   [0, 1, 6, 7] softmax of stream 0 / 1: a thread per row. S from tensor memory, p as f16 pairs over the
 //              first half of S, l and m in registers; O in tensor memory is rescaled only where the maximum grew by
-//              more than 8;
+//              more than 4;
 //   8, 9       [2, 3 of stream 0, 8, 9 of stream 1] conversion of a step's keys to [64][128],
 //   10, 11     [4, 5; 10, 11] of its values to [128][64], both K-major (the keys of a page in the order in which the
 //              pool stores their values);
@@ -108,7 +108,7 @@ __device__ __forceinline__ bool wait_one(uint64_t* a, int use, int* err, int sit
 // Token of a page at place i of its order.
 __host__ __device__ constexpr int token_at(int i) { return (i % 4 / 2) * 8 + (i / 4) * 2 + i % 2; }
 
-// Scales of a page: keys' factor, values' exponent and inverse factor.
+// Scales of a page: keys' factor, values' exponent and inverse factor (of 2^-11 p).
 struct PageScale {
     float k, v_exp, v_inv, pad;
 };
@@ -178,9 +178,8 @@ __device__ __forceinline__ void softmax_step(uint32_t (&s)[64], uint32_t (&out)[
         mx[p] = fmaf(fmaxf(max3(a, b, c), max3(d, e, x[15])), f[p], v_exp[p]);
     }
     const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
-    // The maximum moves only where it grows by more than 8: p stays below 2^8, which f16 holds as well.
-    const float next = m == kNegInf || top > m + 8.f ? fmaxf(m, top) : m;
-    const float base = next == kNegInf ? 0.f : next;
+    const float next = m == kNegInf || top > m + kKv8Lag ? fmaxf(m, top) : m;
+    const float base = next == kNegInf ? 0.f : next - kKv8Lift;
     alpha = next == m ? 1.f : exp2_ftz(m - next);
     // Of each turn: the sums and f16 of the page before, this page's exponentials, the next one's exponents. The warp barrier
     // keeps the turns apart for the compiler (chunks 424 us, so 416).
@@ -196,7 +195,7 @@ __device__ __forceinline__ void softmax_step(uint32_t (&s)[64], uint32_t (&out)[
                 float a, b;
                 part[i & 1] = add2(part[i & 1], e[i]);
                 unpair(e[i], a, b);
-                out[p * 8 + i] = half2_of(a, b);
+                out[p * 8 + i] = half2_weights(a, b);
             }
             float a, b;
             unpair(add2(part[0], part[1]), a, b);
@@ -443,7 +442,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
             auto store = [&](int part) {
                 uint32_t o[32];
                 sums(part, o);
-                const float inv = a0 != a1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+                const float inv = a0 != a1 ? 1.f : l == 0.f ? 0.f : kKv8Unlift / l;
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
                     float x = __uint_as_float(o[e]);
@@ -735,7 +734,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 const int64_t block = static_cast<int64_t>(id) * a.hkv + it.h;
                 const uint32_t sc = page < pages ? *reinterpret_cast<const uint16_t*>(a.scales + block * 2) : 0x7f7fu;
                 const int v_stored = kv8_value_exponent(sc);
-                const PageScale scale = {kv8_power(sc & 0xff), static_cast<float>(v_stored - 127), kv8_inverse(v_stored), 0.f};
+                const PageScale scale = {kv8_power(sc & 0xff), static_cast<float>(v_stored - 127), kv8_inverse(v_stored) * kKv8Unlift, 0.f};
                 const uint8_t* codes = a.kv8 + block * kKv8Bytes;
                 for (int s = 0; s < 8 && u0 + s < share.u1; ++s, ++c) {
                     const int t = F::kTeams == 2 ? (u0 + s - share.u0) & 1 : 0, n = filled[t], raw = F::slot(t, n);

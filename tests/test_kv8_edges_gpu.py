@@ -1,11 +1,11 @@
-"""Attention over the 8-bit pool where factors underflow, against softmax in 64 bits
+"""Attention over the 8-bit pool where factors underflow or weights are far apart, against softmax in 64 bits
 (Attend.check of test_kv8_gpu.py and its tolerances: half a bf16 step, 2^-11 of each weight, fp32 logits)."""
 import math
 
 import pytest
 import torch
 
-from kv8_plain import D, PAGE, fill
+from kv8_plain import D, PAGE, fill, ints
 from test_kv8_gpu import Attend
 
 pytestmark = pytest.mark.gpu
@@ -88,3 +88,74 @@ def test_pages_that_were_only_cleared(cuda, rows):
         page = int(a.table[r, column])
         a.kv8[page], a.scales[page] = 0, 0
     a.check(a.call())
+
+
+def shared_pages(reqs, n, rows, seed):
+    """Requests over the same pages, so that each is one CTA's: every key zero, every value in [1, 1.5]."""
+    a = Attend([n], [rows], 8, 2, seed=seed)
+    need = -(-n // PAGE)
+    at = a.table[0, :need].long()
+    keys = torch.zeros(need, 2, PAGE, D, dtype=torch.float64, device="cuda")
+    values = 1 + torch.randint(0, 5, keys.shape, generator=a.g, device="cuda").double() / 8
+    a.at, a.keys, a.values = at, keys, values
+    a.table, a.lens, a.rows, a.T = a.table.expand(reqs, -1).contiguous(), [n] * reqs, [rows] * reqs, reqs * rows
+    a.q = torch.zeros(a.T, 8, D, device="cuda").bfloat16()
+    a.q[..., 0] = 8
+    a.indptr = ints([rows * i for i in range(reqs + 1)])
+    return a
+
+
+# reqs x rows: two CTAs an SM (296), one (148)
+SINKS = [(600, 1), (300, 4), (300, 6), (300, 20), (150, 50)]
+
+
+@pytest.mark.parametrize("reqs,rows", SINKS)
+@pytest.mark.parametrize("bits", [12.4, 16.4, 20.4, 24.4])
+@pytest.mark.parametrize("at", [0, 1500])
+def test_a_key_that_takes_the_weight(cuda, reqs, rows, bits, at):
+    """One key's logit is `bits` octaves above the others' and its value is 0 (an attention sink): the result is the
+    others' values with their small weights."""
+    n = 1900
+    a = shared_pages(reqs, n, rows, seed=rows)
+    a.keys[at // PAGE, :, at % PAGE, 0] = 20
+    a.values[at // PAGE, :, at % PAGE] = 0
+    fill(a.kv8, a.scales, a.at, 0, a.keys), fill(a.kv8, a.scales, a.at, 1, a.values)
+    a.hide(0, n)
+    scale = bits * math.log(2) / 160
+    out = a.call(scale=scale)
+    check_mean(a, out, n, scale)
+
+
+@pytest.mark.parametrize("reqs,rows", SINKS)
+@pytest.mark.parametrize("bits", [12, 18, 24])
+def test_a_value_that_sets_its_pages_scale(cuda, reqs, rows, bits):
+    """A value of 2^bits with hardly any weight: the page's other tokens and other pages count as before."""
+    n = 1900
+    a = shared_pages(reqs, n, rows, seed=rows)
+    a.keys[3, :, 1, 0] = -240
+    a.keys[3, :, 2, 0] = 0.75  # keeps the page's weights off the powers of two
+    a.values[3] = 0
+    a.values[3, :, 1] = 2.0 ** bits
+    fill(a.kv8, a.scales, a.at, 0, a.keys), fill(a.kv8, a.scales, a.at, 1, a.values)
+    a.hide(0, n)
+    scale = 0.07
+    check_mean(a, a.call(scale=scale), n, scale)
+
+
+def check_mean(a, out, n, scale):
+    """The definition for queries that are all the same, [1st row .. last] of each request. Weights: 2^-11 of each, and
+    2^-36 of the largest; a logit of x: fp32, 2^-17 |x|, twice (as much of a normalised weight)."""
+    m = a.rows[0]
+    for row in {0, m - 1}:
+        seen = n - m + row + 1
+        for h in range(2):
+            x = a.keys[:, h].reshape(-1, D)[:seen, 0] * 8 * scale
+            p = torch.softmax(x, 0)
+            v = a.values[:, h].reshape(-1, D)[:seen]
+            ref = p @ v
+            page = torch.exp2(a.scales[a.at, h, 1].double() - 127).repeat_interleave(PAGE)[:seen]
+            tiny = seen * 2.0 ** -36 * 448 * float((p * page).max())
+            tol = ref * 2 ** -8 + ref * (2 ** -11 + 2 ** -20 + 2 * float(x.abs().max()) * 2 ** -17) + tiny
+            got = out.view(len(a.lens), m, 2, 4, D)[:, row, h].double()
+            err = (got - ref).abs()
+            assert bool((err <= tol).all()), float((err / tol).max())
