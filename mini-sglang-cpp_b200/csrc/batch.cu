@@ -165,6 +165,7 @@ step_tables_kernel(const StepArgs a) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = cluster_ctarank(), size = cluster_nctarank();
     if (tid == 0) bad = 0;
+    __syncthreads();  // ahead of the threads that set it
     pdl_wait();
     pdl_trigger();
     if (rank == 0) {
