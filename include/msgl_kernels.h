@@ -248,7 +248,7 @@ MSGL_API int msgl_decode_advance_masked(const int* next_tokens, int* input_ids, 
  * So kept = accepted length drops rejected drafts, kept = new = 0 frees a finished request. Columns
  * given back keep their entries. All-or-nothing: with a stack that runs out (MSGL_ERR_WORKSPACE,
  * site 710) or over (site 713), lengths below 0 or above max_pages (site 711), more rows than
- * num_tokens (site 712) nothing is written. All arrays are device int32; page_table is
+ * num_tokens (site 712) nothing is written, nor with num_reqs 0. All arrays are device int32; page_table is
  * [num_reqs, max_pages]; num_tokens <= 2^20. Outputs must not be inputs. */
 MSGL_API int msgl_step_tables(const int* kept_lens, const int* new_lens, int* page_table,
                               int max_pages, int* held_pages, int* free_pages, int free_capacity,

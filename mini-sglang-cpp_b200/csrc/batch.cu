@@ -165,7 +165,6 @@ step_tables_kernel(const StepArgs a) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = cluster_ctarank(), size = cluster_nctarank();
     if (tid == 0) bad = 0;
-    __syncthreads();  // ahead of the threads that set it
     pdl_wait();
     pdl_trigger();
     if (rank == 0) {
@@ -174,17 +173,17 @@ step_tables_kernel(const StepArgs a) {
         // Requests [r0, r0 + 1024): inclusive sums of pages given, taken and rows into shared memory.
         auto load = [&](int r0) {
             const int r = r0 + tid;
-            int k = 0, n = 0, h = 0, need = 0;
+            int k = 0, n = 0, h = 0, need = 0, fault = 0;
             if (r < a.B) {
                 k = a.kept[r];
                 n = a.add[r];
                 h = a.held[r];
                 if (k < 0 || n < 0 || h < 0 || h > a.width ||
                     static_cast<int64_t>(k) + n > static_cast<int64_t>(a.width) * a.page) {
-                    atomicOr(&bad, 2);
+                    fault = 2;
                     k = n = h = 0;
                 } else if (n > a.tokens) {
-                    atomicOr(&bad, 4);
+                    fault = 4;
                     k = n = h = 0;
                 }
                 need = (k + n + a.page - 1) / a.page;
@@ -197,7 +196,8 @@ step_tables_kernel(const StepArgs a) {
                     const int y = __shfl_up_sync(0xffffffffu, x[v], o);
                     if (lane >= o) x[v] += y;
                 }
-            __syncthreads();  // the sums of the block before are no longer read
+            __syncthreads();  // the sums of the block before are no longer read, and `bad` is cleared
+            if (fault) atomicOr(&bad, fault);
             if (lane == 31)
 #pragma unroll
                 for (int v = 0; v < 3; ++v) warp_sums[v][warp] = x[v];
