@@ -245,8 +245,11 @@ MSGL_API int msgl_decode_advance_masked(const int* next_tokens, int* input_ids, 
  *   q_indptr [num_reqs + 1] = running sum of new_lens; last_idx[r] = its last row, -1 without rows;
  *   row i of request r: positions = kept + i, slot_mapping = its slot in the page pool; rows behind the
  *   last request, up to num_tokens: position 0, slot -1 (a padding token).
- * So kept = accepted length drops rejected drafts, kept = new = 0 frees a finished request. Columns
- * given back keep their entries. All-or-nothing: with a stack that runs out (MSGL_ERR_WORKSPACE,
+ * So kept = accepted length drops rejected drafts, kept = new = 0 frees a finished request that owns all
+ * its pages. Leading pages that it only borrows (msgl_radix_match: the prefix cache owns them, other
+ * requests may hold them too) must never be given back: kept stays at or above borrowed * page_size, at
+ * the end too (new = 0), which gives back the request's own pages; then the caller sets held_pages[r]
+ * to 0 and unlocks the prefix. Columns given back keep their entries. All-or-nothing: with a stack that runs out (MSGL_ERR_WORKSPACE,
  * site 710) or over (site 713), lengths below 0 or above max_pages (site 711), more rows than
  * num_tokens (site 712) nothing is written, nor with num_reqs 0. All arrays are device int32; page_table is
  * [num_reqs, max_pages]; num_tokens <= 2^20. Outputs must not be inputs. */
