@@ -367,9 +367,11 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0 && F::kQTiles == 2) mbar_arrive(&sh.q_full[t]);
-                if (lane == 0 && F::kQTiles == 1 && t == 0) {  // one tile for both
+                // One tile for both. Stream 1 is told of items in which it has steps: of the others nothing would hold back the next
+                // item's arrival until its MMA warp has met this phase, and a phase that passes unseen is taken for the one before.
+                if (lane == 0 && F::kQTiles == 1 && t == 0) {
                     mbar_arrive(&sh.q_full[0]);
-                    mbar_arrive(&sh.q_full[1]);
+                    if (share.own(it, per_stream, 1) > 0) mbar_arrive(&sh.q_full[1]);
                 }
             }
             for (int i = 0; i < own && ok; ++i, ++done) {
@@ -655,8 +657,6 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
         while (ok) {
             const Share<FEW> share(walk);
             const int own = share.own(walk.it, per_stream, t);
-            // one tile of Q for both streams: every phase of its barrier is met
-            if (F::kQTiles == 1 && own == 0) ok = wait_one(&sh.q_full[t], loaded, a.err, 905);
             auto issue_s = [&](int i) {  // S of the i-th own step into its buffer, which p of two steps before has left
                 if (i >= own || !ok) return;
                 const int n = FEW ? s_count : count + i, st = F::stage(t, n), use = F::use(n), b = s_count & 1;
@@ -708,7 +708,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                     __syncwarp();
                 }
             count += share.u1 - share.u0;
-            if (own > 0 || F::kQTiles == 1) ++loaded;
+            if (own > 0) ++loaded;
             if (!walk.next(a, per_block)) break;
         }
     } else if (warp == 14) {

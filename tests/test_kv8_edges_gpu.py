@@ -159,3 +159,17 @@ def check_mean(a, out, n, scale):
             got = out.view(len(a.lens), m, 2, 4, D)[:, row, h].double()
             err = (got - ref).abs()
             assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.parametrize("rows,hq,hkv", [(6, 64, 8), (12, 32, 8), (20, 8, 8)])
+def test_items_of_one_step_among_longer_ones(cuda, rows, hq, hkv):
+    """Blocks of up to 64 rows, whose second stream has no step in items of up to 64 keys: eight items a CTA, in every order of
+    one, two and three steps, the same bits each time."""
+    from msgl import ops
+    lens = [max(rows, [30, 64, 65, 40, 128, 50, 20, 150, 60][r * r % 9] + r % 5) for r in range(150)]
+    a = Attend(lens, [rows] * 150, hq, hkv, seed=rows)
+    out = a.call()
+    a.check(out)
+    for _ in range(60):
+        assert torch.equal(a.call(), out)
+    assert ops.device_error() == (0, 0)
