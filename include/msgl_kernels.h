@@ -186,7 +186,8 @@ MSGL_API int msgl_sample(const float* logits, int num_rows, int vocab, const flo
  * logits with the same stride): probs[r] = softmax(logits[r] / temperature[r]) in fp32
  * (temperature [num_rows] device, NULL: 1). A row with temperature <= 0 gets 1 at the first index
  * of its maximum and 0 elsewhere (the greedy row of msgl_sample). A row without any logit above
- * -inf gives zeros, one with a NaN or +inf gives NaN. vocab <= 327680. */
+ * -inf gives zeros, one with a NaN or +inf, or with a NaN for its temperature, gives NaN.
+ * vocab <= 327680. */
 MSGL_API int msgl_token_probs(const float* logits, int64_t ldx, int num_rows, int vocab,
                               const float* temperature, float* probs, int64_t ldp,
                               msgl_stream_t stream);

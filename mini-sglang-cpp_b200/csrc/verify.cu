@@ -122,7 +122,7 @@ token_probs_kernel(const float* logits, int64_t ldx, const float* __restrict__ t
         cluster_wait();  // no CTA leaves while its shared memory may be read
         return;
     }
-    const float c = fminf(1.4426950408889634f / T, 3.0e38f);
+    const float factor = 1.4426950408889634f / T, c = factor > 3.0e38f ? 3.0e38f : factor;  // (NaN stays)
     // Each thread against its own maximum: one reduction of (maximum, sum) pairs, and exponentials ahead of it.
     float own = kNegInf;
 #pragma unroll 4
