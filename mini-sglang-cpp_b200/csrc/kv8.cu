@@ -600,8 +600,7 @@ int launch_store(StoreArgs a, int head_dim, int page_size, msgl_stream_t stream)
 // The rows of a kv head (query row x head of its group, at most 8 NT of them) against its pages. MMAs
 // m16n8k16 in f16: S = Q K^T with the rows as M and the 16 keys of a page as two N tiles, then
 // O^T += V^T P^T with 16 dimensions as M, 8 rows as N and the page's keys as K, where S's accumulators are
-// P^T's fragments as they stand. Codes are exact in f16; q is scaled by a power of two per row, which keeps
-// it to 2^-25 of the row's largest value; a page's scales enter the exponent,
+// P^T's fragments as they stand. Codes are exact in f16; q is scaled by a power of two per row (kv8.cuh); a page's scales enter the exponent,
 //   s = (q . k) 2^(q + k exponents) scale log2(e) + (exponent of v),  p = 2^(s - m + 11) in f16 (kv8.cuh),
 // so that O needs no scaling by page, and l adds p 2^-(11 + exponent of v). HBM bound: 4 KB a page and head,
 // 24 or 32 MMAs, 64 conversions.
@@ -812,7 +811,7 @@ __device__ __forceinline__ void load_rows(const Kv8AttnArgs& a, const Kv8Item& i
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         const uint32_t bads = __ballot_sync(0xffffffffu, bad) >> (4 * g) & 0xfu;
-        const int stored = max(1, min(253, static_cast<int>(__float_as_uint(amax) >> 23)));
+        const int stored = kv8_query_exponent(amax);
         const float inv = kv8_inverse(stored);
         // a row with an infinity or a NaN has no defined logit: NaN throughout
         st.qs[t] = bads ? __int_as_float(0x7fffffff) : kv8_power(stored) * a.sl2e;

@@ -64,6 +64,10 @@ __device__ __forceinline__ float exp2_ftz(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Queries of the attention, in f16: a row over 2^(this - 127), which puts its largest element into [2^14, 2^15) (up to 65280
+// next to bf16's largest, less below 2^-112): f16 holds it exactly down to 2^-31 of that, and to 2^-39 behind. (Into [1, 2): to
+// 2^-17 and 2^-25, which shows where the largest element meets zeros.) Sums of products with codes stay below 2^32.
+__device__ __forceinline__ int kv8_query_exponent(float amax) { return max(1, min(239, static_cast<int>(__float_as_uint(amax) >> 23) - 14)); }
 // Weights of the attention, in f16: p = 2^(s - m + kKv8Lift), s with the exponent of the page's values, m the row's running
 // maximum, which moves only where it grows by more than kKv8Lag, so that p <= 2^15. f16 rounds each weight by 2^-12 of itself
 // at most (a code carries a rounding of 2^-4 already) down to 2^-25 of the row's largest and flushes below 2^-36: behind a key

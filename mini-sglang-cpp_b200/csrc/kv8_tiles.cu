@@ -2,8 +2,7 @@
 //
 // Persistent: each CTA takes an equal part of the steps (64 keys) of all items (block of query rows x kv head;
 // rows = query rows x the group's heads); of items shared by CTAs they leave partial sums. Codes are converted to
-// f16 (exactly) into the operands' canonical tiles, q is scaled to f16 by a power of two per row (2^-25 of its
-// largest value). A page's scales enter the exponent: s = (q . k) 2^(q + k exponents) scale log2(e) + (exponent of v),
+// f16 (exactly) into the operands' canonical tiles, q is scaled to f16 by a power of two per row (kv8.cuh). A page's scales enter the exponent: s = (q . k) 2^(q + k exponents) scale log2(e) + (exponent of v),
 // p = 2^(s - m + 11) in f16 (kv8.cuh), so that O needs no scaling by page, and l adds p 2^-(11 + exponent of v).
 //
 // Two streams of up to 128 MMA rows each:
@@ -349,7 +348,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                         bad |= finite2(w[e]) != w[e];
                     }
                 }
-                const int stored = max(1, min(253, static_cast<int>(__float_as_uint(amax) >> 23)));
+                const int stored = kv8_query_exponent(amax);
                 const float inv = a.sl2e < 0.f ? -kv8_inverse(stored) : kv8_inverse(stored);
                 // a row (or a scale) with an infinity or a NaN has no defined logit: NaN throughout, by its sum of weights
                 bad |= !(fabsf(a.sl2e) < __builtin_huge_valf());

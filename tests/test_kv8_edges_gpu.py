@@ -173,3 +173,24 @@ def test_items_of_one_step_among_longer_ones(cuda, rows, hq, hkv):
     for _ in range(60):
         assert torch.equal(a.call(), out)
     assert ops.device_error() == (0, 0)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("big", [2.0 ** 12, 2.0 ** 20, -3e38])
+def test_a_large_query_element_that_meets_zeros(cuda, rows, big):
+    """Dimension 77 of every key is 0: the row's other elements, which are that much smaller, make its logits."""
+    a = Attend([rows + 300, rows], [rows] * 2, 8, 2, seed=rows + 6)
+    pages = torch.arange(len(a.kv8), device="cuda")
+    keys = torch.randn(len(pages), 2, PAGE, D, generator=a.g, device="cuda", dtype=torch.float64) * 2
+    keys[..., 77] = 0
+    fill(a.kv8, a.scales, pages, 0, keys)
+    for r, n in enumerate(a.lens):
+        a.hide(r, n)
+    if abs(big) > 1e30:
+        a.q = (a.q.float() * 2.0 ** 100).bfloat16()
+    a.q[..., 77] = big
+    scale = 0.1 if abs(big) < 1e30 else 0.1 * 2.0 ** -100
+    out = a.call(scale=scale)
+    a.check(out, scale=scale)
+    a.q = -a.q
+    assert torch.equal(a.call(scale=-scale), out)
