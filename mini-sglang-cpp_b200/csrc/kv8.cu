@@ -26,12 +26,9 @@ constexpr float kNegInf = -__builtin_huge_valf();
 // Lane 8 c + i: dimensions 8 i .. 8 i + 7 of one or both halves (keys: rotate-half partners) of the tokens 2 c, 2 c + 1
 // and / or 8 + 2 c, 9 + 2 c: rows are read in pieces of 128 bytes, value units written in 16. Keys are split over the
 // warps by tokens, values by dimensions; with one warp and 64 values a lane the kernel needed 162 registers and 8.5k
-// tokens took 79 us, so 50 (24 of them the append, 29 the query heads by themselves; 52 with near_middle below).
+// tokens took 79 us, so 50 (24 of them the append, 29 the query heads by themselves; 53 with near_middle below).
 // Query heads: eight lanes a head, as in the bf16 append.
 constexpr int kStoreWarps = 4;
-
-// Token of a page at place i of its values' order.
-__device__ __forceinline__ int token_at(int i) { return (i % 4 / 2) * 8 + (i / 4) * 2 + i % 2; }
 
 struct StoreArgs {
     const __nv_bfloat16* qkv;
@@ -227,8 +224,8 @@ __device__ __forceinline__ void norm_turn_exactly(float (&x)[16], const __nv_bfl
 
 // Where each step is rounded to fp32, a value that is within some 2^-23 of the middle of two codes may end on the wrong side:
 // one of 10^6. Tokens with a value that close (6 of its units; the bits behind the code tell) are computed again, exactly
-// but for one rounding, which is 1% of the warps' tokens: 8.5k tokens 52 us for 50, 240 rows behind 6 partials 9.3 for 8.8.
-// (All of them so: 60 and 14.3.) What is left, one of 10^7, are codes below 2^-6, whose middles lie elsewhere.
+// but for one rounding, which is 1% of the warps' tokens: 8.5k tokens 4% more time, 240 rows behind 6 partials 6%.
+// (All of them so: 20% and 60%.) What is left, one of 10^7, are codes below 2^-6, whose middles lie elsewhere.
 __device__ __forceinline__ bool near_middle(float code) { return ((__float_as_uint(code) - 0x80000u + 6u) & 0xfffffu) <= 12u; }
 
 // 4 N values of a head row as sums of partials, to the odd neighbour: N float4 at at + step * v, three parts' loads in flight.
@@ -336,7 +333,8 @@ __device__ __forceinline__ bool find_page(const StoreArgs& a, int task, bool rep
 }
 
 // The exponent of the page's values, of which the two warps of a pair hold 32 a lane each; NaN and infinities become
-// NaN and do not count.
+// NaN and do not count. (A maximum within fp32's rounding of 448 2^e may take the exponent next to the definition's, one page of
+// 10^6: e4m3 of either scale is the same but for subnormals.)
 __device__ __forceinline__ int page_exponent(float (&x)[32], float* maxima, int warp, int lane) {
     float amax = 0.f;
 #pragma unroll
@@ -629,11 +627,6 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 template <int NT>
@@ -1065,8 +1058,8 @@ join_shared_kernel(const Kv8AttnArgs a, int slot_rows) {
 
 // ------------------------------------------------------------------ host side
 // The form by the rows of a block: the query rows of a request x the heads of a group, as long as one block holds them all
-// and so reads the keys once (32 requests over 4096 tokens, 32 / 8 heads: 8 rows 54 us, 16 rows 67, 20 rows, the
-// first on tcgen05, 110 as up to 64; larger ones in kv8_tiles.cu).
+// and so reads the keys once (32 requests over 4096 tokens, 32 / 8 heads: 8 rows 54 us, 16 rows 66, 20 rows, the
+// first on tcgen05, 102 as up to 64; larger ones in kv8_tiles.cu).
 // Workspace: what each CTA goes on with, then the partial sums of two items a CTA.
 struct RowsPlan {
     int rows;  // of a block: MMA rows

@@ -42,6 +42,9 @@ __device__ __forceinline__ float kv8_inverse(int stored) { return __uint_as_floa
 // would not fit the sum.
 __device__ __forceinline__ int kv8_value_exponent(uint32_t scale2) { return max(kKv8Floor, static_cast<int>(scale2 >> 8 & 0xff)); }
 
+// Token of a page at place i of its values' order.
+__host__ __device__ constexpr int token_at(int i) { return (i % 4 / 2) * 8 + (i / 4) * 2 + i % 2; }
+
 // Two e4m3 codes (the low 16 bits) as two halves, exactly.
 __device__ __forceinline__ uint32_t e4m3_to_half2(uint32_t codes) {
     uint32_t h;
@@ -59,10 +62,9 @@ __device__ __forceinline__ uint32_t e4m3_codes2(float x0, float x1) {
     return __nv_cvt_float2_to_fp8x2(make_float2(x0, x1), __NV_SATFINITE, __NV_E4M3);
 }
 
-__device__ __forceinline__ float exp2_ftz(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
 // Queries of the attention, in f16: a row over 2^(this - 127), which puts its largest element into [2^14, 2^15) (up to 65280
 // next to bf16's largest, less below 2^-112): f16 holds it exactly down to 2^-31 of that, and to 2^-39 behind. (Into [1, 2): to

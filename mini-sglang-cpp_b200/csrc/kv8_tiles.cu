@@ -25,8 +25,8 @@
 //
 // Bound: chunks by the softmax, whose two warps a scheduler take 1560 clocks a step (1024 of them exponentials) of
 // 2500, ahead of the MMAs' 1024; few rows by the chain from a step's copy over its conversion to its softmax, 1500
-// clocks a step where HBM would allow 700. Measured: two chunks of 2048 rows over 6k to 8k tokens, 32 / 8 heads, 416 us
-// (920 TFLOP/s); 24 requests x 6 rows over 5k to 20k tokens, 32 / 4 heads, 104 us (3.0 TB/s).
+// clocks a step where HBM would allow 700. Measured: two chunks of 2048 rows over 6k to 8k tokens, 32 / 8 heads, 417 to 424
+// us (905 to 920 TFLOP/s); 24 requests x 6 rows over 5k to 20k tokens, 32 / 4 heads, 107 us (3.0 TB/s).
 #include <algorithm>
 
 #include "kv8.cuh"
@@ -47,9 +47,9 @@ constexpr int kThreads = 512;
 // The forms by the rows of a block. 256: the streams are its halves, and both take every step. 128, 64: both streams
 // hold the block and take every other step, joined at the item's end, so that one's softmax runs while the
 // other's MMAs do. With 64 rows half of the softmax warps would have none: they convert, a team for each stream (one
-// team of eight warps took as long for a step as four for their own; 24 requests x 48 rows 145 us with four
-// warps, 123 with eight as one team, 111 as two). 32 requests over 4096 tokens: 64 rows 112 us, 68 (as 128) 133,
-// 128 rows 130, 132 (as 256) 172, 256 rows 180.
+// team of eight warps took as long for a step as four for their own: 24 requests x 48 rows 18% less time with
+// eight in place of four, 10% less again as two teams). 32 requests over 4096 tokens: 64 rows 104 us, 68 (as 128) 126,
+// 128 rows 135, 132 (as 256) 169, 256 rows 182.
 template <int ROWS>
 struct Form {
     static constexpr bool kFew = ROWS <= 128;
@@ -78,10 +78,6 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {  // A, B f16 K-
     return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
-__device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
 __device__ __forceinline__ bool elect_lane() {
     uint32_t e;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
@@ -103,9 +99,6 @@ __device__ __forceinline__ bool wait_two(uint64_t* a, int use_a, uint64_t* b, in
 __device__ __forceinline__ bool wait_one(uint64_t* a, int use, int* err, int site) {
     return __all_sync(0xffffffffu, mbar_wait(a, use & 1, err, site));
 }
-
-// Token of a page at place i of its order.
-__host__ __device__ constexpr int token_at(int i) { return (i % 4 / 2) * 8 + (i / 4) * 2 + i % 2; }
 
 // Scales of a page: keys' factor, values' exponent and inverse factor (of 2^-11 p).
 struct PageScale {
@@ -181,7 +174,7 @@ __device__ __forceinline__ void softmax_step(uint32_t (&s)[64], uint32_t (&out)[
     const float base = next == kNegInf ? 0.f : next - kKv8Lift;
     alpha = next == m ? 1.f : exp2_ftz(m - next);
     // Of each turn: the sums and f16 of the page before, this page's exponentials, the next one's exponents. The warp barrier
-    // keeps the turns apart for the compiler (chunks 424 us, so 416).
+    // keeps the turns apart for the compiler (chunks 2% less).
     float sum = 0.f;
     uint64_t z[8], e[8];
 #pragma unroll
@@ -360,7 +353,7 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                     const uint32_t w[4] = {u[v].x, u[v].y, u[v].z, u[v].w};
                     uint32_t f[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) f[e] = bad ? 0u : half2_of(bf16lo(w[e]) * inv, bf16hi(w[e]) * inv);
+                    for (int e = 0; e < 4; ++e) f[e] = bad ? 0u : pack_half2(bf16lo(w[e]) * inv, bf16hi(w[e]) * inv);
                     *reinterpret_cast<uint4*>(dst + (v >> 3) * F::kQHalf + (((v & 7) ^ (row & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
                 }
                 fence_proxy_async();
@@ -533,14 +526,14 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                 ++taken[t];
                 uint64_t* empty = keys ? &sh.k_empty[st] : &sh.v_empty[st];
                 // With a team for each stream the codes are read as soon as they are there, ahead of their tile (their slots then come
-                // back earlier: 24 requests x 6 drafted rows 111 us, so 107). One team has not the registers (chunks 431 us, so 440).
+                // back earlier: 24 requests x 6 drafted rows 4% less). One team has not the registers (chunks 2% more).
                 constexpr bool kAhead = F::kTeams == 2;
                 const bool both = !kAhead && use > 0;
                 ok = wait_two(&sh.raw_full[raw], n / 2, both ? empty : &sh.raw_full[raw], both ? use - 1 : n / 2, a.err, 908);
                 if (!ok) break;
                 const uint8_t* src = sRaw + raw * kPages * kKv8Bytes;
                 // The fence before a slot is given back puts its reads ahead of the copy that overwrites it: without, that copy
-                // overtook loads on their way (giving it back after the conversion instead: chunks 557 us, so 440).
+                // overtook loads on their way (giving it back after the conversion instead: chunks a quarter more).
                 if (keys) {
                     const uint8_t* ks = src + k_tok * 64 + k_c * 16;
                     uint8_t* kd = sK + st * kKTile + k_place * 128;
@@ -556,8 +549,8 @@ attend_tiles_kernel(const Kv8AttnArgs a) {
                         *reinterpret_cast<uint4*>(dst + to[0]) = make_uint4(f[0], f[1], f[2], f[3]);
                         *reinterpret_cast<uint4*>(dst + to[1]) = make_uint4(f[4], f[5], f[6], f[7]);
                     };
-                    // 128 rows: all codes first, so that their slot comes back early (130 us for 142, where two steps are all that
-                    // is on its way); else two pages at a time, less code at once (24 x 6 rows 107 us, so 104).
+                    // 128 rows: all codes first, so that their slot comes back early (8% less, where two steps are all that is on
+                    // its way); else two pages at a time, less code at once (24 x 6 rows 3% less).
                     if constexpr (ROWS == 128) {
                         uint4 w[kPages][2];
 #pragma unroll

@@ -41,11 +41,6 @@ __device__ __forceinline__ unsigned long long argmax_key(float v, uint32_t i) {
 // the others reduce, exchange and store. 320 rows of 151936: 88 us, 4.4 TB/s. The parts in registers: 97 us with two
 // CTAs an SM, 137 with one; clusters that walk the rows with the next row's loads in flight (one CTA an SM, and 15
 // clusters of 8 are all that the GPU holds then) 122; clusters of 16: 165.
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 template <int VEC>
 __device__ __forceinline__ void copy_async(float* dst, const float* src) {
     if (VEC == 4) cp_async16(smem_u32(dst), src, true);
@@ -63,7 +58,7 @@ __device__ __forceinline__ void read_part(const float* src, float (&v)[VEC]) {
 // Maximum m and sum s = sum exp2((x - m) c) of a warp's 32 such pairs, in every lane.
 __device__ __forceinline__ void join_pairs(float& m, float& s, float c) {
     const float all = warp_max(m);
-    s = warp_sum(m == kNegInf ? s : s * exp2_approx((m - all) * c));
+    s = warp_sum(m == kNegInf ? s : s * exp2_ftz((m - all) * c));
     m = all;
 }
 
@@ -140,7 +135,7 @@ token_probs_kernel(const float* logits, int64_t ldx, const float* __restrict__ t
         read_part<VEC>(here + i, v);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            v[e] = exp2_approx((v[e] - base) * c);
+            v[e] = exp2_ftz((v[e] - base) * c);
             (e & 1 ? s1 : s0) += v[e];
         }
         write_part<VEC>(here + i, v);
@@ -163,7 +158,7 @@ token_probs_kernel(const float* logits, int64_t ldx, const float* __restrict__ t
     cluster_arrive();  // this CTA's peers are read; waited for at the end
     join_pairs(m, s, c);
     // a row without any logit above -inf: S = 0, zeros (S is NaN where a logit is NaN or +inf)
-    const float f = s == 0.f ? 0.f : (own == kNegInf ? 1.f : exp2_approx((own - m) * c)) / s;
+    const float f = s == 0.f ? 0.f : (own == kNegInf ? 1.f : exp2_ftz((own - m) * c)) / s;
 #pragma unroll 4
     for (int i = tid * VEC; i < count; i += kProbThreads * VEC) {
         float v[VEC];
