@@ -446,8 +446,9 @@ MSGL_API int msgl_qknorm_rope_store_kv8_partials(const float* parts, int nparts,
 /* Attention over the 8-bit pool: single tokens, drafted rows and chunks. q / out [total_q, Hq, 128]
  * bf16, Hq / Hkv in {1, 2, 4, 8}; each row attends the keys up to its own position (a row before the
  * context's first token, or of an empty context, gives zeros); keys and values behind it do not reach
- * it whatever they hold. A row with a NaN or an infinity in its query gives NaN. max_q_len bounds the
- * rows per request, max_seq_len (<= max_pages * 16) the contexts. Recorded as MSGL_ERR_BOUNDS: a
+ * it whatever they hold. A row with a NaN or an infinity in its query gives NaN. Logits are fp32, of up
+ * to 2^26. max_q_len bounds the rows per request, max_seq_len (<= max_pages * 16) the contexts.
+ * Recorded as MSGL_ERR_BOUNDS: a
  * context outside [0, max_seq_len] (clamped, site 900), a request with more than max_q_len rows or
  * rows outside total_q (skipped, site 901), a page outside the pool (page 0 in its place, site 902).
  * The workspace (msgl_paged_attention_kv8_workspace_size, 16-byte aligned) needs no clearing and serves

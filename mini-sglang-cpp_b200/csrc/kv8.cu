@@ -706,7 +706,7 @@ __device__ __forceinline__ void attend_page8(const uint8_t* page, uint32_t scale
         float mx = fmaxf(fmaxf(p[t][0], p[t][1]), fmaxf(p[t][2], p[t][3]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const bool move = mx > st.m[t] + kKv8Lag || st.m[t] == kNegInf;
+        const bool move = kv8_grows(mx, st.m[t]);
         const float next = move ? fmaxf(mx, st.m[t]) : st.m[t];
         alpha[t] = 1.f;
         if (move && next != kNegInf) {
@@ -714,7 +714,7 @@ __device__ __forceinline__ void attend_page8(const uint8_t* page, uint32_t scale
             moved = true;
         }
         st.m[t] = next;
-        const float base = next == kNegInf ? 0.f : next - kKv8Lift;
+        const float base = kv8_base(next);
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -740,8 +740,8 @@ __device__ __forceinline__ void attend_page8(const uint8_t* page, uint32_t scale
     uint32_t pb[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        pb[t][0] = half2_weights(p[t][0], p[t][1]);
-        pb[t][1] = half2_weights(p[t][2], p[t][3]);
+        pb[t][0] = pack_half2(p[t][0], p[t][1]);
+        pb[t][1] = pack_half2(p[t][2], p[t][3]);
     }
     uint32_t hidden = 0;  // 0x80 in the bytes of tokens that some live row does not see
     if (EDGE)

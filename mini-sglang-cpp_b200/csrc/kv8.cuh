@@ -75,14 +75,12 @@ __device__ __forceinline__ int kv8_query_exponent(float amax) { return max(1, mi
 // at most (a code carries a rounding of 2^-4 already) down to 2^-25 of the row's largest and flushes below 2^-36: behind a key
 // that takes nearly all of the weight, or in pages whose values are that much smaller, the others still count. With
 // p = 2^(s - m) <= 2^8 that began at 2^-14 (keys 20 octaves below a sink came out 3% off, 25 octaves lost). The sums of weights
-// stay in fp32, of 2^-kKv8Lift p.
+// stay in fp32, of 2^-kKv8Lift p. Roundings between a logit and its exponent go down, so that p <= 2^15 whatever the logits' size, and
+// up to 2^26 the largest one's p stays above 2^-14.
 constexpr float kKv8Lift = 11.f, kKv8Lag = 4.f, kKv8Unlift = 0x1p-11f;
-// Two weights; where logits of millions differ by their own rounding, the largest f16 value.
-__device__ __forceinline__ uint32_t half2_weights(float lo, float hi) {
-    uint32_t h;
-    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(hi), "f"(lo));
-    return h;
-}
+__device__ __forceinline__ bool kv8_grows(float top, float m) { return top > __fadd_rd(m, kKv8Lag) || m == -__builtin_huge_valf(); }
+// What is subtracted from s.
+__device__ __forceinline__ float kv8_base(float m) { return m == -__builtin_huge_valf() ? 0.f : __fsub_ru(m, kKv8Lift); }
 // Bytes of a word of codes that are NaN, as 0x80 each.
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 __device__ __forceinline__ int64_t larger(int64_t a, int64_t b) { return a > b ? a : b; }

@@ -167,11 +167,11 @@ __device__ __forceinline__ void softmax_step(uint32_t (&s)[64], uint32_t (&out)[
         }
         const float a = max3(x[0], x[1], x[2]), b = max3(x[3], x[4], x[5]), c = max3(x[6], x[7], x[8]);
         const float d = max3(x[9], x[10], x[11]), e = max3(x[12], x[13], x[14]);
-        mx[p] = fmaf(fmaxf(max3(a, b, c), max3(d, e, x[15])), f[p], v_exp[p]);
+        mx[p] = __fmaf_ru(fmaxf(max3(a, b, c), max3(d, e, x[15])), f[p], v_exp[p]);
     }
     const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
-    const float next = m == kNegInf || top > m + kKv8Lag ? fmaxf(m, top) : m;
-    const float base = next == kNegInf ? 0.f : next - kKv8Lift;
+    const float next = kv8_grows(top, m) ? fmaxf(m, top) : m;
+    const float base = kv8_base(next);
     alpha = next == m ? 1.f : exp2_ftz(m - next);
     // Of each turn: the sums and f16 of the page before, this page's exponentials, the next one's exponents. The warp barrier
     // keeps the turns apart for the compiler (chunks 2% less).
@@ -187,7 +187,7 @@ __device__ __forceinline__ void softmax_step(uint32_t (&s)[64], uint32_t (&out)[
                 float a, b;
                 part[i & 1] = add2(part[i & 1], e[i]);
                 unpair(e[i], a, b);
-                out[p * 8 + i] = half2_weights(a, b);
+                out[p * 8 + i] = pack_half2(a, b);
             }
             float a, b;
             unpair(add2(part[0], part[1]), a, b);
@@ -205,7 +205,7 @@ __device__ __forceinline__ void softmax_step(uint32_t (&s)[64], uint32_t (&out)[
         }
         if (k + 1 < kPages) {
             const int p = k + 1;
-            const uint64_t f2 = pair(f[p]), v2 = pair(v_exp[p] - base);
+            const uint64_t f2 = pair(f[p]), v2 = pair(__fsub_rd(v_exp[p], base));
 #pragma unroll
             for (int i = 0; i < 8; ++i) z[i] = fma2(pair(s[p * 16 + 2 * i], s[p * 16 + 2 * i + 1]), f2, v2);
         }

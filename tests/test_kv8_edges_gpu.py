@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from kv8_plain import D, PAGE, fill, ints
+from kv8_plain import D, PAGE, fill, ints, pool_values
 from test_kv8_gpu import Attend
 
 pytestmark = pytest.mark.gpu
@@ -194,3 +194,31 @@ def test_a_large_query_element_that_meets_zeros(cuda, rows, big):
     a.check(out, scale=scale)
     a.q = -a.q
     assert torch.equal(a.call(scale=-scale), out)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 16, 2.0 ** 19, 2.0 ** 20, 2.0 ** 21])
+def test_huge_logits(cuda, rows, size):
+    """Logits of `size` and more: the value of the one key that is ahead of the others by more than fp32's rounding."""
+    a = Attend([rows + 500, rows + 30], [rows] * 2, 8, 2, seed=rows + 7)
+    a.q = (a.q.float() * size).bfloat16()
+    out = a.call()
+    row = sure = 0
+    for r, n in enumerate(a.lens):
+        page = a.table[r, :-(-n // PAGE)].long()
+        keys, values = (pool_values(a.kv8[page], a.scales[page], k).transpose(0, 1).reshape(2, -1, D)[:, :n] for k in (0, 1))
+        pos = torch.arange(n - rows, n, device="cuda")
+        q = a.q[row:row + rows].double().view(rows, 2, 4, D)
+        for h in range(2):
+            s = torch.einsum("mgd,nd->mgn", q[:, h], keys[h]) * D ** -0.5
+            s = s.masked_fill((torch.arange(n, device="cuda") > pos[:, None])[:, None], -math.inf)
+            off = torch.einsum("mgd,nd->mgn", q[:, h].abs(), keys[h].abs()).amax(-1) * D ** -0.5 * 2 ** -17
+            top = torch.topk(s, 2, -1)
+            alone = top.values[..., 0] - top.values[..., 1] > 2 * off + 60
+            want = values[h][top.indices[..., 0]]
+            got = out[row:row + rows].double().view(rows, 2, 4, D)[:, h]
+            assert bool(((got - want).abs() <= want.abs() * 2 ** -8 + 2.0 ** -40)[alone].all())
+            assert bool(torch.isfinite(got).all())
+            sure += int(alone.sum())
+        row += rows
+    assert sure > 8 * row // 2
